@@ -408,6 +408,108 @@ int odi_cuda_add(float* d_x, const float* d_d, int64_t n, void* stream);
 int odi_cuda_argmax(const float* d_logits, int64_t V, odi_cuda_decode_state* d_state, int32_t* d_record,
                     int record_len, void* stream);
 
+/* --- several drafted tokens per step -----------------------------------------
+ * What a step that verifies T drafted tokens (a chain or a tree) of one
+ * sequence does around the T-token products (odi_cuda_matmul): rows of q
+ * rotated and of k, v appended, the tree's attention over the cache, the
+ * adjusted logits and greedy token of every node, and the accepted path's
+ * cache rows moved into place.  The position comes from device memory
+ * (state.pos: the slot of node 0), so a step can be captured and replayed.
+ * The reference decodes one token at a time (context.cpp:84-282); its sampler
+ * has the repetition penalty (sampler.cpp:39-80). */
+
+/* A KV cache of one layer.  ODI_CUDA_KV_F16: K and V are fp16
+ * [kv_heads][ctx][head_dim], the layout of odi_cuda_rope_kv.
+ * ODI_CUDA_KV_I8: K and V each hold int8 codes [kv_heads][ctx][head_dim],
+ * then, from the next multiple of 256 bytes, one fp32 scale per row
+ * [kv_heads][ctx]; value = code * scale, scale = max|row| / 127, codes
+ * rounded half away from zero.  A row with a value that is not finite gets
+ * the scale NaN.  head_dim 64 or 128; k and v 16-byte aligned. */
+enum { ODI_CUDA_KV_F16 = 0, ODI_CUDA_KV_I8 = 1 };
+typedef struct odi_cuda_kv_cache {
+  void* k;
+  void* v;
+  int dtype;
+  int kv_heads;
+  int head_dim;
+  int ctx;
+} odi_cuda_kv_cache;
+
+/* Bytes of K (and again of V); 0 for a shape or dtype that is not supported. */
+size_t odi_cuda_kv_cache_bytes(int dtype, int kv_heads, int head_dim, int ctx);
+
+/* Rows t = 0 .. tokens - 1 of d_qkv are [q heads | k kv_heads | v kv_heads] *
+ * head_dim fp32, ld_qkv apart.  Per head: RMSNorm with d_q_norm / d_k_norm
+ * (head_dim weights; NULL: none), then the rotation of odi_cuda_rope_kv at
+ * position pos + d_depth[t] (NULL: pos + t), its angle reduced in 64 bits.
+ * The rotated q rows go to d_q_out (ld_q apart; it may be d_qkv itself with
+ * the same stride), k and v to cache slot pos + t.  A slot outside the cache
+ * is not written. */
+int odi_cuda_qk_rope_append(const float* d_qkv, int64_t ld_qkv, const float* d_q_norm, const float* d_k_norm,
+                            float eps, float* d_q_out, int64_t ld_q, const odi_cuda_kv_cache* cache,
+                            const odi_cuda_decode_state* d_state, const int32_t* d_depth, int tokens, int heads,
+                            float theta, void* stream);
+
+/* Positions start .. start + count - 1 of K and V (either output may be NULL)
+ * as [kv_heads][count][head_dim] fp16 or fp32, 16-byte aligned. */
+enum { ODI_CUDA_KV_OUT_F16 = 0, ODI_CUDA_KV_OUT_F32 = 1 };
+int odi_cuda_kv_read(const odi_cuda_kv_cache* cache, int start, int count, void* d_k_out, void* d_v_out,
+                     int out_dtype, void* stream);
+
+/* Cache rows d_src[i] -> d_dst[i], i < n, in every kv head of K and V: all
+ * sources are read before any destination is written, and a destination
+ * listed twice takes its last row.  The lists are relative to state.pos
+ * (d_state NULL: absolute); an entry with either end outside the cache is
+ * skipped. */
+#define ODI_CUDA_KV_MOVE_MAX 256
+int odi_cuda_kv_move(const odi_cuda_kv_cache* cache, const int32_t* d_src, const int32_t* d_dst, int n,
+                     const odi_cuda_decode_state* d_state, void* stream);
+
+/* Attention of T = tokens nodes, node t in cache slot pos + t.  d_q: rotated
+ * queries [T][heads * head_dim], rows ld_q apart; d_out [T][heads * head_dim].
+ * A node sees every slot below pos, and tree slot pos + j where bit j % 32 of
+ * d_mask[t * ceil(T / 32) + j / 32] is set (d_mask NULL: j <= t).  Slots
+ * outside the cache are not seen, a node that sees nothing gets zeros, and
+ * what lies in slots that a node does not see (NaN included) does not reach
+ * it.  Grouped-query heads share kv head h / (heads / kv_heads), any ratio.
+ * fp32 scores, softmax and sums.  d_scratch: as for
+ * odi_cuda_attention_decode (16-byte aligned, zero before its first use,
+ * left reusable, calls on one stream only; its first int is the error word,
+ * odi_cuda_workspace_status). */
+#define ODI_CUDA_TREE_MAX 256
+size_t odi_cuda_attention_tree_scratch_bytes(int tokens, int heads, int kv_heads, int head_dim, int ctx);
+int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_cache* cache, float* d_out,
+                            const uint32_t* d_mask, const odi_cuda_decode_state* d_state, int tokens, int heads,
+                            float scale, void* d_scratch, size_t scratch_bytes, void* stream);
+
+/* Per row of logits, in this order, each one fp32 operation: for an id with
+ * count c > 0 in the row's history, l > 0 ? l / repeat : l * repeat, then
+ * - c * frequency, then - presence; + its bias; -inf where its mask bit is 0.
+ * The adjusted row goes to d_out (may be d_logits; NULL: not stored) and its
+ * first largest id to d_tokens (NULL: not wanted): -1 when nothing is above
+ * -inf, NaN never chosen.  opts NULL: no adjustment. */
+typedef struct odi_cuda_logits_opts {
+  float repeat_penalty;        /* > 0; 1: none */
+  float frequency_penalty;     /* 0: none */
+  float presence_penalty;      /* 0: none */
+  const int32_t* history;      /* [rows][history_ld]; NULL: none.  Ids outside the vocabulary are skipped */
+  int64_t history_ld;          /* 0: one history for all rows */
+  const int32_t* history_len;  /* [rows] entries in use, at most history_max; NULL: history_max each */
+  int history_max;             /* at most 65535 */
+  const int32_t* bias_ids;     /* bias_count ids for all rows; an id listed twice takes its last value */
+  const float* bias;
+  int bias_count;              /* at most 65535 */
+  const uint32_t* mask;        /* [rows][mask_ld] words, bit id % 32 of word id / 32 allows id; NULL: all allowed */
+  int64_t mask_ld;             /* 0: one mask for all rows */
+} odi_cuda_logits_opts;
+
+/* Scratch for odi_cuda_logits_adjust with d_tokens: 8-byte aligned, zero
+ * before its first use, left zero (calls on one stream only). */
+size_t odi_cuda_logits_scratch_bytes(int rows);
+int odi_cuda_logits_adjust(const float* d_logits, int64_t ld_logits, float* d_out, int64_t ld_out, int32_t* d_tokens,
+                           int rows, int64_t V, const odi_cuda_logits_opts* opts, void* d_scratch,
+                           size_t scratch_bytes, void* stream);
+
 /* --- the decode step as one call per token ----------------------------------
  * A device-resident decoder of a Llama-shaped model: one token's forward
  * pass (context.cpp:84-282 for a single token, with cpu_backend.cpp:388-619's

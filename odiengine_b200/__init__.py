@@ -97,6 +97,15 @@ SIGNATURES = {
     "odi_cuda_silu_mul": (_int, [_vp, _vp, _i64, _vp]),
     "odi_cuda_add": (_int, [_vp, _vp, _i64, _vp]),
     "odi_cuda_argmax": (_int, [_vp, _i64, _vp, _vp, _int, _vp]),
+    "odi_cuda_kv_cache_bytes": (_sz, [_int, _int, _int, _int]),
+    "odi_cuda_qk_rope_append": (_int, [_vp, _i64, _vp, _vp, ctypes.c_float, _vp, _i64, _vp, _vp, _vp, _int, _int,
+                                       ctypes.c_float, _vp]),
+    "odi_cuda_kv_read": (_int, [_vp, _int, _int, _vp, _vp, _int, _vp]),
+    "odi_cuda_kv_move": (_int, [_vp, _vp, _vp, _int, _vp, _vp]),
+    "odi_cuda_attention_tree_scratch_bytes": (_sz, [_int, _int, _int, _int, _int]),
+    "odi_cuda_attention_tree": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _int, _int, ctypes.c_float, _vp, _sz, _vp]),
+    "odi_cuda_logits_scratch_bytes": (_sz, [_int]),
+    "odi_cuda_logits_adjust": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _vp, _vp, _sz, _vp]),
     "odi_cuda_scatter_signals": (_i64, [_int, _i64, _i64, _i64, _int]),
     "odi_cuda_matmul_scatter": (_int, [_int, _vp, _vp, _i64, _i64, _i64, _int, _vp, _sz, _int, _vp, _vp]),
     "odi_cuda_wait_peers": (_int, [_vp, _vp, _vp, _int, _vp, _vp]),
