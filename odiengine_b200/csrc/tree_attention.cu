@@ -16,8 +16,45 @@
 namespace odi_cuda {
 namespace {
 
-constexpr int TA_BLOCK = 128;  // cache positions per step
+// Rows of one kv head: r = t * G + g for node t and the g-th of the G query
+// heads that share the kv head, R = T * G in all.  A CTA takes NR * 8 of them
+// (blockIdx.y) and every nsplit-th share of the cache (blockIdx.z); its four
+// warps work alone until the end, each on groups of 16 positions:
+//
+//   S^T [16 positions x 8 rows] = K . Q^T     (mma.sync, positions as M)
+//   O^T [hd x 8 rows]          += V^T . P^T   (mma.sync, dims as M)
+//
+// With the rows as the narrow side of the product, 8 rows waste nothing, and
+// both operands that come from the cache are read straight from global memory
+// into the fragments: which dims (or positions) a fragment register holds is
+// free as long as both factors agree, so lane (g, c) takes whole 16-byte
+// pieces -- K: pieces c, c + 4, ... of rows g and g + 8; V: dims 16 g .. 16 g +
+// 15 of positions 2c, 2c + 1, 2c + 8, 2c + 9 -- and no shared memory or barrier
+// stands between the cache and the tensor core.  The next group's pieces are
+// requested as soon as this group's are used up.
+//
+// fp32 results from 16- and 8-bit products:
+//  * int8 cache: q is fixed point, 24 bits against the row's largest value, in
+//    three signed 8-bit digits; the digit products with the codes are exact
+//    in 32-bit integers, and joined and scaled in fp32.
+//  * fp16 cache: q, scaled by a power of two, is the sum of two fp16 values
+//    (22 bits).
+//  * P (times the int8 row's scale of V) is the sum of two fp16 values, so
+//    the codes, or the fp16 values, of V enter unrounded.
+//
+// Softmax: m is a reference, not the running maximum: it moves only when a
+// weight passes 2^15 against it (then to the maximum, and the sums are
+// rescaled), which after the first groups is rare; fp16 pairs hold weights
+// up to 2^16 and down to 2^-24.
+constexpr int TA_WARPS = 4;
+constexpr int TA_THREADS = 32 * TA_WARPS;
 constexpr int TA_SMS = 148;
+constexpr int TA_GROUP = 16;
+constexpr float TA_NONE = -3.402823466e38f;  // reference of a row that has seen nothing
+constexpr float TA_TOP = 32768.f;            // a weight past this moves the reference
+constexpr float TA_UNIT = 16.f;              // the largest weight right after that
+constexpr float TA_VMOST = 0x1p120f;         // factor of an int8 row's scales before any was seen
+constexpr float TA_QMAX = 8290000.f;         // |fixed-point q|: three signed digits, the first within 127
 
 struct TreeArgs {
   const float* q;
@@ -27,125 +64,484 @@ struct TreeArgs {
   const unsigned* mask;
   int mask_words;
   const DecodeState* st;
-  int tokens, heads, nsplit;
+  int tokens, heads, G, R, nsplit;
   float scale;
-  int* count;   // arrivals per (token, head), zero between launches
-  float* part;  // [token][head][split][hd + 2]: running max, sum, accumulator
+  int* count;   // arrivals per (kv head, row tile), zero between launches
+  float* part;  // [kv head][tile][split][row][hd + 2]: reference, sum, accumulator
 };
 
-__device__ __forceinline__ float kv_value(const KvView& c, const void* base, int64_t row, int d) {
-  if (c.dtype == ODI_CUDA_KV_F16) return __half2float(static_cast<const __half*>(base)[row * c.hd + d]);
-  return (float)static_cast<const int8_t*>(base)[row * c.hd + d] *
-         reinterpret_cast<const float*>(static_cast<const uint8_t*>(base) + c.scale_off)[row];
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_h(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 8x8 transpose of 16-bit values held two per lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// Streaming 16-byte load.
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Fragment registers of one group: KW words of K per row and lane, VW of V per
+// position and lane, and the words of Q per lane and row tile.
+template <int HD, bool I8>
+struct Frag {
+  static constexpr int KW = HD * (I8 ? 1 : 2) / 16;  // words of one K row on a lane (4 lanes share a row)
+  static constexpr int VW = HD * (I8 ? 1 : 2) / 32;  // words of one V row on a lane (8 lanes share a row)
+  static constexpr int DIG = I8 ? 3 : 2;             // digits of q
+  static constexpr int QW = KW * DIG;                // words of Q on a lane, per row tile
+  static constexpr int MT = HD / 16;                 // 16-dim tiles of O^T
+};
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p, int piece_stride) {
+  if (N == 2) {
+    const uint2 v = ldg8(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = ldg16(p + (int64_t)i * piece_stride);
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  }
 }
 
-// One CTA per (head, token, split); a lane scores one position, a warp 32.
-template <int HD>
-__global__ void __launch_bounds__(128) tree_attn_kernel(const TreeArgs a) {
-  __shared__ float qs[HD], fold[4][HD + 2];
+template <int HD, int NR, bool I8>
+struct TreeSmem {
+  using F = Frag<HD, I8>;
+  static constexpr int Q = NR * F::QW * 32 * 4;
+  static constexpr int ROWC = NR * 8 * 4;  // per-row factor of the scores
+  static constexpr int FOLD = TA_WARPS * NR * 8 * (HD + 2) * 4;
+  static constexpr int BYTES = ROWC + (Q > FOLD ? Q : FOLD);
+};
+
+template <int HD, int NR, bool I8>
+__global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tree_attn_kernel(const TreeArgs a) {
+  using F = Frag<HD, I8>;
+  constexpr int KW = F::KW, VW = F::VW, DIG = F::DIG, QW = F::QW, MT = F::MT;
+  constexpr int ROWB = HD * (I8 ? 1 : 2);
+  extern __shared__ __align__(16) uint8_t ta_smem[];
+  float* rowc = reinterpret_cast<float*>(ta_smem);
+  uint32_t* qf = reinterpret_cast<uint32_t*>(ta_smem + TreeSmem<HD, NR, I8>::ROWC);  // [NR][QW / 4][lane][4]
+  float* fold = reinterpret_cast<float*>(qf);                                        // [warp][row][HD + 2], at the end
   __shared__ int is_last;
   pdl_launch_dependents();
   pdl_wait();
-  const int h = blockIdx.x, t = blockIdx.y, split = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = h / (a.heads / a.c.kv_heads);
+  const int kvh = blockIdx.x, tile = blockIdx.y, split = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int pos = a.st->pos;
-  const int64_t len = max((int64_t)0, min((int64_t)a.c.ctx, (int64_t)pos + a.tokens));
-  for (int d = threadIdx.x; d < HD; d += 128) qs[d] = a.q[t * a.ld_q + (int64_t)h * HD + d] * a.scale;
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, acc[HD / 32];
-  for (int e = 0; e < HD / 32; ++e) acc[e] = 0.f;
-  for (int64_t p0 = (int64_t)split * TA_BLOCK; p0 < len; p0 += (int64_t)a.nsplit * TA_BLOCK) {
-    const int64_t p = p0 + warp * 32 + lane;
-    bool vis = p < len;
-    if (vis && p >= pos) {
-      const int j = (int)(p - pos);
-      vis = a.mask ? (a.mask[(int64_t)t * a.mask_words + (j >> 5)] >> (j & 31)) & 1u : j <= t;
+  const int len = (int)max(0ll, min((long long)a.c.ctx, (long long)pos + a.tokens));
+  const int ngroups = (len + TA_GROUP - 1) / TA_GROUP;
+
+  // ---- Q: each warp lays out every TA_WARPS-th row: digits, in fragment order
+  for (int n = warp; n < NR * 8; n += TA_WARPS) {
+    const int r = tile * NR * 8 + n;
+    constexpr int PL = HD / 32;
+    float v[PL], am = 0.f;
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < PL; ++e) v[e] = 0.f;
+    if (r < a.R) {
+      const float* src = a.q + (int64_t)(r / a.G) * a.ld_q + (int64_t)(kvh * a.G + r % a.G) * HD;
+#pragma unroll
+      for (int e = 0; e < PL; ++e) v[e] = src[lane * PL + e];
     }
-    float s = -INFINITY;
-    const int64_t row = (int64_t)kvh * a.c.ctx + p;
-    if (vis) {
-      s = 0.f;
-      for (int d = 0; d < HD; ++d) s = fmaf(qs[d], kv_value(a.c, a.c.k, row, d), s);
+#pragma unroll
+    for (int e = 0; e < PL; ++e) am = fmaxf(am, fabsf(v[e])), ok = ok && finite(v[e]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+    ok = __all_sync(0xffffffffu, ok);
+    // a power of two that brings the largest value to 2^13 .. 2^14; I8 fills its digits instead
+    const int ex = min(max((int)(__float_as_uint(am) >> 23) - 127, -100), 126);
+    const float up = I8 ? TA_QMAX : 8192.f;
+    const float lift = __uint_as_float((uint32_t)(127 - ex) << 23);  // 2^-ex
+    const float unit = am * lift;  // 1 .. 2 (2 .. 4 at the top of the range), less where am is tiny
+    const float f = I8 ? (unit > 0.f ? up / unit : 0.f) : up;
+    if (lane == 0) {
+      const double back = am > 0.f ? (double)a.scale * 1.4426950408889634 / ((double)f * (double)lift) : 0.0;
+      rowc[n] = ok ? (float)back : __int_as_float(0x7fc00000);
     }
-    const unsigned seen = __ballot_sync(0xffffffffu, vis);
-    if (!seen) continue;
-    float mx = s;
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float mn = fmaxf(m, mx);
-    const float corr = m == -INFINITY ? 0.f : expf(m - mn);
-    const float pv = vis ? expf(s - mn) : 0.f;
-    float ps = pv;
-    for (int o = 16; o; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-    l = l * corr + ps;
-    for (int e = 0; e < HD / 32; ++e) acc[e] *= corr;
-    for (int i = 0; i < 32; ++i) {
-      const float pi = __shfl_sync(0xffffffffu, pv, i);
-      if (!((seen >> i) & 1u)) continue;  // a position that is not seen is not read
-      for (int e = 0; e < HD / 32; ++e)
-        acc[e] = fmaf(pi, kv_value(a.c, a.c.v, row - lane + i, lane + 32 * e), acc[e]);
-    }
-    m = mn;
-  }
-  if (lane == 0) fold[warp][0] = m, fold[warp][1] = l;
-  for (int e = 0; e < HD / 32; ++e) fold[warp][2 + lane + 32 * e] = acc[e];
-  __syncthreads();
-  const int64_t unit = (int64_t)t * a.heads + h;
-  float* part = a.part + unit * a.nsplit * (HD + 2);
-  auto merge = [&](const float* p, int n, int64_t stride, int d, float* M, float* L) {
-    float mm = -INFINITY, ll = 0.f, aa = 0.f;
-    for (int i = 0; i < n; ++i) {
-      const float mi = __ldcg(p + i * stride);
-      if (mi == -INFINITY) continue;
-      const float mn = fmaxf(mm, mi), fo = expf(mm - mn), fn = expf(mi - mn);
-      ll = ll * fo + p[i * stride + 1] * fn;
-      aa = aa * fo + p[i * stride + 2 + d] * fn;
-      mm = mn;
-    }
-    *M = mm, *L = ll;
-    return aa;
-  };
-  for (int d = threadIdx.x; d < HD; d += 128) {
-    float mm = -INFINITY, ll = 0.f, aa = 0.f;
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, fold[w][0]);
-    for (int w = 0; w < 4; ++w)
-      if (fold[w][0] != -INFINITY) {
-        const float f = expf(fold[w][0] - mm);
-        ll += fold[w][1] * f, aa += fold[w][2 + d] * f;
+    uint8_t* dst = reinterpret_cast<uint8_t*>(qf) + (int64_t)(n >> 3) * QW * 128;
+    const int gn = n & 7;
+#pragma unroll
+    for (int e = 0; e < PL; ++e) {
+      const int d = lane * PL + e;
+      const float x = ok ? v[e] * lift * f : 0.f;
+      if (I8) {
+        // dims 16 ch + 4 w + b sit in byte b of word w of piece ch on lane ch % 4
+        const int ch = d >> 4, w = (d >> 2) & 3, b = d & 3;
+        int i = __float2int_rn(x);
+#pragma unroll
+        for (int k = DIG - 1; k >= 0; --k) {
+          const int lo = (int)(int8_t)(i & 255);
+          i = (i - lo) >> 8;
+          const int word = k * KW + (ch >> 2) * 4 + w;
+          dst[((word >> 2) * 32 + gn * 4 + (ch & 3)) * 16 + (word & 3) * 4 + b] = (uint8_t)lo;
+        }
+      } else {
+        const int ch = d >> 3, w = (d >> 1) & 3, b = d & 1;
+        const __half hi = __float2half_rn(x);
+        const __half lo = __float2half_rn(x - __half2float(hi));
+#pragma unroll
+        for (int k = 0; k < DIG; ++k) {
+          const int word = k * KW + (ch >> 2) * 4 + w;
+          *reinterpret_cast<__half*>(dst + ((word >> 2) * 32 + gn * 4 + (ch & 3)) * 16 + (word & 3) * 4 + 2 * b) = k ? lo : hi;
+        }
       }
-    float* o = part + split * (HD + 2);
-    o[2 + d] = aa;
-    if (d == 0) o[0] = mm, o[1] = ll;
+    }
   }
+  __syncthreads();
+
+  float o[NR][MT][4], m[NR][2], l[NR][2], vs[NR][2], rc[NR][2];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[r][j][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[r][e] = TA_NONE, l[r][e] = 0.f, vs[r][e] = I8 ? TA_VMOST : TA_UNIT, rc[r][e] = rowc[r * 8 + 2 * c + e];
+  }
+  const int64_t head = (int64_t)kvh * a.c.ctx;
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + head * ROWB;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + head * ROWB;
+  const float* ks = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.k) + a.c.scale_off) + head;
+  const float* vsc = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.v) + a.c.scale_off) + head;
+
+  uint32_t kw[2][KW], vw[4][VW];
+  float dk[2], dv[2];
+  auto load_k = [&](int grp) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = min(grp * TA_GROUP + g + 8 * i, len - 1);  // rows past the end repeat the last: not seen
+      load_words<KW>(kw[i], kb + (int64_t)row * ROWB + c * 16, 64);
+      if (I8) dk[i] = __ldg(ks + row), dv[i] = __ldg(vsc + row);
+    }
+  };
+  auto load_v = [&](int grp) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = min(grp * TA_GROUP + 2 * c + (i & 1) + 8 * (i >> 1), len - 1);
+      load_words<VW>(vw[i], vb + (int64_t)row * ROWB + g * (ROWB / 8), 16);
+    }
+  };
+  const int step = a.nsplit * TA_WARPS;
+  int grp = split * TA_WARPS + warp;
+  if (grp < ngroups) load_k(grp), load_v(grp);
+  for (; grp < ngroups; grp += step) {
+    const int p0 = grp * TA_GROUP;
+    const bool edge = p0 + TA_GROUP > pos;  // holds tree slots or ends past the last
+    unsigned bad = 0;                       // positions of the group whose V is not finite (fp16)
+    if (!I8 && edge) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bool fin = true;
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+          fin = fin && (vw[i][w] & 0x7c00u) != 0x7c00u && (vw[i][w] & 0x7c000000u) != 0x7c000000u;
+        unsigned all = __ballot_sync(0xffffffffu, !fin);
+        all |= all >> 16;
+        all |= all >> 8;
+        all |= all >> 4;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
+          if ((all >> cc) & 1u) bad |= 1u << (2 * cc + (i & 1) + 8 * (i >> 1));
+        // whoever sees such a position gets NaN through its sum; nobody else may meet it
+        if ((all >> c) & 1u)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vw[i][w] = 0;
+      }
+    }
+    uint32_t ph[NR][2], pl[NR][2];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float s[4];
+      const uint4* qr = reinterpret_cast<const uint4*>(qf) + r * (QW / 4) * 32 + lane;
+      if (I8) {
+        int acc[DIG][4];
+#pragma unroll
+        for (int k = 0; k < DIG; ++k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[k][e] = 0;
+#pragma unroll
+          for (int w = 0; w < KW; w += 4) {
+            const uint4 b = qr[((k * KW + w) >> 2) * 32];
+            const uint32_t a0[4] = {kw[0][w], kw[1][w], kw[0][w + 1], kw[1][w + 1]};
+            const uint32_t a1[4] = {kw[0][w + 2], kw[1][w + 2], kw[0][w + 3], kw[1][w + 3]};
+            mma_s8(acc[k], a0, b.x, b.y);
+            mma_s8(acc[k], a1, b.z, b.w);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // digits joined: |digit sums| < 2^21, so each is exact in fp32
+          s[e] = fmaf((float)acc[0][e], 65536.f, fmaf((float)acc[1][e], 256.f, (float)acc[DIG - 1][e])) *
+                 (finite(dk[e >> 1]) ? dk[e >> 1] : __int_as_float(0x7fc00000)) * rc[r][e & 1];
+      } else {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = DIG - 1; k >= 0; --k)  // the small halves first
+#pragma unroll
+          for (int w = 0; w < KW; w += 4) {
+            const uint4 b = qr[((k * KW + w) >> 2) * 32];
+            const uint32_t a0[4] = {kw[0][w], kw[1][w], kw[0][w + 1], kw[1][w + 1]};
+            const uint32_t a1[4] = {kw[0][w + 2], kw[1][w + 2], kw[0][w + 3], kw[1][w + 3]};
+            mma_h(acc, a0, b.x, b.y);
+            mma_h(acc, a1, b.z, b.w);
+          }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = acc[e] * rc[r][e & 1];
+      }
+      bool vis[4] = {true, true, true, true};
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = p0 + g + 8 * (e >> 1);
+          const int row = tile * NR * 8 + r * 8 + 2 * c + (e & 1);
+          bool v = key < len && row < a.R;
+          if (v && key >= pos) {
+            const int t = row / a.G, j = key - pos;
+            v = a.mask ? (a.mask[(int64_t)t * a.mask_words + (j >> 5)] >> (j & 31)) & 1u : j <= t;
+          }
+          vis[e] = v;
+          if (!v) s[e] = -INFINITY;
+          else if (!I8 && ((bad >> (g + 8 * (e >> 1))) & 1u)) s[e] = __int_as_float(0x7fc00000);
+        }
+      }
+      float p[4], w[4], top[2];
+      auto weigh = [&]() {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = ex2(s[e] - m[r][e & 1]);
+          w[e] = I8 ? p[e] * (dv[e >> 1] * vs[r][e & 1]) : p[e] * TA_UNIT;
+          if (I8 && !vis[e]) w[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) top[e] = fmaxf(fmaxf(p[e], w[e]), fmaxf(p[2 + e], w[2 + e]));
+      };
+      weigh();
+      if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > TA_TOP)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // each row by itself: a row's result does not depend on its neighbours
+          float mx = fmaxf(s[e], s[2 + e]), dm = 0.f;
+          if (I8) {
+            if (vis[e] && finite(dv[0])) dm = dv[0];
+            if (vis[2 + e] && finite(dv[1])) dm = fmaxf(dm, dv[1]);
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            if (I8) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, x));
+          }
+          if (!(top[e] > TA_TOP)) continue;
+          const float mn = fmaxf(m[r][e], mx);
+          float corr = ex2(m[r][e] - mn);
+          l[r][e] *= corr;
+          m[r][e] = mn;
+          if (I8 && dm > 0.f) {
+            // TA_UNIT over a power of two above the largest scale seen
+            const int ex = max((int)(__float_as_uint(dm) >> 23) - 126, -116);
+            const float nv = __uint_as_float((uint32_t)(131 - ex) << 23);
+            if (nv < vs[r][e]) {
+              corr *= nv / vs[r][e];
+              vs[r][e] = nv;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < MT; ++j) o[r][j][e] *= corr, o[r][j][2 + e] *= corr;
+        }
+        weigh();
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float q0 = p[e], q1 = p[2 + e];
+        l[r][e] += I8 ? (vis[e] && !finite(dv[0]) ? __int_as_float(0x7fc00000) : q0) +
+                            (vis[2 + e] && !finite(dv[1]) ? __int_as_float(0x7fc00000) : q1)
+                      : q0 + q1;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const __half2 hi = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+        const float2 back = __half22float2(hi);
+        const __half2 lo = __floats2half2_rn(w[2 * i] - back.x, w[2 * i + 1] - back.y);
+        ph[r][i] = transpose8(h2u(hi));
+        pl[r][i] = transpose8(h2u(lo));
+      }
+    }
+    if (grp + step < ngroups) load_k(grp + step);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {  // dims 16 g + 2 j (fragment row g) and + 1 (row g + 8)
+      uint32_t af[4];
+      if (I8) {
+        const int wi = j >> 1;
+        const uint32_t sel = (j & 1) ? 0x7362u : 0x5140u;  // bytes 2j, 2j + 1 of two positions
+        const uint32_t t0 = __byte_perm(vw[0][wi] ^ 0x80808080u, vw[1][wi] ^ 0x80808080u, sel);
+        const uint32_t t1 = __byte_perm(vw[2][wi] ^ 0x80808080u, vw[3][wi] ^ 0x80808080u, sel);
+        const __half2 k = __float2half2_rn(1152.f);  // 1024 + (code + 128) in fp16
+        af[0] = h2u(__hsub2(u2h(__byte_perm(t0, 0x64646464u, 0x4140u)), k));
+        af[1] = h2u(__hsub2(u2h(__byte_perm(t0, 0x64646464u, 0x4342u)), k));
+        af[2] = h2u(__hsub2(u2h(__byte_perm(t1, 0x64646464u, 0x4140u)), k));
+        af[3] = h2u(__hsub2(u2h(__byte_perm(t1, 0x64646464u, 0x4342u)), k));
+      } else {
+        af[0] = __byte_perm(vw[0][j], vw[1][j], 0x5410u);
+        af[1] = __byte_perm(vw[0][j], vw[1][j], 0x7632u);
+        af[2] = __byte_perm(vw[2][j], vw[3][j], 0x5410u);
+        af[3] = __byte_perm(vw[2][j], vw[3][j], 0x7632u);
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        mma_h(o[r][j], af, pl[r][0], pl[r][1]);
+        mma_h(o[r][j], af, ph[r][0], ph[r][1]);
+      }
+    }
+    if (grp + step < ngroups) load_v(grp + step);
+  }
+
+  // ---- the warps' shares, then the splits'
+  constexpr int FS = HD + 2;
+  __syncthreads();  // every warp is done with the fragments of Q
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float sum = l[r][e];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      float* f = fold + (warp * NR * 8 + r * 8 + 2 * c + e) * FS;
+      const float inv = 1.f / vs[r][e];  // a power of two
+      if (g == 0) f[0] = m[r][e], f[1] = sum;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        f[2 + MT * 2 * g + 2 * j] = o[r][j][e] * inv;
+        f[2 + MT * 2 * g + 2 * j + 1] = o[r][j][2 + e] * inv;
+      }
+    }
+  __syncthreads();
+  const int64_t unit = (int64_t)kvh * gridDim.y + tile;
+  float* part = a.part + (unit * a.nsplit + split) * (NR * 8 * FS);
+  const int rows = min(NR * 8, a.R - tile * NR * 8);
+  auto store = [&](int n, int d, float v) {
+    const int r = tile * NR * 8 + n;
+    a.out[((int64_t)(r / a.G) * a.heads + kvh * a.G + r % a.G) * HD + d] = v;
+  };
+  for (int i = threadIdx.x; i < rows * HD; i += TA_THREADS) {
+    const int n = i / HD, d = i % HD;
+    float M = TA_NONE, L = 0.f, A = 0.f;
+#pragma unroll
+    for (int w = 0; w < TA_WARPS; ++w) M = fmaxf(M, fold[(w * NR * 8 + n) * FS]);
+#pragma unroll
+    for (int w = 0; w < TA_WARPS; ++w) {
+      const float* f = fold + (w * NR * 8 + n) * FS;
+      const float k = ex2(f[0] - M);
+      L += f[1] * k;
+      A += f[2 + d] * k;
+    }
+    if (a.nsplit == 1) {
+      store(n, d, L == 0.f ? 0.f : A / L);
+    } else {
+      part[n * FS + 2 + d] = A;
+      if (d == 0) part[n * FS] = M, part[n * FS + 1] = L;
+    }
+  }
+  if (a.nsplit == 1) return;
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) is_last = atomicAdd(&a.count[unit], 1) == a.nsplit - 1;
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  for (int d = threadIdx.x; d < HD; d += 128) {
-    float mm, ll;
-    const float aa = merge(part, a.nsplit, HD + 2, d, &mm, &ll);
-    a.out[unit * HD + d] = mm == -INFINITY ? 0.f : aa / ll;
+  const float* all = a.part + unit * a.nsplit * (NR * 8 * FS);
+  for (int i = threadIdx.x; i < rows * HD; i += TA_THREADS) {
+    const int n = i / HD, d = i % HD;
+    const float* p = all + n * FS;
+    float M = TA_NONE, L = 0.f, A = 0.f;
+    for (int k = 0; k < a.nsplit; ++k) M = fmaxf(M, __ldcg(p + (int64_t)k * NR * 8 * FS));
+    for (int k = 0; k < a.nsplit; ++k) {
+      const float* f = p + (int64_t)k * NR * 8 * FS;
+      const float w = ex2(__ldcg(f) - M);
+      L += __ldcg(f + 1) * w;
+      A += __ldcg(f + 2 + d) * w;
+    }
+    store(n, d, L == 0.f ? 0.f : A / L);
   }
   if (threadIdx.x == 0) a.count[unit] = 0;
 }
 
 struct TreePlan {
-  int nsplit;
+  int nr, tiles, nsplit;
   size_t part_off, bytes;
 };
 
+// Rows per CTA: the fewest 8-row tiles (1, 2 or 4) that hold the R rows, at
+// most 32.  Splits: as many CTAs as are resident at once (4, 3 or 2 per SM),
+// each with a group for every warp.
 TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   TreePlan p;
-  const int64_t units = (int64_t)tokens * heads;
-  const int64_t blocks = ((int64_t)ctx + TA_BLOCK - 1) / TA_BLOCK;
-  int64_t want = TA_SMS * 8 / units;
-  want = want < 1 ? 1 : want > 64 ? 64 : want;
-  p.nsplit = (int)(want > blocks ? blocks : want);
+  const int64_t R = (int64_t)tokens * (heads / kv_heads);
+  p.nr = R <= 8 ? 1 : R <= 16 ? 2 : 4;
+  p.tiles = (int)((R + p.nr * 8 - 1) / (p.nr * 8));
+  const int64_t units = (int64_t)kv_heads * p.tiles;
+  const int64_t room = (int64_t)TA_SMS * (p.nr == 1 ? 4 : p.nr == 2 ? 3 : 2);
+  const int64_t most = ((int64_t)ctx + TA_GROUP * TA_WARPS - 1) / (TA_GROUP * TA_WARPS);
+  int64_t want = room / units;
+  want = want < 1 ? 1 : want > most ? most : want;
+  p.nsplit = (int)want;
   p.part_off = (16 + (size_t)units * 4 + 255) / 256 * 256;
-  p.bytes = p.part_off + (size_t)units * p.nsplit * (hd + 2) * 4;
+  p.bytes = p.part_off + (size_t)units * p.nsplit * p.nr * 8 * (hd + 2) * 4;
   return p;
+}
+
+template <int HD, int NR, bool I8>
+cudaError_t launch_tree(const TreeArgs& a, const TreePlan& p, cudaStream_t s) {
+  auto kern = tree_attn_kernel<HD, NR, I8>;
+  constexpr int smem = TreeSmem<HD, NR, I8>::BYTES;
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!attr_set[dev]) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    attr_set[dev] = true;
+  }
+  return launch_pdl_smem(kern, dim3(a.c.kv_heads, p.tiles, p.nsplit), dim3(TA_THREADS), smem, s, a);
+}
+
+template <int HD>
+cudaError_t launch_tree_hd(const TreeArgs& a, const TreePlan& p, cudaStream_t s) {
+  if (a.c.dtype == ODI_CUDA_KV_I8)
+    return p.nr == 1 ? launch_tree<HD, 1, true>(a, p, s) : p.nr == 2 ? launch_tree<HD, 2, true>(a, p, s)
+                                                                     : launch_tree<HD, 4, true>(a, p, s);
+  return p.nr == 1 ? launch_tree<HD, 1, false>(a, p, s) : p.nr == 2 ? launch_tree<HD, 2, false>(a, p, s)
+                                                                    : launch_tree<HD, 4, false>(a, p, s);
 }
 
 bool tree_shape_ok(int tokens, int heads, int kv_heads, int hd, int ctx) {
@@ -183,12 +579,12 @@ int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_ca
   TreeArgs a{};
   a.q = d_q, a.ld_q = ld_q, a.out = d_out, a.c = v, a.mask = d_mask, a.mask_words = (tokens + 31) / 32;
   a.st = reinterpret_cast<const DecodeState*>(d_state);
-  a.tokens = tokens, a.heads = heads, a.nsplit = p.nsplit, a.scale = scale;
+  a.tokens = tokens, a.heads = heads, a.G = heads / v.kv_heads, a.R = tokens * a.G, a.nsplit = p.nsplit;
+  a.scale = scale;
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + 16);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + p.part_off);
-  const dim3 grid(heads, tokens, p.nsplit);
-  const cudaError_t e = v.hd == 128 ? launch_pdl(tree_attn_kernel<128>, grid, dim3(128), (cudaStream_t)stream, a)
-                                    : launch_pdl(tree_attn_kernel<64>, grid, dim3(128), (cudaStream_t)stream, a);
+  const cudaError_t e = v.hd == 128 ? launch_tree_hd<128>(a, p, (cudaStream_t)stream)
+                                    : launch_tree_hd<64>(a, p, (cudaStream_t)stream);
   return kv_launched(e, "attention_tree");
 }
 
