@@ -66,8 +66,8 @@ struct TreeArgs {
   const DecodeState* st;
   int tokens, heads, G, R, nsplit;
   float scale;
-  int* count;   // arrivals per (kv head, row tile), zero between launches
-  float* part;  // [kv head][tile][split][row][hd + 2]: reference, sum, accumulator
+  int* count;   // arrivals per (kv head, row tile, cluster rank), zero between launches
+  float* part;  // [kv head][tile][cluster][row][hd + 2]: reference, sum, accumulator
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -106,6 +106,35 @@ __device__ __forceinline__ uint2 ldg8(const void* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
+__device__ __forceinline__ uint32_t cluster_nranks() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank_of() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Rank k's copy of a shared-memory value.
+__device__ __forceinline__ float peer_f(const float* p, int k) {
+  uint32_t addr;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(k));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 peer_f2(const float2* p, int k) {
+  uint32_t addr;
+  float2 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(k));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // Fragment registers of one group: KW words of K per row and lane, VW of V per
@@ -138,7 +167,7 @@ struct TreeSmem {
   using F = Frag<HD, I8>;
   static constexpr int Q = NR * F::QW * 32 * 4;
   static constexpr int ROWC = NR * 8 * 4;  // per-row factor of the scores
-  static constexpr int FOLD = TA_WARPS * NR * 8 * (HD + 2) * 4;
+  static constexpr int FOLD = TA_WARPS * NR * 8 * HD * 4;
   static constexpr int BYTES = ROWC + (Q > FOLD ? Q : FOLD);
 };
 
@@ -150,7 +179,8 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   extern __shared__ __align__(16) uint8_t ta_smem[];
   float* rowc = reinterpret_cast<float*>(ta_smem);
   uint32_t* qf = reinterpret_cast<uint32_t*>(ta_smem + TreeSmem<HD, NR, I8>::ROWC);  // [NR][QW / 4][lane][4]
-  float* fold = reinterpret_cast<float*>(qf);                                        // [warp][row][HD + 2], at the end
+  float* fold = reinterpret_cast<float*>(qf);                                        // [warp][row][HD], at the end
+  __shared__ float2 ml[TA_WARPS][NR * 8], cta_ml[NR * 8];                            // reference and sum of each row
   __shared__ int is_last;
   pdl_launch_dependents();
   pdl_wait();
@@ -424,8 +454,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
     if (grp + step < ngroups) load_v(grp + step);
   }
 
-  // ---- the warps' shares, then the splits'
-  constexpr int FS = HD + 2;
+  // ---- the warps' shares, then the cluster's, then the clusters'
   __syncthreads();  // every warp is done with the fragments of Q
 #pragma unroll
   for (int r = 0; r < NR; ++r)
@@ -434,74 +463,111 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
       float sum = l[r][e];
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      float* f = fold + (warp * NR * 8 + r * 8 + 2 * c + e) * FS;
+      const int n = r * 8 + 2 * c + e;
+      float* f = fold + (warp * NR * 8 + n) * HD + MT * 2 * g;
       const float inv = 1.f / vs[r][e];  // a power of two
-      if (g == 0) f[0] = m[r][e], f[1] = sum;
+      if (g == 0) ml[warp][n] = make_float2(m[r][e], sum);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        f[2 + MT * 2 * g + 2 * j] = o[r][j][e] * inv;
-        f[2 + MT * 2 * g + 2 * j + 1] = o[r][j][2 + e] * inv;
-      }
+      for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(f + 2 * j) = make_float2(o[r][j][e] * inv, o[r][j][2 + e] * inv);
     }
   __syncthreads();
-  const int64_t unit = (int64_t)kvh * gridDim.y + tile;
-  float* part = a.part + (unit * a.nsplit + split) * (NR * 8 * FS);
   const int rows = min(NR * 8, a.R - tile * NR * 8);
+  for (int i = threadIdx.x; i < rows * HD; i += TA_THREADS) {
+    const int n = i / HD;
+    float M = TA_NONE, A = 0.f;
+#pragma unroll
+    for (int w = 0; w < TA_WARPS; ++w) M = fmaxf(M, ml[w][n].x);
+#pragma unroll
+    for (int w = 0; w < TA_WARPS; ++w) A += fold[w * NR * 8 * HD + i] * ex2(ml[w][n].x - M);
+    fold[i] = A;
+  }
+  if (threadIdx.x < NR * 8) {
+    float M = TA_NONE, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < TA_WARPS; ++w) M = fmaxf(M, ml[w][threadIdx.x].x);
+#pragma unroll
+    for (int w = 0; w < TA_WARPS; ++w) L += ml[w][threadIdx.x].y * ex2(ml[w][threadIdx.x].x - M);
+    cta_ml[threadIdx.x] = make_float2(M, L);
+  }
+  const int C = (int)cluster_nranks(), rank = (int)cluster_rank_of();
+  const int nclusters = a.nsplit / C;
+  const int64_t unit = (int64_t)kvh * gridDim.y + tile;
   auto store = [&](int n, int d, float v) {
     const int r = tile * NR * 8 + n;
     a.out[((int64_t)(r / a.G) * a.heads + kvh * a.G + r % a.G) * HD + d] = v;
   };
-  for (int i = threadIdx.x; i < rows * HD; i += TA_THREADS) {
-    const int n = i / HD, d = i % HD;
-    float M = TA_NONE, L = 0.f, A = 0.f;
+  // Rank k of the cluster joins rows k, k + C, ... from every rank's shared
+  // memory, in rank order.
+  cluster_barrier();
+  const int mine = rows > rank ? (rows - rank + C - 1) / C : 0;
+  float* part = a.part + unit * nclusters * (NR * 8 * (HD + 2));  // [cluster][row][HD + 2]
+  for (int i = threadIdx.x; i < mine * HD; i += TA_THREADS) {
+    const int n = rank + i / HD * C, d = i % HD;
+    float mk[8], lk[8], ak[8], M = TA_NONE, L = 0.f, A = 0.f;
 #pragma unroll
-    for (int w = 0; w < TA_WARPS; ++w) M = fmaxf(M, fold[(w * NR * 8 + n) * FS]);
-#pragma unroll
-    for (int w = 0; w < TA_WARPS; ++w) {
-      const float* f = fold + (w * NR * 8 + n) * FS;
-      const float k = ex2(f[0] - M);
-      L += f[1] * k;
-      A += f[2 + d] * k;
+    for (int k = 0; k < 8; ++k) {
+      if (k < C) {
+        const float2 x = peer_f2(&cta_ml[n], k);
+        mk[k] = x.x, lk[k] = x.y;
+        ak[k] = peer_f(&fold[n * HD + d], k);
+      } else {
+        mk[k] = TA_NONE, lk[k] = 0.f, ak[k] = 0.f;
+      }
     }
-    if (a.nsplit == 1) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) M = fmaxf(M, mk[k]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float w = ex2(mk[k] - M);
+      L += lk[k] * w, A += ak[k] * w;
+    }
+    if (nclusters == 1) {
       store(n, d, L == 0.f ? 0.f : A / L);
     } else {
-      part[n * FS + 2 + d] = A;
-      if (d == 0) part[n * FS] = M, part[n * FS + 1] = L;
+      float* p = part + ((split / C) * NR * 8 + n) * (HD + 2);
+      p[2 + d] = A;
+      if (d == 0) p[0] = M, p[1] = L;
     }
   }
-  if (a.nsplit == 1) return;
+  cluster_barrier();  // no rank leaves while another reads its memory
+  if (nclusters == 1) return;
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) is_last = atomicAdd(&a.count[unit], 1) == a.nsplit - 1;
+  int* count = a.count + unit * 8 + rank;
+  if (threadIdx.x == 0) is_last = atomicAdd(count, 1) == nclusters - 1;
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  const float* all = a.part + unit * a.nsplit * (NR * 8 * FS);
-  for (int i = threadIdx.x; i < rows * HD; i += TA_THREADS) {
-    const int n = i / HD, d = i % HD;
-    const float* p = all + n * FS;
+  for (int i = threadIdx.x; i < mine * HD; i += TA_THREADS) {  // the last of the clusters, for this rank's rows
+    const int n = rank + i / HD * C, d = i % HD;
+    const float* p = part + n * (HD + 2);
+    constexpr int64_t S = NR * 8 * (HD + 2);
     float M = TA_NONE, L = 0.f, A = 0.f;
-    for (int k = 0; k < a.nsplit; ++k) M = fmaxf(M, __ldcg(p + (int64_t)k * NR * 8 * FS));
-    for (int k = 0; k < a.nsplit; ++k) {
-      const float* f = p + (int64_t)k * NR * 8 * FS;
-      const float w = ex2(__ldcg(f) - M);
-      L += __ldcg(f + 1) * w;
-      A += __ldcg(f + 2 + d) * w;
+#pragma unroll 8
+    for (int k = 0; k < nclusters; ++k) M = fmaxf(M, __ldcg(p + k * S));
+#pragma unroll 8
+    for (int k = 0; k < nclusters; ++k) {
+      const float w = ex2(__ldcg(p + k * S) - M);
+      L += __ldcg(p + k * S + 1) * w;
+      A += __ldcg(p + k * S + 2 + d) * w;
     }
     store(n, d, L == 0.f ? 0.f : A / L);
   }
-  if (threadIdx.x == 0) a.count[unit] = 0;
+  if (threadIdx.x == 0) *count = 0;
 }
 
 struct TreePlan {
-  int nr, tiles, nsplit;
+  int nr, tiles, nsplit, cluster;
   size_t part_off, bytes;
 };
 
 // Rows per CTA: the fewest 8-row tiles (1, 2 or 4) that hold the R rows, at
 // most 32.  Splits: as many CTAs as are resident at once (4, 3 or 2 per SM),
-// each with a group for every warp.
+// each with a group for every warp, in clusters of up to 8 that join their
+// shares in shared memory: of the sizes 1 .. 8 the one that leaves the fewest
+// CTAs unused, the larger of two.  (All splits joined by the last CTA through
+// global memory instead took as long as the rest: 74 splits of 8 rows 70 us of
+// 127, 18 splits of 32 rows 100 us of 122.)
 TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   TreePlan p;
   const int64_t R = (int64_t)tokens * (heads / kv_heads);
@@ -512,9 +578,12 @@ TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   const int64_t most = ((int64_t)ctx + TA_GROUP * TA_WARPS - 1) / (TA_GROUP * TA_WARPS);
   int64_t want = room / units;
   want = want < 1 ? 1 : want > most ? most : want;
-  p.nsplit = (int)want;
-  p.part_off = (16 + (size_t)units * 4 + 255) / 256 * 256;
-  p.bytes = p.part_off + (size_t)units * p.nsplit * p.nr * 8 * (hd + 2) * 4;
+  p.cluster = 1;
+  p.nsplit = 1;
+  for (int c = 1; c <= 8 && c <= want; ++c)
+    if (want / c * c >= p.nsplit) p.cluster = c, p.nsplit = (int)(want / c * c);
+  p.part_off = (16 + (size_t)units * 8 * 4 + 255) / 256 * 256;
+  p.bytes = p.part_off + (size_t)units * (p.nsplit / p.cluster) * p.nr * 8 * (hd + 2) * 4;
   return p;
 }
 
@@ -532,7 +601,21 @@ cudaError_t launch_tree(const TreeArgs& a, const TreePlan& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     attr_set[dev] = true;
   }
-  return launch_pdl_smem(kern, dim3(a.c.kv_heads, p.tiles, p.nsplit), dim3(TA_THREADS), smem, s, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.c.kv_heads, p.tiles, p.nsplit);
+  cfg.blockDim = dim3(TA_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = p.cluster;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 template <int HD>
