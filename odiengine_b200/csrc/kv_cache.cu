@@ -62,17 +62,17 @@ __global__ void __launch_bounds__(128) append_kernel(const float* qkv, int64_t l
     if (r0 + n >= rows) break;
     const float* p = src + (int64_t)(r0 + n) * HD;
     if (VEC && PPL == 2) {
-      const float2 a = *reinterpret_cast<const float2*>(p), b = *reinterpret_cast<const float2*>(p + HALF);
+      const float2 a = __ldcg(reinterpret_cast<const float2*>(p)), b = __ldcg(reinterpret_cast<const float2*>(p + HALF));
       lo[n][0] = a.x, lo[n][PPL - 1] = a.y, hi[n][0] = b.x, hi[n][PPL - 1] = b.y;
     } else {
 #pragma unroll
-      for (int e = 0; e < PPL; ++e) lo[n][e] = p[e], hi[n][e] = p[HALF + e];
+      for (int e = 0; e < PPL; ++e) lo[n][e] = __ldcg(p + e), hi[n][e] = __ldcg(p + HALF + e);
     }
   }
-  const int pos = st->pos;
+  const int pos = __ldcg(&st->pos);
   const int64_t slot = (int64_t)pos + t;
   const bool store = slot >= 0 && slot < cache.ctx;
-  const double p = (double)((int64_t)pos + (depth ? depth[t] : t));
+  const double p = (double)((int64_t)pos + (depth ? __ldcg(depth + t) : t));
   float sn[PPL], cs[PPL];
 #pragma unroll
   for (int e = 0; e < PPL; ++e) {
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvView cache, int start, i
     const uint4* p = reinterpret_cast<const uint4*>(base + (row0 * cpr + i) * (I8 ? 16 : 32));
     raw[u][0] = __ldcs(p);
     if (!I8) raw[u][I8 ? 0 : 1] = __ldcs(p + 1);
-    if (I8) d[u] = reinterpret_cast<const float*>(base + cache.scale_off)[row0 + i / cpr];
+    if (I8) d[u] = __ldcg(reinterpret_cast<const float*>(base + cache.scale_off) + row0 + i / cpr);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -219,10 +219,10 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvView cache, const int* _
   __shared__ int s_src[ODI_CUDA_KV_MOVE_MAX], s_dst[ODI_CUDA_KV_MOVE_MAX];
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t pos = st ? st->pos : 0;
+  const int64_t pos = st ? __ldcg(&st->pos) : 0;
   const int tid = threadIdx.x;
   if (tid < n) {
-    const int64_t a = pos + src[tid], b = pos + dst[tid];
+    const int64_t a = pos + __ldcg(src + tid), b = pos + __ldcg(dst + tid);
     const bool ok = a >= 0 && a < cache.ctx && b >= 0 && b < cache.ctx;
     s_src[tid] = ok ? (int)a : -1;
     s_dst[tid] = ok ? (int)b : -1;
@@ -248,9 +248,9 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvView cache, const int* _
   for (int u = 0; u < 4; ++u) {
     const int i = (tid + u * 256) >> 2;
     if (i < n && s_src[i] >= 0)
-      v[u] = *reinterpret_cast<const uint4*>(rows + (int64_t)s_src[i] * row_bytes + (tid & 3) * 16);
+      v[u] = __ldcg(reinterpret_cast<const uint4*>(rows + (int64_t)s_src[i] * row_bytes + (tid & 3) * 16));
   }
-  if (scales && tid < n && s_src[tid] >= 0) d = scale[s_src[tid]];
+  if (scales && tid < n && s_src[tid] >= 0) d = __ldcg(scale + s_src[tid]);
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < 4; ++u) {

@@ -71,12 +71,12 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
   for (int u = 0; u < VPT; ++u) {
     const int64_t id = first + (u * THREADS + tid) * 4;
     if (id >= 0 && id + 3 < a.V) {
-      v[u] = *reinterpret_cast<const float4*>(in + id);
+      v[u] = __ldcg(reinterpret_cast<const float4*>(in + id));
     } else {
-      v[u].x = id >= 0 && id < a.V ? in[id] : 0.f;
-      v[u].y = id + 1 >= 0 && id + 1 < a.V ? in[id + 1] : 0.f;
-      v[u].z = id + 2 >= 0 && id + 2 < a.V ? in[id + 2] : 0.f;
-      v[u].w = id + 3 >= 0 && id + 3 < a.V ? in[id + 3] : 0.f;
+      v[u].x = id >= 0 && id < a.V ? __ldcg(in + id) : 0.f;
+      v[u].y = id + 1 >= 0 && id + 1 < a.V ? __ldcg(in + id + 1) : 0.f;
+      v[u].z = id + 2 >= 0 && id + 2 < a.V ? __ldcg(in + id + 2) : 0.f;
+      v[u].w = id + 3 >= 0 && id + 3 < a.V ? __ldcg(in + id + 3) : 0.f;
     }
   }
   if (lists) {
@@ -84,16 +84,16 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
     __syncthreads();
     if (a.history) {
       const int* hist = a.history + row * a.history_ld;
-      int n = a.history_len ? a.history_len[row] : a.history_max;
+      int n = a.history_len ? __ldcg(a.history_len + row) : a.history_max;
       n = n < a.history_max ? n : a.history_max;
       for (int i = tid; i < n; i += THREADS) {
-        const int id = hist[i];
+        const int id = __ldcg(hist + i);
         if (id >= lo && id < hi) atomicAdd(&words[id - first], 1u);
       }
       __syncthreads();
     }
     for (int i = tid; i < a.bias_count; i += THREADS) {
-      const int id = a.bias_ids[i];
+      const int id = __ldcg(a.bias_ids + i);
       if (id >= lo && id < hi) {  // the low halves no longer change: the maximum is of the entry
         unsigned* w = &words[id - first];
         atomicMax(w, ((unsigned)(i + 1) << 16) | (*(volatile unsigned*)w & 0xffffu));
@@ -124,13 +124,13 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
             x[e] = __fsub_rn(x[e], __fmul_rn((float)c, a.frequency));
             x[e] = __fsub_rn(x[e], a.presence);
           }
-          if (b) x[e] = __fadd_rn(x[e], a.bias[b - 1]);
+          if (b) x[e] = __fadd_rn(x[e], __ldcg(a.bias + b - 1));
         }
       }
     }
     if (mask) {  // four bits from id0 on; ids before the row's first have no bits
       const int64_t i0 = id0 < 0 ? 0 : id0, i3 = id0 + 3 < a.V ? id0 + 3 : a.V - 1;
-      const unsigned bits = __funnelshift_r(mask[i0 >> 5], mask[i3 >> 5], (unsigned)(i0 & 31)) << (int)(i0 - id0);
+      const unsigned bits = __funnelshift_r(__ldcg(mask + (i0 >> 5)), __ldcg(mask + (i3 >> 5)), (unsigned)(i0 & 31)) << (int)(i0 - id0);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (!((bits >> e) & 1u)) x[e] = -INFINITY;

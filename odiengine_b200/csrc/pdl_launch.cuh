@@ -1,5 +1,10 @@
 // pdl_launch.cuh -- launches of the small kernels with programmatic stream
 // serialisation.
+//
+// A kernel launched this way may be resident before the kernels before it
+// have finished, and its SM's L1 may then hold lines that they go on to
+// change.  The kernels of several drafted tokens therefore read what an
+// earlier kernel may have written past L1 (ld.global.cg).
 #pragma once
 
 #include "common.cuh"

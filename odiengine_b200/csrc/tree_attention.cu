@@ -54,7 +54,6 @@ constexpr float TA_NONE = -3.402823466e38f;  // reference of a row that has seen
 constexpr float TA_TOP = 32768.f;            // a weight past this moves the reference
 constexpr float TA_UNIT = 16.f;              // the largest weight right after that
 constexpr float TA_VMOST = 0x1p120f;         // factor of an int8 row's scales before any was seen
-constexpr float TA_QMAX = 8290000.f;         // |fixed-point q|: three signed digits, the first within 127
 
 struct TreeArgs {
   const float* q;
@@ -65,9 +64,9 @@ struct TreeArgs {
   int mask_words;
   const DecodeState* st;
   int tokens, heads, G, R, nsplit;
-  float scale;
+  float scale_log2;  // scale * log2(e)
   int* count;   // arrivals per (kv head, row tile, cluster rank), zero between launches
-  float* part;  // [kv head][tile][cluster][row][hd + 2]: reference, sum, accumulator
+  float* part;  // [kv head][tile][cluster][row][hd + 4]: reference, sum, -, -, accumulator
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -93,17 +92,18 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// Streaming 16-byte load.
+// Loads of what the kernel before this one may have written: from L2, since
+// a line of this SM's L1 may be older than the programmatic wait.
 __device__ __forceinline__ uint4 ldg16(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint2 ldg8(const void* p) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.cg.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint32_t cluster_nranks() {
@@ -121,11 +121,14 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Rank k's copy of a shared-memory value.
-__device__ __forceinline__ float peer_f(const float* p, int k) {
+__device__ __forceinline__ float4 peer_f4(const float4* p, int k) {
   uint32_t addr;
-  float v;
+  float4 v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(k));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ float2 peer_f2(const float2* p, int k) {
@@ -135,7 +138,23 @@ __device__ __forceinline__ float2 peer_f2(const float2* p, int k) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Which of positions p0 .. p0 + 15 node t sees (t < 0: a row past the last, none).
+__device__ __forceinline__ unsigned seen_bits(const TreeArgs& a, int t, int p0, int pos, int len) {
+  if (t < 0) return 0;
+  const int words = a.mask_words, j0 = p0 - pos, w0 = j0 >> 5;
+  auto word = [&](int w) -> unsigned {
+    if (w < 0) return 0xffffffffu;  // below pos: seen by all
+    if (w >= words) return 0;
+    if (a.mask) return __ldcg(a.mask + (int64_t)t * words + w);
+    const int n = t - 32 * w;  // a chain: bits 0 .. t
+    return n >= 31 ? 0xffffffffu : n < 0 ? 0u : (2u << n) - 1u;
+  };
+  const unsigned bits = __funnelshift_r(word(w0), word(w0 + 1), (unsigned)(j0 & 31)) & 0xffffu;
+  return len - p0 < 16 ? bits & ((1u << (len - p0)) - 1u) : bits;
+}
 
 // Fragment registers of one group: KW words of K per row and lane, VW of V per
 // position and lane, and the words of Q per lane and row tile.
@@ -166,7 +185,7 @@ template <int HD, int NR, bool I8>
 struct TreeSmem {
   using F = Frag<HD, I8>;
   static constexpr int Q = NR * F::QW * 32 * 4;
-  static constexpr int ROWC = NR * 8 * 4;  // per-row factor of the scores
+  static constexpr int ROWC = NR * 8 * 8;  // each row's factor of the scores, and its node
   static constexpr int FOLD = TA_WARPS * NR * 8 * HD * 4;
   static constexpr int BYTES = ROWC + (Q > FOLD ? Q : FOLD);
 };
@@ -178,71 +197,126 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   constexpr int ROWB = HD * (I8 ? 1 : 2);
   extern __shared__ __align__(16) uint8_t ta_smem[];
   float* rowc = reinterpret_cast<float*>(ta_smem);
+  int* rowt = reinterpret_cast<int*>(ta_smem) + NR * 8;
   uint32_t* qf = reinterpret_cast<uint32_t*>(ta_smem + TreeSmem<HD, NR, I8>::ROWC);  // [NR][QW / 4][lane][4]
   float* fold = reinterpret_cast<float*>(qf);                                        // [warp][row][HD], at the end
   __shared__ float2 ml[TA_WARPS][NR * 8], cta_ml[NR * 8];                            // reference and sum of each row
+  __shared__ float fac[NR * 8][8];  // the cluster's ranks' factors of this rank's rows
+  __shared__ float2 own_ml[NR * 8];
   __shared__ int is_last;
   pdl_launch_dependents();
   pdl_wait();
   const int kvh = blockIdx.x, tile = blockIdx.y, split = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int pos = a.st->pos;
+  const int pos = __ldcg(&a.st->pos);
   const int len = (int)max(0ll, min((long long)a.c.ctx, (long long)pos + a.tokens));
   const int ngroups = (len + TA_GROUP - 1) / TA_GROUP;
 
-  // ---- Q: each warp lays out every TA_WARPS-th row: digits, in fragment order
-  for (int n = warp; n < NR * 8; n += TA_WARPS) {
-    const int r = tile * NR * 8 + n;
-    constexpr int PL = HD / 32;
-    float v[PL], am = 0.f;
-    bool ok = true;
+  // the first group is requested before anything else
+  const int64_t head = (int64_t)kvh * a.c.ctx;
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + head * ROWB;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + head * ROWB;
+  const float* ks = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.k) + a.c.scale_off) + head;
+  const float* vsc = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.v) + a.c.scale_off) + head;
+
+  uint32_t kw[2][KW], vw[4][VW];
+  float dk[2], dv[2];
+  auto load_k = [&](int grp) {
 #pragma unroll
-    for (int e = 0; e < PL; ++e) v[e] = 0.f;
-    if (r < a.R) {
-      const float* src = a.q + (int64_t)(r / a.G) * a.ld_q + (int64_t)(kvh * a.G + r % a.G) * HD;
+    for (int i = 0; i < 2; ++i) {
+      const int row = min(grp * TA_GROUP + g + 8 * i, len - 1);  // rows past the end repeat the last: not seen
+      load_words<KW>(kw[i], kb + (int64_t)row * ROWB + c * 16, 64);
+      if (I8) dk[i] = __ldcg(ks + row), dv[i] = __ldcg(vsc + row);
+    }
+  };
+  auto load_v = [&](int grp) {
 #pragma unroll
-      for (int e = 0; e < PL; ++e) v[e] = src[lane * PL + e];
+    for (int i = 0; i < 4; ++i) {
+      const int row = min(grp * TA_GROUP + 2 * c + (i & 1) + 8 * (i >> 1), len - 1);
+      load_words<VW>(vw[i], vb + (int64_t)row * ROWB + g * (ROWB / 8), 16);
+    }
+  };
+  const int step = a.nsplit * TA_WARPS;
+  int grp = split * TA_WARPS + warp;
+  if (grp < ngroups) {
+    load_k(grp);
+    load_v(grp);
+  }
+
+  // ---- Q: warp w lays out rows w, w + TA_WARPS, ... as digits in fragment
+  // order.  Each row is scaled by a power of two: to 2^21 .. 8.35e6 as an
+  // integer (three signed digits hold 127 * (2^16 + 2^8 + 1)), or to 2^13 ..
+  // 2^14 as fp16 pairs; rowc takes the scale back out.
+  {
+    constexpr int PL = HD / 32, RW = NR * 8 / TA_WARPS;
+    float v[RW][PL];
+    int rt[RW];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) {
+      const int r = tile * NR * 8 + warp + i * TA_WARPS;
+      rt[i] = r < a.R ? r / a.G : -1;
+#pragma unroll
+      for (int e = 0; e < PL; ++e) v[i][e] = 0.f;
+      if (r < a.R) {
+        const float* src = a.q + (int64_t)rt[i] * a.ld_q + (int64_t)(kvh * a.G + r % a.G) * HD + lane * PL;
+#pragma unroll
+        for (int e = 0; e < PL; ++e) v[i][e] = __ldcg(src + e);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < PL; ++e) am = fmaxf(am, fabsf(v[e])), ok = ok && finite(v[e]);
+    for (int i = 0; i < RW; ++i) {
+      const int n = warp + i * TA_WARPS;
+      float am = 0.f;
+      bool ok = true;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-    ok = __all_sync(0xffffffffu, ok);
-    // a power of two that brings the largest value to 2^13 .. 2^14; I8 fills its digits instead
-    const int ex = min(max((int)(__float_as_uint(am) >> 23) - 127, -100), 126);
-    const float up = I8 ? TA_QMAX : 8192.f;
-    const float lift = __uint_as_float((uint32_t)(127 - ex) << 23);  // 2^-ex
-    const float unit = am * lift;  // 1 .. 2 (2 .. 4 at the top of the range), less where am is tiny
-    const float f = I8 ? (unit > 0.f ? up / unit : 0.f) : up;
-    if (lane == 0) {
-      const double back = am > 0.f ? (double)a.scale * 1.4426950408889634 / ((double)f * (double)lift) : 0.0;
-      rowc[n] = ok ? (float)back : __int_as_float(0x7fc00000);
-    }
-    uint8_t* dst = reinterpret_cast<uint8_t*>(qf) + (int64_t)(n >> 3) * QW * 128;
-    const int gn = n & 7;
+      for (int e = 0; e < PL; ++e) am = fmaxf(am, fabsf(v[i][e])), ok = ok && finite(v[i][e]);
 #pragma unroll
-    for (int e = 0; e < PL; ++e) {
-      const int d = lane * PL + e;
-      const float x = ok ? v[e] * lift * f : 0.f;
+      for (int x = 16; x; x >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, x));
+      ok = __all_sync(0xffffffffu, ok);
+      int ex = (int)(__float_as_uint(am) >> 23) - 127;  // am = 1 .. 2 times 2^ex
+      if (I8 && am * pow2(-min(max(ex, -100), 126)) > 1.99f) ++ex;
+      ex = min(max(ex, -100), 126);
+      const float lift = pow2(-ex), up = I8 ? 4194304.f : 8192.f;
+      if (lane == 0) {
+        // 1 / up and 2^ex are exact; together they may leave the range, so one after the other
+        rowc[n] = ok ? a.scale_log2 * (1.f / up) * pow2(ex) : __int_as_float(0x7fc00000);
+        rowt[n] = rt[i];
+      }
+      uint8_t* dst = reinterpret_cast<uint8_t*>(qf) + (n >> 3) * QW * 128;
+      const int gn = n & 7;
       if (I8) {
         // dims 16 ch + 4 w + b sit in byte b of word w of piece ch on lane ch % 4
-        const int ch = d >> 4, w = (d >> 2) & 3, b = d & 3;
-        int i = __float2int_rn(x);
+        int dig[PL];
+#pragma unroll
+        for (int e = 0; e < PL; ++e) dig[e] = ok ? __float2int_rn(v[i][e] * lift * up) : 0;
+        const int d = lane * PL, ch = d >> 4, w = (d >> 2) & 3, b = d & 3;
 #pragma unroll
         for (int k = DIG - 1; k >= 0; --k) {
-          const int lo = (int)(int8_t)(i & 255);
-          i = (i - lo) >> 8;
+          uint32_t bytes = 0;
+#pragma unroll
+          for (int e = 0; e < PL; ++e) {
+            const int lo = (int)(int8_t)(dig[e] & 255);
+            dig[e] = (dig[e] - lo) >> 8;
+            bytes |= (uint32_t)(lo & 255) << (8 * e);
+          }
           const int word = k * KW + (ch >> 2) * 4 + w;
-          dst[((word >> 2) * 32 + gn * 4 + (ch & 3)) * 16 + (word & 3) * 4 + b] = (uint8_t)lo;
+          uint8_t* at = dst + ((word >> 2) * 32 + gn * 4 + (ch & 3)) * 16 + (word & 3) * 4 + b;
+          if (PL == 4) *reinterpret_cast<uint32_t*>(at) = bytes;
+          else *reinterpret_cast<uint16_t*>(at) = (uint16_t)bytes;
         }
       } else {
-        const int ch = d >> 3, w = (d >> 1) & 3, b = d & 1;
-        const __half hi = __float2half_rn(x);
-        const __half lo = __float2half_rn(x - __half2float(hi));
 #pragma unroll
-        for (int k = 0; k < DIG; ++k) {
-          const int word = k * KW + (ch >> 2) * 4 + w;
-          *reinterpret_cast<__half*>(dst + ((word >> 2) * 32 + gn * 4 + (ch & 3)) * 16 + (word & 3) * 4 + 2 * b) = k ? lo : hi;
+        for (int e = 0; e < PL; e += 2) {
+          const int d = lane * PL + e, ch = d >> 3, w = (d >> 1) & 3;
+          const float x0 = ok ? v[i][e] * lift * up : 0.f, x1 = ok ? v[i][e + 1] * lift * up : 0.f;
+          const __half2 hi = __floats2half2_rn(x0, x1);
+          const float2 back = __half22float2(hi);
+          const __half2 lo = __floats2half2_rn(x0 - back.x, x1 - back.y);
+#pragma unroll
+          for (int k = 0; k < DIG; ++k) {
+            const int word = k * KW + (ch >> 2) * 4 + w;
+            *reinterpret_cast<uint32_t*>(dst + ((word >> 2) * 32 + gn * 4 + (ch & 3)) * 16 + (word & 3) * 4) = h2u(k ? lo : hi);
+          }
         }
       }
     }
@@ -259,32 +333,6 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
 #pragma unroll
     for (int e = 0; e < 2; ++e) m[r][e] = TA_NONE, l[r][e] = 0.f, vs[r][e] = I8 ? TA_VMOST : TA_UNIT, rc[r][e] = rowc[r * 8 + 2 * c + e];
   }
-  const int64_t head = (int64_t)kvh * a.c.ctx;
-  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + head * ROWB;
-  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + head * ROWB;
-  const float* ks = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.k) + a.c.scale_off) + head;
-  const float* vsc = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.v) + a.c.scale_off) + head;
-
-  uint32_t kw[2][KW], vw[4][VW];
-  float dk[2], dv[2];
-  auto load_k = [&](int grp) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = min(grp * TA_GROUP + g + 8 * i, len - 1);  // rows past the end repeat the last: not seen
-      load_words<KW>(kw[i], kb + (int64_t)row * ROWB + c * 16, 64);
-      if (I8) dk[i] = __ldg(ks + row), dv[i] = __ldg(vsc + row);
-    }
-  };
-  auto load_v = [&](int grp) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = min(grp * TA_GROUP + 2 * c + (i & 1) + 8 * (i >> 1), len - 1);
-      load_words<VW>(vw[i], vb + (int64_t)row * ROWB + g * (ROWB / 8), 16);
-    }
-  };
-  const int step = a.nsplit * TA_WARPS;
-  int grp = split * TA_WARPS + warp;
-  if (grp < ngroups) load_k(grp), load_v(grp);
   for (; grp < ngroups; grp += step) {
     const int p0 = grp * TA_GROUP;
     const bool edge = p0 + TA_GROUP > pos;  // holds tree slots or ends past the last
@@ -351,17 +399,14 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
       bool vis[4] = {true, true, true, true};
       if (edge) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = p0 + g + 8 * (e >> 1);
-          const int row = tile * NR * 8 + r * 8 + 2 * c + (e & 1);
-          bool v = key < len && row < a.R;
-          if (v && key >= pos) {
-            const int t = row / a.G, j = key - pos;
-            v = a.mask ? (a.mask[(int64_t)t * a.mask_words + (j >> 5)] >> (j & 31)) & 1u : j <= t;
+        for (int e = 0; e < 2; ++e) {
+          const unsigned see = seen_bits(a, rowt[r * 8 + 2 * c + e], p0, pos, len);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            vis[2 * i + e] = (see >> (g + 8 * i)) & 1u;
+            if (!vis[2 * i + e]) s[2 * i + e] = -INFINITY;
+            else if (!I8 && ((bad >> (g + 8 * i)) & 1u)) s[2 * i + e] = __int_as_float(0x7fc00000);
           }
-          vis[e] = v;
-          if (!v) s[e] = -INFINITY;
-          else if (!I8 && ((bad >> (g + 8 * (e >> 1))) & 1u)) s[e] = __int_as_float(0x7fc00000);
         }
       }
       float p[4], w[4], top[2];
@@ -398,7 +443,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
           if (I8 && dm > 0.f) {
             // TA_UNIT over a power of two above the largest scale seen
             const int ex = max((int)(__float_as_uint(dm) >> 23) - 126, -116);
-            const float nv = __uint_as_float((uint32_t)(131 - ex) << 23);
+            const float nv = pow2(4 - ex);
             if (nv < vs[r][e]) {
               corr *= nv / vs[r][e];
               vs[r][e] = nv;
@@ -472,64 +517,82 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
     }
   __syncthreads();
   const int rows = min(NR * 8, a.R - tile * NR * 8);
-  for (int i = threadIdx.x; i < rows * HD; i += TA_THREADS) {
-    const int n = i / HD;
-    float M = TA_NONE, A = 0.f;
+  constexpr int V4 = HD / 4;
+  float4* fold4 = reinterpret_cast<float4*>(fold);
+  if (threadIdx.x < NR * 8) {  // each warp's factor, the CTA's reference and sum
+    const int n = threadIdx.x;
+    float M = TA_NONE, L = 0.f;
 #pragma unroll
     for (int w = 0; w < TA_WARPS; ++w) M = fmaxf(M, ml[w][n].x);
 #pragma unroll
-    for (int w = 0; w < TA_WARPS; ++w) A += fold[w * NR * 8 * HD + i] * ex2(ml[w][n].x - M);
-    fold[i] = A;
+    for (int w = 0; w < TA_WARPS; ++w) {
+      const float f = ex2(ml[w][n].x - M);
+      L += ml[w][n].y * f;
+      ml[w][n].x = f;
+    }
+    cta_ml[n] = make_float2(M, L);
   }
-  if (threadIdx.x < NR * 8) {
-    float M = TA_NONE, L = 0.f;
+  __syncthreads();
+  auto add = [](float4& x, const float4& y, float f) {
+    x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+  };
+#pragma unroll 2
+  for (int i = threadIdx.x; i < rows * V4; i += TA_THREADS) {
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < TA_WARPS; ++w) M = fmaxf(M, ml[w][threadIdx.x].x);
-#pragma unroll
-    for (int w = 0; w < TA_WARPS; ++w) L += ml[w][threadIdx.x].y * ex2(ml[w][threadIdx.x].x - M);
-    cta_ml[threadIdx.x] = make_float2(M, L);
+    for (int w = 0; w < TA_WARPS; ++w) add(A, fold4[w * NR * 8 * V4 + i], ml[w][i / V4].x);
+    fold4[i] = A;
   }
   const int C = (int)cluster_nranks(), rank = (int)cluster_rank_of();
   const int nclusters = a.nsplit / C;
   const int64_t unit = (int64_t)kvh * gridDim.y + tile;
-  auto store = [&](int n, int d, float v) {
-    const int r = tile * NR * 8 + n;
-    a.out[((int64_t)(r / a.G) * a.heads + kvh * a.G + r % a.G) * HD + d] = v;
+  auto store = [&](int n, int d4, float4 v, float L) {
+    const int r = tile * NR * 8 + n, t = rowt[n];
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    float* out = a.out + ((int64_t)t * a.heads + kvh * a.G + (r - t * a.G)) * HD + d4 * 4;
+    if (L == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+    if (((uintptr_t)out & 15) == 0) *reinterpret_cast<float4*>(out) = v;
+    else out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
   };
   // Rank k of the cluster joins rows k, k + C, ... from every rank's shared
   // memory, in rank order.
-  cluster_barrier();
+  if (C > 1) cluster_barrier();
+  else __syncthreads();
   const int mine = rows > rank ? (rows - rank + C - 1) / C : 0;
-  float* part = a.part + unit * nclusters * (NR * 8 * (HD + 2));  // [cluster][row][HD + 2]
-  for (int i = threadIdx.x; i < mine * HD; i += TA_THREADS) {
-    const int n = rank + i / HD * C, d = i % HD;
-    float mk[8], lk[8], ak[8], M = TA_NONE, L = 0.f, A = 0.f;
+  constexpr int64_t PS = NR * 8 * (HD + 4);               // a cluster's share: [row][HD + 4]
+  float* part = a.part + unit * nclusters * PS;
+  if (threadIdx.x < mine) {
+    const int n = rank + threadIdx.x * C;
+    float2 x[8];
+    float M = TA_NONE, L = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 8; ++k)
+      if (k < C) x[k] = peer_f2(&cta_ml[n], k), M = fmaxf(M, x[k].x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
       if (k < C) {
-        const float2 x = peer_f2(&cta_ml[n], k);
-        mk[k] = x.x, lk[k] = x.y;
-        ak[k] = peer_f(&fold[n * HD + d], k);
-      } else {
-        mk[k] = TA_NONE, lk[k] = 0.f, ak[k] = 0.f;
+        const float f = ex2(x[k].x - M);
+        L += x[k].y * f;
+        fac[threadIdx.x][k] = f;
       }
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) M = fmaxf(M, mk[k]);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float w = ex2(mk[k] - M);
-      L += lk[k] * w, A += ak[k] * w;
-    }
-    if (nclusters == 1) {
-      store(n, d, L == 0.f ? 0.f : A / L);
-    } else {
-      float* p = part + ((split / C) * NR * 8 + n) * (HD + 2);
-      p[2 + d] = A;
-      if (d == 0) p[0] = M, p[1] = L;
-    }
+    own_ml[threadIdx.x] = make_float2(M, L);
+    if (nclusters > 1) *reinterpret_cast<float2*>(part + (split / C) * PS + n * (HD + 4)) = make_float2(M, L);
   }
-  cluster_barrier();  // no rank leaves while another reads its memory
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine * V4; i += TA_THREADS) {
+    const int s = i / V4, d4 = i % V4, n = rank + s * C;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f), y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < C) y[k] = peer_f4(&fold4[n * V4 + d4], k);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < C) add(A, y[k], fac[s][k]);
+    if (nclusters == 1) store(n, d4, A, own_ml[s].y);
+    else *reinterpret_cast<float4*>(part + (split / C) * PS + n * (HD + 4) + 4 + d4 * 4) = A;
+  }
+  if (C > 1) cluster_barrier();  // no rank leaves while another reads its memory
   if (nclusters == 1) return;
   __threadfence();
   __syncthreads();
@@ -538,20 +601,35 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  for (int i = threadIdx.x; i < mine * HD; i += TA_THREADS) {  // the last of the clusters, for this rank's rows
-    const int n = rank + i / HD * C, d = i % HD;
-    const float* p = part + n * (HD + 2);
-    constexpr int64_t S = NR * 8 * (HD + 2);
-    float M = TA_NONE, L = 0.f, A = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < nclusters; ++k) M = fmaxf(M, __ldcg(p + k * S));
-#pragma unroll 8
-    for (int k = 0; k < nclusters; ++k) {
-      const float w = ex2(__ldcg(p + k * S) - M);
-      L += __ldcg(p + k * S + 1) * w;
-      A += __ldcg(p + k * S + 2 + d) * w;
+  for (int i = threadIdx.x; i < mine * V4; i += TA_THREADS) {  // the last of the clusters, for this rank's rows
+    const int d4 = i % V4, n = rank + i / V4 * C;
+    const float* p = part + n * (HD + 4);
+    float M = TA_NONE, L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < nclusters; k0 += 8) {  // online, eight shares requested together
+      float2 x[8];
+      float4 y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* s = p + (k0 + u) * PS;
+        const bool in = k0 + u < nclusters;
+        x[u] = in ? __ldcg(reinterpret_cast<const float2*>(s)) : make_float2(TA_NONE, 0.f);
+        y[u] = in ? __ldcg(reinterpret_cast<const float4*>(s + 4) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
+      const float f0 = ex2(M - top);
+      L *= f0, A.x *= f0, A.y *= f0, A.z *= f0, A.w *= f0;
+      M = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float f = ex2(x[u].x - M);
+        L += x[u].y * f;
+        add(A, y[u], f);
+      }
     }
-    store(n, d, L == 0.f ? 0.f : A / L);
+    store(n, d4, A, L);
   }
   if (threadIdx.x == 0) *count = 0;
 }
@@ -583,7 +661,7 @@ TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   for (int c = 1; c <= 8 && c <= want; ++c)
     if (want / c * c >= p.nsplit) p.cluster = c, p.nsplit = (int)(want / c * c);
   p.part_off = (16 + (size_t)units * 8 * 4 + 255) / 256 * 256;
-  p.bytes = p.part_off + (size_t)units * (p.nsplit / p.cluster) * p.nr * 8 * (hd + 2) * 4;
+  p.bytes = p.part_off + (size_t)units * (p.nsplit / p.cluster) * p.nr * 8 * (hd + 4) * 4;
   return p;
 }
 
@@ -663,7 +741,7 @@ int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_ca
   a.q = d_q, a.ld_q = ld_q, a.out = d_out, a.c = v, a.mask = d_mask, a.mask_words = (tokens + 31) / 32;
   a.st = reinterpret_cast<const DecodeState*>(d_state);
   a.tokens = tokens, a.heads = heads, a.G = heads / v.kv_heads, a.R = tokens * a.G, a.nsplit = p.nsplit;
-  a.scale = scale;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + 16);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + p.part_off);
   const cudaError_t e = v.hd == 128 ? launch_tree_hd<128>(a, p, (cudaStream_t)stream)
