@@ -236,7 +236,12 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
       load_words<VW>(vw[i], vb + (int64_t)row * ROWB + g * (ROWB / 8), 16);
     }
   };
-  const int step = a.nsplit * TA_WARPS;
+  // The host splits for a full cache: of the clusters that the length at hand
+  // does not give two groups per warp, only the first stays.
+  const int C = (int)cluster_nranks(), rank = (int)cluster_rank_of();
+  const int nclusters = max(1, min(a.nsplit / C, (ngroups + 2 * TA_WARPS * C - 1) / (2 * TA_WARPS * C)));
+  if (split >= nclusters * C) return;
+  const int step = nclusters * C * TA_WARPS;
   int grp = split * TA_WARPS + warp;
   if (grp < ngroups) {
     load_k(grp);
@@ -543,8 +548,6 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
     for (int w = 0; w < TA_WARPS; ++w) add(A, fold4[w * NR * 8 * V4 + i], ml[w][i / V4].x);
     fold4[i] = A;
   }
-  const int C = (int)cluster_nranks(), rank = (int)cluster_rank_of();
-  const int nclusters = a.nsplit / C;
   const int64_t unit = (int64_t)kvh * gridDim.y + tile;
   auto store = [&](int n, int d4, float4 v, float L) {
     const int r = tile * NR * 8 + n, t = rowt[n];
@@ -561,7 +564,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   else __syncthreads();
   const int mine = rows > rank ? (rows - rank + C - 1) / C : 0;
   constexpr int64_t PS = NR * 8 * (HD + 4);               // a cluster's share: [row][HD + 4]
-  float* part = a.part + unit * nclusters * PS;
+  float* part = a.part + unit * (a.nsplit / C) * PS;
   if (threadIdx.x < mine) {
     const int n = rank + threadIdx.x * C;
     float2 x[8];

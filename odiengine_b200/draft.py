@@ -46,34 +46,51 @@ class _LogitsOpts(ctypes.Structure):
                 ("mask_ld", ctypes.c_int64)]
 
 
-def _need(t, dtype, what: str, dev=None):
-    if t.dtype != dtype:
+# The current stream's handle and the current device by index, without building
+# torch's Stream object (2.2 us of a call that launches in 3).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _refuse(t, dtype, what: str, dev, shape) -> None:
+    if t.dtype is not dtype:
         raise TypeError(f"{what}: {dtype} wanted, got {t.dtype}")
-    if not t.is_cuda or (dev is not None and t.device != dev):
-        raise ValueError(f"{what}: must be on {dev or 'a CUDA device'}, is on {t.device}")
+    if t.device != dev or not t.is_cuda:
+        raise ValueError(f"{what}: must be on {dev if dev.type == 'cuda' else 'a CUDA device'}, is on {t.device}")
+    raise ValueError(f"{what}: {shape} wanted, got {tuple(t.shape)} strides {t.stride()}")
 
 
-def _flat(t, dtype, what: str, dev, numel: int = None):
-    _need(t, dtype, what, dev)
-    if not t.is_contiguous() or (numel is not None and t.numel() != numel):
-        raise ValueError(f"{what}: must be contiguous with {numel} values, got {tuple(t.shape)}")
+def _flat(t, dtype, what: str, dev, numel: int) -> int:
+    """The address of a contiguous tensor of numel values."""
+    if t.dtype is not dtype or t.device != dev or t.numel() != numel or not t.is_contiguous() or not t.is_cuda:
+        _refuse(t, dtype, what, dev, f"{numel} contiguous values")
+    return t.data_ptr()
 
 
-def _rows2(t, dtype, what: str, dev, width: int) -> int:
-    """A 2-D tensor of rows of unit stride: its row stride in values."""
-    _need(t, dtype, what, dev)
-    if t.dim() != 2 or t.shape[1] != width or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{what}: rows of {width} adjacent values wanted, got {tuple(t.shape)} strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else max(width, t.stride(0))
+def _rows2(t, dtype, what: str, dev, rows, width: int) -> int:
+    """The stride in values of a 2-D tensor of `rows` rows (None: any) of
+    `width` adjacent values."""
+    if t.dtype is dtype and t.device == dev and t.is_cuda and t.dim() == 2:
+        n, w = t.shape
+        if w == width and (rows is None or n == rows):
+            ld, one = t.stride()
+            if one == 1 or w == 1:
+                return ld if n > 1 and ld >= w else max(ld, w) if n <= 1 else 0
+    _refuse(t, dtype, what, dev, f"{'rows' if rows is None else rows} of {width} adjacent values")
 
 
 def _call(dev, stream, fn, *args) -> None:
     """One library call on `dev`, which need not be the current device."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, (stream or torch.cuda.current_stream(dev)).cuda_stream))
+    i = dev.index
+    s = _raw_stream(i) if stream is None else stream.cuda_stream
+    if _current_device() == i:
+        rc = fn(*args, s)
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, (stream or torch.cuda.current_stream(dev)).cuda_stream))
+        with torch.cuda.device(i):
+            rc = fn(*args, s)
+    if rc:
+        check(rc)
 
 
 class KVCache:
@@ -85,10 +102,11 @@ class KVCache:
         if dtype not in KV_DTYPES:
             raise ValueError(f"cache dtype {dtype!r}: one of {sorted(KV_DTYPES)}")
         need = kv_cache_bytes(dtype, kv_heads, head_dim, ctx)
+        want = torch.float16 if dtype == "f16" else torch.uint8
         for t, n in ((k, "k"), (v, "v")):
-            _need(t, torch.float16 if dtype == "f16" else torch.uint8, f"cache {n}", k.device)
-            if not t.is_contiguous() or t.numel() * t.element_size() < need:
-                raise ValueError(f"cache {n}: {need} contiguous bytes wanted")
+            if t.dtype is not want or t.device != k.device or not t.is_cuda or not t.is_contiguous() \
+                    or t.numel() * t.element_size() < need:
+                _refuse(t, want, f"cache {n}", k.device, f"{need} contiguous bytes")
             if t.data_ptr() % 16:
                 raise ValueError(f"cache {n}: must be 16-byte aligned")
         self.k, self.v, self.dtype = k, v, dtype
@@ -121,9 +139,7 @@ def kv_cache_bytes(dtype: str, kv_heads: int, head_dim: int, ctx: int) -> int:
 
 
 def _state_ptr(state, dev) -> int:
-    if state.dtype != torch.int32 or state.numel() != 4 or state.device != dev or not state.is_contiguous():
-        raise ValueError(f"state: int32[4] (odi_cuda_decode_state) on {dev} wanted")
-    return state.data_ptr()
+    return _flat(state, torch.int32, "state (odi_cuda_decode_state)", dev, 4)
 
 
 def qk_rope_append(qkv, cache: KVCache, state, q_out=None, *, heads: int, theta: float, q_norm=None, k_norm=None,
@@ -132,22 +148,16 @@ def qk_rope_append(qkv, cache: KVCache, state, q_out=None, *, heads: int, theta:
     per head (q_norm / k_norm: head_dim weights, or None), rotated at position
     state.pos + depth[t] (depth int32 [T]; None: t), k and v stored at slot
     state.pos + t.  Returns the rotated q in q_out [T, heads * head_dim]."""
-    dev, hd = cache.device, cache.head_dim
-    ld = _rows2(qkv, torch.float32, "qkv", dev, (heads + 2 * cache.kv_heads) * hd)
+    dev, hd, f32 = cache.device, cache.head_dim, torch.float32
+    ld = _rows2(qkv, f32, "qkv", dev, None, (heads + 2 * cache.kv_heads) * hd)
     T = qkv.shape[0]
     if q_out is None:
-        q_out = torch.empty((T, heads * hd), dtype=torch.float32, device=dev)
-    ld_q = _rows2(q_out, torch.float32, "q_out", dev, heads * hd)
-    if q_out.shape[0] != T:
-        raise ValueError("q_out: one row per row of qkv wanted")
-    for t, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is not None:
-            _flat(t, torch.float32, n, dev, hd)
-    if depth is not None:
-        _flat(depth, torch.int32, "depth", dev, T)
-    _call(dev, stream, lib().odi_cuda_qk_rope_append, qkv.data_ptr(), ld, q_norm.data_ptr() if q_norm is not None else None,
-          k_norm.data_ptr() if k_norm is not None else None, eps, q_out.data_ptr(), ld_q, cache._ref,
-          _state_ptr(state, dev), depth.data_ptr() if depth is not None else None, T, heads, theta)
+        q_out = torch.empty((T, heads * hd), dtype=f32, device=dev)
+    ld_q = _rows2(q_out, f32, "q_out", dev, T, heads * hd)
+    _call(dev, stream, lib().odi_cuda_qk_rope_append, qkv.data_ptr(), ld,
+          None if q_norm is None else _flat(q_norm, f32, "q_norm", dev, hd),
+          None if k_norm is None else _flat(k_norm, f32, "k_norm", dev, hd), eps, q_out.data_ptr(), ld_q, cache._ref,
+          _state_ptr(state, dev), None if depth is None else _flat(depth, torch.int32, "depth", dev, T), T, heads, theta)
     return q_out
 
 
@@ -156,16 +166,15 @@ def kv_read(cache: KVCache, start: int, count: int, k_out=None, v_out=None, stre
     fp16 or fp32 by the outputs' type (default: new fp16 tensors)."""
     dev = cache.device
     if k_out is None and v_out is None:
-        k_out, v_out = (torch.empty((cache.kv_heads, count, cache.head_dim), dtype=torch.float16, device=dev)
+        k_out, v_out = (torch.empty((cache.kv_heads, max(count, 0), cache.head_dim), dtype=torch.float16, device=dev)
                         for _ in range(2))
-    ref = k_out if k_out is not None else v_out
-    if ref.dtype not in (torch.float16, torch.float32):
-        raise TypeError(f"kv_read: outputs are fp16 or fp32, not {ref.dtype}")
-    for t in (k_out, v_out):
-        if t is not None:
-            _flat(t, ref.dtype, "kv_read output", dev, cache.kv_heads * count * cache.head_dim)
-    _call(dev, stream, lib().odi_cuda_kv_read, cache._ref, start, count, k_out.data_ptr() if k_out is not None else None,
-          v_out.data_ptr() if v_out is not None else None, 0 if ref.dtype == torch.float16 else 1)
+    t = (v_out if k_out is None else k_out).dtype
+    if t is not torch.float16 and t is not torch.float32:
+        raise TypeError(f"kv_read: outputs are fp16 or fp32, not {t}")
+    n = cache.kv_heads * max(count, 0) * cache.head_dim
+    _call(dev, stream, lib().odi_cuda_kv_read, cache._ref, start, count,
+          None if k_out is None else _flat(k_out, t, "k_out", dev, n),
+          None if v_out is None else _flat(v_out, t, "v_out", dev, n), 0 if t is torch.float16 else 1)
     return k_out, v_out
 
 
@@ -173,15 +182,13 @@ def kv_move(cache: KVCache, src, dst, state=None, stream=None) -> None:
     """Cache rows src[i] -> dst[i] (int32, at most KV_MOVE_MAX) as if all were
     read before any is written; relative to state.pos, or absolute."""
     dev, n = cache.device, src.numel()
-    _flat(src, torch.int32, "src", dev, n)
-    _flat(dst, torch.int32, "dst", dev, n)
-    _call(dev, stream, lib().odi_cuda_kv_move, cache._ref, src.data_ptr(), dst.data_ptr(), n,
-          _state_ptr(state, dev) if state is not None else None)
+    _call(dev, stream, lib().odi_cuda_kv_move, cache._ref, _flat(src, torch.int32, "src", dev, n),
+          _flat(dst, torch.int32, "dst", dev, n), n, None if state is None else _state_ptr(state, dev))
 
 
 def attention_tree_scratch(cache: KVCache, tokens: int, heads: int):
-    """Zeroed scratch for attention_tree calls of this shape on one stream
-    (any layer; a smaller `tokens` fits too if its own size does)."""
+    """Zeroed scratch for attention_tree calls of this shape on one stream, of
+    any layer."""
     n = lib().odi_cuda_attention_tree_scratch_bytes(tokens, heads, cache.kv_heads, cache.head_dim, cache.ctx)
     if not n:
         raise ValueError(f"attention_tree: no such shape (tokens {tokens}, heads {heads}, kv_heads {cache.kv_heads})")
@@ -193,18 +200,18 @@ def attention_tree(q, cache: KVCache, out=None, state=None, *, heads: int, scale
     """Node t's rotated queries q[t] (fp32 [T, heads * head_dim]) over the
     slots below state.pos and the tree slots of its mask row (int32 / uint32
     [T, ceil(T / 32)], bit j: node t sees node j; None: j <= t)."""
-    dev, hd = cache.device, cache.head_dim
-    ld = _rows2(q, torch.float32, "q", dev, heads * hd)
+    dev, w, f32 = cache.device, heads * cache.head_dim, torch.float32
+    ld = _rows2(q, f32, "q", dev, None, w)
     T = q.shape[0]
     if out is None:
-        out = torch.empty((T, heads * hd), dtype=torch.float32, device=dev)
-    _flat(out, torch.float32, "out", dev, T * heads * hd)
-    if mask is not None and (mask.dtype not in (torch.int32, torch.uint32) or mask.device != dev or not mask.is_contiguous()
-                             or mask.shape != (T, (T + 31) // 32)):
-        raise ValueError(f"mask: int32 words {(T, (T + 31) // 32)} on {dev} wanted")
-    _need(scratch, torch.uint8, "scratch", dev)
-    _call(dev, stream, lib().odi_cuda_attention_tree, q.data_ptr(), ld, cache._ref, out.data_ptr(),
-          mask.data_ptr() if mask is not None else None, _state_ptr(state, dev), T, heads, scale, scratch.data_ptr(),
+        out = torch.empty((T, w), dtype=f32, device=dev)
+    if mask is not None:
+        t = mask.dtype
+        if t is not torch.int32 and t is not torch.uint32:
+            raise TypeError("mask: int32 words wanted")
+        mask = _flat(mask, t, "mask", dev, T * ((T + 31) // 32))
+    _call(dev, stream, lib().odi_cuda_attention_tree, q.data_ptr(), ld, cache._ref, _flat(out, f32, "out", dev, T * w),
+          mask, _state_ptr(state, dev), T, heads, scale, _flat(scratch, torch.uint8, "scratch", dev, scratch.numel()),
           scratch.numel())
     return out
 
@@ -221,45 +228,40 @@ def logits_adjust(logits, out=None, tokens=None, *, scratch=None, history=None, 
     not stored) and their greedy tokens (int32 [rows]; None: not wanted).
     history int32 [rows, H] or [1, H] with history_lens int32 [rows];
     bias_ids / bias [n] for all rows; mask int32 words [rows or 1, ceil(V / 32)]."""
-    dev = logits.device
+    dev, f32, i32 = logits.device, torch.float32, torch.int32
     rows, V = logits.shape
-    ld = _rows2(logits, torch.float32, "logits", dev, V)
-    ld_out = 0
-    if out is not None:
-        ld_out = _rows2(out, torch.float32, "out", dev, V)
-        if out.shape[0] != rows:
-            raise ValueError("out: one row per row of logits wanted")
-    if tokens is not None:
-        _flat(tokens, torch.int32, "tokens", dev, rows)
-        if scratch is None:
-            raise ValueError("logits_adjust: tokens need a scratch (logits_scratch)")
-        _need(scratch, torch.uint8, "scratch", dev)
-    o = _LogitsOpts(repeat_penalty, frequency_penalty, presence_penalty)
+    ld = _rows2(logits, f32, "logits", dev, rows, V)
+    h = hl = ids = bv = mk = None
+    h_ld = H = nb = mk_ld = 0
     if history is not None:
-        o.history_ld = _rows2(history, torch.int32, "history", dev, history.shape[-1])
-        if history.shape[0] not in (1, rows):
-            raise ValueError("history: one row, or one per row of logits")
-        if history.shape[0] == 1:
-            o.history_ld = 0
-        o.history, o.history_max = history.data_ptr(), history.shape[1]
+        n, H = history.shape
+        h_ld = _rows2(history, i32, "history", dev, n, H)
+        if n != rows:
+            if n != 1:
+                raise ValueError("history: one row, or one per row of logits")
+            h_ld = 0
+        h = history.data_ptr()
         if history_lens is not None:
-            _flat(history_lens, torch.int32, "history_lens", dev, rows)
-            o.history_len = history_lens.data_ptr()
-    if bias_ids is not None and bias_ids.numel():
-        n = bias_ids.numel()
-        _flat(bias_ids, torch.int32, "bias_ids", dev, n)
-        _flat(bias, torch.float32, "bias", dev, n)
-        o.bias_ids, o.bias, o.bias_count = bias_ids.data_ptr(), bias.data_ptr(), n
+            hl = _flat(history_lens, i32, "history_lens", dev, rows)
+    if bias_ids is not None:
+        nb = bias_ids.numel()
+        ids, bv = _flat(bias_ids, i32, "bias_ids", dev, nb), _flat(bias, f32, "bias", dev, nb)
     if mask is not None:
-        if mask.dtype not in (torch.int32, torch.uint32):
+        n, t = mask.shape[0], mask.dtype
+        if t is not i32 and t is not torch.uint32:
             raise TypeError("mask: int32 words wanted")
-        o.mask_ld = _rows2(mask, mask.dtype, "mask", dev, (V + 31) // 32)
-        if mask.shape[0] not in (1, rows):
-            raise ValueError("mask: one row, or one per row of logits")
-        if mask.shape[0] == 1:
-            o.mask_ld = 0
-        o.mask = mask.data_ptr()
-    _call(dev, stream, lib().odi_cuda_logits_adjust, logits.data_ptr(), ld, out.data_ptr() if out is not None else None,
-          ld_out, tokens.data_ptr() if tokens is not None else None, rows, V, ctypes.addressof(o),
-          scratch.data_ptr() if scratch is not None else None, scratch.numel() if scratch is not None else 0)
+        mk_ld = _rows2(mask, t, "mask", dev, n, (V + 31) // 32)
+        if n != rows:
+            if n != 1:
+                raise ValueError("mask: one row, or one per row of logits")
+            mk_ld = 0
+        mk = mask.data_ptr()
+    o = _LogitsOpts(repeat_penalty, frequency_penalty, presence_penalty, h, h_ld, hl, H, ids, bv, nb, mk, mk_ld)
+    if tokens is not None and scratch is None:
+        raise ValueError("logits_adjust: tokens need a scratch (logits_scratch)")
+    n = 0 if scratch is None else scratch.numel()
+    _call(dev, stream, lib().odi_cuda_logits_adjust, logits.data_ptr(), ld, None if out is None else out.data_ptr(),
+          0 if out is None else _rows2(out, f32, "out", dev, rows, V),
+          None if tokens is None else _flat(tokens, i32, "tokens", dev, rows), rows, V, ctypes.addressof(o),
+          None if scratch is None else _flat(scratch, torch.uint8, "scratch", dev, n), n)
     return out, tokens
