@@ -70,12 +70,12 @@ struct TreeArgs {
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_h(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -370,36 +370,44 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
       if (I8) {
         int acc[DIG][4];
 #pragma unroll
-        for (int k = 0; k < DIG; ++k) {
+        for (int k = 0; k < DIG; ++k)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[k][e] = 0;
 #pragma unroll
-          for (int w = 0; w < KW; w += 4) {
-            const uint4 b = qr[((k * KW + w) >> 2) * 32];
-            const uint32_t a0[4] = {kw[0][w], kw[1][w], kw[0][w + 1], kw[1][w + 1]};
-            const uint32_t a1[4] = {kw[0][w + 2], kw[1][w + 2], kw[0][w + 3], kw[1][w + 3]};
-            mma_s8(acc[k], a0, b.x, b.y);
-            mma_s8(acc[k], a1, b.z, b.w);
-          }
+        for (int w = 0; w < KW; w += 4) {
+          const uint32_t a0[4] = {kw[0][w], kw[1][w], kw[0][w + 1], kw[1][w + 1]};
+          const uint32_t a1[4] = {kw[0][w + 2], kw[1][w + 2], kw[0][w + 3], kw[1][w + 3]};
+          uint4 b[DIG];
+#pragma unroll
+          for (int k = 0; k < DIG; ++k) b[k] = qr[((k * KW + w) >> 2) * 32];
+#pragma unroll
+          for (int k = 0; k < DIG; ++k) mma_s8(acc[k], a0, b[k].x, b[k].y);
+#pragma unroll
+          for (int k = 0; k < DIG; ++k) mma_s8(acc[k], a1, b[k].z, b[k].w);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)  // digits joined: |digit sums| < 2^21, so each is exact in fp32
           s[e] = fmaf((float)acc[0][e], 65536.f, fmaf((float)acc[1][e], 256.f, (float)acc[DIG - 1][e])) *
                  (finite(dk[e >> 1]) ? dk[e >> 1] : __int_as_float(0x7fc00000)) * rc[r][e & 1];
       } else {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        float acc[2 * DIG][4];  // high and low halves, two chains of each
 #pragma unroll
-        for (int k = DIG - 1; k >= 0; --k)  // the small halves first
+        for (int k = 0; k < 2 * DIG; ++k)
 #pragma unroll
-          for (int w = 0; w < KW; w += 4) {
+          for (int e = 0; e < 4; ++e) acc[k][e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; w += 4) {
+          const uint32_t a0[4] = {kw[0][w], kw[1][w], kw[0][w + 1], kw[1][w + 1]};
+          const uint32_t a1[4] = {kw[0][w + 2], kw[1][w + 2], kw[0][w + 3], kw[1][w + 3]};
+#pragma unroll
+          for (int k = 0; k < DIG; ++k) {
             const uint4 b = qr[((k * KW + w) >> 2) * 32];
-            const uint32_t a0[4] = {kw[0][w], kw[1][w], kw[0][w + 1], kw[1][w + 1]};
-            const uint32_t a1[4] = {kw[0][w + 2], kw[1][w + 2], kw[0][w + 3], kw[1][w + 3]};
-            mma_h(acc, a0, b.x, b.y);
-            mma_h(acc, a1, b.z, b.w);
+            mma_h(acc[2 * k], a0, b.x, b.y);
+            mma_h(acc[2 * k + 1], a1, b.z, b.w);
           }
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = acc[e] * rc[r][e & 1];
+        for (int e = 0; e < 4; ++e) s[e] = (acc[0][e] + acc[1][e] + (acc[2][e] + acc[3][e])) * rc[r][e & 1];
       }
       bool vis[4] = {true, true, true, true};
       if (edge) {
@@ -476,30 +484,38 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
       }
     }
     if (grp + step < ngroups) load_k(grp + step);
+    constexpr int JB = NR == 1 ? 4 : NR == 2 ? 2 : 1;  // independent sums between two products into one
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {  // dims 16 g + 2 j (fragment row g) and + 1 (row g + 8)
-      uint32_t af[4];
-      if (I8) {
-        const int wi = j >> 1;
-        const uint32_t sel = (j & 1) ? 0x7362u : 0x5140u;  // bytes 2j, 2j + 1 of two positions
-        const uint32_t t0 = __byte_perm(vw[0][wi] ^ 0x80808080u, vw[1][wi] ^ 0x80808080u, sel);
-        const uint32_t t1 = __byte_perm(vw[2][wi] ^ 0x80808080u, vw[3][wi] ^ 0x80808080u, sel);
-        const __half2 k = __float2half2_rn(1152.f);  // 1024 + (code + 128) in fp16
-        af[0] = h2u(__hsub2(u2h(__byte_perm(t0, 0x64646464u, 0x4140u)), k));
-        af[1] = h2u(__hsub2(u2h(__byte_perm(t0, 0x64646464u, 0x4342u)), k));
-        af[2] = h2u(__hsub2(u2h(__byte_perm(t1, 0x64646464u, 0x4140u)), k));
-        af[3] = h2u(__hsub2(u2h(__byte_perm(t1, 0x64646464u, 0x4342u)), k));
-      } else {
-        af[0] = __byte_perm(vw[0][j], vw[1][j], 0x5410u);
-        af[1] = __byte_perm(vw[0][j], vw[1][j], 0x7632u);
-        af[2] = __byte_perm(vw[2][j], vw[3][j], 0x5410u);
-        af[3] = __byte_perm(vw[2][j], vw[3][j], 0x7632u);
+    for (int j0 = 0; j0 < MT; j0 += JB) {
+      uint32_t af[JB][4];
+#pragma unroll
+      for (int u = 0; u < JB; ++u) {  // dims 16 g + 2 j (fragment row g) and + 1 (row g + 8)
+        const int j = j0 + u;
+        if (I8) {
+          const int wi = j >> 1;
+          const uint32_t sel = (j & 1) ? 0x7362u : 0x5140u;  // bytes 2j, 2j + 1 of two positions
+          const uint32_t t0 = __byte_perm(vw[0][wi] ^ 0x80808080u, vw[1][wi] ^ 0x80808080u, sel);
+          const uint32_t t1 = __byte_perm(vw[2][wi] ^ 0x80808080u, vw[3][wi] ^ 0x80808080u, sel);
+          const __half2 k = __float2half2_rn(1152.f);  // 1024 + (code + 128) in fp16
+          af[u][0] = h2u(__hsub2(u2h(__byte_perm(t0, 0x64646464u, 0x4140u)), k));
+          af[u][1] = h2u(__hsub2(u2h(__byte_perm(t0, 0x64646464u, 0x4342u)), k));
+          af[u][2] = h2u(__hsub2(u2h(__byte_perm(t1, 0x64646464u, 0x4140u)), k));
+          af[u][3] = h2u(__hsub2(u2h(__byte_perm(t1, 0x64646464u, 0x4342u)), k));
+        } else {
+          af[u][0] = __byte_perm(vw[0][j], vw[1][j], 0x5410u);
+          af[u][1] = __byte_perm(vw[0][j], vw[1][j], 0x7632u);
+          af[u][2] = __byte_perm(vw[2][j], vw[3][j], 0x5410u);
+          af[u][3] = __byte_perm(vw[2][j], vw[3][j], 0x7632u);
+        }
       }
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        mma_h(o[r][j], af, pl[r][0], pl[r][1]);
-        mma_h(o[r][j], af, ph[r][0], ph[r][1]);
-      }
+      for (int u = 0; u < JB; ++u)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) mma_h(o[r][j0 + u], af[u], pl[r][0], pl[r][1]);
+#pragma unroll
+      for (int u = 0; u < JB; ++u)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) mma_h(o[r][j0 + u], af[u], ph[r][0], ph[r][1]);
     }
     if (grp + step < ngroups) load_v(grp + step);
   }
