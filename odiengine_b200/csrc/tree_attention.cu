@@ -12,6 +12,7 @@
 #include "internal.h"
 #include "kv_cache.cuh"
 #include "pdl_launch.cuh"
+#include "tree_attention.cuh"
 
 namespace odi_cuda {
 namespace {
@@ -48,26 +49,10 @@ namespace {
 // up to 2^16 and down to 2^-24.
 constexpr int TA_WARPS = 4;
 constexpr int TA_THREADS = 32 * TA_WARPS;
-constexpr int TA_SMS = 148;
 constexpr int TA_GROUP = 16;
-constexpr float TA_NONE = -3.402823466e38f;  // reference of a row that has seen nothing
+constexpr int TA_TC_ROWS = 8;
 constexpr float TA_TOP = 32768.f;            // a weight past this moves the reference
 constexpr float TA_UNIT = 16.f;              // the largest weight right after that
-constexpr float TA_VMOST = 0x1p120f;         // factor of an int8 row's scales before any was seen
-
-struct TreeArgs {
-  const float* q;
-  int64_t ld_q;
-  float* out;
-  KvView c;
-  const unsigned* mask;
-  int mask_words;
-  const DecodeState* st;
-  int tokens, heads, G, R, nsplit;
-  float scale_log2;  // scale * log2(e)
-  int* count;   // arrivals per (kv head, row tile, cluster rank), zero between launches
-  float* part;  // [kv head][tile][cluster][row][hd + 4]: reference, sum, -, -, accumulator
-};
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -85,13 +70,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 // Loads of what the kernel before this one may have written: from L2, since
 // a line of this SM's L1 may be older than the programmatic wait.
 __device__ __forceinline__ uint4 ldg16(const void* p) {
@@ -106,56 +84,6 @@ __device__ __forceinline__ uint2 ldg8(const void* p) {
   asm volatile("ld.global.cg.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint32_t cluster_nranks() {
-  uint32_t n;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
-  return n;
-}
-__device__ __forceinline__ uint32_t cluster_rank_of() {
-  uint32_t n;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
-  return n;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Rank k's copy of a shared-memory value.
-__device__ __forceinline__ float4 peer_f4(const float4* p, int k) {
-  uint32_t addr;
-  float4 v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(k));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 peer_f2(const float2* p, int k) {
-  uint32_t addr;
-  float2 v;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(k));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
-
-// Which of positions p0 .. p0 + 15 node t sees (t < 0: a row past the last, none).
-__device__ __forceinline__ unsigned seen_bits(const TreeArgs& a, int t, int p0, int pos, int len) {
-  if (t < 0) return 0;
-  const int words = a.mask_words, j0 = p0 - pos, w0 = j0 >> 5;
-  auto word = [&](int w) -> unsigned {
-    if (w < 0) return 0xffffffffu;  // below pos: seen by all
-    if (w >= words) return 0;
-    if (a.mask) return __ldcg(a.mask + (int64_t)t * words + w);
-    const int n = t - 32 * w;  // a chain: bits 0 .. t
-    return n >= 31 ? 0xffffffffu : n < 0 ? 0u : (2u << n) - 1u;
-  };
-  const unsigned bits = __funnelshift_r(word(w0), word(w0 + 1), (unsigned)(j0 & 31)) & 0xffffu;
-  return len - p0 < 16 ? bits & ((1u << (len - p0)) - 1u) : bits;
-}
-
 // Fragment registers of one group: KW words of K per row and lane, VW of V per
 // position and lane, and the words of Q per lane and row tile.
 template <int HD, bool I8>
@@ -201,9 +129,6 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   uint32_t* qf = reinterpret_cast<uint32_t*>(ta_smem + TreeSmem<HD, NR, I8>::ROWC);  // [NR][QW / 4][lane][4]
   float* fold = reinterpret_cast<float*>(qf);                                        // [warp][row][HD], at the end
   __shared__ float2 ml[TA_WARPS][NR * 8], cta_ml[NR * 8];                            // reference and sum of each row
-  __shared__ float fac[NR * 8][8];  // the cluster's ranks' factors of this rank's rows
-  __shared__ float2 own_ml[NR * 8];
-  __shared__ int is_last;
   pdl_launch_dependents();
   pdl_wait();
   const int kvh = blockIdx.x, tile = blockIdx.y, split = blockIdx.z;
@@ -340,7 +265,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   }
   for (; grp < ngroups; grp += step) {
     const int p0 = grp * TA_GROUP;
-    const bool edge = p0 + TA_GROUP > pos;  // holds tree slots or ends past the last
+    const bool edge = p0 + TA_GROUP > min(pos, len);  // holds tree slots, or ends past the last
     unsigned bad = 0;                       // positions of the group whose V is not finite (fp16)
     if (!I8 && edge) {
 #pragma unroll
@@ -564,115 +489,38 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
     for (int w = 0; w < TA_WARPS; ++w) add(A, fold4[w * NR * 8 * V4 + i], ml[w][i / V4].x);
     fold4[i] = A;
   }
-  const int64_t unit = (int64_t)kvh * gridDim.y + tile;
-  auto store = [&](int n, int d4, float4 v, float L) {
-    const int r = tile * NR * 8 + n, t = rowt[n];
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    float* out = a.out + ((int64_t)t * a.heads + kvh * a.G + (r - t * a.G)) * HD + d4 * 4;
-    if (L == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-    v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
-    if (((uintptr_t)out & 15) == 0) *reinterpret_cast<float4*>(out) = v;
-    else out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
-  };
-  // Rank k of the cluster joins rows k, k + C, ... from every rank's shared
-  // memory, in rank order.
-  if (C > 1) cluster_barrier();
-  else __syncthreads();
-  const int mine = rows > rank ? (rows - rank + C - 1) / C : 0;
-  constexpr int64_t PS = NR * 8 * (HD + 4);               // a cluster's share: [row][HD + 4]
-  float* part = a.part + unit * (a.nsplit / C) * PS;
-  if (threadIdx.x < mine) {
-    const int n = rank + threadIdx.x * C;
-    float2 x[8];
-    float M = TA_NONE, L = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < C) x[k] = peer_f2(&cta_ml[n], k), M = fmaxf(M, x[k].x);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < C) {
-        const float f = ex2(x[k].x - M);
-        L += x[k].y * f;
-        fac[threadIdx.x][k] = f;
-      }
-    own_ml[threadIdx.x] = make_float2(M, L);
-    if (nclusters > 1) *reinterpret_cast<float2*>(part + (split / C) * PS + n * (HD + 4)) = make_float2(M, L);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < mine * V4; i += TA_THREADS) {
-    const int s = i / V4, d4 = i % V4, n = rank + s * C;
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f), y[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < C) y[k] = peer_f4(&fold4[n * V4 + d4], k);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < C) add(A, y[k], fac[s][k]);
-    if (nclusters == 1) store(n, d4, A, own_ml[s].y);
-    else *reinterpret_cast<float4*>(part + (split / C) * PS + n * (HD + 4) + 4 + d4 * 4) = A;
-  }
-  if (C > 1) cluster_barrier();  // no rank leaves while another reads its memory
-  if (nclusters == 1) return;
-  __threadfence();
-  __syncthreads();
-  int* count = a.count + unit * 8 + rank;
-  if (threadIdx.x == 0) is_last = atomicAdd(count, 1) == nclusters - 1;
-  __syncthreads();
-  if (!is_last) return;
-  __threadfence();
-  for (int i = threadIdx.x; i < mine * V4; i += TA_THREADS) {  // the last of the clusters, for this rank's rows
-    const int d4 = i % V4, n = rank + i / V4 * C;
-    const float* p = part + n * (HD + 4);
-    float M = TA_NONE, L = 0.f;
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 < nclusters; k0 += 8) {  // online, eight shares requested together
-      float2 x[8];
-      float4 y[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float* s = p + (k0 + u) * PS;
-        const bool in = k0 + u < nclusters;
-        x[u] = in ? __ldcg(reinterpret_cast<const float2*>(s)) : make_float2(TA_NONE, 0.f);
-        y[u] = in ? __ldcg(reinterpret_cast<const float4*>(s + 4) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      float top = M;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
-      const float f0 = ex2(M - top);
-      L *= f0, A.x *= f0, A.y *= f0, A.z *= f0, A.w *= f0;
-      M = top;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float f = ex2(x[u].x - M);
-        L += x[u].y * f;
-        add(A, y[u], f);
-      }
-    }
-    store(n, d4, A, L);
-  }
-  if (threadIdx.x == 0) *count = 0;
+  tree_join<HD, NR * 8, TA_THREADS>(a, rowt, cta_ml, fold, rows, C, rank, nclusters);
 }
 
 struct TreePlan {
-  int nr, tiles, nsplit, cluster;
+  bool tc;                          // the tcgen05 kernel
+  int rows, tiles, nsplit, cluster;  // rows per CTA, row tiles
   size_t part_off, bytes;
 };
 
-// Rows per CTA: the fewest 8-row tiles (1, 2 or 4) that hold the R rows, at
-// most 32.  Splits: as many CTAs as are resident at once (4, 3 or 2 per SM),
-// each with a group for every warp, in clusters of up to 8 that join their
-// shares in shared memory: of the sizes 1 .. 8 the one that leaves the fewest
-// CTAs unused, the larger of two.  (All splits joined by the last CTA through
-// global memory instead took as long as the rest: 74 splits of 8 rows 70 us of
-// 127, 18 splits of 32 rows 100 us of 122.)
+// Which kernel, rows per CTA and splits.  Splits: as many CTAs as are
+// resident at once, each with positions of its own, in clusters of up to 8
+// that join their shares in shared memory: of the sizes 1 .. 8 the one that
+// leaves the fewest CTAs unused, the larger of two.  (All splits joined by the
+// last CTA through global memory instead took as long as the rest: 74 splits
+// of 8 rows 70 us of 127, 18 splits of 32 rows 100 us of 122.)
 TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   TreePlan p;
   const int64_t R = (int64_t)tokens * (heads / kv_heads);
-  p.nr = R <= 8 ? 1 : R <= 16 ? 2 : 4;
-  p.tiles = (int)((R + p.nr * 8 - 1) / (p.nr * 8));
+  p.tc = hd == 128 && R > TA_TC_ROWS;
+  int64_t room, block;
+  if (p.tc) {
+    p.rows = R <= 32 ? 32 : 64;
+    room = TA_SMS;
+    block = 128;
+  } else {
+    p.rows = R <= 8 ? 8 : R <= 16 ? 16 : 32;
+    room = TA_SMS * (p.rows == 8 ? 4 : p.rows == 16 ? 3 : 2);
+    block = TA_GROUP * TA_WARPS;
+  }
+  p.tiles = (int)((R + p.rows - 1) / p.rows);
   const int64_t units = (int64_t)kv_heads * p.tiles;
-  const int64_t room = (int64_t)TA_SMS * (p.nr == 1 ? 4 : p.nr == 2 ? 3 : 2);
-  const int64_t most = ((int64_t)ctx + TA_GROUP * TA_WARPS - 1) / (TA_GROUP * TA_WARPS);
+  const int64_t most = ((int64_t)ctx + block - 1) / block;
   int64_t want = room / units;
   want = want < 1 ? 1 : want > most ? most : want;
   p.cluster = 1;
@@ -680,7 +528,7 @@ TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   for (int c = 1; c <= 8 && c <= want; ++c)
     if (want / c * c >= p.nsplit) p.cluster = c, p.nsplit = (int)(want / c * c);
   p.part_off = (16 + (size_t)units * 8 * 4 + 255) / 256 * 256;
-  p.bytes = p.part_off + (size_t)units * (p.nsplit / p.cluster) * p.nr * 8 * (hd + 4) * 4;
+  p.bytes = p.part_off + (size_t)units * (p.nsplit / p.cluster) * p.rows * (hd + 4) * 4;
   return p;
 }
 
@@ -718,9 +566,9 @@ cudaError_t launch_tree(const TreeArgs& a, const TreePlan& p, cudaStream_t s) {
 template <int HD>
 cudaError_t launch_tree_hd(const TreeArgs& a, const TreePlan& p, cudaStream_t s) {
   if (a.c.dtype == ODI_CUDA_KV_I8)
-    return p.nr == 1 ? launch_tree<HD, 1, true>(a, p, s) : p.nr == 2 ? launch_tree<HD, 2, true>(a, p, s)
+    return p.rows == 8 ? launch_tree<HD, 1, true>(a, p, s) : p.rows == 16 ? launch_tree<HD, 2, true>(a, p, s)
                                                                      : launch_tree<HD, 4, true>(a, p, s);
-  return p.nr == 1 ? launch_tree<HD, 1, false>(a, p, s) : p.nr == 2 ? launch_tree<HD, 2, false>(a, p, s)
+  return p.rows == 8 ? launch_tree<HD, 1, false>(a, p, s) : p.rows == 16 ? launch_tree<HD, 2, false>(a, p, s)
                                                                     : launch_tree<HD, 4, false>(a, p, s);
 }
 
@@ -763,7 +611,8 @@ int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_ca
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + 16);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + p.part_off);
-  const cudaError_t e = v.hd == 128 ? launch_tree_hd<128>(a, p, (cudaStream_t)stream)
+  const cudaError_t e = p.tc ? launch_tree_tc(a, p.rows, p.tiles, p.cluster, static_cast<int*>(d_scratch), (cudaStream_t)stream)
+                        : v.hd == 128 ? launch_tree_hd<128>(a, p, (cudaStream_t)stream)
                                     : launch_tree_hd<64>(a, p, (cudaStream_t)stream);
   return kv_launched(e, "attention_tree");
 }

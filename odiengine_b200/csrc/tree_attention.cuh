@@ -1,0 +1,194 @@
+// tree_attention.cuh -- what the two kernels of tree attention share: their
+// arguments, which positions a node sees, and how the shares of the splits
+// join.
+#pragma once
+
+#include "internal.h"
+#include "kv_cache.cuh"
+
+namespace odi_cuda {
+
+constexpr int TA_SMS = 148;
+constexpr float TA_NONE = -3.402823466e38f;  // reference of a row that has seen nothing
+constexpr float TA_VMOST = 0x1p120f;         // factor of an int8 row's scales before any was seen
+
+struct TreeArgs {
+  const float* q;
+  int64_t ld_q;
+  float* out;
+  KvView c;
+  const unsigned* mask;
+  int mask_words;
+  const DecodeState* st;
+  int tokens, heads, G, R, nsplit;
+  float scale_log2;  // scale * log2(e)
+  int* count;   // arrivals per (kv head, row tile, cluster rank), zero between launches
+  float* part;  // [kv head][tile][cluster][row][hd + 4]: reference, sum, -, -, accumulator
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t cluster_nranks() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank_of() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Rank k's copy of a shared-memory value.
+__device__ __forceinline__ float4 peer_f4(const float4* p, int k) {
+  uint32_t addr;
+  float4 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(k));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 peer_f2(const float2* p, int k) {
+  uint32_t addr;
+  float2 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(p)), "r"(k));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// Which of positions p0 .. p0 + 15 node t sees (t < 0: a row past the last, none).
+__device__ __forceinline__ unsigned seen_bits(const TreeArgs& a, int t, int p0, int pos, int len) {
+  if (t < 0) return 0;
+  const int words = a.mask_words, j0 = p0 - pos, w0 = j0 >> 5;
+  auto word = [&](int w) -> unsigned {
+    if (w < 0) return 0xffffffffu;  // below pos: seen by all
+    if (w >= words) return 0;
+    if (a.mask) return __ldcg(a.mask + (int64_t)t * words + w);
+    const int n = t - 32 * w;  // a chain: bits 0 .. t
+    return n >= 31 ? 0xffffffffu : n < 0 ? 0u : (2u << n) - 1u;
+  };
+  const unsigned bits = __funnelshift_r(word(w0), word(w0 + 1), (unsigned)(j0 & 31)) & 0xffffu;
+  return len - p0 < 16 ? bits & ((1u << (len - p0)) - 1u) : bits;
+}
+
+// Joins the shares of one row tile.  Each CTA's share: reference and sum of
+// row n in cta_ml[n], its accumulator in fold[n * HD ..] (both in shared
+// memory, not yet synchronised).  Rank k of the cluster takes rows k, k + C,
+// ... from every rank's shared memory, in rank order; with several clusters
+// the last to arrive joins their shares in cluster order.  Every order is
+// fixed, so repeats are bit-identical.
+template <int HD, int ROWS, int THREADS>
+__device__ __forceinline__ void tree_join(const TreeArgs& a, const int* rowt, float2* cta_ml, float* fold, int rows,
+                                          int C, int rank, int nclusters) {
+  __shared__ float fac[ROWS][8];  // the cluster's ranks' factors of this rank's rows
+  __shared__ float2 own_ml[ROWS];
+  __shared__ int is_last;
+  constexpr int V4 = HD / 4;
+  float4* fold4 = reinterpret_cast<float4*>(fold);
+  const int kvh = blockIdx.x, tile = blockIdx.y, split = blockIdx.z;
+  const int64_t unit = (int64_t)kvh * gridDim.y + tile;
+  auto add = [](float4& x, const float4& y, float f) {
+    x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+  };
+  auto store = [&](int n, int d4, float4 v, float L) {
+    const int r = tile * ROWS + n, t = rowt[n];
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    float* out = a.out + ((int64_t)t * a.heads + kvh * a.G + (r - t * a.G)) * HD + d4 * 4;
+    if (L == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+    if (((uintptr_t)out & 15) == 0) *reinterpret_cast<float4*>(out) = v;
+    else out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
+  };
+  if (C > 1) cluster_barrier();
+  else __syncthreads();
+  const int mine = rows > rank ? (rows - rank + C - 1) / C : 0;
+  constexpr int64_t PS = ROWS * (HD + 4);               // a cluster's share: [row][HD + 4]
+  float* part = a.part + unit * (a.nsplit / C) * PS;
+  if (threadIdx.x < mine) {
+    const int n = rank + threadIdx.x * C;
+    float2 x[8];
+    float M = TA_NONE, L = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < C) x[k] = peer_f2(&cta_ml[n], k), M = fmaxf(M, x[k].x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < C) {
+        const float f = ex2(x[k].x - M);
+        L += x[k].y * f;
+        fac[threadIdx.x][k] = f;
+      }
+    own_ml[threadIdx.x] = make_float2(M, L);
+    if (nclusters > 1) *reinterpret_cast<float2*>(part + (split / C) * PS + n * (HD + 4)) = make_float2(M, L);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < mine * V4; i += THREADS) {
+    const int s = i / V4, d4 = i % V4, n = rank + s * C;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f), y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < C) y[k] = peer_f4(&fold4[n * V4 + d4], k);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < C) add(A, y[k], fac[s][k]);
+    if (nclusters == 1) store(n, d4, A, own_ml[s].y);
+    else *reinterpret_cast<float4*>(part + (split / C) * PS + n * (HD + 4) + 4 + d4 * 4) = A;
+  }
+  if (C > 1) cluster_barrier();  // no rank leaves while another reads its memory
+  if (nclusters == 1) return;
+  __threadfence();
+  __syncthreads();
+  int* count = a.count + unit * 8 + rank;
+  if (threadIdx.x == 0) is_last = atomicAdd(count, 1) == nclusters - 1;
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  for (int i = threadIdx.x; i < mine * V4; i += THREADS) {  // the last of the clusters, for this rank's rows
+    const int d4 = i % V4, n = rank + i / V4 * C;
+    const float* p = part + n * (HD + 4);
+    float M = TA_NONE, L = 0.f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < nclusters; k0 += 8) {  // online, eight shares requested together
+      float2 x[8];
+      float4 y[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float* s = p + (k0 + u) * PS;
+        const bool in = k0 + u < nclusters;
+        x[u] = in ? __ldcg(reinterpret_cast<const float2*>(s)) : make_float2(TA_NONE, 0.f);
+        y[u] = in ? __ldcg(reinterpret_cast<const float4*>(s + 4) + d4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) top = fmaxf(top, x[u].x);
+      const float f0 = ex2(M - top);
+      L *= f0, A.x *= f0, A.y *= f0, A.z *= f0, A.w *= f0;
+      M = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float f = ex2(x[u].x - M);
+        L += x[u].y * f;
+        add(A, y[u], f);
+      }
+    }
+    store(n, d4, A, L);
+  }
+  if (threadIdx.x == 0) *count = 0;
+}
+
+// The tcgen05 kernel (tree_attention_tc.cu): 32 or 64 rows per CTA.
+cudaError_t launch_tree_tc(const TreeArgs& a, int rows_per_cta, int tiles, int cluster, int* err, cudaStream_t s);
+
+}  // namespace odi_cuda

@@ -432,10 +432,12 @@ def test_attention_nodes_that_see_nothing(dr, dt):
 
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
-@pytest.mark.parametrize("pos,ctx,T", [(-2, 16, 5), (-9, 16, 5), (14, 16, 5), (16, 16, 5), (40, 16, 2)])
+@pytest.mark.parametrize("pos,ctx,T", [(-2, 16, 5), (-9, 16, 5), (14, 16, 5), (16, 16, 5), (40, 16, 2),
+                                        (41, 21, 2), (1000, 20, 3), (1000, 130, 40)])
 def test_attention_slots_outside_the_cache(dr, dt, pos, ctx, T):
     """pos < 0 or a tree past the cache's end: those slots are not seen."""
     check_attention(dr, dt, 64, 4, 2, T, pos, ctx, lambda rng, t: np.ones((t, t), bool))
+    check_attention(dr, dt, 128, 8, 1, T, pos, ctx, lambda rng, t: np.ones((t, t), bool))
 
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
