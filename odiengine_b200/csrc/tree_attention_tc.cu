@@ -104,6 +104,14 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
 // 32 lanes x 16 consecutive columns; complete only after ld_wait.
 __device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
@@ -159,7 +167,7 @@ struct Bars {
   uint64_t v_clean[2];
 };
 // What a group's threads share about its rows.
-struct Group {
+struct alignas(16) Group {
   float c[NT];    // factor of the scores
   float m[NT];    // reference
   float lv[NT];   // log2 of vs
@@ -332,50 +340,61 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     }
   } else if (warp == 1) {
     // ---------------- products ----------------
-    if (lane == 0) {
-      const uint32_t q0 = smem_u32(smem + F::Q_OFF), p0 = smem_u32(smem + F::P_OFF), t0 = smem_u32(smem);
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int n) { ok = ok && mbar_wait(bar, n & 1, err, ERR_TREE_WAIT); };
-      auto scores = [&](int i) {
-        const int t = kseq(i), slot = t % F::SLOTS;
-        wait(&bars.tfull[slot], t / F::SLOTS);
-        for (int u = 0; u < SUBS && ok; ++u) {
-          if (i) wait(&bars.s_free[u], i - 1);
-          if (!ok) break;
-          fence_after();
-          const uint32_t d = tmem + u * F::SUBCOLS, kt = t0 + slot * F::TILE, qt = q0 + u * F::QB;
+    // The whole warp runs the loop, so that descriptors stay in uniform
+    // registers, and one elected thread issues: issued from a lane's branch,
+    // with its operands moved there one by one, an instruction took 170 cycles.
+    const uint32_t q0 = smem_u32(smem + F::Q_OFF), p0 = smem_u32(smem + F::P_OFF), t0 = smem_u32(smem);
+    const uint64_t qd0 = desc(q0, 16), pd0 = desc(p0, 16), kd0 = desc(t0, 16), vd0 = desc(t0, I8 ? 16 : F::TILE / 2);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int n) {
+      ok = ok && mbar_wait(bar, n & 1, err, ERR_TREE_WAIT);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    auto scores = [&](int i) {
+      const int t = kseq(i), slot = t % F::SLOTS;
+      wait(&bars.tfull[slot], t / F::SLOTS);
 #pragma unroll
-          for (int k = 0; k < (I8 ? 4 : 8); ++k) {  // 32 bytes of the contraction per instruction
-            const uint64_t ad = desc(kt + (k >> 2) * (F::TILE / 2), 16) + 2 * (k & 3);
-            const uint64_t bd = desc(qt + (k >> 2) * (F::DQ * NT * 128), 16) + 2 * (k & 3);
-            mma<I8>(d, ad, bd, idesc(I8, false, F::SCOLS), k != 0);
-          }
+      for (int u = 0; u < SUBS; ++u) {
+        if (i) wait(&bars.s_free[u], i - 1);
+        if (!ok) return;
+        fence_after();
+        if (elect_one()) {
+          const uint64_t kd = kd0 + (uint32_t)(slot * (F::TILE >> 4)), qd = qd0 + u * (F::QB >> 4);
+#pragma unroll
+          for (int k = 0; k < (I8 ? 4 : 8); ++k)  // 32 bytes of the contraction per instruction
+            mma<I8>(tmem + u * F::SUBCOLS, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3),
+                    qd + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3), idesc(I8, false, F::SCOLS), k != 0);
           commit(&bars.s_full[u]);
+          if (u == SUBS - 1) commit(&bars.tfree[slot]);
         }
-        if (ok) commit(&bars.tfree[slot]);
-      };
-      if (nb) scores(0);
-      for (int i = 0; i < nb && ok; ++i) {
-        if (i + 1 < nb) scores(i + 1);
-        const int t = vseq(i), slot = t % F::SLOTS;
-        wait(&bars.tfull[slot], t / F::SLOTS);
-        for (int u = 0; u < SUBS && ok; ++u) {
-          wait(&bars.p_full[u], i);
-          if (!ok) break;
-          fence_after();
-          const bool fresh = *reinterpret_cast<volatile int*>(&restart[u]) != 0;
-          const uint32_t d = tmem + u * F::SUBCOLS + F::OCOL, vt = t0 + slot * F::TILE, pt = p0 + u * F::PB;
+        __syncwarp();
+      }
+    };
+    if (nb) scores(0);
+    for (int i = 0; i < nb && ok; ++i) {
+      if (i + 1 < nb) scores(i + 1);
+      const int t = vseq(i), slot = t % F::SLOTS;
+      wait(&bars.tfull[slot], t / F::SLOTS);
+#pragma unroll
+      for (int u = 0; u < SUBS; ++u) {
+        wait(&bars.p_full[u], i);
+        if (!ok) break;
+        fence_after();
+        const uint32_t keep = *reinterpret_cast<volatile int*>(&restart[u]) == 0;
+        if (elect_one()) {
+          const uint64_t vd = vd0 + (uint32_t)(slot * (F::TILE >> 4)), pd = pd0 + u * (F::PB >> 4);
           constexpr int KS = I8 ? 4 : 8, KB = BK / KS * 128;  // bytes of 32 or 16 positions
 #pragma unroll
           for (int k = 0; k < KS; ++k)
-            mma<I8>(d, desc(vt + k * KB, I8 ? 16 : F::TILE / 2), desc(pt + k * KB, 16), idesc(I8, true, F::DP * NT),
-                    !(fresh && k == 0));
+            mma<I8>(tmem + u * F::SUBCOLS + F::OCOL, vd + k * (KB >> 4), pd + k * (KB >> 4), idesc(I8, true, F::DP * NT),
+                    k ? 1u : keep);
           commit(&bars.pv_done[u]);
+          if (u == SUBS - 1) commit(&bars.tfree[slot]);
         }
-        if (ok) commit(&bars.tfree[slot]);
+        __syncwarp();
       }
-      if (!ok) dead = 1;
     }
+    if (!ok) dead = 1;
   } else if (warp >= 4) {
     // ---------------- softmax ----------------
     const int sub = (warp >> 2) - 1, wq = warp & 3, kl = wq * 32 + lane, bar = 1 + sub;
