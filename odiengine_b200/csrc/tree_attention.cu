@@ -492,84 +492,45 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   tree_join<HD, NR * 8, TA_THREADS>(a, rowt, cta_ml, fold, rows, C, rank, nclusters);
 }
 
+// Which kernel and how many rows per CTA; room: CTAs resident at once.
 struct TreePlan {
-  bool tc;                          // the tcgen05 kernel
-  int rows, tiles, nsplit, cluster;  // rows per CTA, row tiles
+  bool tc;  // the tcgen05 kernel
+  int rows, tiles, units;
+  int64_t room, most;  // most: CTAs that a full cache gives positions to, per unit
   size_t part_off, bytes;
 };
 
-// Which kernel, rows per CTA and splits.  Splits: as many CTAs as are
-// resident at once, each with positions of its own, in clusters of up to 8
-// that join their shares in shared memory: of the sizes 1 .. 8 the one that
-// leaves the fewest CTAs unused, the larger of two.  (All splits joined by the
-// last CTA through global memory instead took as long as the rest: 74 splits
-// of 8 rows 70 us of 127, 18 splits of 32 rows 100 us of 122.)
 TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   TreePlan p;
   const int64_t R = (int64_t)tokens * (heads / kv_heads);
   p.tc = hd == 128 && R > TA_TC_ROWS;
-  int64_t room, block;
-  if (p.tc) {
-    p.rows = R <= 32 ? 32 : 64;
-    room = TA_SMS;
-    block = 128;
-  } else {
-    p.rows = R <= 8 ? 8 : R <= 16 ? 16 : 32;
-    room = TA_SMS * (p.rows == 8 ? 4 : p.rows == 16 ? 3 : 2);
-    block = TA_GROUP * TA_WARPS;
-  }
+  p.rows = p.tc ? (R <= 32 ? 32 : 64) : R <= 8 ? 8 : R <= 16 ? 16 : 32;
+  p.room = TA_SMS * (p.tc ? 1 : p.rows == 8 ? 4 : p.rows == 16 ? 3 : 2);
   p.tiles = (int)((R + p.rows - 1) / p.rows);
-  const int64_t units = (int64_t)kv_heads * p.tiles;
-  const int64_t most = ((int64_t)ctx + block - 1) / block;
-  int64_t want = room / units;
-  want = want < 1 ? 1 : want > most ? most : want;
-  p.cluster = 1;
-  p.nsplit = 1;
-  for (int c = 1; c <= 8 && c <= want; ++c)
-    if (want / c * c >= p.nsplit) p.cluster = c, p.nsplit = (int)(want / c * c);
-  p.part_off = (16 + (size_t)units * 8 * 4 + 255) / 256 * 256;
-  p.bytes = p.part_off + (size_t)units * (p.nsplit / p.cluster) * p.rows * (hd + 4) * 4;
+  p.units = kv_heads * p.tiles;
+  const int64_t block = p.tc ? 128 : TA_GROUP * TA_WARPS;
+  p.most = ((int64_t)ctx + block - 1) / block;
+  p.part_off = (16 + (size_t)p.units * 8 * 4 + 255) / 256 * 256;
+  const int64_t splits = p.room / p.units;
+  p.bytes = p.part_off + (size_t)p.units * (splits < 1 ? 1 : splits) * p.rows * (hd + 4) * 4;
   return p;
 }
 
 template <int HD, int NR, bool I8>
-cudaError_t launch_tree(const TreeArgs& a, const TreePlan& p, cudaStream_t s) {
+cudaError_t launch_tree(TreeArgs a, const TreePlan& p, cudaStream_t s) {
   auto kern = tree_attn_kernel<HD, NR, I8>;
-  constexpr int smem = TreeSmem<HD, NR, I8>::BYTES;
-  static bool attr_set[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!attr_set[dev]) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    attr_set[dev] = true;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.c.kv_heads, p.tiles, p.nsplit);
-  cfg.blockDim = dim3(TA_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = p.cluster;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, a);
+  static TreeLaunch state;
+  return launch_tree_clusters(state, (const void*)kern, a, p.tiles, p.units, p.room, p.most, TA_THREADS, TreeSmem<HD, NR, I8>::BYTES, s,
+                              [&](const cudaLaunchConfig_t& cfg) { return cudaLaunchKernelEx(&cfg, kern, a); });
 }
 
 template <int HD>
 cudaError_t launch_tree_hd(const TreeArgs& a, const TreePlan& p, cudaStream_t s) {
   if (a.c.dtype == ODI_CUDA_KV_I8)
     return p.rows == 8 ? launch_tree<HD, 1, true>(a, p, s) : p.rows == 16 ? launch_tree<HD, 2, true>(a, p, s)
-                                                                     : launch_tree<HD, 4, true>(a, p, s);
+                                                                          : launch_tree<HD, 4, true>(a, p, s);
   return p.rows == 8 ? launch_tree<HD, 1, false>(a, p, s) : p.rows == 16 ? launch_tree<HD, 2, false>(a, p, s)
-                                                                    : launch_tree<HD, 4, false>(a, p, s);
+                                                                         : launch_tree<HD, 4, false>(a, p, s);
 }
 
 bool tree_shape_ok(int tokens, int heads, int kv_heads, int hd, int ctx) {
@@ -607,11 +568,11 @@ int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_ca
   TreeArgs a{};
   a.q = d_q, a.ld_q = ld_q, a.out = d_out, a.c = v, a.mask = d_mask, a.mask_words = (tokens + 31) / 32;
   a.st = reinterpret_cast<const DecodeState*>(d_state);
-  a.tokens = tokens, a.heads = heads, a.G = heads / v.kv_heads, a.R = tokens * a.G, a.nsplit = p.nsplit;
+  a.tokens = tokens, a.heads = heads, a.G = heads / v.kv_heads, a.R = tokens * a.G;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + 16);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + p.part_off);
-  const cudaError_t e = p.tc ? launch_tree_tc(a, p.rows, p.tiles, p.cluster, static_cast<int*>(d_scratch), (cudaStream_t)stream)
+  const cudaError_t e = p.tc ? launch_tree_tc(a, p.rows, p.tiles, p.units, p.most, static_cast<int*>(d_scratch), (cudaStream_t)stream)
                         : v.hd == 128 ? launch_tree_hd<128>(a, p, (cudaStream_t)stream)
                                     : launch_tree_hd<64>(a, p, (cudaStream_t)stream);
   return kv_launched(e, "attention_tree");

@@ -189,6 +189,70 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const int* rowt, fl
 }
 
 // The tcgen05 kernel (tree_attention_tc.cu): 32 or 64 rows per CTA.
-cudaError_t launch_tree_tc(const TreeArgs& a, int rows_per_cta, int tiles, int cluster, int* err, cudaStream_t s);
+cudaError_t launch_tree_tc(const TreeArgs& a, int rows_per_cta, int tiles, int units, int64_t most, int* err, cudaStream_t s);
+
+// How many clusters of each size a kernel can have resident, by device.
+// Clusters live inside one GPC, so sizes differ: with one CTA per SM of 148,
+// size 2 fills 148 of them, 4 132, 6 132, 7 105, 8 120.
+struct TreeLaunch {
+  bool attr_set[64] = {};
+  int resident[64][9] = {};  // -1: asked and unknown
+};
+
+// Splits each unit's positions over as many CTAs as are resident at once, in
+// clusters that join their shares in shared memory: the size that keeps the
+// most CTAs busy, or a larger one that loses up to an eighth of them, since the
+// clusters of one unit then join through global memory.  (A second wave costs
+// as much as the first: 24 clusters of 6 where 22 fit took 41 us, not 21.)
+template <typename Launch>
+cudaError_t launch_tree_clusters(TreeLaunch& st, const void* kern, TreeArgs& a, int tiles, int units, int64_t room,
+                                 int64_t most, int threads, int smem, cudaStream_t s, Launch&& launch) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!st.attr_set[dev]) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    st.attr_set[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  int cluster = 1;
+  int64_t best = 1;
+  for (int c = 1; c <= 8; ++c) {
+    if (!st.resident[dev][c]) {
+      cfg.gridDim = dim3(1, 1, c);
+      cfg.numAttrs = 1;
+      attr[0].val.clusterDim.z = c;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      st.resident[dev][c] = n > 0 ? n : -1;
+    }
+    int64_t fit = st.resident[dev][c];
+    if (fit * c > room) fit = room / c;
+    int64_t n = fit / units;
+    if (n * c > most) n = most / c;
+    if (n * c * 8 >= best * 7) cluster = c, best = n * c > best ? n * c : best;
+    if (cluster == c) a.nsplit = (int)(n * c);
+  }
+  if (cluster == 1 && a.nsplit < 1) a.nsplit = 1;
+  cfg.gridDim = dim3(a.c.kv_heads, tiles, a.nsplit);
+  attr[0].val.clusterDim.z = cluster;
+  cfg.numAttrs = 2;
+  return launch(cfg);
+}
 
 }  // namespace odi_cuda

@@ -685,19 +685,9 @@ static EncodeFn encode_fn() {
 }
 
 template <bool I8, int SUBS>
-static cudaError_t launch(const TreeArgs& a, int tiles, int cluster, int* err, cudaStream_t s) {
+static cudaError_t launch(TreeArgs a, int tiles, int units, int64_t most, int* err, cudaStream_t s) {
   using F = Cfg<I8, SUBS>;
   auto kern = tree_tc_kernel<I8, SUBS>;
-  static bool attr_set[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!attr_set[dev]) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
-    if (e != cudaSuccess) return e;
-    attr_set[dev] = true;
-  }
   const EncodeFn enc = encode_fn();
   if (!enc) return cudaErrorNotSupported;
   // rows of all heads as one 2-D tensor; a box is one block (fp16: half of its
@@ -712,29 +702,20 @@ static cudaError_t launch(const TreeArgs& a, int tiles, int cluster, int* err, c
             strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.c.kv_heads, tiles, a.nsplit);
-  cfg.blockDim = dim3(F::THREADS);
-  cfg.dynamicSmemBytes = F::SMEM;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = cluster;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kern, a, err, maps[0], maps[1]);
+  static TreeLaunch state;
+  return launch_tree_clusters(state, (const void*)kern, a, tiles, units, TA_SMS, most, F::THREADS, F::SMEM, s,
+                              [&](const cudaLaunchConfig_t& cfg) {
+                                return cudaLaunchKernelEx(&cfg, kern, a, err, maps[0], maps[1]);
+                              });
 }
 
 }  // namespace ttc
 
-cudaError_t launch_tree_tc(const TreeArgs& a, int rows_per_cta, int tiles, int cluster, int* err, cudaStream_t s) {
+cudaError_t launch_tree_tc(const TreeArgs& a, int rows_per_cta, int tiles, int units, int64_t most, int* err, cudaStream_t s) {
+  const bool one = rows_per_cta == 32;
   if (a.c.dtype == ODI_CUDA_KV_I8)
-    return rows_per_cta == 32 ? ttc::launch<true, 1>(a, tiles, cluster, err, s) : ttc::launch<true, 2>(a, tiles, cluster, err, s);
-  return rows_per_cta == 32 ? ttc::launch<false, 1>(a, tiles, cluster, err, s) : ttc::launch<false, 2>(a, tiles, cluster, err, s);
+    return one ? ttc::launch<true, 1>(a, tiles, units, most, err, s) : ttc::launch<true, 2>(a, tiles, units, most, err, s);
+  return one ? ttc::launch<false, 1>(a, tiles, units, most, err, s) : ttc::launch<false, 2>(a, tiles, units, most, err, s);
 }
 
 }  // namespace odi_cuda
