@@ -68,7 +68,7 @@ __device__ __forceinline__ float2 peer_f2(const float2* p, int k) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// Which of positions p0 .. p0 + 15 node t sees (t < 0: a row past the last, none).
+// Which of positions p0 .. p0 + 31 node t sees (t < 0: a row past the last, none).
 __device__ __forceinline__ unsigned seen_bits(const TreeArgs& a, int t, int p0, int pos, int len) {
   if (t < 0) return 0;
   const int words = a.mask_words, j0 = p0 - pos, w0 = j0 >> 5;
@@ -79,8 +79,8 @@ __device__ __forceinline__ unsigned seen_bits(const TreeArgs& a, int t, int p0, 
     const int n = t - 32 * w;  // a chain: bits 0 .. t
     return n >= 31 ? 0xffffffffu : n < 0 ? 0u : (2u << n) - 1u;
   };
-  const unsigned bits = __funnelshift_r(word(w0), word(w0 + 1), (unsigned)(j0 & 31)) & 0xffffu;
-  return len - p0 < 16 ? bits & ((1u << (len - p0)) - 1u) : bits;
+  const unsigned bits = __funnelshift_r(word(w0), word(w0 + 1), (unsigned)(j0 & 31));
+  return len <= p0 ? 0u : len - p0 < 32 ? bits & ((1u << (len - p0)) - 1u) : bits;
 }
 
 // Joins the shares of one row tile.  Each CTA's share: reference and sum of

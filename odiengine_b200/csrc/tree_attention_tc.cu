@@ -3,11 +3,11 @@
 //
 // The same mathematics, row numbering and splits as tree_attention.cu, for
 // head_dim 128 and more rows than one warp's tile holds.  A CTA takes 32 or 64 rows
-// (one or two groups of 32) of one kv head and every nsplit-th block of 128
+// (two groups of 16 or 32) of one kv head and every nsplit-th block of 128
 // positions:
 //
-//   S^T [128 positions x 32 rows] = K . Q^T     positions as M
-//   O^T [128 dims x 32 rows]     += V^T . P^T   dims as M
+//   S^T [128 positions x NT rows] = K . Q^T     positions as M
+//   O^T [128 dims x NT rows]     += V^T . P^T   dims as M
 //
 // With the cache as the M side every instruction is full whatever the number
 // of rows, K and V are used as TMA leaves them in shared memory (K as a
@@ -16,16 +16,17 @@
 //
 // fp32 results from 16- and 8-bit products, as columns of one instruction:
 //  * int8 cache (kind::i8, exact 32-bit integer sums): q is fixed point in
-//    three signed digits (96 columns), P * (V's row scale) fixed point in four
-//    unsigned digits (128 columns): an integer up to 2^32 in units of 2^-24 of
+//    three signed digits (3 NT columns), P * (V's row scale) fixed point in four
+//    unsigned digits (4 NT columns): an integer up to 2^32 in units of 2^-24 of
 //    the largest weight.
-//  * fp16 cache (kind::f16): q and P are each the sum of two fp16 values (64
+//  * fp16 cache (kind::f16): q and P are each the sum of two fp16 values (2 NT
 //    columns); the high and low halves' sums are added in fp32.
 //
 //   warp 0       TMA producer: tiles K0 K1 V0 K2 V1 ... through one ring
-//   warp 1       tensor memory, and the one thread that issues the products
-//   warps 4-7    rows 0-31: thread = position (tensor memory lane) in the
-//   warps 8-11   softmax, = dim when O is read; rows 32-63
+//   warps 1, 2   issue the products, one warp for each group of rows; warp 1
+//                holds the tensor memory
+//   warps 4-7    the first group: thread = position (tensor memory lane) in the
+//   warps 8-11   softmax, = dim when O is read; the second group
 //
 // While one group of rows is in its softmax the tensor core works for the
 // other.  As in tree_attention.cu m is a reference that moves only when a
@@ -46,11 +47,11 @@ namespace ttc {
 
 constexpr int HD = 128;
 constexpr int BK = 128;  // positions per block
-constexpr int NT = 32;   // rows per softmax group
 constexpr int ERR_TREE_WAIT = 64;
 
-template <bool I8, int SUBS>
+template <bool I8, int NT>
 struct Cfg {
+  static constexpr int SUBS = 2;
   static constexpr int DQ = I8 ? 3 : 2, DP = I8 ? 4 : 2;  // digits of q and P
   static constexpr int TILE = BK * HD * (I8 ? 1 : 2);     // K or V of one block
   static constexpr int SLOTS = I8 ? 8 : 4;
@@ -61,7 +62,7 @@ struct Cfg {
   static constexpr int SMEM = P_OFF + SUBS * PB + 1024;   // + alignment slack
   static constexpr int THREADS = 128 + 128 * SUBS;
   static constexpr int ROWS = NT * SUBS;
-  static constexpr int SCOLS = DQ * NT, OCOL = I8 ? 128 : 64, SUBCOLS = I8 ? 256 : 128;
+  static constexpr int SCOLS = DQ * NT, OCOL = (I8 ? 4 : 2) * NT, SUBCOLS = 2 * OCOL;
   static constexpr int TMEM_COLS = SUBCOLS * SUBS;
   // blocks between two moves of O to registers: 255 * 127 * 128 * 256 < 2^31;
   // the fp32 accumulator truncates, about 2^-26 of the sum per instruction
@@ -147,10 +148,16 @@ __device__ __forceinline__ bool group_any(int id, int n, bool v) {
       : "memory");
   return r != 0;
 }
-// An integer sum below 2^22 in size as fp32: the exponent of 1.5 * 2^23 put
-// on its bits (one integer and one fp32 add; the conversion instruction runs at
-// an eighth of their rate).
-__device__ __forceinline__ float small_int(uint32_t i) { return __uint_as_float(i + 0x4B400000u) - 12582912.f; }
+// h * 2^16 + m * 2^8 + l of digit sums below 2^22 in size, as fp32.  Each gets
+// the exponent of 1.5 * 2^23 by an integer add (the conversion instruction runs
+// at an eighth of the rate); m and l are joined first, to a multiple of 2^8:
+// 2^-22 of a product of ordinary size, which is 2^29 and more.
+__device__ __forceinline__ float join_digits(uint32_t h, uint32_t m, uint32_t l) {
+  constexpr float B = 12582912.f;
+  const float hf = __uint_as_float(h + 0x4B400000u) - B;
+  const float ml = fmaf(__uint_as_float(m + 0x4B400000u), 256.f, __uint_as_float(l + 0x4B400000u)) - B * 257.f;
+  return fmaf(hf, 65536.f, ml);
+}
 // fp32 -> unsigned with the same order
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -167,24 +174,28 @@ struct Bars {
   uint64_t v_clean[2];
 };
 // What a group's threads share about its rows.
+template <int NT>
 struct alignas(16) Group {
   float c[NT];    // factor of the scores
   float m[NT];    // reference
   float lv[NT];   // log2 of vs
   float vs[NT];   // factor of the weights (int8: of weight * scale)
   float fo[NT], fl[NT];  // factors of O and of the sums when the reference moves
-  uint32_t mx[4][NT], dm[4][NT], need[4];
+  uint32_t mx[4][32], dm[4][32], need[4];
+  float lv_top;          // the largest lv
+  int lv_same;           // all lv are equal
 };
 
-template <bool I8, int SUBS>
-__global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
+template <bool I8, int NT>
+__global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
     tree_tc_kernel(const TreeArgs a, int* err, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
-  using F = Cfg<I8, SUBS>;
+  using F = Cfg<I8, NT>;
+  constexpr int SUBS = F::SUBS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Bars<SUBS> bars;
-  __shared__ Group groups[SUBS];
+  __shared__ Group<NT> groups[SUBS];
   __shared__ int rowt[F::ROWS];
   __shared__ float2 cta_ml[F::ROWS];
   __shared__ uint32_t tmem_slot;
@@ -197,7 +208,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
 
   pdl_launch_dependents();
   if (tid == 0) {
-    for (int i = 0; i < 8; ++i) mbar_init(&bars.tfull[i], 1), mbar_init(&bars.tfree[i], 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&bars.tfull[i], 1), mbar_init(&bars.tfree[i], SUBS);
     for (int i = 0; i < SUBS; ++i) {
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.s_free[i], 128);
@@ -264,12 +275,13 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       const float lift = pow2(-ex), up = I8 ? 4194304.f : 8192.f;
       const int sub = n / NT, ln = n % NT;
       if (lane == 0) {
-        Group& gr = groups[sub];
+        Group<NT>& gr = groups[sub];
         gr.c[ln] = ok ? a.scale_log2 * (1.f / up) * pow2(ex) : __int_as_float(0x7fc00000);
         gr.m[ln] = TA_NONE;
         gr.lv[ln] = I8 ? 120.f : 4.f;
         gr.vs[ln] = I8 ? TA_VMOST : 16.f;
         gr.fo[ln] = gr.fl[ln] = 1.f;
+        if (ln == 0) gr.lv_top = I8 ? 120.f : 4.f, gr.lv_same = 1;
         rowt[n] = rt[i];
       }
       uint8_t* q = smem + F::Q_OFF + sub * F::QB;
@@ -338,12 +350,13 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       for (int u = t < F::SLOTS ? 0 : t - F::SLOTS; u < t; ++u)
         mbar_wait(&bars.tfull[u % F::SLOTS], (u / F::SLOTS) & 1, err, ERR_TREE_WAIT);
     }
-  } else if (warp == 1) {
+  } else if (warp <= SUBS) {
     // ---------------- products ----------------
     // The whole warp runs the loop, so that descriptors stay in uniform
     // registers, and one elected thread issues: issued from a lane's branch,
     // with its operands moved there one by one, an instruction took 170 cycles.
-    const uint32_t q0 = smem_u32(smem + F::Q_OFF), p0 = smem_u32(smem + F::P_OFF), t0 = smem_u32(smem);
+    const int u = warp - 1;  // one warp for each group of rows: neither waits for the other's softmax
+    const uint32_t q0 = smem_u32(smem + F::Q_OFF + u * F::QB), p0 = smem_u32(smem + F::P_OFF + u * F::PB), t0 = smem_u32(smem);
     const uint64_t qd0 = desc(q0, 16), pd0 = desc(p0, 16), kd0 = desc(t0, 16), vd0 = desc(t0, I8 ? 16 : F::TILE / 2);
     bool ok = true;
     auto wait = [&](uint64_t* bar, int n) {
@@ -353,52 +366,46 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     auto scores = [&](int i) {
       const int t = kseq(i), slot = t % F::SLOTS;
       wait(&bars.tfull[slot], t / F::SLOTS);
+      if (i) wait(&bars.s_free[u], i - 1);
+      if (!ok) return;
+      fence_after();
+      if (elect_one()) {
+        const uint64_t kd = kd0 + (uint32_t)(slot * (F::TILE >> 4));
 #pragma unroll
-      for (int u = 0; u < SUBS; ++u) {
-        if (i) wait(&bars.s_free[u], i - 1);
-        if (!ok) return;
-        fence_after();
-        if (elect_one()) {
-          const uint64_t kd = kd0 + (uint32_t)(slot * (F::TILE >> 4)), qd = qd0 + u * (F::QB >> 4);
-#pragma unroll
-          for (int k = 0; k < (I8 ? 4 : 8); ++k)  // 32 bytes of the contraction per instruction
-            mma<I8>(tmem + u * F::SUBCOLS, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3),
-                    qd + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3), idesc(I8, false, F::SCOLS), k != 0);
-          commit(&bars.s_full[u]);
-          if (u == SUBS - 1) commit(&bars.tfree[slot]);
-        }
-        __syncwarp();
+        for (int k = 0; k < (I8 ? 4 : 8); ++k)  // 32 bytes of the contraction per instruction
+          mma<I8>(tmem + u * F::SUBCOLS, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3),
+                  qd0 + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3), idesc(I8, false, F::SCOLS), k != 0);
+        commit(&bars.s_full[u]);
+        commit(&bars.tfree[slot]);
       }
+      __syncwarp();
     };
     if (nb) scores(0);
     for (int i = 0; i < nb && ok; ++i) {
       if (i + 1 < nb) scores(i + 1);
       const int t = vseq(i), slot = t % F::SLOTS;
       wait(&bars.tfull[slot], t / F::SLOTS);
+      wait(&bars.p_full[u], i);
+      if (!ok) break;
+      fence_after();
+      const uint32_t keep = *reinterpret_cast<volatile int*>(&restart[u]) == 0;
+      if (elect_one()) {
+        const uint64_t vd = vd0 + (uint32_t)(slot * (F::TILE >> 4));
+        constexpr int KS = I8 ? 4 : 8, KB = BK / KS * 128;  // bytes of 32 or 16 positions
 #pragma unroll
-      for (int u = 0; u < SUBS; ++u) {
-        wait(&bars.p_full[u], i);
-        if (!ok) break;
-        fence_after();
-        const uint32_t keep = *reinterpret_cast<volatile int*>(&restart[u]) == 0;
-        if (elect_one()) {
-          const uint64_t vd = vd0 + (uint32_t)(slot * (F::TILE >> 4)), pd = pd0 + u * (F::PB >> 4);
-          constexpr int KS = I8 ? 4 : 8, KB = BK / KS * 128;  // bytes of 32 or 16 positions
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-            mma<I8>(tmem + u * F::SUBCOLS + F::OCOL, vd + k * (KB >> 4), pd + k * (KB >> 4), idesc(I8, true, F::DP * NT),
-                    k ? 1u : keep);
-          commit(&bars.pv_done[u]);
-          if (u == SUBS - 1) commit(&bars.tfree[slot]);
-        }
-        __syncwarp();
+        for (int k = 0; k < KS; ++k)
+          mma<I8>(tmem + u * F::SUBCOLS + F::OCOL, vd + k * (KB >> 4), pd0 + k * (KB >> 4), idesc(I8, true, F::DP * NT),
+                  k ? 1u : keep);
+        commit(&bars.pv_done[u]);
+        commit(&bars.tfree[slot]);
       }
+      __syncwarp();
     }
     if (!ok) dead = 1;
   } else if (warp >= 4) {
     // ---------------- softmax ----------------
     const int sub = (warp >> 2) - 1, wq = warp & 3, kl = wq * 32 + lane, bar = 1 + sub;
-    Group& gr = groups[sub];
+    Group<NT>& gr = groups[sub];
     const uint32_t s_tm = tmem + sub * F::SUBCOLS + ((uint32_t)(wq * 32) << 16), o_tm = s_tm + F::OCOL;
     uint8_t* prow = smem + F::P_OFF + sub * F::PB + kl * 128;
     const float* ks = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.k) + a.c.scale_off) + head;
@@ -452,7 +459,8 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       __syncwarp();
       fence_after();
       float s[NT];
-      const float dkk = finite(dk) ? dk : nan;
+      // a row whose scale of K or V is not finite gives NaN to who sees it
+      const float dkk = finite(dk) && finite(dv) ? dk : nan, dvv = finite(dv) ? dv : 0.f;
 #pragma unroll
       for (int c0 = 0; c0 < NT; c0 += 16) {
         uint32_t r[F::DQ][16];
@@ -462,10 +470,9 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
           if (I8)
-            s[c0 + n] = fmaf(small_int(r[0][n]), 65536.f, fmaf(small_int(r[1][n]), 256.f, small_int(r[F::DQ - 1][n]))) * dkk *
-                        gr.c[c0 + n];
+            s[c0 + n] = join_digits(r[0][n], r[1][n], r[F::DQ - 1][n]) * dkk;
           else
-            s[c0 + n] = (__uint_as_float(r[0][n]) + __uint_as_float(r[1][n])) * gr.c[c0 + n];
+            s[c0 + n] = __uint_as_float(r[0][n]) + __uint_as_float(r[1][n]);
         }
       }
       fence_before();
@@ -476,8 +483,9 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         if (!I8) {
           // V rows that are past the end or not finite leave the tile; who
           // sees such a row gets NaN through its score, nobody else meets it.
-          // The first group does it, the second waits (it is at most one block
-          // behind: its P of this block is awaited before the next but one).
+          // The first group does it and the second waits: two such tiles on, the
+          // first is held until the second group's products on this one are done
+          // (the tile's slot).
           if (sub == 0) {
             const int t = vseq(i), slot = t % F::SLOTS;
             ok = mbar_wait(&bars.tfull[slot], (t / F::SLOTS) & 1, err, ERR_TREE_WAIT) && ok;
@@ -503,16 +511,12 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           }
           ++edges;
         }
-        const int j = key - pos, w = j >> 5;
-        if (key >= len) vis = 0;
-        else if (j >= 0) {
-          vis = 0;
-          for (int n = 0; n < NT; ++n) {
-            const int t = rowt[sub * NT + n];
-            bool see = t >= 0;
-            if (see) see = a.mask ? (__ldcg(a.mask + (int64_t)t * a.mask_words + w) >> (j & 31)) & 1u : j <= t;
-            vis |= (uint32_t)see << n;
-          }
+        // lane n: which of the warp's 32 positions row n sees; then its transpose
+        const uint32_t rowsee = lane < NT ? seen_bits(a, rowt[sub * NT + lane], p0 + wq * 32, pos, len) : 0u;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const uint32_t b = __ballot_sync(0xffffffffu, (rowsee >> k) & 1u);
+          if (lane == k) vis = b;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -520,25 +524,29 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           else if (!I8 && bad) s[n] = nan;
         }
       }
-      // does a weight leave its range?  int8: digits hold weight * scale * vs below 2^32
-      const float ldv = I8 ? __log2f(dv) : 0.f;
+      // does a weight leave its range?  int8: digits hold weight * scale * vs
+      // below 2^32 (lv_top is the bound of every row's vs)
       constexpr float TOP = I8 ? 31.f : 11.f;
+      const float ldv = I8 ? __log2f(dvv) : 0.f;
       float top = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float x = s[n] - gr.m[n];
-        top = fmaxf(top, I8 ? fmaxf(x - 29.f, x + (ldv + gr.lv[n])) : x);
+      for (int n = 0; n < NT; n += 4) {
+        const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[n]), m4 = *reinterpret_cast<const float4*>(&gr.m[n]);
+        top = fmaxf(top, fmaxf(fmaf(s[n], c4.x, -m4.x), fmaf(s[n + 1], c4.y, -m4.y)));
+        top = fmaxf(top, fmaxf(fmaf(s[n + 2], c4.z, -m4.z), fmaf(s[n + 3], c4.w, -m4.w)));
       }
+      if (I8) top += fmaxf(-29.f, ldv + gr.lv_top);
       if (!ok) dead = 1;
       bool fresh = i == 0;
       __syncwarp();
       if (group_any(bar, 128, top > TOP || !ok)) {
         if (group_any(bar, 128, *reinterpret_cast<volatile int*>(&dead) != 0)) break;
         uint32_t mx = 0, dm = 0, need = 0;
-        const uint32_t dvb = I8 && finite(dv) ? __float_as_uint(dv) : 0u;
+        const uint32_t dvb = I8 ? __float_as_uint(dvv) : 0u;
+#pragma unroll
         for (int n = 0; n < NT; ++n) {  // lane n keeps row n
-          const float sn = s[n], x = sn - gr.m[n];
-          const bool over = (I8 ? fmaxf(x - 29.f, x + (ldv + gr.lv[n])) : x) > TOP;
+          const float sn = s[n] * gr.c[n], x = fmaf(s[n], gr.c[n], -gr.m[n]);
+          const bool over = (I8 ? x + fmaxf(-29.f, ldv + gr.lv[n]) : x) > TOP;
           const uint32_t hi = __reduce_max_sync(0xffffffffu, sn == sn ? ordered(sn) : 0u);
           const uint32_t dmn = I8 ? __reduce_max_sync(0xffffffffu, (vis >> n) & 1u ? dvb : 0u) : 0u;
           if (__any_sync(0xffffffffu, over)) need |= 1u << n;
@@ -549,25 +557,36 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         if (lane == 0) gr.need[wq] = need;
         group_sync(bar, 128);
         if (wq == 0) {
-          const int n = lane;
-          float fo = 1.f, fl = 1.f;
-          if (((gr.need[0] | gr.need[1] | gr.need[2] | gr.need[3]) >> n) & 1u) {  // each row by itself
-            const float mn = fmaxf(gr.m[n], unordered(max(max(gr.mx[0][n], gr.mx[1][n]), max(gr.mx[2][n], gr.mx[3][n]))));
-            fo = fl = ex2(gr.m[n] - mn);
-            gr.m[n] = mn;
-            if (I8) {
-              const uint32_t d = max(max(gr.dm[0][n], gr.dm[1][n]), max(gr.dm[2][n], gr.dm[3][n]));
-              const int ex = max((int)(d >> 23) - 126, -96);  // a power of two above the largest scale
-              if (d && (float)(24 - ex) < gr.lv[n]) {
-                const float nv = pow2(24 - ex);
-                fo *= nv / gr.vs[n];
-                gr.vs[n] = nv;
-                gr.lv[n] = (float)(24 - ex);
+          if (lane < NT) {
+            const int n = lane;
+            float fo = 1.f, fl = 1.f;
+            if (((gr.need[0] | gr.need[1] | gr.need[2] | gr.need[3]) >> n) & 1u) {  // each row by itself
+              const float mn = fmaxf(gr.m[n], unordered(max(max(gr.mx[0][n], gr.mx[1][n]), max(gr.mx[2][n], gr.mx[3][n]))));
+              fo = fl = ex2(gr.m[n] - mn);
+              gr.m[n] = mn;
+              if (I8) {
+                const uint32_t d = max(max(gr.dm[0][n], gr.dm[1][n]), max(gr.dm[2][n], gr.dm[3][n]));
+                const int ex = max((int)(d >> 23) - 126, -96);  // a power of two above the largest scale
+                if (d && (float)(24 - ex) < gr.lv[n]) {
+                  const float nv = pow2(24 - ex);
+                  fo *= nv / gr.vs[n];
+                  gr.vs[n] = nv;
+                  gr.lv[n] = (float)(24 - ex);
+                }
               }
             }
+            gr.fo[n] = fo, gr.fl[n] = fl;
           }
-          gr.fo[n] = fo;
-          gr.fl[n] = fl;
+          __syncwarp();
+          if (I8) {
+            float hi = gr.lv[lane % NT], lo = hi;
+#pragma unroll
+            for (int x = 16; x; x >>= 1) {
+              hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, x));
+              lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, x));
+            }
+            if (lane == 0) gr.lv_top = hi, gr.lv_same = hi == lo;
+          }
         }
         group_sync(bar, 128);
         flush(i, true);
@@ -580,19 +599,27 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       // weights, as digits, into the operand tile
       if (i && !mbar_wait(&bars.pv_done[sub], (i - 1) & 1, err, ERR_TREE_WAIT)) dead = 1;
       if (I8) {
-        const float dvv = finite(dv) ? dv : 0.f, one = finite(dv) ? 1.f : nan;
+        const float dvs = dvv * gr.vs[0];
+        const bool same = gr.lv_same;
 #pragma unroll
         for (int c0 = 0; c0 < NT; c0 += 16) {
           uint32_t w[4][4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
+            const int n0 = c0 + 4 * q;
+            const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[n0]), m4 = *reinterpret_cast<const float4*>(&gr.m[n0]);
+            const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, mm[4] = {m4.x, m4.y, m4.z, m4.w};
+            float f[4] = {dvs, dvs, dvs, dvs};
+            if (!same) {
+              const float4 v4 = *reinterpret_cast<const float4*>(&gr.vs[n0]);
+              f[0] = dvv * v4.x, f[1] = dvv * v4.y, f[2] = dvv * v4.z, f[3] = dvv * v4.w;
+            }
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int n = c0 + 4 * q + e;
-              const float p = ex2(s[n] - gr.m[n]);
-              l[n] += (vis >> n) & 1u ? p * one : 0.f;
-              const float x = fmaf(p, dvv * gr.vs[n], 0.5f);  // 0.5 .. 2^32: its integer part is the weight
+              const float p = ex2(fmaf(s[n0 + e], cc[e], -mm[e]));
+              l[n0 + e] += p;
+              const float x = fmaf(p, f[e], 0.5f);  // 0.5 .. 2^32: its integer part is the weight
               const float h = __fmaf_rz(x, 0x1p-16f, 8388608.f);
               hi[e] = __float_as_uint(h);
               lo[e] = __float_as_uint(__fadd_rz(fmaf(-65536.f, h - 8388608.f, x), 8388608.f));
@@ -606,25 +633,31 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(prow + (((2 * k + c0 / 16) ^ (kl & 7)) << 4)) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+            *reinterpret_cast<uint4*>(prow + (((k * (NT / 16) + c0 / 16) ^ (kl & 7)) << 4)) =
+                make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
         }
       } else {
 #pragma unroll
         for (int c0 = 0; c0 < NT; c0 += 8) {
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int n = c0 + 2 * e;
-            const float pa = ex2(s[n] - gr.m[n]), pb = ex2(s[n + 1] - gr.m[n + 1]);
-            l[n] += pa, l[n + 1] += pb;
-            const float xa = pa * 16.f, xb = pb * 16.f;
-            const __half2 h = __floats2half2_rn(xa, xb);
-            const float2 back = __half22float2(h);
-            hi[e] = h2u(h);
-            lo[e] = h2u(__floats2half2_rn(xa - back.x, xb - back.y));
+          for (int h = 0; h < 2; ++h) {
+            const int n0 = c0 + 4 * h;
+            const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[n0]), m4 = *reinterpret_cast<const float4*>(&gr.m[n0]);
+            const float p0 = ex2(fmaf(s[n0], c4.x, -m4.x)), p1 = ex2(fmaf(s[n0 + 1], c4.y, -m4.y));
+            const float p2 = ex2(fmaf(s[n0 + 2], c4.z, -m4.z)), p3 = ex2(fmaf(s[n0 + 3], c4.w, -m4.w));
+            l[n0] += p0, l[n0 + 1] += p1, l[n0 + 2] += p2, l[n0 + 3] += p3;
+            const float x[4] = {p0 * 16.f, p1 * 16.f, p2 * 16.f, p3 * 16.f};
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const __half2 t = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+              const float2 back = __half22float2(t);
+              hi[2 * h + e] = h2u(t);
+              lo[2 * h + e] = h2u(__floats2half2_rn(x[2 * e] - back.x, x[2 * e + 1] - back.y));
+            }
           }
           *reinterpret_cast<uint4*>(prow + (((c0 / 8) ^ (kl & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(prow + (((4 + c0 / 8) ^ (kl & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(prow + (((NT / 8 + c0 / 8) ^ (kl & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
       if (kl == 0) *reinterpret_cast<volatile int*>(&restart[sub]) = fresh;
@@ -641,12 +674,16 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
   float* fold = reinterpret_cast<float*>(smem);  // [row][HD]: the ring is idle
   if (warp >= 4) {
     const int sub = (warp >> 2) - 1, wq = warp & 3;
-    Group& gr = groups[sub];
+    Group<NT>& gr = groups[sub];
 #pragma unroll
     for (int n = 0; n < NT; ++n) fold[(sub * NT + n) * HD + wq * 32 + lane] = facc[n] * (1.f / gr.vs[n]);  // a power of two
-    // sums over the group's 128 positions: after 31 exchanges lane n of a warp holds row n's
+    // sums over the group's 128 positions: after the exchanges lane n (and n +
+    // 16, of 16 rows) of a warp holds row n's
+    if (NT == 16)
 #pragma unroll
-    for (int w = 16; w; w >>= 1) {
+      for (int n = 0; n < NT; ++n) l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+#pragma unroll
+    for (int w = NT / 2; w; w >>= 1) {
       const bool up = lane & w;
 #pragma unroll
       for (int n = 0; n < w; ++n) {
@@ -656,7 +693,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     }
     gr.mx[wq][lane] = __float_as_uint(l[0]);
     group_sync(1 + sub, 128);
-    if (wq == 0) {
+    if (wq == 0 && lane < NT) {
       float L = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) L += __uint_as_float(gr.mx[k][lane]);
@@ -684,10 +721,10 @@ static EncodeFn encode_fn() {
   return fn;
 }
 
-template <bool I8, int SUBS>
+template <bool I8, int NT>
 static cudaError_t launch(TreeArgs a, int tiles, int units, int64_t most, int* err, cudaStream_t s) {
-  using F = Cfg<I8, SUBS>;
-  auto kern = tree_tc_kernel<I8, SUBS>;
+  using F = Cfg<I8, NT>;
+  auto kern = tree_tc_kernel<I8, NT>;
   const EncodeFn enc = encode_fn();
   if (!enc) return cudaErrorNotSupported;
   // rows of all heads as one 2-D tensor; a box is one block (fp16: half of its
@@ -714,8 +751,8 @@ static cudaError_t launch(TreeArgs a, int tiles, int units, int64_t most, int* e
 cudaError_t launch_tree_tc(const TreeArgs& a, int rows_per_cta, int tiles, int units, int64_t most, int* err, cudaStream_t s) {
   const bool one = rows_per_cta == 32;
   if (a.c.dtype == ODI_CUDA_KV_I8)
-    return one ? ttc::launch<true, 1>(a, tiles, units, most, err, s) : ttc::launch<true, 2>(a, tiles, units, most, err, s);
-  return one ? ttc::launch<false, 1>(a, tiles, units, most, err, s) : ttc::launch<false, 2>(a, tiles, units, most, err, s);
+    return one ? ttc::launch<true, 16>(a, tiles, units, most, err, s) : ttc::launch<true, 32>(a, tiles, units, most, err, s);
+  return one ? ttc::launch<false, 16>(a, tiles, units, most, err, s) : ttc::launch<false, 32>(a, tiles, units, most, err, s);
 }
 
 }  // namespace odi_cuda
