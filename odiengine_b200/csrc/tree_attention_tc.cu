@@ -2,37 +2,41 @@
 // sm_100a tensor cores (tcgen05.mma, accumulators in tensor memory).
 //
 // The same mathematics, row numbering and splits as tree_attention.cu, for
-// head_dim 128 and more rows than one warp's tile holds.  A CTA takes 32 or 64 rows
-// (two groups of 16 or 32) of one kv head and every nsplit-th block of 128
-// positions:
+// head_dim 128 and more rows per kv head than one 8-row tile.  A CTA takes 32
+// or 64 rows (one or two groups of 32) of one kv head and every nsplit-th
+// block of 128 positions:
 //
-//   S^T [128 positions x NT rows] = K . Q^T     positions as M
-//   O^T [128 dims x NT rows]     += V^T . P^T   dims as M
+//   S^T [128 positions x 32 rows] = K . Q^T     positions as M
+//   O^T [128 dims x 32 rows]     += V^T . P^T   dims as M
 //
 // With the cache as the M side every instruction is full whatever the number
 // of rows, K and V are used as TMA leaves them in shared memory (K as a
-// K-major operand, V, the same bytes order, as an MN-major one), and each is
+// K-major operand, V, in the same byte order, as an MN-major one), and each is
 // fetched once for all the CTA's rows.
 //
 // fp32 results from 16- and 8-bit products, as columns of one instruction:
 //  * int8 cache (kind::i8, exact 32-bit integer sums): q is fixed point in
-//    three signed digits (3 NT columns), P * (V's row scale) fixed point in four
-//    unsigned digits (4 NT columns): an integer up to 2^32 in units of 2^-24 of
+//    three signed digits (96 columns), P * (V's row scale) fixed point in four
+//    unsigned digits (128 columns): an integer up to 2^32 in units of 2^-24 of
 //    the largest weight.
-//  * fp16 cache (kind::f16): q and P are each the sum of two fp16 values (2 NT
+//  * fp16 cache (kind::f16): q and P are each the sum of two fp16 values (64
 //    columns); the high and low halves' sums are added in fp32.
 //
 //   warp 0       TMA producer: tiles K0 K1 V0 K2 V1 ... through one ring
 //   warps 1, 2   issue the products, one warp for each group of rows; warp 1
 //                holds the tensor memory
-//   warps 4-7    the first group: thread = position (tensor memory lane) in the
-//   warps 8-11   softmax, = dim when O is read; the second group
+//   warps 4-11   a warpgroup per group of rows (of one group, one for each half
+//                of its rows): thread = position (tensor memory lane) in the
+//                softmax, = dim when O is read
 //
 // While one group of rows is in its softmax the tensor core works for the
-// other.  As in tree_attention.cu m is a reference that moves only when a
+// others.  As in tree_attention.cu m is a reference that moves only when a
 // weight would leave its range; then (and every few blocks, so that integer
 // sums cannot overflow and fp32 sums stay short) O moves from tensor memory
 // to fp32 registers and starts again.
+//
+// The softmax bounds the kernel: about 12 instructions per score (packed fp32
+// pairs where two scores share an operation).
 //
 // Every wait is bounded; a wait that gives up sets the error word, all roles
 // leave their loops, copies in flight are waited for and the tensor memory is
@@ -47,11 +51,12 @@ namespace ttc {
 
 constexpr int HD = 128;
 constexpr int BK = 128;  // positions per block
+constexpr int NT = 32;   // rows per group
 constexpr int ERR_TREE_WAIT = 64;
 
-template <bool I8, int NT>
+template <bool I8, int SUBS_>
 struct Cfg {
-  static constexpr int SUBS = 2;
+  static constexpr int SUBS = SUBS_;                      // groups of rows
   static constexpr int DQ = I8 ? 3 : 2, DP = I8 ? 4 : 2;  // digits of q and P
   static constexpr int TILE = BK * HD * (I8 ? 1 : 2);     // K or V of one block
   static constexpr int SLOTS = I8 ? 8 : 4;
@@ -60,7 +65,14 @@ struct Cfg {
   static constexpr int Q_OFF = SLOTS * TILE;
   static constexpr int P_OFF = Q_OFF + SUBS * QB;
   static constexpr int SMEM = P_OFF + SUBS * PB + 1024;   // + alignment slack
-  static constexpr int THREADS = 128 + 128 * SUBS;
+  static constexpr int HALVES = SUBS == 1 ? 2 : 1;        // softmax threads per position and group
+  static constexpr int NH = NT / HALVES;                  // rows of a group per softmax thread
+  static constexpr int GT = 128 * HALVES;                 // softmax threads of a group
+  static constexpr int THREADS = 128 + SUBS * GT;
+  // with two groups the launch's registers (168 a thread) are shared out anew
+  // between the first warpgroup and the softmax's
+  static constexpr int REGS_LAUNCH = 168, REGS_FIRST = 40, REGS_SOFT = 232;
+  static_assert(SUBS == 1 || 128 * REGS_FIRST + SUBS * GT * REGS_SOFT <= THREADS * REGS_LAUNCH, "register split");
   static constexpr int ROWS = NT * SUBS;
   static constexpr int SCOLS = DQ * NT, OCOL = (I8 ? 4 : 2) * NT, SUBCOLS = 2 * OCOL;
   static constexpr int TMEM_COLS = SUBCOLS * SUBS;
@@ -113,22 +125,20 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(r));
   return r != 0;
 }
-// 32 lanes x 16 consecutive columns; complete only after ld_wait.
-__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
+// 32 lanes x 8 consecutive columns; complete only after ld_wait.
+__device__ __forceinline__ void ld8(uint32_t addr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
 }
 // The registers of the loads before it pass through, so no use moves ahead of it.
 template <int N>
-__device__ __forceinline__ void ld_wait(uint32_t (&r)[N][16]) {
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[N][8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int k = 0; k < N; ++k)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(r[k][i]));
+    for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(r[k][i]));
 }
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -148,16 +158,26 @@ __device__ __forceinline__ bool group_any(int id, int n, bool v) {
       : "memory");
   return r != 0;
 }
-// h * 2^16 + m * 2^8 + l of digit sums below 2^22 in size, as fp32.  Each gets
-// the exponent of 1.5 * 2^23 by an integer add (the conversion instruction runs
-// at an eighth of the rate); m and l are joined first, to a multiple of 2^8:
-// 2^-22 of a product of ordinary size, which is 2^29 and more.
-__device__ __forceinline__ float join_digits(uint32_t h, uint32_t m, uint32_t l) {
+// The integer sums of S start from the bits of 1.5 * 2^23, so that they are read
+// back as the fp32 value 1.5 * 2^23 + sum (|sum| < 2^22) without a conversion,
+// which runs at an eighth of an add's rate.  Two scores at a time: h * 2^16 + m *
+// 2^8 + l; m and l are joined first, to a multiple of 2^8, which is 2^-21 of a
+// product of ordinary size (2^29 and more).
+constexpr uint32_t S_START = 0x4B400000u;
+__device__ __forceinline__ float2 f2(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 bits2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 join_digits(float2 h, float2 m, float2 l) {
   constexpr float B = 12582912.f;
-  const float hf = __uint_as_float(h + 0x4B400000u) - B;
-  const float ml = fmaf(__uint_as_float(m + 0x4B400000u), 256.f, __uint_as_float(l + 0x4B400000u)) - B * 257.f;
-  return fmaf(hf, 65536.f, ml);
+  const float2 ml = __fadd2_rn(__ffma2_rn(m, f2(256.f), l), f2(-B * 257.f));
+  return __ffma2_rn(__fadd2_rn(h, f2(-B)), f2(65536.f), ml);
 }
+// 16 columns of this lane set to v.
+__device__ __forceinline__ void st16(uint32_t addr, uint32_t v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(addr),
+               "r"(v)
+               : "memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // fp32 -> unsigned with the same order
 __device__ __forceinline__ uint32_t ordered(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -174,28 +194,27 @@ struct Bars {
   uint64_t v_clean[2];
 };
 // What a group's threads share about its rows.
-template <int NT>
 struct alignas(16) Group {
-  float c[NT];    // factor of the scores
-  float m[NT];    // reference
-  float lv[NT];   // log2 of vs
-  float vs[NT];   // factor of the weights (int8: of weight * scale)
+  float c[NT];           // factor of the scores, positive
+  float nm[NT];          // minus the reference
+  float lv[NT];          // log2 of vs
+  float vs[NT];          // int8: factor of weight * scale
   float fo[NT], fl[NT];  // factors of O and of the sums when the reference moves
-  uint32_t mx[4][32], dm[4][32], need[4];
-  float lv_top;          // the largest lv
-  int lv_same;           // all lv are equal
+  uint32_t mx[4][NT], dm[4][NT], need[2][4];
+  float lv_top[2];       // the largest lv of each half
+  int lv_same[2];        // all lv of the half are equal
 };
 
-template <bool I8, int NT>
-__global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
+template <bool I8, int SUBS>
+__global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     tree_tc_kernel(const TreeArgs a, int* err, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
-  using F = Cfg<I8, NT>;
-  constexpr int SUBS = F::SUBS;
+  using F = Cfg<I8, SUBS>;
+  constexpr int NH = F::NH, HALVES = F::HALVES, GT = F::GT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Bars<SUBS> bars;
-  __shared__ Group<NT> groups[SUBS];
+  __shared__ Group groups[SUBS];
   __shared__ int rowt[F::ROWS];
   __shared__ float2 cta_ml[F::ROWS];
   __shared__ uint32_t tmem_slot;
@@ -211,8 +230,8 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
     for (int i = 0; i < 8; ++i) mbar_init(&bars.tfull[i], 1), mbar_init(&bars.tfree[i], SUBS);
     for (int i = 0; i < SUBS; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.s_free[i], 128);
-      mbar_init(&bars.p_full[i], 128);
+      mbar_init(&bars.s_free[i], GT);
+      mbar_init(&bars.p_full[i], GT);
       mbar_init(&bars.pv_done[i], 1);
     }
     mbar_init(&bars.v_clean[0], 128);
@@ -274,21 +293,22 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
       ex = min(max(ex, -100), 126);
       const float lift = pow2(-ex), up = I8 ? 4194304.f : 8192.f;
       const int sub = n / NT, ln = n % NT;
+      const float sign = a.scale_log2 < 0.f ? -1.f : a.scale_log2 > 0.f ? 1.f : 0.f;  // c stays positive
       if (lane == 0) {
-        Group<NT>& gr = groups[sub];
-        gr.c[ln] = ok ? a.scale_log2 * (1.f / up) * pow2(ex) : __int_as_float(0x7fc00000);
-        gr.m[ln] = TA_NONE;
-        gr.lv[ln] = I8 ? 120.f : 4.f;
-        gr.vs[ln] = I8 ? TA_VMOST : 16.f;
+        Group& gr = groups[sub];
+        gr.c[ln] = ok ? fmaxf(fabsf(a.scale_log2) * (1.f / up) * pow2(ex), 1e-37f) : __int_as_float(0x7fc00000);
+        gr.nm[ln] = -TA_NONE;
+        gr.lv[ln] = I8 ? 120.f : 0.f;
+        gr.vs[ln] = I8 ? TA_VMOST : 1.f;
         gr.fo[ln] = gr.fl[ln] = 1.f;
-        if (ln == 0) gr.lv_top = I8 ? 120.f : 4.f, gr.lv_same = 1;
+        if (ln % NH == 0) gr.lv_top[ln / NH] = I8 ? 120.f : 0.f, gr.lv_same[ln / NH] = 1;
         rowt[n] = rt[i];
       }
       uint8_t* q = smem + F::Q_OFF + sub * F::QB;
       if (I8) {
         int dig[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dig[e] = ok ? __float2int_rn(v[i][e] * lift * up) : 0;
+        for (int e = 0; e < 4; ++e) dig[e] = ok ? __float2int_rn(v[i][e] * lift * up * sign) : 0;
 #pragma unroll
         for (int k = F::DQ - 1; k >= 0; --k) {  // digit 0 the highest
           uint32_t bytes = 0;
@@ -305,7 +325,7 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
         uint32_t w[2][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float x0 = ok ? v[i][2 * e] * lift * up : 0.f, x1 = ok ? v[i][2 * e + 1] * lift * up : 0.f;
+          const float x0 = ok ? v[i][2 * e] * lift * up * sign : 0.f, x1 = ok ? v[i][2 * e + 1] * lift * up * sign : 0.f;
           const __half2 hi = __floats2half2_rn(x0, x1);
           const float2 back = __half22float2(hi);
           w[0][e] = h2u(hi);
@@ -326,7 +346,10 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
   fence_after();
   const uint32_t tmem = tmem_slot;
 
-  float facc[NT], l[NT];
+  float facc[NH];
+  float2 l2[NH / 2];
+  if (warp < 4) {
+    if (SUBS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_FIRST));
   if (warp == 0) {
     // ---------------- producer ----------------
     if (lane == 0) {
@@ -355,8 +378,9 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
     // The whole warp runs the loop, so that descriptors stay in uniform
     // registers, and one elected thread issues: issued from a lane's branch,
     // with its operands moved there one by one, an instruction took 170 cycles.
-    const int u = warp - 1;  // one warp for each group of rows: neither waits for the other's softmax
+    const int u = warp - 1;  // one warp for each group: neither waits for the other's softmax
     const uint32_t q0 = smem_u32(smem + F::Q_OFF + u * F::QB), p0 = smem_u32(smem + F::P_OFF + u * F::PB), t0 = smem_u32(smem);
+    const uint32_t d0 = tmem + u * F::SUBCOLS;
     const uint64_t qd0 = desc(q0, 16), pd0 = desc(p0, 16), kd0 = desc(t0, 16), vd0 = desc(t0, I8 ? 16 : F::TILE / 2);
     bool ok = true;
     auto wait = [&](uint64_t* bar, int n) {
@@ -366,15 +390,15 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
     auto scores = [&](int i) {
       const int t = kseq(i), slot = t % F::SLOTS;
       wait(&bars.tfull[slot], t / F::SLOTS);
-      if (i) wait(&bars.s_free[u], i - 1);
+      wait(&bars.s_free[u], i);
       if (!ok) return;
       fence_after();
       if (elect_one()) {
         const uint64_t kd = kd0 + (uint32_t)(slot * (F::TILE >> 4));
 #pragma unroll
         for (int k = 0; k < (I8 ? 4 : 8); ++k)  // 32 bytes of the contraction per instruction
-          mma<I8>(tmem + u * F::SUBCOLS, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3),
-                  qd0 + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3), idesc(I8, false, F::SCOLS), k != 0);
+          mma<I8>(d0, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3), qd0 + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3),
+                  idesc(I8, false, F::SCOLS), I8 || k != 0);
         commit(&bars.s_full[u]);
         commit(&bars.tfree[slot]);
       }
@@ -394,25 +418,46 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
         constexpr int KS = I8 ? 4 : 8, KB = BK / KS * 128;  // bytes of 32 or 16 positions
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          mma<I8>(tmem + u * F::SUBCOLS + F::OCOL, vd + k * (KB >> 4), pd0 + k * (KB >> 4), idesc(I8, true, F::DP * NT),
-                  k ? 1u : keep);
+          mma<I8>(d0 + F::OCOL, vd + k * (KB >> 4), pd0 + k * (KB >> 4), idesc(I8, true, F::DP * NT), k ? 1u : keep);
         commit(&bars.pv_done[u]);
         commit(&bars.tfree[slot]);
       }
       __syncwarp();
     }
     if (!ok) dead = 1;
-  } else if (warp >= 4) {
+  }
+    // A warp of this group that is done must not take registers back before the
+    // softmax warps have had theirs: they would wait for good.
+    __syncwarp();
+    if (SUBS == 2) {
+      group_sync(4, F::THREADS);
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REGS_LAUNCH));
+    }
+  } else {
     // ---------------- softmax ----------------
-    const int sub = (warp >> 2) - 1, wq = warp & 3, kl = wq * 32 + lane, bar = 1 + sub;
-    Group<NT>& gr = groups[sub];
-    const uint32_t s_tm = tmem + sub * F::SUBCOLS + ((uint32_t)(wq * 32) << 16), o_tm = s_tm + F::OCOL;
+    if (SUBS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REGS_SOFT));
+    const int sub = HALVES == 2 ? 0 : (warp >> 2) - 1, half = HALVES == 2 ? (warp >> 2) - 1 : 0, wq = warp & 3, kl = wq * 32 + lane, bar = 1 + sub;
+    const int h0 = half * NH;  // this thread's rows: h0 .. h0 + NH - 1 of the group
+    Group& gr = groups[sub];
+    const uint32_t s_tm = tmem + sub * F::SUBCOLS + h0 + ((uint32_t)(wq * 32) << 16), o_tm = s_tm + F::OCOL;
     uint8_t* prow = smem + F::P_OFF + sub * F::PB + kl * 128;
+    const int psw = kl & 7;  // swizzle of this row's 16-byte pieces
     const float* ks = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.k) + a.c.scale_off) + head;
     const float* vsc = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.v) + a.c.scale_off) + head;
     const float nan = __int_as_float(0x7fc00000);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) facc[n] = 0.f, l[n] = 0.f;
+    for (int n = 0; n < NH; ++n) facc[n] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NH / 2; ++n) l2[n] = f2(0.f);
+    if (I8) {
+#pragma unroll
+      for (int k = 0; k < F::DQ; ++k)
+#pragma unroll
+        for (int n = 0; n < NH; n += 16) st16(s_tm + k * NT + n, S_START);
+      st_wait();
+    }
+    fence_before();
+    mbar_arrive(&bars.s_free[sub]);
     float dk = 0.f, dv = 0.f, dk_next = 0.f, dv_next = 0.f;
     auto request = [&](int i) {
       const int key = min((split + i * stride) * BK + kl, len - 1);
@@ -426,13 +471,13 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
         __syncwarp();
         fence_after();
 #pragma unroll
-        for (int c0 = 0; c0 < NT; c0 += 16) {
-          uint32_t r[F::DP][16];
+        for (int c0 = 0; c0 < NH; c0 += 8) {
+          uint32_t r[F::DP][8];
 #pragma unroll
-          for (int k = 0; k < F::DP; ++k) ld16(o_tm + k * NT + c0, r[k]);
+          for (int k = 0; k < F::DP; ++k) ld8(o_tm + k * NT + c0, r[k]);
           ld_wait(r);
 #pragma unroll
-          for (int n = 0; n < 16; ++n) {
+          for (int n = 0; n < 8; ++n) {
             float x;
             if (I8)  // digit 0 the lowest
               x = fmaf((float)(int)r[F::DP - 1][n], 16777216.f,
@@ -446,7 +491,10 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
       }
       if (moved)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) facc[n] *= gr.fo[n], l[n] *= gr.fl[n];
+        for (int n = 0; n < NH; ++n) {
+          facc[n] *= gr.fo[h0 + n];
+          (n & 1 ? l2[n / 2].y : l2[n / 2].x) *= gr.fl[h0 + n];
+        }
     };
     int since = 0, edges = 0;
     for (int i = 0; i < nb; ++i) {
@@ -458,22 +506,30 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
       bool ok = mbar_wait(&bars.s_full[sub], i & 1, err, ERR_TREE_WAIT);
       __syncwarp();
       fence_after();
-      float s[NT];
+      float2 s2[NH / 2];
       // a row whose scale of K or V is not finite gives NaN to who sees it
       const float dkk = finite(dk) && finite(dv) ? dk : nan, dvv = finite(dv) ? dv : 0.f;
 #pragma unroll
-      for (int c0 = 0; c0 < NT; c0 += 16) {
-        uint32_t r[F::DQ][16];
+      for (int c0 = 0; c0 < NH; c0 += 8) {
+        uint32_t r[F::DQ][8];
 #pragma unroll
-        for (int k = 0; k < F::DQ; ++k) ld16(s_tm + k * NT + c0, r[k]);
+        for (int k = 0; k < F::DQ; ++k) ld8(s_tm + k * NT + c0, r[k]);
         ld_wait(r);
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
+        for (int n = 0; n < 4; ++n) {
+          const float2 hi = bits2(r[0][2 * n], r[0][2 * n + 1]), lo = bits2(r[1][2 * n], r[1][2 * n + 1]);
           if (I8)
-            s[c0 + n] = join_digits(r[0][n], r[1][n], r[F::DQ - 1][n]) * dkk;
+            s2[c0 / 2 + n] = __fmul2_rn(join_digits(hi, lo, bits2(r[F::DQ - 1][2 * n], r[F::DQ - 1][2 * n + 1])), f2(dkk));
           else
-            s[c0 + n] = __uint_as_float(r[0][n]) + __uint_as_float(r[1][n]);
+            s2[c0 / 2 + n] = __fadd2_rn(hi, lo);
         }
+      }
+      if (I8) {
+#pragma unroll
+        for (int k = 0; k < F::DQ; ++k)
+#pragma unroll
+          for (int n = 0; n < NH; n += 16) st16(s_tm + k * NT + n, S_START);
+        st_wait();
       }
       fence_before();
       mbar_arrive(&bars.s_free[sub]);
@@ -483,10 +539,10 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
         if (!I8) {
           // V rows that are past the end or not finite leave the tile; who
           // sees such a row gets NaN through its score, nobody else meets it.
-          // The first group does it and the second waits: two such tiles on, the
-          // first is held until the second group's products on this one are done
-          // (the tile's slot).
-          if (sub == 0) {
+          // The first half of the first group does it and the others wait: two
+          // such tiles on, it is held until everybody's products on this one are
+          // done (the tile's slot).
+          if (sub == 0 && half == 0) {
             const int t = vseq(i), slot = t % F::SLOTS;
             ok = mbar_wait(&bars.tfull[slot], (t / F::SLOTS) & 1, err, ERR_TREE_WAIT) && ok;
             uint8_t* vrow = smem + slot * F::TILE + kl * 128;
@@ -512,58 +568,62 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
           ++edges;
         }
         // lane n: which of the warp's 32 positions row n sees; then its transpose
-        const uint32_t rowsee = lane < NT ? seen_bits(a, rowt[sub * NT + lane], p0 + wq * 32, pos, len) : 0u;
+        const uint32_t rowsee = lane < NH ? seen_bits(a, rowt[sub * NT + h0 + lane], p0 + wq * 32, pos, len) : 0u;
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
           const uint32_t b = __ballot_sync(0xffffffffu, (rowsee >> k) & 1u);
           if (lane == k) vis = b;
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (!((vis >> n) & 1u)) s[n] = -INFINITY;
-          else if (!I8 && bad) s[n] = nan;
+        for (int n = 0; n < NH; ++n) {
+          float& s = n & 1 ? s2[n / 2].y : s2[n / 2].x;
+          if (!((vis >> n) & 1u)) s = -INFINITY;
+          else if (!I8 && bad) s = nan;
         }
       }
       // does a weight leave its range?  int8: digits hold weight * scale * vs
       // below 2^32 (lv_top is the bound of every row's vs)
-      constexpr float TOP = I8 ? 31.f : 11.f;
+      constexpr float TOP = I8 ? 31.f : 15.f;
       const float ldv = I8 ? __log2f(dvv) : 0.f;
       float top = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; n += 4) {
-        const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[n]), m4 = *reinterpret_cast<const float4*>(&gr.m[n]);
-        top = fmaxf(top, fmaxf(fmaf(s[n], c4.x, -m4.x), fmaf(s[n + 1], c4.y, -m4.y)));
-        top = fmaxf(top, fmaxf(fmaf(s[n + 2], c4.z, -m4.z), fmaf(s[n + 3], c4.w, -m4.w)));
+      for (int n = 0; n < NH; n += 4) {
+        const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[h0 + n]), m4 = *reinterpret_cast<const float4*>(&gr.nm[h0 + n]);
+        const float2 x = __ffma2_rn(s2[n / 2], make_float2(c4.x, c4.y), make_float2(m4.x, m4.y));
+        const float2 y = __ffma2_rn(s2[n / 2 + 1], make_float2(c4.z, c4.w), make_float2(m4.z, m4.w));
+        top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(y.x, y.y)));
       }
-      if (I8) top += fmaxf(-29.f, ldv + gr.lv_top);
+      if (I8) top += fmaxf(-29.f, ldv + gr.lv_top[half]);
       if (!ok) dead = 1;
       bool fresh = i == 0;
       __syncwarp();
-      if (group_any(bar, 128, top > TOP || !ok)) {
-        if (group_any(bar, 128, *reinterpret_cast<volatile int*>(&dead) != 0)) break;
+      if (group_any(bar, GT, top > TOP || !ok)) {
+        if (group_any(bar, GT, *reinterpret_cast<volatile int*>(&dead) != 0)) break;
         uint32_t mx = 0, dm = 0, need = 0;
         const uint32_t dvb = I8 ? __float_as_uint(dvv) : 0u;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {  // lane n keeps row n
-          const float sn = s[n] * gr.c[n], x = fmaf(s[n], gr.c[n], -gr.m[n]);
-          const bool over = (I8 ? x + fmaxf(-29.f, ldv + gr.lv[n]) : x) > TOP;
+        for (int n = 0; n < NH; ++n) {  // lane n keeps row n
+          const float s = n & 1 ? s2[n / 2].y : s2[n / 2].x, sn = s * gr.c[h0 + n], x = fmaf(s, gr.c[h0 + n], gr.nm[h0 + n]);
+          const bool over = (I8 ? x + fmaxf(-29.f, ldv + gr.lv[h0 + n]) : x) > TOP;
           const uint32_t hi = __reduce_max_sync(0xffffffffu, sn == sn ? ordered(sn) : 0u);
           const uint32_t dmn = I8 ? __reduce_max_sync(0xffffffffu, (vis >> n) & 1u ? dvb : 0u) : 0u;
           if (__any_sync(0xffffffffu, over)) need |= 1u << n;
           if (lane == n) mx = hi, dm = dmn;
         }
-        gr.mx[wq][lane] = mx;
-        gr.dm[wq][lane] = dm;
-        if (lane == 0) gr.need[wq] = need;
-        group_sync(bar, 128);
+        if (lane < NH) gr.mx[wq][h0 + lane] = mx, gr.dm[wq][h0 + lane] = dm;
+        if (lane == 0) gr.need[half][wq] = need;
+        group_sync(bar, GT);
         if (wq == 0) {
-          if (lane < NT) {
-            const int n = lane;
+          if (lane < NH) {
+            const int n = h0 + lane;
             float fo = 1.f, fl = 1.f;
-            if (((gr.need[0] | gr.need[1] | gr.need[2] | gr.need[3]) >> n) & 1u) {  // each row by itself
-              const float mn = fmaxf(gr.m[n], unordered(max(max(gr.mx[0][n], gr.mx[1][n]), max(gr.mx[2][n], gr.mx[3][n]))));
-              fo = fl = ex2(gr.m[n] - mn);
-              gr.m[n] = mn;
+            const uint32_t* nd = gr.need[half];
+            if (((nd[0] | nd[1] | nd[2] | nd[3]) >> lane) & 1u) {  // each row by itself
+              // fp16: the largest weight becomes 2^4, so that the low halves reach 2^-28 of it
+              const float top4 = unordered(max(max(gr.mx[0][n], gr.mx[1][n]), max(gr.mx[2][n], gr.mx[3][n]))) - (I8 ? 0.f : 4.f);
+              const float mn = fmaxf(-gr.nm[n], top4);
+              fo = fl = ex2(-gr.nm[n] - mn);
+              gr.nm[n] = -mn;
               if (I8) {
                 const uint32_t d = max(max(gr.dm[0][n], gr.dm[1][n]), max(gr.dm[2][n], gr.dm[3][n]));
                 const int ex = max((int)(d >> 23) - 126, -96);  // a power of two above the largest scale
@@ -579,16 +639,16 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
           }
           __syncwarp();
           if (I8) {
-            float hi = gr.lv[lane % NT], lo = hi;
+            float hi = gr.lv[h0 + lane % NH], lo = hi;
 #pragma unroll
             for (int x = 16; x; x >>= 1) {
               hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, x));
               lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, x));
             }
-            if (lane == 0) gr.lv_top = hi, gr.lv_same = hi == lo;
+            if (lane == 0) gr.lv_top[half] = hi, gr.lv_same[half] = hi == lo;
           }
         }
-        group_sync(bar, 128);
+        group_sync(bar, GT);
         flush(i, true);
         fresh = true;
       } else if (since >= F::PERIOD) {
@@ -599,73 +659,72 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
       // weights, as digits, into the operand tile
       if (i && !mbar_wait(&bars.pv_done[sub], (i - 1) & 1, err, ERR_TREE_WAIT)) dead = 1;
       if (I8) {
-        const float dvs = dvv * gr.vs[0];
-        const bool same = gr.lv_same;
+        const float dvs = dvv * gr.vs[h0];
+        const bool same = gr.lv_same[half];
 #pragma unroll
-        for (int c0 = 0; c0 < NT; c0 += 16) {
-          uint32_t w[4][4];
+        for (int r0 = 0; r0 < NH; r0 += 16) {  // a 16-byte piece of every digit
+        uint32_t w[4][4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int n0 = c0 + 4 * q;
-            const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[n0]), m4 = *reinterpret_cast<const float4*>(&gr.m[n0]);
-            const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, mm[4] = {m4.x, m4.y, m4.z, m4.w};
-            float f[4] = {dvs, dvs, dvs, dvs};
-            if (!same) {
-              const float4 v4 = *reinterpret_cast<const float4*>(&gr.vs[n0]);
-              f[0] = dvv * v4.x, f[1] = dvv * v4.y, f[2] = dvv * v4.z, f[3] = dvv * v4.w;
-            }
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float p = ex2(fmaf(s[n0 + e], cc[e], -mm[e]));
-              l[n0 + e] += p;
-              const float x = fmaf(p, f[e], 0.5f);  // 0.5 .. 2^32: its integer part is the weight
-              const float h = __fmaf_rz(x, 0x1p-16f, 8388608.f);
-              hi[e] = __float_as_uint(h);
-              lo[e] = __float_as_uint(__fadd_rz(fmaf(-65536.f, h - 8388608.f, x), 8388608.f));
-            }
-            const uint32_t l01 = __byte_perm(lo[0], lo[1], 0x5140u), l23 = __byte_perm(lo[2], lo[3], 0x5140u);
-            const uint32_t h01 = __byte_perm(hi[0], hi[1], 0x5140u), h23 = __byte_perm(hi[2], hi[3], 0x5140u);
-            w[0][q] = __byte_perm(l01, l23, 0x5410u);
-            w[1][q] = __byte_perm(l01, l23, 0x7632u);
-            w[2][q] = __byte_perm(h01, h23, 0x5410u);
-            w[3][q] = __byte_perm(h01, h23, 0x7632u);
+        for (int q = 0; q < 4; ++q) {
+          const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[h0 + r0 + 4 * q]), m4 = *reinterpret_cast<const float4*>(&gr.nm[h0 + r0 + 4 * q]);
+          float2 f[2] = {f2(dvs), f2(dvs)};
+          if (!same) {
+            const float4 v4 = *reinterpret_cast<const float4*>(&gr.vs[h0 + r0 + 4 * q]);
+            f[0] = make_float2(dvv * v4.x, dvv * v4.y), f[1] = make_float2(dvv * v4.z, dvv * v4.w);
           }
+          float2 hi[2], lo[2];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(prow + (((k * (NT / 16) + c0 / 16) ^ (kl & 7)) << 4)) =
-                make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+          for (int e = 0; e < 2; ++e) {
+            const float2 x = e ? __ffma2_rn(s2[r0 / 2 + 2 * q + 1], make_float2(c4.z, c4.w), make_float2(m4.z, m4.w))
+                               : __ffma2_rn(s2[r0 / 2 + 2 * q], make_float2(c4.x, c4.y), make_float2(m4.x, m4.y));
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            l2[r0 / 2 + 2 * q + e] = __fadd2_rn(l2[r0 / 2 + 2 * q + e], p);
+            const float2 y = __ffma2_rn(p, f[e], f2(0.5f));  // 0.5 .. 2^32: its integer part is the weight
+            hi[e] = __ffma2_rz(y, f2(0x1p-16f), f2(8388608.f));
+            lo[e] = __fadd2_rz(__ffma2_rn(__fadd2_rn(hi[e], f2(-8388608.f)), f2(-65536.f), y), f2(8388608.f));
+          }
+          auto u = [](float x) { return __float_as_uint(x); };
+          const uint32_t l01 = __byte_perm(u(lo[0].x), u(lo[0].y), 0x5140u), l23 = __byte_perm(u(lo[1].x), u(lo[1].y), 0x5140u);
+          const uint32_t h01 = __byte_perm(u(hi[0].x), u(hi[0].y), 0x5140u), h23 = __byte_perm(u(hi[1].x), u(hi[1].y), 0x5140u);
+          w[0][q] = __byte_perm(l01, l23, 0x5410u);
+          w[1][q] = __byte_perm(l01, l23, 0x7632u);
+          w[2][q] = __byte_perm(h01, h23, 0x5410u);
+          w[3][q] = __byte_perm(h01, h23, 0x7632u);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint4*>(prow + (((2 * k + (h0 + r0) / 16) ^ psw) << 4)) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
         }
       } else {
 #pragma unroll
-        for (int c0 = 0; c0 < NT; c0 += 8) {
+        for (int c0 = 0; c0 < NH / 8; ++c0) {  // eight rows: one 16-byte piece of high halves, one of low
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int n0 = c0 + 4 * h;
-            const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[n0]), m4 = *reinterpret_cast<const float4*>(&gr.m[n0]);
-            const float p0 = ex2(fmaf(s[n0], c4.x, -m4.x)), p1 = ex2(fmaf(s[n0 + 1], c4.y, -m4.y));
-            const float p2 = ex2(fmaf(s[n0 + 2], c4.z, -m4.z)), p3 = ex2(fmaf(s[n0 + 3], c4.w, -m4.w));
-            l[n0] += p0, l[n0 + 1] += p1, l[n0 + 2] += p2, l[n0 + 3] += p3;
-            const float x[4] = {p0 * 16.f, p1 * 16.f, p2 * 16.f, p3 * 16.f};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const __half2 t = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-              const float2 back = __half22float2(t);
-              hi[2 * h + e] = h2u(t);
-              lo[2 * h + e] = h2u(__floats2half2_rn(x[2 * e] - back.x, x[2 * e + 1] - back.y));
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int n = 4 * c0 + e;
+            const float2 x = __ffma2_rn(s2[n], *reinterpret_cast<const float2*>(&gr.c[h0 + 2 * n]), *reinterpret_cast<const float2*>(&gr.nm[h0 + 2 * n]));
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            l2[n] = __fadd2_rn(l2[n], p);
+            const __half2 t = __floats2half2_rn(p.x, p.y);
+            const float2 d = __ffma2_rn(__half22float2(t), f2(-1.f), p);
+            hi[e] = h2u(t);
+            lo[e] = h2u(__floats2half2_rn(d.x, d.y));
           }
-          *reinterpret_cast<uint4*>(prow + (((c0 / 8) ^ (kl & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(prow + (((NT / 8 + c0 / 8) ^ (kl & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(prow + (((h0 / 8 + c0) ^ psw) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(prow + (((4 + h0 / 8 + c0) ^ psw) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
-      if (kl == 0) *reinterpret_cast<volatile int*>(&restart[sub]) = fresh;
+      if (kl == 0 && half == 0) *reinterpret_cast<volatile int*>(&restart[sub]) = fresh;
       fence_proxy_async_smem();
       fence_before();
       mbar_arrive(&bars.p_full[sub]);
     }
     if (nb) flush(nb, false);
+    __syncwarp();
+    if (SUBS == 2) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_LAUNCH));
+      group_sync(4, F::THREADS);
+    }
   }
   __syncwarp();
   fence_before();
@@ -673,17 +732,21 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
   fence_after();
   float* fold = reinterpret_cast<float*>(smem);  // [row][HD]: the ring is idle
   if (warp >= 4) {
-    const int sub = (warp >> 2) - 1, wq = warp & 3;
-    Group<NT>& gr = groups[sub];
+    const int sub = HALVES == 2 ? 0 : (warp >> 2) - 1, h0 = HALVES == 2 ? ((warp >> 2) - 1) * NH : 0, wq = warp & 3;
+    Group& gr = groups[sub];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) fold[(sub * NT + n) * HD + wq * 32 + lane] = facc[n] * (1.f / gr.vs[n]);  // a power of two
-    // sums over the group's 128 positions: after the exchanges lane n (and n +
-    // 16, of 16 rows) of a warp holds row n's
-    if (NT == 16)
+    for (int n = 0; n < NH; ++n)  // 1 / vs is a power of two
+      fold[(sub * NT + h0 + n) * HD + wq * 32 + lane] = facc[n] * (1.f / gr.vs[h0 + n]);
+    // sums over the group's 128 positions: after the exchanges lane n (of 16
+    // rows, and n + 16) of a warp holds row n's
+    float l[NH];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+    for (int n = 0; n < NH; ++n) {
+      l[n] = n & 1 ? l2[n / 2].y : l2[n / 2].x;
+      if (NH == 16) l[n] += __shfl_xor_sync(0xffffffffu, l[n], 16);
+    }
 #pragma unroll
-    for (int w = NT / 2; w; w >>= 1) {
+    for (int w = NH / 2; w; w >>= 1) {
       const bool up = lane & w;
 #pragma unroll
       for (int n = 0; n < w; ++n) {
@@ -691,13 +754,13 @@ __global__ void __launch_bounds__(Cfg<I8, NT>::THREADS, 1)
         l[n] = keep + __shfl_xor_sync(0xffffffffu, send, w);
       }
     }
-    gr.mx[wq][lane] = __float_as_uint(l[0]);
-    group_sync(1 + sub, 128);
-    if (wq == 0 && lane < NT) {
+    if (lane < NH) gr.mx[wq][h0 + lane] = __float_as_uint(l[0]);
+    group_sync(1 + sub, GT);
+    if (wq == 0 && lane < NH) {
       float L = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) L += __uint_as_float(gr.mx[k][lane]);
-      cta_ml[sub * NT + lane] = make_float2(gr.m[lane], L);
+      for (int k = 0; k < 4; ++k) L += __uint_as_float(gr.mx[k][h0 + lane]);
+      cta_ml[sub * NT + h0 + lane] = make_float2(-gr.nm[h0 + lane], L);
     }
   }
   if (warp == 1)
@@ -721,10 +784,10 @@ static EncodeFn encode_fn() {
   return fn;
 }
 
-template <bool I8, int NT>
+template <bool I8, int SUBS>
 static cudaError_t launch(TreeArgs a, int tiles, int units, int64_t most, int* err, cudaStream_t s) {
-  using F = Cfg<I8, NT>;
-  auto kern = tree_tc_kernel<I8, NT>;
+  using F = Cfg<I8, SUBS>;
+  auto kern = tree_tc_kernel<I8, SUBS>;
   const EncodeFn enc = encode_fn();
   if (!enc) return cudaErrorNotSupported;
   // rows of all heads as one 2-D tensor; a box is one block (fp16: half of its
@@ -751,8 +814,8 @@ static cudaError_t launch(TreeArgs a, int tiles, int units, int64_t most, int* e
 cudaError_t launch_tree_tc(const TreeArgs& a, int rows_per_cta, int tiles, int units, int64_t most, int* err, cudaStream_t s) {
   const bool one = rows_per_cta == 32;
   if (a.c.dtype == ODI_CUDA_KV_I8)
-    return one ? ttc::launch<true, 16>(a, tiles, units, most, err, s) : ttc::launch<true, 32>(a, tiles, units, most, err, s);
-  return one ? ttc::launch<false, 16>(a, tiles, units, most, err, s) : ttc::launch<false, 32>(a, tiles, units, most, err, s);
+    return one ? ttc::launch<true, 1>(a, tiles, units, most, err, s) : ttc::launch<true, 2>(a, tiles, units, most, err, s);
+  return one ? ttc::launch<false, 1>(a, tiles, units, most, err, s) : ttc::launch<false, 2>(a, tiles, units, most, err, s);
 }
 
 }  // namespace odi_cuda

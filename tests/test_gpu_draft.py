@@ -491,6 +491,24 @@ def test_attention_query_sizes(dr, dt, qstd):
     assert (np.abs(out - ref) <= 2 * w * np.abs(V).max()).all()
 
 
+@pytest.mark.parametrize("dt", ["f16", "i8"])
+@pytest.mark.parametrize("hd,T", [(64, 9), (128, 1), (128, 9)])
+@pytest.mark.parametrize("scale", [0.0, -0.09, 1e-30])
+def test_attention_any_scale(dr, dt, hd, T, scale):
+    """Zero (the mean of what is seen), negative and tiny scales, with nodes masked."""
+    rng = np.random.default_rng(13)
+    H, KV, pos, ctx = 8, 2, 200, 256
+    c = dr.KVCache.new(dt, KV, hd, ctx)
+    fill(c, rng, 0, pos + T, garbage=np.nan)
+    q = (1.5 * rng.standard_normal((T, H, hd))).astype(np.float32)
+    vis = random_tree(rng, T)
+    out = dr.attention_tree(dev(q.reshape(T, -1)), c, None, state(pos), heads=H, scale=scale, mask=dev(words(vis)),
+                            scratch=dr.attention_tree_scratch(c, T, H)).cpu().numpy().reshape(T, H, hd)
+    K, V = (np.nan_to_num(x) for x in values64(c))
+    ref, S = attend64(q.astype(np.float64), K, V, vis, pos, float(np.float32(scale)))
+    assert (np.abs(out - ref) <= 2 * (hd * U * S + 8 * U)[..., None] * np.abs(V).max()).all()
+
+
 def test_attention_two_caches_one_scratch_and_graph(dr):
     """One scratch serves the layers of a step; a captured step replays with
     another position."""
