@@ -184,11 +184,11 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
       const int r = tile * NR * 8 + warp + i * TA_WARPS;
-      rt[i] = r < a.R ? r / a.G : -1;
+      rt[i] = r < a.R ? row_node(a, r) : -1;
 #pragma unroll
       for (int e = 0; e < PL; ++e) v[i][e] = 0.f;
       if (r < a.R) {
-        const float* src = a.q + (int64_t)rt[i] * a.ld_q + (int64_t)(kvh * a.G + r % a.G) * HD + lane * PL;
+        const float* src = a.q + (int64_t)rt[i] * a.ld_q + (int64_t)(kvh * a.G + r - rt[i] * a.G) * HD + lane * PL;
 #pragma unroll
         for (int e = 0; e < PL; ++e) v[i][e] = __ldcg(src + e);
       }
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
     for (int w = 0; w < TA_WARPS; ++w) add(A, fold4[w * NR * 8 * V4 + i], ml[w][i / V4].x);
     fold4[i] = A;
   }
-  tree_join<HD, NR * 8, TA_THREADS>(a, rowt, cta_ml, fold, rows, C, rank, nclusters);
+  tree_join<HD, NR * 8, TA_THREADS>(a, threadIdx.x, rowt, cta_ml, fold, rows, C, rank, nclusters);
 }
 
 // Which kernel and how many rows per CTA; room: CTAs resident at once.
@@ -569,6 +569,7 @@ int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_ca
   a.q = d_q, a.ld_q = ld_q, a.out = d_out, a.c = v, a.mask = d_mask, a.mask_words = (tokens + 31) / 32;
   a.st = reinterpret_cast<const DecodeState*>(d_state);
   a.tokens = tokens, a.heads = heads, a.G = heads / v.kv_heads, a.R = tokens * a.G;
+  a.inv_G = (unsigned)((0x100000000ull + a.G - 1) / a.G);
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + 16);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + p.part_off);

@@ -21,6 +21,7 @@ struct TreeArgs {
   int mask_words;
   const DecodeState* st;
   int tokens, heads, G, R, nsplit;
+  unsigned inv_G;    // ceil(2^32 / G): r / G = r * inv_G >> 32 for the rows there are (G > 1)
   float scale_log2;  // scale * log2(e)
   int* count;   // arrivals per (kv head, row tile, cluster rank), zero between launches
   float* part;  // [kv head][tile][cluster][row][hd + 4]: reference, sum, -, -, accumulator
@@ -65,6 +66,10 @@ __device__ __forceinline__ float2 peer_f2(const float2* p, int k) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
+// The node of row r.
+__device__ __forceinline__ int row_node(const TreeArgs& a, int r) {
+  return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.inv_G);
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
@@ -88,9 +93,19 @@ __device__ __forceinline__ unsigned seen_bits(const TreeArgs& a, int t, int p0, 
 // memory, not yet synchronised).  Rank k of the cluster takes rows k, k + C,
 // ... from every rank's shared memory, in rank order; with several clusters
 // the last to arrive joins their shares in cluster order.  Every order is
-// fixed, so repeats are bit-identical.
+// fixed, so repeats are bit-identical.  The CTA's other threads meanwhile call
+// tree_join_rest, which has the same barriers.
+__device__ __forceinline__ void tree_join_rest(int C, int nclusters) {
+  if (C > 1) cluster_barrier();
+  else __syncthreads();
+  __syncthreads();
+  if (C > 1) cluster_barrier();
+  if (nclusters == 1) return;
+  __syncthreads();
+  __syncthreads();
+}
 template <int HD, int ROWS, int THREADS>
-__device__ __forceinline__ void tree_join(const TreeArgs& a, const int* rowt, float2* cta_ml, float* fold, int rows,
+__device__ __forceinline__ void tree_join(const TreeArgs& a, int tid, const int* rowt, float2* cta_ml, float* fold, int rows,
                                           int C, int rank, int nclusters) {
   __shared__ float fac[ROWS][8];  // the cluster's ranks' factors of this rank's rows
   __shared__ float2 own_ml[ROWS];
@@ -116,8 +131,8 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const int* rowt, fl
   const int mine = rows > rank ? (rows - rank + C - 1) / C : 0;
   constexpr int64_t PS = ROWS * (HD + 4);               // a cluster's share: [row][HD + 4]
   float* part = a.part + unit * (a.nsplit / C) * PS;
-  if (threadIdx.x < mine) {
-    const int n = rank + threadIdx.x * C;
+  if (tid < mine) {
+    const int n = rank + tid * C;
     float2 x[8];
     float M = TA_NONE, L = 0.f;
 #pragma unroll
@@ -128,13 +143,13 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const int* rowt, fl
       if (k < C) {
         const float f = ex2(x[k].x - M);
         L += x[k].y * f;
-        fac[threadIdx.x][k] = f;
+        fac[tid][k] = f;
       }
-    own_ml[threadIdx.x] = make_float2(M, L);
+    own_ml[tid] = make_float2(M, L);
     if (nclusters > 1) *reinterpret_cast<float2*>(part + (split / C) * PS + n * (HD + 4)) = make_float2(M, L);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < mine * V4; i += THREADS) {
+  for (int i = tid; i < mine * V4; i += THREADS) {
     const int s = i / V4, d4 = i % V4, n = rank + s * C;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f), y[8];
 #pragma unroll
@@ -151,11 +166,11 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const int* rowt, fl
   __threadfence();
   __syncthreads();
   int* count = a.count + unit * 8 + rank;
-  if (threadIdx.x == 0) is_last = atomicAdd(count, 1) == nclusters - 1;
+  if (tid == 0) is_last = atomicAdd(count, 1) == nclusters - 1;
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  for (int i = threadIdx.x; i < mine * V4; i += THREADS) {  // the last of the clusters, for this rank's rows
+  for (int i = tid; i < mine * V4; i += THREADS) {  // the last of the clusters, for this rank's rows
     const int d4 = i % V4, n = rank + i / V4 * C;
     const float* p = part + n * (HD + 4);
     float M = TA_NONE, L = 0.f;
@@ -185,7 +200,7 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, const int* rowt, fl
     }
     store(n, d4, A, L);
   }
-  if (threadIdx.x == 0) *count = 0;
+  if (tid == 0) *count = 0;
 }
 
 // The tcgen05 kernel (tree_attention_tc.cu): 32 or 64 rows per CTA.

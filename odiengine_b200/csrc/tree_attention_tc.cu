@@ -79,7 +79,6 @@ struct Cfg {
   // blocks between two moves of O to registers: 255 * 127 * 128 * 256 < 2^31;
   // the fp32 accumulator truncates, about 2^-26 of the sum per instruction
   static constexpr int PERIOD = I8 ? 256 : 4;
-  static_assert(ROWS * HD * 4 <= SLOTS * TILE, "the joins' shares reuse the ring");
   static_assert(SMEM <= 222 * 1024, "shared memory, beside the static part");
 };
 
@@ -252,6 +251,20 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
   const int seqs = 2 * nb;                     // tiles K0 K1 V0 K2 V1 ...
   auto vseq = [&](int i) { return min(2 * i + 2, 2 * nb - 1); };
   auto kseq = [&](int i) { return i ? 2 * i - 1 : 0; };
+  auto request_tile = [&](int t) {  // one thread of warp 0
+    const int slot = t % F::SLOTS;
+    const bool isk = t == 0 || (t == seqs - 1 ? false : (t & 1));
+    const int i = t == 0 ? 0 : isk ? (t + 1) / 2 : t == seqs - 1 ? nb - 1 : t / 2 - 1;
+    const int row = (int)(head + (int64_t)(split + i * stride) * BK);
+    uint8_t* dst = smem + slot * F::TILE;
+    mbar_arrive_expect_tx(&bars.tfull[slot], F::TILE);
+    const CUtensorMap* map = isk ? &kmap : &vmap;
+    tma_2d(dst, map, 0, row, &bars.tfull[slot]);
+    if (!I8) tma_2d(dst + F::TILE / 2, map, 64, row, &bars.tfull[slot]);
+  };
+  // the first tiles are on their way while the other warps lay out Q
+  if (tid == 0)
+    for (int t = 0; t < seqs && t < F::SLOTS; ++t) request_tile(t);
 
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
@@ -260,27 +273,32 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // ---- Q: digits as K-major operand rows n' = digit * 32 + n
-  {
-    constexpr int NW = F::THREADS / 32, RW = (F::ROWS + NW - 1) / NW;
+  if (warp >= 4) {
+    constexpr int NW = F::THREADS / 32 - 4, RW = F::ROWS / NW;
+    const bool vec = !(((uintptr_t)a.q & 15) | (a.ld_q & 3));
     float v[RW][4];
     int rt[RW];
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
-      const int n = warp + i * NW, r = tile * F::ROWS + n;
-      const bool in = n < F::ROWS && r < a.R;
-      rt[i] = in ? r / a.G : -1;
+      const int n = warp - 4 + i * NW, r = tile * F::ROWS + n;
+      const bool in = r < a.R;
+      rt[i] = in ? row_node(a, r) : -1;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[i][e] = 0.f;
       if (in) {
         const float* src = a.q + (int64_t)rt[i] * a.ld_q + (int64_t)(kvh * a.G + r - rt[i] * a.G) * HD + lane * 4;
+        if (vec) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+          v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[i][e] = __ldcg(src + e);
+          for (int e = 0; e < 4; ++e) v[i][e] = __ldcg(src + e);
+        }
       }
     }
 #pragma unroll
     for (int i = 0; i < RW; ++i) {
-      const int n = warp + i * NW;
-      if (n >= F::ROWS) break;
+      const int n = warp - 4 + i * NW;
       float am = 0.f;
       bool ok = true;
 #pragma unroll
@@ -346,28 +364,18 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
   fence_after();
   const uint32_t tmem = tmem_slot;
 
-  float facc[NH];
-  float2 l2[NH / 2];
   if (warp < 4) {
     if (SUBS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_FIRST));
   if (warp == 0) {
     // ---------------- producer ----------------
     if (lane == 0) {
-      int t = 0;
+      int t = min(seqs, F::SLOTS);
       for (; t < seqs; ++t) {
-        const int slot = t % F::SLOTS;
-        if (!mbar_wait(&bars.tfree[slot], ((t / F::SLOTS) & 1) ^ 1, err, ERR_TREE_WAIT)) {
+        if (!mbar_wait(&bars.tfree[t % F::SLOTS], ((t / F::SLOTS) & 1) ^ 1, err, ERR_TREE_WAIT)) {
           dead = 1;
           break;
         }
-        const bool isk = t == 0 || (t == seqs - 1 ? false : (t & 1));
-        const int i = t == 0 ? 0 : isk ? (t + 1) / 2 : t == seqs - 1 ? nb - 1 : t / 2 - 1;
-        const int row = (int)(head + (int64_t)(split + i * stride) * BK);
-        uint8_t* dst = smem + slot * F::TILE;
-        mbar_arrive_expect_tx(&bars.tfull[slot], F::TILE);
-        const CUtensorMap* map = isk ? &kmap : &vmap;
-        tma_2d(dst, map, 0, row, &bars.tfull[slot]);
-        if (!I8) tma_2d(dst + F::TILE / 2, map, 64, row, &bars.tfull[slot]);
+        request_tile(t);
       }
       // every issued copy has landed before the CTA can retire
       for (int u = t < F::SLOTS ? 0 : t - F::SLOTS; u < t; ++u)
@@ -426,13 +434,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     }
     if (!ok) dead = 1;
   }
-    // A warp of this group that is done must not take registers back before the
-    // softmax warps have had theirs: they would wait for good.
-    __syncwarp();
-    if (SUBS == 2) {
-      group_sync(4, F::THREADS);
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REGS_LAUNCH));
-    }
+    tree_join_rest(C, nclusters);
   } else {
     // ---------------- softmax ----------------
     if (SUBS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REGS_SOFT));
@@ -445,6 +447,8 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     const float* ks = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.k) + a.c.scale_off) + head;
     const float* vsc = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.c.v) + a.c.scale_off) + head;
     const float nan = __int_as_float(0x7fc00000);
+    float facc[NH];
+    float2 l2[NH / 2];
 #pragma unroll
     for (int n = 0; n < NH; ++n) facc[n] = 0.f;
 #pragma unroll
@@ -503,39 +507,10 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         dk = dk_next, dv = dv_next;
         if (i + 1 < nb) request(i + 1);
       }
-      bool ok = mbar_wait(&bars.s_full[sub], i & 1, err, ERR_TREE_WAIT);
-      __syncwarp();
-      fence_after();
-      float2 s2[NH / 2];
-      // a row whose scale of K or V is not finite gives NaN to who sees it
-      const float dkk = finite(dk) && finite(dv) ? dk : nan, dvv = finite(dv) ? dv : 0.f;
-#pragma unroll
-      for (int c0 = 0; c0 < NH; c0 += 8) {
-        uint32_t r[F::DQ][8];
-#pragma unroll
-        for (int k = 0; k < F::DQ; ++k) ld8(s_tm + k * NT + c0, r[k]);
-        ld_wait(r);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const float2 hi = bits2(r[0][2 * n], r[0][2 * n + 1]), lo = bits2(r[1][2 * n], r[1][2 * n + 1]);
-          if (I8)
-            s2[c0 / 2 + n] = __fmul2_rn(join_digits(hi, lo, bits2(r[F::DQ - 1][2 * n], r[F::DQ - 1][2 * n + 1])), f2(dkk));
-          else
-            s2[c0 / 2 + n] = __fadd2_rn(hi, lo);
-        }
-      }
-      if (I8) {
-#pragma unroll
-        for (int k = 0; k < F::DQ; ++k)
-#pragma unroll
-          for (int n = 0; n < NH; n += 16) st16(s_tm + k * NT + n, S_START);
-        st_wait();
-      }
-      fence_before();
-      mbar_arrive(&bars.s_free[sub]);
       uint32_t vis = 0xffffffffu;  // bit n: row n sees this position
-      if (p0 + BK > min(pos, len)) {  // holds tree slots, or ends past the last
-        bool bad = false;
+      bool ok = true, bad = false;
+      const bool edge = p0 + BK > min(pos, len);  // holds tree slots, or ends past the last
+      if (edge) {  // which of them are seen, while the scores are on their way
         if (!I8) {
           // V rows that are past the end or not finite leave the tile; who
           // sees such a row gets NaN through its score, nobody else meets it.
@@ -574,6 +549,38 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           const uint32_t b = __ballot_sync(0xffffffffu, (rowsee >> k) & 1u);
           if (lane == k) vis = b;
         }
+      }
+      ok = mbar_wait(&bars.s_full[sub], i & 1, err, ERR_TREE_WAIT) && ok;
+      __syncwarp();
+      fence_after();
+      float2 s2[NH / 2];
+      // a row whose scale of K or V is not finite gives NaN to who sees it
+      const float dkk = finite(dk) && finite(dv) ? dk : nan, dvv = finite(dv) ? dv : 0.f;
+#pragma unroll
+      for (int c0 = 0; c0 < NH; c0 += 8) {
+        uint32_t r[F::DQ][8];
+#pragma unroll
+        for (int k = 0; k < F::DQ; ++k) ld8(s_tm + k * NT + c0, r[k]);
+        ld_wait(r);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float2 hi = bits2(r[0][2 * n], r[0][2 * n + 1]), lo = bits2(r[1][2 * n], r[1][2 * n + 1]);
+          if (I8)
+            s2[c0 / 2 + n] = __fmul2_rn(join_digits(hi, lo, bits2(r[F::DQ - 1][2 * n], r[F::DQ - 1][2 * n + 1])), f2(dkk));
+          else
+            s2[c0 / 2 + n] = __fadd2_rn(hi, lo);
+        }
+      }
+      if (I8) {
+#pragma unroll
+        for (int k = 0; k < F::DQ; ++k)
+#pragma unroll
+          for (int n = 0; n < NH; n += 16) st16(s_tm + k * NT + n, S_START);
+        st_wait();
+      }
+      fence_before();
+      mbar_arrive(&bars.s_free[sub]);
+      if (edge) {
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
           float& s = n & 1 ? s2[n / 2].y : s2[n / 2].x;
@@ -720,23 +727,12 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       mbar_arrive(&bars.p_full[sub]);
     }
     if (nb) flush(nb, false);
-    __syncwarp();
-    if (SUBS == 2) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_LAUNCH));
-      group_sync(4, F::THREADS);
-    }
-  }
-  __syncwarp();
-  fence_before();
-  __syncthreads();
-  fence_after();
-  float* fold = reinterpret_cast<float*>(smem);  // [row][HD]: the ring is idle
-  if (warp >= 4) {
-    const int sub = HALVES == 2 ? 0 : (warp >> 2) - 1, h0 = HALVES == 2 ? ((warp >> 2) - 1) * NH : 0, wq = warp & 3;
-    Group& gr = groups[sub];
+    // O and the sums of this group's rows, in its own P tile
+    float* fold = reinterpret_cast<float*>(smem + F::P_OFF);  // [row][HD]
+    static_assert(F::PB == NT * HD * 4, "a group's rows fill its P tile");
 #pragma unroll
     for (int n = 0; n < NH; ++n)  // 1 / vs is a power of two
-      fold[(sub * NT + h0 + n) * HD + wq * 32 + lane] = facc[n] * (1.f / gr.vs[h0 + n]);
+      fold[(sub * NT + h0 + n) * HD + kl] = facc[n] * (1.f / gr.vs[h0 + n]);
     // sums over the group's 128 positions: after the exchanges lane n (of 16
     // rows, and n + 16) of a warp holds row n's
     float l[NH];
@@ -755,17 +751,21 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       }
     }
     if (lane < NH) gr.mx[wq][h0 + lane] = __float_as_uint(l[0]);
-    group_sync(1 + sub, GT);
+    group_sync(bar, GT);
     if (wq == 0 && lane < NH) {
       float L = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) L += __uint_as_float(gr.mx[k][h0 + lane]);
       cta_ml[sub * NT + h0 + lane] = make_float2(-gr.nm[h0 + lane], L);
     }
+    fence_before();
+    tree_join<HD, F::ROWS, SUBS * GT>(a, tid - 128, rowt, cta_ml, fold, min(F::ROWS, a.R - tile * F::ROWS), C, rank, nclusters);
   }
-  if (warp == 1)
+  // past the join's barriers nobody reads tensor memory
+  if (warp == 1) {
+    fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F::TMEM_COLS) : "memory");
-  tree_join<HD, F::ROWS, F::THREADS>(a, rowt, cta_ml, fold, min(F::ROWS, a.R - tile * F::ROWS), C, rank, nclusters);
+  }
 }
 
 // cuTensorMapEncodeTiled, from the driver that the runtime already loaded.
