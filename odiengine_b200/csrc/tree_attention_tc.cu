@@ -177,13 +177,27 @@ __device__ __forceinline__ void st16(uint32_t addr, uint32_t v) {
                : "memory");
 }
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// fp32 -> unsigned with the same order
-__device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float unordered(uint32_t u) {
-  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+// The lane's share of a column-wise maximum: value(n) of N columns on each of 32
+// lanes; lane n (N = 16: also n + 16) gets column n's largest.
+template <int N, typename V>
+__device__ __forceinline__ float lane_max(V&& value) {
+  const int lane = threadIdx.x & 31;
+  float x[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    x[n] = value(n);
+    if (N == 16) x[n] = fmaxf(x[n], __shfl_xor_sync(0xffffffffu, x[n], 16));
+  }
+#pragma unroll
+  for (int w = N / 2; w; w >>= 1) {
+    const bool up = lane & w;
+#pragma unroll
+    for (int n = 0; n < w; ++n) {
+      const float send = up ? x[n] : x[n + w], keep = up ? x[n + w] : x[n];
+      x[n] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, send, w));
+    }
+  }
+  return x[0];
 }
 
 template <int SUBS>
@@ -199,7 +213,7 @@ struct alignas(16) Group {
   float lv[NT];          // log2 of vs
   float vs[NT];          // int8: factor of weight * scale
   float fo[NT], fl[NT];  // factors of O and of the sums when the reference moves
-  uint32_t mx[4][NT], dm[4][NT], need[2][4];
+  float mx[4][NT], dm[4][NT];
   float lv_top[2];       // the largest lv of each half
   int lv_same[2];        // all lv of the half are equal
 };
@@ -272,49 +286,54 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // ---- Q: digits as K-major operand rows n' = digit * 32 + n
+  // ---- Q: digits as K-major operand rows n' = digit * 32 + n; eight lanes per
+  // row, 16 dims each
   if (warp >= 4) {
-    constexpr int NW = F::THREADS / 32 - 4, RW = F::ROWS / NW;
+    constexpr int PASS = F::ROWS / 32;  // 8 warps of 4 rows
     const bool vec = !(((uintptr_t)a.q & 15) | (a.ld_q & 3));
-    float v[RW][4];
-    int rt[RW];
+    const int l8 = lane & 7;
+    float v[PASS][16];
+    int rt[PASS];
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const int n = warp - 4 + i * NW, r = tile * F::ROWS + n;
-      const bool in = r < a.R;
-      rt[i] = in ? row_node(a, r) : -1;
+    for (int i = 0; i < PASS; ++i) {
+      const int r = tile * F::ROWS + i * 32 + (warp - 4) * 4 + (lane >> 3);
+      rt[i] = r < a.R ? row_node(a, r) : -1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[i][e] = 0.f;
-      if (in) {
-        const float* src = a.q + (int64_t)rt[i] * a.ld_q + (int64_t)(kvh * a.G + r - rt[i] * a.G) * HD + lane * 4;
+      for (int e = 0; e < 16; ++e) v[i][e] = 0.f;
+      if (r < a.R) {
+        const float* src = a.q + (int64_t)rt[i] * a.ld_q + (int64_t)(kvh * a.G + r - rt[i] * a.G) * HD + l8 * 16;
         if (vec) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
-          v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src) + e);
+            v[i][4 * e] = x.x, v[i][4 * e + 1] = x.y, v[i][4 * e + 2] = x.z, v[i][4 * e + 3] = x.w;
+          }
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[i][e] = __ldcg(src + e);
+          for (int e = 0; e < 16; ++e) v[i][e] = __ldcg(src + e);
         }
       }
     }
+    const float sign = a.scale_log2 < 0.f ? -1.f : a.scale_log2 > 0.f ? 1.f : 0.f;  // the scores' factor stays positive
 #pragma unroll
-    for (int i = 0; i < RW; ++i) {
-      const int n = warp - 4 + i * NW;
-      float am = 0.f;
-      bool ok = true;
+    for (int i = 0; i < PASS; ++i) {
+      const int n = i * 32 + (warp - 4) * 4 + (lane >> 3), sub = n / NT, ln = n % NT;
+      float am = 0.f, sum = 0.f;  // sum * 0 is 0 only if every value is finite
 #pragma unroll
-      for (int e = 0; e < 4; ++e) am = fmaxf(am, fabsf(v[i][e])), ok = ok && finite(v[i][e]);
+      for (int e = 0; e < 16; ++e) am = fmaxf(am, fabsf(v[i][e])), sum = fmaf(v[i][e], 0.f, sum);
 #pragma unroll
-      for (int x = 16; x; x >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, x));
-      ok = __all_sync(0xffffffffu, ok);
+      for (int x = 4; x; x >>= 1) {
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, x));
+        sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      }
+      const bool ok = sum == 0.f;
       int ex = (int)(__float_as_uint(am) >> 23) - 127;
       if (I8 && am * pow2(-min(max(ex, -100), 126)) > 1.99f) ++ex;
       ex = min(max(ex, -100), 126);
-      const float lift = pow2(-ex), up = I8 ? 4194304.f : 8192.f;
-      const int sub = n / NT, ln = n % NT;
-      const float sign = a.scale_log2 < 0.f ? -1.f : a.scale_log2 > 0.f ? 1.f : 0.f;  // c stays positive
-      if (lane == 0) {
+      const float lift = ok ? pow2(-ex) : 0.f, up = (I8 ? 4194304.f : 8192.f) * sign;
+      if (l8 == 0) {
         Group& gr = groups[sub];
-        gr.c[ln] = ok ? fmaxf(fabsf(a.scale_log2) * (1.f / up) * pow2(ex), 1e-37f) : __int_as_float(0x7fc00000);
+        gr.c[ln] = ok ? fmaxf(fabsf(a.scale_log2) * (I8 ? 1.f / 4194304.f : 1.f / 8192.f) * pow2(ex), 1e-37f) : __int_as_float(0x7fc00000);
         gr.nm[ln] = -TA_NONE;
         gr.lv[ln] = I8 ? 120.f : 0.f;
         gr.vs[ln] = I8 ? TA_VMOST : 1.f;
@@ -324,36 +343,42 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       }
       uint8_t* q = smem + F::Q_OFF + sub * F::QB;
       if (I8) {
-        int dig[4];
+        int dig[16];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dig[e] = ok ? __float2int_rn(v[i][e] * lift * up * sign) : 0;
+        for (int e = 0; e < 16; ++e) dig[e] = ok ? __float2int_rn(v[i][e] * lift * up) : 0;
 #pragma unroll
         for (int k = F::DQ - 1; k >= 0; --k) {  // digit 0 the highest
-          uint32_t bytes = 0;
+          uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int lo = (int)(int8_t)(dig[e] & 255);
-            dig[e] = (dig[e] - lo) >> 8;
-            bytes |= (uint32_t)(lo & 255) << (8 * e);
+          for (int j = 0; j < 4; ++j) {
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int lo = (int)(int8_t)(dig[4 * j + e] & 255);
+              dig[4 * j + e] = (dig[4 * j + e] - lo) >> 8;
+              bytes |= (uint32_t)(lo & 255) << (8 * e);
+            }
+            w[j] = bytes;
           }
           const int row = k * NT + ln;
-          *reinterpret_cast<uint32_t*>(q + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) = bytes;
+          *reinterpret_cast<uint4*>(q + row * 128 + ((l8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-      } else {
-        uint32_t w[2][2];
+      } else {  // two pieces of 64 dims, each [64 rows][128 bytes]
+        uint8_t* piece = q + (l8 >> 2) * (F::DQ * NT * 128);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x0 = ok ? v[i][2 * e] * lift * up * sign : 0.f, x1 = ok ? v[i][2 * e + 1] * lift * up * sign : 0.f;
-          const __half2 hi = __floats2half2_rn(x0, x1);
-          const float2 back = __half22float2(hi);
-          w[0][e] = h2u(hi);
-          w[1][e] = h2u(__floats2half2_rn(x0 - back.x, x1 - back.y));
-        }
+        for (int j = 0; j < 2; ++j) {
+          uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int k = 0; k < F::DQ; ++k) {  // two pieces of 64 dims, each [64 rows][128 bytes]
-          const int row = k * NT + ln, d = lane * 4;
-          *reinterpret_cast<uint2*>(q + (d >> 6) * (F::DQ * NT * 128) + row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 7) * 2) =
-              make_uint2(w[k][0], w[k][1]);
+          for (int e = 0; e < 4; ++e) {
+            const float x0 = ok ? v[i][8 * j + 2 * e] * lift * up : 0.f, x1 = ok ? v[i][8 * j + 2 * e + 1] * lift * up : 0.f;
+            const __half2 h = __floats2half2_rn(x0, x1);
+            const float2 back = __half22float2(h);
+            hi[e] = h2u(h);
+            lo[e] = h2u(__floats2half2_rn(x0 - back.x, x1 - back.y));
+          }
+          const int ch = (l8 & 3) * 2 + j;
+          *reinterpret_cast<uint4*>(piece + ln * 128 + ((ch ^ (ln & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(piece + (NT + ln) * 128 + ((ch ^ (ln & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
     }
@@ -500,6 +525,13 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           (n & 1 ? l2[n / 2].y : l2[n / 2].x) *= gr.fl[h0 + n];
         }
     };
+    // which of the warp's 32 positions lane n's row sees; of this CTA's first
+    // block that needs it, asked for now
+    auto row_sees = [&](int i) {
+      return lane < NH ? seen_bits(a, rowt[sub * NT + h0 + lane], (split + i * stride) * BK + wq * 32, pos, len) : 0u;
+    };
+    const int b0 = min(pos, len) / BK, first_edge = pos <= 0 || b0 <= split ? 0 : (b0 - split + stride - 1) / stride;
+    const uint32_t first_sees = first_edge < nb ? row_sees(first_edge) : 0u;
     int since = 0, edges = 0;
     for (int i = 0; i < nb; ++i) {
       const int p0 = (split + i * stride) * BK, key = p0 + kl;
@@ -542,8 +574,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           }
           ++edges;
         }
-        // lane n: which of the warp's 32 positions row n sees; then its transpose
-        const uint32_t rowsee = lane < NH ? seen_bits(a, rowt[sub * NT + h0 + lane], p0 + wq * 32, pos, len) : 0u;
+        const uint32_t rowsee = i == first_edge ? first_sees : row_sees(i);
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
           const uint32_t b = __ballot_sync(0xffffffffu, (rowsee >> k) & 1u);
@@ -606,35 +637,36 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       __syncwarp();
       if (group_any(bar, GT, top > TOP || !ok)) {
         if (group_any(bar, GT, *reinterpret_cast<volatile int*>(&dead) != 0)) break;
-        uint32_t mx = 0, dm = 0, need = 0;
-        const uint32_t dvb = I8 ? __float_as_uint(dvv) : 0u;
-#pragma unroll
-        for (int n = 0; n < NH; ++n) {  // lane n keeps row n
-          const float s = n & 1 ? s2[n / 2].y : s2[n / 2].x, sn = s * gr.c[h0 + n], x = fmaf(s, gr.c[h0 + n], gr.nm[h0 + n]);
-          const bool over = (I8 ? x + fmaxf(-29.f, ldv + gr.lv[h0 + n]) : x) > TOP;
-          const uint32_t hi = __reduce_max_sync(0xffffffffu, sn == sn ? ordered(sn) : 0u);
-          const uint32_t dmn = I8 ? __reduce_max_sync(0xffffffffu, (vis >> n) & 1u ? dvb : 0u) : 0u;
-          if (__any_sync(0xffffffffu, over)) need |= 1u << n;
-          if (lane == n) mx = hi, dm = dmn;
+        // Lane n (of 16 rows, and n + 16) gets the largest score of row n among the
+        // warp's positions, and the largest scale of V among those that it sees.
+        const float mx = lane_max<NH>([&](int n) {
+          const float s = (n & 1 ? s2[n / 2].y : s2[n / 2].x) * gr.c[h0 + n];
+          return s == s ? s : -INFINITY;
+        });
+        float dm = 0.f;
+        if (I8) {
+          if (edge)
+            dm = lane_max<NH>([&](int n) { return (vis >> n) & 1u ? dvv : 0.f; });
+          else
+            dm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(dvv)));
         }
         if (lane < NH) gr.mx[wq][h0 + lane] = mx, gr.dm[wq][h0 + lane] = dm;
-        if (lane == 0) gr.need[half][wq] = need;
         group_sync(bar, GT);
         if (wq == 0) {
           if (lane < NH) {
             const int n = h0 + lane;
             float fo = 1.f, fl = 1.f;
-            const uint32_t* nd = gr.need[half];
-            if (((nd[0] | nd[1] | nd[2] | nd[3]) >> lane) & 1u) {  // each row by itself
+            const float top = fmaxf(fmaxf(gr.mx[0][n], gr.mx[1][n]), fmaxf(gr.mx[2][n], gr.mx[3][n]));
+            const float d = fmaxf(fmaxf(gr.dm[0][n], gr.dm[1][n]), fmaxf(gr.dm[2][n], gr.dm[3][n]));
+            // each row by itself: moved if its own largest weight and scale may leave the range
+            if (top + gr.nm[n] + (I8 ? fmaxf(-29.f, __log2f(d) + gr.lv[n]) : 0.f) > TOP) {
               // fp16: the largest weight becomes 2^4, so that the low halves reach 2^-28 of it
-              const float top4 = unordered(max(max(gr.mx[0][n], gr.mx[1][n]), max(gr.mx[2][n], gr.mx[3][n]))) - (I8 ? 0.f : 4.f);
-              const float mn = fmaxf(-gr.nm[n], top4);
+              const float mn = fmaxf(-gr.nm[n], top - (I8 ? 0.f : 4.f));
               fo = fl = ex2(-gr.nm[n] - mn);
               gr.nm[n] = -mn;
               if (I8) {
-                const uint32_t d = max(max(gr.dm[0][n], gr.dm[1][n]), max(gr.dm[2][n], gr.dm[3][n]));
-                const int ex = max((int)(d >> 23) - 126, -96);  // a power of two above the largest scale
-                if (d && (float)(24 - ex) < gr.lv[n]) {
+                const int ex = max((int)(__float_as_uint(d) >> 23) - 126, -96);  // a power of two above the largest scale
+                if (d > 0.f && (float)(24 - ex) < gr.lv[n]) {
                   const float nv = pow2(24 - ex);
                   fo *= nv / gr.vs[n];
                   gr.vs[n] = nv;
@@ -750,12 +782,12 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         l[n] = keep + __shfl_xor_sync(0xffffffffu, send, w);
       }
     }
-    if (lane < NH) gr.mx[wq][h0 + lane] = __float_as_uint(l[0]);
+    if (lane < NH) gr.mx[wq][h0 + lane] = l[0];
     group_sync(bar, GT);
     if (wq == 0 && lane < NH) {
       float L = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) L += __uint_as_float(gr.mx[k][h0 + lane]);
+      for (int k = 0; k < 4; ++k) L += gr.mx[k][h0 + lane];
       cta_ml[sub * NT + h0 + lane] = make_float2(-gr.nm[h0 + lane], L);
     }
     fence_before();
