@@ -98,7 +98,6 @@ __device__ __forceinline__ unsigned seen_bits(const TreeArgs& a, int t, int p0, 
 __device__ __forceinline__ void tree_join_rest(int C, int nclusters) {
   if (C > 1) cluster_barrier();
   else __syncthreads();
-  __syncthreads();
   if (C > 1) cluster_barrier();
   if (nclusters == 1) return;
   __syncthreads();
@@ -107,8 +106,6 @@ __device__ __forceinline__ void tree_join_rest(int C, int nclusters) {
 template <int HD, int ROWS, int THREADS>
 __device__ __forceinline__ void tree_join(const TreeArgs& a, int tid, const int* rowt, float2* cta_ml, float* fold, int rows,
                                           int C, int rank, int nclusters) {
-  __shared__ float fac[ROWS][8];  // the cluster's ranks' factors of this rank's rows
-  __shared__ float2 own_ml[ROWS];
   __shared__ int is_last;
   constexpr int V4 = HD / 4;
   float4* fold4 = reinterpret_cast<float4*>(fold);
@@ -131,35 +128,31 @@ __device__ __forceinline__ void tree_join(const TreeArgs& a, int tid, const int*
   const int mine = rows > rank ? (rows - rank + C - 1) / C : 0;
   constexpr int64_t PS = ROWS * (HD + 4);               // a cluster's share: [row][HD + 4]
   float* part = a.part + unit * (a.nsplit / C) * PS;
-  if (tid < mine) {
-    const int n = rank + tid * C;
+  for (int i = tid; i < mine * V4; i += THREADS) {
+    const int n = rank + i / V4 * C, d4 = i % V4;
     float2 x[8];
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f), y[8];
     float M = TA_NONE, L = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (k < C) x[k] = peer_f2(&cta_ml[n], k), M = fmaxf(M, x[k].x);
+      if (k < C) x[k] = peer_f2(&cta_ml[n], k), y[k] = peer_f4(&fold4[n * V4 + d4], k);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < C) M = fmaxf(M, x[k].x);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (k < C) {
         const float f = ex2(x[k].x - M);
         L += x[k].y * f;
-        fac[tid][k] = f;
+        add(A, y[k], f);
       }
-    own_ml[tid] = make_float2(M, L);
-    if (nclusters > 1) *reinterpret_cast<float2*>(part + (split / C) * PS + n * (HD + 4)) = make_float2(M, L);
-  }
-  __syncthreads();
-  for (int i = tid; i < mine * V4; i += THREADS) {
-    const int s = i / V4, d4 = i % V4, n = rank + s * C;
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f), y[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < C) y[k] = peer_f4(&fold4[n * V4 + d4], k);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < C) add(A, y[k], fac[s][k]);
-    if (nclusters == 1) store(n, d4, A, own_ml[s].y);
-    else *reinterpret_cast<float4*>(part + (split / C) * PS + n * (HD + 4) + 4 + d4 * 4) = A;
+    if (nclusters == 1) {
+      store(n, d4, A, L);
+    } else {
+      float* p = part + (split / C) * PS + n * (HD + 4);
+      *reinterpret_cast<float4*>(p + 4 + d4 * 4) = A;
+      if (d4 == 0) *reinterpret_cast<float2*>(p) = make_float2(M, L);
+    }
   }
   if (C > 1) cluster_barrier();  // no rank leaves while another reads its memory
   if (nclusters == 1) return;

@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
             bad = key >= len;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const uint4 x = *reinterpret_cast<const uint4*>(vrow + (e >> 3) * (F::TILE / 2) + (e & 7) * 16);
+              const uint4 x = *reinterpret_cast<const uint4*>(vrow + (e >> 3) * (F::TILE / 2) + ((e ^ kl) & 7) * 16);  // neighbours on other banks
               const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) bad = bad || (w[j] & 0x7c00u) == 0x7c00u || (w[j] & 0x7c000000u) == 0x7c000000u;
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
             if (bad)
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                *reinterpret_cast<uint4*>(vrow + (e >> 3) * (F::TILE / 2) + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(vrow + (e >> 3) * (F::TILE / 2) + ((e ^ kl) & 7) * 16) = make_uint4(0, 0, 0, 0);
             bad_row[edges & 1][kl] = bad;
             fence_proxy_async_smem();
             mbar_arrive(&bars.v_clean[edges & 1]);
