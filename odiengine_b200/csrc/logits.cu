@@ -17,10 +17,12 @@
 namespace odi_cuda {
 namespace {
 
-// One CTA takes SLICE ids of one row: its logits are requested first, then
-// the row's history and the biases are sorted into a word per id in shared
-// memory -- the count in the low half, the last bias entry + 1 in the high
-// half -- and each id is adjusted and stored once.  So the row is read and
+// One CTA takes SLICE ids of one row.  Everything it reads is requested at
+// once -- its logits and mask words, the first entries of the row's history and
+// of the biases -- so a CTA pays one round trip to memory; then the history and
+// the biases are sorted into a word per id in shared memory -- the count in the
+// low half, the last bias entry + 1 in the high half -- and each id is adjusted
+// and stored once.  So the row is read and
 // written once whatever the penalties, and the history is re-read (from L2)
 // once per slice.  The slice starts on a 16-byte boundary of the row's own
 // address, whatever the vocabulary and row stride.  The slices' best ids meet
@@ -28,9 +30,7 @@ namespace {
 // inverted id, so equal values keep the lowest id and the order in which CTAs
 // arrive does not matter.  The row's last CTA writes the token and zeroes the
 // row's scratch for the next call.
-constexpr int SLICE = 4096;
 constexpr int THREADS = 256;
-constexpr int VPT = SLICE / (4 * THREADS);  // 16-byte pieces per thread
 
 struct LogitsArgs {
   const float* in;
@@ -52,7 +52,12 @@ struct LogitsArgs {
   unsigned* arrived;         // [rows]
 };
 
+// VPT: 16-byte pieces per thread.  Four for many rows; one where the CTAs of
+// all rows would not fill the SMs, so that a row spreads over more of them.
+template <int VPT>
 __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
+  constexpr int SLICE = 4 * THREADS * VPT;
+  constexpr int HPT = 4;  // history entries per thread requested ahead
   __shared__ unsigned words[SLICE];
   __shared__ unsigned long long warp_best[THREADS / 32];
   pdl_launch_dependents();
@@ -79,31 +84,47 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
       v[u].w = id + 3 >= 0 && id + 3 < a.V ? __ldcg(in + id + 3) : 0.f;
     }
   }
+  const unsigned* mask = a.mask ? a.mask + row * a.mask_ld : nullptr;
+  unsigned mlo[VPT], mhi[VPT];
+#pragma unroll
+  for (int u = 0; u < VPT; ++u) {  // the words of four ids from id0 on
+    mlo[u] = mhi[u] = 0;
+    const int64_t id0 = first + (u * THREADS + tid) * 4;
+    if (mask && id0 + 3 >= 0 && id0 < a.V) {
+      const int64_t i0 = id0 < 0 ? 0 : id0, i3 = id0 + 3 < a.V ? id0 + 3 : a.V - 1;
+      mlo[u] = __ldcg(mask + (i0 >> 5));
+      mhi[u] = __ldcg(mask + (i3 >> 5));
+    }
+  }
   if (lists) {
     const int64_t lo = first < 0 ? 0 : first, hi = first + SLICE < a.V ? first + SLICE : a.V;
+    const int* hist = a.history ? a.history + row * a.history_ld : nullptr;
+    int n = !hist ? 0 : a.history_len ? __ldcg(a.history_len + row) : a.history_max;
+    int h[HPT];
+#pragma unroll
+    for (int u = 0; u < HPT; ++u) h[u] = tid + u * THREADS < a.history_max && hist ? __ldcg(hist + tid + u * THREADS) : -1;
+    const int b0 = tid < a.bias_count ? __ldcg(a.bias_ids + tid) : -1;
+    n = n < a.history_max ? n : a.history_max;
     __syncthreads();
-    if (a.history) {
-      const int* hist = a.history + row * a.history_ld;
-      int n = a.history_len ? __ldcg(a.history_len + row) : a.history_max;
-      n = n < a.history_max ? n : a.history_max;
-      for (int i = tid; i < n; i += THREADS) {
-        const int id = __ldcg(hist + i);
-        if (id >= lo && id < hi) atomicAdd(&words[id - first], 1u);
-      }
-      __syncthreads();
-    }
+    auto count = [&](int id) {
+      if (id >= lo && id < hi) atomicAdd(&words[id - first], 1u);
+    };
+#pragma unroll
+    for (int u = 0; u < HPT; ++u)
+      if (tid + u * THREADS < n) count(h[u]);
+    for (int i = tid + HPT * THREADS; i < n; i += THREADS) count(__ldcg(hist + i));
+    __syncthreads();
     for (int i = tid; i < a.bias_count; i += THREADS) {
-      const int id = __ldcg(a.bias_ids + i);
+      const int id = i == tid ? b0 : __ldcg(a.bias_ids + i);
       if (id >= lo && id < hi) {  // the low halves no longer change: the maximum is of the entry
         unsigned* w = &words[id - first];
         atomicMax(w, ((unsigned)(i + 1) << 16) | (*(volatile unsigned*)w & 0xffffu));
       }
     }
-    __syncthreads();
+    if (a.bias_count) __syncthreads();
   }
   float bv = -INFINITY;
   int64_t bi = -1;
-  const unsigned* mask = a.mask ? a.mask + row * a.mask_ld : nullptr;
   float* out = a.out ? a.out + row * a.ld_out : nullptr;
   const bool out_vec = out && (((uintptr_t)out >> 2) & 3) == (unsigned)shift;
 #pragma unroll
@@ -129,8 +150,8 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
       }
     }
     if (mask) {  // four bits from id0 on; ids before the row's first have no bits
-      const int64_t i0 = id0 < 0 ? 0 : id0, i3 = id0 + 3 < a.V ? id0 + 3 : a.V - 1;
-      const unsigned bits = __funnelshift_r(__ldcg(mask + (i0 >> 5)), __ldcg(mask + (i3 >> 5)), (unsigned)(i0 & 31)) << (int)(i0 - id0);
+      const int64_t i0 = id0 < 0 ? 0 : id0;
+      const unsigned bits = __funnelshift_r(mlo[u], mhi[u], (unsigned)(i0 & 31)) << (int)(i0 - id0);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (!((bits >> e) & 1u)) x[e] = -INFINITY;
@@ -223,8 +244,11 @@ int odi_cuda_logits_adjust(const float* d_logits, int64_t ld_logits, float* d_ou
   a.best = static_cast<unsigned long long*>(d_scratch);
   a.arrived = reinterpret_cast<unsigned*>(a.best + rows);
   // a row may start up to three ids past a 16-byte boundary
-  const dim3 grid((unsigned)((V + 3 + SLICE - 1) / SLICE), rows);
-  return kv_launched(launch_pdl(logits_kernel, grid, dim3(THREADS), (cudaStream_t)stream, a), "logits_adjust");
+  auto ctas = [&](int vpt) { return (unsigned)((V + 3 + 4 * THREADS * vpt - 1) / (4 * THREADS * vpt)); };
+  cudaStream_t s = (cudaStream_t)stream;
+  const cudaError_t e = (int64_t)ctas(4) * rows >= 148 * 2 ? launch_pdl(logits_kernel<4>, dim3(ctas(4), rows), dim3(THREADS), s, a)
+                                                           : launch_pdl(logits_kernel<1>, dim3(ctas(1), rows), dim3(THREADS), s, a);
+  return kv_launched(e, "logits_adjust");
 }
 
 }  // extern "C"
