@@ -64,24 +64,27 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
   const int tid = threadIdx.x;
   const bool lists = a.history || a.bias_count;
   if (lists)
-    for (int i = tid; i < SLICE / 4; i += THREADS) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) reinterpret_cast<uint4*>(words)[u * THREADS + tid] = make_uint4(0, 0, 0, 0);
   pdl_wait();
   const int64_t row = blockIdx.y;
   const float* in = a.in + row * a.ld_in;
-  // ids of this slice: first .. first + SLICE - 1, clipped to the vocabulary
-  const int shift = (int)(((uintptr_t)in >> 2) & 3);
-  const int64_t first = (int64_t)blockIdx.x * SLICE - shift;
+  // ids of this slice: first .. first + SLICE - 1, clipped to the vocabulary.
+  // Ids, and the ends of a slice past the last, fit 32 bits (V <= 2^31 - 2^16).
+  const int V = (int)a.V, shift = (int)(((uintptr_t)in >> 2) & 3);
+  const int first = (int)blockIdx.x * SLICE - shift;
+  const bool inner = first >= 0 && first <= V - SLICE;  // every id of the slice is a token
   float4 v[VPT];
 #pragma unroll
   for (int u = 0; u < VPT; ++u) {
-    const int64_t id = first + (u * THREADS + tid) * 4;
-    if (id >= 0 && id + 3 < a.V) {
+    const int id = first + (u * THREADS + tid) * 4;
+    if (inner || (id >= 0 && id < V - 3)) {
       v[u] = __ldcg(reinterpret_cast<const float4*>(in + id));
     } else {
-      v[u].x = id >= 0 && id < a.V ? __ldcg(in + id) : 0.f;
-      v[u].y = id + 1 >= 0 && id + 1 < a.V ? __ldcg(in + id + 1) : 0.f;
-      v[u].z = id + 2 >= 0 && id + 2 < a.V ? __ldcg(in + id + 2) : 0.f;
-      v[u].w = id + 3 >= 0 && id + 3 < a.V ? __ldcg(in + id + 3) : 0.f;
+      v[u].x = id >= 0 && id < V ? __ldcg(in + id) : 0.f;
+      v[u].y = id + 1 >= 0 && id + 1 < V ? __ldcg(in + id + 1) : 0.f;
+      v[u].z = id + 2 >= 0 && id + 2 < V ? __ldcg(in + id + 2) : 0.f;
+      v[u].w = id + 3 >= 0 && id + 3 < V ? __ldcg(in + id + 3) : 0.f;
     }
   }
   const unsigned* mask = a.mask ? a.mask + row * a.mask_ld : nullptr;
@@ -89,34 +92,34 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
 #pragma unroll
   for (int u = 0; u < VPT; ++u) {  // the words of four ids from id0 on
     mlo[u] = mhi[u] = 0;
-    const int64_t id0 = first + (u * THREADS + tid) * 4;
-    if (mask && id0 + 3 >= 0 && id0 < a.V) {
-      const int64_t i0 = id0 < 0 ? 0 : id0, i3 = id0 + 3 < a.V ? id0 + 3 : a.V - 1;
-      mlo[u] = __ldcg(mask + (i0 >> 5));
-      mhi[u] = __ldcg(mask + (i3 >> 5));
+    const int id0 = first + (u * THREADS + tid) * 4;
+    if (mask && (inner || (id0 + 3 >= 0 && id0 < V))) {
+      mlo[u] = __ldcg(mask + (max(id0, 0) >> 5));
+      mhi[u] = __ldcg(mask + (min(id0 + 3, V - 1) >> 5));
     }
   }
   if (lists) {
-    const int64_t lo = first < 0 ? 0 : first, hi = first + SLICE < a.V ? first + SLICE : a.V;
+    const int lo = max(first, 0), span = max(min(first + SLICE, V) - lo, 0);  // the last slice may hold no id
     const int* hist = a.history ? a.history + row * a.history_ld : nullptr;
     int n = !hist ? 0 : a.history_len ? __ldcg(a.history_len + row) : a.history_max;
     int h[HPT];
 #pragma unroll
-    for (int u = 0; u < HPT; ++u) h[u] = tid + u * THREADS < a.history_max && hist ? __ldcg(hist + tid + u * THREADS) : -1;
+    for (int u = 0; u < HPT; ++u) h[u] = hist && tid + u * THREADS < a.history_max ? __ldcg(hist + tid + u * THREADS) : -1;
     const int b0 = tid < a.bias_count ? __ldcg(a.bias_ids + tid) : -1;
-    n = n < a.history_max ? n : a.history_max;
+    n = min(n, a.history_max);
     __syncthreads();
-    auto count = [&](int id) {
-      if (id >= lo && id < hi) atomicAdd(&words[id - first], 1u);
-    };
+    auto mine = [&](int id) { return (unsigned)(id - lo) < (unsigned)span && id >= 0; };
 #pragma unroll
     for (int u = 0; u < HPT; ++u)
-      if (tid + u * THREADS < n) count(h[u]);
-    for (int i = tid + HPT * THREADS; i < n; i += THREADS) count(__ldcg(hist + i));
+      if (tid + u * THREADS < n && mine(h[u])) atomicAdd(&words[h[u] - first], 1u);
+    for (int i = tid + HPT * THREADS; i < n; i += THREADS) {
+      const int id = __ldcg(hist + i);
+      if (mine(id)) atomicAdd(&words[id - first], 1u);
+    }
     __syncthreads();
     for (int i = tid; i < a.bias_count; i += THREADS) {
       const int id = i == tid ? b0 : __ldcg(a.bias_ids + i);
-      if (id >= lo && id < hi) {  // the low halves no longer change: the maximum is of the entry
+      if (mine(id)) {  // the low halves no longer change: the maximum is of the entry
         unsigned* w = &words[id - first];
         atomicMax(w, ((unsigned)(i + 1) << 16) | (*(volatile unsigned*)w & 0xffffu));
       }
@@ -124,19 +127,18 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
     if (a.bias_count) __syncthreads();
   }
   float bv = -INFINITY;
-  int64_t bi = -1;
+  int bi = -1;
   float* out = a.out ? a.out + row * a.ld_out : nullptr;
   const bool out_vec = out && (((uintptr_t)out >> 2) & 3) == (unsigned)shift;
 #pragma unroll
   for (int u = 0; u < VPT; ++u) {
-    const int slot = (u * THREADS + tid) * 4;
-    const int64_t id0 = first + slot;
-    if (id0 + 3 < 0 || id0 >= a.V) continue;
+    const int slot = (u * THREADS + tid) * 4, id0 = first + slot;
+    if (!inner && (id0 + 3 < 0 || id0 >= V)) continue;
     float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
     if (lists) {
       const uint4 w4 = *reinterpret_cast<const uint4*>(&words[slot]);
-      const unsigned w[4] = {w4.x, w4.y, w4.z, w4.w};
       if (w4.x | w4.y | w4.z | w4.w) {
+        const unsigned w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned c = w[e] & 0xffffu, b = w[e] >> 16;
@@ -150,25 +152,29 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
       }
     }
     if (mask) {  // four bits from id0 on; ids before the row's first have no bits
-      const int64_t i0 = id0 < 0 ? 0 : id0;
-      const unsigned bits = __funnelshift_r(mlo[u], mhi[u], (unsigned)(i0 & 31)) << (int)(i0 - id0);
+      const int i0 = max(id0, 0);
+      const unsigned bits = __funnelshift_r(mlo[u], mhi[u], (unsigned)(i0 & 31)) << (i0 - id0);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (!((bits >> e) & 1u)) x[e] = -INFINITY;
     }
-    const bool whole = id0 >= 0 && id0 + 3 < a.V;
-    if (out) {
-      if (whole && out_vec) {
-        *reinterpret_cast<float4*>(out + id0) = make_float4(x[0], x[1], x[2], x[3]);
-      } else {
+    const bool whole = inner || (id0 >= 0 && id0 < V - 3);
+    if (whole) {
+      if (out_vec) *reinterpret_cast<float4*>(out + id0) = make_float4(x[0], x[1], x[2], x[3]);
+      else if (out) out[id0] = x[0], out[id0 + 1] = x[1], out[id0 + 2] = x[2], out[id0 + 3] = x[3];
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (id0 + e >= 0 && id0 + e < a.V) out[id0 + e] = x[e];
+      for (int e = 0; e < 4; ++e) {
+        const bool in_row = id0 + e >= 0 && id0 + e < V;
+        if (out && in_row) out[id0 + e] = x[e];
+        if (!in_row) x[e] = -INFINITY;
       }
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if ((whole || (id0 + e >= 0 && id0 + e < a.V)) && x[e] > bv) bv = x[e], bi = id0 + e;  // ids ascend
+    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));  // NaN is passed over
+    if (top > bv) {  // ids ascend: the first of equal values stays
+      bv = top;
+      bi = id0 + (x[0] == top ? 0 : x[1] == top ? 1 : x[2] == top ? 2 : 3);
+    }
   }
   if (!a.tokens) return;
   // order-preserving image of the value (-0 as +0); 0: nothing above -inf
@@ -212,7 +218,7 @@ int odi_cuda_logits_adjust(const float* d_logits, int64_t ld_logits, float* d_ou
                            size_t scratch_bytes, void* stream) {
   auto bad = [](const char* m) { return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, m); };
   if (!d_logits || (!d_out && !d_tokens)) return bad("logits_adjust: null argument");
-  if (rows < 0 || rows > 65535 || V < 1 || V > 0x7ffffff0) return bad("logits_adjust: rows or vocabulary out of range");
+  if (rows < 0 || rows > 65535 || V < 1 || V > 0x7fff0000) return bad("logits_adjust: rows or vocabulary out of range");
   if (ld_logits < V || (d_out && ld_out < V)) return bad("logits_adjust: a row stride is shorter than the vocabulary");
   if (d_out == d_logits && ld_out != ld_logits) return bad("logits_adjust: in place needs one row stride");
   if (((uintptr_t)d_logits | (uintptr_t)d_out | (uintptr_t)d_tokens) & 3) return bad("logits_adjust: misaligned buffer");

@@ -93,7 +93,7 @@ def test_logits_refusals():
             setattr(opts, k, v)
         return L.odi_cuda_logits_adjust(x, ld, out, ldo, tok, rows, V, ctypes.byref(opts), scr, n, None)
 
-    for kw in (dict(x=None), dict(out=None, tok=None), dict(rows=-1), dict(rows=70000), dict(V=0), dict(ld=99),
+    for kw in (dict(x=None), dict(out=None, tok=None), dict(rows=-1), dict(rows=70000), dict(V=0), dict(V=0x7fff0001, ld=1 << 31, ldo=1 << 31), dict(ld=99),
                dict(ldo=99), dict(x=A, out=A, ldo=101), dict(x=A + 2), dict(scr=None), dict(scr=A + 4), dict(n=31),
                dict(repeat_penalty=0.0), dict(repeat_penalty=float("nan")), dict(frequency_penalty=float("inf")),
                dict(presence_penalty=float("nan")), dict(history=A, history_ld=3, history_max=4),
