@@ -55,7 +55,7 @@ struct LogitsArgs {
 // VPT: 16-byte pieces per thread.  Four for many rows; one where the CTAs of
 // all rows would not fill the SMs, so that a row spreads over more of them.
 template <int VPT>
-__global__ void __launch_bounds__(THREADS) logits_kernel(const LogitsArgs a) {
+__global__ void __launch_bounds__(THREADS, VPT == 4 ? 5 : 1) logits_kernel(const LogitsArgs a) {
   constexpr int SLICE = 4 * THREADS * VPT;
   constexpr int HPT = 4;  // history entries per thread requested ahead
   __shared__ unsigned words[SLICE];
