@@ -423,7 +423,7 @@ int odi_cuda_argmax(const float* d_logits, int64_t V, odi_cuda_decode_state* d_s
  * ODI_CUDA_KV_I8: K and V each hold int8 codes [kv_heads][ctx][head_dim],
  * then, from the next multiple of 256 bytes, one fp32 scale per row
  * [kv_heads][ctx]; value = code * scale, scale = max|row| / 127, codes
- * rounded half away from zero.  A row with a value that is not finite gets
+ * rounded half away from zero (a writer of its own may use any scale >= 0).  A row with a value that is not finite gets
  * the scale NaN.  head_dim 64 or 128; k and v 16-byte aligned. */
 enum { ODI_CUDA_KV_F16 = 0, ODI_CUDA_KV_I8 = 1 };
 typedef struct odi_cuda_kv_cache {
@@ -475,7 +475,8 @@ int odi_cuda_kv_move(const odi_cuda_kv_cache* cache, const int32_t* d_src, const
  * fp32 scores, softmax and sums.  d_scratch: as for
  * odi_cuda_attention_decode (16-byte aligned, zero before its first use,
  * left reusable, calls on one stream only; its first int is the error word,
- * odi_cuda_workspace_status). */
+ * odi_cuda_workspace_status); its size depends on head_dim alone, and calls
+ * of different shapes may share it.  int8 rows' scales are not negative. */
 #define ODI_CUDA_TREE_MAX 256
 size_t odi_cuda_attention_tree_scratch_bytes(int tokens, int heads, int kv_heads, int head_dim, int ctx);
 int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_cache* cache, float* d_out,

@@ -510,9 +510,12 @@ TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   p.units = kv_heads * p.tiles;
   const int64_t block = p.tc ? 128 : TA_GROUP * TA_WARPS;
   p.most = ((int64_t)ctx + block - 1) / block;
-  p.part_off = (16 + (size_t)p.units * 8 * 4 + 255) / 256 * 256;
-  const int64_t splits = p.room / p.units;
-  p.bytes = p.part_off + (size_t)p.units * (splits < 1 ? 1 : splits) * p.rows * (hd + 4) * 4;
+  // The scratch is laid out alike whatever the number of tokens, so that calls
+  // of any T may share one: counters and shares are used only by units split
+  // over several clusters, whose CTAs are all resident -- at most 4 per SM of 8
+  // rows, 3 of 16, 2 of 32, 1 of 64.
+  p.part_off = (16 + (size_t)TA_SMS * 4 * 8 * 4 + 255) / 256 * 256;
+  p.bytes = p.part_off + (size_t)TA_SMS * 64 * (hd + 4) * 4;
   return p;
 }
 

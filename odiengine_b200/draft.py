@@ -8,7 +8,9 @@ tokens (a chain or a tree) of one sequence in one pass, on device tensors.
     kv_read          cache rows out as fp16 / fp32
 
 over a :class:`KVCache` of fp16 rows (the layout of the decode step) or of
-int8 rows with one scale each (half the bytes).  Calls are asynchronous on
+int8 rows with one scale each (half the bytes).  :class:`DraftVerifier` is the
+step made of them and of the library's products, for the models of
+odiengine_b200.decode.  Calls are asynchronous on
 `stream` (default: the tensors' device's current stream); errors are
 :class:`odiengine_b200.OdiCudaError`, or ValueError / TypeError for tensors
 that do not fit.  The position is device resident (`state`, the decode
@@ -21,7 +23,7 @@ import ctypes
 
 import torch
 
-from . import check, lib
+from . import FLAG_PDL, MatmulOpts, check, lib
 
 KV_F16, KV_I8 = 0, 1                      # ODI_CUDA_KV_*
 KV_DTYPES = {"f16": KV_F16, "i8": KV_I8}
@@ -187,8 +189,8 @@ def kv_move(cache: KVCache, src, dst, state=None, stream=None) -> None:
 
 
 def attention_tree_scratch(cache: KVCache, tokens: int, heads: int):
-    """Zeroed scratch for attention_tree calls of this shape on one stream, of
-    any layer."""
+    """Zeroed scratch for attention_tree calls on one stream: of any layer, any
+    number of tokens and any heads of this head_dim."""
     n = lib().odi_cuda_attention_tree_scratch_bytes(tokens, heads, cache.kv_heads, cache.head_dim, cache.ctx)
     if not n:
         raise ValueError(f"attention_tree: no such shape (tokens {tokens}, heads {heads}, kv_heads {cache.kv_heads})")
@@ -265,3 +267,167 @@ def logits_adjust(logits, out=None, tokens=None, *, scratch=None, history=None, 
           None if tokens is None else _flat(tokens, i32, "tokens", dev, rows), rows, V, ctypes.addressof(o),
           None if scratch is None else _flat(scratch, torch.uint8, "scratch", dev, n), n)
     return out, tokens
+
+
+class DraftVerifier:
+    """Greedy decoding of one sequence that checks drafted tokens, a tree of
+    them per step: the model of decode.DecodeModel (its fused step, for T
+    tokens at once) over a cache of fp16 or int8 rows.
+
+        v = DraftVerifier(cfg, seeded_model(cfg, interleave_gate_up=False), cache="i8")
+        v.start(prompt)
+        new = v.verify(drafted_tokens, parents)   # 1 .. 1 + len(drafted) tokens
+
+    The weights keep gate|up in [gate | up] order (the SwiGLU prologue reads
+    it).  q_norms / k_norms: per-layer head_dim weights of models that norm q
+    and k per head.  history: how many of the last tokens (the node's own
+    ancestors included) the penalties of verify count."""
+
+    def __init__(self, cfg, weights, *, cache: str = "f16", max_nodes: int = 64, history: int = 0, q_norms=None,
+                 k_norms=None, norm_eps: float = 1e-6, device=None):
+        if weights.gu_interleaved:
+            raise ValueError("DraftVerifier needs gate|up weights in [gate | up] order (interleave_gate_up=False)")
+        if not 1 <= max_nodes <= TREE_MAX:
+            raise ValueError(f"max_nodes: 1 to {TREE_MAX}")
+        self.cfg, self.w = cfg, weights
+        self.device = dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.max_nodes, self.history = max_nodes, history
+        self.q_norms, self.k_norms, self.norm_eps = q_norms, k_norms, norm_eps
+        self.caches = [KVCache.new(cache, cfg.kv_heads, cfg.head_dim, cfg.ctx, dev) for _ in range(cfg.layers)]
+        T, f32 = max_nodes, torch.float32
+        self.x = torch.empty((T, cfg.hidden), dtype=f32, device=dev)
+        self.qkv = torch.empty((T, cfg.qkv_rows), dtype=f32, device=dev)
+        self.q = torch.empty((T, cfg.heads * cfg.head_dim), dtype=f32, device=dev)
+        self.attn = torch.empty_like(self.q)
+        self.gu = torch.empty((T, 2 * cfg.ffn), dtype=f32, device=dev)
+        self.logits = torch.empty((T, cfg.vocab), dtype=f32, device=dev)
+        self.greedy = torch.empty(T, dtype=torch.int32, device=dev)
+        # an odi_cuda_decode_state per node: its token, and the slot of node 0
+        self.states = torch.zeros((T, 4), dtype=torch.int32, device=dev)
+        self.scratch = attention_tree_scratch(self.caches[0], T, cfg.heads)
+        self.logits_ws = logits_scratch(T, dev)
+        for lw in weights.layers:
+            for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown):
+                dw._ws_for(T, cfg.act_mode, dev)
+        weights.output._ws_for(T, cfg.act_mode, dev)
+        self.pos, self.pending, self.tokens = 0, None, []
+
+    # ---- the forward pass of T nodes --------------------------------------
+    def _product(self, dw, x, y, T, norm=None, swiglu=False, accumulate=False):
+        o = MatmulOpts(None if norm is None else norm.data_ptr(), self.cfg.eps, int(swiglu), int(accumulate), None, 0, None)
+        ws = dw._ws
+        check(lib().odi_cuda_matmul_fused(dw.dtype, dw.data_ptr, x.data_ptr(), y.data_ptr(), T, dw.N, dw.K,
+                                          self.cfg.act_mode, ws.data_ptr(), ws.numel(), FLAG_PDL, ctypes.byref(o),
+                                          _raw_stream(self.device.index)))
+
+    def _forward(self, tokens, depth, mask, logits: bool) -> None:
+        """Nodes at slots pos .. pos + T - 1; logits rows 0 .. T - 1."""
+        cfg, T = self.cfg, len(tokens)
+        host = torch.tensor([[t, self.pos, 0, 0] for t in tokens], dtype=torch.int32)
+        self.states[:T].copy_(host)
+        state, stream = self.states[0], _raw_stream(self.device.index)
+        for t in range(T):
+            check(lib().odi_cuda_embed(self.w.token_embd.data_ptr(), cfg.vocab, cfg.hidden, self.states.data_ptr() + 16 * t,
+                                       self.x.data_ptr() + 4 * cfg.hidden * t, None, None, None, stream))
+        for i, lw in enumerate(self.w.layers):
+            self._product(lw.wqkv, self.x, self.qkv, T, norm=lw.attn_norm)
+            qk_rope_append(self.qkv[:T], self.caches[i], state, self.q[:T], heads=cfg.heads, theta=cfg.theta,
+                           q_norm=self.q_norms[i] if self.q_norms else None,
+                           k_norm=self.k_norms[i] if self.k_norms else None, eps=self.norm_eps, depth=depth)
+            attention_tree(self.q[:T], self.caches[i], self.attn[:T], state, heads=cfg.heads,
+                           scale=cfg.head_dim ** -0.5, scratch=self.scratch, mask=mask)
+            self._product(lw.wo, self.attn, self.x, T, accumulate=True)
+            self._product(lw.wgu, self.x, self.gu, T, norm=lw.ffn_norm)
+            self._product(lw.wdown, self.gu, self.x, T, swiglu=True, accumulate=True)
+        if logits:
+            self._product(self.w.output, self.x, self.logits, T, norm=self.w.out_norm)
+
+    def status(self) -> int:
+        """OR of the device error words (0: no bounded wait gave up)."""
+        words = [self.scratch[:4].view(torch.int32)]
+        for lw in self.w.layers:
+            words += [dw._ws[:4].view(torch.int32) for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown)]
+        words.append(self.w.output._ws[:4].view(torch.int32))
+        v = 0
+        for x in torch.cat(words).cpu().tolist():
+            v |= x
+        return v
+
+    def _check(self) -> None:
+        st = self.status()
+        if st:
+            raise RuntimeError(f"draft verification: a bounded device wait gave up (error word {st:#x})")
+
+    # ---- sequences ---------------------------------------------------------
+    def start(self, prompt) -> None:
+        """A new sequence: all but the prompt's last token into the cache,
+        max_nodes at a time; the last one is what verify starts from."""
+        if not prompt or any(not 0 <= t < self.cfg.vocab for t in prompt):
+            raise ValueError("start: a prompt of tokens of the vocabulary wanted")
+        if len(prompt) > self.cfg.ctx:
+            raise ValueError("prompt longer than the context")
+        self.pos, self.tokens = 0, list(prompt)
+        with torch.cuda.device(self.device):
+            for i in range(0, len(prompt) - 1, self.max_nodes):
+                chunk = prompt[i:min(i + self.max_nodes, len(prompt) - 1)]
+                self._forward(chunk, None, None, False)
+                self.pos += len(chunk)
+            self._check()
+        self.pending = prompt[-1]
+
+    def verify(self, drafted=(), parents=None, **adjust) -> list:
+        """Checks drafted tokens: node 0 is the pending token, drafted[i] is
+        node i + 1 with parent node parents[i] <= i (None: a chain).  Returns
+        the greedy tokens along the accepted path: one, plus one for every
+        drafted token on it.  The last returned token is pending (not in the
+        cache).  adjust: logits_adjust's penalties, biases and mask (mask rows
+        per node, or one)."""
+        T = 1 + len(drafted)
+        parents = list(range(T - 1)) if parents is None else list(parents)
+        if self.pending is None:
+            raise RuntimeError("verify: start a sequence first")
+        if T > self.max_nodes or len(parents) != T - 1 or any(not 0 <= p <= i for i, p in enumerate(parents)):
+            raise ValueError(f"verify: at most {self.max_nodes - 1} drafted tokens, each after its parent")
+        if any(not 0 <= t < self.cfg.vocab for t in drafted):
+            raise ValueError("verify: drafted token outside the vocabulary")
+        if self.pos + T > self.cfg.ctx:
+            raise ValueError("verification would run past the context")
+        nodes = [self.pending, *drafted]
+        up = [-1, *parents]
+        depth, sees, path = [], [], []
+        for i, p in enumerate(up):
+            depth.append(0 if p < 0 else depth[p] + 1)
+            sees.append((0 if p < 0 else sees[p]) | (1 << i))
+            path.append([i] if p < 0 else path[p] + [i])
+        dev = self.device
+        with torch.cuda.device(dev):
+            W = (T + 31) // 32
+            words = [[(s >> (32 * w)) & 0xFFFFFFFF for w in range(W)] for s in sees]
+            mask = torch.tensor([[x - (1 << 32) if x >> 31 else x for x in r] for r in words], dtype=torch.int32).to(dev)
+            self._forward(nodes, torch.tensor(depth, dtype=torch.int32).to(dev), mask, True)
+            if self.history:
+                rows = [(self.tokens + [nodes[j] for j in path[i][1:]])[-self.history:] for i in range(T)]
+                H = max(len(r) for r in rows)
+                adjust = {**adjust, "history": torch.tensor([r + [-1] * (H - len(r)) for r in rows], dtype=torch.int32).to(dev)}
+            logits_adjust(self.logits[:T], self.logits[:T], self.greedy[:T], scratch=self.logits_ws, **adjust)
+            greedy = self.greedy[:T].tolist()
+            self._check()
+            at, kept, out = 0, [0], [greedy[0]]
+            while True:
+                nxt = next((i for i in range(at + 1, T) if up[i] == at and nodes[i] == greedy[at]), None)
+                if nxt is None:
+                    break
+                at = nxt
+                kept.append(at)
+                out.append(greedy[at])
+            if out[-1] < 0:
+                raise RuntimeError("verify: the mask allows no token")
+            if kept != list(range(len(kept))):  # a branch: its rows to the slots after the root's
+                src = torch.tensor(kept, dtype=torch.int32).to(dev)
+                dst = torch.arange(len(kept), dtype=torch.int32).to(dev)
+                for c in self.caches:
+                    kv_move(c, src, dst, state=self.states[0])
+        self.pos += len(kept)
+        self.pending = out[-1]
+        self.tokens += out
+        return out

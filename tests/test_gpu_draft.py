@@ -544,6 +544,28 @@ def test_attention_two_caches_one_scratch_and_graph(dr):
             assert torch.equal(own, o)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_shapes_share_one_scratch(dr, hd):
+    """Calls of different numbers of tokens, dtypes and lengths, one scratch,
+    alternating: each as with a scratch of its own (the joins through it leave
+    its counters zero whatever came before)."""
+    import torch
+
+    rng = np.random.default_rng(21)
+    H, KV, ctx = 8, 2, 30000
+    cs = [dr.KVCache.new(dt, KV, hd, ctx) for dt in ("f16", "i8")]
+    for c in cs:
+        fill(c, rng)
+    scr = dr.attention_tree_scratch(cs[0], 1, H)
+    assert scr.numel() == dr.attention_tree_scratch(cs[1], 256, 64).numel()
+    for T, pos in ((1, 29000), (13, 29900), (1, 200), (70, 15000), (3, 29997), (256, 20000), (1, 29999), (2, 29000)):
+        q = dev(rng.standard_normal((T, H * hd)).astype(np.float32))
+        for c in cs:
+            a = dr.attention_tree(q, c, None, state(pos), heads=H, scale=0.1, scratch=scr)
+            b = dr.attention_tree(q, c, None, state(pos), heads=H, scale=0.1, scratch=dr.attention_tree_scratch(c, T, H))
+            assert torch.equal(a, b), (T, pos)
+
+
 def test_attention_long_offsets_past_32_bits(dr):
     """kv_heads * ctx * head_dim past 2^31 values: the last head's rows are the
     ones read."""

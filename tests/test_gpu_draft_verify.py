@@ -1,0 +1,170 @@
+"""DraftVerifier: the drafted-token operators run together, as a step that
+verifies a tree, against the float64 restatement of the forward pass
+(oracle/llama.py) and against the one-token decode step.
+
+Tolerances are those of the decode step's tests, of the logits' scale: 2e-3
+with fp32 activations and an fp16 cache; 6e-2 with Q8 activations or an int8
+cache (a code is off by half a step, 1/254 of its row's largest value, as an
+activation's is)."""
+import numpy as np
+import pytest
+
+from oracle.llama import LlamaRef
+from test_gpu_decode import _oracle_weights, _tiny
+
+pytestmark = pytest.mark.gpu
+
+
+def model(act_mode, seed=7):
+    from odiengine_b200.decode import seeded_model
+
+    cfg = _tiny(act_mode)
+    return cfg, seeded_model(cfg, seed=seed, interleave_gate_up=False)
+
+
+def oracle_rows(ref, prefix, tokens, parents):
+    """Each node's logits after prefix and its ancestors (one path at a time)."""
+    paths = [[0]]
+    for p in parents:
+        paths.append(paths[p] + [len(paths)])
+    rows = []
+    for path in paths:
+        for j, n in enumerate(path):
+            lg = ref.step(tokens[n], len(prefix) + j)
+        rows.append(lg)
+    return np.stack(rows)
+
+
+@pytest.mark.parametrize("act_mode,cache,tol", [(1, "f16", 2e-3), (1, "i8", 6e-2), (0, "f16", 6e-2), (0, "i8", 6e-2)])
+def test_tree_logits_match_oracle(cuda_lib, act_mode, cache, tol):
+    from odiengine_b200.draft import DraftVerifier
+
+    cfg, mw = model(act_mode)
+    ref = LlamaRef(cfg, _oracle_weights(cuda_lib, cfg, mw))
+    v = DraftVerifier(cfg, mw, cache=cache, max_nodes=12)
+    prompt = [5, 17, 999, 3, 250, 8, 41, 700, 2, 90, 33, 61, 7, 500, 123]  # two chunks of the cache's rows
+    v.start(prompt)
+    for p, t in enumerate(prompt[:-1]):
+        ref.step(t, p)
+    assert v.pos == len(prompt) - 1
+    drafted = [4, 9, 600, 31, 2, 77, 12, 300]
+    parents = [0, 0, 1, 1, 2, 3, 6, 0]
+    want = oracle_rows(ref, prompt[:-1], [prompt[-1]] + drafted, parents)
+    kept_before = [c.k.clone() for c in v.caches]
+    out = v.verify(drafted, parents)
+    got = v.logits[:9].cpu().numpy().astype(np.float64)
+    scale = np.abs(want).max()
+    assert (np.abs(got - want) <= tol * scale).all(), np.abs(got - want).max() / scale
+    assert out == [int(np.argmax(got[0]))] or len(out) > 1
+    if cache == "f16":  # the prompt's rows are as they were
+        for a, c in zip(kept_before, v.caches):
+            assert (a[:, :len(prompt) - 1] == c.k[:, :len(prompt) - 1]).all()
+
+
+@pytest.mark.parametrize("cache", ["f16", "i8"])
+def test_drafts_do_not_change_what_is_generated(cuda_lib, cache):
+    """Good drafts, bad drafts, branches with the right token behind wrong
+    ones: every call returns the tokens of undrafted greedy decoding, more at
+    a time when the drafts were right; rows of the accepted path end up where
+    undrafted decoding has them."""
+    from odiengine_b200.draft import DraftVerifier, kv_read
+
+    cfg, mw = model(1)
+    prompt = [5, 17, 999, 3, 250]
+    plain = DraftVerifier(cfg, mw, cache=cache)
+    plain.start(prompt)
+    want = []
+    for _ in range(24):
+        want += plain.verify()
+    v = DraftVerifier(cfg, mw, cache=cache, max_nodes=32)
+    v.start(prompt)
+    got, calls, rng = [], 0, np.random.default_rng(0)
+    while len(got) < 20:
+        n = len(got)
+        w = lambda i: want[n + i]  # noqa: E731
+        bad = [int(t) for t in rng.integers(0, cfg.vocab, 6)]
+        kind = calls % 4
+        if kind == 0:    # a right chain of three
+            out, least = v.verify([w(0), w(1), w(2)]), 4
+        elif kind == 1:  # wrong first children, then the right one with a right child
+            out, least = v.verify([(w(0) + 1) % cfg.vocab, (w(0) + 2) % cfg.vocab, w(0), bad[0], w(1)], [0, 0, 0, 1, 3]), 3
+        elif kind == 2:  # nothing right
+            out, least = v.verify([(w(0) + 1) % cfg.vocab, bad[1]]), 1
+        else:            # right, then wrong
+            out, least = v.verify([w(0), (w(1) + 1) % cfg.vocab]), 2
+        assert len(out) >= least and out == want[n:n + len(out)], (kind, out, want[n:n + 6])
+        got += out
+        calls += 1
+    assert v.pos == plain.pos - (len(want) - len(got)) and v.status() == 0
+    n = v.pos
+    for a, b in zip(v.caches, plain.caches):
+        for x, y in zip(kv_read(a, 0, n), kv_read(b, 0, n)):
+            # the same rows up to the rounding of T-token and one-token steps
+            assert (x.float() - y.float()).abs().max() <= 2e-2 * y.float().abs().max()
+
+
+def test_matches_the_decode_step(cuda_lib):
+    """The verifier's tokens are those of DecodeModel's fused step wherever
+    the top-2 gap exceeds the rounding of either."""
+    from odiengine_b200.decode import DecodeModel
+    from odiengine_b200.draft import DraftVerifier
+
+    cfg, mw = model(1, seed=3)
+    dm = DecodeModel(cfg, mw, mode="fused")
+    prompt = [9, 1, 44, 723]
+    dm.prefill(prompt[:-1])
+    dm.reset(prompt[-1], len(prompt) - 1)
+    v = DraftVerifier(cfg, mw)
+    v.start(prompt)
+    for _ in range(10):
+        a, b = dm.generate(1), v.verify()
+        la, lb = dm.logits.cpu().numpy(), v.logits[0].cpu().numpy()
+        assert np.abs(la - lb).max() <= 4e-3 * np.abs(la).max()
+        top = np.sort(la)[-2:]
+        if top[1] - top[0] <= 8e-3 * np.abs(la).max():
+            break
+        assert a == b
+
+
+def test_penalties_masks_and_refusals(cuda_lib):
+    import torch
+
+    from odiengine_b200.draft import DraftVerifier
+
+    cfg, mw = model(1)
+    v = DraftVerifier(cfg, mw, max_nodes=8, history=16)
+    with pytest.raises(RuntimeError):
+        v.verify()
+    v.start([5, 17, 999])
+    first = v.verify()[0]
+    lg = v.logits[0].clone()
+    # banned, the token gives way to the next; a mask leaves one token
+    v.start([5, 17, 999])
+    second = v.verify(bias_ids=torch.tensor([first], dtype=torch.int32, device="cuda"),
+                      bias=torch.tensor([-float("inf")], device="cuda"))[0]
+    lg[first] = -float("inf")
+    assert second == int(lg.argmax()) != first
+    mask = torch.zeros((1, (cfg.vocab + 31) // 32), dtype=torch.int32, device="cuda")
+    mask[0, 3] = 1 << 5
+    v.start([5, 17, 999])
+    assert v.verify(mask=mask) == [101]
+    mask.zero_()
+    v.start([5, 17, 999])
+    with pytest.raises(RuntimeError):
+        v.verify(mask=mask)
+    v.start([5, 17, 999])
+    v.verify([first], repeat_penalty=1.5, presence_penalty=0.5)  # node 1 counts its ancestor too
+    for bad in (dict(drafted=[1] * 8), dict(drafted=[1], parents=[1]), dict(drafted=[cfg.vocab]), dict(drafted=[1, 2], parents=[0])):
+        with pytest.raises(ValueError):
+            v.verify(**bad)
+    with pytest.raises(ValueError):
+        v.start([])
+    with pytest.raises(ValueError):
+        v.start(list(range(cfg.ctx + 1)))
+    v.start(list(range(cfg.ctx)))
+    assert len(v.verify()) == 1  # the context's last slot
+    with pytest.raises(ValueError):
+        v.verify()
+    from odiengine_b200.decode import seeded_model
+    with pytest.raises(ValueError):
+        DraftVerifier(cfg, seeded_model(cfg, interleave_gate_up=True))
