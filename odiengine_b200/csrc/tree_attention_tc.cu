@@ -125,19 +125,19 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 // 32 lanes x 8 consecutive columns; complete only after ld_wait.
-__device__ __forceinline__ void ld8(uint32_t addr, uint32_t (&r)[8]) {
+__device__ __forceinline__ void ld8(uint32_t addr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(addr));
 }
 // The registers of the loads before it pass through, so no use moves ahead of it.
-template <int N>
-__device__ __forceinline__ void ld_wait(uint32_t (&r)[N][8]) {
+template <int N, int W>
+__device__ __forceinline__ void ld_wait(uint32_t (&r)[N][W]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int k = 0; k < N; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(r[k][i]));
+    for (int i = 0; i < W; ++i) asm volatile("" : "+r"(r[k][i]));
 }
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -587,19 +587,20 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       float2 s2[NH / 2];
       // a row whose scale of K or V is not finite gives NaN to who sees it
       const float dkk = finite(dk) && finite(dv) ? dk : nan, dvv = finite(dv) ? dv : 0.f;
+      {
+        uint32_t r[F::DQ][NH];  // all of this thread's sums at once: one latency
 #pragma unroll
-      for (int c0 = 0; c0 < NH; c0 += 8) {
-        uint32_t r[F::DQ][8];
+        for (int n = 0; n < NH; n += 8)
 #pragma unroll
-        for (int k = 0; k < F::DQ; ++k) ld8(s_tm + k * NT + c0, r[k]);
+          for (int k = 0; k < F::DQ; ++k) ld8(s_tm + k * NT + n, &r[k][n]);
         ld_wait(r);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
+        for (int n = 0; n < NH / 2; ++n) {
           const float2 hi = bits2(r[0][2 * n], r[0][2 * n + 1]), lo = bits2(r[1][2 * n], r[1][2 * n + 1]);
           if (I8)
-            s2[c0 / 2 + n] = __fmul2_rn(join_digits(hi, lo, bits2(r[F::DQ - 1][2 * n], r[F::DQ - 1][2 * n + 1])), f2(dkk));
+            s2[n] = __fmul2_rn(join_digits(hi, lo, bits2(r[F::DQ - 1][2 * n], r[F::DQ - 1][2 * n + 1])), f2(dkk));
           else
-            s2[c0 / 2 + n] = __fadd2_rn(hi, lo);
+            s2[n] = __fadd2_rn(hi, lo);
         }
       }
       if (I8) {
