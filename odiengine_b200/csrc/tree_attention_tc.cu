@@ -124,20 +124,68 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(r));
   return r != 0;
 }
-// 32 lanes x 8 consecutive columns; complete only after ld_wait.
-__device__ __forceinline__ void ld8(uint32_t addr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(addr));
+// 32 lanes x N consecutive columns of each digit, `stride` columns apart.  Loads
+// and wait are one statement: no use of a register can move ahead of the wait.
+#define TA_OUT8(r) "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]), "=r"((r)[6]), "=r"((r)[7])
+#define TA_OUT16(r) TA_OUT8(r), TA_OUT8((r) + 8)
+#define TA_OUT32(r) TA_OUT16(r), TA_OUT16((r) + 16)
+__device__ __forceinline__ void ld_digits(uint32_t (&r)[2][8], uint32_t addr, uint32_t stride) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : TA_OUT8(r[0]), TA_OUT8(r[1])
+      : "r"(addr), "r"(addr + 1 * stride)
+      : "memory");
 }
-// The registers of the loads before it pass through, so no use moves ahead of it.
-template <int N, int W>
-__device__ __forceinline__ void ld_wait(uint32_t (&r)[N][W]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-#pragma unroll
-    for (int i = 0; i < W; ++i) asm volatile("" : "+r"(r[k][i]));
+__device__ __forceinline__ void ld_digits(uint32_t (&r)[2][16], uint32_t addr, uint32_t stride) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : TA_OUT16(r[0]), TA_OUT16(r[1])
+      : "r"(addr), "r"(addr + 1 * stride)
+      : "memory");
+}
+__device__ __forceinline__ void ld_digits(uint32_t (&r)[2][32], uint32_t addr, uint32_t stride) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : TA_OUT32(r[0]), TA_OUT32(r[1])
+      : "r"(addr), "r"(addr + 1 * stride)
+      : "memory");
+}
+__device__ __forceinline__ void ld_digits(uint32_t (&r)[3][16], uint32_t addr, uint32_t stride) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%48];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%49];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47}, [%50];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : TA_OUT16(r[0]), TA_OUT16(r[1]), TA_OUT16(r[2])
+      : "r"(addr), "r"(addr + 1 * stride), "r"(addr + 2 * stride)
+      : "memory");
+}
+__device__ __forceinline__ void ld_digits(uint32_t (&r)[3][32], uint32_t addr, uint32_t stride) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%96];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%97];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%98];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : TA_OUT32(r[0]), TA_OUT32(r[1]), TA_OUT32(r[2])
+      : "r"(addr), "r"(addr + 1 * stride), "r"(addr + 2 * stride)
+      : "memory");
+}
+__device__ __forceinline__ void ld_digits(uint32_t (&r)[4][8], uint32_t addr, uint32_t stride) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%33];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16,%17,%18,%19,%20,%21,%22,%23}, [%34];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24,%25,%26,%27,%28,%29,%30,%31}, [%35];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : TA_OUT8(r[0]), TA_OUT8(r[1]), TA_OUT8(r[2]), TA_OUT8(r[3])
+      : "r"(addr), "r"(addr + 1 * stride), "r"(addr + 2 * stride), "r"(addr + 3 * stride)
+      : "memory");
 }
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -502,9 +550,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
 #pragma unroll
         for (int c0 = 0; c0 < NH; c0 += 8) {
           uint32_t r[F::DP][8];
-#pragma unroll
-          for (int k = 0; k < F::DP; ++k) ld8(o_tm + k * NT + c0, r[k]);
-          ld_wait(r);
+          ld_digits(r, o_tm + c0, NT);
 #pragma unroll
           for (int n = 0; n < 8; ++n) {
             float x;
@@ -589,11 +635,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       const float dkk = finite(dk) && finite(dv) ? dk : nan, dvv = finite(dv) ? dv : 0.f;
       {
         uint32_t r[F::DQ][NH];  // all of this thread's sums at once: one latency
-#pragma unroll
-        for (int n = 0; n < NH; n += 8)
-#pragma unroll
-          for (int k = 0; k < F::DQ; ++k) ld8(s_tm + k * NT + n, &r[k][n]);
-        ld_wait(r);
+        ld_digits(r, s_tm, NT);
 #pragma unroll
         for (int n = 0; n < NH / 2; ++n) {
           const float2 hi = bits2(r[0][2 * n], r[0][2 * n + 1]), lo = bits2(r[1][2 * n], r[1][2 * n + 1]);
