@@ -88,10 +88,11 @@ def test_logits_refusals():
     L = ob.lib()
 
     def call(x=A, ld=100, out=B, ldo=100, tok=A, rows=2, V=100, scr=A, n=32, **o):
-        opts = draft._LogitsOpts(1.0, 0.0, 0.0)
-        for k, v in o.items():
-            setattr(opts, k, v)
-        return L.odi_cuda_logits_adjust(x, ld, out, ldo, tok, rows, V, ctypes.byref(opts), scr, n, None)
+        f = dict(repeat_penalty=1.0, frequency_penalty=0.0, presence_penalty=0.0, history=0, history_ld=0, history_len=0,
+                 history_max=0, bias_ids=0, bias=0, bias_count=0, mask=0, mask_ld=0)
+        assert set(o) <= set(f)
+        opts = draft._LOGITS_OPTS.pack(*{**f, **o}.values())
+        return L.odi_cuda_logits_adjust(x, ld, out, ldo, tok, rows, V, opts, scr, n, None)
 
     for kw in (dict(x=None), dict(out=None, tok=None), dict(rows=-1), dict(rows=70000), dict(V=0), dict(V=0x7fff0001, ld=1 << 31, ldo=1 << 31), dict(ld=99),
                dict(ldo=99), dict(x=A, out=A, ldo=101), dict(x=A + 2), dict(scr=None), dict(scr=A + 4), dict(n=31),
@@ -116,4 +117,4 @@ def test_tensors_that_do_not_fit_are_refused():
     with pytest.raises(ValueError):
         draft.logits_adjust(z(2, 5), z(2, 5))
     with pytest.raises(ValueError):
-        draft._state_ptr(z(4, dtype=torch.int32), torch.device("cuda", 0))
+        draft._state_ptr(z(4, dtype=torch.int32), 0)
