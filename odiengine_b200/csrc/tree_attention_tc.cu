@@ -44,6 +44,8 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "tree_attention.cuh"
 
 namespace odi_cuda {
@@ -741,42 +743,49 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       // weights, as digits, into the operand tile
       if (i && !mbar_wait(&bars.pv_done[sub], (i - 1) & 1, err, ERR_TREE_WAIT)) dead = 1;
       if (I8) {
-        const float dvs = dvv * gr.vs[h0];
-        const bool same = gr.lv_same[half];
+        // one factor for all rows as long as each has met the same largest scale (a
+        // choice made per value, by selects, took 85 instructions of 800 per block)
+        auto digits = [&](auto uniform) {
+          const float dvs = dvv * gr.vs[h0];
 #pragma unroll
-        for (int r0 = 0; r0 < NH; r0 += 16) {  // a 16-byte piece of every digit
-        uint32_t w[4][4];
+          for (int r0 = 0; r0 < NH; r0 += 16) {  // a 16-byte piece of every digit
+            uint32_t w[4][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[h0 + r0 + 4 * q]), m4 = *reinterpret_cast<const float4*>(&gr.nm[h0 + r0 + 4 * q]);
-          float2 f[2] = {f2(dvs), f2(dvs)};
-          if (!same) {
-            const float4 v4 = *reinterpret_cast<const float4*>(&gr.vs[h0 + r0 + 4 * q]);
-            f[0] = make_float2(dvv * v4.x, dvv * v4.y), f[1] = make_float2(dvv * v4.z, dvv * v4.w);
+            for (int q = 0; q < 4; ++q) {
+              const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[h0 + r0 + 4 * q]), m4 = *reinterpret_cast<const float4*>(&gr.nm[h0 + r0 + 4 * q]);
+              float2 f[2] = {f2(dvs), f2(dvs)};
+              if (!uniform) {
+                const float4 v4 = *reinterpret_cast<const float4*>(&gr.vs[h0 + r0 + 4 * q]);
+                f[0] = make_float2(dvv * v4.x, dvv * v4.y), f[1] = make_float2(dvv * v4.z, dvv * v4.w);
+              }
+              float2 hi[2], lo[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float2 x = e ? __ffma2_rn(s2[r0 / 2 + 2 * q + 1], make_float2(c4.z, c4.w), make_float2(m4.z, m4.w))
+                                   : __ffma2_rn(s2[r0 / 2 + 2 * q], make_float2(c4.x, c4.y), make_float2(m4.x, m4.y));
+                const float2 p = make_float2(ex2(x.x), ex2(x.y));
+                l2[r0 / 2 + 2 * q + e] = __fadd2_rn(l2[r0 / 2 + 2 * q + e], p);
+                const float2 y = __ffma2_rn(p, f[e], f2(0.5f));  // 0.5 .. 2^32: its integer part is the weight
+                hi[e] = __ffma2_rz(y, f2(0x1p-16f), f2(8388608.f));
+                lo[e] = __fadd2_rz(__ffma2_rn(__fadd2_rn(hi[e], f2(-8388608.f)), f2(-65536.f), y), f2(8388608.f));
+              }
+              auto u = [](float x) { return __float_as_uint(x); };
+              const uint32_t l01 = __byte_perm(u(lo[0].x), u(lo[0].y), 0x5140u), l23 = __byte_perm(u(lo[1].x), u(lo[1].y), 0x5140u);
+              const uint32_t h01 = __byte_perm(u(hi[0].x), u(hi[0].y), 0x5140u), h23 = __byte_perm(u(hi[1].x), u(hi[1].y), 0x5140u);
+              w[0][q] = __byte_perm(l01, l23, 0x5410u);
+              w[1][q] = __byte_perm(l01, l23, 0x7632u);
+              w[2][q] = __byte_perm(h01, h23, 0x5410u);
+              w[3][q] = __byte_perm(h01, h23, 0x7632u);
           }
-          float2 hi[2], lo[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 x = e ? __ffma2_rn(s2[r0 / 2 + 2 * q + 1], make_float2(c4.z, c4.w), make_float2(m4.z, m4.w))
-                               : __ffma2_rn(s2[r0 / 2 + 2 * q], make_float2(c4.x, c4.y), make_float2(m4.x, m4.y));
-            const float2 p = make_float2(ex2(x.x), ex2(x.y));
-            l2[r0 / 2 + 2 * q + e] = __fadd2_rn(l2[r0 / 2 + 2 * q + e], p);
-            const float2 y = __ffma2_rn(p, f[e], f2(0.5f));  // 0.5 .. 2^32: its integer part is the weight
-            hi[e] = __ffma2_rz(y, f2(0x1p-16f), f2(8388608.f));
-            lo[e] = __fadd2_rz(__ffma2_rn(__fadd2_rn(hi[e], f2(-8388608.f)), f2(-65536.f), y), f2(8388608.f));
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(prow + (((2 * k + (h0 + r0) / 16) ^ psw) << 4)) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
           }
-          auto u = [](float x) { return __float_as_uint(x); };
-          const uint32_t l01 = __byte_perm(u(lo[0].x), u(lo[0].y), 0x5140u), l23 = __byte_perm(u(lo[1].x), u(lo[1].y), 0x5140u);
-          const uint32_t h01 = __byte_perm(u(hi[0].x), u(hi[0].y), 0x5140u), h23 = __byte_perm(u(hi[1].x), u(hi[1].y), 0x5140u);
-          w[0][q] = __byte_perm(l01, l23, 0x5410u);
-          w[1][q] = __byte_perm(l01, l23, 0x7632u);
-          w[2][q] = __byte_perm(h01, h23, 0x5410u);
-          w[3][q] = __byte_perm(h01, h23, 0x7632u);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<uint4*>(prow + (((2 * k + (h0 + r0) / 16) ^ psw) << 4)) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
-        }
+        };
+        if (gr.lv_same[half])
+          digits(std::true_type());
+        else
+          digits(std::false_type());
       } else {
 #pragma unroll
         for (int c0 = 0; c0 < NH / 8; ++c0) {  // eight rows: one 16-byte piece of high halves, one of low
