@@ -178,17 +178,6 @@ __device__ __forceinline__ void ld_digits(uint32_t (&r)[3][32], uint32_t addr, u
       : "r"(addr), "r"(addr + 1 * stride), "r"(addr + 2 * stride)
       : "memory");
 }
-__device__ __forceinline__ void ld_digits(uint32_t (&r)[4][8], uint32_t addr, uint32_t stride) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%32];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%33];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16,%17,%18,%19,%20,%21,%22,%23}, [%34];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%24,%25,%26,%27,%28,%29,%30,%31}, [%35];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : TA_OUT8(r[0]), TA_OUT8(r[1]), TA_OUT8(r[2]), TA_OUT8(r[3])
-      : "r"(addr), "r"(addr + 1 * stride), "r"(addr + 2 * stride), "r"(addr + 3 * stride)
-      : "memory");
-}
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -207,18 +196,17 @@ __device__ __forceinline__ bool group_any(int id, int n, bool v) {
       : "memory");
   return r != 0;
 }
-// The integer sums of S start from the bits of 1.5 * 2^23, so that they are read
-// back as the fp32 value 1.5 * 2^23 + sum (|sum| < 2^22) without a conversion,
-// which runs at an eighth of an add's rate.  Two scores at a time: h * 2^16 + m *
-// 2^8 + l; m and l are joined first, to a multiple of 2^8, which is 2^-21 of a
-// product of ordinary size (2^29 and more).
+// The integer sums of S start from the bits of B = 1.5 * 2^23, so that they are
+// read back as the fp32 value B + sum (|sum| < 2^22) without a conversion, which
+// runs at an eighth of an add's rate.  Two scores at a time: h * 2^16 + m * 2^8 +
+// l; m and l are joined first, to a multiple of 2^8, which is 2^-21 of a product
+// of ordinary size (2^29 and more); what the Bs add up to leaves with h, exactly.
 constexpr uint32_t S_START = 0x4B400000u;
 __device__ __forceinline__ float2 f2(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 bits2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 __device__ __forceinline__ float2 join_digits(float2 h, float2 m, float2 l) {
   constexpr float B = 12582912.f;
-  const float2 ml = __fadd2_rn(__ffma2_rn(m, f2(256.f), l), f2(-B * 257.f));
-  return __ffma2_rn(__fadd2_rn(h, f2(-B)), f2(65536.f), ml);
+  return __fadd2_rn(__ffma2_rn(h, f2(65536.f), f2(-B * 65793.f)), __ffma2_rn(m, f2(256.f), l));
 }
 // 16 columns of this lane set to v.
 __device__ __forceinline__ void st16(uint32_t addr, uint32_t v) {
@@ -260,12 +248,14 @@ struct Bars {
 struct alignas(16) Group {
   float c[NT];           // factor of the scores, positive
   float nm[NT];          // minus the reference
+  float nx[NT];          // the same, or 0 for a row without one
   float lv[NT];          // log2 of vs
   float vs[NT];          // int8: factor of weight * scale
   float fo[NT], fl[NT];  // factors of O and of the sums when the reference moves
   float mx[4][NT], dm[4][NT];
   float lv_top[2];       // the largest lv of each half
   int lv_same[2];        // all lv of the half are equal
+  int none[2];           // some row of the half has no reference yet
 };
 
 template <bool I8, int SUBS>
@@ -384,11 +374,12 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       if (l8 == 0) {
         Group& gr = groups[sub];
         gr.c[ln] = ok ? fmaxf(fabsf(a.scale_log2) * (I8 ? 1.f / 4194304.f : 1.f / 8192.f) * pow2(ex), 1e-37f) : __int_as_float(0x7fc00000);
-        gr.nm[ln] = -TA_NONE;
+        gr.nm[ln] = ok ? -TA_NONE : 0.f;  // of a row of NaNs any will do
+        gr.nx[ln] = 0.f;
         gr.lv[ln] = I8 ? 120.f : 0.f;
         gr.vs[ln] = I8 ? TA_VMOST : 1.f;
         gr.fo[ln] = gr.fl[ln] = 1.f;
-        if (ln % NH == 0) gr.lv_top[ln / NH] = I8 ? 120.f : 0.f, gr.lv_same[ln / NH] = 1;
+        if (ln % NH == 0) gr.lv_top[ln / NH] = I8 ? 120.f : 0.f, gr.lv_same[ln / NH] = gr.none[ln / NH] = 1;
         rowt[n] = rt[i];
       }
       uint8_t* q = smem + F::Q_OFF + sub * F::QB;
@@ -551,17 +542,18 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         fence_after();
 #pragma unroll
         for (int c0 = 0; c0 < NH; c0 += 8) {
-          uint32_t r[F::DP][8];
-          ld_digits(r, o_tm + c0, NT);
+          if (I8) {  // two low digits of each row, then, 64 columns on, two high ones
+            uint32_t r[2][16];
+            ld_digits(r, o_tm + h0 + 2 * c0, 2 * NT);
 #pragma unroll
-          for (int n = 0; n < 8; ++n) {
-            float x;
-            if (I8)  // digit 0 the lowest
-              x = fmaf((float)(int)r[F::DP - 1][n], 16777216.f,
-                       fmaf((float)(int)r[F::DP - 2][n], 65536.f, fmaf((float)(int)r[1][n], 256.f, (float)(int)r[0][n])));
-            else
-              x = __uint_as_float(r[0][n]) + __uint_as_float(r[1][n]);
-            facc[c0 + n] += x;
+            for (int n = 0; n < 8; ++n)
+              facc[c0 + n] += fmaf((float)(int)r[1][2 * n + 1], 16777216.f,
+                                   fmaf((float)(int)r[1][2 * n], 65536.f, fmaf((float)(int)r[0][2 * n + 1], 256.f, (float)(int)r[0][2 * n])));
+          } else {
+            uint32_t r[2][8];
+            ld_digits(r, o_tm + c0, NT);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) facc[c0 + n] += __uint_as_float(r[0][n]) + __uint_as_float(r[1][n]);
           }
         }
         fence_before();
@@ -632,19 +624,26 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       ok = mbar_wait(&bars.s_full[sub], i & 1, err, ERR_TREE_WAIT) && ok;
       __syncwarp();
       fence_after();
-      float2 s2[NH / 2];
+      float2 x2[NH / 2];  // factor * score - reference, base 2
       // a row whose scale of K or V is not finite gives NaN to who sees it
       const float dkk = finite(dk) && finite(dv) ? dk : nan, dvv = finite(dv) ? dv : 0.f;
       {
         uint32_t r[F::DQ][NH];  // all of this thread's sums at once: one latency
         ld_digits(r, s_tm, NT);
 #pragma unroll
-        for (int n = 0; n < NH / 2; ++n) {
-          const float2 hi = bits2(r[0][2 * n], r[0][2 * n + 1]), lo = bits2(r[1][2 * n], r[1][2 * n + 1]);
-          if (I8)
-            s2[n] = __fmul2_rn(join_digits(hi, lo, bits2(r[F::DQ - 1][2 * n], r[F::DQ - 1][2 * n + 1])), f2(dkk));
-          else
-            s2[n] = __fadd2_rn(hi, lo);
+        for (int n = 0; n < NH / 2; n += 2) {
+          const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[h0 + 2 * n]), m4 = *reinterpret_cast<const float4*>(&gr.nx[h0 + 2 * n]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int a0 = 2 * (n + e), a1 = a0 + 1;
+            const float2 hi = bits2(r[0][a0], r[0][a1]), lo = bits2(r[1][a0], r[1][a1]);
+            float2 s;
+            if (I8)
+              s = __fmul2_rn(join_digits(hi, lo, bits2(r[F::DQ - 1][a0], r[F::DQ - 1][a1])), f2(dkk));
+            else
+              s = __fadd2_rn(hi, lo);
+            x2[n + e] = __ffma2_rn(s, e ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y), e ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y));
+          }
         }
       }
       if (I8) {
@@ -659,9 +658,9 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       if (edge) {
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
-          float& s = n & 1 ? s2[n / 2].y : s2[n / 2].x;
-          if (!((vis >> n) & 1u)) s = -INFINITY;
-          else if (!I8 && bad) s = nan;
+          float& x = n & 1 ? x2[n / 2].y : x2[n / 2].x;
+          if (!((vis >> n) & 1u)) x = -INFINITY;
+          else if (!I8 && bad) x = nan;
         }
       }
       // does a weight leave its range?  int8: digits hold weight * scale * vs
@@ -670,23 +669,21 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       const float ldv = I8 ? __log2f(dvv) : 0.f;
       float top = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NH; n += 4) {
-        const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[h0 + n]), m4 = *reinterpret_cast<const float4*>(&gr.nm[h0 + n]);
-        const float2 x = __ffma2_rn(s2[n / 2], make_float2(c4.x, c4.y), make_float2(m4.x, m4.y));
-        const float2 y = __ffma2_rn(s2[n / 2 + 1], make_float2(c4.z, c4.w), make_float2(m4.z, m4.w));
-        top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(y.x, y.y)));
-      }
+      for (int n = 0; n < NH / 2; ++n) top = fmaxf(top, fmaxf(x2[n].x, x2[n].y));
       if (I8) top += fmaxf(-29.f, ldv + gr.lv_top[half]);
       if (!ok) dead = 1;
       bool fresh = i == 0;
       __syncwarp();
-      if (group_any(bar, GT, top > TOP || !ok)) {
+      if (group_any(bar, GT, top > TOP || gr.none[half] || !ok)) {
         if (group_any(bar, GT, *reinterpret_cast<volatile int*>(&dead) != 0)) break;
         // Lane n (of 16 rows, and n + 16) gets the largest score of row n among the
         // warp's positions, and the largest scale of V among those that it sees.
+#pragma unroll
+        for (int n = 0; n < NH / 2; ++n)  // without the reference; the new one is added below
+          x2[n] = __fadd2_rn(x2[n], make_float2(-gr.nx[h0 + 2 * n], -gr.nx[h0 + 2 * n + 1]));
         const float mx = lane_max<NH>([&](int n) {
-          const float s = (n & 1 ? s2[n / 2].y : s2[n / 2].x) * gr.c[h0 + n];
-          return s == s ? s : -INFINITY;
+          const float x = n & 1 ? x2[n / 2].y : x2[n / 2].x;
+          return x == x ? x : -INFINITY;
         });
         float dm = 0.f;
         if (I8) {
@@ -720,7 +717,10 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
               }
             }
             gr.fo[n] = fo, gr.fl[n] = fl;
+            gr.nx[n] = gr.nm[n] == -TA_NONE ? 0.f : gr.nm[n];
           }
+          const bool none = __any_sync(0xffffffffu, lane < NH && gr.nm[h0 + lane % NH] == -TA_NONE);
+          if (lane == 0) gr.none[half] = none;
           __syncwarp();
           if (I8) {
             float hi = gr.lv[h0 + lane % NH], lo = hi;
@@ -733,6 +733,8 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           }
         }
         group_sync(bar, GT);
+#pragma unroll
+        for (int n = 0; n < NH / 2; ++n) x2[n] = __fadd2_rn(x2[n], *reinterpret_cast<const float2*>(&gr.nx[h0 + 2 * n]));
         flush(i, true);
         fresh = true;
       } else if (since >= F::PERIOD) {
@@ -748,38 +750,27 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         auto digits = [&](auto uniform) {
           const float dvs = dvv * gr.vs[h0];
 #pragma unroll
-          for (int r0 = 0; r0 < NH; r0 += 16) {  // a 16-byte piece of every digit
-            uint32_t w[4][4];
+          for (int r0 = 0; r0 < NH; r0 += 8) {  // a 16-byte piece of low digits, one of high
+            uint32_t lw[4], hw[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float4 c4 = *reinterpret_cast<const float4*>(&gr.c[h0 + r0 + 4 * q]), m4 = *reinterpret_cast<const float4*>(&gr.nm[h0 + r0 + 4 * q]);
-              float2 f[2] = {f2(dvs), f2(dvs)};
+            for (int e = 0; e < 4; ++e) {
+              const int n = r0 / 2 + e;
+              float2 f = f2(dvs);
               if (!uniform) {
-                const float4 v4 = *reinterpret_cast<const float4*>(&gr.vs[h0 + r0 + 4 * q]);
-                f[0] = make_float2(dvv * v4.x, dvv * v4.y), f[1] = make_float2(dvv * v4.z, dvv * v4.w);
+                const float2 vs = *reinterpret_cast<const float2*>(&gr.vs[h0 + 2 * n]);
+                f = make_float2(dvv * vs.x, dvv * vs.y);
               }
-              float2 hi[2], lo[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float2 x = e ? __ffma2_rn(s2[r0 / 2 + 2 * q + 1], make_float2(c4.z, c4.w), make_float2(m4.z, m4.w))
-                                   : __ffma2_rn(s2[r0 / 2 + 2 * q], make_float2(c4.x, c4.y), make_float2(m4.x, m4.y));
-                const float2 p = make_float2(ex2(x.x), ex2(x.y));
-                l2[r0 / 2 + 2 * q + e] = __fadd2_rn(l2[r0 / 2 + 2 * q + e], p);
-                const float2 y = __ffma2_rn(p, f[e], f2(0.5f));  // 0.5 .. 2^32: its integer part is the weight
-                hi[e] = __ffma2_rz(y, f2(0x1p-16f), f2(8388608.f));
-                lo[e] = __fadd2_rz(__ffma2_rn(__fadd2_rn(hi[e], f2(-8388608.f)), f2(-65536.f), y), f2(8388608.f));
-              }
-              auto u = [](float x) { return __float_as_uint(x); };
-              const uint32_t l01 = __byte_perm(u(lo[0].x), u(lo[0].y), 0x5140u), l23 = __byte_perm(u(lo[1].x), u(lo[1].y), 0x5140u);
-              const uint32_t h01 = __byte_perm(u(hi[0].x), u(hi[0].y), 0x5140u), h23 = __byte_perm(u(hi[1].x), u(hi[1].y), 0x5140u);
-              w[0][q] = __byte_perm(l01, l23, 0x5410u);
-              w[1][q] = __byte_perm(l01, l23, 0x7632u);
-              w[2][q] = __byte_perm(h01, h23, 0x5410u);
-              w[3][q] = __byte_perm(h01, h23, 0x7632u);
-          }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint4*>(prow + (((2 * k + (h0 + r0) / 16) ^ psw) << 4)) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+              const float2 p = make_float2(ex2(x2[n].x), ex2(x2[n].y));
+              l2[n] = __fadd2_rn(l2[n], p);
+              const float2 y = __ffma2_rn(p, f, f2(0.5f));  // 0.5 .. 2^32: its integer part is the weight
+              const float2 hi = __ffma2_rz(y, f2(0x1p-16f), f2(0x1p23f));
+              // y - 65536 * (hi - 2^23) + 2^23; all but the last rounding is exact
+              const float2 lo = __fadd2_rz(y, __ffma2_rn(hi, f2(-65536.f), f2(0x1p39f + 0x1p23f)));
+              lw[e] = __byte_perm(__float_as_uint(lo.x), __float_as_uint(lo.y), 0x5410u);
+              hw[e] = __byte_perm(__float_as_uint(hi.x), __float_as_uint(hi.y), 0x5410u);
+            }
+            *reinterpret_cast<uint4*>(prow + ((((h0 + r0) / 8) ^ psw) << 4)) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+            *reinterpret_cast<uint4*>(prow + (((4 + (h0 + r0) / 8) ^ psw) << 4)) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
           }
         };
         if (gr.lv_same[half])
@@ -793,8 +784,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int n = 4 * c0 + e;
-            const float2 x = __ffma2_rn(s2[n], *reinterpret_cast<const float2*>(&gr.c[h0 + 2 * n]), *reinterpret_cast<const float2*>(&gr.nm[h0 + 2 * n]));
-            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            const float2 p = make_float2(ex2(x2[n].x), ex2(x2[n].y));
             l2[n] = __fadd2_rn(l2[n], p);
             const __half2 t = __floats2half2_rn(p.x, p.y);
             const float2 d = __ffma2_rn(__half22float2(t), f2(-1.f), p);
