@@ -55,6 +55,7 @@ constexpr int HD = 128;
 constexpr int BK = 128;  // positions per block
 constexpr int NT = 32;   // rows per group
 constexpr int ERR_TREE_WAIT = 64;
+constexpr int START_BYTES = 32 * 16;
 
 template <bool I8, int SUBS_>
 struct Cfg {
@@ -66,7 +67,12 @@ struct Cfg {
   static constexpr int PB = BK * 128;                     // one 128-byte row per position
   static constexpr int Q_OFF = SLOTS * TILE;
   static constexpr int P_OFF = Q_OFF + SUBS * QB;
-  static constexpr int SMEM = P_OFF + SUBS * PB + 1024;   // + alignment slack
+  // int8: what the sums of S start from.  Copied by the tensor core's own
+  // instructions in 32-row pieces: 187 us where the softmax threads stored it
+  // (54 of their 616 instructions per block), 181 now, 206 in 128-row pieces
+  // (64 nodes over 32641 positions).
+  static constexpr int START_OFF = P_OFF + SUBS * PB;
+  static constexpr int SMEM = START_OFF + (I8 ? START_BYTES : 0) + 1024;  // + alignment slack
   static constexpr int HALVES = SUBS == 1 ? 2 : 1;        // softmax threads per position and group
   static constexpr int NH = NT / HALVES;                  // rows of a group per softmax thread
   static constexpr int GT = 128 * HALVES;                 // softmax threads of a group
@@ -90,6 +96,15 @@ struct Cfg {
 // pieces of the M side `lbo` bytes apart.
 __device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo) {
   return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// Rows of 16 bytes, groups of 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t desc_rows16(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (8ull << 16) | (8ull << 32) | (1ull << 46);
+}
+// 4 columns of tensor memory, the same 32 rows for each warp's lanes, from shared
+// memory, before the products that the same thread issues next.
+__device__ __forceinline__ void copy_rows16(uint32_t d, uint64_t src) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(d), "l"(src) : "memory");
 }
 constexpr uint32_t IDESC_M128 = 8u << 24;
 __host__ __device__ constexpr uint32_t idesc(bool i8, bool mn, int n) {
@@ -208,13 +223,6 @@ __device__ __forceinline__ float2 join_digits(float2 h, float2 m, float2 l) {
   constexpr float B = 12582912.f;
   return __fadd2_rn(__ffma2_rn(h, f2(65536.f), f2(-B * 65793.f)), __ffma2_rn(m, f2(256.f), l));
 }
-// 16 columns of this lane set to v.
-__device__ __forceinline__ void st16(uint32_t addr, uint32_t v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1,%1};" ::"r"(addr),
-               "r"(v)
-               : "memory");
-}
-__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // The lane's share of a column-wise maximum: value(n) of N columns on each of 32
 // lanes; lane n (N = 16: also n + 16) gets column n's largest.
 template <int N, typename V>
@@ -424,6 +432,8 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       }
     }
   }
+  if (I8 && tid >= 128)
+    for (int i = tid - 128; i < START_BYTES / 4; i += SUBS * GT) reinterpret_cast<uint32_t*>(smem + F::START_OFF)[i] = S_START;
   fence_proxy_async_smem();
   fence_before();
   __syncthreads();
@@ -464,11 +474,14 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     auto scores = [&](int i) {
       const int t = kseq(i), slot = t % F::SLOTS;
       wait(&bars.tfull[slot], t / F::SLOTS);
-      wait(&bars.s_free[u], i);
+      if (i) wait(&bars.s_free[u], i - 1);
       if (!ok) return;
       fence_after();
       if (elect_one()) {
         const uint64_t kd = kd0 + (uint32_t)(slot * (F::TILE >> 4));
+        if (I8)
+#pragma unroll
+          for (int k = 0; k < F::SCOLS; k += 4) copy_rows16(d0 + k, desc_rows16(smem_u32(smem + F::START_OFF)));
 #pragma unroll
         for (int k = 0; k < (I8 ? 4 : 8); ++k)  // 32 bytes of the contraction per instruction
           mma<I8>(d0, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3), qd0 + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3),
@@ -519,15 +532,6 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     for (int n = 0; n < NH; ++n) facc[n] = 0.f;
 #pragma unroll
     for (int n = 0; n < NH / 2; ++n) l2[n] = f2(0.f);
-    if (I8) {
-#pragma unroll
-      for (int k = 0; k < F::DQ; ++k)
-#pragma unroll
-        for (int n = 0; n < NH; n += 16) st16(s_tm + k * NT + n, S_START);
-      st_wait();
-    }
-    fence_before();
-    mbar_arrive(&bars.s_free[sub]);
     float dk = 0.f, dv = 0.f, dk_next = 0.f, dv_next = 0.f;
     auto request = [&](int i) {
       const int key = min((split + i * stride) * BK + kl, len - 1);
@@ -645,13 +649,6 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
             x2[n + e] = __ffma2_rn(s, e ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y), e ? make_float2(m4.z, m4.w) : make_float2(m4.x, m4.y));
           }
         }
-      }
-      if (I8) {
-#pragma unroll
-        for (int k = 0; k < F::DQ; ++k)
-#pragma unroll
-          for (int n = 0; n < NH; n += 16) st16(s_tm + k * NT + n, S_START);
-        st_wait();
       }
       fence_before();
       mbar_arrive(&bars.s_free[sub]);
