@@ -35,8 +35,14 @@
 // sums cannot overflow and fp32 sums stay short) O moves from tensor memory
 // to fp32 registers and starts again.
 //
-// The softmax bounds the kernel: about 12 instructions per score (packed fp32
-// pairs where two scores share an operation).
+// The softmax bounds the kernel: 17 instructions per score (packed fp32 pairs
+// where two scores share an operation), of which two warps per scheduler issue
+// one every 2.3 cycles.  64 nodes, 64 / 8 heads, 32641 int8 positions: 182 us,
+// where fetching the cache takes 11 and 69 GFLOP at the fp16 rate 41; without
+// any products the same loop takes 176.  Smaller shares for more warps (16 of 16
+// rows: 212 us, the work per block that does not depend on rows doubles), a vote
+// without a barrier (234 where this took 224) and scores one block ahead of the
+// weights (200) were slower.
 //
 // Every wait is bounded; a wait that gives up sets the error word, all roles
 // leave their loops, copies in flight are waited for and the tensor memory is
@@ -77,8 +83,9 @@ struct Cfg {
   static constexpr int NH = NT / HALVES;                  // rows of a group per softmax thread
   static constexpr int GT = 128 * HALVES;                 // softmax threads of a group
   static constexpr int THREADS = 128 + SUBS * GT;
-  // with two groups the launch's registers (168 a thread) are shared out anew
-  // between the first warpgroup and the softmax's
+  // with two groups the launch's registers are shared out anew between the first
+  // warpgroup and the softmax's, which holds 96 sums, 32 scores, 32 weights' sums
+  // and 32 values of O per thread
   static constexpr int REGS_LAUNCH = 168, REGS_FIRST = 40, REGS_SOFT = 232;
   static_assert(SUBS == 1 || 128 * REGS_FIRST + SUBS * GT * REGS_SOFT <= THREADS * REGS_LAUNCH, "register split");
   static constexpr int ROWS = NT * SUBS;
@@ -442,77 +449,77 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
 
   if (warp < 4) {
     if (SUBS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_FIRST));
-  if (warp == 0) {
-    // ---------------- producer ----------------
-    if (lane == 0) {
-      int t = min(seqs, F::SLOTS);
-      for (; t < seqs; ++t) {
-        if (!mbar_wait(&bars.tfree[t % F::SLOTS], ((t / F::SLOTS) & 1) ^ 1, err, ERR_TREE_WAIT)) {
-          dead = 1;
-          break;
+    if (warp == 0) {
+      // ---------------- producer ----------------
+      if (lane == 0) {
+        int t = min(seqs, F::SLOTS);
+        for (; t < seqs; ++t) {
+          if (!mbar_wait(&bars.tfree[t % F::SLOTS], ((t / F::SLOTS) & 1) ^ 1, err, ERR_TREE_WAIT)) {
+            dead = 1;
+            break;
+          }
+          request_tile(t);
         }
-        request_tile(t);
+        // every issued copy has landed before the CTA can retire
+        for (int u = t < F::SLOTS ? 0 : t - F::SLOTS; u < t; ++u)
+          mbar_wait(&bars.tfull[u % F::SLOTS], (u / F::SLOTS) & 1, err, ERR_TREE_WAIT);
       }
-      // every issued copy has landed before the CTA can retire
-      for (int u = t < F::SLOTS ? 0 : t - F::SLOTS; u < t; ++u)
-        mbar_wait(&bars.tfull[u % F::SLOTS], (u / F::SLOTS) & 1, err, ERR_TREE_WAIT);
+    } else if (warp <= SUBS) {
+      // ---------------- products ----------------
+      // The whole warp runs the loop, so that descriptors stay in uniform
+      // registers, and one elected thread issues: issued from a lane's branch,
+      // with its operands moved there one by one, an instruction took 170 cycles.
+      const int u = warp - 1;  // one warp for each group: neither waits for the other's softmax
+      const uint32_t q0 = smem_u32(smem + F::Q_OFF + u * F::QB), p0 = smem_u32(smem + F::P_OFF + u * F::PB), t0 = smem_u32(smem);
+      const uint32_t d0 = tmem + u * F::SUBCOLS;
+      const uint64_t qd0 = desc(q0, 16), pd0 = desc(p0, 16), kd0 = desc(t0, 16), vd0 = desc(t0, I8 ? 16 : F::TILE / 2);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int n) {
+        ok = ok && mbar_wait(bar, n & 1, err, ERR_TREE_WAIT);
+        ok = __all_sync(0xffffffffu, ok);
+      };
+      auto scores = [&](int i) {
+        const int t = kseq(i), slot = t % F::SLOTS;
+        wait(&bars.tfull[slot], t / F::SLOTS);
+        if (i) wait(&bars.s_free[u], i - 1);
+        if (!ok) return;
+        fence_after();
+        if (elect_one()) {
+          const uint64_t kd = kd0 + (uint32_t)(slot * (F::TILE >> 4));
+          if (I8)
+#pragma unroll
+            for (int k = 0; k < F::SCOLS; k += 4) copy_rows16(d0 + k, desc_rows16(smem_u32(smem + F::START_OFF)));
+#pragma unroll
+          for (int k = 0; k < (I8 ? 4 : 8); ++k)  // 32 bytes of the contraction per instruction
+            mma<I8>(d0, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3), qd0 + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3),
+                    idesc(I8, false, F::SCOLS), I8 || k != 0);
+          commit(&bars.s_full[u]);
+          commit(&bars.tfree[slot]);
+        }
+        __syncwarp();
+      };
+      if (nb) scores(0);
+      for (int i = 0; i < nb && ok; ++i) {
+        if (i + 1 < nb) scores(i + 1);
+        const int t = vseq(i), slot = t % F::SLOTS;
+        wait(&bars.tfull[slot], t / F::SLOTS);
+        wait(&bars.p_full[u], i);
+        if (!ok) break;
+        fence_after();
+        const uint32_t keep = *reinterpret_cast<volatile int*>(&restart[u]) == 0;
+        if (elect_one()) {
+          const uint64_t vd = vd0 + (uint32_t)(slot * (F::TILE >> 4));
+          constexpr int KS = I8 ? 4 : 8, KB = BK / KS * 128;  // bytes of 32 or 16 positions
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            mma<I8>(d0 + F::OCOL, vd + k * (KB >> 4), pd0 + k * (KB >> 4), idesc(I8, true, F::DP * NT), k ? 1u : keep);
+          commit(&bars.pv_done[u]);
+          commit(&bars.tfree[slot]);
+        }
+        __syncwarp();
+      }
+      if (!ok) dead = 1;
     }
-  } else if (warp <= SUBS) {
-    // ---------------- products ----------------
-    // The whole warp runs the loop, so that descriptors stay in uniform
-    // registers, and one elected thread issues: issued from a lane's branch,
-    // with its operands moved there one by one, an instruction took 170 cycles.
-    const int u = warp - 1;  // one warp for each group: neither waits for the other's softmax
-    const uint32_t q0 = smem_u32(smem + F::Q_OFF + u * F::QB), p0 = smem_u32(smem + F::P_OFF + u * F::PB), t0 = smem_u32(smem);
-    const uint32_t d0 = tmem + u * F::SUBCOLS;
-    const uint64_t qd0 = desc(q0, 16), pd0 = desc(p0, 16), kd0 = desc(t0, 16), vd0 = desc(t0, I8 ? 16 : F::TILE / 2);
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, int n) {
-      ok = ok && mbar_wait(bar, n & 1, err, ERR_TREE_WAIT);
-      ok = __all_sync(0xffffffffu, ok);
-    };
-    auto scores = [&](int i) {
-      const int t = kseq(i), slot = t % F::SLOTS;
-      wait(&bars.tfull[slot], t / F::SLOTS);
-      if (i) wait(&bars.s_free[u], i - 1);
-      if (!ok) return;
-      fence_after();
-      if (elect_one()) {
-        const uint64_t kd = kd0 + (uint32_t)(slot * (F::TILE >> 4));
-        if (I8)
-#pragma unroll
-          for (int k = 0; k < F::SCOLS; k += 4) copy_rows16(d0 + k, desc_rows16(smem_u32(smem + F::START_OFF)));
-#pragma unroll
-        for (int k = 0; k < (I8 ? 4 : 8); ++k)  // 32 bytes of the contraction per instruction
-          mma<I8>(d0, kd + (k >> 2) * (F::TILE / 2 >> 4) + 2 * (k & 3), qd0 + (k >> 2) * (F::DQ * NT * 128 >> 4) + 2 * (k & 3),
-                  idesc(I8, false, F::SCOLS), I8 || k != 0);
-        commit(&bars.s_full[u]);
-        commit(&bars.tfree[slot]);
-      }
-      __syncwarp();
-    };
-    if (nb) scores(0);
-    for (int i = 0; i < nb && ok; ++i) {
-      if (i + 1 < nb) scores(i + 1);
-      const int t = vseq(i), slot = t % F::SLOTS;
-      wait(&bars.tfull[slot], t / F::SLOTS);
-      wait(&bars.p_full[u], i);
-      if (!ok) break;
-      fence_after();
-      const uint32_t keep = *reinterpret_cast<volatile int*>(&restart[u]) == 0;
-      if (elect_one()) {
-        const uint64_t vd = vd0 + (uint32_t)(slot * (F::TILE >> 4));
-        constexpr int KS = I8 ? 4 : 8, KB = BK / KS * 128;  // bytes of 32 or 16 positions
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          mma<I8>(d0 + F::OCOL, vd + k * (KB >> 4), pd0 + k * (KB >> 4), idesc(I8, true, F::DP * NT), k ? 1u : keep);
-        commit(&bars.pv_done[u]);
-        commit(&bars.tfree[slot]);
-      }
-      __syncwarp();
-    }
-    if (!ok) dead = 1;
-  }
     tree_join_rest(C, nclusters);
   } else {
     // ---------------- softmax ----------------
