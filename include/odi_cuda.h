@@ -443,8 +443,8 @@ size_t odi_cuda_kv_cache_bytes(int dtype, int kv_heads, int head_dim, int ctx);
  * (head_dim weights; NULL: none), then the rotation of odi_cuda_rope_kv at
  * position pos + d_depth[t] (NULL: pos + t), its angle reduced in 64 bits.
  * The rotated q rows go to d_q_out (ld_q apart; it may be d_qkv itself with
- * the same stride), k and v to cache slot pos + t.  A slot outside the cache
- * is not written. */
+ * the same stride, and otherwise may not overlap it), k and v to cache slot
+ * pos + t.  A slot outside the cache is not written. */
 int odi_cuda_qk_rope_append(const float* d_qkv, int64_t ld_qkv, const float* d_q_norm, const float* d_k_norm,
                             float eps, float* d_q_out, int64_t ld_q, const odi_cuda_kv_cache* cache,
                             const odi_cuda_decode_state* d_state, const int32_t* d_depth, int tokens, int heads,
@@ -466,7 +466,8 @@ int odi_cuda_kv_move(const odi_cuda_kv_cache* cache, const int32_t* d_src, const
                      const odi_cuda_decode_state* d_state, void* stream);
 
 /* Attention of T = tokens nodes, node t in cache slot pos + t.  d_q: rotated
- * queries [T][heads * head_dim], rows ld_q apart; d_out [T][heads * head_dim].
+ * queries [T][heads * head_dim], rows ld_q apart; d_out [T][heads * head_dim],
+ * which may not overlap them.
  * A node sees every slot below pos, and tree slot pos + j where bit j % 32 of
  * d_mask[t * ceil(T / 32) + j / 32] is set (d_mask NULL: j <= t).  Slots
  * outside the cache are not seen, a node that sees nothing gets zeros, and
@@ -486,7 +487,8 @@ int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_ca
 /* Per row of logits, in this order, each one fp32 operation: for an id with
  * count c > 0 in the row's history, l > 0 ? l / repeat : l * repeat, then
  * - c * frequency, then - presence; + its bias; -inf where its mask bit is 0.
- * The adjusted row goes to d_out (may be d_logits; NULL: not stored) and its
+ * The adjusted row goes to d_out (may be d_logits with the same stride, and
+ * otherwise may not overlap it; NULL: not stored) and its
  * first largest id to d_tokens (NULL: not wanted): -1 when nothing is above
  * -inf, NaN never chosen.  opts NULL: no adjustment. */
 typedef struct odi_cuda_logits_opts {

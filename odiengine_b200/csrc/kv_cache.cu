@@ -336,8 +336,12 @@ int odi_cuda_qk_rope_append(const float* d_qkv, int64_t ld_qkv, const float* d_q
   const int64_t rows = heads + 2ll * v.kv_heads;
   if (ld_qkv < rows * v.hd || ld_q < (int64_t)heads * v.hd)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append: a row stride is shorter than its row");
+  if (((uintptr_t)d_qkv | (uintptr_t)d_q_out | (uintptr_t)d_q_norm | (uintptr_t)d_k_norm | (uintptr_t)d_state | (uintptr_t)d_depth) & 3)
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append: misaligned buffer");
   if ((int64_t)tokens * rows > 0x7fffffffll)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append: too many rows");
+  if ((d_q_out != d_qkv || ld_q != ld_qkv) && rows_overlap(d_qkv, ld_qkv, rows * v.hd, d_q_out, ld_q, (int64_t)heads * v.hd, tokens))
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append: d_q_out overlaps d_qkv and is not d_qkv itself");
   TurnTable tab;
   const double step = pow((double)theta, -2.0 / v.hd);
   double f = 0.15915494309189533577;  // 1 / (2 pi)
@@ -395,6 +399,8 @@ int odi_cuda_kv_move(const odi_cuda_kv_cache* cache, const int32_t* d_src, const
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_move: 0 to ODI_CUDA_KV_MOVE_MAX rows per call");
   if (!n) return ODI_CUDA_OK;
   if (!d_src || !d_dst) return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_move: null argument");
+  if (((uintptr_t)d_src | (uintptr_t)d_dst | (uintptr_t)d_state) & 3)
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_move: misaligned list");
   const int row_bytes = v.hd * (v.dtype == ODI_CUDA_KV_F16 ? 2 : 1);
   const cudaError_t e = launch_pdl(kv_move_kernel, dim3(row_bytes / 64, v.kv_heads, 2), dim3(256), (cudaStream_t)stream,
                                    v, d_src, d_dst, n, reinterpret_cast<const DecodeState*>(d_state));

@@ -224,8 +224,9 @@ int odi_cuda_logits_adjust(const float* d_logits, int64_t ld_logits, float* d_ou
   if (!d_logits || (!d_out && !d_tokens)) return bad("logits_adjust: null argument");
   if (rows < 0 || rows > 65535 || V < 1 || V > 0x7fff0000) return bad("logits_adjust: rows or vocabulary out of range");
   if (ld_logits < V || (d_out && ld_out < V)) return bad("logits_adjust: a row stride is shorter than the vocabulary");
-  if (d_out == d_logits && ld_out != ld_logits) return bad("logits_adjust: in place needs one row stride");
   if (((uintptr_t)d_logits | (uintptr_t)d_out | (uintptr_t)d_tokens) & 3) return bad("logits_adjust: misaligned buffer");
+  if (d_out && (d_out != d_logits || ld_out != ld_logits) && rows_overlap(d_logits, ld_logits, V, d_out, ld_out, V, rows))
+    return bad("logits_adjust: the output overlaps the logits and is not the logits themselves");
   if (d_tokens && (!d_scratch || ((uintptr_t)d_scratch & 7) || scratch_bytes < odi_cuda_logits_scratch_bytes(rows)))
     return bad("logits_adjust: scratch missing, misaligned or too small");
   LogitsArgs a{};
@@ -237,6 +238,9 @@ int odi_cuda_logits_adjust(const float* d_logits, int64_t ld_logits, float* d_ou
       return bad("logits_adjust: penalties must be finite and the repetition penalty positive");
     if (opts->history_max < 0 || opts->history_max > 65535 || opts->bias_count < 0 || opts->bias_count > 65535)
       return bad("logits_adjust: at most 65535 history tokens and biases");
+    if (((uintptr_t)opts->history | (uintptr_t)opts->history_len | (uintptr_t)opts->bias_ids | (uintptr_t)opts->bias |
+         (uintptr_t)opts->mask) & 3)
+      return bad("logits_adjust: misaligned list");
     if (opts->history && opts->history_ld != 0 && opts->history_ld < opts->history_max)
       return bad("logits_adjust: history stride shorter than its row");
     if (opts->bias_count && (!opts->bias_ids || !opts->bias)) return bad("logits_adjust: null biases");

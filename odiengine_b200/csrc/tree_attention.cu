@@ -575,8 +575,10 @@ int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_ca
     return bad("attention_tree: 1 to ODI_CUDA_TREE_MAX tokens, heads (at most 1024) a multiple of kv_heads");
   if (ld_q < (int64_t)heads * v.hd) return bad("attention_tree: the query stride is shorter than its row");
   if (!isfinite(scale)) return bad("attention_tree: the scale must be finite");
-  if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_mask) & 3 || ((uintptr_t)d_scratch & 15))
+  if (((uintptr_t)d_q | (uintptr_t)d_out | (uintptr_t)d_mask | (uintptr_t)d_state) & 3 || ((uintptr_t)d_scratch & 15))
     return bad("attention_tree: misaligned buffer");
+  const int64_t width = (int64_t)heads * v.hd;
+  if (rows_overlap(d_q, ld_q, width, d_out, width, width, tokens)) return bad("attention_tree: the output overlaps the queries");
   const TreePlan p = tree_plan(tokens, heads, v.kv_heads, v.hd, v.ctx);
   if (scratch_bytes < p.bytes) return bad("attention_tree: scratch too small");
   TreeArgs a{};

@@ -48,12 +48,17 @@ def test_every_operator_refuses_a_bad_cache(bad, code):
 def test_append_refusals():
     L, c = ob.lib(), ctypes.byref(cache())
 
-    def call(qkv=A, ld=768, out=B, ldq=256, st=A, T=1, H=2, theta=1e4):
-        return L.odi_cuda_qk_rope_append(qkv, ld, None, None, 1e-6, out, ldq, c, st, None, T, H, theta, None)
+    def call(qkv=A, ld=768, out=B, ldq=256, st=A, T=1, H=2, theta=1e4, qn=None, kn=None, depth=None):
+        return L.odi_cuda_qk_rope_append(qkv, ld, qn, kn, 1e-6, out, ldq, c, st, depth, T, H, theta, None)
 
     for kw in (dict(qkv=None), dict(out=None), dict(st=None), dict(T=0), dict(T=-1), dict(H=0), dict(ld=767),
-               dict(ldq=255), dict(theta=0.0), dict(theta=float("nan")), dict(T=1 << 30)):
+               dict(ldq=255), dict(theta=0.0), dict(theta=float("nan")), dict(T=1 << 30), dict(qkv=A + 2), dict(out=B + 1),
+               dict(st=A + 2), dict(qn=A + 1), dict(kn=A + 2), dict(depth=A + 3),
+               # q rows over qkv's: another stride, another column, a row further, the last row's end
+               dict(out=A, T=2), dict(out=A + 4, ldq=768, T=2), dict(out=A + 768 * 4, ldq=768, T=2),
+               dict(out=A + (768 + 767) * 4, ldq=768, T=2)):
         refused(call(**kw))
+
 
 
 def test_read_and_move_refusals():
@@ -63,8 +68,9 @@ def test_read_and_move_refusals():
         refused(L.odi_cuda_kv_read(c, *a, None))
     refused(L.odi_cuda_kv_read(c, 0, 1, A, B, 2, None), DTYPE)
     assert L.odi_cuda_kv_read(c, 64, 0, None, None, 0, None) == 0  # nothing to read
-    for a in ((A, B, -1), (A, B, draft.KV_MOVE_MAX + 1), (None, B, 1), (A, None, 1)):
+    for a in ((A, B, -1), (A, B, draft.KV_MOVE_MAX + 1), (None, B, 1), (A, None, 1), (A + 2, B, 1), (A, B + 1, 1)):
         refused(L.odi_cuda_kv_move(c, *a, None, None))
+    refused(L.odi_cuda_kv_move(c, A, B, 1, A + 2, None))
     assert L.odi_cuda_kv_move(c, None, None, 0, None, None) == 0
 
 
@@ -78,8 +84,11 @@ def test_attention_refusals():
 
     for kw in (dict(q=None), dict(out=None), dict(st=None), dict(scr=None), dict(T=0), dict(T=draft.TREE_MAX + 1),
                dict(H=5), dict(H=0), dict(H=2048, ld=1 << 20), dict(ld=767), dict(scale=float("inf")),
-               dict(scale=float("nan")), dict(n=need - 1), dict(scr=A + 4), dict(q=A + 2), dict(mask=A + 1)):
+               dict(scale=float("nan")), dict(n=need - 1), dict(scr=A + 4), dict(q=A + 2), dict(mask=A + 1), dict(st=A + 2)):
         refused(call(**kw))
+    for off, ld, T, clash in ((768, 768, 1, False), (767, 768, 1, True), (-768, 768, 1, False), (768, 768, 2, True),
+                              (1536, 768, 2, False), (768, 1536, 1, False), (768, 2304, 2, False), (768, 2303, 2, True)):
+        refused(call(out=A + 4 * off, ld=ld, T=T, n=0), word="overlap" if clash else "scratch")
     for a in ((0, 6, 2, 128, 64), (257, 6, 2, 128, 64), (4, 5, 2, 128, 64), (4, 6, 2, 80, 64), (4, 6, 2, 128, 0)):
         assert L.odi_cuda_attention_tree_scratch_bytes(*a) == 0
 
@@ -99,8 +108,17 @@ def test_logits_refusals():
                dict(repeat_penalty=0.0), dict(repeat_penalty=float("nan")), dict(frequency_penalty=float("inf")),
                dict(presence_penalty=float("nan")), dict(history=A, history_ld=3, history_max=4),
                dict(history=A, history_max=65536), dict(bias_count=-1), dict(bias_count=65536), dict(bias_count=1),
-               dict(bias_count=1, bias_ids=A), dict(mask=A, mask_ld=3)):
+               dict(bias_count=1, bias_ids=A), dict(mask=A, mask_ld=3), dict(history=A + 1, history_max=1), dict(mask=A + 2, mask_ld=4),
+               dict(history_len=A + 2), dict(bias_count=1, bias_ids=A + 2, bias=A), dict(bias_count=1, bias_ids=A, bias=A + 3)):
         refused(call(**kw))
+    # rows of 100: an output over the logits is refused, one beside them or in the
+    # gaps of their stride is not (the missing scratch is, after it)
+    for off, ldo, ld, rows, clash in ((0, 101, 100, 2, True), (1, 100, 100, 1, True), (99, 100, 100, 1, True),
+                                      (100, 100, 100, 1, False), (100, 100, 100, 2, True), (200, 100, 100, 2, False),
+                                      (100, 200, 200, 5, False), (101, 200, 200, 5, True), (99, 200, 200, 5, True),
+                                      (-100, 200, 200, 5, False), (-99, 200, 200, 5, True), (150, 250, 250, 9, False),
+                                      (100, 400, 200, 3, False), (100, 350, 200, 3, True), (0, 100, 100, 2, False)):
+        refused(call(ld=ld, out=A + 4 * off, ldo=ldo, rows=rows, scr=None), word="overlap" if clash else "scratch")
     assert L.odi_cuda_logits_scratch_bytes(0) == 0 and L.odi_cuda_logits_scratch_bytes(3) == 48
 
 
