@@ -286,7 +286,8 @@ class DraftVerifier:
         if not 1 <= max_nodes <= TREE_MAX:
             raise ValueError(f"max_nodes: 1 to {TREE_MAX}")
         self.cfg, self.w = cfg, weights
-        self.device = dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        dev = torch.device("cuda" if device is None else device)
+        self.device = dev = torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev
         self.max_nodes, self.history = max_nodes, history
         self.q_norms, self.k_norms, self.norm_eps = q_norms, k_norms, norm_eps
         self.caches = [KVCache.new(cache, cfg.kv_heads, cfg.head_dim, cfg.ctx, dev) for _ in range(cfg.layers)]
@@ -386,6 +387,9 @@ class DraftVerifier:
             raise ValueError(f"verify: at most {self.max_nodes - 1} drafted tokens, each after its parent")
         if any(not 0 <= t < self.cfg.vocab for t in drafted):
             raise ValueError("verify: drafted token outside the vocabulary")
+        if not self.history and adjust.get("history") is None and (
+                adjust.get("repeat_penalty", 1.0), adjust.get("frequency_penalty", 0.0), adjust.get("presence_penalty", 0.0)) != (1.0, 0.0, 0.0):
+            raise ValueError("verify: penalties count a history (DraftVerifier(history=...))")
         if self.pos + T > self.cfg.ctx:
             raise ValueError("verification would run past the context")
         nodes = [self.pending, *drafted]

@@ -126,6 +126,38 @@ def test_matches_the_decode_step(cuda_lib):
         assert a == b
 
 
+@pytest.mark.parametrize("cache", ["f16", "i8"])
+def test_steps_of_256_nodes(cuda_lib, cache):
+    """A prompt taken 256 tokens at a time, and a chain of 255 drafts, give what
+    steps of 7 nodes give, within the roundings of the products' paths."""
+    import dataclasses
+
+    from odiengine_b200.decode import seeded_model
+    from odiengine_b200.draft import DraftVerifier
+
+    cfg = dataclasses.replace(_tiny(1), ctx=640)
+    mw = seeded_model(cfg, seed=7, interleave_gate_up=False)
+    rng = np.random.default_rng(4)
+    prompt = [int(t) for t in rng.integers(0, cfg.vocab, 301)]
+    wide, narrow = DraftVerifier(cfg, mw, cache=cache, max_nodes=256), DraftVerifier(cfg, mw, cache=cache, max_nodes=7)
+    out = []
+    for v in (wide, narrow):
+        v.start(prompt)
+        assert v.pos == 300
+        out.append(v.verify())
+    a, b = (v.logits[0].cpu().numpy() for v in (wide, narrow))
+    assert np.abs(a - b).max() <= (4e-3 if cache == "f16" else 6e-2) * np.abs(b).max()
+    drafted = [int(t) for t in rng.integers(0, cfg.vocab, 255)]
+    wide.start(prompt)
+    got = wide.verify(drafted)
+    assert got[:1] == out[0] and wide.status() == 0
+    a = wide.logits[200].cpu().numpy()  # the node after prompt + 200 drafts
+    narrow.start(prompt + drafted[:200])
+    narrow.verify()
+    b = narrow.logits[0].cpu().numpy()
+    assert np.abs(a - b).max() <= (4e-3 if cache == "f16" else 6e-2) * np.abs(b).max()
+
+
 def test_penalties_masks_and_refusals(cuda_lib):
     import torch
 
@@ -165,6 +197,10 @@ def test_penalties_masks_and_refusals(cuda_lib):
     assert len(v.verify()) == 1  # the context's last slot
     with pytest.raises(ValueError):
         v.verify()
+    plain = DraftVerifier(cfg, mw, device="cuda")
+    plain.start([5, 17, 999])
+    with pytest.raises(ValueError):  # nothing that it could count
+        plain.verify(repeat_penalty=1.5)
     from odiengine_b200.decode import seeded_model
     with pytest.raises(ValueError):
         DraftVerifier(cfg, seeded_model(cfg, interleave_gate_up=True))
