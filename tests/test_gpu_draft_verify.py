@@ -6,6 +6,8 @@ Tolerances are those of the decode step's tests, of the logits' scale: 2e-3
 with fp32 activations and an fp16 cache; 6e-2 with Q8 activations or an int8
 cache (a code is off by half a step, 1/254 of its row's largest value, as an
 activation's is)."""
+import dataclasses
+
 import numpy as np
 import pytest
 
@@ -15,10 +17,10 @@ from test_gpu_decode import _oracle_weights, _tiny
 pytestmark = pytest.mark.gpu
 
 
-def model(act_mode, seed=7):
+def model(act_mode, seed=7, head_dim=64):
     from odiengine_b200.decode import seeded_model
 
-    cfg = _tiny(act_mode)
+    cfg = dataclasses.replace(_tiny(act_mode), head_dim=head_dim)
     return cfg, seeded_model(cfg, seed=seed, interleave_gate_up=False)
 
 
@@ -36,10 +38,11 @@ def oracle_rows(ref, prefix, tokens, parents):
 
 
 @pytest.mark.parametrize("act_mode,cache,tol", [(1, "f16", 2e-3), (1, "i8", 6e-2), (0, "f16", 6e-2), (0, "i8", 6e-2)])
-def test_tree_logits_match_oracle(cuda_lib, act_mode, cache, tol):
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_tree_logits_match_oracle(cuda_lib, act_mode, cache, tol, head_dim):
     from odiengine_b200.draft import DraftVerifier
 
-    cfg, mw = model(act_mode)
+    cfg, mw = model(act_mode, head_dim=head_dim)
     ref = LlamaRef(cfg, _oracle_weights(cuda_lib, cfg, mw))
     v = DraftVerifier(cfg, mw, cache=cache, max_nodes=12)
     prompt = [5, 17, 999, 3, 250, 8, 41, 700, 2, 90, 33, 61, 7, 500, 123]  # two chunks of the cache's rows
@@ -61,15 +64,15 @@ def test_tree_logits_match_oracle(cuda_lib, act_mode, cache, tol):
             assert (a[:, :len(prompt) - 1] == c.k[:, :len(prompt) - 1]).all()
 
 
-@pytest.mark.parametrize("cache", ["f16", "i8"])
-def test_drafts_do_not_change_what_is_generated(cuda_lib, cache):
+@pytest.mark.parametrize("cache,head_dim", [("f16", 64), ("i8", 64), ("f16", 128), ("i8", 128)])
+def test_drafts_do_not_change_what_is_generated(cuda_lib, cache, head_dim):
     """Good drafts, bad drafts, branches with the right token behind wrong
     ones: every call returns the tokens of undrafted greedy decoding, more at
     a time when the drafts were right; rows of the accepted path end up where
     undrafted decoding has them."""
     from odiengine_b200.draft import DraftVerifier, kv_read
 
-    cfg, mw = model(1)
+    cfg, mw = model(1, head_dim=head_dim)
     prompt = [5, 17, 999, 3, 250]
     plain = DraftVerifier(cfg, mw, cache=cache)
     plain.start(prompt)
@@ -126,16 +129,14 @@ def test_matches_the_decode_step(cuda_lib):
         assert a == b
 
 
-@pytest.mark.parametrize("cache", ["f16", "i8"])
-def test_steps_of_256_nodes(cuda_lib, cache):
+@pytest.mark.parametrize("cache,head_dim", [("f16", 64), ("i8", 64), ("f16", 128), ("i8", 128)])
+def test_steps_of_256_nodes(cuda_lib, cache, head_dim):
     """A prompt taken 256 tokens at a time, and a chain of 255 drafts, give what
     steps of 7 nodes give, within the roundings of the products' paths."""
-    import dataclasses
-
     from odiengine_b200.decode import seeded_model
     from odiengine_b200.draft import DraftVerifier
 
-    cfg = dataclasses.replace(_tiny(1), ctx=640)
+    cfg = dataclasses.replace(_tiny(1), ctx=640, head_dim=head_dim)
     mw = seeded_model(cfg, seed=7, interleave_gate_up=False)
     rng = np.random.default_rng(4)
     prompt = [int(t) for t in rng.integers(0, cfg.vocab, 301)]
