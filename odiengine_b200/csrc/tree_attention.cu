@@ -514,13 +514,20 @@ TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   TreePlan p;
   const int64_t R = (int64_t)tokens * (heads / kv_heads);
   p.tc = hd == 128 && R > TA_TC_ROWS;
-  // 64 rows per CTA: 1.39 us per block of 128 positions, 32 rows 0.98
-  p.rows = p.tc ? (R <= 32 ? 32 : 64) : R <= 8 ? 8 : R <= 16 ? 16 : 32;
+  const int64_t block = p.tc ? 128 : TA_GROUP * TA_WARPS;
+  p.most = ((int64_t)ctx + block - 1) / block;
+  // A CTA of 32 rows takes 0.98 us per block of 128 positions, one of 64 rows
+  // 1.39 and about 3.4 more to start and to join.  32 / 8 heads, us with 32 and
+  // with 64 rows: 52 rows per kv head over 4000 positions 14.6 and 17.3, 16000
+  // 26.1 and 25.7, 32000 41.8 and 37.8; 256 rows over 500 12.4 and 15.0, 2000
+  // 18.2 and 19.7, 4000 24.8 and 23.4, 32000 126 and 88; 96 rows over 32000 (three
+  // tiles against two) 52.6 and 55.6.
+  const int64_t t32 = (R + 31) / 32, t64 = (R + 63) / 64;
+  const bool narrow = kv_heads * p.most * (98 * t32 - 139 * t64) < 340 * TA_SMS;
+  p.rows = p.tc ? (narrow ? 32 : 64) : R <= 8 ? 8 : R <= 16 ? 16 : 32;
   p.room = TA_SMS * (p.tc ? 1 : p.rows == 8 ? 4 : p.rows == 16 ? 3 : 2);
   p.tiles = (int)((R + p.rows - 1) / p.rows);
   p.units = kv_heads * p.tiles;
-  const int64_t block = p.tc ? 128 : TA_GROUP * TA_WARPS;
-  p.most = ((int64_t)ctx + block - 1) / block;
   // The scratch is laid out alike whatever the number of tokens, so that calls
   // of any T may share one: counters and shares are used only by units split
   // over several clusters, whose CTAs are all resident -- at most 4 per SM of 8

@@ -404,6 +404,13 @@ ATT = [  # hd, heads, kv_heads, T, pos, ctx
     (128, 4, 4, 3, 2500, 2600),
     (128, 40, 8, 7, 4090, 4200),
     (64, 40, 8, 31, 1023, 1100),
+    (128, 32, 8, 13, 4001, 8192),
+    # so much work that a CTA takes 64 rows
+    (128, 8, 1, 200, 333, 5000),
+    (128, 16, 2, 64, 1200, 7300),
+    (128, 64, 8, 64, 1500, 2000),
+    (128, 40, 1, 256, 0, 700),
+    (128, 33, 1, 129, 77, 1600),
 ]
 
 
@@ -414,9 +421,9 @@ def test_attention(dr, dt, hd, H, KV, T, pos, ctx):
 
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
-@pytest.mark.parametrize("T,pos", [(1, 5), (9, 0), (70, 200)])
-def test_attention_chain_without_a_mask(dr, dt, T, pos):
-    check_attention(dr, dt, 128, 8, 2, T, pos, 300, None)
+@pytest.mark.parametrize("T,pos,H,ctx", [(1, 5, 8, 300), (9, 0, 8, 300), (70, 200, 8, 300), (70, 200, 64, 2000)])
+def test_attention_chain_without_a_mask(dr, dt, T, pos, H, ctx):
+    check_attention(dr, dt, 128, H, 2, T, pos, ctx, None)
 
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
@@ -427,8 +434,9 @@ def test_attention_nodes_that_see_nothing(dr, dt):
         v[::3] = False
         return v
 
-    out = check_attention(dr, dt, 128, 8, 4, 20, 0, 64, some)
-    assert not out[::3].any()
+    for H, KV, ctx in ((8, 4, 64), (64, 1, 6000)):  # 32 and 64 rows per CTA
+        out = check_attention(dr, dt, 128, H, KV, 20, 0, ctx, some)
+        assert not out[::3].any()
 
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
@@ -441,14 +449,22 @@ def test_attention_slots_outside_the_cache(dr, dt, pos, ctx, T):
 
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
+@pytest.mark.parametrize("pos", [-20, -100, 2890, 2900, 5000])
+def test_attention_many_rows_outside_the_cache(dr, dt, pos):
+    """The same with 64 rows per CTA."""
+    check_attention(dr, dt, 128, 64, 1, 40, pos, 2900, lambda rng, t: np.ones((t, t), bool))
+
+
+@pytest.mark.parametrize("dt", ["f16", "i8"])
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-def test_attention_nonfinite_nodes_stay_with_who_sees_them(dr, dt, bad):
+@pytest.mark.parametrize("H,KV,ctx", [(8, 2, 256), (64, 1, 4900)])  # 32 and 64 rows per CTA
+def test_attention_nonfinite_nodes_stay_with_who_sees_them(dr, dt, bad, H, KV, ctx):
     """K and V of one tree slot are not finite: nodes that do not see it get
     what they get without it; nodes that see it get NaN."""
     import torch
 
     rng = np.random.default_rng(3)
-    hd, H, KV, T, pos, ctx, j = 128, 8, 2, 24, 150, 256, 4
+    hd, T, pos, j = 128, 24, 150, 4
     c = dr.KVCache.new(dt, KV, hd, ctx)
     fill(c, rng, 0, pos + T)
     q = dev((1.5 * rng.standard_normal((T, H * hd))).astype(np.float32))
@@ -472,13 +488,14 @@ def test_attention_nonfinite_nodes_stay_with_who_sees_them(dr, dt, bad):
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
 @pytest.mark.parametrize("qstd", [0.0, 1e-6, 40.0, 1e4])
-def test_attention_query_sizes(dr, dt, qstd):
+@pytest.mark.parametrize("H,KV,T,ctx", [(8, 2, 6, 800), (256, 1, 9, 3400)])  # 32 and 64 rows per CTA
+def test_attention_query_sizes(dr, dt, qstd, H, KV, T, ctx):
     """Equal scores, tiny ones, and scores of which one key takes all (the
     softmax tolerance then scales with S)."""
     import torch
 
     rng = np.random.default_rng(11)
-    hd, H, KV, T, pos, ctx = 128, 8, 2, 6, 700, 800
+    hd, pos = 128, 700
     c = dr.KVCache.new(dt, KV, hd, ctx)
     fill(c, rng, 0, pos + T, garbage=np.nan)
     q = (qstd * rng.standard_normal((T, H, hd))).astype(np.float32)
@@ -492,12 +509,12 @@ def test_attention_query_sizes(dr, dt, qstd):
 
 
 @pytest.mark.parametrize("dt", ["f16", "i8"])
-@pytest.mark.parametrize("hd,T", [(64, 9), (128, 1), (128, 9)])
+@pytest.mark.parametrize("hd,T,H,KV,ctx", [(64, 9, 8, 2, 256), (128, 1, 8, 2, 256), (128, 9, 8, 2, 256), (128, 9, 256, 1, 3400)])
 @pytest.mark.parametrize("scale", [0.0, -0.09, 1e-30])
-def test_attention_any_scale(dr, dt, hd, T, scale):
+def test_attention_any_scale(dr, dt, hd, T, scale, H, KV, ctx):
     """Zero (the mean of what is seen), negative and tiny scales, with nodes masked."""
     rng = np.random.default_rng(13)
-    H, KV, pos, ctx = 8, 2, 200, 256
+    pos = 200
     c = dr.KVCache.new(dt, KV, hd, ctx)
     fill(c, rng, 0, pos + T, garbage=np.nan)
     q = (1.5 * rng.standard_normal((T, H, hd))).astype(np.float32)
