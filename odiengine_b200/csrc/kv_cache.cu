@@ -25,28 +25,32 @@ __device__ __forceinline__ float warp_sum_all(float v) {
   return v;
 }
 
-// Rotations per position, theta^(-2i/hd) / (2 pi), in 64 bits: the angle of a
-// far position is a large number of turns, and only its fraction matters.
-// pos * turns is rounded to 2^-53 of itself and the whole turns dropped
-// before the value becomes fp32, so the angle is good to 2^-24 of a turn at
-// every position (in fp32 it is off by 6e-3 rad at position 100,000).  Made
-// on the host, one pow and head_dim / 2 products per call.
-struct TurnTable {
-  double turns[64];
+// Turns per position of pair i, r^i / (2 pi) with r = theta^(-2/hd), in 64 bits:
+// the angle of a far position is a large number of turns, and only its fraction
+// matters.  The product is good to about 2^-50 of itself and the whole turns
+// are dropped before it becomes fp32, so the angle is good to 2^-24 of a turn up
+// to position 2^27 (in fp32 it is off by 6e-3 rad at position 100,000).  A lane
+// makes its pair's power from the squares of r, five products by its own bits: a
+// table of all pairs as a kernel argument, of which every lane reads another
+// entry, serialises in the constant cache (512 tokens of 64/8 heads out of L2:
+// 9.6 us, 6.7 this way).
+struct Turns {
+  double r;          // from one pair to the next
+  double square[5];  // PPL pairs on, twice as many, ...
 };
 
 // One warp takes NH consecutive heads of one token (of the token's heads + 2
 // kv_heads rows of q, k and v), all loaded before the first is used.  Lane l
 // holds pairs l * PPL .. + PPL - 1 and their partners head_dim / 2 higher, so
 // its angles serve all its heads.  Bound by HBM for many tokens -- 512 tokens
-// of 64/8 heads read and write 39.8 MB in 11.2 us, 3.6 TB/s -- and by latency
-// for few: one token of 32/8 heads takes 4.3 us.
+// of 64/8 heads read and write 39.8 MB in 8.8 us, 4.5 TB/s -- and by latency for few: one
+// token of 32/8 heads takes 4 us.
 template <int HD, int NH, bool VEC>
 __global__ void __launch_bounds__(128) append_kernel(const float* qkv, int64_t ld, const float* __restrict__ q_norm,
                                                      const float* __restrict__ k_norm, float eps, float* q_out,
                                                      int64_t ld_q, KvView cache, const DecodeState* st,
                                                      const int* __restrict__ depth, int tokens, int heads,
-                                                     const __grid_constant__ TurnTable tab) {
+                                                     const __grid_constant__ Turns turns) {
   constexpr int PPL = HD / 64, HALF = HD / 2;
   pdl_launch_dependents();
   pdl_wait();
@@ -74,10 +78,13 @@ __global__ void __launch_bounds__(128) append_kernel(const float* qkv, int64_t l
   const int64_t slot = (int64_t)pos + t;
   const bool store = slot >= 0 && slot < cache.ctx;
   const double p = (double)((int64_t)pos + (depth ? __ldcg(depth + t) : t));
+  double x = p * 0.15915494309189533577;  // 1 / (2 pi)
+#pragma unroll
+  for (int k = 0; k < 5; ++k) x *= (lane >> k) & 1 ? turns.square[k] : 1.0;
   float sn[PPL], cs[PPL];
 #pragma unroll
   for (int e = 0; e < PPL; ++e) {
-    const double x = p * tab.turns[lane * PPL + e];
+    if (e) x *= turns.r;
     sincospif(2.0f * (float)(x - rint(x)), &sn[e], &cs[e]);
   }
 #pragma unroll
@@ -268,13 +275,13 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvView cache, const int* _
 template <int HD, int NH>
 cudaError_t launch_append(bool vec, const float* qkv, int64_t ld, const float* qn, const float* kn, float eps,
                           float* q_out, int64_t ld_q, const KvView& c, const DecodeState* st, const int* depth,
-                          int tokens, int heads, const TurnTable& tab, cudaStream_t s) {
+                          int tokens, int heads, const Turns& turns, cudaStream_t s) {
   const int groups = (heads + 2 * c.kv_heads + NH - 1) / NH;
   const dim3 grid((unsigned)(((int64_t)tokens * groups + 3) / 4));
   return vec ? launch_pdl(append_kernel<HD, NH, true>, grid, dim3(128), s, qkv, ld, qn, kn, eps, q_out, ld_q, c, st,
-                          depth, tokens, heads, tab)
+                          depth, tokens, heads, turns)
              : launch_pdl(append_kernel<HD, NH, false>, grid, dim3(128), s, qkv, ld, qn, kn, eps, q_out, ld_q, c, st,
-                          depth, tokens, heads, tab);
+                          depth, tokens, heads, turns);
 }
 
 }  // namespace
@@ -342,11 +349,10 @@ int odi_cuda_qk_rope_append(const float* d_qkv, int64_t ld_qkv, const float* d_q
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append: too many rows");
   if ((d_q_out != d_qkv || ld_q != ld_qkv) && rows_overlap(d_qkv, ld_qkv, rows * v.hd, d_q_out, ld_q, (int64_t)heads * v.hd, tokens))
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append: d_q_out overlaps d_qkv and is not d_qkv itself");
-  TurnTable tab;
-  const double step = pow((double)theta, -2.0 / v.hd);
-  double f = 0.15915494309189533577;  // 1 / (2 pi)
-  for (int i = 0; i < v.hd / 2; ++i, f *= step) tab.turns[i] = f;
-  for (int i = v.hd / 2; i < 64; ++i) tab.turns[i] = 0.0;
+  Turns turns;
+  turns.r = pow((double)theta, -2.0 / v.hd);
+  double sq = v.hd == 128 ? turns.r * turns.r : turns.r;
+  for (int k = 0; k < 5; ++k, sq *= sq) turns.square[k] = sq;
   // 8-byte accesses where both buffers and strides allow them
   const bool vec = !(((uintptr_t)d_qkv | (uintptr_t)d_q_out) & 7) && !((ld_qkv | ld_q) & 1);
   const DecodeState* st = reinterpret_cast<const DecodeState*>(d_state);
@@ -357,14 +363,14 @@ int odi_cuda_qk_rope_append(const float* d_qkv, int64_t ld_qkv, const float* d_q
   cudaError_t e;
   if (v.hd == 128)
     e = many ? launch_append<128, 4>(vec, d_qkv, ld_qkv, d_q_norm, d_k_norm, eps, d_q_out, ld_q, v, st, d_depth,
-                                     tokens, heads, tab, s)
+                                     tokens, heads, turns, s)
              : launch_append<128, 1>(vec, d_qkv, ld_qkv, d_q_norm, d_k_norm, eps, d_q_out, ld_q, v, st, d_depth,
-                                     tokens, heads, tab, s);
+                                     tokens, heads, turns, s);
   else
     e = many ? launch_append<64, 4>(vec, d_qkv, ld_qkv, d_q_norm, d_k_norm, eps, d_q_out, ld_q, v, st, d_depth,
-                                    tokens, heads, tab, s)
+                                    tokens, heads, turns, s)
              : launch_append<64, 1>(vec, d_qkv, ld_qkv, d_q_norm, d_k_norm, eps, d_q_out, ld_q, v, st, d_depth,
-                                    tokens, heads, tab, s);
+                                    tokens, heads, turns, s);
   return kv_launched(e, "qk_rope_append");
 }
 
