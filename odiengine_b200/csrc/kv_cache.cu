@@ -43,8 +43,8 @@ struct Turns {
 // kv_heads rows of q, k and v), all loaded before the first is used.  Lane l
 // holds pairs l * PPL .. + PPL - 1 and their partners head_dim / 2 higher, so
 // its angles serve all its heads.  Bound by HBM for many tokens -- 512 tokens
-// of 64/8 heads read and write 39.8 MB in 8.8 us, 4.5 TB/s -- and by latency for few: one
-// token of 32/8 heads takes 4 us.
+// of 64/8 heads read and write 39.8 MB in 8.8 us, 4.5 TB/s -- and by latency for
+// few: one token of 32/8 heads takes 3.3 us.
 template <int HD, int NH, bool VEC>
 __global__ void __launch_bounds__(128) append_kernel(const float* qkv, int64_t ld, const float* __restrict__ q_norm,
                                                      const float* __restrict__ k_norm, float eps, float* q_out,
@@ -159,63 +159,67 @@ __global__ void __launch_bounds__(128) append_kernel(const float* qkv, int64_t l
 }
 
 // Rows start .. start + count of K (blockIdx.z = 0) and V (1) as fp16 or
-// fp32, [kv_head][count][hd].  A thread converts four 16-value chunks, one
-// block apart, loaded together.  HBM bound: 32001 int8 positions of 8 heads to
-// fp16 are 199 MB in 38 us, 5.2 TB/s, three quarters of them writes; 77
-// positions take 3.8 us.
+// fp32, [kv_head][count][hd].  A thread makes one 16-byte piece of the output at
+// a time, two 256 pieces apart, so that a warp's stores are whole lines.  HBM
+// bound: 32001 int8 positions of 8 heads to fp16 are 199 MB in 31.1 us, 6.4
+// TB/s, three quarters of them writes (37.7 with 32 bytes per thread in two
+// stores; 38.7, 31.9 and 31.2 with one, two and four pieces and stores that are
+// not marked as streaming).  77 positions take 1.3 us.
+constexpr int READ_U = 2;
 template <bool I8, bool OUT16>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvView cache, int start, int count, void* k_out, void* v_out) {
-  constexpr int U = 4;
+  constexpr int U = READ_U, CH = OUT16 ? 8 : 4;  // pieces per thread, values per piece
   pdl_launch_dependents();
   pdl_wait();
   void* out = blockIdx.z ? v_out : k_out;
   if (!out) return;
   const uint8_t* base = static_cast<const uint8_t*>(blockIdx.z ? cache.v : cache.k);
-  const int cpr = cache.hd / 16;  // chunks per row: 4 or 8
-  const int64_t total = (int64_t)count * cpr;
+  const int shift = (cache.hd == 128 ? 7 : 6) - (OUT16 ? 3 : 2);  // pieces per row, log2
+  const int64_t total = (int64_t)count << shift;
   const int h = blockIdx.y;
   const int64_t row0 = (int64_t)h * cache.ctx + start;
   const int64_t i0 = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
-  uint4 raw[U][I8 ? 1 : 2];
+  uint32_t raw[U][I8 ? CH / 4 : CH / 2];
   float d[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t i = i0 + u * 256;
     if (i >= total) break;
-    const uint4* p = reinterpret_cast<const uint4*>(base + (row0 * cpr + i) * (I8 ? 16 : 32));
-    raw[u][0] = __ldcs(p);
-    if (!I8) raw[u][I8 ? 0 : 1] = __ldcs(p + 1);
-    if (I8) d[u] = __ldcg(reinterpret_cast<const float*>(base + cache.scale_off) + row0 + i / cpr);
+    const uint8_t* p = base + ((row0 << shift) + i) * (CH * (I8 ? 1 : 2));
+    if constexpr (sizeof raw[u] == 16) {
+      const uint4 x = __ldcs(reinterpret_cast<const uint4*>(p));
+      raw[u][0] = x.x, raw[u][1] = x.y, raw[u][2] = x.z, raw[u][3] = x.w;
+    } else if constexpr (sizeof raw[u] == 8) {
+      const uint2 x = __ldcs(reinterpret_cast<const uint2*>(p));
+      raw[u][0] = x.x, raw[u][1] = x.y;
+    } else {
+      raw[u][0] = __ldcs(reinterpret_cast<const unsigned*>(p));
+    }
+    if (I8) d[u] = __ldcg(reinterpret_cast<const float*>(base + cache.scale_off) + row0 + (i >> shift));
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t i = i0 + u * 256;
     if (i >= total) break;
-    float x[16];
+    float x[CH];
     if (I8) {
-      const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = (float)(int8_t)(w[e / 4] >> (8 * (e % 4))) * d[u];
+      for (int e = 0; e < CH; ++e) x[e] = (float)(int8_t)(raw[u][e / 4] >> (8 * (e % 4))) * d[u];
     } else {
-      const __half2* w = reinterpret_cast<const __half2*>(raw[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 f = __half22float2(w[e]);
+      for (int e = 0; e < CH / 2; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw[u][e]));
         x[2 * e] = f.x, x[2 * e + 1] = f.y;
       }
     }
-    const int64_t o = ((int64_t)h * total + i) * 16;
-    if (OUT16) {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(out) + o);
-      __half2 y[8];
+    uint4* dst = reinterpret_cast<uint4*>(out) + h * total + i;
+    if constexpr (OUT16) {
+      __half2 y[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-      dst[0] = reinterpret_cast<uint4*>(y)[0];
-      dst[1] = reinterpret_cast<uint4*>(y)[1];
+      for (int e = 0; e < 4; ++e) y[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+      __stcs(dst, *reinterpret_cast<uint4*>(y));
     } else {
-      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + o);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+      __stcs(reinterpret_cast<float4*>(dst), make_float4(x[0], x[1], x[2], x[3]));
     }
   }
 }
@@ -386,9 +390,9 @@ int odi_cuda_kv_read(const odi_cuda_kv_cache* cache, int start, int count, void*
   if (!d_k_out && !d_v_out) return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_read: no output");
   if (((uintptr_t)d_k_out | (uintptr_t)d_v_out) & 15)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_read: outputs must be 16-byte aligned");
-  const int64_t chunks = (int64_t)count * (v.hd / 16);
-  const dim3 grid((unsigned)((chunks + 1023) / 1024), v.kv_heads, 2);
   const bool i8 = v.dtype == ODI_CUDA_KV_I8, o16 = out_dtype == ODI_CUDA_KV_OUT_F16;
+  const int64_t pieces = (int64_t)count * (v.hd / (o16 ? 8 : 4));
+  const dim3 grid((unsigned)((pieces + 256 * READ_U - 1) / (256 * READ_U)), v.kv_heads, 2);
   cudaStream_t s = (cudaStream_t)stream;
   const cudaError_t e = i8 ? (o16 ? launch_pdl(kv_read_kernel<true, true>, grid, dim3(256), s, v, start, count, d_k_out, d_v_out)
                                   : launch_pdl(kv_read_kernel<true, false>, grid, dim3(256), s, v, start, count, d_k_out, d_v_out))
