@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvView cache, int start, i
 // independently, so a CTA takes 64 bytes of every listed row: it loads them
 // all, waits, then stores, which is what makes overlapping lists safe.  With
 // n <= 256 rows a thread holds at most four 16-byte pieces.  Latency bound: 5
-// rows of 8 heads 4.5 us, 100 rows of 32 heads 6.9.
+// rows of 8 heads 2.3 us in a graph, 100 rows of 32 heads 6.9.
 __global__ void __launch_bounds__(256) kv_move_kernel(KvView cache, const int* __restrict__ src,
                                                       const int* __restrict__ dst, int n, const DecodeState* st) {
   __shared__ int s_src[ODI_CUDA_KV_MOVE_MAX], s_dst[ODI_CUDA_KV_MOVE_MAX];

@@ -30,9 +30,9 @@ namespace {
 // inverted id, so equal values keep the lowest id and the order in which CTAs
 // arrive does not matter.  The row's last CTA writes the token and zeroes the
 // row's scratch for the next call.  64 rows of 128259 ids, 67 MB read and
-// written: 24 us, 2.8 TB/s (10.3 at the copy peak); the lists' pass through
-// shared memory and the comparisons of each CTA are not hidden by its
-// neighbours' loads.  One row of 32000: 5.7 us, latency.
+// written, 1000 history ids and 300 biases each: 21 to 24 us (10.3 at the copy
+// peak), 11.1 without lists; a CTA's pass over the lists and its barriers are not
+// hidden by its neighbours' loads.  One row of 32000: 3.9 us, latency.
 constexpr int THREADS = 256;
 
 struct LogitsArgs {

@@ -49,8 +49,8 @@ namespace {
 // up to 2^16 and down to 2^-24.
 //
 // Bound by the fetch of the cache for long ones: one token, 64 / 8 heads, 131001
-// int8 positions 62 us, 277 MB at 4.5 TB/s (the copy peak gives 42); 518 fp16
-// positions of 32 / 32 heads take 10 us, of which the fetch is 1.3: latency of
+// int8 positions 59 us, 277 MB at 4.7 TB/s (the copy peak gives 42); 518 fp16
+// positions of 32 / 32 heads take 9.3 us, of which the fetch is 1.3: latency of
 // launch, first loads and join.
 constexpr int TA_WARPS = 4;
 constexpr int TA_THREADS = 32 * TA_WARPS;
