@@ -80,6 +80,19 @@ def _rows2(t, dtype, what: str, dev: int, rows, width: int) -> int:
     _refuse(t, dtype, what, dev, f"{'rows' if rows is None else rows} of {width} adjacent values")
 
 
+def _per_row(t, dtype, what: str, dev: int, rows: int, width: int) -> int:
+    """The stride between the rows of a list for each of `rows` rows, or 0 for
+    one list that all share: t has one row, or is one row expanded."""
+    n = t.shape[0]
+    if n != rows and n != 1:
+        raise ValueError(f"{what}: one row, or one per row of logits")
+    ld = _rows2(t, dtype, what, dev, n, width)
+    # rows that overlap otherwise (a sliding window's view) are rows of their own
+    if not ld and n > 1 and t.stride(0):
+        raise ValueError(f"{what}: rows of {width} values that start {t.stride(0)} apart overlap; pass a contiguous copy")
+    return ld if n == rows else 0
+
+
 def _call(dev: int, stream, fn, *args) -> None:
     """One library call on device `dev`, which need not be the current one."""
     s = _raw_stream(dev) if stream is None else stream.cuda_stream
@@ -226,34 +239,26 @@ def logits_adjust(logits, out=None, tokens=None, *, scratch=None, history=None, 
     """Rows of logits [rows, V] adjusted into `out` (may be `logits`; None:
     not stored) and their greedy tokens (int32 [rows]; None: not wanted).
     history int32 [rows, H] or [1, H] with history_lens int32 [rows];
-    bias_ids / bias [n] for all rows; mask int32 words [rows or 1, ceil(V / 32)]."""
+    bias_ids / bias [n] for all rows; mask int32 words [rows or 1, ceil(V / 32)].
+    One row, also one expanded to all rows, serves them all; rows that overlap
+    otherwise are refused."""
     dev, f32, i32 = logits.get_device(), torch.float32, torch.int32
     rows, V = logits.shape
     ld = _rows2(logits, f32, "logits", dev, rows, V)
     h = hl = ids = bv = mk = h_ld = H = nb = mk_ld = 0
     if history is not None:
-        n, H = history.shape
-        h_ld = _rows2(history, i32, "history", dev, n, H)
-        if n != rows:
-            if n != 1:
-                raise ValueError("history: one row, or one per row of logits")
-            h_ld = 0
-        h = history.data_ptr()
+        H = history.shape[1]
+        h, h_ld = history.data_ptr(), _per_row(history, i32, "history", dev, rows, H)
         if history_lens is not None:
             hl = _flat(history_lens, i32, "history_lens", dev, rows)
     if bias_ids is not None:
         nb = bias_ids.numel()
         ids, bv = _flat(bias_ids, i32, "bias_ids", dev, nb), _flat(bias, f32, "bias", dev, nb)
     if mask is not None:
-        n, t = mask.shape[0], mask.dtype
+        t = mask.dtype
         if t is not i32 and t is not torch.uint32:
             raise TypeError("mask: int32 words wanted")
-        mk_ld = _rows2(mask, t, "mask", dev, n, (V + 31) // 32)
-        if n != rows:
-            if n != 1:
-                raise ValueError("mask: one row, or one per row of logits")
-            mk_ld = 0
-        mk = mask.data_ptr()
+        mk, mk_ld = mask.data_ptr(), _per_row(mask, t, "mask", dev, rows, (V + 31) // 32)
     o = _LOGITS_OPTS.pack(repeat_penalty, frequency_penalty, presence_penalty, h, h_ld, hl, H, ids, bv, nb, mk, mk_ld)
     if tokens is not None and scratch is None:
         raise ValueError("logits_adjust: tokens need a scratch (logits_scratch)")

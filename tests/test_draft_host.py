@@ -1,0 +1,61 @@
+"""What the drafted-token calls hand to the library, and what DraftVerifier
+keeps between calls.  No GPU: tensors that say they are on cuda:0, and library
+calls that are recorded, not made."""
+import pytest
+import torch
+
+from odiengine_b200 import draft
+
+
+class OnGpu:
+    """A CPU tensor that passes for one of cuda:0 (its memory is never followed)."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return 0
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+    monkeypatch.setattr(draft, "_call", lambda dev, stream, fn, *args: made.append((fn.__name__, args)))
+    return made
+
+
+def z(*shape, dtype=torch.float32):
+    return OnGpu(torch.zeros(shape, dtype=dtype))
+
+
+def logits_opts(calls, **kw):
+    """The options that logits_adjust packs for 4 rows of 64."""
+    draft.logits_adjust(z(4, 64), z(4, 64), **kw)
+    name, args = calls[-1]
+    assert name == "odi_cuda_logits_adjust"
+    keys = ("repeat", "frequency", "presence", "history", "history_ld", "history_len", "history_max", "bias_ids", "bias",
+            "bias_count", "mask", "mask_ld")
+    return dict(zip(keys, draft._LOGITS_OPTS.unpack(args[7])))
+
+
+@pytest.mark.parametrize("what,width", [("history", 5), ("mask", 2)])
+def test_rows_that_overlap_are_not_one_row(calls, what, width):
+    """A stride of 0 means one row for all rows of logits; a sliding window's
+    rows (stride 1) are rows of their own, and refused."""
+    i32 = torch.int32
+    full = torch.zeros((4, width), dtype=i32)
+    assert logits_opts(calls, **{what: OnGpu(full)})[what + "_ld"] == width
+    assert logits_opts(calls, **{what: OnGpu(torch.zeros((4, width + 3), dtype=i32)[:, :width])})[what + "_ld"] == width + 3
+    for one in (full[:1], full[:1].expand(4, width)):
+        assert logits_opts(calls, **{what: OnGpu(one)})[what + "_ld"] == 0
+    n = len(calls)
+    for view in (torch.zeros(width + 3, dtype=i32).unfold(0, width, 1), torch.zeros(4 * width, dtype=i32).as_strided((4, width), (width - 1, 1))):
+        assert view.shape == (4, width)
+        with pytest.raises(ValueError, match="overlap"):
+            logits_opts(calls, **{what: OnGpu(view)})
+    with pytest.raises(ValueError):
+        logits_opts(calls, **{what: OnGpu(full[:3])})
+    assert len(calls) == n
