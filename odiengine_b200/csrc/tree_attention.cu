@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           p[e] = ex2(s[e] - m[r][e & 1]);
-          w[e] = I8 ? p[e] * (dv[e >> 1] * vs[r][e & 1]) : p[e] * TA_UNIT;
+          w[e] = I8 ? p[e] * fminf(dv[e >> 1] * vs[r][e & 1], TA_FINITE) : p[e] * TA_UNIT;
           if (I8 && !vis[e]) w[e] = 0.f;
         }
 #pragma unroll

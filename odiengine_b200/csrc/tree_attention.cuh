@@ -27,6 +27,8 @@ struct TreeArgs {
   float* part;  // [kv head][tile][cluster][row][hd + 4]: reference, sum, -, -, accumulator
 };
 
+constexpr float TA_FINITE = 3.0e38f;         // bound of a factor: 0 times it is 0
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

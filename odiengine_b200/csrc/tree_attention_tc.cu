@@ -752,7 +752,8 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         // one factor for all rows as long as each has met the same largest scale (a
         // choice made per value, by selects, took 85 instructions of 800 per block)
         auto digits = [&](auto uniform) {
-          const float dvs = dvv * gr.vs[h0];
+          // finite, so that a weight of 0 (a slot not seen) stays 0 whatever its scale
+          const float dvs = fminf(dvv * gr.vs[h0], TA_FINITE);
 #pragma unroll
           for (int r0 = 0; r0 < NH; r0 += 8) {  // a 16-byte piece of low digits, one of high
             uint32_t lw[4], hw[4];
@@ -762,7 +763,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
               float2 f = f2(dvs);
               if (!uniform) {
                 const float2 vs = *reinterpret_cast<const float2*>(&gr.vs[h0 + 2 * n]);
-                f = make_float2(dvv * vs.x, dvv * vs.y);
+                f = make_float2(fminf(dvv * vs.x, TA_FINITE), fminf(dvv * vs.y, TA_FINITE));
               }
               const float2 p = make_float2(ex2(x2[n].x), ex2(x2[n].y));
               l2[n] = __fadd2_rn(l2[n], p);
