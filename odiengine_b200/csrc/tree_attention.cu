@@ -400,6 +400,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
 #pragma unroll
           for (int j = 0; j < MT; ++j) o[r][j][e] *= corr, o[r][j][2 + e] *= corr;
         }
+        __syncwarp();  // movmatrix and the products below want the whole warp
         weigh();
       }
 #pragma unroll

@@ -46,7 +46,10 @@ __device__ __forceinline__ uint32_t cluster_rank_of() {
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
   return n;
 }
+// The barriers' .aligned forms (these, and bar.sync by its number) want whole
+// warps, and their callers come from branches of some lanes.
 __device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

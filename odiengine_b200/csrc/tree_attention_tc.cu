@@ -207,9 +207,13 @@ __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x,
       "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void group_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void group_sync(int id, int n) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
 __device__ __forceinline__ bool group_any(int id, int n, bool v) {
   uint32_t r;
+  __syncwarp();
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
       "bar.red.or.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -677,7 +681,6 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       if (I8) top += fmaxf(-29.f, ldv + gr.lv_top[half]);
       if (!ok) dead = 1;
       bool fresh = i == 0;
-      __syncwarp();
       if (group_any(bar, GT, top > TOP || gr.none[half] || !ok)) {
         if (group_any(bar, GT, *reinterpret_cast<volatile int*>(&dead) != 0)) break;
         // Lane n (of 16 rows, and n + 16) gets the largest score of row n among the
