@@ -11,7 +11,9 @@ over a :class:`KVCache` of fp16 rows (the layout of the decode step) or of
 int8 rows with one scale each (half the bytes).  :class:`DraftVerifier` is the
 step made of them and of the library's products, for the models of
 odiengine_b200.decode.  Calls are asynchronous on
-`stream` (default: the tensors' device's current stream); errors are
+`stream` (default: the tensors' device's current stream), where outputs that
+a call makes are allocated too; tensors of another stream that are handed in
+are the caller's to order and to keep (Tensor.record_stream).  Errors are
 :class:`odiengine_b200.OdiCudaError`, or ValueError / TypeError for tensors
 that do not fit.  The position is device resident (`state`, the decode
 step's odi_cuda_decode_state as int32[4]), so calls can be captured in a CUDA
@@ -105,6 +107,15 @@ def _call(dev: int, stream, fn, *args) -> None:
         check(rc)
 
 
+def _new(shape, dtype, cache, stream):
+    """An output that a call makes: allocated on the stream that writes it, so
+    that its memory is neither still in use elsewhere nor handed out again."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=cache.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=cache.device)
+
+
 class KVCache:
     """One layer's K and V.  `k`, `v`: fp16 [kv_heads, ctx, head_dim] ("f16",
     what DecodeModel keeps per layer), or uint8 of :func:`kv_cache_bytes`
@@ -164,7 +175,7 @@ def qk_rope_append(qkv, cache: KVCache, state, q_out=None, *, heads: int, theta:
     ld = _rows2(qkv, f32, "qkv", dev, None, (heads + 2 * cache.kv_heads) * hd)
     T = qkv.shape[0]
     if q_out is None:
-        q_out = torch.empty((T, heads * hd), dtype=f32, device=cache.device)
+        q_out = _new((T, heads * hd), f32, cache, stream)
     ld_q = _rows2(q_out, f32, "q_out", dev, T, heads * hd)
     _call(dev, stream, lib().odi_cuda_qk_rope_append, qkv.data_ptr(), ld,
           None if q_norm is None else _flat(q_norm, f32, "q_norm", dev, hd),
@@ -178,8 +189,7 @@ def kv_read(cache: KVCache, start: int, count: int, k_out=None, v_out=None, stre
     fp16 or fp32 by the outputs' type (default: new fp16 tensors)."""
     dev = cache.index
     if k_out is None and v_out is None:
-        k_out, v_out = (torch.empty((cache.kv_heads, max(count, 0), cache.head_dim), dtype=torch.float16, device=cache.device)
-                        for _ in range(2))
+        k_out, v_out = (_new((cache.kv_heads, max(count, 0), cache.head_dim), torch.float16, cache, stream) for _ in range(2))
     t = (v_out if k_out is None else k_out).dtype
     if t is not torch.float16 and t is not torch.float32:
         raise TypeError(f"kv_read: outputs are fp16 or fp32, not {t}")
@@ -216,7 +226,7 @@ def attention_tree(q, cache: KVCache, out=None, state=None, *, heads: int, scale
     ld = _rows2(q, f32, "q", dev, None, w)
     T = q.shape[0]
     if out is None:
-        out = torch.empty((T, w), dtype=f32, device=cache.device)
+        out = _new((T, w), f32, cache, stream)
     if mask is not None:
         t = mask.dtype
         if t is not torch.int32 and t is not torch.uint32:

@@ -35,3 +35,48 @@ def test_a_large_scale_stays_with_who_sees_it(dr, hd, H, KV, ctx, T, big):  # no
     clean = dr.attention_tree(q, c, None, state(pos), **kw).cpu().numpy()
     scales(c, c.v)[:, pos + j] = big
     assert np.array_equal(dr.attention_tree(q, c, None, state(pos), **kw).cpu().numpy(), clean)
+
+
+# ---- streams ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("op", ["append", "read", "attention"])
+def test_outputs_are_allocated_on_the_stream_that_writes_them(dr, op):  # noqa: F811
+    """A block that was freed while work of the current stream still reads it is
+    not what a call on another stream writes to."""
+    import torch
+
+    rng = np.random.default_rng(6)
+    hd, H, KV, T, ctx = 128, 16, 16, 128, 256
+    c = dr.KVCache.new("f16", KV, hd, ctx)
+    fill(c, rng)
+    x = dev(rng.standard_normal((T, (H + 2 * KV) * hd)).astype(np.float32))
+    q = dev(rng.standard_normal((T, H * hd)).astype(np.float32))
+    scr, st = dr.attention_tree_scratch(c, T, H), state(10)
+    s = torch.cuda.Stream()
+
+    def call(**kw):
+        if op == "append":
+            return dr.qk_rope_append(x, c, st, heads=H, theta=1e4, **kw)
+        if op == "read":
+            return torch.cat([t.flatten() for t in dr.kv_read(c, 3, T, **kw)])
+        return dr.attention_tree(q, c, None, st, heads=H, scale=0.1, scratch=scr, **kw)
+
+    want = call()
+    torch.cuda.synchronize()
+    # two blocks of the outputs' size (both outputs of a read), and a reader of them that comes late
+    n, dt = (T * H * hd, torch.float32) if op != "read" else (KV * T * hd, torch.float16)
+    blocks = [torch.full((n,), 3.0, dtype=dt, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    late = [b * 2 for b in blocks]
+    del blocks
+    if op == "read":
+        k, v = dr.kv_read(c, 3, T, stream=s)
+        s.synchronize()
+        got = torch.cat([k.flatten(), v.flatten()])
+    else:
+        got = call(stream=s)
+        s.synchronize()
+    torch.cuda.synchronize()
+    assert all((x == 6.0).all() for x in late)
+    assert torch.equal(got, want)
