@@ -26,7 +26,7 @@ import struct
 
 import torch
 
-from . import FLAG_PDL, MatmulOpts, check, lib
+from . import FLAG_PDL, MatmulOpts, check, lib, new_workspace, workspace_bytes
 
 KV_F16, KV_I8 = 0, 1                      # ODI_CUDA_KV_*
 KV_DTYPES = {"f16": KV_F16, "i8": KV_I8}
@@ -318,16 +318,16 @@ class DraftVerifier:
         self.states = torch.zeros((T, 4), dtype=torch.int32, device=dev)
         self.scratch = attention_tree_scratch(self.caches[0], T, cfg.heads)
         self.logits_ws = logits_scratch(T, dev)
-        for lw in weights.layers:
-            for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown):
-                dw._ws_for(T, cfg.act_mode, dev)
-        weights.output._ws_for(T, cfg.act_mode, dev)
+        # one workspace for all products (the steps' calls are on one stream), and
+        # not the weights' own: other models and verifiers may run on those
+        products = [dw for lw in weights.layers for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown)] + [weights.output]
+        self.products_ws = new_workspace(max(workspace_bytes(dw.dtype, T, dw.N, dw.K, cfg.act_mode) for dw in products), dev)
         self.pos, self.pending, self.tokens = 0, None, []
 
     # ---- the forward pass of T nodes --------------------------------------
     def _product(self, dw, x, y, T, norm=None, swiglu=False, accumulate=False):
         o = MatmulOpts(None if norm is None else norm.data_ptr(), self.cfg.eps, int(swiglu), int(accumulate), None, 0, None)
-        ws = dw._ws
+        ws = self.products_ws
         check(lib().odi_cuda_matmul_fused(dw.dtype, dw.data_ptr, x.data_ptr(), y.data_ptr(), T, dw.N, dw.K,
                                           self.cfg.act_mode, ws.data_ptr(), ws.numel(), FLAG_PDL, ctypes.byref(o),
                                           _raw_stream(self.device.index)))
@@ -356,10 +356,7 @@ class DraftVerifier:
 
     def status(self) -> int:
         """OR of the device error words (0: no bounded wait gave up)."""
-        words = [self.scratch[:4].view(torch.int32)]
-        for lw in self.w.layers:
-            words += [dw._ws[:4].view(torch.int32) for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown)]
-        words.append(self.w.output._ws[:4].view(torch.int32))
+        words = [ws[:4].view(torch.int32) for ws in (self.scratch, self.products_ws)]
         v = 0
         for x in torch.cat(words).cpu().tolist():
             v |= x

@@ -205,3 +205,46 @@ def test_penalties_masks_and_refusals(cuda_lib):
     from odiengine_b200.decode import seeded_model
     with pytest.raises(ValueError):
         DraftVerifier(cfg, seeded_model(cfg, interleave_gate_up=True))
+
+
+def test_verifiers_keep_their_workspaces(cuda_lib):
+    """Two verifiers and a DecodeModel over the same weights: building one
+    leaves the others' workspaces alone, and steps that run at the same time on
+    two streams give what they give one after the other."""
+    import threading
+
+    import torch
+
+    from odiengine_b200.decode import DecodeModel
+    from odiengine_b200.draft import DraftVerifier
+
+    cfg, mw = model(0)  # Q8: a product of several tokens quantises them into its workspace
+    dm = DecodeModel(cfg, mw, mode="fused")
+    held = [dw._ws for lw in mw.layers for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown)] + [mw.output._ws]
+    vs = [DraftVerifier(cfg, mw, max_nodes=n) for n in (8, 32)]
+    now = [dw._ws for lw in mw.layers for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown)] + [mw.output._ws]
+    assert all(a is b for a, b in zip(held, now)) and dm.status() == 0
+    rng = np.random.default_rng(12)
+    nodes = [[int(t) for t in rng.integers(0, cfg.vocab, n)] for n in (8, 32)]
+    for v, n in zip(vs, nodes):
+        v.start([5, 17, n[0]])
+    want, streams = [], [torch.cuda.Stream() for _ in vs]
+    for v, n in zip(vs, nodes):
+        v._forward(n, None, None, True)
+        want.append(v.logits[:len(n)].clone())
+    torch.cuda.synchronize()
+    wrong = [0, 0]
+
+    def run(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(60):
+                vs[i]._forward(nodes[i], None, None, True)
+                wrong[i] += not torch.equal(vs[i].logits[:len(nodes[i])], want[i])
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert wrong == [0, 0] and all(v.status() == 0 for v in vs)
