@@ -375,7 +375,8 @@ class DraftVerifier:
             raise ValueError("start: a prompt of tokens of the vocabulary wanted")
         if len(prompt) > self.cfg.ctx:
             raise ValueError("prompt longer than the context")
-        self.pos, self.tokens = 0, list(prompt)
+        # no sequence until the prompt has run
+        self.pos, self.pending, self.tokens = 0, None, list(prompt)
         with torch.cuda.device(self.device):
             for i in range(0, len(prompt) - 1, self.max_nodes):
                 chunk = prompt[i:min(i + self.max_nodes, len(prompt) - 1)]

@@ -59,3 +59,41 @@ def test_rows_that_overlap_are_not_one_row(calls, what, width):
     with pytest.raises(ValueError):
         logits_opts(calls, **{what: OnGpu(full[:3])})
     assert len(calls) == n
+
+
+# ---- sequences -------------------------------------------------------------------------------------------------
+
+@pytest.fixture
+def verifier(monkeypatch):
+    """A DraftVerifier without a device: its forward pass does nothing."""
+    import contextlib
+    import types
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(draft.DraftVerifier, "_forward", lambda self, *a: None)
+    monkeypatch.setattr(draft.DraftVerifier, "_check", lambda self: None)
+    v = object.__new__(draft.DraftVerifier)
+    v.cfg = types.SimpleNamespace(vocab=100, ctx=64)
+    v.device, v.max_nodes, v.history = torch.device("cpu"), 4, 0
+    v.pos, v.pending, v.tokens = 0, None, []
+    return v
+
+
+@pytest.mark.parametrize("where", ["_forward", "_check"])
+def test_a_prompt_that_failed_leaves_no_sequence(verifier, monkeypatch, where):
+    """start that raises midway leaves nothing that verify could go on from,
+    the sequence before it neither."""
+    verifier.start([1, 2, 3])
+    assert verifier.pending == 3 and verifier.pos == 2
+
+    def fail(self, *a):
+        raise RuntimeError("a launch failed")
+
+    with monkeypatch.context() as m:
+        m.setattr(draft.DraftVerifier, where, fail)
+        with pytest.raises(RuntimeError, match="a launch failed"):
+            verifier.start([4, 5, 6, 7, 8, 9])
+    with pytest.raises(RuntimeError, match="start a sequence"):
+        verifier.verify()
+    verifier.start([7, 8])
+    assert verifier.pending == 8 and verifier.tokens == [7, 8]
