@@ -65,6 +65,8 @@ def _refuse(t, dtype, what: str, dev: int, shape) -> None:
 # -1 for a tensor that is on no GPU.
 def _flat(t, dtype, what: str, dev: int, numel: int) -> int:
     """The address of a contiguous tensor of numel values."""
+    if t is None:
+        raise TypeError(f"{what}: a tensor of {dtype} wanted, got None")
     if t.dtype is not dtype or t.get_device() != dev or dev < 0 or t.numel() != numel or not t.is_contiguous():
         _refuse(t, dtype, what, dev, f"{numel} contiguous values")
     return t.data_ptr()
@@ -225,6 +227,7 @@ def attention_tree(q, cache: KVCache, out=None, state=None, *, heads: int, scale
     dev, w, f32 = cache.index, heads * cache.head_dim, torch.float32
     ld = _rows2(q, f32, "q", dev, None, w)
     T = q.shape[0]
+    st, n = _state_ptr(state, dev), 0 if scratch is None else scratch.numel()
     if out is None:
         out = _new((T, w), f32, cache, stream)
     if mask is not None:
@@ -233,8 +236,7 @@ def attention_tree(q, cache: KVCache, out=None, state=None, *, heads: int, scale
             raise TypeError("mask: int32 words wanted")
         mask = _flat(mask, t, "mask", dev, T * ((T + 31) // 32))
     _call(dev, stream, lib().odi_cuda_attention_tree, q.data_ptr(), ld, cache._ref, _flat(out, f32, "out", dev, T * w),
-          mask, _state_ptr(state, dev), T, heads, scale, _flat(scratch, torch.uint8, "scratch", dev, scratch.numel()),
-          scratch.numel())
+          mask, st, T, heads, scale, _flat(scratch, torch.uint8, "scratch", dev, n), n)
     return out
 
 
@@ -261,9 +263,13 @@ def logits_adjust(logits, out=None, tokens=None, *, scratch=None, history=None, 
         h, h_ld = history.data_ptr(), _per_row(history, i32, "history", dev, rows, H)
         if history_lens is not None:
             hl = _flat(history_lens, i32, "history_lens", dev, rows)
+    elif history_lens is not None:
+        raise ValueError("logits_adjust: history_lens without a history")
     if bias_ids is not None:
         nb = bias_ids.numel()
         ids, bv = _flat(bias_ids, i32, "bias_ids", dev, nb), _flat(bias, f32, "bias", dev, nb)
+    elif bias is not None:
+        raise ValueError("logits_adjust: bias without bias_ids")
     if mask is not None:
         t = mask.dtype
         if t is not i32 and t is not torch.uint32:

@@ -97,3 +97,32 @@ def test_a_prompt_that_failed_leaves_no_sequence(verifier, monkeypatch, where):
         verifier.verify()
     verifier.start([7, 8])
     assert verifier.pending == 8 and verifier.tokens == [7, 8]
+
+
+# ---- arguments left out ----------------------------------------------------------------------------------------
+
+def test_what_is_missing_is_named(calls):
+    """A list without its partner, or a state or scratch left out, is a
+    TypeError or ValueError that names it, and no call."""
+    import types
+
+    c = types.SimpleNamespace(index=0, kv_heads=2, head_dim=64, ctx=8, device="cpu", _ref=0)
+    q, out = z(1, 256), z(1, 256)
+    st, scr, i32 = z(4, dtype=torch.int32), z(1024, dtype=torch.uint8), torch.int32
+    with pytest.raises(TypeError, match="state"):
+        draft.attention_tree(q, c, out, heads=4, scale=0.1, scratch=scr)
+    with pytest.raises(TypeError, match="scratch"):
+        draft.attention_tree(q, c, out, st, heads=4, scale=0.1, scratch=None)
+    with pytest.raises(TypeError, match="state"):
+        draft.qk_rope_append(z(1, 512), c, None, q, heads=4, theta=1e4)
+    x = z(4, 64)
+    with pytest.raises(TypeError, match="bias"):
+        draft.logits_adjust(x, x, bias_ids=z(3, dtype=i32))
+    with pytest.raises(ValueError, match="bias_ids"):
+        draft.logits_adjust(x, x, bias=z(3))
+    with pytest.raises(ValueError, match="history"):
+        draft.logits_adjust(x, x, history_lens=z(4, dtype=i32))
+    assert not calls
+    draft.attention_tree(q, c, out, st, heads=4, scale=0.1, scratch=scr)
+    draft.logits_adjust(x, x, bias_ids=z(3, dtype=i32), bias=z(3))
+    assert len(calls) == 2
