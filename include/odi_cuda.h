@@ -472,7 +472,8 @@ int odi_cuda_kv_move(const odi_cuda_kv_cache* cache, const int32_t* d_src, const
  * d_mask[t * ceil(T / 32) + j / 32] is set (d_mask NULL: j <= t).  Slots
  * outside the cache are not seen, a node that sees nothing gets zeros, and
  * what lies in slots that a node does not see (NaN included) does not reach
- * it.  Grouped-query heads share kv head h / (heads / kv_heads), any ratio.
+ * it.  A seen key or value (int8: a scale) that is not finite makes the
+ * outputs NaN; a score of -inf may count as a weight of 0 instead.  Grouped-query heads share kv head h / (heads / kv_heads), any ratio.
  * fp32 scores, softmax and sums.  d_scratch: as for
  * odi_cuda_attention_decode (16-byte aligned, zero before its first use,
  * left reusable, calls on one stream only; its first int is the error word,

@@ -37,6 +37,47 @@ def test_a_large_scale_stays_with_who_sees_it(dr, hd, H, KV, ctx, T, big):  # no
     assert np.array_equal(dr.attention_tree(q, c, None, state(pos), **kw).cpu().numpy(), clean)
 
 
+@pytest.mark.parametrize("dt", ["f16", "i8"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("hd,H,KV,ctx,T", SHAPES)
+def test_nonfinite_rows_reach_all_of_who_sees_them(dr, dt, bad, which, hd, H, KV, ctx, T):  # noqa: F811
+    """One value of a tree slot's K or V (int8: the row's scale) is not finite:
+    every output of a node that sees it is NaN, of every head, and the others
+    are what they are without it.  (An fp16 key's infinity stands against
+    queries of either sign: exp(-inf) is a weight of 0, and the header allows NaN.)"""
+    rng = np.random.default_rng(9)
+    pos, j = 150, 3
+    c = dr.KVCache.new(dt, KV, hd, ctx)
+    fill(c, rng, 0, pos + T)
+    q = dev((1.5 * rng.standard_normal((T, H * hd))).astype(np.float32))
+    vis = random_tree(rng, T)
+    vis[j + 1:, j] &= rng.random(T - j - 1) < 0.5
+    vis[-1, j] = False
+    kw = dict(heads=H, scale=0.1, scratch=dr.attention_tree_scratch(c, T, H), mask=dev(words(vis)))
+    clean = dr.attention_tree(q, c, None, state(pos), **kw).cpu().numpy()
+    half = getattr(c, which)
+    if dt == "f16":
+        half[:, pos + j, 5] = bad
+    elif not (bad < 0):  # scales are not negative
+        scales(c, half)[:, pos + j] = bad
+    else:
+        return
+    got = dr.attention_tree(q, c, None, state(pos), **kw).cpu().numpy()
+    nan = np.isnan(got.reshape(T, H, hd))
+    if dt == "f16" and which == "k" and np.isinf(bad):
+        sees = vis.copy()
+        sees[:, j] = False
+        without = dr.attention_tree(q, c, None, state(pos), **{**kw, "mask": dev(words(sees))}).cpu().numpy().reshape(T, H, hd)
+        below = (q.cpu().numpy().reshape(T, H, hd)[..., 5] * bad < 0) & vis[:, j, None]  # scores of -inf
+        assert (nan.all(-1) == nan.any(-1)).all()
+        zero = below & ~nan.any(-1)
+        assert np.array_equal(got.reshape(T, H, hd)[zero], without[zero])
+        nan[zero] = True
+    assert nan[vis[:, j]].all()
+    assert vis[:, j].any() and not vis[:, j].all() and np.array_equal(got[~vis[:, j]], clean[~vis[:, j]])
+
+
 # ---- streams ---------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("op", ["append", "read", "attention"])
