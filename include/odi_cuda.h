@@ -473,12 +473,17 @@ int odi_cuda_kv_move(const odi_cuda_kv_cache* cache, const int32_t* d_src, const
  * outside the cache are not seen, a node that sees nothing gets zeros, and
  * what lies in slots that a node does not see (NaN included) does not reach
  * it.  A seen key or value (int8: a scale) that is not finite makes the
- * outputs NaN; a score of -inf may count as a weight of 0 instead.  Grouped-query heads share kv head h / (heads / kv_heads), any ratio.
- * fp32 scores, softmax and sums.  d_scratch: as for
- * odi_cuda_attention_decode (16-byte aligned, zero before its first use,
- * left reusable, calls on one stream only; its first int is the error word,
- * odi_cuda_workspace_status); its size depends on head_dim alone, and calls
- * of different shapes may share it.  int8 rows' scales are not negative. */
+ * outputs NaN; a score of -inf may count as a weight of 0 instead.
+ * Grouped-query heads share kv head h / (heads / kv_heads), any ratio.
+ * Scores, softmax and sums are fp32.  Into the products go, of an int8 cache, q
+ * to within 2^-22 of its head's largest value, and weight * scale to within 2^-22
+ * of itself or 2^-25 of the largest, whichever is more; of an fp16 cache, q to
+ * within 2^-22 of each value, and weights to within 2^-22 of themselves or 2^-36
+ * of the largest (a key with nearly all the weight and values of 0 leaves the
+ * others at that).  d_scratch: as for odi_cuda_attention_decode (16-byte
+ * aligned, zero before its first use, left reusable, calls on one stream only;
+ * its first int is the error word, odi_cuda_workspace_status); its size depends
+ * on head_dim alone, and calls of different shapes may share it.  int8 rows' scales are not negative. */
 #define ODI_CUDA_TREE_MAX 256
 size_t odi_cuda_attention_tree_scratch_bytes(int tokens, int heads, int kv_heads, int head_dim, int ctx);
 int odi_cuda_attention_tree(const float* d_q, int64_t ld_q, const odi_cuda_kv_cache* cache, float* d_out,

@@ -44,9 +44,10 @@ namespace {
 //    the codes, or the fp16 values, of V enter unrounded.
 //
 // Softmax: m is a reference, not the running maximum: it moves only when a
-// weight passes 2^15 against it (then to the maximum, and the sums are
-// rescaled), which after the first groups is rare; fp16 pairs hold weights
-// up to 2^16 and down to 2^-24.
+// weight (int8: weight * scale, what the values enter with) passes 2^15 against
+// it, by whole powers of two to where the largest is 2^8 (fp16: 2^12), and the
+// sums are scaled; fp16 pairs hold 22 bits of weights from 2^-3 and smaller ones
+// to within 2^-25, 2^-33 (2^-37) of the largest.
 //
 // Bound by the fetch of the cache for long ones: one token, 64 / 8 heads, 131001
 // int8 positions 59 us, 277 MB at 4.7 TB/s (the copy peak gives 42); 518 fp16
@@ -62,7 +63,10 @@ constexpr int TA_GROUP = 16;
 // 15.8 / 44.7 and 9.0 / 12.1 / 28.5.  The length is not known on the host.
 constexpr int TA_TC_ROWS = 8;
 constexpr float TA_TOP = 32768.f;            // a weight past this moves the reference
-constexpr float TA_UNIT = 16.f;              // the largest weight right after that
+// log2 of the largest right after that.  An fp16 cache's scales, those of its
+// values, are not known: its unit is 2^4 finer.
+template <bool I8>
+constexpr float TA_UNIT = I8 ? 8.f : 12.f;
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
   }
   __syncthreads();
 
-  float o[NR][MT][4], m[NR][2], l[NR][2], vs[NR][2], rc[NR][2];
+  float o[NR][MT][4], m[NR][2], l[NR][2], rc[NR][2];
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
 #pragma unroll
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[r][j][e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) m[r][e] = TA_NONE, l[r][e] = 0.f, vs[r][e] = I8 ? TA_VMOST : TA_UNIT, rc[r][e] = rowc[r * 8 + 2 * c + e];
+    for (int e = 0; e < 2; ++e) m[r][e] = TA_NONE, l[r][e] = 0.f, rc[r][e] = rowc[r * 8 + 2 * c + e];
   }
   for (; grp < ngroups; grp += step) {
     const int p0 = grp * TA_GROUP;
@@ -297,6 +301,14 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
           for (int w = 0; w < VW; ++w) vw[i][w] = 0;
       }
     }
+    float dvc[2];  // a scale near 0 stands for 2^-64: a key whose values are nothing moves no reference
+    if (I8)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // a row whose scale of K or V is not finite gives NaN to who sees it
+        if (!finite(dv[i])) dk[i] = __int_as_float(0x7fc00000), dv[i] = 0.f;
+        if (!finite(dk[i])) dk[i] = __int_as_float(0x7fc00000);
+        dvc[i] = fmaxf(dv[i], 0x1p-64f);
+      }
     uint32_t ph[NR][2], pl[NR][2];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -323,7 +335,7 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
 #pragma unroll
         for (int e = 0; e < 4; ++e)  // digits joined: |digit sums| < 2^21, so each is exact in fp32
           s[e] = fmaf((float)acc[0][e], 65536.f, fmaf((float)acc[1][e], 256.f, (float)acc[DIG - 1][e])) *
-                 (finite(dk[e >> 1]) ? dk[e >> 1] : __int_as_float(0x7fc00000)) * rc[r][e & 1];
+                 dk[e >> 1] * rc[r][e & 1];
       } else {
         float acc[2 * DIG][4];  // high and low halves, two chains of each
 #pragma unroll
@@ -344,59 +356,42 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[e] = (acc[0][e] + acc[1][e] + (acc[2][e] + acc[3][e])) * rc[r][e & 1];
       }
-      bool vis[4] = {true, true, true, true};
       if (edge) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const unsigned see = seen_bits(a, rowt[r * 8 + 2 * c + e], p0, pos, len);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            vis[2 * i + e] = (see >> (g + 8 * i)) & 1u;
-            if (!vis[2 * i + e]) s[2 * i + e] = -INFINITY;
+            if (!((see >> (g + 8 * i)) & 1u)) s[2 * i + e] = -INFINITY;
             else if (!I8 && ((bad >> (g + 8 * i)) & 1u)) s[2 * i + e] = __int_as_float(0x7fc00000);
           }
         }
       }
-      float p[4], w[4], top[2];
+      float p[4], top[2];
+      // weights, and each row's largest on this lane
       auto weigh = [&]() {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = ex2(s[e] - m[r][e & 1]);
-          w[e] = I8 ? p[e] * fminf(dv[e >> 1] * vs[r][e & 1], TA_FINITE) : p[e] * TA_UNIT;
-          if (I8 && !vis[e]) w[e] = 0.f;
-        }
+        for (int e = 0; e < 4; ++e) p[e] = ex2(s[e] - m[r][e & 1]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) top[e] = fmaxf(fmaxf(p[e], w[e]), fmaxf(p[2 + e], w[2 + e]));
+        for (int e = 0; e < 2; ++e)
+          top[e] = I8 ? fmaxf(p[e] * dvc[0], p[2 + e] * dvc[1]) : fmaxf(p[e], p[2 + e]);
       };
       weigh();
       if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > TA_TOP)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // each row by itself: a row's result does not depend on its neighbours
-          float mx = fmaxf(s[e], s[2 + e]), dm = 0.f;
-          if (I8) {
-            if (vis[e] && finite(dv[0])) dm = dv[0];
-            if (vis[2 + e] && finite(dv[1])) dm = fmaxf(dm, dv[1]);
-          }
+          float mx = fmaxf(s[e], s[2 + e]);
+          if (I8) mx = fmaxf(s[e] + __log2f(dvc[0]), s[2 + e] + __log2f(dvc[1]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) {
             top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            if (I8) dm = fmaxf(dm, __shfl_xor_sync(0xffffffffu, dm, x));
           }
           if (!(top[e] > TA_TOP)) continue;
-          const float mn = fmaxf(m[r][e], mx);
-          float corr = ex2(m[r][e] - mn);
-          l[r][e] *= corr;
+          const float mn = ceilf(mx) - TA_UNIT<I8>, d = m[r][e] - mn;
+          const float corr = d < -126.f ? 0.f : pow2((int)d);
           m[r][e] = mn;
-          if (I8 && dm > 0.f) {
-            // TA_UNIT over a power of two above the largest scale seen
-            const int ex = max((int)(__float_as_uint(dm) >> 23) - 126, -116);
-            const float nv = pow2(4 - ex);
-            if (nv < vs[r][e]) {
-              corr *= nv / vs[r][e];
-              vs[r][e] = nv;
-            }
-          }
+          l[r][e] *= corr;
 #pragma unroll
           for (int j = 0; j < MT; ++j) o[r][j][e] *= corr, o[r][j][2 + e] *= corr;
         }
@@ -404,12 +399,10 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
         weigh();
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float q0 = p[e], q1 = p[2 + e];
-        l[r][e] += I8 ? (vis[e] && !finite(dv[0]) ? __int_as_float(0x7fc00000) : q0) +
-                            (vis[2 + e] && !finite(dv[1]) ? __int_as_float(0x7fc00000) : q1)
-                      : q0 + q1;
-      }
+      for (int e = 0; e < 2; ++e) l[r][e] += p[e] + p[2 + e];
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = I8 ? p[e] * dv[e >> 1] : p[e];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const __half2 hi = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
@@ -467,10 +460,9 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
       for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
       const int n = r * 8 + 2 * c + e;
       float* f = fold + (warp * NR * 8 + n) * HD + MT * 2 * g;
-      const float inv = 1.f / vs[r][e];  // a power of two
       if (g == 0) ml[warp][n] = make_float2(m[r][e], sum);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(f + 2 * j) = make_float2(o[r][j][e] * inv, o[r][j][2 + e] * inv);
+      for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(f + 2 * j) = make_float2(o[r][j][e], o[r][j][2 + e]);
     }
   __syncthreads();
   const int rows = min(NR * 8, a.R - tile * NR * 8);

@@ -10,7 +10,6 @@ namespace odi_cuda {
 
 constexpr int TA_SMS = 148;
 constexpr float TA_NONE = -3.402823466e38f;  // reference of a row that has seen nothing
-constexpr float TA_VMOST = 0x1p120f;         // factor of an int8 row's scales before any was seen
 
 struct TreeArgs {
   const float* q;
@@ -27,7 +26,6 @@ struct TreeArgs {
   float* part;  // [kv head][tile][cluster][row][hd + 4]: reference, sum, -, -, accumulator
 };
 
-constexpr float TA_FINITE = 3.0e38f;         // bound of a factor: 0 times it is 0
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -16,11 +16,12 @@
 //
 // fp32 results from 16- and 8-bit products, as columns of one instruction:
 //  * int8 cache (kind::i8, exact 32-bit integer sums): q is fixed point in
-//    three signed digits (96 columns), P * (V's row scale) fixed point in four
-//    unsigned digits (128 columns): an integer up to 2^32 in units of 2^-24 of
-//    the largest weight.
-//  * fp16 cache (kind::f16): q and P are each the sum of two fp16 values (64
-//    columns); the high and low halves' sums are added in fp32.
+//    three signed digits (96 columns), |dq_i| <= 2^-22 max |q|; P * (V's row
+//    scale) in four unsigned digits (128 columns), an integer below 2^32.
+//  * fp16 cache (kind::f16): q is the sum of two fp16 values (22 bits), P is
+//    hi + 2^-11 lo (64 columns each); the two sums are joined in fp32.  With the
+//    low half scaled so, a weight of up to 2^15 has 22 bits down to 2^-14 and an
+//    absolute error of 2^-37 below.
 //
 //   warp 0       TMA producer: tiles K0 K1 V0 K2 V1 ... through one ring
 //   warps 1, 2   issue the products, one warp for each group of rows; warp 1
@@ -31,15 +32,17 @@
 //
 // While one group of rows is in its softmax the tensor core works for the
 // others.  As in tree_attention.cu m is a reference that moves only when a
-// weight would leave its range; then (and every few blocks, so that integer
-// sums cannot overflow and fp32 sums stay short) O moves from tensor memory
-// to fp32 registers and starts again.
+// weight (int8: weight * scale, what the values enter with) would leave its
+// range, by whole powers of two.  Only the row that moves takes its O out of
+// tensor memory then, to fp32 registers; all rows do every few blocks, always
+// the same ones (integer sums cannot overflow so, and fp32 sums, which truncate,
+// stay short).
 //
 // The softmax bounds the kernel: 17 instructions per score (packed fp32 pairs
 // where two scores share an operation), of which two warps per scheduler issue
-// one every 2.3 cycles.  64 nodes, 64 / 8 heads, 32641 int8 positions: 182 us,
-// where fetching the cache takes 11 and 69 GFLOP at the fp16 rate 41; without
-// any products the same loop takes 176.  Smaller shares for more warps (16 of 16
+// one every 2.3 cycles.  64 nodes, 64 / 8 heads, 32641 int8 positions: 185 us (fp16:
+// 168), where fetching the cache takes 11 and 69 GFLOP at the fp16 rate 41; the
+// loop without any products took 176 where the whole took 182.  Smaller shares for more warps (16 of 16
 // rows: 212 us, the work per block that does not depend on rows doubles), a vote
 // without a barrier (234 where this took 224) and scores one block ahead of the
 // weights (200) were slower.
@@ -62,6 +65,7 @@ constexpr int BK = 128;  // positions per block
 constexpr int NT = 32;   // rows per group
 constexpr int ERR_TREE_WAIT = 64;
 constexpr int START_BYTES = 32 * 16;
+constexpr float P_LOW = 0x1p-11f;  // fp16: the unit of P's low half, which keeps it from the subnormals
 
 template <bool I8, int SUBS_>
 struct Cfg {
@@ -75,7 +79,7 @@ struct Cfg {
   static constexpr int P_OFF = Q_OFF + SUBS * QB;
   // int8: what the sums of S start from.  Copied by the tensor core's own
   // instructions in 32-row pieces: 187 us where the softmax threads stored it
-  // (54 of their 616 instructions per block), 181 now, 206 in 128-row pieces
+  // (54 of their 616 instructions per block), 182 this way, 206 in 128-row pieces
   // (64 nodes over 32641 positions).
   static constexpr int START_OFF = P_OFF + SUBS * PB;
   static constexpr int SMEM = START_OFF + (I8 ? START_BYTES : 0) + 1024;  // + alignment slack
@@ -91,9 +95,15 @@ struct Cfg {
   static constexpr int ROWS = NT * SUBS;
   static constexpr int SCOLS = DQ * NT, OCOL = (I8 ? 4 : 2) * NT, SUBCOLS = 2 * OCOL;
   static constexpr int TMEM_COLS = SUBCOLS * SUBS;
-  // blocks between two moves of O to registers: 255 * 127 * 128 * 256 < 2^31;
+  // blocks between two moves of all O to registers: 255 * 128 * 128 * 256 < 2^31;
   // the fp32 accumulator truncates, about 2^-26 of the sum per instruction
   static constexpr int PERIOD = I8 ? 256 : 4;
+  // Weights in P, log2: what they stay below, and the largest right after a move.
+  // int8: an integer below 2^32, so to within 2^-25 of the largest, either way;
+  // 64 nodes over 32641 positions 185 us, 189 with the largest at 2^24 and the
+  // dither left out, 198 and 207 at 2^27 and 2^29: rows move more often, and a
+  // block in which one does costs two.  fp16: to within 2^-37, 2^-43 of the largest.
+  static constexpr float P_TOP = I8 ? 31.9f : 15.f, P_UNIT = I8 ? 26.f : 8.f;
   static_assert(SMEM <= 222 * 1024, "shared memory, beside the static part");
 };
 
@@ -200,6 +210,26 @@ __device__ __forceinline__ void ld_digits(uint32_t (&r)[3][32], uint32_t addr, u
       : "r"(addr), "r"(addr + 1 * stride), "r"(addr + 2 * stride)
       : "memory");
 }
+__device__ __forceinline__ void st_digits(const uint32_t (&r)[2][8], uint32_t addr, uint32_t stride) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7};\n\t"
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%17], {%8,%9,%10,%11,%12,%13,%14,%15};\n\t"
+      "tcgen05.wait::st.sync.aligned;" ::"r"(r[0][0]), "r"(r[0][1]), "r"(r[0][2]), "r"(r[0][3]), "r"(r[0][4]), "r"(r[0][5]),
+      "r"(r[0][6]), "r"(r[0][7]), "r"(r[1][0]), "r"(r[1][1]), "r"(r[1][2]), "r"(r[1][3]), "r"(r[1][4]), "r"(r[1][5]),
+      "r"(r[1][6]), "r"(r[1][7]), "r"(addr), "r"(addr + 1 * stride)
+      : "memory");
+}
+__device__ __forceinline__ void st_digits(const uint32_t (&r)[2][16], uint32_t addr, uint32_t stride) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[k][0]),
+        "r"(r[k][1]), "r"(r[k][2]), "r"(r[k][3]), "r"(r[k][4]), "r"(r[k][5]), "r"(r[k][6]), "r"(r[k][7]), "r"(r[k][8]),
+        "r"(r[k][9]), "r"(r[k][10]), "r"(r[k][11]), "r"(r[k][12]), "r"(r[k][13]), "r"(r[k][14]), "r"(r[k][15]),
+        "r"(addr + k * stride)
+        : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -265,16 +295,14 @@ struct Bars {
 };
 // What a group's threads share about its rows.
 struct alignas(16) Group {
-  float c[NT];           // factor of the scores, positive
-  float nm[NT];          // minus the reference
-  float nx[NT];          // the same, or 0 for a row without one
-  float lv[NT];          // log2 of vs
-  float vs[NT];          // int8: factor of weight * scale
-  float fo[NT], fl[NT];  // factors of O and of the sums when the reference moves
-  float mx[4][NT], dm[4][NT];
-  float lv_top[2];       // the largest lv of each half
-  int lv_same[2];        // all lv of the half are equal
-  int none[2];           // some row of the half has no reference yet
+  float c[NT];      // factor of the scores, positive
+  float nm[NT];     // minus the reference, a whole number
+  float nx[NT];     // the same, or 0 for a row without one
+  float dx[NT];     // how far it moved
+  float fo[NT];     // factor of O and of the sums then
+  float mx[4][NT];
+  unsigned scaled[2];  // rows of each half whose sums it scales
+  int none[2];         // some row of the half has no reference yet
 };
 
 template <bool I8, int SUBS>
@@ -290,7 +318,6 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
   __shared__ int rowt[F::ROWS];
   __shared__ float2 cta_ml[F::ROWS];
   __shared__ uint32_t tmem_slot;
-  __shared__ int restart[SUBS];
   __shared__ int dead;  // a wait gave up
   __shared__ uint8_t bad_row[2][BK];  // fp16: V rows taken out of the last two tiles that hold tree slots
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -395,10 +422,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         gr.c[ln] = ok ? fmaxf(fabsf(a.scale_log2) * (I8 ? 1.f / 4194304.f : 1.f / 8192.f) * pow2(ex), 1e-37f) : __int_as_float(0x7fc00000);
         gr.nm[ln] = ok ? -TA_NONE : 0.f;  // of a row of NaNs any will do
         gr.nx[ln] = 0.f;
-        gr.lv[ln] = I8 ? 120.f : 0.f;
-        gr.vs[ln] = I8 ? TA_VMOST : 1.f;
-        gr.fo[ln] = gr.fl[ln] = 1.f;
-        if (ln % NH == 0) gr.lv_top[ln / NH] = I8 ? 120.f : 0.f, gr.lv_same[ln / NH] = gr.none[ln / NH] = 1;
+        if (ln % NH == 0) gr.none[ln / NH] = 1;
         rowt[n] = rt[i];
       }
       uint8_t* q = smem + F::Q_OFF + sub * F::QB;
@@ -510,7 +534,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
         wait(&bars.p_full[u], i);
         if (!ok) break;
         fence_after();
-        const uint32_t keep = *reinterpret_cast<volatile int*>(&restart[u]) == 0;
+        const uint32_t keep = i % F::PERIOD != 0;
         if (elect_one()) {
           const uint64_t vd = vd0 + (uint32_t)(slot * (F::TILE >> 4));
           constexpr int KS = I8 ? 4 : 8, KB = BK / KS * 128;  // bytes of 32 or 16 positions
@@ -549,36 +573,44 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       dk_next = __ldcg(ks + key), dv_next = __ldcg(vsc + key);
     };
     if (I8 && nb) request(0);
-    // O's sums so far, out of tensor memory
-    auto flush = [&](int i, bool moved) {
-      if (i) {
-        if (!mbar_wait(&bars.pv_done[sub], (i - 1) & 1, err, ERR_TREE_WAIT)) dead = 1;
-        __syncwarp();
-        fence_after();
+    auto wait_pv = [&](int i) {  // O holds the products of the blocks before i
+      if (!mbar_wait(&bars.pv_done[sub], (i - 1) & 1, err, ERR_TREE_WAIT)) dead = 1;
+      __syncwarp();
+      fence_after();
+    };
+    // O's sums so far of eight rows from c0 on, out of tensor memory.  `only`: of the
+    // rows with a bit there (the same for all threads), whose sums then go on from 0.
+    auto take = [&](int c0, auto only, unsigned rows) {
+      constexpr bool all = !decltype(only)::value;
+      if (I8) {  // two low digits of each row, then, 64 columns on, two high ones
+        uint32_t r[2][16];
+        ld_digits(r, o_tm + h0 + 2 * c0, 2 * NT);
 #pragma unroll
-        for (int c0 = 0; c0 < NH; c0 += 8) {
-          if (I8) {  // two low digits of each row, then, 64 columns on, two high ones
-            uint32_t r[2][16];
-            ld_digits(r, o_tm + h0 + 2 * c0, 2 * NT);
-#pragma unroll
-            for (int n = 0; n < 8; ++n)
-              facc[c0 + n] += fmaf((float)(int)r[1][2 * n + 1], 16777216.f,
-                                   fmaf((float)(int)r[1][2 * n], 65536.f, fmaf((float)(int)r[0][2 * n + 1], 256.f, (float)(int)r[0][2 * n])));
-          } else {
-            uint32_t r[2][8];
-            ld_digits(r, o_tm + c0, NT);
-#pragma unroll
-            for (int n = 0; n < 8; ++n) facc[c0 + n] += __uint_as_float(r[0][n]) + __uint_as_float(r[1][n]);
+        for (int n = 0; n < 8; ++n) {
+          const float x = fmaf((float)(int)r[1][2 * n + 1], 16777216.f,
+                               fmaf((float)(int)r[1][2 * n], 65536.f, fmaf((float)(int)r[0][2 * n + 1], 256.f, (float)(int)r[0][2 * n])));
+          if (all || ((rows >> n) & 1u)) {
+            facc[c0 + n] += x;
+            r[0][2 * n] = r[0][2 * n + 1] = r[1][2 * n] = r[1][2 * n + 1] = 0;
           }
         }
-        fence_before();
-      }
-      if (moved)
+        if (!all) st_digits(r, o_tm + h0 + 2 * c0, 2 * NT);
+      } else {
+        uint32_t r[2][8];
+        ld_digits(r, o_tm + c0, NT);
 #pragma unroll
-        for (int n = 0; n < NH; ++n) {
-          facc[n] *= gr.fo[h0 + n];
-          (n & 1 ? l2[n / 2].y : l2[n / 2].x) *= gr.fl[h0 + n];
-        }
+        for (int n = 0; n < 8; ++n)
+          if (all || ((rows >> n) & 1u)) {
+            facc[c0 + n] += fmaf(__uint_as_float(r[1][n]), P_LOW, __uint_as_float(r[0][n]));
+            r[0][n] = r[1][n] = 0;
+          }
+        if (!all) st_digits(r, o_tm + c0, NT);
+      }
+    };
+    auto take_all = [&]() {
+#pragma unroll
+      for (int c0 = 0; c0 < NH; c0 += 8) take(c0, std::false_type(), 0);
+      fence_before();
     };
     // which of the warp's 32 positions lane n's row sees; of this CTA's first
     // block that needs it, asked for now
@@ -587,7 +619,11 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
     };
     const int b0 = min(pos, len) / BK, first_edge = pos <= 0 || b0 <= split ? 0 : (b0 - split + stride - 1) / stride;
     const uint32_t first_sees = first_edge < nb ? row_sees(first_edge) : 0u;
-    int since = 0, edges = 0;
+    // int8: what a weight's integer part is taken after adding; spread over 0 .. 1
+    // by the golden ratio from position to position, so that weights below a unit
+    // are kept in the mean
+    const float dither = (float)((unsigned)kl * 0x9E3779B9u >> 9) * 0x1p-23f;
+    int edges = 0;
     for (int i = 0; i < nb; ++i) {
       const int p0 = (split + i * stride) * BK, key = p0 + kl;
       if (I8) {
@@ -671,120 +707,98 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           else if (!I8 && bad) x = nan;
         }
       }
-      // does a weight leave its range?  int8: digits hold weight * scale * vs
-      // below 2^32 (lv_top is the bound of every row's vs)
-      constexpr float TOP = I8 ? 31.f : 15.f;
-      const float ldv = I8 ? __log2f(dvv) : 0.f;
+      // does a weight leave its range?  (A scale near 0 stands for 2^-64, so that
+      // a key whose values are nothing moves no reference, and overflows none.)
+      const float ldv = I8 ? __log2f(fmaxf(dvv, 0x1p-64f)) : 0.f;
       float top = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NH / 2; ++n) top = fmaxf(top, fmaxf(x2[n].x, x2[n].y));
-      if (I8) top += fmaxf(-29.f, ldv + gr.lv_top[half]);
+      top += ldv;
       if (!ok) dead = 1;
-      bool fresh = i == 0;
-      if (group_any(bar, GT, top > TOP || gr.none[half] || !ok)) {
+      const bool fresh = i % F::PERIOD == 0;  // O starts again
+      bool drained = false;
+      if (group_any(bar, GT, top > F::P_TOP || gr.none[half] || !ok)) {
         if (group_any(bar, GT, *reinterpret_cast<volatile int*>(&dead) != 0)) break;
-        // Lane n (of 16 rows, and n + 16) gets the largest score of row n among the
-        // warp's positions, and the largest scale of V among those that it sees.
-#pragma unroll
-        for (int n = 0; n < NH / 2; ++n)  // without the reference; the new one is added below
-          x2[n] = __fadd2_rn(x2[n], make_float2(-gr.nx[h0 + 2 * n], -gr.nx[h0 + 2 * n + 1]));
+        // Lane n (of 16 rows, and n + 16) gets row n's largest weight among the
+        // warp's positions.
         const float mx = lane_max<NH>([&](int n) {
-          const float x = n & 1 ? x2[n / 2].y : x2[n / 2].x;
+          const float x = (n & 1 ? x2[n / 2].y : x2[n / 2].x) + ldv;
           return x == x ? x : -INFINITY;
         });
-        float dm = 0.f;
-        if (I8) {
-          if (edge)
-            dm = lane_max<NH>([&](int n) { return (vis >> n) & 1u ? dvv : 0.f; });
-          else
-            dm = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(dvv)));
-        }
-        if (lane < NH) gr.mx[wq][h0 + lane] = mx, gr.dm[wq][h0 + lane] = dm;
+        if (lane < NH) gr.mx[wq][h0 + lane] = mx;
         group_sync(bar, GT);
         if (wq == 0) {
+          bool scaled = false, none = false;
           if (lane < NH) {
             const int n = h0 + lane;
-            float fo = 1.f, fl = 1.f;
-            const float top = fmaxf(fmaxf(gr.mx[0][n], gr.mx[1][n]), fmaxf(gr.mx[2][n], gr.mx[3][n]));
-            const float d = fmaxf(fmaxf(gr.dm[0][n], gr.dm[1][n]), fmaxf(gr.dm[2][n], gr.dm[3][n]));
-            // each row by itself: moved if its own largest weight and scale may leave the range
-            if (top + gr.nm[n] + (I8 ? fmaxf(-29.f, __log2f(d) + gr.lv[n]) : 0.f) > TOP) {
-              // fp16: the largest weight becomes 2^4, so that the low halves reach 2^-28 of it
-              const float mn = fmaxf(-gr.nm[n], top - (I8 ? 0.f : 4.f));
-              fo = fl = ex2(-gr.nm[n] - mn);
-              gr.nm[n] = -mn;
-              if (I8) {
-                const int ex = max((int)(__float_as_uint(d) >> 23) - 126, -96);  // a power of two above the largest scale
-                if (d > 0.f && (float)(24 - ex) < gr.lv[n]) {
-                  const float nv = pow2(24 - ex);
-                  fo *= nv / gr.vs[n];
-                  gr.vs[n] = nv;
-                  gr.lv[n] = (float)(24 - ex);
-                }
-              }
+            const float m = fmaxf(fmaxf(gr.mx[0][n], gr.mx[1][n]), fmaxf(gr.mx[2][n], gr.mx[3][n]));
+            float dx = 0.f, fo = 1.f;
+            none = gr.nm[n] == -TA_NONE;
+            if (m > (none ? -INFINITY : F::P_TOP)) {  // each row by itself
+              const float from = none ? 0.f : gr.nm[n], to = from + (F::P_UNIT - ceilf(m));
+              dx = to - from;
+              scaled = !none;
+              if (scaled) fo = dx < -126.f ? 0.f : pow2((int)dx);
+              gr.nm[n] = gr.nx[n] = to;
+              none = false;
             }
-            gr.fo[n] = fo, gr.fl[n] = fl;
-            gr.nx[n] = gr.nm[n] == -TA_NONE ? 0.f : gr.nm[n];
+            gr.dx[n] = dx, gr.fo[n] = fo;
           }
-          const bool none = __any_sync(0xffffffffu, lane < NH && gr.nm[h0 + lane % NH] == -TA_NONE);
-          if (lane == 0) gr.none[half] = none;
-          __syncwarp();
-          if (I8) {
-            float hi = gr.lv[h0 + lane % NH], lo = hi;
-#pragma unroll
-            for (int x = 16; x; x >>= 1) {
-              hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, x));
-              lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, x));
-            }
-            if (lane == 0) gr.lv_top[half] = hi, gr.lv_same[half] = hi == lo;
-          }
+          none = __any_sync(0xffffffffu, none);
+          const unsigned rows = __ballot_sync(0xffffffffu, scaled);
+          if (lane == 0) gr.none[half] = none, gr.scaled[half] = rows;
         }
         group_sync(bar, GT);
 #pragma unroll
-        for (int n = 0; n < NH / 2; ++n) x2[n] = __fadd2_rn(x2[n], *reinterpret_cast<const float2*>(&gr.nx[h0 + 2 * n]));
-        flush(i, true);
-        fresh = true;
-      } else if (since >= F::PERIOD) {
-        flush(i, false);
-        fresh = true;
-      }
-      since = fresh ? 1 : since + 1;
-      // weights, as digits, into the operand tile
-      if (i && !mbar_wait(&bars.pv_done[sub], (i - 1) & 1, err, ERR_TREE_WAIT)) dead = 1;
-      if (I8) {
-        // one factor for all rows as long as each has met the same largest scale (a
-        // choice made per value, by selects, took 85 instructions of 800 per block)
-        auto digits = [&](auto uniform) {
-          // finite, so that a weight of 0 (a slot not seen) stays 0 whatever its scale
-          const float dvs = fminf(dvv * gr.vs[h0], TA_FINITE);
+        for (int n = 0; n < NH / 2; ++n) x2[n] = __fadd2_rn(x2[n], *reinterpret_cast<const float2*>(&gr.dx[h0 + 2 * n]));
+        const unsigned rows = gr.scaled[half];
+        if (rows) {
+          if (i) wait_pv(i);
+          if (i && fresh) take_all();
+          drained = true;
 #pragma unroll
-          for (int r0 = 0; r0 < NH; r0 += 8) {  // a 16-byte piece of low digits, one of high
-            uint32_t lw[4], hw[4];
+          for (int c0 = 0; c0 < NH; c0 += 8) {
+            const unsigned some = (rows >> c0) & 0xffu;
+            if (!some) continue;
+            if (!fresh) take(c0, std::true_type(), some);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int n = r0 / 2 + e;
-              float2 f = f2(dvs);
-              if (!uniform) {
-                const float2 vs = *reinterpret_cast<const float2*>(&gr.vs[h0 + 2 * n]);
-                f = make_float2(fminf(dvv * vs.x, TA_FINITE), fminf(dvv * vs.y, TA_FINITE));
-              }
-              const float2 p = make_float2(ex2(x2[n].x), ex2(x2[n].y));
-              l2[n] = __fadd2_rn(l2[n], p);
-              const float2 y = __ffma2_rn(p, f, f2(0.5f));  // 0.5 .. 2^32: its integer part is the weight
-              const float2 hi = __ffma2_rz(y, f2(0x1p-16f), f2(0x1p23f));
-              // y - 65536 * (hi - 2^23) + 2^23; all but the last rounding is exact
-              const float2 lo = __fadd2_rz(y, __ffma2_rn(hi, f2(-65536.f), f2(0x1p39f + 0x1p23f)));
-              lw[e] = __byte_perm(__float_as_uint(lo.x), __float_as_uint(lo.y), 0x5410u);
-              hw[e] = __byte_perm(__float_as_uint(hi.x), __float_as_uint(hi.y), 0x5410u);
+            for (int n = 0; n < 8; ++n) {
+              const float f = gr.fo[h0 + c0 + n];
+              facc[c0 + n] *= f;
+              (n & 1 ? l2[(c0 + n) / 2].y : l2[(c0 + n) / 2].x) *= f;
             }
-            *reinterpret_cast<uint4*>(prow + ((((h0 + r0) / 8) ^ psw) << 4)) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-            *reinterpret_cast<uint4*>(prow + (((4 + (h0 + r0) / 8) ^ psw) << 4)) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
           }
-        };
-        if (gr.lv_same[half])
-          digits(std::true_type());
-        else
-          digits(std::false_type());
+          fence_before();
+        }
+      }
+      if (i && !drained) {
+        if (fresh) {
+          wait_pv(i);
+          take_all();
+        } else if (!mbar_wait(&bars.pv_done[sub], (i - 1) & 1, err, ERR_TREE_WAIT)) {
+          dead = 1;
+        }
+      }
+      // weights into the operand tile
+      if (I8) {
+#pragma unroll
+        for (int r0 = 0; r0 < NH; r0 += 8) {  // a 16-byte piece of low digits, one of high
+          uint32_t lw[4], hw[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int n = r0 / 2 + e;
+            const float2 p = make_float2(ex2(x2[n].x), ex2(x2[n].y));
+            l2[n] = __fadd2_rn(l2[n], p);
+            const float2 y = __ffma2_rn(p, f2(dvv), f2(dither));  // below 2^32: its integer part is the weight
+            const float2 hi = __ffma2_rz(y, f2(0x1p-16f), f2(0x1p23f));
+            // y - 65536 * (hi - 2^23) + 2^23; all but the last rounding is exact
+            const float2 lo = __fadd2_rz(y, __ffma2_rn(hi, f2(-65536.f), f2(0x1p39f + 0x1p23f)));
+            lw[e] = __byte_perm(__float_as_uint(lo.x), __float_as_uint(lo.y), 0x5410u);
+            hw[e] = __byte_perm(__float_as_uint(hi.x), __float_as_uint(hi.y), 0x5410u);
+          }
+          *reinterpret_cast<uint4*>(prow + ((((h0 + r0) / 8) ^ psw) << 4)) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+          *reinterpret_cast<uint4*>(prow + (((4 + (h0 + r0) / 8) ^ psw) << 4)) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+        }
       } else {
 #pragma unroll
         for (int c0 = 0; c0 < NH / 8; ++c0) {  // eight rows: one 16-byte piece of high halves, one of low
@@ -795,7 +809,7 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
             const float2 p = make_float2(ex2(x2[n].x), ex2(x2[n].y));
             l2[n] = __fadd2_rn(l2[n], p);
             const __half2 t = __floats2half2_rn(p.x, p.y);
-            const float2 d = __ffma2_rn(__half22float2(t), f2(-1.f), p);
+            const float2 d = __fmul2_rn(__ffma2_rn(__half22float2(t), f2(-1.f), p), f2(1.f / P_LOW));  // exact
             hi[e] = h2u(t);
             lo[e] = h2u(__floats2half2_rn(d.x, d.y));
           }
@@ -803,18 +817,19 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
           *reinterpret_cast<uint4*>(prow + (((4 + h0 / 8 + c0) ^ psw) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
       }
-      if (kl == 0 && half == 0) *reinterpret_cast<volatile int*>(&restart[sub]) = fresh;
       fence_proxy_async_smem();
       fence_before();
       mbar_arrive(&bars.p_full[sub]);
     }
-    if (nb) flush(nb, false);
+    if (nb) {
+      wait_pv(nb);
+      take_all();
+    }
     // O and the sums of this group's rows, in its own P tile
     float* fold = reinterpret_cast<float*>(smem + F::P_OFF);  // [row][HD]
     static_assert(F::PB == NT * HD * 4, "a group's rows fill its P tile");
 #pragma unroll
-    for (int n = 0; n < NH; ++n)  // 1 / vs is a power of two
-      fold[(sub * NT + h0 + n) * HD + kl] = facc[n] * (1.f / gr.vs[h0 + n]);
+    for (int n = 0; n < NH; ++n) fold[(sub * NT + h0 + n) * HD + kl] = facc[n];
     // sums over the group's 128 positions: after the exchanges lane n (of 16
     // rows, and n + 16) of a warp holds row n's
     float l[NH];

@@ -78,6 +78,89 @@ def test_nonfinite_rows_reach_all_of_who_sees_them(dr, dt, bad, which, hd, H, KV
     assert vis[:, j].any() and not vis[:, j].all() and np.array_equal(got[~vis[:, j]], clean[~vis[:, j]])
 
 
+@pytest.mark.parametrize("hd,H,KV,ctx,T", SHAPES)
+@pytest.mark.parametrize("big", [1e27, 3e38])
+def test_a_large_scale_of_no_weight(dr, hd, H, KV, ctx, T, big):  # noqa: F811
+    """A row that all see, of any finite V scale, whose weight is below 2^-150 (0
+    in fp32): nobody's outputs change, nor the bits that other rows keep."""
+    rng = np.random.default_rng(15)
+    pos, j = 150, 100
+    c = dr.KVCache.new("i8", KV, hd, ctx)
+    fill(c, rng, 0, pos + T)
+    q = dev(np.abs(rng.standard_normal((T, H * hd))).astype(np.float32) + 0.5)
+    c.k[:KV * ctx * hd].view(KV, ctx, hd)[:, j] = 256 - 127  # codes of -127: scores of -0.1 * 4 * 127 * 64 * 0.5 and below
+    scales(c, c.k)[:, j] = 4.0
+    kw = dict(heads=H, scale=0.1, scratch=dr.attention_tree_scratch(c, T, H))
+    before = dr.attention_tree(q, c, None, state(pos), **kw).cpu().numpy()
+    scales(c, c.v)[:, j] = big
+    after = dr.attention_tree(q, c, None, state(pos), **kw).cpu().numpy()
+    assert np.isfinite(before).all() and np.array_equal(before, after)
+
+
+def attend64_gpu(q, k, v, pos, scale):
+    """q [T, H, hd], k and v [KV, pos + T, hd], float64 on the GPU, a chain."""
+    import torch
+
+    T, H, hd = q.shape
+    KV, n = k.shape[:2]
+    vis = torch.arange(n, device="cuda")[None] <= pos + torch.arange(T, device="cuda")[:, None]
+    out = torch.empty_like(q)
+    for h in range(KV):
+        g = slice(h * (H // KV), (h + 1) * (H // KV))
+        s = torch.einsum("tgd,nd->tgn", q[:, g], k[h]) * scale
+        out[:, g] = torch.einsum("tgn,nd->tgd", torch.softmax(s.masked_fill(~vis[:, None], -np.inf), -1), v[h])
+    return out
+
+
+@pytest.mark.parametrize("dt", ["f16", "i8"])
+@pytest.mark.parametrize("hd,H,KV,T", [(128, 8, 1, 1), (128, 32, 4, 2), (128, 8, 1, 64), (64, 8, 2, 13)])
+@pytest.mark.parametrize("at", [0, 20001])
+@pytest.mark.parametrize("gap", [6, 10, 14, 18])
+def test_one_key_outweighs_all(dr, dt, hd, H, KV, T, at, gap):  # noqa: F811
+    """One key `gap` nats above the mean of 30,000 others (in real models the first
+    position is one), its values ordinary, small or 0, the others' with and
+    without a mean.  The 2-norm is held to 1e-5, as for ordinary scores.
+
+    A weight of an fp16 cache enters to within half of fp16's last 2^-24, against a
+    largest of more than 2^11: 2^-36 of the key's.  Where that key's values are 0
+    this is not small against the output: N such roundings, each of its own sign,
+    of values of size 1."""
+    import torch
+
+    rng = np.random.default_rng(17 * gap + T)
+    n, ctx, scale = 30_000, 30_100, hd ** -0.5
+    pos = n - T
+    k0, v0 = rng.standard_normal((2, KV, n, hd))
+    q = rng.standard_normal((T, H, hd))
+    q[..., 5], k0[..., 5] = 4.0, 0.0
+    k0[:, at], k0[:, at, 5] = 0.0, gap / (4.0 * scale)
+    qd = dev(q.astype(np.float32))
+    c = dr.KVCache.new(dt, KV, hd, ctx)
+    scr = dr.attention_tree_scratch(c, T, H)
+    for size, mean in ((1.0, 0.0), (0.02, 0.0), (0.02, 0.5), (1.0, 0.5), (0.0, 0.0)):
+        v = v0 + mean
+        v[:, at] *= size
+        rows = []
+        for half, x in ((c.k, k0), (c.v, v)):
+            x = torch.from_numpy(x).cuda()
+            if dt == "f16":
+                half[:, :n] = x.half()
+                rows.append(half[:, :n].double())
+            else:
+                d = (x.abs().amax(-1, keepdim=True) / 127).float()
+                codes = torch.round(x / torch.where(d > 0, d, 1.0).double())
+                half[:KV * ctx * hd].view(torch.int8).view(KV, ctx, hd)[:, :n] = codes.to(torch.int8)
+                scales(c, half)[:, :n] = d[..., 0]
+                rows.append(codes * d.double())
+        out = dr.attention_tree(qd.view(T, -1), c, None, state(pos), heads=H, scale=scale, scratch=scr)
+        ref = attend64_gpu(qd.double(), *rows, pos, scale)
+        err, norm = float((out.view(T, H, hd).double() - ref).norm()), float(ref.norm())
+        tol = 1e-5 * norm
+        if dt == "f16" and size == 0.0:
+            tol += 2.0 ** -36 * (n * ref.numel()) ** 0.5
+        assert err <= tol, (size, mean, err / norm, tol / norm)
+
+
 # ---- streams ---------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("op", ["append", "read", "attention"])
