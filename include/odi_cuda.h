@@ -480,7 +480,8 @@ int odi_cuda_kv_move(const odi_cuda_kv_cache* cache, const int32_t* d_src, const
  * of itself or 2^-25 of the largest, whichever is more; of an fp16 cache, q to
  * within 2^-22 of each value, and weights to within 2^-22 of themselves or 2^-36
  * of the largest (a key with nearly all the weight and values of 0 leaves the
- * others at that).  d_scratch: as for odi_cuda_attention_decode (16-byte
+ * others at that).  Calls are repeatable bit for bit, and a node's outputs do
+ * not depend on the other nodes' queries.  d_scratch: as for odi_cuda_attention_decode (16-byte
  * aligned, zero before its first use, left reusable, calls on one stream only;
  * its first int is the error word, odi_cuda_workspace_status); its size depends
  * on head_dim alone, and calls of different shapes may share it.  int8 rows' scales are not negative. */

@@ -36,7 +36,7 @@
 // range, by whole powers of two.  Only the row that moves takes its O out of
 // tensor memory then, to fp32 registers; all rows do every few blocks, always
 // the same ones (integer sums cannot overflow so, and fp32 sums, which truncate,
-// stay short).
+// stay short): a row's bits do not depend on the rows beside it.
 //
 // The softmax bounds the kernel: 17 instructions per score (packed fp32 pairs
 // where two scores share an operation), of which two warps per scheduler issue

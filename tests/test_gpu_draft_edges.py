@@ -161,6 +161,25 @@ def test_one_key_outweighs_all(dr, dt, hd, H, KV, T, at, gap):  # noqa: F811
         assert err <= tol, (size, mean, err / norm, tol / norm)
 
 
+@pytest.mark.parametrize("dt", ["f16", "i8"])
+@pytest.mark.parametrize("hd,H,KV,T,n", [(128, 8, 8, 7, 5000), (128, 32, 8, 8, 30000), (128, 64, 8, 64, 9000), (64, 8, 1, 9, 6000)])
+def test_rows_do_not_depend_on_each_other(dr, dt, hd, H, KV, T, n):  # noqa: F811
+    """Every other node's queries are other ones, of other sizes: the bits of the
+    nodes between them stay, over many blocks of positions per CTA."""
+    rng = np.random.default_rng(23)
+    c = dr.KVCache.new(dt, KV, hd, n + 64)
+    fill(c, rng, 0, n + T)
+    q = (1.7 * rng.standard_normal((T, H * hd))).astype(np.float32)
+    kw = dict(heads=H, scale=hd ** -0.5, scratch=dr.attention_tree_scratch(c, T, H))
+    want = dr.attention_tree(dev(q), c, None, state(n), **kw).cpu().numpy()
+    for size in (0.0, 6.0, 40.0, np.nan):
+        other = q.copy()
+        other[1::2] = size * rng.standard_normal((T // 2, H * hd))
+        got = dr.attention_tree(dev(other), c, None, state(n), **kw).cpu().numpy()
+        assert np.array_equal(got[::2], want[::2])
+        assert not np.array_equal(got[1::2], want[1::2])
+
+
 # ---- streams ---------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("op", ["append", "read", "attention"])
