@@ -220,10 +220,9 @@ __global__ void __launch_bounds__(TA_THREADS, NR == 1 ? 4 : NR == 2 ? 3 : 2) tre
       int ex = (int)(__float_as_uint(am) >> 23) - 127;  // am = 1 .. 2 times 2^ex
       if (I8 && am * pow2(-min(max(ex, -100), 126)) > 1.99f) ++ex;
       ex = min(max(ex, -100), 126);
-      const float lift = pow2(-ex), up = I8 ? 4194304.f : 8192.f;
+      const float lift = pow2(-ex), up = I8 ? q_units(am) : 8192.f;
       if (lane == 0) {
-        // 1 / up and 2^ex are exact; together they may leave the range, so one after the other
-        rowc[n] = ok ? a.scale_log2 * (1.f / up) * pow2(ex) : __int_as_float(0x7fc00000);
+        rowc[n] = ok ? q_factor(a.scale_log2, 1.f / up, ex) : __int_as_float(0x7fc00000);
         rowt[n] = rt[i];
       }
       uint8_t* dst = reinterpret_cast<uint8_t*>(qf) + (n >> 3) * QW * 128;

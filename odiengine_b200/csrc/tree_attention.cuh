@@ -74,6 +74,13 @@ __device__ __forceinline__ int row_node(const TreeArgs& a, int r) {
   return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.inv_G);
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 .. 127
+// What a q row of largest value am, brought to 1 .. 1.99, is multiplied by for three
+// signed digits; rows past 1.99 * 2^126 can only be brought to 1.99 .. 4.
+__device__ __forceinline__ float q_units(float am) { return am > 1.99f * 0x1p126f ? 1048576.f : 4194304.f; }
+// scale * inv_unit * 2^ex, in the order that stays in fp32's normal range.
+__device__ __forceinline__ float q_factor(float scale, float inv_unit, int ex) {
+  return ex > 0 ? scale * pow2(ex) * inv_unit : scale * inv_unit * pow2(ex);
+}
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // Which of positions p0 .. p0 + 31 node t sees (t < 0: a row past the last, none).

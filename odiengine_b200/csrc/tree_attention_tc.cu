@@ -416,10 +416,10 @@ __global__ void __launch_bounds__(Cfg<I8, SUBS>::THREADS, 1)
       int ex = (int)(__float_as_uint(am) >> 23) - 127;
       if (I8 && am * pow2(-min(max(ex, -100), 126)) > 1.99f) ++ex;
       ex = min(max(ex, -100), 126);
-      const float lift = ok ? pow2(-ex) : 0.f, up = (I8 ? 4194304.f : 8192.f) * sign;
+      const float lift = ok ? pow2(-ex) : 0.f, unit = I8 ? q_units(am) : 8192.f, up = unit * sign;
       if (l8 == 0) {
         Group& gr = groups[sub];
-        gr.c[ln] = ok ? fmaxf(fabsf(a.scale_log2) * (I8 ? 1.f / 4194304.f : 1.f / 8192.f) * pow2(ex), 1e-37f) : __int_as_float(0x7fc00000);
+        gr.c[ln] = ok ? fmaxf(q_factor(fabsf(a.scale_log2), 1.f / unit, ex), 1e-37f) : __int_as_float(0x7fc00000);
         gr.nm[ln] = ok ? -TA_NONE : 0.f;  // of a row of NaNs any will do
         gr.nx[ln] = 0.f;
         if (ln % NH == 0) gr.none[ln / NH] = 1;

@@ -97,6 +97,31 @@ def test_a_large_scale_of_no_weight(dr, hd, H, KV, ctx, T, big):  # noqa: F811
     assert np.isfinite(before).all() and np.array_equal(before, after)
 
 
+@pytest.mark.parametrize("dt", ["f16", "i8"])
+@pytest.mark.parametrize("hd,H,KV,ctx,T", SHAPES)
+@pytest.mark.parametrize("size", [1e38, 3.4e38])
+def test_queries_of_any_finite_size(dr, dt, hd, H, KV, ctx, T, size):  # noqa: F811
+    """Queries up to fp32's largest, with a scale that brings the scores back: q
+    enters to within 2^-20 (int8; 2^-22 fp16) of its largest value, so a score of
+    hd such products is off by at most hd 2^-20 of the largest, and the rest as in
+    test_gpu_draft."""
+    rng = np.random.default_rng(31)
+    pos = 150
+    c = dr.KVCache.new(dt, KV, hd, ctx)
+    fill(c, rng, 0, pos + T)
+    q = rng.uniform(-1, 1, (T, H, hd))
+    q /= np.abs(q).max(-1, keepdims=True)
+    q = (q * size).astype(np.float32)
+    scale = 0.2 / size
+    vis = random_tree(rng, T)
+    out = dr.attention_tree(dev(q.reshape(T, -1)), c, None, state(pos), heads=H, scale=scale, mask=dev(words(vis)),
+                            scratch=dr.attention_tree_scratch(c, T, H)).cpu().numpy().reshape(T, H, hd)
+    K, V = values64(c)
+    ref, S = attend64(q.astype(np.float64), K, V, vis, pos, float(np.float32(scale)))
+    ds = hd * 2.0 ** -24 * S + 0.2 * hd * 2.0 ** -20 * np.abs(K).max()
+    assert (np.abs(out - ref) <= 2 * (ds + 8 * 2.0 ** -24)[..., None] * np.abs(V).max()).all()
+
+
 def attend64_gpu(q, k, v, pos, scale):
     """q [T, H, hd], k and v [KV, pos + T, hd], float64 on the GPU, a chain."""
     import torch
