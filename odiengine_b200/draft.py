@@ -134,6 +134,10 @@ class KVCache:
                 _refuse(t, want, f"cache {n}", k.get_device(), f"{need} contiguous bytes")
             if t.data_ptr() % 16:
                 raise ValueError(f"cache {n}: must be 16-byte aligned")
+            if dtype == "f16" and t.dim() == 3 and tuple(t.shape) != (kv_heads, ctx, head_dim):
+                raise ValueError(f"cache {n}: [{kv_heads}, {ctx}, {head_dim}] wanted, got {tuple(t.shape)}")
+        if abs(k.data_ptr() - v.data_ptr()) < need:
+            raise ValueError("cache: k and v share memory")
         self.k, self.v, self.dtype = k, v, dtype
         self.kv_heads, self.head_dim, self.ctx = kv_heads, head_dim, ctx
         self.device, self.index = k.device, k.get_device()

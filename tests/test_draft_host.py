@@ -10,6 +10,8 @@ from odiengine_b200 import draft
 class OnGpu:
     """A CPU tensor that passes for one of cuda:0 (its memory is never followed)."""
 
+    is_cuda = True
+
     def __init__(self, t):
         self.t = t
 
@@ -59,6 +61,37 @@ def test_rows_that_overlap_are_not_one_row(calls, what, width):
     with pytest.raises(ValueError):
         logits_opts(calls, **{what: OnGpu(full[:3])})
     assert len(calls) == n
+
+
+# ---- caches ----------------------------------------------------------------------------------------------------
+
+def aligned(n, dtype):
+    """n values from a 16-byte boundary on."""
+    t = torch.zeros(n + 16, dtype=dtype)
+    return t[(-t.data_ptr() % 16) // t.element_size():][:n]
+
+
+def test_cache_halves_that_do_not_fit_are_refused():
+    """K and V in one memory, and an fp16 tensor of another cache's shape (its
+    heads would be read from other places than it has them)."""
+    f16, n = torch.float16, 2 * 8 * 64
+    buf = aligned(3 * n, f16)
+    k, v = buf[:n].view(2, 8, 64), buf[n:2 * n].view(2, 8, 64)
+    c = draft.KVCache(OnGpu(k), OnGpu(v), "f16", 2, 64, 8)
+    assert (c._struct.k, c._struct.v) == (k.data_ptr(), v.data_ptr())
+    draft.KVCache(OnGpu(buf[:n]), OnGpu(buf[n:]), "f16", 2, 64, 8)  # flat, and longer than it has to be
+    for other in (k, buf[n - 8:2 * n - 8].view(2, 8, 64)):
+        with pytest.raises(ValueError, match="share"):
+            draft.KVCache(OnGpu(k), OnGpu(other), "f16", 2, 64, 8)
+    with pytest.raises(ValueError, match="wanted"):
+        draft.KVCache(OnGpu(buf[:n].view(2, 8, 64)), OnGpu(buf[n:2 * n].view(8, 2, 64)), "f16", 2, 64, 8)
+    with pytest.raises(ValueError, match="wanted"):
+        draft.KVCache(OnGpu(buf[:n].view(2, 8, 64)), OnGpu(v), "f16", 2, 64, 4)
+    need = draft.kv_cache_bytes("i8", 2, 64, 8)
+    u8 = aligned(2 * need, torch.uint8)
+    draft.KVCache(OnGpu(u8[:need]), OnGpu(u8[need:]), "i8", 2, 64, 8)
+    with pytest.raises(ValueError, match="share"):
+        draft.KVCache(OnGpu(u8[:need]), OnGpu(u8[16:need + 16]), "i8", 2, 64, 8)
 
 
 # ---- sequences -------------------------------------------------------------------------------------------------
