@@ -290,6 +290,10 @@ def logits_adjust(logits, out=None, tokens=None, *, scratch=None, history=None, 
     return out, tokens
 
 
+# what verify hands on to logits_adjust
+_VERIFY_ADJUST = {"repeat_penalty", "frequency_penalty", "presence_penalty", "bias_ids", "bias", "mask"}
+
+
 class DraftVerifier:
     """Greedy decoding of one sequence that checks drafted tokens, a tree of
     them per step: the model of decode.DecodeModel (its fused step, for T
@@ -401,7 +405,12 @@ class DraftVerifier:
         the greedy tokens along the accepted path: one, plus one for every
         drafted token on it.  The last returned token is pending (not in the
         cache).  adjust: logits_adjust's penalties, biases and mask (mask rows
-        per node, or one)."""
+        per node, or one); without a history of the verifier's own also its
+        history and history_lens."""
+        other = set(adjust) - _VERIFY_ADJUST - (set() if self.history else {"history", "history_lens"})
+        if other:
+            raise TypeError(f"verify: no argument {', '.join(sorted(other))}" +
+                            (" (the verifier counts its own history)" if self.history else ""))
         T = 1 + len(drafted)
         parents = list(range(T - 1)) if parents is None else list(parents)
         if self.pending is None:

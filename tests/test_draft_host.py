@@ -132,6 +132,20 @@ def test_a_prompt_that_failed_leaves_no_sequence(verifier, monkeypatch, where):
     assert verifier.pending == 8 and verifier.tokens == [7, 8]
 
 
+def test_verify_takes_what_adjusts_the_logits_only(verifier):
+    """Another stream, other outputs, or a history beside the verifier's own
+    would be ordered or counted wrongly: refused before anything runs."""
+    verifier.start([1, 2, 3])
+    for bad in (dict(stream=None), dict(out=None), dict(tokens=None), dict(scratch=None), dict(penalty=1.1)):
+        with pytest.raises(TypeError, match=next(iter(bad))):
+            verifier.verify(**bad)
+    verifier.history = 8
+    for bad in (dict(history=z(1, 3, dtype=torch.int32)), dict(history_lens=z(1, dtype=torch.int32))):
+        with pytest.raises(TypeError, match="history"):
+            verifier.verify(**bad)
+    assert verifier.pending == 3 and verifier.pos == 2
+
+
 # ---- arguments left out ----------------------------------------------------------------------------------------
 
 def test_what_is_missing_is_named(calls):
