@@ -50,17 +50,17 @@ namespace {
 // to within 2^-25, 2^-33 (2^-37) of the largest.
 //
 // Bound by the fetch of the cache for long ones: one token, 64 / 8 heads, 131001
-// int8 positions 59 us, 277 MB at 4.7 TB/s (the copy peak gives 42); 518 fp16
-// positions of 32 / 32 heads take 9.3 us, of which the fetch is 1.3: latency of
+// int8 positions 58.5 us, 277 MB at 4.7 TB/s (the copy peak gives 42); 518 fp16
+// positions of 32 / 32 heads take 9.6 us, of which the fetch is 1.3: latency of
 // launch, first loads and join.
 constexpr int TA_WARPS = 4;
 constexpr int TA_THREADS = 32 * TA_WARPS;
 constexpr int TA_GROUP = 16;
 // Rows per kv head above which (head_dim 128) the tcgen05 kernel runs.  32 / 8
 // heads, 500 / 4000 / 32000 positions, us here and there: 8 rows of int8 5.9 /
-// 11.8 / 21.0 and 8.6 / 11.3 / 24.8, of fp16 6.4 / 13.4 / 33.3 and 8.9 / 11.9 /
-// 28.2; 12 rows of int8 8.5 / 14.1 / 32.2 and 8.7 / 11.6 / 24.9, of fp16 8.6 /
-// 15.8 / 44.7 and 9.0 / 12.1 / 28.5.  The length is not known on the host.
+// 11.8 / 20.9 and 7.3 / 10.4 / 23.1, of fp16 6.5 / 13.5 / 33.4 and 8.1 / 11.2 /
+// 27.5; 12 rows of int8 8.1 / 13.8 / 29.8 and 7.3 / 10.5 / 23.4, of fp16 8.9 /
+// 15.9 / 44.0 and 8.3 / 11.2 / 27.6.  The length is not known on the host.
 constexpr int TA_TC_ROWS = 8;
 constexpr float TA_TOP = 32768.f;            // a weight past this moves the reference
 // log2 of the largest right after that.  An fp16 cache's scales, those of its
@@ -510,10 +510,12 @@ TreePlan tree_plan(int tokens, int heads, int kv_heads, int hd, int ctx) {
   p.most = ((int64_t)ctx + block - 1) / block;
   // A CTA of 32 rows takes 0.98 us per block of 128 positions, one of 64 rows
   // 1.39 and about 3.4 more to start and to join.  32 / 8 heads, us with 32 and
-  // with 64 rows: 52 rows per kv head over 4000 positions 14.6 and 17.3, 16000
-  // 26.1 and 25.7, 32000 41.8 and 37.8; 256 rows over 500 12.4 and 15.0, 2000
-  // 18.2 and 19.7, 4000 24.8 and 23.4, 32000 126 and 88; 96 rows over 32000 (three
-  // tiles against two) 52.6 and 55.6.
+  // with 64 rows, of int8 (fp16): 52 rows per kv head over 4000 positions 13.8 and
+  // 15.0 (14.1 and 15.5), 16000 24.6 and 23.7 (25.7 and 23.6), 32000 39.4 and 35.0
+  // (41.1 and 35.4); 256 rows over 500 11.2 and 12.5 (11.8 and 13.3), 2000 17.3 and
+  // 17.5 (17.6 and 17.7), 4000 24.3 and 22.2 (24.3 and 21.4), 32000 120 and 96.5
+  // (128 and 87); 96 rows over 32000 (three tiles against two) 51.1 and 56.9 (51.9
+  // and 52.8).
   const int64_t t32 = (R + 31) / 32, t64 = (R + 63) / 64;
   const bool narrow = kv_heads * p.most * (98 * t32 - 139 * t64) < 340 * TA_SMS;
   p.rows = p.tc ? (narrow ? 32 : 64) : R <= 8 ? 8 : R <= 16 ? 16 : 32;

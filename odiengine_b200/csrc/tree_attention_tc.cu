@@ -40,7 +40,7 @@
 //
 // The softmax bounds the kernel: 17 instructions per score (packed fp32 pairs
 // where two scores share an operation), of which two warps per scheduler issue
-// one every 2.3 cycles.  64 nodes, 64 / 8 heads, 32641 int8 positions: 185 us (fp16:
+// one every 2.3 cycles.  64 nodes, 64 / 8 heads, 32641 int8 positions: 183 us (fp16:
 // 168), where fetching the cache takes 11 and 69 GFLOP at the fp16 rate 41; the
 // loop without any products took 176 where the whole took 182.  Smaller shares for more warps (16 of 16
 // rows: 212 us, the work per block that does not depend on rows doubles), a vote
@@ -100,8 +100,8 @@ struct Cfg {
   static constexpr int PERIOD = I8 ? 256 : 4;
   // Weights in P, log2: what they stay below, and the largest right after a move.
   // int8: an integer below 2^32, so to within 2^-25 of the largest, either way;
-  // 64 nodes over 32641 positions 185 us, 189 with the largest at 2^24 and the
-  // dither left out, 198 and 207 at 2^27 and 2^29: rows move more often, and a
+  // 64 nodes over 32641 positions 183 us, 198 and 207 with the largest at 2^27 and
+  // 2^29: rows move more often, and a
   // block in which one does costs two.  fp16: to within 2^-37, 2^-43 of the largest.
   static constexpr float P_TOP = I8 ? 31.9f : 15.f, P_UNIT = I8 ? 26.f : 8.f;
   static_assert(SMEM <= 222 * 1024, "shared memory, beside the static part");

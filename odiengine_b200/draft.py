@@ -42,7 +42,7 @@ class _KvCacheStruct(ctypes.Structure):
 
 
 # odi_cuda_logits_opts (include/odi_cuda.h) in native layout: packed bytes take
-# 1 us less of the host than a ctypes structure (a call of one row: 10.1 -> 8.9 us).
+# 1 us less of the host than a ctypes structure (a call of one row: 10.1 -> 9.1 us).
 _LOGITS_OPTS = struct.Struct("@fffPqPiPPiPq")  # a null pointer is 0
 
 
