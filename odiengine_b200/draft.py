@@ -21,6 +21,7 @@ graph.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import struct
 
@@ -306,7 +307,8 @@ class DraftVerifier:
     The weights keep gate|up in [gate | up] order (the SwiGLU prologue reads
     it).  q_norms / k_norms: per-layer head_dim weights of models that norm q
     and k per head.  history: how many of the last tokens (the node's own
-    ancestors included) the penalties of verify count."""
+    ancestors included) the penalties of verify count.  Calls run on the current
+    stream, which may differ from call to call; one at a time."""
 
     def __init__(self, cfg, weights, *, cache: str = "f16", max_nodes: int = 64, history: int = 0, q_norms=None,
                  k_norms=None, norm_eps: float = 1e-6, device=None):
@@ -337,6 +339,21 @@ class DraftVerifier:
         products = [dw for lw in weights.layers for dw in (lw.wqkv, lw.wo, lw.wgu, lw.wdown)] + [weights.output]
         self.products_ws = new_workspace(max(workspace_bytes(dw.dtype, T, dw.N, dw.K, cfg.act_mode) for dw in products), dev)
         self.pos, self.pending, self.tokens = 0, None, []
+        # the last call's work, for a next call on another stream (the fills above,
+        # rows on their way into place)
+        self._last = torch.cuda.Event()
+        self._last.record(torch.cuda.current_stream(dev))
+
+    @contextlib.contextmanager
+    def _ordered(self):
+        """On the verifier's device, with the current stream after the last call's work."""
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream()
+            stream.wait_event(self._last)
+            try:
+                yield
+            finally:
+                self._last.record(stream)
 
     # ---- the forward pass of T nodes --------------------------------------
     def _product(self, dw, x, y, T, norm=None, swiglu=False, accumulate=False):
@@ -391,7 +408,7 @@ class DraftVerifier:
             raise ValueError("prompt longer than the context")
         # no sequence until the prompt has run
         self.pos, self.pending, self.tokens = 0, None, list(prompt)
-        with torch.cuda.device(self.device):
+        with self._ordered():
             for i in range(0, len(prompt) - 1, self.max_nodes):
                 chunk = prompt[i:min(i + self.max_nodes, len(prompt) - 1)]
                 self._forward(chunk, None, None, False)
@@ -432,7 +449,7 @@ class DraftVerifier:
             sees.append((0 if p < 0 else sees[p]) | (1 << i))
             path.append([i] if p < 0 else path[p] + [i])
         dev = self.device
-        with torch.cuda.device(dev):
+        with self._ordered():
             W = (T + 31) // 32
             words = [[(s >> (32 * w)) & 0xFFFFFFFF for w in range(W)] for s in sees]
             mask = torch.tensor([[x - (1 << 32) if x >> 31 else x for x in r] for r in words], dtype=torch.int32).to(dev)

@@ -103,6 +103,7 @@ def verifier(monkeypatch):
     import types
 
     monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(draft.DraftVerifier, "_ordered", lambda self: contextlib.nullcontext(), raising=False)
     monkeypatch.setattr(draft.DraftVerifier, "_forward", lambda self, *a: None)
     monkeypatch.setattr(draft.DraftVerifier, "_check", lambda self: None)
     v = object.__new__(draft.DraftVerifier)

@@ -248,3 +248,34 @@ def test_verifiers_keep_their_workspaces(cuda_lib):
         t.join()
     torch.cuda.synchronize()
     assert wrong == [0, 0] and all(v.status() == 0 for v in vs)
+
+
+@pytest.mark.parametrize("cache", ["f16", "i8"])
+def test_calls_on_other_streams_follow_each_other(cuda_lib, cache):
+    """A verifier made on one stream (whose fills come late) and called on others
+    (where a branch's rows come late into place) gives what it gives on one."""
+    import torch
+
+    from odiengine_b200.draft import DraftVerifier
+
+    cfg, mw = model(1)
+    prompt = [5, 17, 999, 3, 250]
+    plain = DraftVerifier(cfg, mw, cache=cache)
+    plain.start(prompt)
+    want = []
+    for _ in range(6):
+        want += plain.verify()
+    drafts = [(want[0] + 1) % cfg.vocab, want[0], want[1]]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda._sleep(100_000_000)
+    v = DraftVerifier(cfg, mw, cache=cache, max_nodes=8)
+    with torch.cuda.stream(streams[0]):
+        v.start(prompt)
+    with torch.cuda.stream(streams[1]):
+        first = v.verify(drafts, [0, 0, 2])  # the second branch is right: its rows move
+        torch.cuda._sleep(100_000_000)
+    with torch.cuda.stream(streams[2]):
+        second = v.verify()
+    torch.cuda.synchronize()
+    assert first == want[:3] and second == want[3:4]
