@@ -451,7 +451,8 @@ int odi_cuda_qk_rope_append(const float* d_qkv, int64_t ld_qkv, const float* d_q
                             float theta, void* stream);
 
 /* Positions start .. start + count - 1 of K and V (either output may be NULL)
- * as [kv_heads][count][head_dim] fp16 or fp32, 16-byte aligned. */
+ * as [kv_heads][count][head_dim] fp16 or fp32, 16-byte aligned, which may
+ * overlap neither each other nor the cache. */
 enum { ODI_CUDA_KV_OUT_F16 = 0, ODI_CUDA_KV_OUT_F32 = 1 };
 int odi_cuda_kv_read(const odi_cuda_kv_cache* cache, int start, int count, void* d_k_out, void* d_v_out,
                      int out_dtype, void* stream);

@@ -390,6 +390,17 @@ int odi_cuda_kv_read(const odi_cuda_kv_cache* cache, int start, int count, void*
   if (!d_k_out && !d_v_out) return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_read: no output");
   if (((uintptr_t)d_k_out | (uintptr_t)d_v_out) & 15)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_read: outputs must be 16-byte aligned");
+  // pieces are read and written in no order
+  const size_t out_bytes = (size_t)v.kv_heads * count * v.hd * (out_dtype == ODI_CUDA_KV_OUT_F16 ? 2 : 4);
+  const size_t cache_bytes = odi_cuda_kv_cache_bytes(v.dtype, v.kv_heads, v.hd, v.ctx);
+  const auto clash = [](const void* a, size_t n, const void* b, size_t m) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
+  };
+  for (const void* o : {d_k_out, d_v_out})
+    if (clash(o, out_bytes, v.k, cache_bytes) || clash(o, out_bytes, v.v, cache_bytes))
+      return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_read: an output overlaps the cache");
+  if (clash(d_k_out, out_bytes, d_v_out, out_bytes))
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "kv_read: the outputs overlap");
   const bool i8 = v.dtype == ODI_CUDA_KV_I8, o16 = out_dtype == ODI_CUDA_KV_OUT_F16;
   const int64_t pieces = (int64_t)count * (v.hd / (o16 ? 8 : 4));
   const dim3 grid((unsigned)((pieces + 256 * READ_U - 1) / (256 * READ_U)), v.kv_heads, 2);

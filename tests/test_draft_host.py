@@ -94,6 +94,23 @@ def test_cache_halves_that_do_not_fit_are_refused():
         draft.KVCache(OnGpu(u8[:need]), OnGpu(u8[16:need + 16]), "i8", 2, 64, 8)
 
 
+def test_read_refuses_outputs_over_each_other_or_the_cache():
+    """Addresses of nothing: no call below reaches a launch."""
+    import ctypes
+
+    import odiengine_b200 as ob
+
+    L, K, V = ob.lib(), 0x100000, 0x200000
+    c = ctypes.byref(draft._KvCacheStruct(K, V, draft.KV_F16, 2, 64, 100))  # 25,600 bytes each
+    size, out = 2 * 10 * 64 * 2, 0x300000                                   # 10 positions as fp16
+    for k, v, dt in ((out, out, 0), (out, out + size - 16, 0), (out + size, out + 16, 0), (out, out + size, 1),
+                     (K, None, 0), (None, K + 25600 - 16, 0), (V - size + 16, out, 0), (out, V, 0)):
+        assert L.odi_cuda_kv_read(c, 0, 10, k, v, dt, None) == 2
+        assert "overlap" in L.odi_cuda_last_error().decode()
+    rows = draft._KvCacheStruct(K, V, draft.KV_I8, 2, 64, 100)              # the scales are the cache's too
+    assert L.odi_cuda_kv_read(ctypes.byref(rows), 0, 10, K + 12800, out, 0, None) == 2
+
+
 # ---- sequences -------------------------------------------------------------------------------------------------
 
 @pytest.fixture
