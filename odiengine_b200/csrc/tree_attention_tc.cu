@@ -40,12 +40,13 @@
 //
 // The softmax bounds the kernel: 17 instructions per score (packed fp32 pairs
 // where two scores share an operation), of which two warps per scheduler issue
-// one every 2.3 cycles.  64 nodes, 64 / 8 heads, 32641 int8 positions: 183 us (fp16:
-// 168), where fetching the cache takes 11 and 69 GFLOP at the fp16 rate 41; the
-// loop without any products took 176 where the whole took 182.  Smaller shares for more warps (16 of 16
-// rows: 212 us, the work per block that does not depend on rows doubles), a vote
-// without a barrier (234 where this took 224) and scores one block ahead of the
-// weights (200) were slower.
+// one every 2.3 cycles.  64 nodes, 64 / 8 heads, 32641 int8 positions: 183 us
+// (fp16: 168), where fetching the cache takes 11 and 69 GFLOP at the fp16 rate 41;
+// the loop without any products took 176 where the whole took 182.  Smaller shares
+// for more warps (16 of 16 rows: 212 us, the work per block that does not depend on
+// rows doubles), a vote without a barrier (234 where this took 224), scores one
+// block ahead of the weights (200) and V turned into fp16 in shared memory by four
+// more warps (220) were slower.
 //
 // Every wait is bounded; a wait that gives up sets the error word, all roles
 // leave their loops, copies in flight are waited for and the tensor memory is
@@ -101,8 +102,8 @@ struct Cfg {
   // Weights in P, log2: what they stay below, and the largest right after a move.
   // int8: an integer below 2^32, so to within 2^-25 of the largest, either way;
   // 64 nodes over 32641 positions 183 us, 198 and 207 with the largest at 2^27 and
-  // 2^29: rows move more often, and a
-  // block in which one does costs two.  fp16: to within 2^-37, 2^-43 of the largest.
+  // 2^29, since a block in which a row moves costs two.  fp16: to within 2^-37, which
+  // is 2^-44 to 2^-45 of the largest.
   static constexpr float P_TOP = I8 ? 31.9f : 15.f, P_UNIT = I8 ? 26.f : 8.f;
   static_assert(SMEM <= 222 * 1024, "shared memory, beside the static part");
 };
