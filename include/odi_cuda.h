@@ -521,6 +521,147 @@ int odi_cuda_logits_adjust(const float* d_logits, int64_t ld_logits, float* d_ou
                            int rows, int64_t V, const odi_cuda_logits_opts* opts, void* d_scratch,
                            size_t scratch_bytes, void* stream);
 
+/* --- several requests over a paged cache ------------------------------------
+ * One step of a batch of requests: each brings new tokens (one, a chain of
+ * drafts, a chunk of its prompt) and keeps its cache rows in pages that all
+ * requests share.  odi_cuda_paged_step hands out pages and lists the step's
+ * rows; odi_cuda_qk_rope_append_paged writes rows into pages;
+ * odi_cuda_attention_paged attends over them; odi_cuda_verify_sampled checks
+ * drafted tokens by the target's distribution.  The lengths stay on the
+ * device, so a step can be captured and replayed.  The reference runs one
+ * sequence over one contiguous cache (context.cpp:84-282). */
+
+/* One layer's cache: k and v are [num_pages][kv_heads][page_size][head_dim],
+ * 16-byte aligned.  page_size 16, 32, 64 or 128; head_dim 64 or 128. */
+enum { ODI_CUDA_PAGED_F16 = 0, ODI_CUDA_PAGED_BF16 = 1 };
+typedef struct odi_cuda_paged_cache {
+  void* k;
+  void* v;
+  int dtype;
+  int kv_heads;
+  int head_dim;
+  int page_size;
+  int num_pages;
+} odi_cuda_paged_cache;
+
+/* Who holds which page, for all layers (device memory).  table
+ * [requests][max_pages]: page of each page_size positions of a request;
+ * lens [requests]: positions it holds; free_pages [num_pages]: a stack of
+ * free pages, *free_count of them. */
+typedef struct odi_cuda_page_tables {
+  int32_t* table;
+  int32_t* lens;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int requests;
+  int max_pages;
+  int page_size;
+  int num_pages;
+} odi_cuda_page_tables;
+
+/* A step's rows (device memory, written by odi_cuda_paged_step).  Row r of
+ * request b, starts[b] <= r < starts[b + 1], is its token number r -
+ * starts[b].  lens[b]: positions of the request with its new ones, 0 if it
+ * was refused.  positions, slots [max_rows]: each row's position and its
+ * place in the cache, page * page_size + place in the page; -1 behind the
+ * last row and in refused requests.  work: odi_cuda_paged_work_bytes, 16-byte
+ * aligned; its first word is the step's status.  requests as in the tables,
+ * at most ODI_CUDA_PAGED_MAX_REQUESTS; max_new: new tokens of one request at
+ * most; heads, kv_heads: of the attention that reads the batch (heads a
+ * multiple of kv_heads, at most 64 times). */
+enum { ODI_CUDA_PAGED_MAX_REQUESTS = 2048, ODI_CUDA_PAGED_MAX_ROWS = 262144 };
+typedef struct odi_cuda_paged_batch {
+  int32_t* starts;
+  int32_t* lens;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* work;
+  int requests;
+  int max_rows;
+  int max_new;
+  int heads;
+  int kv_heads;
+  int page_size;
+} odi_cuda_paged_batch;
+
+/* Bits of a step's status; 0: every request got its rows. */
+enum {
+  ODI_CUDA_PAGED_NO_PAGES = 1,       /* refused: not enough free pages */
+  ODI_CUDA_PAGED_TOO_LONG = 2,       /* refused: longer than max_pages pages */
+  ODI_CUDA_PAGED_BAD_NEW = 4,        /* refused: new below 0 or above max_new */
+  ODI_CUDA_PAGED_TOO_MANY_ROWS = 8,  /* refused: rows past max_rows */
+  ODI_CUDA_PAGED_BAD_KEEP = 16,      /* keep below 0 or above lens: brought into range */
+  ODI_CUDA_PAGED_BAD_LENGTH = 32     /* lens below 0 or above max_pages pages: brought into range */
+};
+
+/* Bytes of odi_cuda_paged_batch.work; 0 for sizes out of range. */
+size_t odi_cuda_paged_work_bytes(int requests, int max_rows, int max_new, int heads, int kv_heads);
+
+/* Request b keeps its first d_keep[b] positions (NULL: all), and takes
+ * d_new[b] more.  Pages that fall free go back before any is taken (a
+ * request that keeps 0 and takes 0 is over); a request whose pages are not
+ * there is refused: it keeps what it kept, its rows have no slots, and
+ * attention leaves its rows as they were.  Requests are served in their
+ * order.  d_prefix (NULL: 0): the first d_prefix[b] positions see one another
+ * both ways, once they are in the cache. */
+int odi_cuda_paged_step(const odi_cuda_page_tables* tables, const odi_cuda_paged_batch* batch, const int32_t* d_keep,
+                        const int32_t* d_new, const int32_t* d_prefix, void* stream);
+
+/* The first `tokens` rows of d_qkv are [q heads | k kv_heads | v kv_heads] *
+ * head_dim fp32, ld_qkv apart.  Per head: RMSNorm with d_q_norm / d_k_norm
+ * (head_dim weights; NULL: none), then the rotation of odi_cuda_rope_kv at
+ * the row's position, its angle reduced in 64 bits.  k and v go to the row's
+ * slot, rotated q rows, rounded to the cache's type, to d_q_out (ld_q apart,
+ * even; 4-byte aligned; it may not overlap d_qkv).  Rows without a slot are
+ * not written. */
+int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const float* d_q_norm, const float* d_k_norm,
+                                  float eps, void* d_q_out, int64_t ld_q, const odi_cuda_paged_cache* cache,
+                                  const odi_cuda_paged_batch* batch, int tokens, int heads, float theta, void* stream);
+
+/* out[r] = softmax(s) v over the positions that row r's token sees: its own,
+ * those before it, and its request's prefix.  s = scale * q . k; with softcap
+ * > 0: softcap * tanh(s / softcap); with d_slopes (fp32 [heads]): minus
+ * slope * |i - j|.  d_q: rotated rows of the cache's type, ld_q apart (even),
+ * heads * head_dim values; d_out: of the cache's type or fp32, ld_out apart;
+ * both 4-byte aligned, and they may not overlap.  tokens: rows that d_q and
+ * d_out have.  Rows behind the batch's last, and of refused requests, are
+ * left as they were.  A row all of whose scores are -inf is zero.  Scores,
+ * softmax and sums are fp32; the weights are rounded to the cache's type.
+ * scale is positive.
+ * Scratch: odi_cuda_attention_paged_scratch_bytes, 16-byte aligned, zero
+ * before its first use; calls of any layer, and of any batch that needs no
+ * more, on one stream share it.  Its first word is an error word (odi_cuda_workspace_status):
+ * a bounded wait that gave up, or a table entry that names no page (such a
+ * page reads as zeros). */
+enum { ODI_CUDA_PAGED_OUT_CACHE = 0, ODI_CUDA_PAGED_OUT_F32 = 1 };
+size_t odi_cuda_attention_paged_scratch_bytes(int requests, int max_rows, int max_new, int heads, int kv_heads, int head_dim);
+int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged_cache* cache,
+                             const odi_cuda_page_tables* tables, const odi_cuda_paged_batch* batch, void* d_out,
+                             int64_t ld_out, int out_dtype, int tokens, float scale, float softcap, const float* d_slopes,
+                             void* d_scratch, size_t scratch_bytes, void* stream);
+
+/* Drafted tokens against the target's distribution p = softmax(logits /
+ * temperature).  Rows starts[b] .. starts[b + 1] - 1 of d_logits (rows x V
+ * fp32, ld apart) belong to request b; d_tokens[r] is the token of row r, so
+ * the draft that row r's logits judge is d_tokens[r + 1] of the same
+ * request.  It is kept iff u_accept[r] * q(draft) < p(draft), q being row r
+ * of d_draft_probs (rows x V fp32, ld_probs apart), or 1 (NULL: a drafter
+ * that gives one token).  accepted[b]: drafts kept before the first that is
+ * not.  next[b]: the token after them, drawn with u_next[b] from max(p - q,
+ * 0) of the row that refused (from p if that is 0 everywhere), or from p of
+ * the last row: the first id whose running sum is over u_next times the
+ * whole.  Random numbers are in [0, 1).  A draft outside the vocabulary is
+ * refused.  -inf logits have no weight, +inf ones share it all; a row with a
+ * NaN or with no finite logit keeps no draft and gives -1, as does a request
+ * without rows.  In 64 bits throughout.
+ * Scratch: 16-byte aligned, zero before its first use, for calls that need
+ * no more on one stream.  rows up to 65535, requests up to 16384. */
+size_t odi_cuda_verify_scratch_bytes(int rows, int requests, int64_t V);
+int odi_cuda_verify_sampled(const float* d_logits, int64_t ld, const int32_t* d_tokens, const int32_t* d_starts, int rows,
+                            int requests, int64_t V, double temperature, const float* d_draft_probs, int64_t ld_probs,
+                            const float* d_u_accept, const float* d_u_next, int32_t* d_accepted, int32_t* d_next,
+                            void* d_scratch, size_t scratch_bytes, void* stream);
+
 /* --- the decode step as one call per token ----------------------------------
  * A device-resident decoder of a Llama-shaped model: one token's forward
  * pass (context.cpp:84-282 for a single token, with cpu_backend.cpp:388-619's

@@ -106,6 +106,16 @@ SIGNATURES = {
     "odi_cuda_attention_tree": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _int, _int, ctypes.c_float, _vp, _sz, _vp]),
     "odi_cuda_logits_scratch_bytes": (_sz, [_int]),
     "odi_cuda_logits_adjust": (_int, [_vp, _i64, _vp, _i64, _vp, _int, _i64, _vp, _vp, _sz, _vp]),
+    "odi_cuda_paged_work_bytes": (_sz, [_int, _int, _int, _int, _int]),
+    "odi_cuda_paged_step": (_int, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "odi_cuda_qk_rope_append_paged": (_int, [_vp, _i64, _vp, _vp, ctypes.c_float, _vp, _i64, _vp, _vp, _int, _int,
+                                             ctypes.c_float, _vp]),
+    "odi_cuda_attention_paged_scratch_bytes": (_sz, [_int, _int, _int, _int, _int, _int]),
+    "odi_cuda_attention_paged": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _int, _int, ctypes.c_float, ctypes.c_float,
+                                        _vp, _vp, _sz, _vp]),
+    "odi_cuda_verify_scratch_bytes": (_sz, [_int, _int, _i64]),
+    "odi_cuda_verify_sampled": (_int, [_vp, _i64, _vp, _vp, _int, _int, _i64, ctypes.c_double, _vp, _i64, _vp, _vp, _vp,
+                                       _vp, _vp, _sz, _vp]),
     "odi_cuda_scatter_signals": (_i64, [_int, _i64, _i64, _i64, _int]),
     "odi_cuda_matmul_scatter": (_int, [_int, _vp, _vp, _i64, _i64, _i64, _int, _vp, _sz, _int, _vp, _vp]),
     "odi_cuda_wait_peers": (_int, [_vp, _vp, _vp, _int, _vp, _vp]),

@@ -1,0 +1,66 @@
+// paged.cuh -- several requests over a paged KV cache: what the kernels of
+// paged_step.cu, paged_append.cu and paged_attention*.cu share.
+//
+// A layer's K and V are [num_pages][kv_heads][page_size][head_dim]: one page of
+// one kv head is one contiguous run of rows, the shape that the decode step's
+// cache has for a whole context, so a box of a tensor map is (part of) a page.
+// One block table serves all layers.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "../../include/odi_cuda.h"
+#include "common.cuh"
+
+namespace odi_cuda {
+
+struct PagedView {
+  void* k;
+  void* v;
+  int dtype;  // ODI_CUDA_PAGED_F16 / ODI_CUDA_PAGED_BF16
+  int kv_heads, hd, page_size, num_pages;
+  int page_shift;
+};
+
+// How attention cuts a batch's rows: an item is up to `rows` of the new tokens *
+// G rows of one request (row r: token r / G, head r % G of each kv head's
+// group), over tiles of `tile` positions.
+struct PagedGeometry {
+  int G, rows, tile;
+  int64_t max_items;
+};
+
+// Words of odi_cuda_paged_batch.work.
+constexpr int PW_STATUS = 0, PW_ITEMS = 1, PW_TILES = 2, PW_HEADER = 16;
+inline __host__ __device__ int64_t paged_round4(int64_t n) { return (n + 3) & ~3ll; }
+struct PagedWork {
+  const int* prefix;  // [requests]
+  const int* cum;     // [items + 1]: tiles of the items before
+  const int2* info;   // [items]: request, item within the request
+};
+inline __host__ __device__ PagedWork paged_work(const int* work, int requests, int64_t max_items) {
+  const int* prefix = work + PW_HEADER;
+  const int* cum = prefix + paged_round4(requests);
+  return {prefix, cum, reinterpret_cast<const int2*>(cum + paged_round4(max_items + 1))};
+}
+
+// Checks of a caller's descriptors; `who` opens the error message.
+int paged_view(const odi_cuda_paged_cache* c, PagedView* v, const char* who);
+int paged_batch_ok(const odi_cuda_paged_batch* b, PagedGeometry* g, const char* who);
+bool paged_geometry(int requests, int max_rows, int max_new, int heads, int kv_heads, PagedGeometry* g);
+
+inline bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128; }
+inline int page_shift_of(int p) { return p == 16 ? 4 : p == 32 ? 5 : p == 64 ? 6 : 7; }
+// Rows of an item and positions of a tile, by the most rows a request has per kv
+// head: the two widths of the mma.sync kernel.
+inline void paged_kind(int64_t most, int* rows, int* tile) {
+  *rows = most <= 16 ? 16 : 32;
+  *tile = 64;
+}
+
+// Positions of the batch that row r of request b sees: those below the result.
+__device__ __forceinline__ int paged_limit(int first, int token, int len, int prefix) {
+  return min(len, max(first + token + 1, prefix));
+}
+
+}  // namespace odi_cuda

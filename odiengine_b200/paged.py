@@ -1,0 +1,249 @@
+"""Several requests over a paged KV cache: the operators of a step in which
+every request brings new tokens (one, a chain of drafts, a chunk of its
+prompt), on device tensors.
+
+    paged_step              pages handed out, the step's rows and slots
+    qk_rope_append_paged    per-head q/k norm + rotation, k and v rows into pages
+    attention_paged         every new token over its request's pages
+    verify_sampled          drafts against the target's probabilities
+
+over :class:`PagedCache` (a layer's pages, fp16 or bf16), :class:`PageTables`
+(who holds which page, one for all layers) and :class:`PagedBatch` (a step's
+rows).  :class:`PagedDecoder` is the step made of them and of the library's
+products, for the models of odiengine_b200.decode.  Calls are asynchronous on
+`stream` (default: the tensors' device's current stream), where outputs that a
+call makes are allocated too; tensors of another stream that are handed in are
+the caller's to order and to keep (Tensor.record_stream).  Errors are
+:class:`odiengine_b200.OdiCudaError`, or ValueError / TypeError for tensors
+that do not fit.  Lengths and rows stay on the device, so calls can be captured
+in a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import lib
+from .draft import _call, _flat, _refuse, _rows2
+
+PAGED_DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # ODI_CUDA_PAGED_*
+PAGE_SIZES = (16, 32, 64, 128)
+OUT_CACHE, OUT_F32 = 0, 1                             # ODI_CUDA_PAGED_OUT_*
+# a step's status (ODI_CUDA_PAGED_*)
+NO_PAGES, TOO_LONG, BAD_NEW, TOO_MANY_ROWS, BAD_KEEP, BAD_LENGTH = 1, 2, 4, 8, 16, 32
+
+
+class _CacheStruct(ctypes.Structure):
+    """odi_cuda_paged_cache (include/odi_cuda.h)."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("page_size", ctypes.c_int), ("num_pages", ctypes.c_int)]
+
+
+class _TablesStruct(ctypes.Structure):
+    """odi_cuda_page_tables (include/odi_cuda.h)."""
+
+    _fields_ = [("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+                ("free_count", ctypes.c_void_p), ("requests", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("num_pages", ctypes.c_int)]
+
+
+class _BatchStruct(ctypes.Structure):
+    """odi_cuda_paged_batch (include/odi_cuda.h)."""
+
+    _fields_ = [("starts", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("slots", ctypes.c_void_p), ("work", ctypes.c_void_p), ("requests", ctypes.c_int),
+                ("max_rows", ctypes.c_int), ("max_new", ctypes.c_int), ("heads", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("page_size", ctypes.c_int)]
+
+
+def _new(shape, dtype, device, stream):
+    """An output that a call makes, allocated on the stream that writes it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+class PagedCache:
+    """One layer's K and V: fp16 or bf16 [num_pages, kv_heads, page_size, head_dim]."""
+
+    def __init__(self, k, v):
+        if k.dtype not in PAGED_DTYPES:
+            raise TypeError(f"cache k: fp16 or bf16 wanted, got {k.dtype}")
+        if k.dim() != 4:
+            raise ValueError(f"cache k: [num_pages, kv_heads, page_size, head_dim] wanted, got {tuple(k.shape)}")
+        for t, n in ((k, "k"), (v, "v")):
+            if t.dtype is not k.dtype or t.device != k.device or not t.is_cuda or not t.is_contiguous() or t.shape != k.shape:
+                _refuse(t, k.dtype, f"cache {n}", k.get_device(), f"contiguous {tuple(k.shape)}")
+            if t.data_ptr() % 16:
+                raise ValueError(f"cache {n}: must be 16-byte aligned")
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        if self.page_size not in PAGE_SIZES or self.head_dim not in (64, 128):
+            raise ValueError(f"cache: page_size of {PAGE_SIZES} and head_dim 64 or 128 wanted, got {tuple(k.shape)}")
+        if abs(k.data_ptr() - v.data_ptr()) < k.numel() * 2:
+            raise ValueError("cache: k and v share memory")
+        self.k, self.v, self.dtype = k, v, k.dtype
+        self.device, self.index = k.device, k.get_device()
+        self._struct = _CacheStruct(k.data_ptr(), v.data_ptr(), PAGED_DTYPES[k.dtype], self.kv_heads, self.head_dim,
+                                    self.page_size, self.num_pages)
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def new(cls, dtype, num_pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> "PagedCache":
+        """Empty (zero) pages."""
+        return cls(*(torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=dtype, device=device) for _ in range(2)))
+
+    @property
+    def nbytes(self) -> int:
+        return 2 * self.k.numel() * 2
+
+
+class PageTables:
+    """Who holds which page.  int32 tensors: table [requests, max_pages], lens
+    [requests], free [num_pages] (a stack of free pages) and free_count [1]."""
+
+    def __init__(self, table, lens, free, free_count, page_size: int):
+        i32, dev = torch.int32, table.get_device()
+        if table.dim() != 2:
+            raise ValueError(f"table: [requests, max_pages] wanted, got {tuple(table.shape)}")
+        self.requests, self.max_pages = table.shape
+        self.num_pages, self.page_size = free.numel(), page_size
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size: one of {PAGE_SIZES}")
+        self._struct = _TablesStruct(
+            _flat(table, i32, "table", dev, self.requests * self.max_pages), _flat(lens, i32, "lens", dev, self.requests),
+            _flat(free, i32, "free", dev, self.num_pages), _flat(free_count, i32, "free_count", dev, 1), self.requests,
+            self.max_pages, page_size, self.num_pages)
+        self.table, self.lens, self.free, self.free_count = table, lens, free, free_count
+        self.device, self.index = table.device, dev
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def new(cls, requests: int, max_pages: int, num_pages: int, page_size: int, device="cuda") -> "PageTables":
+        """Tables of requests that hold nothing, every page free (page 0 is taken first)."""
+        i32 = torch.int32
+        return cls(torch.full((requests, max_pages), -1, dtype=i32, device=device), torch.zeros(requests, dtype=i32, device=device),
+                   torch.arange(num_pages - 1, -1, -1, dtype=i32, device=device),
+                   torch.full((1,), num_pages, dtype=i32, device=device), page_size)
+
+
+class PagedBatch:
+    """A step's rows, written by paged_step: starts [requests + 1], lens
+    [requests], positions and slots [max_rows] (int32).  max_new: new tokens of
+    one request at most; it says which attention kernel suits, so a batch of
+    single tokens and one of prompts' chunks are best kept apart."""
+
+    def __init__(self, tables: PageTables, *, max_rows: int, max_new: int, heads: int, kv_heads: int):
+        n = lib().odi_cuda_paged_work_bytes(tables.requests, max_rows, max_new, heads, kv_heads)
+        if not n:
+            raise ValueError(f"no batch of {tables.requests} requests, max_rows {max_rows}, max_new {max_new}, heads {heads}, "
+                             f"kv_heads {kv_heads}")
+        new = lambda k: torch.zeros(k, dtype=torch.int32, device=tables.device)  # noqa: E731
+        self.starts, self.lens = new(tables.requests + 1), new(tables.requests)
+        self.positions, self.slots, self.work = new(max_rows), new(max_rows), new(n // 4)
+        self.requests, self.max_rows, self.max_new, self.heads, self.kv_heads = tables.requests, max_rows, max_new, heads, kv_heads
+        self.page_size, self.device, self.index = tables.page_size, tables.device, tables.index
+        self._struct = _BatchStruct(self.starts.data_ptr(), self.lens.data_ptr(), self.positions.data_ptr(),
+                                    self.slots.data_ptr(), self.work.data_ptr(), self.requests, max_rows, max_new, heads,
+                                    kv_heads, self.page_size)
+        self._ref = ctypes.addressof(self._struct)
+
+    def status(self) -> int:
+        """The last step's status bits (NO_PAGES, ...); waits for it."""
+        return int(self.work[0].item())
+
+
+def paged_step(tables: PageTables, batch: PagedBatch, new, keep=None, prefix=None, stream=None) -> None:
+    """Request b keeps keep[b] of its positions (None: all) and takes new[b]
+    more (int32 [requests]); prefix[b] positions see one another both ways.
+    Tables and batch are brought up to date."""
+    dev, B = tables.index, tables.requests
+    i32 = torch.int32
+    _call(dev, stream, lib().odi_cuda_paged_step, tables._ref, batch._ref,
+          None if keep is None else _flat(keep, i32, "keep", dev, B), _flat(new, i32, "new", dev, B),
+          None if prefix is None else _flat(prefix, i32, "prefix", dev, B))
+
+
+def qk_rope_append_paged(qkv, cache: PagedCache, batch: PagedBatch, q_out=None, *, heads: int, theta: float, q_norm=None,
+                         k_norm=None, eps: float = 1e-6, stream=None):
+    """The batch's rows of qkv [T, (heads + 2 kv_heads) * head_dim] fp32: q and
+    k normed per head (q_norm / k_norm: head_dim weights, or None) and rotated
+    at their positions, k and v stored at their slots.  Returns the rotated q
+    in q_out [T, heads * head_dim] of the cache's type."""
+    dev, hd, f32 = cache.index, cache.head_dim, torch.float32
+    ld = _rows2(qkv, f32, "qkv", dev, None, (heads + 2 * cache.kv_heads) * hd)
+    T = qkv.shape[0]
+    if q_out is None:
+        q_out = _new((T, heads * hd), cache.dtype, cache.device, stream)
+    ld_q = _rows2(q_out, cache.dtype, "q_out", dev, T, heads * hd)
+    _call(dev, stream, lib().odi_cuda_qk_rope_append_paged, qkv.data_ptr(), ld,
+          None if q_norm is None else _flat(q_norm, f32, "q_norm", dev, hd),
+          None if k_norm is None else _flat(k_norm, f32, "k_norm", dev, hd), eps, q_out.data_ptr(), ld_q, cache._ref,
+          batch._ref, T, heads, theta)
+    return q_out
+
+
+def attention_paged_scratch(cache: PagedCache, batch: PagedBatch):
+    """Zeroed scratch for attention_paged calls on one stream: of any layer, and
+    of any batch that needs no more."""
+    n = lib().odi_cuda_attention_paged_scratch_bytes(batch.requests, batch.max_rows, batch.max_new, batch.heads, batch.kv_heads,
+                                                     cache.head_dim)
+    return torch.zeros(n, dtype=torch.uint8, device=cache.device)
+
+
+def attention_paged(q, cache: PagedCache, tables: PageTables, batch: PagedBatch, out=None, *, scale: float, softcap: float = 0.0,
+                    slopes=None, scratch, stream=None):
+    """The batch's rows of q (rotated, of the cache's type, [T, heads *
+    head_dim]) over their requests' positions: those up to a row's own, and its
+    request's prefix.  softcap: scores are capped by softcap * tanh(s /
+    softcap); slopes fp32 [heads]: scores lose slope * distance.  out: of the
+    cache's type (the default) or fp32; rows behind the batch's last are left."""
+    dev, w = cache.index, batch.heads * cache.head_dim
+    ld = _rows2(q, cache.dtype, "q", dev, None, w)
+    T = q.shape[0]
+    if out is None:
+        out = _new((T, w), cache.dtype, cache.device, stream)
+    o32 = out.dtype is torch.float32
+    ld_o = _rows2(out, torch.float32 if o32 else cache.dtype, "out", dev, T, w)
+    n = 0 if scratch is None else scratch.numel()
+    _call(dev, stream, lib().odi_cuda_attention_paged, q.data_ptr(), ld, cache._ref, tables._ref, batch._ref, out.data_ptr(),
+          ld_o, OUT_F32 if o32 else OUT_CACHE, T, scale, softcap,
+          None if slopes is None else _flat(slopes, torch.float32, "slopes", dev, batch.heads),
+          _flat(scratch, torch.uint8, "scratch", dev, n), n)
+    return out
+
+
+def verify_scratch(rows: int, requests: int, vocab: int, device="cuda"):
+    """Zeroed scratch for verify_sampled calls of up to these sizes on one stream."""
+    n = lib().odi_cuda_verify_scratch_bytes(rows, requests, vocab)
+    if not n:
+        raise ValueError(f"verify_sampled: no such sizes (rows {rows}, requests {requests}, vocabulary {vocab})")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def verify_sampled(logits, tokens, starts, u_accept, u_next, accepted=None, next=None, *, temperature: float = 1.0,
+                   draft_probs=None, scratch, stream=None):
+    """Drafts against p = softmax(logits / temperature).  logits fp32 [rows, V],
+    rows starts[b] .. starts[b + 1] - 1 (int32 [requests + 1]) being request
+    b's; tokens int32 [rows]: each row's token, so row r judges the draft
+    tokens[r + 1].  It is kept iff u_accept[r] * q < p, with q row r of
+    draft_probs fp32 [rows, V] (None: 1).  Returns accepted and next (int32
+    [requests]): drafts kept, and the token after them, drawn with u_next."""
+    dev, f32, i32 = logits.get_device(), torch.float32, torch.int32
+    R, V = logits.shape
+    B = starts.numel() - 1
+    ld = _rows2(logits, f32, "logits", dev, R, V)
+    if accepted is None:
+        accepted = _new((B,), i32, logits.device, stream)
+    if next is None:
+        next = _new((B,), i32, logits.device, stream)
+    n = 0 if scratch is None else scratch.numel()
+    _call(dev, stream, lib().odi_cuda_verify_sampled, logits.data_ptr(), ld, _flat(tokens, i32, "tokens", dev, R),
+          _flat(starts, i32, "starts", dev, B + 1), R, B, V, temperature,
+          None if draft_probs is None else draft_probs.data_ptr(),
+          0 if draft_probs is None else _rows2(draft_probs, f32, "draft_probs", dev, R, V),
+          _flat(u_accept, f32, "u_accept", dev, R), _flat(u_next, f32, "u_next", dev, B), _flat(accepted, i32, "accepted", dev, B),
+          _flat(next, i32, "next", dev, B), _flat(scratch, torch.uint8, "scratch", dev, n), n)
+    return accepted, next
