@@ -571,12 +571,14 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.cap_log2 = softcap * 1.4426950408889634f;
   a.slopes = d_slopes;
   a.vec = !((uintptr_t)d_q & 15) && !(ld_q & 7);
+  a.vec_out = !((uintptr_t)d_out & 15) && !(ld_out & 7);
   a.least = 1;
   a.err = static_cast<int*>(d_scratch);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + PART_OFF);
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + COUNT_OFF);
   const bool fancy = softcap > 0.f || d_slopes;
-  return kv_launched(launch_paged_mma(a, g.rows / 16, fancy, (cudaStream_t)stream), "attention_paged");
+  cudaStream_t s = (cudaStream_t)stream;
+  return kv_launched(g.rows <= 32 ? launch_paged_mma(a, g.rows / 16, fancy, s) : launch_paged_tc(a, fancy, s), "attention_paged");
 }
 
 }  // extern "C"

@@ -35,7 +35,7 @@ struct PagedAttnArgs {
   float scale_log2;  // scale * log2(e), or scale / cap where there is a cap
   float cap_log2;    // cap * log2(e), or 0
   const float* slopes;
-  int vec;           // q and its stride allow 16-byte loads
+  int vec, vec_out;  // q, out and their strides allow 16-byte accesses
   int least;         // tiles per CTA at least
   float* part;       // [2 * CTAs][rows][HD + 2]
   int* count;        // arrivals per unit, zero between launches
