@@ -31,17 +31,17 @@ struct PagedGeometry {
 };
 
 // Words of odi_cuda_paged_batch.work.
-constexpr int PW_STATUS = 0, PW_ITEMS = 1, PW_TILES = 2, PW_HEADER = 16;
-inline __host__ __device__ int64_t paged_round4(int64_t n) { return (n + 3) & ~3ll; }
-struct PagedWork {
-  const int* prefix;  // [requests]
-  const int* cum;     // [items + 1]: tiles of the items before
-  const int2* info;   // [items]: request, item within the request
+constexpr int PW_STATUS = 0, PW_ITEMS = 2, PW_TILES = 3, PW_HEADER = 16;
+struct alignas(16) PagedItem {
+  int b, i;              // request, item within the request
+  int start, past, len;  // its first row; positions before its new ones; all of them
+  int prefix;
+  int tile0, tiles;      // tiles of the items before; its own
 };
-inline __host__ __device__ PagedWork paged_work(const int* work, int requests, int64_t max_items) {
-  const int* prefix = work + PW_HEADER;
-  const int* cum = prefix + paged_round4(requests);
-  return {prefix, cum, reinterpret_cast<const int2*>(cum + paged_round4(max_items + 1))};
+static_assert(sizeof(PagedItem) == 32, "two 16-byte loads");
+// PW_ITEMS of them.
+inline __host__ __device__ const PagedItem* paged_items(const int* work) {
+  return reinterpret_cast<const PagedItem*>(work + PW_HEADER);
 }
 
 // Checks of a caller's descriptors; `who` opens the error message.

@@ -13,6 +13,8 @@
 #include <cuda.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "internal.h"
 #include "kv_cache.cuh"
 #include "paged.cuh"
@@ -28,8 +30,8 @@ struct PagedAttnArgs {
   PagedView c;
   const int* table;
   int max_pages;
-  const int *starts, *lens, *header;
-  PagedWork w;
+  const int* header;  // the batch's work words
+  int max_items;
   int G, out_rows;
   unsigned inv_G;    // ceil(2^32 / G): r / G = r * inv_G >> 32 (G > 1)
   float scale_log2;  // scale * log2(e), or scale / cap where there is a cap
@@ -93,52 +95,106 @@ __device__ __forceinline__ void pa_tma(void* dst, const CUtensorMap* map, int x,
       : "memory");
 }
 
-// A run of tiles, piece by piece.
+// A piece of a unit, as the producer warp hands it on in shared memory.
 struct PagedPiece {
-  int kvh, item, b, i;  // kv head; item of the batch, its request and place there
-  int t0, t1, tn;       // this CTA's tiles of the unit, and all of them
+  PagedItem it;  // tile0, tiles: the unit's, of all (kv head, item) units' tiles
+  int kvh, unit;
+  int t0, t1;    // this CTA's tiles of the unit
+  int rows;      // of the item, that there are rows of q for
+  int least;     // positions below it are seen by every row of the item
+  int poison;    // V has values that are not finite where not every row looks
+  int last;      // no piece: the run is over
 };
+// The share of tiles that a CTA takes.
 struct PagedRun {
   int64_t x, end, share;
   int items, tiles;
-  PagedPiece p;
+  int kvh, item;
+  PagedItem it;  // of `item`
 };
-// The first unit of the run [x, end): all threads of the CTA, `slot` in shared memory.
-__device__ __forceinline__ bool run_begin(const PagedAttnArgs& a, PagedRun& r, int* slot) {
-  r.items = __ldcg(a.header + PW_ITEMS);
-  r.tiles = __ldcg(a.header + PW_TILES);
+struct PagedFound {
+  PagedItem it;
+  int item;
+};
+__device__ __forceinline__ PagedItem load_item(const PagedItem* p) {
+  const int4 u = __ldcg(reinterpret_cast<const int4*>(p)), v = __ldcg(reinterpret_cast<const int4*>(p) + 1);
+  return {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+}
+// The first unit of this CTA's run; false (in all threads, before any barrier) if
+// there is none.  The list's first items are read along with its length: one round
+// trip where the item is among them.
+__device__ __forceinline__ bool run_begin(const PagedAttnArgs& a, PagedRun& r, PagedFound* found) {
+  const PagedItem* list = paged_items(a.header);
+  int i = threadIdx.x;
+  PagedItem x{};
+  const int2 head = __ldcg(reinterpret_cast<const int2*>(a.header) + PW_ITEMS / 2);
+  static_assert(PW_ITEMS == 2 && PW_TILES == 3, "one load");
+  if (i < a.max_items) x = load_item(list + i);
+  r.items = head.x, r.tiles = head.y;
   const int64_t all = (int64_t)r.tiles * a.c.kv_heads;
   r.share = max((all + gridDim.x - 1) / gridDim.x, (int64_t)a.least);
   r.x = r.share * blockIdx.x;
   r.end = min(all, r.x + r.share);
   if (r.x >= all) return false;
-  r.p.kvh = (int)(r.x / r.tiles);
-  const int rem = (int)(r.x - (int64_t)r.p.kvh * r.tiles);
-  for (int i = threadIdx.x; i < r.items; i += blockDim.x)
-    if (__ldcg(a.w.cum + i) <= rem && rem < __ldcg(a.w.cum + i + 1)) *slot = i;
+  r.kvh = (int)(r.x / r.tiles);
+  const int rem = (int)(r.x - (int64_t)r.kvh * r.tiles);
+  while (i < r.items) {
+    if (x.tile0 <= rem && rem < x.tile0 + x.tiles) found->it = x, found->item = i;
+    i += blockDim.x;
+    if (i < r.items) x = load_item(list + i);
+  }
   __syncthreads();
-  r.p.item = *slot;
+  r.it = found->it, r.item = found->item;
   return true;
 }
 // The piece at x, and x moved past it.
-__device__ __forceinline__ void run_piece(const PagedAttnArgs& a, PagedRun& r) {
-  const int c0 = __ldcg(a.w.cum + r.p.item), c1 = __ldcg(a.w.cum + r.p.item + 1);
-  const int2 info = __ldcg(a.w.info + r.p.item);
-  r.p.b = info.x, r.p.i = info.y;
-  r.p.tn = c1 - c0;
-  r.p.t0 = (int)(r.x - (int64_t)r.p.kvh * r.tiles) - c0;
-  r.p.t1 = (int)min((int64_t)r.p.tn, r.p.t0 + (r.end - r.x));
-  r.x += max(1, r.p.t1 - r.p.t0);
+__device__ __forceinline__ PagedPiece run_piece(const PagedAttnArgs& a, PagedRun& r, int rows_per_item) {
+  PagedPiece p;
+  p.it = r.it;
+  p.kvh = r.kvh, p.unit = r.kvh * r.items + r.item;
+  p.t0 = (int)(r.x - (int64_t)r.kvh * r.tiles) - r.it.tile0;
+  p.t1 = (int)min((int64_t)r.it.tiles, p.t0 + (r.end - r.x));
+  p.rows = min(rows_per_item, min(r.it.len - r.it.past, a.out_rows - r.it.start) * a.G - r.it.i * rows_per_item);
+  p.least = paged_limit(r.it.past, pa_token(a, r.it.i * rows_per_item), r.it.len, r.it.prefix);
+  p.poison = p.last = 0;
+  r.x += max(1, p.t1 - p.t0);
+  return p;
 }
-__device__ __forceinline__ void run_next(PagedRun& r) {
-  if (++r.p.item == r.items) r.p.item = 0, ++r.p.kvh;
+__device__ __forceinline__ void run_next(const PagedAttnArgs& a, PagedRun& r) {
+  if (++r.item == r.items) r.item = 0, ++r.kvh;
+  r.it = load_item(paged_items(a.header) + r.item);
+}
+// Where a unit's pieces are: CTA c's first tile is c * share; what begins the unit
+// is the CTA's second place, what goes on with one its first.
+__device__ __forceinline__ int64_t unit_tile(const PagedRun& r, const PagedPiece& p) {
+  return (int64_t)p.kvh * r.tiles + p.it.tile0;
+}
+__device__ __forceinline__ float* piece_part(const PagedAttnArgs& a, const PagedRun& r, int64_t cta, int64_t ux, int stride) {
+  return a.part + (2 * cta + (r.share * cta <= ux ? 1 : 0)) * stride;
 }
 
+// Devices whose kernel may take its shared memory; set again by whoever comes twice
+// at once, which changes nothing.
+struct PagedReady {
+  std::atomic<uint64_t> devices{0};
+  cudaError_t set(const void* kern, int smem) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    if (dev < 64 && devices.load(std::memory_order_acquire) >> dev & 1) return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) return e;
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared))
+      return e;
+    if (dev < 64) devices.fetch_or(1ull << dev, std::memory_order_release);
+    return cudaSuccess;
+  }
+};
+
 cudaError_t paged_maps(const PagedView& c, int tile, CUtensorMap* maps);
-cudaError_t launch_paged_mma(PagedAttnArgs& a, int mt, bool fancy, cudaStream_t s);
+cudaError_t launch_paged_mma(PagedAttnArgs& a, int groups, bool fancy, cudaStream_t s);
 cudaError_t launch_paged_tc(PagedAttnArgs& a, bool fancy, cudaStream_t s);
 
 constexpr int PAGED_SMS = 148, PAGED_ROWS_MAX = 256;
-constexpr int paged_ctas(int rows) { return rows <= 32 ? 2 * PAGED_SMS : PAGED_SMS; }
+// CTAs of a call: two per SM of the narrow kernel, else one
+constexpr int paged_ctas(int rows) { return rows <= 16 ? 2 * PAGED_SMS : PAGED_SMS; }
 
 }  // namespace odi_cuda

@@ -109,14 +109,9 @@ __device__ __forceinline__ void st32(const uint32_t* r, uint32_t addr) {
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-struct Piece {  // a piece, as the producer hands it on
+struct Piece {
   PagedPiece p;
-  int start, past, len, prefix;
-  int rows;    // of the item, that there are rows of q for
   int end[2];  // tiles of the unit that each half of its rows sees
-  int least;   // positions below it are seen by every row
-  int poison;  // V has values that are not finite where not every row looks
-  int last;    // no piece: the run is over
 };
 struct Bars {
   uint64_t full[8], empty[8];
@@ -136,7 +131,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   __shared__ Bars bars;
   __shared__ Piece pieces[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int first_item, is_last;
+  __shared__ PagedFound found;
+  __shared__ int is_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   pdl_launch_dependents();
@@ -153,7 +149,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(&bars.v_clean, 128);
     mbar_init(&bars.join, 256);
     mbar_init(&bars.drain, 1);
-    first_item = 0;
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -167,7 +162,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = tmem_slot;
   pdl_wait();
   PagedRun run;
-  const bool any = run_begin(a, run, &first_item);  // has a barrier, unless it returns false in all threads
+  const bool any = run_begin(a, run, &found);  // has a barrier, unless it returns false in all threads
   const int P = a.c.page_size;
   auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, a.err, ERR_PAGED_WAIT); };
 
@@ -181,11 +176,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     int n = 0, k = 0;  // tiles (of K or V) and pieces so far
     bool ok = true;
     while (ok && run.x < run.end) {
-      run_piece(a, run);
-      const PagedPiece p = run.p;
-      const int len = __ldcg(a.lens + p.b), start = __ldcg(a.starts + p.b), n_new = __ldcg(a.starts + p.b + 1) - start;
-      const int prefix = __ldcg(a.w.prefix + p.b);
-      const int* row = a.table + (int64_t)p.b * a.max_pages;
+      const PagedPiece p = run_piece(a, run, ROWS);
+      const int len = p.it.len;
+      const int* row = a.table + (int64_t)p.it.b * a.max_pages;
       auto entry = [&](int t) {
         const int pos = t * TILE + box * BR;
         return box < boxes && t < p.t1 && pos < len ? __ldcg(row + (pos >> a.c.page_shift)) : -1;
@@ -195,19 +188,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) {
         Piece& d = pieces[k & 1];
         d.p = p;
-        d.start = start, d.len = len, d.past = len - n_new, d.prefix = prefix;
-        const int all = min(ROWS, n_new * a.G - p.i * ROWS);
-        d.rows = min(all, (a.out_rows - start) * a.G - p.i * ROWS);
+        const int all = min(ROWS, (len - p.it.past) * a.G - p.it.i * ROWS);
         for (int h = 0; h < 2; ++h) {
-          const int last_row = p.i * ROWS + min(all, (h + 1) * HALF_ROWS) - 1;
-          const int tiles = (paged_limit(len - n_new, pa_token(a, last_row), len, prefix) + TILE - 1) / TILE;
+          const int last_row = p.it.i * ROWS + min(all, (h + 1) * HALF_ROWS) - 1;
+          const int tiles = (paged_limit(p.it.past, pa_token(a, last_row), len, p.it.prefix) + TILE - 1) / TILE;
           d.end[h] = all > h * HALF_ROWS ? max(p.t0, min(p.t1, tiles)) : p.t0;
         }
-        d.least = paged_limit(len - n_new, pa_token(a, p.i * ROWS), len, prefix);
-        d.poison = 0, d.last = 0;
         mbar_arrive(&bars.d_full[k & 1]);
       }
       ++k;
+      if (run.x < run.end) run_next(a, run);
       for (int t = p.t0; ok && t < p.t1; ++t) {
         const int pos = t * TILE + box * BR;
         const int next = entry(t + 1);
@@ -230,11 +220,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         page = next;
       }
-      run_next(run);
     }
     if (k < 2 || wait(&bars.d_empty[k & 1], k / 2 - 1)) {
       if (lane == 0) {
-        pieces[k & 1].last = 1;
+        pieces[k & 1].p.last = 1;
         mbar_arrive(&bars.d_full[k & 1]);
       }
     }
@@ -263,8 +252,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int k = 0; ok; ++k) {
       if (!wait(&bars.d_full[k & 1], k / 2)) break;
       const Piece& d = pieces[k & 1];
-      if (d.last) break;
-      const int t0 = d.p.t0, t1 = d.p.t1, least = d.least, end0 = d.end[0], end1 = d.end[1];
+      if (d.p.last) break;
+      const int t0 = d.p.t0, t1 = d.p.t1, least = d.p.least, end0 = d.end[0], end1 = d.end[1];
       auto end = [&](int h) { return h ? end1 : end0; };
       for (int t = t0 - 1; ok && t < t1; ++t) {
         const int sv = (n + 2 * (t - t0) + 1) % ST, iv = (n + 2 * (t - t0) + 1) / ST;
@@ -320,15 +309,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int k = 0; ok; ++k) {
       if (!wait(&bars.d_full[k & 1], k / 2)) break;
       Piece& d = pieces[k & 1];
-      if (d.last) break;
+      if (d.p.last) break;
       const PagedPiece p = d.p;
-      const int start = d.start, past = d.past, len = d.len, rows = d.rows, t0 = p.t0, t1 = p.t1, t_end = d.end[h], end1 = d.end[1];
-      const int least = d.least;
+      const int start = p.it.start, past = p.it.past, len = p.it.len, rows = p.rows, least = p.least;
+      const int t0 = p.t0, t1 = p.t1, t_end = d.end[h], end1 = d.end[1];
       const bool mine = t_end > t0;
-      const int R = p.i * ROWS + row, token = pa_token(a, R), head = p.kvh * a.G + R - token * a.G;
-      const int lim = row < rows ? paged_limit(past, token, len, d.prefix) : 0;
+      const int R = p.it.i * ROWS + row, token = pa_token(a, R), head = p.kvh * a.G + R - token * a.G;
+      const int lim = row < rows ? paged_limit(past, token, len, p.it.prefix) : 0;
       // positions below it are seen by all rows of this half
-      const int least_h = paged_limit(past, pa_token(a, p.i * ROWS + h * HALF_ROWS), len, d.prefix);
+      const int least_h = paged_limit(past, pa_token(a, p.it.i * ROWS + h * HALF_ROWS), len, p.it.prefix);
       const float slope = FANCY && a.slopes && row < rows ? __ldg(a.slopes + head) * 1.4426950408889634f : 0.f;
       if (mine) {
         // Q: 16-byte pieces, HD / 8 to a row
@@ -339,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int r = i / PER, ch = i % PER;
           uint4 x = make_uint4(0, 0, 0, 0);
           if (h * HALF_ROWS + r < rows) {
-            const int RR = p.i * ROWS + h * HALF_ROWS + r, tk = pa_token(a, RR);
+            const int RR = p.it.i * ROWS + h * HALF_ROWS + r, tk = pa_token(a, RR);
             const T* src = q + (int64_t)(start + tk) * a.ld_q + (int64_t)(p.kvh * a.G + RR - tk * a.G) * HD + ch * 8;
             if (a.vec) {
               x = __ldcg(reinterpret_cast<const uint4*>(src));
@@ -437,7 +426,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (any_bad) *reinterpret_cast<uint4*>(x) = make_uint4(z[0], z[1], z[2], z[3]);
               bad = bad || any_bad;
             }
-            if (bad && pos < len) d.poison = 1;
+            if (bad && pos < len) d.p.poison = 1;
           }
           fence_proxy_async_smem();
           mbar_arrive(&bars.v_clean);
@@ -453,9 +442,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         fence_after();
       }
       const float L = sum.x + sum.y;
-      const bool whole = t0 == 0 && t1 == p.tn, fix = d.poison != 0;
-      const int64_t ux = (int64_t)p.kvh * run.tiles + __ldcg(a.w.cum + p.item);
-      float* part = a.part + (int64_t)(2 * blockIdx.x + (run.share * blockIdx.x <= ux ? 1 : 0)) * ROWS * (HD + 2);
+      const bool whole = t0 == 0 && t1 == p.it.tiles, fix = d.p.poison != 0;
+      const int64_t ux = unit_tile(run, p);
+      constexpr int STRIDE = ROWS * (HD + 2);
+      float* part = piece_part(a, run, blockIdx.x, ux, STRIDE);
       auto store = [&](const float (&v)[32], int c) {  // 32 values of the row from dim c on
         const int64_t at = (int64_t)(start + token) * a.ld_out + (int64_t)head * HD + c;
         if (a.out32) {
@@ -488,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]);
           if (fix)
             for (int j = max(t0 * TILE, least); j < min(t1 * TILE, lim); ++j) {
-              const int page = __ldcg(a.table + (int64_t)p.b * a.max_pages + (j >> a.c.page_shift));
+              const int page = __ldcg(a.table + (int64_t)p.it.b * a.max_pages + (j >> a.c.page_shift));
               if ((unsigned)page >= (unsigned)a.c.num_pages) continue;
               const unsigned short* src = reinterpret_cast<const unsigned short*>(a.c.v) +
                                           (((int64_t)page * a.c.kv_heads + p.kvh) * P + (j & (P - 1))) * HD + c;
@@ -512,19 +502,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!whole) {
         *reinterpret_cast<float2*>(part + ROWS * HD + 2 * row) = make_float2(ref, L);
-        const int64_t c_first = ux / run.share, c_last = (ux + p.tn - 1) / run.share;
-        const int unit = p.kvh * run.items + p.item;
+        const int64_t c_first = ux / run.share, c_last = (ux + p.it.tiles - 1) / run.share;
         __threadfence();
         mbar_arrive(&bars.join);
         ok = wait(&bars.join, joins++);
         if (!ok) break;
-        if (tid == 0) is_last = atomicAdd(a.count + unit, 1) == (int)(c_last - c_first);
+        if (tid == 0) is_last = atomicAdd(a.count + p.unit, 1) == (int)(c_last - c_first);
         mbar_arrive(&bars.join);
         ok = wait(&bars.join, joins++);
         if (!ok) break;
         if (is_last) {
           __threadfence();
-          auto piece = [&](int64_t c) { return a.part + (2 * c + (run.share * c <= ux ? 1 : 0)) * ROWS * (HD + 2); };
+          auto piece = [&](int64_t c) { return piece_part(a, run, c, ux, STRIDE); };
           float top = -INFINITY, all = 0.f;
           for (int64_t c = c_first; c <= c_last; ++c)
             top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row)).x);
@@ -554,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int e = 0; e < 32; ++e) v[e] *= inv;
             if (row < rows) store(v, d0);
           }
-          if (tid == 0) a.count[unit] = 0;
+          if (tid == 0) a.count[p.unit] = 0;
         }
         // nobody sets is_last again before all have read it
         mbar_arrive(&bars.join);
@@ -580,13 +569,8 @@ static cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
   auto kern = paged_tc_kernel<T, HD, FANCY>;
   CUtensorMap maps[2];
   if (cudaError_t e = paged_maps(a.c, TILE, maps)) return e;
-  static thread_local uint64_t ready = 0;  // devices whose kernel may take this much shared memory
-  int dev = 0;
-  if (cudaError_t e = cudaGetDevice(&dev)) return e;
-  if (dev > 63 || !(ready >> dev & 1)) {
-    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM)) return e;
-    if (dev < 64) ready |= 1ull << dev;
-  }
+  static PagedReady ready;
+  if (cudaError_t e = ready.set((const void*)kern, F::SMEM)) return e;
   return launch_pdl_smem(kern, dim3(paged_ctas(ROWS)), dim3(THREADS), F::SMEM, s, a, maps[0], maps[1]);
 }
 

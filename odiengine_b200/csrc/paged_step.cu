@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_consta
     }
   }
   if (rank == C - 1) {  // attention's work list, in the order of rows
-    const PagedWork work = paged_work(a.b.work, B, a.g.max_items);
+    PagedItem* list = const_cast<PagedItem*>(paged_items(a.b.work));
     int* s_item0 = s_drop0;
     base = {0, 0, 0};
     for (int b0 = 0; b0 < B; b0 += THREADS) {
@@ -204,10 +204,7 @@ __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_consta
       if (b < B && s_take0[b] >= 0) items = (int)(((int64_t)(s_row0[b + 1] - s_row0[b]) * a.g.G + a.g.rows - 1) / a.g.rows);
       Sum3 total;
       const Sum3 e = block_scan({items, 0, 0}, &total, warps);
-      if (b < B) {
-        s_item0[b] = base.a + e.a;
-        const_cast<int*>(work.prefix)[b] = a.prefix ? __ldcg(a.prefix + b) : 0;
-      }
+      if (b < B) s_item0[b] = base.a + e.a;
       base.a += total.a;
     }
     const int items = base.a;
@@ -215,21 +212,21 @@ __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_consta
     __syncthreads();
     for (int i0 = 0; i0 < items; i0 += THREADS) {
       const int i = i0 + tid;
-      int tiles = 0;
+      PagedItem x{};
       if (i < items) {
         const int b = last_at_most(s_item0, B, i), k = i - s_item0[b], n_rows = s_row0[b + 1] - s_row0[b];
         const int token = (int)((min((int64_t)n_rows * a.g.G, (int64_t)(k + 1) * a.g.rows) - 1) / a.g.G);
-        const int lim = paged_limit(s_keep[b], token, s_keep[b] + n_rows, a.prefix ? __ldcg(a.prefix + b) : 0);
-        tiles = (lim + a.g.tile - 1) / a.g.tile;
-        const_cast<int2*>(work.info)[i] = make_int2(b, k);
+        x.b = b, x.i = k, x.start = s_row0[b], x.past = s_keep[b], x.len = s_keep[b] + n_rows;
+        x.prefix = a.prefix ? __ldcg(a.prefix + b) : 0;
+        x.tiles = (paged_limit(x.past, token, x.len, x.prefix) + a.g.tile - 1) / a.g.tile;
       }
       Sum3 total;
-      const Sum3 e = block_scan({tiles, 0, 0}, &total, warps);
-      if (i < items) const_cast<int*>(work.cum)[i] = base.a + e.a;
+      const Sum3 e = block_scan({x.tiles, 0, 0}, &total, warps);
+      x.tile0 = base.a + e.a;
+      if (i < items) list[i] = x;
       base.a += total.a;
     }
     if (tid == 0) {
-      const_cast<int*>(work.cum)[items] = base.a;
       a.b.work[PW_ITEMS] = items;
       a.b.work[PW_TILES] = base.a;
     }
@@ -311,7 +308,7 @@ extern "C" {
 size_t odi_cuda_paged_work_bytes(int requests, int max_rows, int max_new, int heads, int kv_heads) {
   PagedGeometry g;
   if (!paged_geometry(requests, max_rows, max_new, heads, kv_heads, &g)) return 0;
-  return 4 * (size_t)(PW_HEADER + paged_round4(requests) + paged_round4(g.max_items + 1) + 2 * g.max_items);
+  return 4 * (size_t)PW_HEADER + sizeof(PagedItem) * (size_t)g.max_items;
 }
 
 int odi_cuda_paged_step(const odi_cuda_page_tables* t, const odi_cuda_paged_batch* batch, const int32_t* d_keep,
