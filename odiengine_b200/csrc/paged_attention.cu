@@ -53,7 +53,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
                : "memory");
 }
 
-// MG: groups of 16 rows.  One group: two CTAs of 113 KB per SM; two: one CTA.
+// MG: groups of 16 rows.  One group: two CTAs per SM; two: one.
 template <int HD, int MG>
 struct Cfg {
   static constexpr int PLANE = TILE * 128, SLOT = HD / 64 * PLANE;  // K or V of one tile
@@ -61,9 +61,14 @@ struct Cfg {
   static constexpr int FOLD = 4 * 16 * HD * 4;  // a group's sums
   static constexpr int FOLD_OFF = ST * SLOT;
   static constexpr int SMEM = FOLD_OFF + MG * FOLD;
-  static constexpr int THREADS = 128 * MG + 32, PER_SM = MG == 1 ? 2 : 1;
+  static constexpr int THREADS = 128 * MG + 128, PER_SM = MG == 1 ? 2 : 1;
+  // the launch's registers are shared out anew: a warp at the products holds O (64),
+  // Q (32) and operands
+  static constexpr int REGS_LAUNCH = MG == 1 ? 128 : 168, REGS_FEW = 80, REGS_MMA = MG == 1 ? 176 : 208;
+  static_assert(128 * REGS_FEW + 128 * MG * REGS_MMA <= THREADS * REGS_LAUNCH, "register split");
   static_assert(PER_SM * (SMEM + 2048) <= 228 * 1024, "shared memory, with 1 KB static and 1 KB of the system's");
 };
+constexpr int JOINERS = 96;  // threads that join and write out
 
 template <typename T, int HD, int MG, bool FANCY>
 __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
@@ -73,7 +78,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   using H = Half16<T>;
   constexpr int KS = HD / 16, ROWS = 16 * MG, ST = F::ST, PLANES = HD / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t full[ST], empty[ST], d_full[2], d_empty[2], cbar;
+  __shared__ uint64_t full[ST], empty[ST], d_full[2], d_empty[2], fold_full, fold_empty, jbar;
   __shared__ PagedPiece pieces[2];
   __shared__ float2 wml[4 * MG][16];
   __shared__ PagedFound found;
@@ -83,9 +88,12 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 4 * MG);
-    for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4 * MG);
-    mbar_init(&cbar, 128 * MG);
+    for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4 * MG + 3);
+    mbar_init(&fold_full, 4 * MG);
+    mbar_init(&fold_empty, 3);
+    mbar_init(&jbar, JOINERS);
     fence_mbar_init();
+    prefetch_map(&kmap), prefetch_map(&vmap);
   }
   __syncthreads();
   pdl_wait();
@@ -94,6 +102,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   const int P = a.c.page_size;
   auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, a.err, ERR_PAGED_WAIT); };
 
+  if (warp >= 4 * MG) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_FEW));
   if (warp == 4 * MG) {
     // ---- producer: a lane brings one box of K or V, one 64-dim half of it
     const int BR = min(P, TILE), boxes = TILE / BR;
@@ -104,12 +114,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     while (ok && run.x < run.end) {
       const PagedPiece p = run_piece(a, run, ROWS);
       const int len = p.it.len;
-      const int* row = a.table + (int64_t)p.it.b * a.max_pages;
-      auto entry = [&](int t) {
-        const int pos = t * TILE + box * BR;
-        return box < boxes && t < p.t1 && pos < len ? __ldcg(row + (pos >> a.c.page_shift)) : -1;
-      };
-      int page = entry(p.t0);
+      PagedNames names(a, p, TILE);
       if (k >= 2 && !wait(&d_empty[k & 1], k / 2 - 1)) break;
       if (lane == 0) {
         pieces[k & 1] = p;
@@ -119,8 +124,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       if (run.x < run.end) run_next(a, run);
       for (int t = p.t0; ok && t < p.t1; ++t) {
         const int pos = t * TILE + box * BR;
-        const int next = entry(t + 1);
         const int live = min(boxes, (len - t * TILE + BR - 1) / BR);
+        const int page = names.at(pos >> a.c.page_shift);
         int y = (page * a.c.kv_heads + p.kvh) * P + (pos & (P - 1));
         if (box < live && (unsigned)page >= (unsigned)a.c.num_pages) {  // names no page: zeros, and the error word
           y = rows_all;
@@ -136,7 +141,6 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
           __syncwarp();
           if (box < live) pa_tma(smem + s * F::SLOT + plane * F::PLANE + box * BR * 128, v ? &vmap : &kmap, plane * 64, y, &full[s]);
         }
-        page = next;
       }
     }
     if (ok && (k < 2 || wait(&d_empty[k & 1], k / 2 - 1)) && lane == 0) {
@@ -147,15 +151,148 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     return;
   }
 
-  // ---- consumers: a warp has 16 rows and positions 16 wq .. + 15 of every tile
+  // ---- joins, beside the products of the next piece: the four warps of a group,
+  // and the pieces of a unit
+  const int jt = tid - (128 * MG + 32);
+  const float* folds = reinterpret_cast<const float*>(smem + F::FOLD_OFF);
+  int syncs = 0;
+  auto sync = [&]() {  // of the joiners, bounded
+    mbar_arrive(&jbar);
+    return wait(&jbar, syncs++);
+  };
+  for (int k = 0;; ++k) {
+    if (!wait(&d_full[k & 1], k / 2)) return;
+    const PagedPiece& p = pieces[k & 1];
+    if (p.last) return;
+    const int t0 = p.t0, t1 = p.t1, rows = p.rows, least = p.least, len = p.it.len;
+    const bool whole = t0 == 0 && t1 == p.it.tiles;
+    constexpr int STRIDE = ROWS * (HD + 2);
+    float* part = piece_part(a, p, blockIdx.x, STRIDE);
+    // a row's value divided by its sum, to where it goes
+    auto store = [&](int r, int d, float4 v, float inv) {
+      v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
+      const int R = p.it.i * ROWS + r, token = pa_token(a, R);
+      const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)(p.kvh * a.G + R - token * a.G) * HD + d;
+      if (a.out32) {
+        float* y = static_cast<float*>(a.out) + at;
+        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
+      } else {
+        uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at);
+        const uint32_t lo = H::pack(v.x, v.y), hi = H::pack(v.z, v.w);
+        if (a.vec_out) *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
+        else y[0] = lo, y[1] = hi;
+      }
+    };
+    if (!wait(&fold_full, k)) return;
+    const bool fix = p.poison;
+#pragma unroll 1
+    for (int i = jt; i < rows * (HD / 4); i += JOINERS) {
+      const int r = i / (HD / 4), d = i % (HD / 4) * 4, mg = r >> 4, fr = r & 15;
+      float2 ml[4];
+      float top = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) ml[w] = wml[mg * 4 + w][fr], top = fmaxf(top, ml[w].x);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = ml[w].x == top ? 1.f : pa_ex2(ml[w].x - top);
+        L += ml[w].y * f;
+        const float4 x = *reinterpret_cast<const float4*>(folds + mg * (F::FOLD / 4) + (w * 16 + fr) * HD +
+                                                          (((d >> 3) ^ (fr & 7)) & (HD / 8 - 1)) * 8 + (d & 4));
+        v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
+      }
+      if (fix) {
+        const int row_lim = paged_limit(p.it.past, pa_token(a, p.it.i * ROWS + r), len, p.it.prefix);
+        for (int j = max(t0 * TILE, least); j < min(t1 * TILE, row_lim); ++j) {
+          const int page = __ldcg(a.table + (int64_t)p.it.b * a.max_pages + (j >> a.c.page_shift));
+          if ((unsigned)page >= (unsigned)a.c.num_pages) continue;
+          const unsigned short* src = static_cast<const unsigned short*>(a.c.v) +
+                                      (((int64_t)page * a.c.kv_heads + p.kvh) * P + (j & (P - 1))) * HD + d;
+          float y[4];
+          for (int e = 0; e < 4; ++e) {
+            y[e] = H::up(__ldcg(src + e));
+            if (fabsf(y[e]) <= 3.402823466e38f) y[e] = 0.f;
+          }
+          v.x += y[0], v.y += y[1], v.z += y[2], v.w += y[3];
+        }
+      }
+      if (whole) {
+        store(r, d, v, L == 0.f ? 0.f : 1.f / L);
+      } else {
+        *reinterpret_cast<float4*>(part + r * HD + d) = v;
+        if (d == 0) *reinterpret_cast<float2*>(part + ROWS * HD + 2 * r) = make_float2(top, L);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&fold_empty);
+    if (!whole) {
+      // the last piece to arrive joins them all
+      const int c0 = p.c0, c1 = p.c1;
+      if (!sync()) return;
+      if (jt == 0) {
+        __threadfence();
+        is_last = atomicAdd(a.count + p.unit, 1) == c1 - c0;
+        __threadfence();
+      }
+      if (!sync()) return;
+      if (is_last) {
+        // three places of the unit by two pieces at a time, so that loads overlap
+#pragma unroll 1
+        for (int i0 = jt; i0 < rows * (HD / 4); i0 += 3 * JOINERS) {
+          float top[3], L[3];
+          float4 v[3];
+          int at[3];
+#pragma unroll
+          for (int u = 0; u < 3; ++u) {
+            top[u] = -INFINITY, L[u] = 0.f, v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            at[u] = min(i0 + u * JOINERS, rows * (HD / 4) - 1);
+          }
+#pragma unroll 1
+          for (int q0 = c0; q0 <= c1; q0 += 2) {
+            float2 ml[3][2];
+            float4 x[3][2];
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const float* src = piece_part(a, p, min(q0 + w, c1), STRIDE);
+#pragma unroll
+              for (int u = 0; u < 3; ++u) {
+                ml[u][w] = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * (at[u] / (HD / 4))));
+                x[u][w] = __ldcg(reinterpret_cast<const float4*>(src) + at[u]);
+              }
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              if (q0 + w > c1) break;
+#pragma unroll
+              for (int u = 0; u < 3; ++u) {
+                const float now = fmaxf(top[u], ml[u][w].x);
+                const float fo = top[u] == now ? 1.f : pa_ex2(top[u] - now), fn = ml[u][w].x == now ? 1.f : pa_ex2(ml[u][w].x - now);
+                top[u] = now;
+                L[u] = L[u] * fo + ml[u][w].y * fn;
+                v[u].x = v[u].x * fo + x[u][w].x * fn, v[u].y = v[u].y * fo + x[u][w].y * fn;
+                v[u].z = v[u].z * fo + x[u][w].z * fn, v[u].w = v[u].w * fo + x[u][w].w * fn;
+              }
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 3; ++u)
+            if (i0 + u * JOINERS < rows * (HD / 4))
+              store(at[u] / (HD / 4), at[u] % (HD / 4) * 4, v[u], L[u] == 0.f ? 0.f : 1.f / L[u]);
+        }
+        if (jt == 0) a.count[p.unit] = 0;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&d_empty[k & 1]);
+  }
+  }
+
+  // ---- products: a warp has 16 rows and positions 16 wq .. + 15 of every tile
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REGS_MMA));
   const int g = lane >> 2, c = lane & 3, mg = warp >> 2, wq = warp & 3;
   const uint32_t base = smem_u32(smem);
   float* fold = reinterpret_cast<float*>(smem + F::FOLD_OFF + mg * F::FOLD);
-  int n = 0, syncs = 0;
-  auto sync = [&]() {  // of the consumers, bounded
-    mbar_arrive(&cbar);
-    return wait(&cbar, syncs++);
-  };
+  int n = 0;
   for (int k = 0;; ++k) {
     if (!wait(&d_full[k & 1], k / 2)) return;
     PagedPiece& p = pieces[k & 1];
@@ -199,12 +336,18 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         const int pr = wq * 16 + (lane >> 4) * 8 + (lane & 7);
         const uint32_t ka = base + sk * F::SLOT + pr * 128;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          uint32_t b[4];
-          const int chunk = 2 * ks + (lane >> 3 & 1);
-          ldsm4(b, ka + (chunk >> 3) * F::PLANE + (((chunk & 7) ^ (pr & 7)) << 4));
-          mma<T>(sc[0], qf[ks], b[0], b[1]);
-          mma<T>(sc[1], qf[ks], b[2], b[3]);
+        for (int k0 = 0; k0 < KS; k0 += 4) {
+          uint32_t b[4][4];
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            const int chunk = 2 * (k0 + ks) + (lane >> 3 & 1);
+            ldsm4(b[ks], ka + (chunk >> 3) * F::PLANE + (((chunk & 7) ^ (pr & 7)) << 4));
+          }
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {
+            mma<T>(sc[0], qf[k0 + ks], b[ks][0], b[ks][1]);
+            mma<T>(sc[1], qf[k0 + ks], b[ks][2], b[ks][3]);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -262,28 +405,36 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         const uint32_t va = base + sv * F::SLOT + pr * 128;
         const int j0 = pw + 2 * c;
 #pragma unroll
-        for (int dt = 0; dt < KS; ++dt) {
-          uint32_t b[4];
-          const int chunk = 2 * dt + (lane >> 4);
-          ldsm4_t(b, va + (chunk >> 3) * F::PLANE + (((chunk & 7) ^ (pr & 7)) << 4));
+        for (int d0 = 0; d0 < KS; d0 += 4) {
+          uint32_t b[4][4];
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            const int chunk = 2 * (d0 + dt) + (lane >> 4);
+            ldsm4_t(b[dt], va + (chunk >> 3) * F::PLANE + (((chunk & 7) ^ (pr & 7)) << 4));
+          }
           if (masked) {
             // What not every row sees must not reach the rows that do not: 0 * NaN is
             // NaN.  Values that are not finite leave here; rows that see them get them
             // when the piece ends.
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int j = j0 + (i & 1) * 8 + e;
-                const uint32_t ex = H::EXP << (16 * e);
-                if (j >= least && (b[i] & ex) == ex) {
-                  b[i] &= ~(0xffffu << (16 * e));
-                  bad = bad || j < len;
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int j = j0 + (i & 1) * 8 + e;
+                  const uint32_t ex = H::EXP << (16 * e);
+                  if (j >= least && (b[dt][i] & ex) == ex) {
+                    b[dt][i] &= ~(0xffffu << (16 * e));
+                    bad = bad || j < len;
+                  }
                 }
-              }
           }
-          mma<T>(o[2 * dt], pf, b[0], b[1]);
-          mma<T>(o[2 * dt + 1], pf, b[2], b[3]);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            mma<T>(o[2 * (d0 + dt)], pf, b[dt][0], b[dt][1]);
+            mma<T>(o[2 * (d0 + dt) + 1], pf, b[dt][2], b[dt][3]);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -291,11 +442,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       if (lane == 0) mbar_arrive(&empty[sv]);
     }
 
-    // ---- the piece is over: the four warps of a group join
-    const bool whole = t0 == 0 && t1 == p.it.tiles;
-    const int64_t ux = unit_tile(run, p);
-    constexpr int STRIDE = ROWS * (HD + 2);
-    float* part = piece_part(a, run, blockIdx.x, ux, STRIDE);
+    // ---- the piece is over: to the joiners
+    if (k > 0 && !wait(&fold_empty, k - 1)) return;
     if (live_group) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -310,105 +458,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       }
       if (bad) p.poison = 1;
     }
-    if (!sync()) return;
-    // a row's value divided by its sum, to where it goes
-    auto store = [&](int r, int d, float4 v, float inv) {
-      v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
-      const int R = p.it.i * ROWS + r, token = pa_token(a, R);
-      const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)(p.kvh * a.G + R - token * a.G) * HD + d;
-      if (a.out32) {
-        float* y = static_cast<float*>(a.out) + at;
-        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
-      } else {
-        uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at);
-        const uint32_t lo = H::pack(v.x, v.y), hi = H::pack(v.z, v.w);
-        if (a.vec_out) *reinterpret_cast<uint2*>(y) = make_uint2(lo, hi);
-        else y[0] = lo, y[1] = hi;
-      }
-    };
-    const int gt = tid & 127, fr = gt >> 3;  // the row of the group that this thread joins
-    if (fr < rows) {
-      const int r = mg * 16 + fr;
-      float2 ml[4];
-      float top = -INFINITY, L = 0.f, f[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) ml[w] = wml[mg * 4 + w][fr], top = fmaxf(top, ml[w].x);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        f[w] = ml[w].x == top ? 1.f : pa_ex2(ml[w].x - top);
-        L += ml[w].y * f[w];
-      }
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      const bool fix = p.poison;
-#pragma unroll
-      for (int d0 = 0; d0 < HD; d0 += 32) {
-        const int d = d0 + (gt & 7) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(fold + (w * 16 + fr) * HD + (((d >> 3) ^ (fr & 7)) & (HD / 8 - 1)) * 8 + (d & 4));
-          v.x = fmaf(x.x, f[w], v.x), v.y = fmaf(x.y, f[w], v.y), v.z = fmaf(x.z, f[w], v.z), v.w = fmaf(x.w, f[w], v.w);
-        }
-        if (fix) {
-          const int row_lim = paged_limit(past, pa_token(a, R0 + fr), len, p.it.prefix);
-          for (int j = max(t0 * TILE, least); j < min(t1 * TILE, row_lim); ++j) {
-            const int page = __ldcg(a.table + (int64_t)p.it.b * a.max_pages + (j >> a.c.page_shift));
-            if ((unsigned)page >= (unsigned)a.c.num_pages) continue;
-            const unsigned short* src = static_cast<const unsigned short*>(a.c.v) +
-                                        (((int64_t)page * a.c.kv_heads + p.kvh) * P + (j & (P - 1))) * HD + d;
-            float y[4];
-            for (int e = 0; e < 4; ++e) {
-              y[e] = H::up(__ldcg(src + e));
-              if (fabsf(y[e]) <= 3.402823466e38f) y[e] = 0.f;
-            }
-            v.x += y[0], v.y += y[1], v.z += y[2], v.w += y[3];
-          }
-        }
-        if (whole) store(r, d, v, inv);
-        else *reinterpret_cast<float4*>(part + r * HD + d) = v;
-      }
-      if (!whole && (gt & 7) == 0) *reinterpret_cast<float2*>(part + ROWS * HD + 2 * r) = make_float2(top, L);
-    }
-    if (!whole) {
-      // the last piece to arrive joins them all
-      const int64_t c_first = ux / run.share, c_last = (ux + p.it.tiles - 1) / run.share;
-      __threadfence();
-      if (!sync()) return;
-      if (tid == 0) is_last = atomicAdd(a.count + p.unit, 1) == (int)(c_last - c_first);
-      if (!sync()) return;
-      if (is_last) {
-        __threadfence();
-        for (int i = tid; i < p.rows * (HD / 4); i += 128 * MG) {
-          const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-          float top = -INFINITY, L = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int64_t q0 = c_first; q0 <= c_last; q0 += 8) {
-            float2 ml[8];
-            float4 x[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              const float* src = piece_part(a, run, min(q0 + u, c_last), ux, STRIDE);
-              ml[u] = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * r));
-              x[u] = __ldcg(reinterpret_cast<const float4*>(src + r * HD + d));
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-              if (q0 + u > c_last) break;
-              const float now = fmaxf(top, ml[u].x);
-              const float fo = top == now ? 1.f : pa_ex2(top - now), fn = ml[u].x == now ? 1.f : pa_ex2(ml[u].x - now);
-              top = now;
-              L = L * fo + ml[u].y * fn;
-              v.x = v.x * fo + x[u].x * fn, v.y = v.y * fo + x[u].y * fn;
-              v.z = v.z * fo + x[u].z * fn, v.w = v.w * fo + x[u].w * fn;
-            }
-          }
-          store(r, d, v, L == 0.f ? 0.f : 1.f / L);
-        }
-        if (tid == 0) a.count[p.unit] = 0;
-      }
-    }
-    if (!sync()) return;  // fold, wml and is_last are read
-    if (lane == 0) mbar_arrive(&d_empty[k & 1]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&fold_full), mbar_arrive(&d_empty[k & 1]);
   }
 }
 
@@ -531,7 +582,9 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.slopes = d_slopes;
   a.vec = !((uintptr_t)d_q & 15) && !(ld_q & 7);
   a.vec_out = !((uintptr_t)d_out & 15) && !(ld_out & 7);
-  a.least = 1;
+  // a CTA takes three tiles at least: one token of 32 heads over 518 positions takes
+  // 11.2 us so, 12.9 with one tile and 15.0 with five
+  a.least = 3;
   a.err = static_cast<int*>(d_scratch);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + PART_OFF);
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + COUNT_OFF);

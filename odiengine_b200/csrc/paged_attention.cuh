@@ -95,11 +95,17 @@ __device__ __forceinline__ void pa_tma(void* dst, const CUtensorMap* map, int x,
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // A piece of a unit, as the producer warp hands it on in shared memory.
 struct PagedPiece {
   PagedItem it;  // tile0, tiles: the unit's, of all (kv head, item) units' tiles
   int kvh, unit;
   int t0, t1;    // this CTA's tiles of the unit
+  int c0, c1;    // the first and last CTA that have tiles of it
+  int first_place;  // CTA c0's place for its piece
   int rows;      // of the item, that there are rows of q for
   int least;     // positions below it are seen by every row of the item
   int poison;    // V has values that are not finite where not every row looks
@@ -116,6 +122,10 @@ struct PagedFound {
   PagedItem it;
   int item;
 };
+// a / b, both below 2^32 but for calls of absurd size.
+__device__ __forceinline__ int64_t pa_div(int64_t a, int64_t b) {
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
 __device__ __forceinline__ PagedItem load_item(const PagedItem* p) {
   const int4 u = __ldcg(reinterpret_cast<const int4*>(p)), v = __ldcg(reinterpret_cast<const int4*>(p) + 1);
   return {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
@@ -132,11 +142,11 @@ __device__ __forceinline__ bool run_begin(const PagedAttnArgs& a, PagedRun& r, P
   if (i < a.max_items) x = load_item(list + i);
   r.items = head.x, r.tiles = head.y;
   const int64_t all = (int64_t)r.tiles * a.c.kv_heads;
-  r.share = max((all + gridDim.x - 1) / gridDim.x, (int64_t)a.least);
+  r.share = max(pa_div(all + gridDim.x - 1, gridDim.x), (int64_t)a.least);
   r.x = r.share * blockIdx.x;
   r.end = min(all, r.x + r.share);
   if (r.x >= all) return false;
-  r.kvh = (int)(r.x / r.tiles);
+  r.kvh = (int)pa_div(r.x, r.tiles);
   const int rem = (int)(r.x - (int64_t)r.kvh * r.tiles);
   while (i < r.items) {
     if (x.tile0 <= rem && rem < x.tile0 + x.tiles) found->it = x, found->item = i;
@@ -157,6 +167,10 @@ __device__ __forceinline__ PagedPiece run_piece(const PagedAttnArgs& a, PagedRun
   p.rows = min(rows_per_item, min(r.it.len - r.it.past, a.out_rows - r.it.start) * a.G - r.it.i * rows_per_item);
   p.least = paged_limit(r.it.past, pa_token(a, r.it.i * rows_per_item), r.it.len, r.it.prefix);
   p.poison = p.last = 0;
+  const int64_t ux = (int64_t)r.kvh * r.tiles + r.it.tile0;  // the unit's first tile
+  p.c0 = p.c1 = blockIdx.x;
+  if (p.t0 || p.t1 < r.it.tiles) p.c0 = (int)pa_div(ux, r.share), p.c1 = (int)pa_div(ux + r.it.tiles - 1, r.share);
+  p.first_place = r.share * p.c0 <= ux ? 1 : 0;
   r.x += max(1, p.t1 - p.t0);
   return p;
 }
@@ -164,13 +178,33 @@ __device__ __forceinline__ void run_next(const PagedAttnArgs& a, PagedRun& r) {
   if (++r.item == r.items) r.item = 0, ++r.kvh;
   r.it = load_item(paged_items(a.header) + r.item);
 }
-// Where a unit's pieces are: CTA c's first tile is c * share; what begins the unit
-// is the CTA's second place, what goes on with one its first.
-__device__ __forceinline__ int64_t unit_tile(const PagedRun& r, const PagedPiece& p) {
-  return (int64_t)p.kvh * r.tiles + p.it.tile0;
-}
-__device__ __forceinline__ float* piece_part(const PagedAttnArgs& a, const PagedRun& r, int64_t cta, int64_t ux, int stride) {
-  return a.part + (2 * cta + (r.share * cta <= ux ? 1 : 0)) * stride;
+// The pages of a piece for the producer warp: 32 entries of the table in the warp's
+// registers and the next 32 on their way, so that no tile waits for its names (a load
+// per tile, even one tile ahead, held a CTA to a tile per round trip: 0.95 us).
+struct PagedNames {
+  const int* row;
+  int last, block, cur, next;  // entries there are; the 32 at hand
+  __device__ __forceinline__ PagedNames(const PagedAttnArgs& a, const PagedPiece& p, int tile)
+      : row(a.table + (int64_t)p.it.b * a.max_pages) {
+    last = (min(p.it.len, p.t1 * tile) + a.c.page_size - 1) >> a.c.page_shift;
+    block = (p.t0 * tile >> a.c.page_shift) >> 5;
+    cur = load(block), next = load(block + 1);
+  }
+  __device__ __forceinline__ int load(int b) const {
+    const int i = b * 32 + (threadIdx.x & 31);
+    return i < last ? __ldcg(row + i) : -1;
+  }
+  // Entry i, the whole warp asking for entries of one block of 32, at or behind the last's.
+  __device__ __forceinline__ int at(int i) {
+    const int b = __shfl_sync(0xffffffffu, i, 0) >> 5;
+    if (b != block) block = b, cur = next, next = load(b + 1);
+    return __shfl_sync(0xffffffffu, cur, i & 31);
+  }
+};
+// Where CTA c's piece of the unit is.  A CTA has two places: one for the piece that
+// goes on with a unit, one for the piece that begins one, which only c0's can be.
+__device__ __forceinline__ float* piece_part(const PagedAttnArgs& a, const PagedPiece& p, int cta, int stride) {
+  return a.part + (int64_t)(2 * cta + (cta == p.c0 ? p.first_place : 0)) * stride;
 }
 
 // Devices whose kernel may take its shared memory; set again by whoever comes twice

@@ -178,12 +178,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     while (ok && run.x < run.end) {
       const PagedPiece p = run_piece(a, run, ROWS);
       const int len = p.it.len;
-      const int* row = a.table + (int64_t)p.it.b * a.max_pages;
-      auto entry = [&](int t) {
-        const int pos = t * TILE + box * BR;
-        return box < boxes && t < p.t1 && pos < len ? __ldcg(row + (pos >> a.c.page_shift)) : -1;
-      };
-      int page = entry(p.t0);
+      PagedNames names(a, p, TILE);
       if (k >= 2 && !wait(&bars.d_empty[k & 1], k / 2 - 1)) break;
       if (lane == 0) {
         Piece& d = pieces[k & 1];
@@ -200,8 +195,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (run.x < run.end) run_next(a, run);
       for (int t = p.t0; ok && t < p.t1; ++t) {
         const int pos = t * TILE + box * BR;
-        const int next = entry(t + 1);
         const int live = min(boxes, (len - t * TILE + BR - 1) / BR);
+        const int page = names.at(pos >> a.c.page_shift);
         int y = (page * a.c.kv_heads + p.kvh) * P + (pos & (P - 1));
         if (box < live && (unsigned)page >= (unsigned)a.c.num_pages) {  // names no page: zeros, and the error word
           y = rows_all;
@@ -218,7 +213,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (box < live)
             pa_tma(smem + s * F::SLOT + plane * F::PLANE + box * BR * 128, v ? &vmap : &kmap, plane * 64, y, &bars.full[s]);
         }
-        page = next;
       }
     }
     if (k < 2 || wait(&bars.d_empty[k & 1], k / 2 - 1)) {
@@ -443,9 +437,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       const float L = sum.x + sum.y;
       const bool whole = t0 == 0 && t1 == p.it.tiles, fix = d.p.poison != 0;
-      const int64_t ux = unit_tile(run, p);
       constexpr int STRIDE = ROWS * (HD + 2);
-      float* part = piece_part(a, run, blockIdx.x, ux, STRIDE);
+      float* part = piece_part(a, p, blockIdx.x, STRIDE);
       auto store = [&](const float (&v)[32], int c) {  // 32 values of the row from dim c on
         const int64_t at = (int64_t)(start + token) * a.ld_out + (int64_t)head * HD + c;
         if (a.out32) {
@@ -502,22 +495,22 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!whole) {
         *reinterpret_cast<float2*>(part + ROWS * HD + 2 * row) = make_float2(ref, L);
-        const int64_t c_first = ux / run.share, c_last = (ux + p.it.tiles - 1) / run.share;
+        const int c0 = p.c0, c1 = p.c1;
         __threadfence();
         mbar_arrive(&bars.join);
         ok = wait(&bars.join, joins++);
         if (!ok) break;
-        if (tid == 0) is_last = atomicAdd(a.count + p.unit, 1) == (int)(c_last - c_first);
+        if (tid == 0) is_last = atomicAdd(a.count + p.unit, 1) == c1 - c0;
         mbar_arrive(&bars.join);
         ok = wait(&bars.join, joins++);
         if (!ok) break;
         if (is_last) {
           __threadfence();
-          auto piece = [&](int64_t c) { return piece_part(a, run, c, ux, STRIDE); };
+          auto piece = [&](int c) { return piece_part(a, p, c, STRIDE); };
           float top = -INFINITY, all = 0.f;
-          for (int64_t c = c_first; c <= c_last; ++c)
+          for (int c = c0; c <= c1; ++c)
             top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row)).x);
-          for (int64_t c = c_first; c <= c_last; ++c) {
+          for (int c = c0; c <= c1; ++c) {
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row));
             all += ml.y * (ml.x == top ? 1.f : pa_ex2(ml.x - top));
           }
@@ -527,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             float v[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = 0.f;
-            for (int64_t c = c_first; c <= c_last; ++c) {
+            for (int c = c0; c <= c1; ++c) {
               const float* src = piece(c);
               const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * row));
               if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
