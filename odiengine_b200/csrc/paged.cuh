@@ -55,7 +55,7 @@ inline int page_shift_of(int p) { return p == 16 ? 4 : p == 32 ? 5 : p == 64 ? 6
 // head: the two widths of the mma.sync kernel, and the tcgen05 kernel's.
 inline void paged_kind(int64_t most, int* rows, int* tile) {
   *rows = most <= 16 ? 16 : most <= 32 ? 32 : 256;
-  *tile = most <= 32 ? 64 : 128;
+  *tile = 64;
 }
 
 // Positions of the batch that row r of request b sees: those below the result.

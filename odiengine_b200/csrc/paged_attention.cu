@@ -590,7 +590,7 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + COUNT_OFF);
   const bool fancy = softcap > 0.f || d_slopes;
   cudaStream_t s = (cudaStream_t)stream;
-  return kv_launched(g.rows <= 32 ? launch_paged_mma(a, g.rows / 16, fancy, s) : launch_paged_tc(a, fancy, s), "attention_paged");
+  return kv_launched(g.rows <= 32 ? launch_paged_mma(a, g.rows / 16, fancy, s) : launch_paged_tc(a, s), "attention_paged");
 }
 
 }  // extern "C"

@@ -225,7 +225,7 @@ struct PagedReady {
 
 cudaError_t paged_maps(const PagedView& c, int tile, CUtensorMap* maps);
 cudaError_t launch_paged_mma(PagedAttnArgs& a, int groups, bool fancy, cudaStream_t s);
-cudaError_t launch_paged_tc(PagedAttnArgs& a, bool fancy, cudaStream_t s);
+cudaError_t launch_paged_tc(PagedAttnArgs& a, cudaStream_t s);
 
 constexpr int PAGED_SMS = 148, PAGED_ROWS_MAX = 256;
 // CTAs of a call: two per SM of the narrow kernel, else one

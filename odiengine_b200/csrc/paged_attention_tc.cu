@@ -4,17 +4,20 @@
 // An item is up to 256 rows (new tokens * heads per kv head) of one request and kv
 // head, as two halves of 128 whose work alternates:
 //
-//   S [128 rows x 128 positions] = Q K^T    Q and K in shared memory
-//   O [128 rows x head_dim]     += P V      P in tensor memory, where S was
+//   S [128 rows x 64 positions] = Q K^T     Q and K in shared memory
+//   O [128 rows x head_dim]    += P V       P in tensor memory, where S was
 //
 //   warps 0-3, 4-7  softmax of the two halves: thread = row
-//   warp 8          TMA producer: K and V tiles of 128 positions, page by page
-//   warp 9          issues the products; holds the tensor memory
-//   warps 10, 11    only make the warpgroup whole, for its registers
+//   warp 8          TMA producer: K and V tiles of 64 positions, page by page
+//   warps 9, 10     issue the products, one warp a half; warp 9 holds the tensor memory
+//   warp 11         idle
 //
-// While one half is in its softmax the tensor core works for the other.  The
-// running reference of a row moves only when a weight would pass 2^8, so O is
-// rescaled a few times per row.
+// Each half has two S, so that the scores of the next tile are there when the
+// weights of this one are done.  (One S of 128 positions a half, which leaves the
+// tensor core no more than the other half's work during a softmax: 2048 tokens of
+// 64/8 heads over 14,001 positions took 3400 cycles per 128 positions.)  The running
+// reference of a row moves only when a weight would pass 2^8, so O is rescaled a few
+// times per row.
 //
 // Every wait is bounded; a role whose wait gives up sets the error word and
 // leaves its loop, and the CTA ends at one barrier that every role reaches.
@@ -24,21 +27,28 @@
 namespace odi_cuda {
 namespace ptc {
 
-constexpr int TILE = 128, ROWS = 256, HALF_ROWS = 128, THREADS = 384;
-// The launch's registers are shared out anew: a softmax thread holds a row of 128
-// scores, the others next to nothing.
-constexpr int REGS_LAUNCH = 168, REGS_FEW = 72, REGS_SOFT = 216;
-static_assert(128 * REGS_FEW + 256 * REGS_SOFT <= THREADS * REGS_LAUNCH, "register split");
+constexpr int TILE = 64, ROWS = 256, HALF_ROWS = 128, THREADS = 384;
 constexpr float MOVE = 8.f;
+// Of eight pairs of weights one is exponentiated on the FMA pipe.  The loop over 64
+// scores of a row, two warps per scheduler: 933 cycles so, 1188 without, 964 with
+// three; without the order that the volatile statements keep 1290.
+constexpr int ON_FMA = 1;
+__device__ __forceinline__ float ex2_here(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 template <int HD>
 struct Cfg {
-  static constexpr int PLANE = 128 * 128;               // 128 rows of 128 bytes: half the dims of head_dim 128
-  static constexpr int SLOT = HD / 64 * PLANE;          // K or V of one tile, Q of one half
-  static constexpr int ST = HD == 128 ? 4 : 8;
+  static constexpr int PLANE = TILE * 128, SLOT = HD / 64 * PLANE;      // K or V of one tile, in planes of 64 dims
+  static constexpr int Q_PLANE = HALF_ROWS * 128, Q_HALF = HD / 64 * Q_PLANE;
+  static constexpr int ST = HD == 128 ? 8 : 12;
+  static_assert(ST / 2 < 8, "v_clean");
   static constexpr int Q_OFF = ST * SLOT;
-  static constexpr int SMEM = Q_OFF + 2 * SLOT + 1024;  // + alignment slack
-  static constexpr int S_COL = 0, O_COL = 256, COLS = 512;
+  static constexpr int SMEM = Q_OFF + 2 * Q_HALF + 1024;  // + alignment slack
+  // tensor memory: two S per half, then an O per half
+  static constexpr int O_COL = 256, COLS = 512;
 };
 
 __device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo) {
@@ -76,29 +86,32 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(r));
   return r != 0;
 }
-// Tensor memory of the warp's 32 rows, 32 or 128 columns.  Loads and wait are one
+// Tensor memory of the warp's 32 rows, 16 or 64 columns.  Loads and wait are one
 // statement: no use of a register can move ahead of the wait.
 #define PT_OUT8(r) "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]), "=r"((r)[6]), "=r"((r)[7])
 #define PT_OUT32(r) PT_OUT8(r), PT_OUT8((r) + 8), PT_OUT8((r) + 16), PT_OUT8((r) + 24)
 #define PT_IN8(r) "r"((r)[0]), "r"((r)[1]), "r"((r)[2]), "r"((r)[3]), "r"((r)[4]), "r"((r)[5]), "r"((r)[6]), "r"((r)[7])
 #define PT_IN32(r) PT_IN8(r), PT_IN8((r) + 8), PT_IN8((r) + 16), PT_IN8((r) + 24)
-__device__ __forceinline__ void ld32(uint32_t (&r)[32], uint32_t addr) {
+__device__ __forceinline__ void ld16(uint32_t (&r)[16], uint32_t addr) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : PT_OUT32(r)
+      : PT_OUT8(r), PT_OUT8((r) + 8)
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void ld128(uint32_t (&r)[128], uint32_t addr) {
+__device__ __forceinline__ void st16(const uint32_t* r, uint32_t addr) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::PT_IN8(r),
+               PT_IN8((r) + 8), "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ld64(uint32_t (&r)[64], uint32_t addr) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : PT_OUT32(r), PT_OUT32((r) + 32), PT_OUT32((r) + 64), PT_OUT32((r) + 96)
-      : "r"(addr), "r"(addr + 32), "r"(addr + 64), "r"(addr + 96)
+      : PT_OUT32(r), PT_OUT32((r) + 32)
+      : "r"(addr), "r"(addr + 32)
       : "memory");
 }
 __device__ __forceinline__ void st32(const uint32_t* r, uint32_t addr) {
@@ -109,17 +122,47 @@ __device__ __forceinline__ void st32(const uint32_t* r, uint32_t addr) {
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one of them is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+// 2^x of two scores on the FMA pipe, which has room where the special function unit
+// (16 a cycle and SM) has none: x = n + f with n whole and |f| <= 1/2, 2^f as the
+// polynomial of degree 5 with the least largest relative error (2^-23.8) among those
+// that are 1 at 0, n into the exponent.  Below 2^-126 the result is 0.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = fmaxf(x.x, -127.f), x.y = fmaxf(x.y, -127.f);
+  constexpr float M = 12582912.f;  // 1.5 * 2^23: adding it rounds to whole numbers
+  const float2 t = __fadd2_rn(x, make_float2(M, M));
+  const float2 n = __fadd2_rn(t, make_float2(-M, -M));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  constexpr float C1 = 0.6931465864181519f, C2 = 0.24022166430950165f, C3 = 0.055510472506284714f, C4 = 0.009674952365458012f,
+                  C5 = 0.0013202981790527701f;
+  float2 p = __ffma2_rn(f, make_float2(C5, C5), make_float2(C4, C4));
+  p = __ffma2_rn(p, f, make_float2(C3, C3));
+  p = __ffma2_rn(p, f, make_float2(C2, C2));
+  p = __ffma2_rn(p, f, make_float2(C1, C1));
+  p = __ffma2_rn(p, f, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+// What a score goes through: nothing but the scale; a distance bias; a cap (and a bias).
+enum { PLAIN = 0, BIAS = 1, CAP = 2 };
+
 struct Piece {
   PagedPiece p;
   int end[2];  // tiles of the unit that each half of its rows sees
 };
 struct Bars {
-  uint64_t full[8], empty[8];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2], v_clean;
-  uint64_t d_full[2], d_empty[2], join, drain;
+  uint64_t full[12], empty[12];
+  uint64_t s_full[2][2], p_full[2][2];  // of a half's two S
+  uint64_t q_full[2], pv_done[2][2];    // in turn too: a half can wait two products ahead
+  uint64_t v_clean[8];  // in turn: a half can be ahead of the other by the tiles that the ring holds
+  uint64_t d_full[2], d_empty[2], join, drain[2];
 };
 
-template <typename T, int HD, bool FANCY>
+template <typename T, int HD, int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
     paged_tc_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap) {
@@ -137,18 +180,18 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   pdl_launch_dependents();
   if (tid == 0) {
-    for (int i = 0; i < ST; ++i) mbar_init(&bars.full[i], 1), mbar_init(&bars.empty[i], 1);
+    for (int i = 0; i < ST; ++i) mbar_init(&bars.full[i], 1), mbar_init(&bars.empty[i], 2);
     for (int i = 0; i < 2; ++i) {
+      for (int b = 0; b < 2; ++b) mbar_init(&bars.s_full[i][b], 1), mbar_init(&bars.p_full[i][b], 128);
       mbar_init(&bars.q_full[i], 128);
-      mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 128);
-      mbar_init(&bars.pv_done[i], 1);
+      mbar_init(&bars.pv_done[i][0], 1), mbar_init(&bars.pv_done[i][1], 1);
       mbar_init(&bars.d_full[i], 1);
-      mbar_init(&bars.d_empty[i], 9);
+      mbar_init(&bars.d_empty[i], 10);
     }
-    mbar_init(&bars.v_clean, 128);
+    for (int i = 0; i < 8; ++i) mbar_init(&bars.v_clean[i], 128);
     mbar_init(&bars.join, 256);
-    mbar_init(&bars.drain, 1);
+    mbar_init(&bars.drain[0], 1), mbar_init(&bars.drain[1], 1);
+    prefetch_map(&kmap), prefetch_map(&vmap);
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -166,10 +209,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int P = a.c.page_size;
   auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, a.err, ERR_PAGED_WAIT); };
 
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
   if (any && warp == 8) {
-    // ---- producer
+    // ---- producer: K0 K1 V0 K2 V1 ... V of a piece, as the products want them
     const int BR = min(P, TILE), boxes = TILE / BR;
     const int box = lane / PLANES, plane = lane % PLANES;
     const int rows_all = a.c.num_pages * a.c.kv_heads * P;
@@ -193,17 +234,22 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       ++k;
       if (run.x < run.end) run_next(a, run);
-      for (int t = p.t0; ok && t < p.t1; ++t) {
-        const int pos = t * TILE + box * BR;
-        const int live = min(boxes, (len - t * TILE + BR - 1) / BR);
-        const int page = names.at(pos >> a.c.page_shift);
-        int y = (page * a.c.kv_heads + p.kvh) * P + (pos & (P - 1));
-        if (box < live && (unsigned)page >= (unsigned)a.c.num_pages) {  // names no page: zeros, and the error word
-          y = rows_all;
-          atomicOr(a.err, ERR_PAGED_PAGE);
+      int y_next = 0, live_next = 0;  // of the tile whose K went last, for its V
+      for (int t = p.t0; ok && t <= p.t1; ++t) {
+        const int y_v = y_next, live_v = live_next;
+        if (t < p.t1) {
+          const int pos = t * TILE + box * BR;
+          live_next = min(boxes, (len - t * TILE + BR - 1) / BR);
+          const int page = names.at(pos >> a.c.page_shift);
+          y_next = (page * a.c.kv_heads + p.kvh) * P + (pos & (P - 1));
+          if (box < live_next && (unsigned)page >= (unsigned)a.c.num_pages) {  // names no page: zeros, and the error word
+            y_next = rows_all;
+            atomicOr(a.err, ERR_PAGED_PAGE);
+          }
         }
-        for (int v = 0; v < 2; ++v, ++n) {
-          const int s = n % ST;
+        for (int v = 0; v < 2; ++v) {
+          if (v ? t == p.t0 : t == p.t1) continue;
+          const int s = n % ST, live = v ? live_v : live_next, y = v ? y_v : y_next;
           if (n >= ST && !wait(&bars.empty[s], n / ST - 1)) {
             ok = false;
             break;
@@ -212,6 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           __syncwarp();
           if (box < live)
             pa_tma(smem + s * F::SLOT + plane * F::PLANE + box * BR * 128, v ? &vmap : &kmap, plane * 64, y, &bars.full[s]);
+          ++n;
         }
       }
     }
@@ -222,108 +269,107 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     for (int i = max(0, n - ST); i < n; ++i) wait(&bars.full[i % ST], i / ST);  // no copy outlives the CTA
-  } else if (any && warp == 9) {
-    // ---- products
-    const uint32_t ring = smem_u32(smem), q = ring + F::Q_OFF;
+  } else if (any && (warp == 9 || warp == 10)) {
+    // ---- products of one half
+    const int h = warp - 9;
+    const uint32_t ring = smem_u32(smem), q = ring + F::Q_OFF + h * F::Q_HALF, s_col = tmem + h * 128, o_col = tmem + F::O_COL + h * 128;
     constexpr uint32_t ID_S = idesc<H::BF>(TILE, false), ID_O = idesc<H::BF>(HD, true);
-    int n = 0, c_clean = 0, c_q[2] = {0, 0}, c_p[2] = {0, 0};
-    auto scores = [&](int h, int s) {  // S of half h from the K tile in slot s
-      if (elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {
-          const uint32_t off = (ks / 4) * F::PLANE + (ks % 4) * 32;
-          mma_ss(tmem + F::S_COL + h * 128, desc(q + h * F::SLOT + off, 0), desc(ring + s * F::SLOT + off, 0), ID_S, ks > 0);
-        }
-        commit(&bars.s_full[h]);
-      }
-      __syncwarp();
-    };
-    auto release = [&](int s) {
-      if (elect_one()) commit(&bars.empty[s]);
-      __syncwarp();
-    };
+    int n = 0, c_clean = 0, c_q = 0, c_s = 0, c_p = 0;  // tiles of the half so far: its S in turn
     bool ok = true;
     for (int k = 0; ok; ++k) {
       if (!wait(&bars.d_full[k & 1], k / 2)) break;
       const Piece& d = pieces[k & 1];
       if (d.p.last) break;
-      const int t0 = d.p.t0, t1 = d.p.t1, least = d.p.least, end0 = d.end[0], end1 = d.end[1];
-      auto end = [&](int h) { return h ? end1 : end0; };
-      for (int t = t0 - 1; ok && t < t1; ++t) {
-        const int sv = (n + 2 * (t - t0) + 1) % ST, iv = (n + 2 * (t - t0) + 1) / ST;
-        const int sk = (n + 2 * (t + 1 - t0)) % ST, ik = (n + 2 * (t + 1 - t0)) / ST;
-        if (t >= t0) {
-          ok = wait(&bars.full[sv], iv);
-          if (ok && (t + 1) * TILE > least) ok = wait(&bars.v_clean, c_clean++);
-        }
-        bool have_k = false;
-        for (int h = 0; ok && h < 2; ++h) {
-          if (t >= t0 && t < end(h)) {
-            ok = wait(&bars.p_full[h], c_p[h]++);
+      const int t0 = d.p.t0, tiles = d.p.t1 - t0, m0 = max(0, d.p.least / TILE - t0), end = d.end[h] - t0;
+      if (end > 0) ok = wait(&bars.q_full[h], c_q++);
+      // tile i of the piece: K is load 0, 1, 3, 5 ..., V load 2, 4, ... and the last
+      for (int i = -2; ok && i < tiles; ++i) {
+        const int nk = n + (i + 2 ? 2 * (i + 2) - 1 : 0), nv = n + min(2 * i + 2, 2 * tiles - 1);
+        if (i >= 0) {
+          const int b = c_p & 1;
+          if (i < end) {
+            ok = wait(&bars.p_full[h][b], c_p >> 1) && wait(&bars.full[nv % ST], nv / ST);
+            if (ok && i >= m0) ok = wait(&bars.v_clean[(c_clean + i - m0) & 7], (c_clean + i - m0) >> 3);
             if (!ok) break;
             fence_after();
             if (elect_one()) {
+              const uint64_t v = desc(ring + nv % ST * F::SLOT, F::PLANE);
 #pragma unroll
-              for (int ks = 0; ks < TILE / 16; ++ks)
-                mma_ts(tmem + F::O_COL + h * 128, tmem + F::S_COL + h * 128 + ks * 8, desc(ring + sv * F::SLOT + ks * 2048, F::PLANE),
-                       ID_O, t > t0 || ks > 0);
-              commit(&bars.pv_done[h]);
+              for (int ks = 0; ks < TILE / 16; ++ks) mma_ts(o_col, s_col + b * 64 + ks * 8, v + ks * (2048 >> 4), ID_O, i > 0 || ks > 0);
+              commit(&bars.pv_done[h][b]);
+              commit(&bars.empty[nv % ST]);
             }
             __syncwarp();
-          }
-          if (t + 1 < end(h)) {
-            if (!have_k) ok = wait(&bars.full[sk], ik), have_k = true;
-            if (ok && t < t0) ok = wait(&bars.q_full[h], c_q[h]++);
+            // the next S goes where this P is: an order that nothing but the wait gives
+            if (i + 2 < end) ok = wait(&bars.pv_done[h][b], c_p >> 1);
+            ++c_p;
+          } else {  // not before it is there: the slot's next tile has a release of its own
+            ok = wait(&bars.full[nv % ST], nv / ST);
             if (!ok) break;
-            fence_after();
-            scores(h, sk);
+            if (lane == 0) mbar_arrive(&bars.empty[nv % ST]);
           }
         }
-        if (!ok) break;
-        if (t >= t0) release(sv);
-        if (t + 1 < t1) release(sk);
+        if (i + 2 < end) {
+          ok = ok && wait(&bars.full[nk % ST], nk / ST);
+          if (!ok) break;
+          fence_after();
+          if (elect_one()) {
+            const int b = c_s & 1;
+            const uint64_t qd = desc(q, 0), kd = desc(ring + nk % ST * F::SLOT, 0);
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks)
+              mma_ss(s_col + b * 64, qd + (((ks / 4) * F::Q_PLANE + (ks % 4) * 32) >> 4), kd + (((ks / 4) * F::PLANE + (ks % 4) * 32) >> 4),
+                     ID_S, ks > 0);
+            commit(&bars.s_full[h][b]);
+            commit(&bars.empty[nk % ST]);
+          }
+          __syncwarp();
+          ++c_s;
+        } else if (i + 2 < tiles) {
+          ok = ok && wait(&bars.full[nk % ST], nk / ST);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&bars.empty[nk % ST]);
+        }
       }
-      n += 2 * (t1 - t0);
+      n += 2 * tiles, c_clean += max(0, tiles - m0);
       if (lane == 0) mbar_arrive(&bars.d_empty[k & 1]);
     }
     // products in flight end before the tensor memory goes
-    if (elect_one()) commit(&bars.drain);
+    if (elect_one()) commit(&bars.drain[h]);
     __syncwarp();
-    wait(&bars.drain, 0);
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
+    wait(&bars.drain[h], 0);
+  } else if (any && warp < 8) {
     // ---- softmax: thread = row
-    const int h = warp >> 2, row = tid;  // row of the item
+    const int h = warp >> 2, hr = tid & 127, row = tid;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + F::S_COL + h * 128, o_addr = tmem + lanes + F::O_COL + h * 128;
-    uint8_t* qs = smem + F::Q_OFF + h * F::SLOT;
-    int n = 0, c_s = 0, c_pv = 0, joins = 0;
-    bool ok = any;
+    const uint32_t o_addr = tmem + lanes + F::O_COL + h * 128;
+    uint8_t* qs = smem + F::Q_OFF + h * F::Q_HALF;
+    int n = 0, c_s = 0, c_pv = 0, c_clean = 0, joins = 0;
+    bool ok = true;
     for (int k = 0; ok; ++k) {
       if (!wait(&bars.d_full[k & 1], k / 2)) break;
       Piece& d = pieces[k & 1];
       if (d.p.last) break;
-      const PagedPiece p = d.p;
-      const int start = p.it.start, past = p.it.past, len = p.it.len, rows = p.rows, least = p.least;
-      const int t0 = p.t0, t1 = p.t1, t_end = d.end[h], end1 = d.end[1];
+      const PagedPiece& p = d.p;
+      const int rows = p.rows, t0 = p.t0, t1 = p.t1, t_end = d.end[h];
       const bool mine = t_end > t0;
+      const int m0 = max(t0, p.least / TILE);  // the first tile that not every row sees whole
       const int R = p.it.i * ROWS + row, token = pa_token(a, R), head = p.kvh * a.G + R - token * a.G;
-      const int lim = row < rows ? paged_limit(past, token, len, p.it.prefix) : 0;
+      const int lim = row < rows ? paged_limit(p.it.past, token, p.it.len, p.it.prefix) : 0;
       // positions below it are seen by all rows of this half
-      const int least_h = paged_limit(past, pa_token(a, p.it.i * ROWS + h * HALF_ROWS), len, p.it.prefix);
-      const float slope = FANCY && a.slopes && row < rows ? __ldg(a.slopes + head) * 1.4426950408889634f : 0.f;
+      const int least_h = paged_limit(p.it.past, pa_token(a, p.it.i * ROWS + h * HALF_ROWS), p.it.len, p.it.prefix);
+      const float slope = MODE != PLAIN && a.slopes && row < rows ? __ldg(a.slopes + head) * 1.4426950408889634f : 0.f;
       if (mine) {
         // Q: 16-byte pieces, HD / 8 to a row
         constexpr int PER = HD / 8;
         const T* q = static_cast<const T*>(a.q);
 #pragma unroll 4
-        for (int i = tid & 127; i < HALF_ROWS * PER; i += 128) {
+        for (int i = hr; i < HALF_ROWS * PER; i += 128) {
           const int r = i / PER, ch = i % PER;
           uint4 x = make_uint4(0, 0, 0, 0);
           if (h * HALF_ROWS + r < rows) {
             const int RR = p.it.i * ROWS + h * HALF_ROWS + r, tk = pa_token(a, RR);
-            const T* src = q + (int64_t)(start + tk) * a.ld_q + (int64_t)(p.kvh * a.G + RR - tk * a.G) * HD + ch * 8;
+            const T* src = q + (int64_t)(p.it.start + tk) * a.ld_q + (int64_t)(p.kvh * a.G + RR - tk * a.G) * HD + ch * 8;
             if (a.vec) {
               x = __ldcg(reinterpret_cast<const uint4*>(src));
             } else {
@@ -331,85 +377,121 @@ __global__ void __launch_bounds__(THREADS, 1)
               x = make_uint4(__ldcg(s4), __ldcg(s4 + 1), __ldcg(s4 + 2), __ldcg(s4 + 3));
             }
           }
-          *reinterpret_cast<uint4*>(qs + (ch >> 3) * F::PLANE + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+          *reinterpret_cast<uint4*>(qs + (ch >> 3) * F::Q_PLANE + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
         }
         fence_proxy_async_smem();
         mbar_arrive(&bars.q_full[h]);
       }
       float ref = -INFINITY;
-      float2 sum = make_float2(0.f, 0.f);
+      float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
       for (int t = t0; t < t_end; ++t) {
-        ok = wait(&bars.s_full[h], c_s++);
+        const int b = c_s & 1;
+        const uint32_t s_addr = tmem + lanes + h * 128 + b * 64;
+        ok = wait(&bars.s_full[h][b], c_s >> 1);
+        ++c_s;
         if (!ok) break;
+        __syncwarp();
         fence_after();
-        uint32_t s[128];
-        ld128(s, s_addr);
-        float mx = -INFINITY;
-        const int rel = lim - t * TILE;
-        if (FANCY) {
-          const int away = past + token - t * TILE;
+        uint32_t s[64];
+        ld64(s, s_addr);
+        const int col0 = t * TILE;
+        if (MODE == CAP) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c) {
-            float x = __uint_as_float(s[c]) * a.scale_log2;
-            if (a.cap_log2 != 0.f) x = a.cap_log2 * pa_tanh(x);
-            x = fmaf(-slope, (float)abs(away - c), x);
-            s[c] = __float_as_uint(x);
+          for (int c = 0; c < 64; ++c) s[c] = __float_as_uint(a.cap_log2 * pa_tanh(__uint_as_float(s[c]) * a.scale_log2));
+        }
+        if (MODE == BIAS || (MODE == CAP && a.slopes)) {
+          const int away = p.it.past + token - col0;  // the row's own column
+          const float scale = MODE == CAP ? 1.f : a.scale_log2;
+          const float2 sc2 = make_float2(scale, scale), sl2 = make_float2(slope, slope);
+          if (__any_sync(0xffffffffu, lim - col0 > away + 1 && away < 63)) {
+            // part of the tile lies behind the row and is seen: distances have a sign
+            const float a0 = (float)away;
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              s[c] = __float_as_uint(fmaf(-slope, fabsf((float)c - a0), __uint_as_float(s[c]) * scale));
+          } else {
+            const float b0 = -slope * (float)away;
+            const float2 b2 = make_float2(b0, b0);
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+              const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2,
+                                          __ffma2_rn(make_float2((float)c, (float)(c + 1)), sl2, b2));
+              s[c] = __float_as_uint(x.x), s[c + 1] = __float_as_uint(x.y);
+            }
           }
         }
-        if ((t + 1) * TILE > least_h) {
+        if (col0 + 64 > least_h) {
+          const int rel = lim - col0;  // columns that the row sees
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
+          for (int c = 0; c < 64; ++c)
             if (c >= rel) s[c] = 0xff800000u;
         }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 128; ++c) mx = fmaxf(mx, __uint_as_float(s[c]));
-        const float scale = FANCY ? 1.f : a.scale_log2;
-        mx *= scale;
-        const bool move = mx > ref + MOVE;
+        for (int c = 0; c < 64; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) m4[e] = max3(m4[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1]));
+        const float scale = MODE == PLAIN ? a.scale_log2 : 1.f;
+        const float mx = max3(max3(m4[0], m4[1], m4[2]), m4[3], -INFINITY) * scale;
+        const bool move = !(mx <= ref + MOVE);
         if (__any_sync(0xffffffffu, move)) {
-          const float top = move ? mx : ref;
+          // a NaN among the scores, or +inf, leaves no weight: the row is NaN from here on
+          const float top = !move ? ref : mx == INFINITY ? __int_as_float(0x7fc00000) : mx;
           const float f = top == ref ? 1.f : pa_ex2(ref - top);
           ref = top;
-          sum.x *= f, sum.y *= f;
+          sum[0].x *= f, sum[0].y *= f, sum[1].x *= f, sum[1].y *= f;
           if (t > t0) {
-            ok = wait(&bars.pv_done[h], c_pv - 1);
+            ok = wait(&bars.pv_done[h][(c_pv - 1) & 1], (c_pv - 1) >> 1);
             if (!ok) break;
+            __syncwarp();
             fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16];
+              ld16(o, o_addr + c);
 #pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-              uint32_t o[32];
-              ld32(o, o_addr + c);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              st32(o, o_addr + c);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              st16(o, o_addr + c);
             }
           }
         }
         const float nref = ref == -INFINITY ? 0.f : -ref;
         const float2 sc2 = make_float2(scale, scale), nr2 = make_float2(nref, nref);
+        // eight pairs at a time, sums and packing one group behind
+        float2 w[2][8];
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, nr2);
-          const float2 w = make_float2(pa_ex2(x.x), pa_ex2(x.y));
-          sum = __fadd2_rn(sum, w);
-          s[c / 2] = H::pack(w.x, w.y);
+        for (int g = 0; g <= 4; ++g) {
+          if (g < 4) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              w[g & 1][e] = __ffma2_rn(make_float2(__uint_as_float(s[16 * g + 2 * e]), __uint_as_float(s[16 * g + 2 * e + 1])), sc2, nr2);
+#pragma unroll
+            for (int e = 0; e < 8 - ON_FMA; ++e) w[g & 1][e] = make_float2(ex2_here(w[g & 1][e].x), ex2_here(w[g & 1][e].y));
+#pragma unroll
+            for (int e = 8 - ON_FMA; e < 8; ++e) w[g & 1][e] = exp2_fma(w[g & 1][e]);
+          }
+          if (g > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 v = w[(g - 1) & 1][e];
+              sum[e & 1] = __fadd2_rn(sum[e & 1], v);
+              s[8 * (g - 1) + e] = H::pack(v.x, v.y);
+            }
+          }
         }
         st32(s, s_addr);
-        st32(s + 32, s_addr + 32);
         wait_st();
-        if ((t + 1) * TILE > least && h == (t < end1 ? 1 : 0)) {
-          // the last half at work takes what is not finite out of V: thread = position
-          const int iv = n + 2 * (t - t0) + 1;
+        if (t >= m0 && h == (t < d.end[1] ? 1 : 0)) {
+          // the last half at work takes what is not finite out of V: thread = position, half its dims
+          const int iv = n + min(2 * (t - t0) + 2, 2 * (t1 - t0) - 1), r = hr & 63, pos = t * TILE + r;
           ok = wait(&bars.full[iv % ST], iv / ST);
           if (!ok) break;
-          const int r = tid & 127, pos = t * TILE + r;
-          if (pos >= least) {
-            uint8_t* v = smem + (iv % ST) * F::SLOT + r * 128;
+          if (pos >= p.least) {
             bool bad = false;
-#pragma unroll
-            for (int ch = 0; ch < HD / 8; ++ch) {
-              uint32_t* x = reinterpret_cast<uint32_t*>(v + (ch >> 3) * F::PLANE + (((ch & 7) ^ (r & 7)) << 4));
-              uint4 y = *reinterpret_cast<uint4*>(x);
+#pragma unroll 1
+            for (int ch = (hr >> 6) * (HD / 16); ch < ((hr >> 6) + 1) * (HD / 16); ++ch) {
+              uint4* x = reinterpret_cast<uint4*>(smem + iv % ST * F::SLOT + r * 128 + (ch >> 3) * F::PLANE + (((ch & 7) ^ (r & 7)) << 4));
+              const uint4 y = *x;
               uint32_t z[4] = {y.x, y.y, y.z, y.w};
               bool any_bad = false;
 #pragma unroll
@@ -417,77 +499,75 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if ((z[e] & H::EXP) == H::EXP) z[e] &= 0xffff0000u, any_bad = true;
                 if ((z[e] & (H::EXP << 16)) == H::EXP << 16) z[e] &= 0xffffu, any_bad = true;
               }
-              if (any_bad) *reinterpret_cast<uint4*>(x) = make_uint4(z[0], z[1], z[2], z[3]);
+              if (any_bad) *x = make_uint4(z[0], z[1], z[2], z[3]);
               bad = bad || any_bad;
             }
-            if (bad && pos < len) d.p.poison = 1;
+            if (bad && pos < p.it.len) d.p.poison = 1;
           }
           fence_proxy_async_smem();
-          mbar_arrive(&bars.v_clean);
+          mbar_arrive(&bars.v_clean[(c_clean + t - m0) & 7]);
         }
         fence_before();
-        mbar_arrive(&bars.p_full[h]);
+        mbar_arrive(&bars.p_full[h][b]);
         ++c_pv;
       }
+      if (ok && mine) ok = wait(&bars.pv_done[h][(c_pv - 1) & 1], (c_pv - 1) >> 1);
       if (!ok) break;
-      if (mine) {
-        ok = wait(&bars.pv_done[h], c_pv - 1);
-        if (!ok) break;
-        fence_after();
-      }
-      const float L = sum.x + sum.y;
-      const bool whole = t0 == 0 && t1 == p.it.tiles, fix = d.p.poison != 0;
+      __syncwarp();
+      fence_after();
+      const float L = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      const bool whole = t0 == 0 && t1 == p.it.tiles, fix = p.poison != 0;
       constexpr int STRIDE = ROWS * (HD + 2);
       float* part = piece_part(a, p, blockIdx.x, STRIDE);
-      auto store = [&](const float (&v)[32], int c) {  // 32 values of the row from dim c on
-        const int64_t at = (int64_t)(start + token) * a.ld_out + (int64_t)head * HD + c;
+      auto store = [&](const float (&v)[16], int c) {  // 16 values of the row from dim c on
+        const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)head * HD + c;
         if (a.out32) {
           float* y = static_cast<float*>(a.out) + at;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y[e] = v[e];
+          for (int e = 0; e < 16; ++e) y[e] = v[e];
         } else {
-          uint32_t w[16];
+          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = H::pack(v[2 * e], v[2 * e + 1]);
+          for (int e = 0; e < 8; ++e) w[e] = H::pack(v[2 * e], v[2 * e + 1]);
           uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at);
           if (a.vec_out) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 2; ++e)
               reinterpret_cast<uint4*>(y)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = w[e];
+            for (int e = 0; e < 8; ++e) y[e] = w[e];
           }
         }
       };
       if (mine) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t o[32];
-          ld32(o, o_addr + c);
-          float v[32];
+        for (int c = 0; c < HD; c += 16) {
+          uint32_t o[16];
+          ld16(o, o_addr + c);
+          float v[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]);
+          for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(o[e]);
           if (fix)
-            for (int j = max(t0 * TILE, least); j < min(t1 * TILE, lim); ++j) {
+            for (int j = max(t0 * TILE, p.least); j < min(t1 * TILE, lim); ++j) {
               const int page = __ldcg(a.table + (int64_t)p.it.b * a.max_pages + (j >> a.c.page_shift));
               if ((unsigned)page >= (unsigned)a.c.num_pages) continue;
               const unsigned short* src = reinterpret_cast<const unsigned short*>(a.c.v) +
                                           (((int64_t)page * a.c.kv_heads + p.kvh) * P + (j & (P - 1))) * HD + c;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
+              for (int e = 0; e < 16; ++e) {
                 const float y = H::up(__ldcg(src + e));
                 if (!(fabsf(y) <= 3.402823466e38f)) v[e] += y;
               }
             }
           if (whole) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] *= inv;
+            for (int e = 0; e < 16; ++e) v[e] *= inv;
             if (row < rows) store(v, c);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
+            for (int e = 0; e < 16; e += 4)
               *reinterpret_cast<float4*>(part + ((c + e) / 4 * ROWS + row) * 4) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           }
         }
@@ -496,44 +576,46 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!whole) {
         *reinterpret_cast<float2*>(part + ROWS * HD + 2 * row) = make_float2(ref, L);
         const int c0 = p.c0, c1 = p.c1;
-        __threadfence();
         mbar_arrive(&bars.join);
         ok = wait(&bars.join, joins++);
         if (!ok) break;
-        if (tid == 0) is_last = atomicAdd(a.count + p.unit, 1) == c1 - c0;
+        if (tid == 0) {
+          __threadfence();
+          is_last = atomicAdd(a.count + p.unit, 1) == c1 - c0;
+          __threadfence();
+        }
         mbar_arrive(&bars.join);
         ok = wait(&bars.join, joins++);
         if (!ok) break;
         if (is_last) {
-          __threadfence();
           auto piece = [&](int c) { return piece_part(a, p, c, STRIDE); };
           float top = -INFINITY, all = 0.f;
-          for (int c = c0; c <= c1; ++c)
-            top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row)).x);
+          for (int c = c0; c <= c1; ++c) top = max3(top, __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row)).x, -INFINITY);
           for (int c = c0; c <= c1; ++c) {
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row));
             all += ml.y * (ml.x == top ? 1.f : pa_ex2(ml.x - top));
           }
           const float inv = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll 1
-          for (int d0 = 0; d0 < HD; d0 += 32) {
-            float v[32];
+          for (int d0 = 0; d0 < HD; d0 += 16) {
+            float v[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+            for (int e = 0; e < 16; ++e) v[e] = 0.f;
+#pragma unroll 2
             for (int c = c0; c <= c1; ++c) {
               const float* src = piece(c);
               const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * row));
               if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
               const float f = ml.x == top ? 1.f : pa_ex2(ml.x - top);
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
+              for (int e = 0; e < 16; e += 4) {
                 const float4 x = __ldcg(reinterpret_cast<const float4*>(src + ((d0 + e) / 4 * ROWS + row) * 4));
                 v[e] = fmaf(x.x, f, v[e]), v[e + 1] = fmaf(x.y, f, v[e + 1]);
                 v[e + 2] = fmaf(x.z, f, v[e + 2]), v[e + 3] = fmaf(x.w, f, v[e + 3]);
               }
             }
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] *= inv;
+            for (int e = 0; e < 16; ++e) v[e] *= inv;
             if (row < rows) store(v, d0);
           }
           if (tid == 0) a.count[p.unit] = 0;
@@ -543,7 +625,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ok = wait(&bars.join, joins++);
         if (!ok) break;
       }
-      n += 2 * (t1 - t0);
+      n += 2 * (t1 - t0), c_clean += max(0, t1 - m0);
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.d_empty[k & 1]);
     }
@@ -556,10 +638,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-template <typename T, int HD, bool FANCY>
+template <typename T, int HD, int MODE>
 static cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
   using F = Cfg<HD>;
-  auto kern = paged_tc_kernel<T, HD, FANCY>;
+  auto kern = paged_tc_kernel<T, HD, MODE>;
   CUtensorMap maps[2];
   if (cudaError_t e = paged_maps(a.c, TILE, maps)) return e;
   static PagedReady ready;
@@ -569,15 +651,19 @@ static cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
 
 }  // namespace ptc
 
-cudaError_t launch_paged_tc(PagedAttnArgs& a, bool fancy, cudaStream_t s) {
+cudaError_t launch_paged_tc(PagedAttnArgs& a, cudaStream_t s) {
   using namespace ptc;
   static_assert(ROWS == PAGED_ROWS_MAX, "the scratch's pieces");
-  if (a.c.dtype == ODI_CUDA_PAGED_BF16) {
-    if (a.c.hd == 128) return fancy ? launch<__nv_bfloat16, 128, true>(a, s) : launch<__nv_bfloat16, 128, false>(a, s);
-    return fancy ? launch<__nv_bfloat16, 64, true>(a, s) : launch<__nv_bfloat16, 64, false>(a, s);
-  }
-  if (a.c.hd == 128) return fancy ? launch<__half, 128, true>(a, s) : launch<__half, 128, false>(a, s);
-  return fancy ? launch<__half, 64, true>(a, s) : launch<__half, 64, false>(a, s);
+  const int mode = a.cap_log2 != 0.f ? CAP : a.slopes ? BIAS : PLAIN;
+  auto by_mode = [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    return mode == CAP ? launch<T, HD, CAP>(a, s) : mode == BIAS ? launch<T, HD, BIAS>(a, s) : launch<T, HD, PLAIN>(a, s);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (a.c.dtype == ODI_CUDA_PAGED_BF16) return a.c.hd == 128 ? by_mode(__nv_bfloat16{}, D128{}) : by_mode(__nv_bfloat16{}, D64{});
+  return a.c.hd == 128 ? by_mode(__half{}, D128{}) : by_mode(__half{}, D64{});
 }
 
 }  // namespace odi_cuda
