@@ -75,6 +75,11 @@ struct Half16<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float up(uint16_t x) { return __half2float(__ushort_as_half(x)); }
+  // Pairs: 0 * x + y, NaN where x is not finite.
+  static __device__ __forceinline__ uint32_t times0(uint32_t x, uint32_t y) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0)), *reinterpret_cast<const __half2*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
 };
 template <>
 struct Half16<__nv_bfloat16> {
@@ -85,6 +90,11 @@ struct Half16<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float up(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+  static __device__ __forceinline__ uint32_t times0(uint32_t x, uint32_t y) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __bfloat162bfloat162(__ushort_as_bfloat16(0)),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&y));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
 };
 
 __device__ __forceinline__ void pa_tma(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {

@@ -10,7 +10,7 @@
 //   warps 0-3, 4-7  softmax of the two halves: thread = row
 //   warp 8          TMA producer: K and V tiles of 64 positions, page by page
 //   warps 9, 10     issue the products, one warp a half; warp 9 holds the tensor memory
-//   warp 11         idle
+//   warp 11         brings Q
 //
 // Each half has two S, so that the scores of the next tile are there when the
 // weights of this one are done.  (One S of 128 positions a half, which leaves the
@@ -157,7 +157,7 @@ struct Piece {
 struct Bars {
   uint64_t full[12], empty[12];
   uint64_t s_full[2][2], p_full[2][2];  // of a half's two S
-  uint64_t q_full[2], pv_done[2][2];    // in turn too: a half can wait two products ahead
+  uint64_t q_full[2], q_empty[2], pv_done[2][2];    // in turn too: a half can wait two products ahead
   uint64_t v_clean[8];  // in turn: a half can be ahead of the other by the tiles that the ring holds
   uint64_t d_full[2], d_empty[2], join, drain[2];
 };
@@ -183,10 +183,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < ST; ++i) mbar_init(&bars.full[i], 1), mbar_init(&bars.empty[i], 2);
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) mbar_init(&bars.s_full[i][b], 1), mbar_init(&bars.p_full[i][b], 128);
-      mbar_init(&bars.q_full[i], 128);
+      mbar_init(&bars.q_full[i], 1);
+      mbar_init(&bars.q_empty[i], 1);
       mbar_init(&bars.pv_done[i][0], 1), mbar_init(&bars.pv_done[i][1], 1);
       mbar_init(&bars.d_full[i], 1);
-      mbar_init(&bars.d_empty[i], 10);
+      mbar_init(&bars.d_empty[i], 11);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&bars.v_clean[i], 128);
     mbar_init(&bars.join, 256);
@@ -322,6 +323,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                      ID_S, ks > 0);
             commit(&bars.s_full[h][b]);
             commit(&bars.empty[nk % ST]);
+            if (i + 3 == end) commit(&bars.q_empty[h]);
           }
           __syncwarp();
           ++c_s;
@@ -338,12 +340,54 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (elect_one()) commit(&bars.drain[h]);
     __syncwarp();
     wait(&bars.drain[h], 0);
+  } else if (any && warp == 11) {
+    // ---- Q of a piece, as soon as the products of the piece before have read theirs:
+    // 16-byte pieces, HD / 8 to a row, rows that there are none of zero
+    constexpr int PER = HD / 8;
+    const int ch = lane % PER, r0 = lane / PER;
+    const T* q = static_cast<const T*>(a.q) + ch * 8;
+    int c_q[2] = {0, 0};
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      if (!wait(&bars.d_full[k & 1], k / 2)) break;
+      const Piece& d = pieces[k & 1];
+      const PagedPiece& p = d.p;
+      if (p.last) break;
+      for (int h = 0; ok && h < 2; ++h) {
+        if (d.end[h] <= p.t0) continue;
+        if (c_q[h]) ok = wait(&bars.q_empty[h], c_q[h] - 1);
+        if (!ok) break;
+        ++c_q[h];
+        const uint32_t dst = smem_u32(smem + F::Q_OFF + h * F::Q_HALF + (ch >> 3) * F::Q_PLANE);
+        const T* base = q + p.it.start * a.ld_q + (int64_t)p.kvh * a.G * HD;
+        const int R0 = p.it.i * ROWS + h * HALF_ROWS, live = p.rows - h * HALF_ROWS;
+#pragma unroll 4
+        for (int r = r0; r < HALF_ROWS; r += 32 / PER) {
+          const int tk = pa_token(a, R0 + r);
+          const T* src = r < live ? base + tk * a.ld_q + (R0 + r - tk * a.G) * HD : q;
+          const uint32_t to = dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+          if (a.vec) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(r < live ? 16 : 0) : "memory");
+          } else {
+            const unsigned* s4 = reinterpret_cast<const unsigned*>(src);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < live) x = make_uint4(__ldcg(s4), __ldcg(s4 + 1), __ldcg(s4 + 2), __ldcg(s4 + 3));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_full[h]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.d_empty[k & 1]);
+    }
   } else if (any && warp < 8) {
     // ---- softmax: thread = row
     const int h = warp >> 2, hr = tid & 127, row = tid;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lanes + F::O_COL + h * 128;
-    uint8_t* qs = smem + F::Q_OFF + h * F::Q_HALF;
     int n = 0, c_s = 0, c_pv = 0, c_clean = 0, joins = 0;
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -359,29 +403,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       // positions below it are seen by all rows of this half
       const int least_h = paged_limit(p.it.past, pa_token(a, p.it.i * ROWS + h * HALF_ROWS), p.it.len, p.it.prefix);
       const float slope = MODE != PLAIN && a.slopes && row < rows ? __ldg(a.slopes + head) * 1.4426950408889634f : 0.f;
-      if (mine) {
-        // Q: 16-byte pieces, HD / 8 to a row
-        constexpr int PER = HD / 8;
-        const T* q = static_cast<const T*>(a.q);
-#pragma unroll 4
-        for (int i = hr; i < HALF_ROWS * PER; i += 128) {
-          const int r = i / PER, ch = i % PER;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (h * HALF_ROWS + r < rows) {
-            const int RR = p.it.i * ROWS + h * HALF_ROWS + r, tk = pa_token(a, RR);
-            const T* src = q + (int64_t)(p.it.start + tk) * a.ld_q + (int64_t)(p.kvh * a.G + RR - tk * a.G) * HD + ch * 8;
-            if (a.vec) {
-              x = __ldcg(reinterpret_cast<const uint4*>(src));
-            } else {
-              const unsigned* s4 = reinterpret_cast<const unsigned*>(src);
-              x = make_uint4(__ldcg(s4), __ldcg(s4 + 1), __ldcg(s4 + 2), __ldcg(s4 + 3));
-            }
-          }
-          *reinterpret_cast<uint4*>(qs + (ch >> 3) * F::Q_PLANE + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&bars.q_full[h]);
-      }
       float ref = -INFINITY;
       float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
       for (int t = t0; t < t_end; ++t) {
@@ -487,22 +508,33 @@ __global__ void __launch_bounds__(THREADS, 1)
           ok = wait(&bars.full[iv % ST], iv / ST);
           if (!ok) break;
           if (pos >= p.least) {
-            bool bad = false;
-#pragma unroll 1
-            for (int ch = (hr >> 6) * (HD / 16); ch < ((hr >> 6) + 1) * (HD / 16); ++ch) {
-              uint4* x = reinterpret_cast<uint4*>(smem + iv % ST * F::SLOT + r * 128 + (ch >> 3) * F::PLANE + (((ch & 7) ^ (r & 7)) << 4));
-              const uint4 y = *x;
-              uint32_t z[4] = {y.x, y.y, y.z, y.w};
-              bool any_bad = false;
+            uint8_t* v = smem + iv % ST * F::SLOT + r * 128;
+            auto at = [&](int e) {
+              const int ch = (hr >> 6) * (HD / 16) + e;
+              return reinterpret_cast<uint4*>(v + (ch >> 3) * F::PLANE + (((ch & 7) ^ (r & 7)) << 4));
+            };
+            uint4 z[HD / 16];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((z[e] & H::EXP) == H::EXP) z[e] &= 0xffff0000u, any_bad = true;
-                if ((z[e] & (H::EXP << 16)) == H::EXP << 16) z[e] &= 0xffffu, any_bad = true;
-              }
-              if (any_bad) *x = make_uint4(z[0], z[1], z[2], z[3]);
-              bad = bad || any_bad;
+            for (int e = 0; e < HD / 16; ++e) z[e] = *at(e);
+            uint32_t zero = 0;  // 0 times all values: 0 if every one is finite
+#pragma unroll
+            for (int e = 0; e < HD / 16; ++e) {
+              zero = H::times0(z[e].x, zero), zero = H::times0(z[e].y, zero);
+              zero = H::times0(z[e].z, zero), zero = H::times0(z[e].w, zero);
             }
-            if (bad && pos < p.it.len) d.p.poison = 1;
+            if (zero & 0x7fff7fffu) {
+              if (pos < p.it.len) d.p.poison = 1;
+#pragma unroll 1
+              for (int e = 0; e < HD / 16; ++e) {
+                uint32_t* x = reinterpret_cast<uint32_t*>(at(e));
+                for (int i = 0; i < 4; ++i) {
+                  uint32_t y = x[i];
+                  if ((y & H::EXP) == H::EXP) y &= 0xffff0000u;
+                  if ((y & (H::EXP << 16)) == H::EXP << 16) y &= 0xffffu;
+                  x[i] = y;
+                }
+              }
+            }
           }
           fence_proxy_async_smem();
           mbar_arrive(&bars.v_clean[(c_clean + t - m0) & 7]);
@@ -590,33 +622,41 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (is_last) {
           auto piece = [&](int c) { return piece_part(a, p, c, STRIDE); };
           float top = -INFINITY, all = 0.f;
+#pragma unroll 4
           for (int c = c0; c <= c1; ++c) top = max3(top, __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row)).x, -INFINITY);
-          for (int c = c0; c <= c1; ++c) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row));
-            all += ml.y * (ml.x == top ? 1.f : pa_ex2(ml.x - top));
-          }
-          const float inv = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll 1
-          for (int d0 = 0; d0 < HD; d0 += 16) {
-            float v[16];
+          for (int d0 = 0; d0 < HD; d0 += 32) {
+            float v[32];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = 0.f;
+            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+            all = 0.f;
 #pragma unroll 2
             for (int c = c0; c <= c1; ++c) {
               const float* src = piece(c);
               const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * row));
-              if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw nothing
-              const float f = ml.x == top ? 1.f : pa_ex2(ml.x - top);
+              float4 x[8];
 #pragma unroll
-              for (int e = 0; e < 16; e += 4) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(src + ((d0 + e) / 4 * ROWS + row) * 4));
-                v[e] = fmaf(x.x, f, v[e]), v[e + 1] = fmaf(x.y, f, v[e + 1]);
-                v[e + 2] = fmaf(x.z, f, v[e + 2]), v[e + 3] = fmaf(x.w, f, v[e + 3]);
+              for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(src + ((d0 / 4 + e) * ROWS + row) * 4));
+              // a piece in which the row saw nothing left no sums
+              const bool some = !(ml.x == -INFINITY && ml.y == 0.f);
+              const float f = ml.x == top ? 1.f : pa_ex2(ml.x - top);
+              if (some) {
+                all = fmaf(ml.y, f, all);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  v[4 * e] = fmaf(x[e].x, f, v[4 * e]), v[4 * e + 1] = fmaf(x[e].y, f, v[4 * e + 1]);
+                  v[4 * e + 2] = fmaf(x[e].z, f, v[4 * e + 2]), v[4 * e + 3] = fmaf(x[e].w, f, v[4 * e + 3]);
+                }
               }
             }
+            const float inv = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] *= inv;
-            if (row < rows) store(v, d0);
+            for (int g = 0; g < 32; g += 16) {
+              float y[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) y[e] = v[g + e] * inv;
+              if (row < rows) store(y, d0 + g);
+            }
           }
           if (tid == 0) a.count[p.unit] = 0;
         }
