@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     while (ok && run.x < run.end) {
       const PagedPiece p = run_piece(a, run, ROWS);
       const int len = p.it.len;
-      PagedNames names(a, p, TILE);
+      PagedNames names(a, p, TILE, false);
       if (k >= 2 && !wait(&d_empty[k & 1], k / 2 - 1)) break;
       if (lane == 0) {
         pieces[k & 1] = p;
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
             float x = sc[i >> 1][2 * e + (i & 1)] * a.scale_log2;
             const int j = pw + (i >> 1) * 8 + 2 * c + (i & 1);
             if (FANCY) {
-              if (a.cap_log2 != 0.f) x = a.cap_log2 * pa_tanh(x);
+              if (a.cap_log2 != 0.f) x = pa_cap(x, a.cap_log2);
               x = fmaf(-slope[e], (float)abs(tok[e] - j), x);
             }
             if (masked && j >= lim[e]) x = -INFINITY;
@@ -577,7 +577,7 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.header = batch->work, a.max_items = (int)g.max_items;
   a.G = g.G, a.out_rows = tokens;
   a.inv_G = g.G > 1 ? (unsigned)(((1ull << 32) + g.G - 1) / g.G) : 0;
-  a.scale_log2 = softcap > 0.f ? scale / softcap : scale * 1.4426950408889634f;
+  a.scale_log2 = (softcap > 0.f ? 2.f * (scale / softcap) : scale) * 1.4426950408889634f;
   a.cap_log2 = softcap * 1.4426950408889634f;
   a.slopes = d_slopes;
   a.vec = !((uintptr_t)d_q & 15) && !(ld_q & 7);

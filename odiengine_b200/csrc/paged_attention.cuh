@@ -34,7 +34,7 @@ struct PagedAttnArgs {
   int max_items;
   int G, out_rows;
   unsigned inv_G;    // ceil(2^32 / G): r / G = r * inv_G >> 32 (G > 1)
-  float scale_log2;  // scale * log2(e), or scale / cap where there is a cap
+  float scale_log2;  // scale * log2(e); with a cap 2 scale / cap * log2(e)
   float cap_log2;    // cap * log2(e), or 0
   const float* slopes;
   int vec, vec_out;  // q, out and their strides allow 16-byte accesses
@@ -56,10 +56,8 @@ __device__ __forceinline__ float pa_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh(x) = 1 - 2 / (e^2x + 1): to about 2^-23 of 1, which the cap then scales.
-__device__ __forceinline__ float pa_tanh(float x) {
-  return fmaf(-2.f, pa_rcp(pa_ex2(x * 2.885390081777927f) + 1.f), 1.f);
-}
+// cap * tanh(x), x as 2 x log2(e): cap * (1 - 2 / (e^2x + 1)), to about 2^-23 of the cap.
+__device__ __forceinline__ float pa_cap(float x, float cap) { return fmaf(-2.f * cap, pa_rcp(pa_ex2(x) + 1.f), cap); }
 __device__ __forceinline__ int pa_token(const PagedAttnArgs& a, int r) {
   return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.inv_G);
 }
@@ -193,21 +191,22 @@ __device__ __forceinline__ void run_next(const PagedAttnArgs& a, PagedRun& r) {
 // per tile, even one tile ahead, held a CTA to a tile per round trip: 0.95 us).
 struct PagedNames {
   const int* row;
+  int step;  // of the blocks: 1, or -1 from the last tile to the first
   int last, block, cur, next;  // entries there are; the 32 at hand
-  __device__ __forceinline__ PagedNames(const PagedAttnArgs& a, const PagedPiece& p, int tile)
-      : row(a.table + (int64_t)p.it.b * a.max_pages) {
+  __device__ __forceinline__ PagedNames(const PagedAttnArgs& a, const PagedPiece& p, int tile, bool down)
+      : row(a.table + (int64_t)p.it.b * a.max_pages), step(down ? -1 : 1) {
     last = (min(p.it.len, p.t1 * tile) + a.c.page_size - 1) >> a.c.page_shift;
-    block = (p.t0 * tile >> a.c.page_shift) >> 5;
-    cur = load(block), next = load(block + 1);
+    block = ((down ? p.t1 - 1 : p.t0) * tile >> a.c.page_shift) >> 5;
+    cur = load(block), next = load(block + step);
   }
   __device__ __forceinline__ int load(int b) const {
     const int i = b * 32 + (threadIdx.x & 31);
-    return i < last ? __ldcg(row + i) : -1;
+    return i >= 0 && i < last ? __ldcg(row + i) : -1;
   }
-  // Entry i, the whole warp asking for entries of one block of 32, at or behind the last's.
+  // Entry i, the whole warp asking for entries of one block of 32, at or next to the last's.
   __device__ __forceinline__ int at(int i) {
     const int b = __shfl_sync(0xffffffffu, i, 0) >> 5;
-    if (b != block) block = b, cur = next, next = load(b + 1);
+    if (b != block) block = b, cur = next, next = load(b + step);
     return __shfl_sync(0xffffffffu, cur, i & 31);
   }
 };

@@ -169,6 +169,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   using F = Cfg<HD>;
   using H = Half16<T>;
   constexpr int ST = F::ST, PLANES = HD / 64;
+  // With a distance bias a long piece goes from its last tile to its first: scores
+  // only fall that way, and the reference stays where the first tiles put it (2048
+  // tokens over 4000 positions 396 us, 492 the other way).  Otherwise the tiles that
+  // not every row sees whole come last, when their V is there (seven prompts, of 5 to
+  // 19 tiles: 104 us, 116 the other way).
+  auto downward = [](const PagedPiece& p) { return MODE == BIAS && p.t1 - p.t0 > 24; };
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ Bars bars;
@@ -220,7 +226,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     while (ok && run.x < run.end) {
       const PagedPiece p = run_piece(a, run, ROWS);
       const int len = p.it.len;
-      PagedNames names(a, p, TILE);
+      const bool down = downward(p);
+      PagedNames names(a, p, TILE, down);
       if (k >= 2 && !wait(&bars.d_empty[k & 1], k / 2 - 1)) break;
       if (lane == 0) {
         Piece& d = pieces[k & 1];
@@ -236,10 +243,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       ++k;
       if (run.x < run.end) run_next(a, run);
       int y_next = 0, live_next = 0;  // of the tile whose K went last, for its V
-      for (int t = p.t0; ok && t <= p.t1; ++t) {
+      const int tiles = p.t1 - p.t0;
+      for (int i = 0; ok && i <= tiles; ++i) {
         const int y_v = y_next, live_v = live_next;
-        if (t < p.t1) {
-          const int pos = t * TILE + box * BR;
+        if (i < tiles) {
+          const int t = down ? p.t1 - 1 - i : p.t0 + i, pos = t * TILE + box * BR;
           live_next = min(boxes, (len - t * TILE + BR - 1) / BR);
           const int page = names.at(pos >> a.c.page_shift);
           y_next = (page * a.c.kv_heads + p.kvh) * P + (pos & (P - 1));
@@ -249,7 +257,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         for (int v = 0; v < 2; ++v) {
-          if (v ? t == p.t0 : t == p.t1) continue;
+          if (v ? i == 0 : i == tiles) continue;
           const int s = n % ST, live = v ? live_v : live_next, y = v ? y_v : y_next;
           if (n >= ST && !wait(&bars.empty[s], n / ST - 1)) {
             ok = false;
@@ -281,41 +289,45 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!wait(&bars.d_full[k & 1], k / 2)) break;
       const Piece& d = pieces[k & 1];
       if (d.p.last) break;
-      const int t0 = d.p.t0, tiles = d.p.t1 - t0, m0 = max(0, d.p.least / TILE - t0), end = d.end[h] - t0;
-      if (end > 0) ok = wait(&bars.q_full[h], c_q++);
+      const int tiles = d.p.t1 - d.p.t0, mine = d.end[h] - d.p.t0;
+      const bool down = downward(d.p);
+      const int first = down ? tiles - mine : 0, end = down ? tiles : mine;  // the half's tiles in the piece's order
+      const int clean = max(0, d.p.t1 - max(d.p.t0, d.p.least / TILE)), c0 = down ? 0 : tiles - clean;  // those that V is checked in
+      if (mine > 0) ok = wait(&bars.q_full[h], c_q++);
       // tile i of the piece: K is load 0, 1, 3, 5 ..., V load 2, 4, ... and the last
       for (int i = -2; ok && i < tiles; ++i) {
         const int nk = n + (i + 2 ? 2 * (i + 2) - 1 : 0), nv = n + min(2 * i + 2, 2 * tiles - 1);
-        if (i >= 0) {
+        if (i >= first && i < end && i >= 0) {
           const int b = c_p & 1;
-          if (i < end) {
-            ok = wait(&bars.p_full[h][b], c_p >> 1) && wait(&bars.full[nv % ST], nv / ST);
-            if (ok && i >= m0) ok = wait(&bars.v_clean[(c_clean + i - m0) & 7], (c_clean + i - m0) >> 3);
-            if (!ok) break;
-            fence_after();
-            if (elect_one()) {
-              const uint64_t v = desc(ring + nv % ST * F::SLOT, F::PLANE);
-#pragma unroll
-              for (int ks = 0; ks < TILE / 16; ++ks) mma_ts(o_col, s_col + b * 64 + ks * 8, v + ks * (2048 >> 4), ID_O, i > 0 || ks > 0);
-              commit(&bars.pv_done[h][b]);
-              commit(&bars.empty[nv % ST]);
-            }
-            __syncwarp();
-            // the next S goes where this P is: an order that nothing but the wait gives
-            if (i + 2 < end) ok = wait(&bars.pv_done[h][b], c_p >> 1);
-            ++c_p;
-          } else {  // not before it is there: the slot's next tile has a release of its own
-            ok = wait(&bars.full[nv % ST], nv / ST);
-            if (!ok) break;
-            if (lane == 0) mbar_arrive(&bars.empty[nv % ST]);
-          }
-        }
-        if (i + 2 < end) {
-          ok = ok && wait(&bars.full[nk % ST], nk / ST);
+          ok = wait(&bars.p_full[h][b], c_p >> 1) && wait(&bars.full[nv % ST], nv / ST);
+          const int cc = c_clean + i - c0;
+          if (ok && i >= c0 && i < c0 + clean) ok = wait(&bars.v_clean[cc & 7], cc >> 3);
           if (!ok) break;
+          ++c_p;
           fence_after();
           if (elect_one()) {
-            const int b = c_s & 1;
+            const uint64_t v = desc(ring + nv % ST * F::SLOT, F::PLANE);
+#pragma unroll
+            for (int ks = 0; ks < TILE / 16; ++ks) mma_ts(o_col, s_col + b * 64 + ks * 8, v + ks * (2048 >> 4), ID_O, i > first || ks > 0);
+            commit(&bars.pv_done[h][b]);
+            commit(&bars.empty[nv % ST]);
+          }
+          __syncwarp();
+        } else if (i >= 0) {  // not before it is there: the slot's next tile has a release of its own
+          ok = wait(&bars.full[nv % ST], nv / ST);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&bars.empty[nv % ST]);
+        }
+        if (i + 2 >= tiles) continue;
+        ok = wait(&bars.full[nk % ST], nk / ST);
+        if (i + 2 >= first && i + 2 < end) {
+          // S goes where the P of two tiles before was: an order that nothing but a wait gives
+          const int b = c_s & 1;
+          if (ok && c_s > 1) ok = wait(&bars.pv_done[h][b], (c_s >> 1) - 1);
+          if (!ok) break;
+          ++c_s;
+          fence_after();
+          if (elect_one()) {
             const uint64_t qd = desc(q, 0), kd = desc(ring + nk % ST * F::SLOT, 0);
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks)
@@ -326,14 +338,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (i + 3 == end) commit(&bars.q_empty[h]);
           }
           __syncwarp();
-          ++c_s;
-        } else if (i + 2 < tiles) {
-          ok = ok && wait(&bars.full[nk % ST], nk / ST);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(&bars.empty[nk % ST]);
+        } else if (ok && lane == 0) {
+          mbar_arrive(&bars.empty[nk % ST]);
         }
       }
-      n += 2 * tiles, c_clean += max(0, tiles - m0);
+      n += 2 * tiles, c_clean += clean;
       if (lane == 0) mbar_arrive(&bars.d_empty[k & 1]);
     }
     // products in flight end before the tensor memory goes
@@ -396,8 +405,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (d.p.last) break;
       const PagedPiece& p = d.p;
       const int rows = p.rows, t0 = p.t0, t1 = p.t1, t_end = d.end[h];
-      const bool mine = t_end > t0;
-      const int m0 = max(t0, p.least / TILE);  // the first tile that not every row sees whole
+      const bool mine = t_end > t0, down = downward(p);
+      const int clean = max(0, t1 - max(t0, p.least / TILE));  // tiles that not every row sees whole
       const int R = p.it.i * ROWS + row, token = pa_token(a, R), head = p.kvh * a.G + R - token * a.G;
       const int lim = row < rows ? paged_limit(p.it.past, token, p.it.len, p.it.prefix) : 0;
       // positions below it are seen by all rows of this half
@@ -405,7 +414,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const float slope = MODE != PLAIN && a.slopes && row < rows ? __ldg(a.slopes + head) * 1.4426950408889634f : 0.f;
       float ref = -INFINITY;
       float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-      for (int t = t0; t < t_end; ++t) {
+      for (int i = 0; i < t_end - t0; ++i) {
+        const int t = down ? t_end - 1 - i : t0 + i;
         const int b = c_s & 1;
         const uint32_t s_addr = tmem + lanes + h * 128 + b * 64;
         ok = wait(&bars.s_full[h][b], c_s >> 1);
@@ -418,27 +428,23 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int col0 = t * TILE;
         if (MODE == CAP) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) s[c] = __float_as_uint(a.cap_log2 * pa_tanh(__uint_as_float(s[c]) * a.scale_log2));
+          for (int c = 0; c < 64; ++c) s[c] = __float_as_uint(pa_cap(__uint_as_float(s[c]) * a.scale_log2, a.cap_log2));
         }
         if (MODE == BIAS || (MODE == CAP && a.slopes)) {
           const int away = p.it.past + token - col0;  // the row's own column
-          const float scale = MODE == CAP ? 1.f : a.scale_log2;
-          const float2 sc2 = make_float2(scale, scale), sl2 = make_float2(slope, slope);
+          const float scale = MODE == CAP ? 1.f : a.scale_log2, b0 = -slope * (float)away;
+          const float2 sc2 = make_float2(scale, scale);
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2,
+                                        make_float2(fmaf(slope, (float)c, b0), fmaf(slope, (float)(c + 1), b0)));
+            s[c] = __float_as_uint(x.x), s[c + 1] = __float_as_uint(x.y);
+          }
           if (__any_sync(0xffffffffu, lim - col0 > away + 1 && away < 63)) {
-            // part of the tile lies behind the row and is seen: distances have a sign
-            const float a0 = (float)away;
+            // part of the tile lies behind the row and is seen: it is as far the other way
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              s[c] = __float_as_uint(fmaf(-slope, fabsf((float)c - a0), __uint_as_float(s[c]) * scale));
-          } else {
-            const float b0 = -slope * (float)away;
-            const float2 b2 = make_float2(b0, b0);
-#pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-              const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2,
-                                          __ffma2_rn(make_float2((float)c, (float)(c + 1)), sl2, b2));
-              s[c] = __float_as_uint(x.x), s[c + 1] = __float_as_uint(x.y);
-            }
+              if (c > away) s[c] = __float_as_uint(fmaf(-2.f * slope, (float)(c - away), __uint_as_float(s[c])));
           }
         }
         if (col0 + 64 > least_h) {
@@ -461,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const float f = top == ref ? 1.f : pa_ex2(ref - top);
           ref = top;
           sum[0].x *= f, sum[0].y *= f, sum[1].x *= f, sum[1].y *= f;
-          if (t > t0) {
+          if (i > 0) {
             ok = wait(&bars.pv_done[h][(c_pv - 1) & 1], (c_pv - 1) >> 1);
             if (!ok) break;
             __syncwarp();
@@ -502,9 +508,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         st32(s, s_addr);
         wait_st();
-        if (t >= m0 && h == (t < d.end[1] ? 1 : 0)) {
+        if (t >= t1 - clean && h == (t < d.end[1] ? 1 : 0)) {
           // the last half at work takes what is not finite out of V: thread = position, half its dims
-          const int iv = n + min(2 * (t - t0) + 2, 2 * (t1 - t0) - 1), r = hr & 63, pos = t * TILE + r;
+          const int ip = down ? t1 - 1 - t : t - t0, cc = c_clean + (down ? ip : ip - (t1 - t0 - clean));
+          const int iv = n + min(2 * ip + 2, 2 * (t1 - t0) - 1), r = hr & 63, pos = t * TILE + r;
           ok = wait(&bars.full[iv % ST], iv / ST);
           if (!ok) break;
           if (pos >= p.least) {
@@ -537,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           fence_proxy_async_smem();
-          mbar_arrive(&bars.v_clean[(c_clean + t - m0) & 7]);
+          mbar_arrive(&bars.v_clean[cc & 7]);
         }
         fence_before();
         mbar_arrive(&bars.p_full[h][b]);
@@ -665,7 +672,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         ok = wait(&bars.join, joins++);
         if (!ok) break;
       }
-      n += 2 * (t1 - t0), c_clean += max(0, t1 - m0);
+      n += 2 * (t1 - t0), c_clean += clean;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.d_empty[k & 1]);
     }
