@@ -508,6 +508,20 @@ cudaError_t paged_maps(const PagedView& c, int tile, CUtensorMap* maps) {
   return cudaSuccess;
 }
 
+// q as [token][head][dim], boxes of 64 dims by the heads of a group by some tokens.
+cudaError_t paged_q_map(const PagedAttnArgs& a, int tokens, CUtensorMap* map) {
+  const EncodeFn enc = encode_fn();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.c.hd, (cuuint64_t)a.c.kv_heads * a.G, (cuuint64_t)a.out_rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.c.hd * 2, (cuuint64_t)a.ld_q * 2};
+  const cuuint32_t box[3] = {64u, (cuuint32_t)a.G, (cuuint32_t)tokens}, ones[3] = {1, 1, 1};
+  return enc(map, a.c.dtype == ODI_CUDA_PAGED_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+             const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? cudaSuccess
+             : cudaErrorInvalidValue;
+}
+
 cudaError_t launch_paged_mma(PagedAttnArgs& a, int groups, bool fancy, cudaStream_t s) {
   const bool bf = a.c.dtype == ODI_CUDA_PAGED_BF16;
   auto by_rows = [&](auto t, auto hd) {

@@ -38,6 +38,7 @@ struct PagedAttnArgs {
   float cap_log2;    // cap * log2(e), or 0
   const float* slopes;
   int vec, vec_out;  // q, out and their strides allow 16-byte accesses
+  int q_boxes;       // Q comes by TMA
   int least;         // tiles per CTA at least
   float* part;       // [2 * CTAs][rows][HD + 2]
   int* count;        // arrivals per unit, zero between launches
@@ -233,6 +234,7 @@ struct PagedReady {
 };
 
 cudaError_t paged_maps(const PagedView& c, int tile, CUtensorMap* maps);
+cudaError_t paged_q_map(const PagedAttnArgs& a, int tokens, CUtensorMap* map);
 cudaError_t launch_paged_mma(PagedAttnArgs& a, int groups, bool fancy, cudaStream_t s);
 cudaError_t launch_paged_tc(PagedAttnArgs& a, cudaStream_t s);
 

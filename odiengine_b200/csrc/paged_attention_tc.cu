@@ -150,6 +150,14 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
 // What a score goes through: nothing but the scale; a distance bias; a cap (and a bias).
 enum { PLAIN = 0, BIAS = 1, CAP = 2 };
 
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
 struct Piece {
   PagedPiece p;
   int end[2];  // tiles of the unit that each half of its rows sees
@@ -165,7 +173,7 @@ struct Bars {
 template <typename T, int HD, int MODE>
 __global__ void __launch_bounds__(THREADS, 1)
     paged_tc_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
-                    const __grid_constant__ CUtensorMap vmap) {
+                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap) {
   using F = Cfg<HD>;
   using H = Half16<T>;
   constexpr int ST = F::ST, PLANES = HD / 64;
@@ -350,8 +358,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
     wait(&bars.drain[h], 0);
   } else if (any && warp == 11) {
-    // ---- Q of a piece, as soon as the products of the piece before have read theirs:
-    // 16-byte pieces, HD / 8 to a row, rows that there are none of zero
+    // ---- Q of a piece, as soon as the products of the piece before have read theirs.
+    // 128 rows are a box of whole tokens where the group divides 128; else 16-byte
+    // pieces, HD / 8 to a row (a half of 128 dims takes 4 us so, 1 as boxes).  Rows that
+    // there are none of are zero or another request's: nothing of them is kept.
     constexpr int PER = HD / 8;
     const int ch = lane % PER, r0 = lane / PER;
     const T* q = static_cast<const T*>(a.q) + ch * 8;
@@ -367,6 +377,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (c_q[h]) ok = wait(&bars.q_empty[h], c_q[h] - 1);
         if (!ok) break;
         ++c_q[h];
+        if (a.q_boxes) {
+          if (lane == 0) {
+            const int token = p.it.start + (p.it.i * ROWS + h * HALF_ROWS) / a.G;
+            mbar_arrive_expect_tx(&bars.q_full[h], F::Q_HALF);
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl)
+              tma_3d(smem + F::Q_OFF + h * F::Q_HALF + pl * F::Q_PLANE, &qmap, pl * 64, p.kvh * a.G, token, &bars.q_full[h]);
+          }
+          continue;
+        }
         const uint32_t dst = smem_u32(smem + F::Q_OFF + h * F::Q_HALF + (ch >> 3) * F::Q_PLANE);
         const T* base = q + p.it.start * a.ld_q + (int64_t)p.kvh * a.G * HD;
         const int R0 = p.it.i * ROWS + h * HALF_ROWS, live = p.rows - h * HALF_ROWS;
@@ -460,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int e = 0; e < 4; ++e) m4[e] = max3(m4[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1]));
         const float scale = MODE == PLAIN ? a.scale_log2 : 1.f;
         const float mx = max3(max3(m4[0], m4[1], m4[2]), m4[3], -INFINITY) * scale;
-        const bool move = !(mx <= ref + MOVE);
+        const bool move = !(mx <= ref + MOVE) && ref == ref;  // a row that is NaN stays so
         if (__any_sync(0xffffffffu, move)) {
           // a NaN among the scores, or +inf, leaves no weight: the row is NaN from here on
           const float top = !move ? ref : mx == INFINITY ? __int_as_float(0x7fc00000) : mx;
@@ -686,14 +706,19 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 template <typename T, int HD, int MODE>
-static cudaError_t launch(const PagedAttnArgs& a, cudaStream_t s) {
+static cudaError_t launch(PagedAttnArgs& a, cudaStream_t s) {
   using F = Cfg<HD>;
   auto kern = paged_tc_kernel<T, HD, MODE>;
-  CUtensorMap maps[2];
+  CUtensorMap maps[3];
   if (cudaError_t e = paged_maps(a.c, TILE, maps)) return e;
+  // whole tokens of a group: boxes of 64 dims, G heads, 128 / G tokens
+  a.q_boxes = a.vec && HALF_ROWS % a.G == 0;
+  maps[2] = maps[0];
+  if (a.q_boxes)
+    if (cudaError_t e = paged_q_map(a, HALF_ROWS / a.G, &maps[2])) return e;
   static PagedReady ready;
   if (cudaError_t e = ready.set((const void*)kern, F::SMEM)) return e;
-  return launch_pdl_smem(kern, dim3(paged_ctas(ROWS)), dim3(THREADS), F::SMEM, s, a, maps[0], maps[1]);
+  return launch_pdl_smem(kern, dim3(paged_ctas(ROWS)), dim3(THREADS), F::SMEM, s, a, maps[0], maps[1], maps[2]);
 }
 
 }  // namespace ptc
