@@ -8,10 +8,12 @@
 // the first page dropped back first.  Who gets which page follows from exclusive
 // sums over the requests, so a step is the same whatever order the blocks run in.
 //
-// One cluster: every CTA sums the requests' counts for itself (the lists are
-// short), then they share out the requests' pages and the step's rows; two
-// cluster barriers stand between drops, takes and the rows' reads of the table.
-// Latency bound.
+// One CTA for short lists.  Else a cluster: every CTA sums the requests' counts for
+// itself (the lists are short), then they share out the requests' pages and the
+// step's rows.  One barrier stands between drops and takes; a row on a page that this
+// step takes reads the free list, as the table's writer does, so that rows need not
+// wait for the table.  Bound by latency: three round trips to memory (lists, dropped
+// entries, taken pages) and four sums over the block.
 #include <cstdio>
 
 #include "internal.h"
@@ -22,7 +24,6 @@
 namespace odi_cuda {
 namespace {
 
-constexpr int THREADS = 1024, WARPS = THREADS / 32;
 constexpr int MAX_B = ODI_CUDA_PAGED_MAX_REQUESTS;
 // what keeps a request from getting its rows
 constexpr int REFUSED = ODI_CUDA_PAGED_BAD_NEW | ODI_CUDA_PAGED_TOO_LONG | ODI_CUDA_PAGED_TOO_MANY_ROWS | ODI_CUDA_PAGED_NO_PAGES;
@@ -37,34 +38,32 @@ struct StepArgs {
   int page_shift;
 };
 
-struct Sum3 {
-  int a, b, c;
+struct Sum2 {
+  int a, b;
 };
-// Exclusive sums over the block's threads; `total` gets the sums of all.
-__device__ __forceinline__ Sum3 block_scan(Sum3 v, Sum3* total, Sum3* warps) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
-  Sum3 s = v;
+// Exclusive sums over the block's threads; `total` gets the sums of all.  `warps` is
+// a buffer that no other sum uses.
+template <int WARPS>
+__device__ __forceinline__ Sum2 block_scan(Sum2 v, Sum2* total, Sum2* warps) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Sum2 s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, s.a, o), b = __shfl_up_sync(0xffffffffu, s.b, o),
-              c = __shfl_up_sync(0xffffffffu, s.c, o);
-    if (lane >= o) s.a += a, s.b += b, s.c += c;
+    const int a = __shfl_up_sync(0xffffffffu, s.a, o), b = __shfl_up_sync(0xffffffffu, s.b, o);
+    if (lane >= o) s.a += a, s.b += b;
   }
-  __syncthreads();  // the last scan's sums have been read
   if (lane == 31) warps[warp] = s;
   __syncthreads();
-  Sum3 w = lane < n ? warps[lane] : Sum3{0, 0, 0};
+  Sum2 w = lane < WARPS ? warps[lane] : Sum2{0, 0};
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, w.a, o), b = __shfl_up_sync(0xffffffffu, w.b, o),
-              c = __shfl_up_sync(0xffffffffu, w.c, o);
-    if (lane >= o) w.a += a, w.b += b, w.c += c;
+  for (int o = 1; o < WARPS; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, w.a, o), b = __shfl_up_sync(0xffffffffu, w.b, o);
+    if (lane >= o) w.a += a, w.b += b;
   }
-  *total = {__shfl_sync(0xffffffffu, w.a, 31), __shfl_sync(0xffffffffu, w.b, 31), __shfl_sync(0xffffffffu, w.c, 31)};
+  *total = {__shfl_sync(0xffffffffu, w.a, WARPS - 1), __shfl_sync(0xffffffffu, w.b, WARPS - 1)};
   const int before = max(warp - 1, 0);
-  const Sum3 p = {__shfl_sync(0xffffffffu, w.a, before), __shfl_sync(0xffffffffu, w.b, before),
-                  __shfl_sync(0xffffffffu, w.c, before)};
-  return {s.a - v.a + (warp ? p.a : 0), s.b - v.b + (warp ? p.b : 0), s.c - v.c + (warp ? p.c : 0)};
+  const Sum2 p = {__shfl_sync(0xffffffffu, w.a, before), __shfl_sync(0xffffffffu, w.b, before)};
+  return {s.a - v.a + (warp ? p.a : 0), s.b - v.b + (warp ? p.b : 0)};
 }
 
 __device__ __forceinline__ void step_barrier(int C) {
@@ -87,106 +86,127 @@ __device__ __forceinline__ int last_at_most(const int* first, int n, int x) {
   return lo;
 }
 
+// CHUNKS * THREADS requests at most, `CHUNKS` per thread.
+template <int THREADS, int CHUNKS>
 __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_constant__ StepArgs a) {
+  constexpr int WARPS = THREADS / 32, ROOM = CHUNKS * THREADS;
   // per request: positions kept; first row; rank of its first page dropped (later:
   // its first item); rank of its first page taken, or -1 for one that is refused
-  __shared__ int s_keep[MAX_B], s_row0[MAX_B + 1], s_drop0[MAX_B], s_take0[MAX_B];
-  __shared__ Sum3 warps[32];
+  __shared__ int s_keep[ROOM], s_row0[ROOM + 1], s_drop0[ROOM], s_take0[ROOM];
+  __shared__ Sum2 warps[4][CHUNKS][WARPS], tiles_of[2][WARPS];
   __shared__ int s_status, s_taken;
   pdl_launch_dependents();
+  const int tid = threadIdx.x;
+  if (tid == 0) s_status = s_taken = 0;
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = gridDim.x, rank = blockIdx.x, B = a.t.requests;
   const int shift = a.page_shift, P = 1 << shift;
   const int cap = (int)min((long long)a.t.max_pages << shift, 0x7fffffffll);
   const int n = min(max(__ldcg(a.t.free_count), 0), a.t.num_pages);
-  if (tid == 0) s_status = s_taken = 0;
   auto pages = [&](int len) { return (int)(((long long)len + P - 1) >> shift); };
   struct Want {
-    int len, keep, rows, drops, takes, bad;
-  };
-  auto want = [&](int b) {
-    Want w{};
-    int fresh = __ldcg(a.fresh + b);
-    w.len = __ldcg(a.t.lens + b);
-    int keep = a.keep ? __ldcg(a.keep + b) : w.len;
-    if (w.len < 0 || w.len > cap) w.bad |= ODI_CUDA_PAGED_BAD_LENGTH, w.len = min(max(w.len, 0), cap);
-    if (keep < 0 || keep > w.len) w.bad |= a.keep ? ODI_CUDA_PAGED_BAD_KEEP : 0, keep = min(max(keep, 0), w.len);
-    w.keep = keep;
-    w.rows = min(max(fresh, 0), a.b.max_rows);
-    if (fresh < 0 || fresh > a.b.max_new) w.bad |= ODI_CUDA_PAGED_BAD_NEW;
-    else if (fresh > cap - keep) w.bad |= ODI_CUDA_PAGED_TOO_LONG;
-    w.drops = pages(w.len) - pages(keep);
-    w.takes = w.bad & REFUSED ? 0 : pages(keep + w.rows) - pages(keep);
-    return w;
-  };
+    int had, keep, rows, takes, bad, row0;
+  } w[CHUNKS];
   // ---- what goes, and where rows begin
-  Sum3 base = {0, 0, 0};
-  for (int b0 = 0; b0 < B; b0 += THREADS) {
-    const int b = b0 + tid;
-    Want w{};
-    if (b < B) w = want(b);
-    Sum3 total;
-    const Sum3 e = block_scan({w.drops, w.rows, 0}, &total, warps);
+  Sum2 base = {0, 0};
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int b = c * THREADS + tid;
+    w[c] = {};
     if (b < B) {
-      s_keep[b] = w.keep;
+      const int fresh = __ldcg(a.fresh + b);
+      int len = __ldcg(a.t.lens + b), keep = a.keep ? __ldcg(a.keep + b) : len;
+      if (len < 0 || len > cap) w[c].bad |= ODI_CUDA_PAGED_BAD_LENGTH, len = min(max(len, 0), cap);
+      if (keep < 0 || keep > len) w[c].bad |= a.keep ? ODI_CUDA_PAGED_BAD_KEEP : 0, keep = min(max(keep, 0), len);
+      w[c].rows = min(max(fresh, 0), a.b.max_rows);
+      if (fresh < 0 || fresh > a.b.max_new) w[c].bad |= ODI_CUDA_PAGED_BAD_NEW;
+      else if (fresh > cap - keep) w[c].bad |= ODI_CUDA_PAGED_TOO_LONG;
+      w[c].had = pages(len), w[c].keep = keep;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int b = c * THREADS + tid;
+    Sum2 total;
+    const Sum2 e = block_scan<WARPS>({b < B ? w[c].had - pages(w[c].keep) : 0, w[c].rows}, &total, warps[0][c]);
+    if (b < B) {
+      s_keep[b] = w[c].keep;
       s_drop0[b] = base.a + e.a;
-      s_row0[b] = min(base.b + e.b, a.b.max_rows);
+      s_row0[b] = w[c].row0 = min(base.b + e.b, a.b.max_rows);
+      if (w[c].rows && w[c].row0 + w[c].rows > a.b.max_rows) w[c].bad |= ODI_CUDA_PAGED_TOO_MANY_ROWS;
+      w[c].takes = w[c].bad & REFUSED ? 0 : pages(w[c].keep + w[c].rows) - pages(w[c].keep);
     }
     base.a += total.a, base.b += total.b;
   }
   const int drops = base.a, rows = min(base.b, a.b.max_rows);
-  if (tid == 0) s_row0[B] = rows;
-  __syncthreads();
   const int top = min(n + drops, a.t.num_pages);  // a table that names pages twice cannot push past the list's end
-  for (int b = rank * WARPS + warp; b < B; b += C * WARPS) {
-    const int len = min(max(__ldcg(a.t.lens + b), 0), cap);
-    const int j0 = pages(s_keep[b]), j1 = pages(len), r0 = s_drop0[b];
-    int* row = a.t.table + (int64_t)b * a.t.max_pages;
-    for (int j = j0 + lane; j < j1; j += 32) {
-      const int at = n + drops - 1 - (r0 + j - j0);
-      if (at < a.t.num_pages) a.t.free_pages[at] = __ldcg(row + j);
-      row[j] = -1;
-    }
-  }
-  // ---- what comes: every CTA again for itself, before the lengths change.
-  // A request whose pages are not there, and those after it that need some, take
-  // none; so the pages that are taken are those of the first ranks.
-  base = {0, 0, 0};
-  for (int b0 = 0; b0 < B; b0 += THREADS) {
-    const int b = b0 + tid;
-    Want w{};
+  if (tid == 0) s_row0[B] = rows;
+  // ---- what comes.  A request whose pages are not there, and those after it that need
+  // some, take none; so the pages that are taken are those of the first ranks.
+  base = {0, 0};
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int b = c * THREADS + tid;
+    Sum2 total;
+    const Sum2 e = block_scan<WARPS>({w[c].takes, 0}, &total, warps[1][c]);
     if (b < B) {
-      w = want(b);
-      if (w.rows && s_row0[b] + w.rows > a.b.max_rows) w.bad |= ODI_CUDA_PAGED_TOO_MANY_ROWS;
-      if (w.bad & REFUSED) w.takes = 0;
-    }
-    Sum3 total;
-    const Sum3 e = block_scan({w.takes, 0, 0}, &total, warps);
-    if (b < B) {
-      const int last = base.a + e.a + w.takes;
-      if (w.takes && last > top) w.bad |= ODI_CUDA_PAGED_NO_PAGES;
-      const bool granted = !(w.bad & REFUSED);
+      const int last = base.a + e.a + w[c].takes;
+      if (w[c].takes && last > top) w[c].bad |= ODI_CUDA_PAGED_NO_PAGES;
+      const bool granted = !(w[c].bad & REFUSED);
       s_take0[b] = granted ? base.a + e.a : -1;
-      if (granted && w.takes) atomicMax(&s_taken, last);
-      if (w.bad) atomicOr(&s_status, w.bad);
+      if (granted && w[c].takes) atomicMax(&s_taken, last);
+      if (w[c].bad) atomicOr(&s_status, w[c].bad);
     }
     base.a += total.a;
   }
+  __syncthreads();
+  // a page dropped per thread, a row per thread
+  for (int k = rank * THREADS + tid; k < drops; k += C * THREADS) {
+    const int b = last_at_most(s_drop0, B, k), at = n + drops - 1 - k;
+    int* entry = a.t.table + (int64_t)b * a.t.max_pages + pages(s_keep[b]) + k - s_drop0[b];
+    if (at < a.t.num_pages) a.t.free_pages[at] = __ldcg(entry);
+    *entry = -1;
+  }
   step_barrier(C);  // drops are on the list, and every CTA has read the lengths
-  for (int b = rank * WARPS + warp; b < B; b += C * WARPS) {
-    const int r0 = s_take0[b];
-    if (r0 < 0) continue;
-    const int j0 = pages(s_keep[b]), j1 = pages(s_keep[b] + s_row0[b + 1] - s_row0[b]);
-    int* row = a.t.table + (int64_t)b * a.t.max_pages;
-    for (int j = j0 + lane; j < j1; j += 32) row[j] = __ldcg(a.t.free_pages + (top - 1 - (r0 + j - j0)));
+  constexpr int U = THREADS < 1024 ? 1 : 4;  // rows of a thread whose loads overlap
+  for (int q = rank * THREADS + tid; q < a.b.max_rows; q += U * C * THREADS) {
+    int pos[U], page[U], *entry[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = q + u * C * THREADS;
+      pos[u] = page[u] = -1, entry[u] = nullptr;
+      if (r >= rows) continue;
+      const int b = last_at_most(s_row0, B, r), first = s_take0[b];
+      if (first < 0) continue;
+      pos[u] = s_keep[b] + r - s_row0[b];
+      const int j = pos[u] >> shift, kept = pages(s_keep[b]);
+      int* e = a.t.table + (int64_t)b * a.t.max_pages + j;
+      if (j < kept) {
+        page[u] = __ldcg(e);
+      } else {  // a page that the request takes: its first row writes the table
+        page[u] = __ldcg(a.t.free_pages + (top - 1 - (first + j - kept)));
+        if (!(pos[u] & (P - 1))) entry[u] = e;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = q + u * C * THREADS;
+      if (r >= a.b.max_rows) break;
+      if (entry[u]) *entry[u] = page[u];
+      a.b.positions[r] = pos[u];
+      a.b.slots[r] = (unsigned)page[u] < (unsigned)a.t.num_pages ? (page[u] << shift) + (pos[u] & (P - 1)) : -1;
+    }
   }
   if (rank == 0) {
-    for (int b = tid; b < B; b += THREADS) {
-      const int n_rows = s_row0[b + 1] - s_row0[b], len = s_keep[b] + (s_take0[b] >= 0 ? n_rows : 0);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int b = c * THREADS + tid;
+      if (b >= B) break;
+      const bool granted = s_take0[b] >= 0;
+      const int len = w[c].keep + (granted ? w[c].rows : 0);
       a.t.lens[b] = len;
-      a.b.lens[b] = s_take0[b] >= 0 ? len : 0;
-      a.b.starts[b] = s_row0[b];
+      a.b.lens[b] = granted ? len : 0;
+      a.b.starts[b] = w[c].row0;
     }
     if (tid == 0) {
       a.b.starts[B] = rows;
@@ -196,19 +216,20 @@ __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_consta
   }
   if (rank == C - 1) {  // attention's work list, in the order of rows
     PagedItem* list = const_cast<PagedItem*>(paged_items(a.b.work));
-    int* s_item0 = s_drop0;
-    base = {0, 0, 0};
-    for (int b0 = 0; b0 < B; b0 += THREADS) {
-      const int b = b0 + tid;
+    int* s_item0 = s_drop0;  // every warp is past the drops
+    base = {0, 0};
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int b = c * THREADS + tid;
       int items = 0;
-      if (b < B && s_take0[b] >= 0) items = (int)(((int64_t)(s_row0[b + 1] - s_row0[b]) * a.g.G + a.g.rows - 1) / a.g.rows);
-      Sum3 total;
-      const Sum3 e = block_scan({items, 0, 0}, &total, warps);
+      if (b < B && s_take0[b] >= 0) items = (int)(((int64_t)w[c].rows * a.g.G + a.g.rows - 1) / a.g.rows);
+      Sum2 total;
+      const Sum2 e = block_scan<WARPS>({items, 0}, &total, warps[2][c]);
       if (b < B) s_item0[b] = base.a + e.a;
       base.a += total.a;
     }
     const int items = base.a;
-    base = {0, 0, 0};
+    base = {0, 0};
     __syncthreads();
     for (int i0 = 0; i0 < items; i0 += THREADS) {
       const int i = i0 + tid;
@@ -220,8 +241,8 @@ __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_consta
         x.prefix = a.prefix ? __ldcg(a.prefix + b) : 0;
         x.tiles = (paged_limit(x.past, token, x.len, x.prefix) + a.g.tile - 1) / a.g.tile;
       }
-      Sum3 total;
-      const Sum3 e = block_scan({x.tiles, 0, 0}, &total, warps);
+      Sum2 total;
+      const Sum2 e = block_scan<WARPS>({x.tiles, 0}, &total, tiles_of[i0 / THREADS & 1]);
       x.tile0 = base.a + e.a;
       if (i < items) list[i] = x;
       base.a += total.a;
@@ -230,20 +251,6 @@ __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_consta
       a.b.work[PW_ITEMS] = items;
       a.b.work[PW_TILES] = base.a;
     }
-  }
-  step_barrier(C);  // the table is whole
-  for (int r = rank * THREADS + tid; r < a.b.max_rows; r += C * THREADS) {
-    int pos = -1, slot = -1;
-    if (r < rows) {
-      const int b = last_at_most(s_row0, B, r);
-      if (s_take0[b] >= 0) {
-        pos = s_keep[b] + r - s_row0[b];
-        const int page = __ldcg(a.t.table + (int64_t)b * a.t.max_pages + (pos >> shift));
-        if ((unsigned)page < (unsigned)a.t.num_pages) slot = (page << shift) + (pos & (P - 1));
-      }
-    }
-    a.b.positions[r] = pos;
-    a.b.slots[r] = slot;
   }
 }
 
@@ -327,11 +334,12 @@ int odi_cuda_paged_step(const odi_cuda_page_tables* t, const odi_cuda_paged_batc
       (int64_t)t->max_pages * t->page_size > 0x7fffffffll)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: page_size, max_pages or num_pages out of range");
   a.t = *t, a.b = *batch, a.keep = d_keep, a.fresh = d_new, a.prefix = d_prefix, a.page_shift = page_shift_of(t->page_size);
-  // one CTA where its threads see to everything at once; else eight
-  const int C = batch->max_rows <= 2 * THREADS && t->requests <= 4 * WARPS ? 1 : 8;
+  // one CTA where its threads see to everything in a few passes; else eight
+  const bool small = t->requests <= 256 && batch->max_rows <= 1024;
+  const int C = small ? 1 : 8;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(small ? 256 : 1024);
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -340,7 +348,9 @@ int odi_cuda_paged_step(const odi_cuda_page_tables* t, const odi_cuda_paged_batc
   attr[1].val.clusterDim.x = C, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = C > 1 ? 2 : 1;
-  return kv_launched(cudaLaunchKernelEx(&cfg, paged_step_kernel, a), "paged_step");
+  return kv_launched(small ? cudaLaunchKernelEx(&cfg, paged_step_kernel<256, 1>, a)
+                           : cudaLaunchKernelEx(&cfg, paged_step_kernel<1024, MAX_B / 1024>, a),
+                     "paged_step");
 }
 
 }  // extern "C"
