@@ -302,13 +302,14 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     const bool live_group = rows > 0;
     uint32_t qf[KS][4];
     float o[HD / 8][4], m[2], l[2], slope[2];
-    int lim[2], tok[2];
+    int lim[2];
+    float tok[2];
     bool bad = false;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const bool live = e * 8 + g < rows;
       const int R = R0 + (live ? e * 8 + g : 0), token = pa_token(a, R), head = p.kvh * a.G + R - token * a.G;
-      tok[e] = past + token;
+      tok[e] = (float)(past + token);
       lim[e] = live ? paged_limit(past, token, len, p.it.prefix) : 0;
       slope[e] = FANCY && a.slopes && live ? __ldg(a.slopes + head) * 1.4426950408889634f : 0.f;
       m[e] = -INFINITY, l[e] = 0.f;
@@ -354,6 +355,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         if (lane == 0) mbar_arrive(&empty[sk]);
         // ---- scores, weights
         float mx[2];
+        const float at = (float)(pw + 2 * c);  // positions are whole below 2^24
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           mx[e] = -INFINITY;
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
             const int j = pw + (i >> 1) * 8 + 2 * c + (i & 1);
             if (FANCY) {
               if (a.cap_log2 != 0.f) x = pa_cap(x, a.cap_log2);
-              x = fmaf(-slope[e], (float)abs(tok[e] - j), x);
+              x = fmaf(-slope[e], fabsf(tok[e] - (at + (float)((i >> 1) * 8 + (i & 1)))), x);
             }
             if (masked && j >= lim[e]) x = -INFINITY;
             sc[i >> 1][2 * e + (i & 1)] = x;
