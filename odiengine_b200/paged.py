@@ -20,12 +20,13 @@ in a CUDA graph.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
 
-from . import lib
-from .draft import _call, _flat, _refuse, _rows2
+from . import FLAG_PDL, MatmulOpts, check, lib, new_workspace, workspace_bytes
+from .draft import _call, _flat, _raw_stream, _refuse, _rows2, logits_adjust, logits_scratch
 
 PAGED_DTYPES = {torch.float16: 0, torch.bfloat16: 1}  # ODI_CUDA_PAGED_*
 PAGE_SIZES = (16, 32, 64, 128)
@@ -247,3 +248,223 @@ def verify_sampled(logits, tokens, starts, u_accept, u_next, accepted=None, next
           _flat(u_accept, f32, "u_accept", dev, R), _flat(u_next, f32, "u_next", dev, B), _flat(accepted, i32, "accepted", dev, B),
           _flat(next, i32, "next", dev, B), _flat(scratch, torch.uint8, "scratch", dev, n), n)
     return accepted, next
+
+
+class _Pass:
+    """What a forward pass of up to max_rows rows keeps: its batch and scratch."""
+
+    def __init__(self, cache, tables, max_rows: int, max_new: int, heads: int):
+        self.batch = PagedBatch(tables, max_rows=max_rows, max_new=max_new, heads=heads, kv_heads=cache.kv_heads)
+        self.scratch = attention_paged_scratch(cache, self.batch)
+
+
+class PagedDecoder:
+    """Decoding of several sequences at once, over one paged cache: the model of
+    decode.DecodeModel for every request's new tokens in one pass.
+
+        d = PagedDecoder(cfg, seeded_model(cfg, interleave_gate_up=False), requests=8, num_pages=512)
+        a, b = d.add([1, 2, 3]), d.add(prompt)
+        while d.left(b): d.step()          # prompts go in `chunk` tokens at a time
+        new = d.step({a: [5, 9]})          # drafted tokens after a's pending one
+        d.finish(a)                        # its pages are free again
+
+    step returns, for every request whose prompt is in the cache, the tokens
+    that follow: those drafts that the target keeps, and one more.  With a
+    temperature they are sampled (drafts are verified by verify_sampled, random
+    numbers from `generator` or a generator of its own); without one greedy.  The
+    weights keep gate|up in [gate | up] order.  softcap, slopes: the model's
+    capped scores or distance biases.  Calls run on the current stream, which may
+    differ from call to call; one at a time."""
+
+    def __init__(self, cfg, weights, *, requests: int, num_pages: int, page_size: int = 16, dtype=torch.float16,
+                 max_drafts: int = 7, chunk: int = 256, temperature=None, generator=None, softcap: float = 0.0, slopes=None,
+                 device=None):
+        if weights.gu_interleaved:
+            raise ValueError("PagedDecoder needs gate|up weights in [gate | up] order (interleave_gate_up=False)")
+        if max_drafts < 0 or chunk < 1 or requests < 1:
+            raise ValueError("PagedDecoder: max_drafts 0 or more, chunk and requests 1 or more")
+        if temperature is not None and not 1e-6 <= temperature <= 1e6:
+            raise ValueError("temperature: 1e-6 to 1e6, or None for greedy decoding")
+        self.cfg, self.w, self.temperature = cfg, weights, temperature
+        dev = torch.device("cuda" if device is None else device)
+        self.device = dev = torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev
+        self.requests, self.max_drafts, self.chunk = requests, max_drafts, chunk
+        self.softcap, self.slopes = softcap, slopes
+        self.page_size, self.num_pages = page_size, num_pages
+        with torch.cuda.device(dev):
+            self.caches = [PagedCache.new(dtype, num_pages, cfg.kv_heads, page_size, cfg.head_dim, dev) for _ in range(cfg.layers)]
+            self.tables = PageTables.new(requests, -(-cfg.ctx // page_size), num_pages, page_size, dev)
+            decode_rows = requests * (1 + max_drafts)
+            self.rows = T = max(decode_rows, chunk)
+            # single tokens and drafts apart from chunks: they have kernels of their own
+            self._decode = _Pass(self.caches[0], self.tables, decode_rows, 1 + max_drafts, cfg.heads)
+            self._chunks = _Pass(self.caches[0], self.tables, T, chunk, cfg.heads)
+            f32, w = torch.float32, cfg.heads * cfg.head_dim
+            new = lambda *s, dt=f32: torch.empty(s, dtype=dt, device=dev)  # noqa: E731
+            self.x, self.qkv, self.q = new(T, cfg.hidden), new(T, cfg.qkv_rows), new(T, w, dt=dtype)
+            self.attn, self.gu = new(T, w), new(T, 2 * cfg.ffn)
+            self.logits = new(decode_rows, cfg.vocab)
+            self.states = torch.zeros((T, 4), dtype=torch.int32, device=dev)
+            self.verify_ws = verify_scratch(decode_rows, requests, cfg.vocab, dev)
+            self.greedy_ws, self.greedy = logits_scratch(decode_rows, dev), new(decode_rows, dt=torch.int32)
+            self.generator = torch.Generator(device=dev) if generator is None else generator
+            products = [m for lw in weights.layers for m in (lw.wqkv, lw.wo, lw.wgu, lw.wdown)] + [weights.output]
+            self.products_ws = new_workspace(max(workspace_bytes(m.dtype, T, m.N, m.K, cfg.act_mode) for m in products), dev)
+            self._last = torch.cuda.Event()
+            self._last.record(torch.cuda.current_stream(dev))
+        # per request: tokens to go into the cache (a prompt's rest, then the pending
+        # token), and how many positions it holds; None: free
+        self._todo, self._len = [None] * requests, [0] * requests
+
+    @contextlib.contextmanager
+    def _ordered(self):
+        """On the decoder's device, with the current stream after the last call's work."""
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream()
+            stream.wait_event(self._last)
+            try:
+                yield
+            finally:
+                self._last.record(stream)
+
+    def _product(self, dw, x, y, T, norm=None, swiglu=False, accumulate=False):
+        o = MatmulOpts(None if norm is None else norm.data_ptr(), self.cfg.eps, int(swiglu), int(accumulate), None, 0, None)
+        ws = self.products_ws
+        check(lib().odi_cuda_matmul_fused(dw.dtype, dw.data_ptr, x.data_ptr(), y.data_ptr(), T, dw.N, dw.K, self.cfg.act_mode,
+                                          ws.data_ptr(), ws.numel(), FLAG_PDL, ctypes.byref(o), _raw_stream(self.device.index)))
+
+    def _forward(self, p: _Pass, tokens: dict, logits: bool) -> None:
+        """The new tokens of some requests, {request: tokens}, in the requests' order."""
+        cfg, rows = self.cfg, [t for b in range(self.requests) for t in tokens.get(b, ())]
+        T, stream = len(rows), _raw_stream(self.device.index)
+        host = torch.tensor([self._len, [len(tokens.get(b, ())) for b in range(self.requests)]], dtype=torch.int32)
+        keep, fresh = host.to(self.device)
+        paged_step(self.tables, p.batch, fresh, keep=keep)
+        self.states[:T].copy_(torch.tensor([[t, 0, 0, 0] for t in rows], dtype=torch.int32))
+        for r in range(T):
+            check(lib().odi_cuda_embed(self.w.token_embd.data_ptr(), cfg.vocab, cfg.hidden, self.states.data_ptr() + 16 * r,
+                                       self.x.data_ptr() + 4 * cfg.hidden * r, None, None, None, stream))
+        for cache, lw in zip(self.caches, self.w.layers):
+            self._product(lw.wqkv, self.x, self.qkv, T, norm=lw.attn_norm)
+            qk_rope_append_paged(self.qkv[:T], cache, p.batch, self.q[:T], heads=cfg.heads, theta=cfg.theta)
+            attention_paged(self.q[:T], cache, self.tables, p.batch, self.attn[:T], scale=cfg.head_dim ** -0.5,
+                            softcap=self.softcap, slopes=self.slopes, scratch=p.scratch)
+            self._product(lw.wo, self.attn, self.x, T, accumulate=True)
+            self._product(lw.wgu, self.x, self.gu, T, norm=lw.ffn_norm)
+            self._product(lw.wdown, self.gu, self.x, T, swiglu=True, accumulate=True)
+        if logits:
+            self._product(self.w.output, self.x, self.logits, T, norm=self.w.out_norm)
+
+    def status(self) -> int:
+        """OR of the device error words (0: no bounded wait gave up, every page was one)."""
+        words = [ws[:4].view(torch.int32) for ws in (self._decode.scratch, self._chunks.scratch, self.products_ws)]
+        v = 0
+        for x in torch.cat(words).cpu().tolist():
+            v |= x
+        return v
+
+    def _check(self, p: _Pass) -> None:
+        st, refused = self.status(), p.batch.status()
+        if st or refused:
+            raise RuntimeError(f"paged decoding: a device wait gave up or a page was none (error word {st:#x}), or a request "
+                               f"was refused (status {refused})")
+
+    def _pages(self, n: int) -> int:
+        return -(-n // self.page_size)
+
+    @property
+    def free_pages(self) -> int:
+        """Pages that no request's positions need."""
+        return self.num_pages - sum(self._pages(n) for n in self._len)
+
+    # ---- requests ------------------------------------------------------------
+    def add(self, prompt) -> int:
+        """A new request; its prompt goes into the cache with the next steps."""
+        prompt = list(prompt)
+        if not prompt or any(not 0 <= t < self.cfg.vocab for t in prompt):
+            raise ValueError("add: a prompt of tokens of the vocabulary wanted")
+        if len(prompt) > self.cfg.ctx:
+            raise ValueError("add: prompt longer than the context")
+        b = next((b for b in range(self.requests) if self._todo[b] is None), None)
+        if b is None:
+            raise RuntimeError(f"add: all {self.requests} requests are in use")
+        self._todo[b], self._len[b] = prompt, 0
+        return b
+
+    def left(self, request: int) -> int:
+        """Prompt tokens that are not in the cache yet, but for the last."""
+        return len(self._tokens(request)) - 1
+
+    def finish(self, request: int) -> None:
+        """The request is over: its pages go back with the next step."""
+        self._tokens(request)
+        self._todo[request], self._len[request] = None, 0
+
+    def _tokens(self, b) -> list:
+        if not 0 <= b < self.requests or self._todo[b] is None:
+            raise ValueError(f"no request {b}")
+        return self._todo[b]
+
+    def step(self, drafts=None) -> dict:
+        """One step of every request: a chunk of those whose prompt is not in the
+        cache; the pending token, and drafts[request] after it, of the others.
+        Returns {request: new tokens} of the latter; the last of them is pending."""
+        drafts = dict(drafts or {})
+        for b, d in drafts.items():
+            if self.left(b):
+                raise ValueError(f"step: request {b} has prompt left")
+            if len(d) > self.max_drafts or any(not 0 <= t < self.cfg.vocab for t in d):
+                raise ValueError(f"step: at most {self.max_drafts} drafted tokens of the vocabulary")
+        live = [b for b in range(self.requests) if self._todo[b] is not None]
+        room, chunks = self.chunk, {}
+        for b in live:
+            n = min(room, len(self._todo[b]) - 1)
+            if n > 0:
+                chunks[b] = self._todo[b][:n]
+                room -= n
+        decode = {b: [self._todo[b][0], *drafts.get(b, ())] for b in live if len(self._todo[b]) == 1}
+        need = {b: self._len[b] + len(t) for b, t in (*chunks.items(), *decode.items())}
+        if any(n > self.cfg.ctx for n in need.values()):
+            raise ValueError("step: a request would run past the context")
+        if sum(self._pages(need.get(b, self._len[b])) for b in range(self.requests)) > self.num_pages:
+            raise RuntimeError("step: not enough free pages")
+        out = {}
+        with self._ordered():
+            if chunks:
+                self._forward(self._chunks, chunks, False)
+                self._check(self._chunks)
+                for b, t in chunks.items():
+                    self._len[b] += len(t)
+                    self._todo[b] = self._todo[b][len(t):]
+            if decode:
+                self._forward(self._decode, decode, True)
+                accepted, nxt = self._choose(decode)
+                self._check(self._decode)
+                if any(nxt[b] < 0 for b in decode):
+                    raise RuntimeError("step: logits without a finite value")
+                for b, t in decode.items():
+                    out[b] = [*t[1:1 + accepted[b]], nxt[b]]
+                    self._len[b] += 1 + accepted[b]
+                    self._todo[b] = [nxt[b]]
+        return out
+
+    def _choose(self, decode: dict):
+        """Drafts kept and the next token of each request, by the last pass's logits."""
+        T = sum(len(t) for t in decode.values())
+        if self.temperature is None:
+            _, g = logits_adjust(self.logits[:T], None, self.greedy[:T], scratch=self.greedy_ws)
+            greedy, accepted, nxt, r = g.tolist(), [0] * self.requests, [-1] * self.requests, 0
+            for b in range(self.requests):
+                t = decode.get(b, [])
+                while accepted[b] + 1 < len(t) and t[accepted[b] + 1] == greedy[r + accepted[b]]:
+                    accepted[b] += 1
+                if t:
+                    nxt[b] = greedy[r + accepted[b]]
+                r += len(t)
+            return accepted, nxt
+        u = torch.rand(T + self.requests, device=self.device, generator=self.generator)
+        self.u_accept, self.u_next = u[:T], u[T:]
+        tokens = self.states[:T, 0].contiguous()
+        accepted, nxt = verify_sampled(self.logits[:T], tokens, self._decode.batch.starts, self.u_accept, self.u_next,
+                                       temperature=self.temperature, scratch=self.verify_ws)
+        return accepted.tolist(), nxt.tolist()
