@@ -97,6 +97,10 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   }
   __syncthreads();
   pdl_wait();
+  if (smem_u32(smem) & 1023u) {  // the swizzle counts from there
+    if (tid == 0) atomicOr(a.err, ERR_PAGED_WAIT);
+    return;
+  }
   PagedRun run;
   if (!run_begin(a, run, &found)) return;
   const int P = a.c.page_size;
@@ -126,7 +130,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         const int pos = t * TILE + box * BR;
         const int live = min(boxes, (len - t * TILE + BR - 1) / BR);
         const int page = names.at(pos >> a.c.page_shift);
-        int y = (page * a.c.kv_heads + p.kvh) * P + (pos & (P - 1));
+        int y = (int)(((unsigned)page * a.c.kv_heads + p.kvh) * P) + (pos & (P - 1));
         if (box < live && (unsigned)page >= (unsigned)a.c.num_pages) {  // names no page: zeros, and the error word
           y = rows_all;
           atomicOr(a.err, ERR_PAGED_PAGE);

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int t = down ? p.t1 - 1 - i : p.t0 + i, pos = t * TILE + box * BR;
           live_next = min(boxes, (len - t * TILE + BR - 1) / BR);
           const int page = names.at(pos >> a.c.page_shift);
-          y_next = (page * a.c.kv_heads + p.kvh) * P + (pos & (P - 1));
+          y_next = (int)(((unsigned)page * a.c.kv_heads + p.kvh) * P) + (pos & (P - 1));
           if (box < live_next && (unsigned)page >= (unsigned)a.c.num_pages) {  // names no page: zeros, and the error word
             y_next = rows_all;
             atomicOr(a.err, ERR_PAGED_PAGE);

@@ -333,6 +333,8 @@ int odi_cuda_paged_step(const odi_cuda_page_tables* t, const odi_cuda_paged_batc
       (int64_t)t->num_pages * t->page_size > 0x7fffffffll || (int64_t)t->requests * t->max_pages > (1 << 30) ||
       (int64_t)t->max_pages * t->page_size > 0x7fffffffll)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: page_size, max_pages or num_pages out of range");
+  if (a.g.max_items * ((int64_t)t->max_pages * t->page_size / a.g.tile + 1) > 0x7fffffffll)
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: more work than 2^31 tiles");
   a.t = *t, a.b = *batch, a.keep = d_keep, a.fresh = d_new, a.prefix = d_prefix, a.page_shift = page_shift_of(t->page_size);
   // one CTA where its threads see to everything in a few passes; else eight
   const bool small = t->requests <= 256 && batch->max_rows <= 1024;

@@ -212,6 +212,40 @@ def test_attention(cuda_lib, past, new, heads, kv, hd, dtype, P, option):
     assert cuda_lib_status(s.scratch) == 0
 
 
+@pytest.mark.parametrize("past,new,heads,kv,hd,dtype,P", [([4000], [200], 64, 64, 64, "f16", 16), ([3500], [70], 96, 48, 128, "bf16", 64)])
+@pytest.mark.parametrize("option", ["slopes", "all"])
+def test_attention_long_pieces_with_a_bias(cuda_lib, past, new, heads, kv, hd, dtype, P, option):
+    """Steep and flat biases over runs of tiles long enough to go from the last tile
+    to the first; a NaN among the new tokens' values."""
+    from odiengine_b200 import paged
+
+    s = Setup(past, new, heads, kv, hd, dtype, P, prefix=[past[0] + 20] if option == "all" else None)
+    slot = int(s.batch.slots[new[0] // 2])
+    s.cache.v[slot // P, :, slot % P, 3] = math.nan
+    slopes = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)
+    out = paged.attention_paged(s.q, s.cache, s.tables, s.batch, scale=1 / math.sqrt(hd), slopes=slopes, scratch=s.scratch)
+    s.check(out, 1 / math.sqrt(hd), 0.0, slopes)
+    assert cuda_lib_status(s.scratch) == 0
+
+
+@pytest.mark.parametrize("new", [[2, 1], [9, 5], [40, 90]])
+@pytest.mark.parametrize("heads", [4, 6])
+@pytest.mark.parametrize("shift,pad", [(2, 0), (0, 6), (2, 2)])
+def test_attention_of_rows_that_are_not_aligned(cuda_lib, new, heads, shift, pad):
+    """Queries and outputs on 4-byte boundaries, at odd strides."""
+    from odiengine_b200 import paged
+
+    s = Setup([100, 3], new, heads, 2, 128, "bf16", 32)
+    T, w = s.q.shape
+    wide = torch.full((T, w + shift + pad), math.nan, dtype=s.q.dtype, device="cuda")
+    q = wide[:, shift:shift + w]
+    q.copy_(s.q)
+    out = torch.full((T, w + shift + pad), 5.0, dtype=s.q.dtype, device="cuda")
+    paged.attention_paged(q, s.cache, s.tables, s.batch, out[:, shift:shift + w], scale=0.09, scratch=s.scratch)
+    s.check(out[:, shift:shift + w], 0.09)
+    assert (out[:, :shift] == 5).all() and (out[:, shift + w:] == 5).all()
+
+
 def cuda_lib_status(scratch):
     return int(scratch[:4].view(torch.int32).item())
 

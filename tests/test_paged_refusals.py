@@ -97,6 +97,9 @@ def test_step_refusals():
                 dict(free=A + 3), dict(count=A + 2), dict(requests=2), dict(max_pages=0), dict(page_size=32), dict(page_size=20),
                 dict(num_pages=0), dict(num_pages=1 << 28), dict(max_pages=1 << 29)):
         refused(step(t=tables(**bad)))
+    # more tiles than a work list can count
+    refused(step(t=tables(requests=2048, max_pages=1 << 18, page_size=16), b=batch(requests=2048, max_rows=262144, max_new=262144, heads=64, kv_heads=1)),
+            word="tiles")
     refused(step(new=None))
     for k in ("keep", "new", "prefix"):
         refused(step(**{k: A + 2}))
