@@ -52,9 +52,9 @@ bool paged_geometry(int requests, int max_rows, int max_new, int heads, int kv_h
 inline bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128; }
 inline int page_shift_of(int p) { return p == 16 ? 4 : p == 32 ? 5 : p == 64 ? 6 : 7; }
 // Rows of an item and positions of a tile, by the most rows a request has per kv
-// head: the two widths of the mma.sync kernel, and the tcgen05 kernel's.
+// head: the two widths of the mma.sync kernel, and the two of the tcgen05 kernel.
 inline void paged_kind(int64_t most, int* rows, int* tile) {
-  *rows = most <= 16 ? 16 : most <= 32 ? 32 : 256;
+  *rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 128 ? 128 : 256;
   *tile = 64;
 }
 

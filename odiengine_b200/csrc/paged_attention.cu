@@ -551,7 +551,7 @@ extern "C" {
 // Error word, pieces, then a counter per unit.  The pieces' place has one size,
 // so that a scratch serves any batch whose counters fit.
 constexpr size_t PART_OFF = 256, COUNT_OFF = PART_OFF + (size_t)2 * PAGED_SMS * PAGED_ROWS_MAX * (128 + 2) * 4;
-static_assert(2 * paged_ctas(16) * 16 <= 2 * PAGED_SMS * PAGED_ROWS_MAX, "pieces of the narrow items");
+static_assert(paged_ctas(16) * 16 <= PAGED_SMS * PAGED_ROWS_MAX && paged_ctas(128) * 128 <= PAGED_SMS * PAGED_ROWS_MAX, "pieces of narrow items");
 
 size_t odi_cuda_attention_paged_scratch_bytes(int requests, int max_rows, int max_new, int heads, int kv_heads, int head_dim) {
   PagedGeometry g;
@@ -610,7 +610,7 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + COUNT_OFF);
   const bool fancy = softcap > 0.f || d_slopes;
   cudaStream_t s = (cudaStream_t)stream;
-  return kv_launched(g.rows <= 32 ? launch_paged_mma(a, g.rows / 16, fancy, s) : launch_paged_tc(a, s), "attention_paged");
+  return kv_launched(g.rows <= 32 ? launch_paged_mma(a, g.rows / 16, fancy, s) : launch_paged_tc(a, g.rows, s), "attention_paged");
 }
 
 }  // extern "C"

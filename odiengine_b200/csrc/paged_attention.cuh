@@ -236,10 +236,10 @@ struct PagedReady {
 cudaError_t paged_maps(const PagedView& c, int tile, CUtensorMap* maps);
 cudaError_t paged_q_map(const PagedAttnArgs& a, int tokens, CUtensorMap* map);
 cudaError_t launch_paged_mma(PagedAttnArgs& a, int groups, bool fancy, cudaStream_t s);
-cudaError_t launch_paged_tc(PagedAttnArgs& a, cudaStream_t s);
+cudaError_t launch_paged_tc(PagedAttnArgs& a, int rows, cudaStream_t s);
 
 constexpr int PAGED_SMS = 148, PAGED_ROWS_MAX = 256;
-// CTAs of a call: two per SM of the narrow kernel, else one
-constexpr int paged_ctas(int rows) { return rows <= 16 ? 2 * PAGED_SMS : PAGED_SMS; }
+// CTAs of a call: two per SM of the kernels' narrow forms, else one
+constexpr int paged_ctas(int rows) { return rows == 16 || rows == 128 ? 2 * PAGED_SMS : PAGED_SMS; }
 
 }  // namespace odi_cuda

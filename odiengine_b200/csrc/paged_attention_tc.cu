@@ -1,16 +1,17 @@
 // paged_attention_tc.cu -- attention of chunks of new tokens over a paged cache on
 // the sm_100a tensor cores (tcgen05.mma, accumulators in tensor memory).
 //
-// An item is up to 256 rows (new tokens * heads per kv head) of one request and kv
-// head, as two halves of 128 whose work alternates:
+// An item is up to 128 or 256 rows (new tokens * heads per kv head) of one request
+// and kv head, as one half or two halves of 128 whose work alternates (with one half
+// the other CTA of the SM alternates with it):
 //
 //   S [128 rows x 64 positions] = Q K^T     Q and K in shared memory
 //   O [128 rows x head_dim]    += P V       P in tensor memory, where S was
 //
-//   warps 0-3, 4-7  softmax of the two halves: thread = row
-//   warp 8          TMA producer: K and V tiles of 64 positions, page by page
-//   warps 9, 10     issue the products, one warp a half; warp 9 holds the tensor memory
-//   warp 11         brings Q
+//   warps 0-3 of a half  softmax: thread = row
+//   then four more       the TMA producer (K and V tiles of 64 positions, page by
+//                        page); two that issue the products, one a half, of which the
+//                        first holds the tensor memory; one that brings Q
 //
 // Each half has two S, so that the scores of the next tile are there when the
 // weights of this one are done.  (One S of 128 positions a half, which leaves the
@@ -27,7 +28,7 @@
 namespace odi_cuda {
 namespace ptc {
 
-constexpr int TILE = 64, ROWS = 256, HALF_ROWS = 128, THREADS = 384;
+constexpr int TILE = 64, HALF_ROWS = 128;
 constexpr float MOVE = 8.f;
 // Of eight pairs of weights one is exponentiated on the FMA pipe.  The loop over 64
 // scores of a row, two warps per scheduler: 933 cycles so, 1188 without, 964 with
@@ -39,16 +40,23 @@ __device__ __forceinline__ float ex2_here(float x) {
   return y;
 }
 
-template <int HD>
+// NH: halves of an item.  One: two CTAs per SM; two: one.
+template <int HD, int NH>
 struct Cfg {
   static constexpr int PLANE = TILE * 128, SLOT = HD / 64 * PLANE;      // K or V of one tile, in planes of 64 dims
   static constexpr int Q_PLANE = HALF_ROWS * 128, Q_HALF = HD / 64 * Q_PLANE;
-  static constexpr int ST = HD == 128 ? 8 : 12;
+  static constexpr int ST = (HD == 128 ? 4 : NH == 1 ? 8 : 6) * NH;
   static_assert(ST / 2 < 8, "v_clean");
   static constexpr int Q_OFF = ST * SLOT;
-  static constexpr int SMEM = Q_OFF + 2 * Q_HALF + 1024;  // + alignment slack
+  static constexpr int SMEM = Q_OFF + NH * Q_HALF + 1024;  // + alignment slack
+  static constexpr int ROWS = NH * HALF_ROWS, THREADS = NH * 128 + 128, PER_SM = 2 / NH;
+  static_assert(PER_SM * (SMEM + 2048) <= 228 * 1024, "shared memory, with 1 KB static and 1 KB of the system's");
+  // the launch's registers are shared out anew: a softmax thread holds a tile's scores
+  // and weights
+  static constexpr int REGS_LAUNCH = NH == 1 ? 128 : 168, REGS_FEW = 72, REGS_SOFT = NH == 1 ? 184 : 216;
+  static_assert(128 * REGS_FEW + 128 * NH * REGS_SOFT <= THREADS * REGS_LAUNCH, "register split");
   // tensor memory: two S per half, then an O per half
-  static constexpr int O_COL = 256, COLS = 512;
+  static constexpr int O_COL = NH * 128, COLS = NH * 256;
 };
 
 __device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo) {
@@ -170,13 +178,14 @@ struct Bars {
   uint64_t d_full[2], d_empty[2], join, drain[2];
 };
 
-template <typename T, int HD, int MODE>
-__global__ void __launch_bounds__(THREADS, 1)
+template <typename T, int HD, int MODE, int NH>
+__global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
     paged_tc_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap) {
-  using F = Cfg<HD>;
+  using F = Cfg<HD, NH>;
   using H = Half16<T>;
-  constexpr int ST = F::ST, PLANES = HD / 64;
+  constexpr int ST = F::ST, PLANES = HD / 64, ROWS = F::ROWS;
+  constexpr int PRODUCER = 4 * NH, PRODUCTS = PRODUCER + 1, LOADER = PRODUCER + 3;  // warps
   // With a distance bias a long piece goes from its last tile to its first: scores
   // only fall that way, and the reference stays where the first tiles put it (2048
   // tokens over 4000 positions 396 us, 492 the other way).  Otherwise the tiles that
@@ -194,22 +203,22 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   pdl_launch_dependents();
   if (tid == 0) {
-    for (int i = 0; i < ST; ++i) mbar_init(&bars.full[i], 1), mbar_init(&bars.empty[i], 2);
+    for (int i = 0; i < ST; ++i) mbar_init(&bars.full[i], 1), mbar_init(&bars.empty[i], NH);
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) mbar_init(&bars.s_full[i][b], 1), mbar_init(&bars.p_full[i][b], 128);
       mbar_init(&bars.q_full[i], 1);
       mbar_init(&bars.q_empty[i], 1);
       mbar_init(&bars.pv_done[i][0], 1), mbar_init(&bars.pv_done[i][1], 1);
       mbar_init(&bars.d_full[i], 1);
-      mbar_init(&bars.d_empty[i], 11);
+      mbar_init(&bars.d_empty[i], 5 * NH + 1);
     }
     for (int i = 0; i < 8; ++i) mbar_init(&bars.v_clean[i], 128);
-    mbar_init(&bars.join, 256);
+    mbar_init(&bars.join, 128 * NH);
     mbar_init(&bars.drain[0], 1), mbar_init(&bars.drain[1], 1);
     prefetch_map(&kmap), prefetch_map(&vmap);
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == PRODUCTS) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(F::COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -224,7 +233,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int P = a.c.page_size;
   auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, a.err, ERR_PAGED_WAIT); };
 
-  if (any && warp == 8) {
+  if (warp >= PRODUCER) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_FEW));
+  if (any && warp == PRODUCER) {
     // ---- producer: K0 K1 V0 K2 V1 ... V of a piece, as the products want them
     const int BR = min(P, TILE), boxes = TILE / BR;
     const int box = lane / PLANES, plane = lane % PLANES;
@@ -241,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         Piece& d = pieces[k & 1];
         d.p = p;
         const int all = min(ROWS, (len - p.it.past) * a.G - p.it.i * ROWS);
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < NH; ++h) {
           const int last_row = p.it.i * ROWS + min(all, (h + 1) * HALF_ROWS) - 1;
           const int tiles = (paged_limit(p.it.past, pa_token(a, last_row), len, p.it.prefix) + TILE - 1) / TILE;
           d.end[h] = all > h * HALF_ROWS ? max(p.t0, min(p.t1, tiles)) : p.t0;
@@ -286,9 +297,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     for (int i = max(0, n - ST); i < n; ++i) wait(&bars.full[i % ST], i / ST);  // no copy outlives the CTA
-  } else if (any && (warp == 9 || warp == 10)) {
+  } else if (any && warp >= PRODUCTS && warp < PRODUCTS + NH) {
     // ---- products of one half
-    const int h = warp - 9;
+    const int h = warp - PRODUCTS;
     const uint32_t ring = smem_u32(smem), q = ring + F::Q_OFF + h * F::Q_HALF, s_col = tmem + h * 128, o_col = tmem + F::O_COL + h * 128;
     constexpr uint32_t ID_S = idesc<H::BF>(TILE, false), ID_O = idesc<H::BF>(HD, true);
     int n = 0, c_clean = 0, c_q = 0, c_s = 0, c_p = 0;  // tiles of the half so far: its S in turn
@@ -357,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (elect_one()) commit(&bars.drain[h]);
     __syncwarp();
     wait(&bars.drain[h], 0);
-  } else if (any && warp == 11) {
+  } else if (any && warp == LOADER) {
     // ---- Q of a piece, as soon as the products of the piece before have read theirs.
     // 128 rows are a box of whole tokens where the group divides 128; else 16-byte
     // pieces, HD / 8 to a row (a half of 128 dims takes 4 us so, 1 as boxes).  Rows that
@@ -372,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Piece& d = pieces[k & 1];
       const PagedPiece& p = d.p;
       if (p.last) break;
-      for (int h = 0; ok && h < 2; ++h) {
+      for (int h = 0; ok && h < NH; ++h) {
         if (d.end[h] <= p.t0) continue;
         if (c_q[h]) ok = wait(&bars.q_empty[h], c_q[h] - 1);
         if (!ok) break;
@@ -412,13 +423,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.d_empty[k & 1]);
     }
-  } else if (any && warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REGS_SOFT));
     // ---- softmax: thread = row
     const int h = warp >> 2, hr = tid & 127, row = tid;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_addr = tmem + lanes + F::O_COL + h * 128;
     int n = 0, c_s = 0, c_pv = 0, c_clean = 0, joins = 0;
-    bool ok = true;
+    bool ok = any;
     for (int k = 0; ok; ++k) {
       if (!wait(&bars.d_full[k & 1], k / 2)) break;
       Piece& d = pieces[k & 1];
@@ -528,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         st32(s, s_addr);
         wait_st();
-        if (t >= t1 - clean && h == (t < d.end[1] ? 1 : 0)) {
+        if (t >= t1 - clean && (NH == 1 || h == (t < d.end[1] ? 1 : 0))) {
           // the last half at work takes what is not finite out of V: thread = position, half its dims
           const int ip = down ? t1 - 1 - t : t - t0, cc = c_clean + (down ? ip : ip - (t1 - t0 - clean));
           const int iv = n + min(2 * ip + 2, 2 * (t1 - t0) - 1), r = hr & 63, pos = t * TILE + r;
@@ -699,16 +712,16 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == PRODUCTS) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F::COLS) : "memory");
   }
 }
 
-template <typename T, int HD, int MODE>
+template <typename T, int HD, int MODE, int NH>
 static cudaError_t launch(PagedAttnArgs& a, cudaStream_t s) {
-  using F = Cfg<HD>;
-  auto kern = paged_tc_kernel<T, HD, MODE>;
+  using F = Cfg<HD, NH>;
+  auto kern = paged_tc_kernel<T, HD, MODE, NH>;
   CUtensorMap maps[3];
   if (cudaError_t e = paged_maps(a.c, TILE, maps)) return e;
   // whole tokens of a group: boxes of 64 dims, G heads, 128 / G tokens
@@ -718,24 +731,27 @@ static cudaError_t launch(PagedAttnArgs& a, cudaStream_t s) {
     if (cudaError_t e = paged_q_map(a, HALF_ROWS / a.G, &maps[2])) return e;
   static PagedReady ready;
   if (cudaError_t e = ready.set((const void*)kern, F::SMEM)) return e;
-  return launch_pdl_smem(kern, dim3(paged_ctas(ROWS)), dim3(THREADS), F::SMEM, s, a, maps[0], maps[1], maps[2]);
+  return launch_pdl_smem(kern, dim3(paged_ctas(F::ROWS)), dim3(F::THREADS), F::SMEM, s, a, maps[0], maps[1], maps[2]);
 }
 
 }  // namespace ptc
 
-cudaError_t launch_paged_tc(PagedAttnArgs& a, cudaStream_t s) {
+cudaError_t launch_paged_tc(PagedAttnArgs& a, int rows, cudaStream_t s) {
   using namespace ptc;
-  static_assert(ROWS == PAGED_ROWS_MAX, "the scratch's pieces");
+  static_assert(Cfg<128, 2>::ROWS == PAGED_ROWS_MAX, "the scratch's pieces");
   const int mode = a.cap_log2 != 0.f ? CAP : a.slopes ? BIAS : PLAIN;
-  auto by_mode = [&](auto t, auto hd) {
+  auto by_mode = [&](auto t, auto hd, auto nh) {
     using T = decltype(t);
-    constexpr int HD = decltype(hd)::value;
-    return mode == CAP ? launch<T, HD, CAP>(a, s) : mode == BIAS ? launch<T, HD, BIAS>(a, s) : launch<T, HD, PLAIN>(a, s);
+    constexpr int HD = decltype(hd)::value, NH = decltype(nh)::value;
+    return mode == CAP ? launch<T, HD, CAP, NH>(a, s) : mode == BIAS ? launch<T, HD, BIAS, NH>(a, s) : launch<T, HD, PLAIN, NH>(a, s);
+  };
+  auto by_rows = [&](auto t, auto hd) {
+    return rows == HALF_ROWS ? by_mode(t, hd, std::integral_constant<int, 1>{}) : by_mode(t, hd, std::integral_constant<int, 2>{});
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;
-  if (a.c.dtype == ODI_CUDA_PAGED_BF16) return a.c.hd == 128 ? by_mode(__nv_bfloat16{}, D128{}) : by_mode(__nv_bfloat16{}, D64{});
-  return a.c.hd == 128 ? by_mode(__half{}, D128{}) : by_mode(__half{}, D64{});
+  if (a.c.dtype == ODI_CUDA_PAGED_BF16) return a.c.hd == 128 ? by_rows(__nv_bfloat16{}, D128{}) : by_rows(__nv_bfloat16{}, D64{});
+  return a.c.hd == 128 ? by_rows(__half{}, D128{}) : by_rows(__half{}, D64{});
 }
 
 }  // namespace odi_cuda
