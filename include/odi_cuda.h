@@ -627,7 +627,8 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
  * d_out have.  Rows behind the batch's last, and of refused requests, are
  * left as they were.  A row all of whose scores are -inf is zero.  Scores,
  * softmax and sums are fp32; the weights are rounded to the cache's type.
- * scale is positive.
+ * scale is positive; softcap is at most 1024 (a capped score is off by 2^-21
+ * of the cap at most).
  * Scratch: odi_cuda_attention_paged_scratch_bytes, 16-byte aligned, zero
  * before its first use; calls of any layer, and of any batch that needs no
  * more, on one stream share it.  Its first word is an error word (odi_cuda_workspace_status):

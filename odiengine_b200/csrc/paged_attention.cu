@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)(p.kvh * a.G + R - token * a.G) * HD + d;
       if (a.out32) {
         float* y = static_cast<float*>(a.out) + at;
-        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
+        if (a.vec_out) *reinterpret_cast<float4*>(y) = v;
+        else y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
       } else {
         uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at);
         const uint32_t lo = H::pack(v.x, v.y), hi = H::pack(v.z, v.w);
@@ -578,6 +579,11 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: more tokens than the batch has rows");
   if (!(scale > 0.f) || !isfinite(scale) || !(softcap >= 0.f) || !isfinite(softcap))
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: scale must be positive, softcap 0 or more");
+  // a capped score is off by 2^-21 of the cap at most, which up to here stays below
+  // what the rounding of a weight to fp16 costs
+  const float scale_log2 = (softcap > 0.f ? 2.f * (scale / softcap) : scale) * 1.4426950408889634f;
+  if (softcap > 1024.f || !isfinite(scale_log2))
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: softcap is 1024 at most; scale, or scale / softcap, is out of range");
   const int64_t width = (int64_t)batch->heads * a.c.hd;
   if (ld_q < width || ld_out < width || ld_q > (1ll << 40) || ld_out > (1ll << 40))
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: a row stride is shorter than its row");
@@ -597,7 +603,7 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.header = batch->work, a.max_items = (int)g.max_items;
   a.G = g.G, a.out_rows = tokens;
   a.inv_G = g.G > 1 ? (unsigned)(((1ull << 32) + g.G - 1) / g.G) : 0;
-  a.scale_log2 = (softcap > 0.f ? 2.f * (scale / softcap) : scale) * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.cap_log2 = softcap * 1.4426950408889634f;
   a.slopes = d_slopes;
   a.vec = !((uintptr_t)d_q & 15) && !(ld_q & 7);

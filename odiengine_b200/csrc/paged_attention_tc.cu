@@ -595,8 +595,14 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
         const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)head * HD + c;
         if (a.out32) {
           float* y = static_cast<float*>(a.out) + at;
+          if (a.vec_out) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] = v[e];
+            for (int e = 0; e < 4; ++e)
+              reinterpret_cast<float4*>(y)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = v[e];
+          }
         } else {
           uint32_t w[8];
 #pragma unroll

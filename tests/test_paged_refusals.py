@@ -125,6 +125,13 @@ def test_attention_refusals():
     assert attend(T=0) == 0
 
 
+def test_caps_out_of_range_are_refused():
+    # scale / softcap past fp32, scale * log2(e) past fp32, a cap whose rounding the scores would show
+    for kw in (dict(cap=1e-39), dict(cap=1e-30, scale=1e10), dict(scale=3e38), dict(cap=1024.5)):
+        refused(attend(**kw))
+    assert attend(T=0, cap=1024.0) == 0
+
+
 def test_verify_refusals():
     n = ob.lib().odi_cuda_verify_scratch_bytes(5, 2, 100)
 
