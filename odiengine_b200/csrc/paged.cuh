@@ -24,9 +24,10 @@ struct PagedView {
 
 // How attention cuts a batch's rows: an item is up to `rows` of the new tokens *
 // G rows of one request (row r: token r / G, head r % G of each kv head's
-// group), over tiles of `tile` positions.
+// group), over tiles of `tile` positions.  `extra`: what beginning and ending an item
+// costs, in tiles.
 struct PagedGeometry {
-  int G, rows, tile;
+  int G, rows, tile, extra;
   int64_t max_items;
 };
 
@@ -36,7 +37,7 @@ struct alignas(16) PagedItem {
   int b, i;              // request, item within the request
   int start, past, len;  // its first row; positions before its new ones; all of them
   int prefix;
-  int tile0, tiles;      // tiles of the items before; its own
+  int tile0, tiles;      // tiles, and extra ones, of the items before; its own tiles
 };
 static_assert(sizeof(PagedItem) == 32, "two 16-byte loads");
 // PW_ITEMS of them.
@@ -53,9 +54,15 @@ inline bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 1
 inline int page_shift_of(int p) { return p == 16 ? 4 : p == 32 ? 5 : p == 64 ? 6 : 7; }
 // Rows of an item and positions of a tile, by the most rows a request has per kv
 // head: the two widths of the mma.sync kernel, and the two of the tcgen05 kernel.
-inline void paged_kind(int64_t most, int* rows, int* tile) {
+// What an item costs beside its tiles, measured as tiles.  tcgen05: 2048 tokens of
+// 64/8 heads alone 93 us with 4, 134 with 0 (a run of short items was 14 of them),
+// 105 with 2, 93 with 5; seven prompts of 32/32 heads of 64 dims 91, 87, 88, 91.
+// mma.sync: 256 requests of one token over 10 to 600 positions 72.5 us with 2, 75.5
+// with 0, 71.5 with 4; 16 requests of 2 to 5 tokens 58.5, 58.5, 60.5.
+inline void paged_kind(int64_t most, int* rows, int* tile, int* extra) {
   *rows = most <= 16 ? 16 : most <= 32 ? 32 : most <= 128 ? 128 : 256;
   *tile = 64;
+  *extra = *rows <= 32 ? 2 : 4;
 }
 
 // Positions of the batch that row r of request b sees: those below the result.

@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     while (ok && run.x < run.end) {
       const PagedPiece p = run_piece(a, run, ROWS);
       const int len = p.it.len;
+      if (p.t1 <= p.t0) break;
       PagedNames names(a, p, TILE, false);
       if (k >= 2 && !wait(&d_empty[k & 1], k / 2 - 1)) break;
       if (lane == 0) {
@@ -601,6 +602,7 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.q = d_q, a.ld_q = ld_q, a.out = d_out, a.ld_out = ld_out, a.out32 = out32;
   a.table = tables->table, a.max_pages = tables->max_pages;
   a.header = batch->work, a.max_items = (int)g.max_items;
+  a.extra = g.extra;
   a.G = g.G, a.out_rows = tokens;
   a.inv_G = g.G > 1 ? (unsigned)(((1ull << 32) + g.G - 1) / g.G) : 0;
   a.scale_log2 = scale_log2;

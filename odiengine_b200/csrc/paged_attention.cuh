@@ -4,7 +4,8 @@
 // The work of a call is the tiles of all (kv head, item) units in a row:
 // kv_heads times the batch's list of items.  CTA c takes the share-long run of
 // them from c * share on, whatever units it cuts, so that every CTA has the same
-// number of tiles however the requests' lengths lie.  A unit inside one run is
+// number of tiles however the requests' lengths lie; an item counts for some more than
+// it has, for what its beginning and its end cost.  A unit inside one run is
 // finished there; the pieces of one that is cut go to the scratch, and the last
 // CTA to arrive joins them in the order of the positions.  Which pieces there are
 // depends on the lengths alone, so repeats are bit-identical.
@@ -40,6 +41,7 @@ struct PagedAttnArgs {
   int vec, vec_out;  // q, out and their strides allow 16-byte accesses
   int q_boxes;       // Q comes by TMA
   int least;         // tiles per CTA at least
+  int extra;         // tiles that an item counts beside its own
   float* part;       // [2 * CTAs][rows][HD + 2]
   int* count;        // arrivals per unit, zero between launches
   int* err;
@@ -114,7 +116,6 @@ struct PagedPiece {
   int kvh, unit;
   int t0, t1;    // this CTA's tiles of the unit
   int c0, c1;    // the first and last CTA that have tiles of it
-  int first_place;  // CTA c0's place for its piece
   int rows;      // of the item, that there are rows of q for
   int least;     // positions below it are seen by every row of the item
   int poison;    // V has values that are not finite where not every row looks
@@ -158,7 +159,7 @@ __device__ __forceinline__ bool run_begin(const PagedAttnArgs& a, PagedRun& r, P
   r.kvh = (int)pa_div(r.x, r.tiles);
   const int rem = (int)(r.x - (int64_t)r.kvh * r.tiles);
   while (i < r.items) {
-    if (x.tile0 <= rem && rem < x.tile0 + x.tiles) found->it = x, found->item = i;
+    if (x.tile0 <= rem && rem < x.tile0 + x.tiles + a.extra) found->it = x, found->item = i;
     i += blockDim.x;
     if (i < r.items) x = load_item(list + i);
   }
@@ -166,21 +167,22 @@ __device__ __forceinline__ bool run_begin(const PagedAttnArgs& a, PagedRun& r, P
   r.it = found->it, r.item = found->item;
   return true;
 }
-// The piece at x, and x moved past it.
+// The piece at x, and x moved past it.  An item's extra tiles come before its own; a
+// run that ends among them has no piece of it (t1 <= t0), and no piece after it.
 __device__ __forceinline__ PagedPiece run_piece(const PagedAttnArgs& a, PagedRun& r, int rows_per_item) {
   PagedPiece p;
   p.it = r.it;
   p.kvh = r.kvh, p.unit = r.kvh * r.items + r.item;
-  p.t0 = (int)(r.x - (int64_t)r.kvh * r.tiles) - r.it.tile0;
-  p.t1 = (int)min((int64_t)r.it.tiles, p.t0 + (r.end - r.x));
+  const int64_t ux = (int64_t)r.kvh * r.tiles + r.it.tile0 + a.extra;  // the unit's first tile
+  const int64_t next = min(r.end, ux + r.it.tiles);
+  p.t0 = (int)max((int64_t)0, r.x - ux);
+  p.t1 = (int)(next - ux);
   p.rows = min(rows_per_item, min(r.it.len - r.it.past, a.out_rows - r.it.start) * a.G - r.it.i * rows_per_item);
   p.least = paged_limit(r.it.past, pa_token(a, r.it.i * rows_per_item), r.it.len, r.it.prefix);
   p.poison = p.last = 0;
-  const int64_t ux = (int64_t)r.kvh * r.tiles + r.it.tile0;  // the unit's first tile
   p.c0 = p.c1 = blockIdx.x;
   if (p.t0 || p.t1 < r.it.tiles) p.c0 = (int)pa_div(ux, r.share), p.c1 = (int)pa_div(ux + r.it.tiles - 1, r.share);
-  p.first_place = r.share * p.c0 <= ux ? 1 : 0;
-  r.x += max(1, p.t1 - p.t0);
+  r.x = max(r.x + 1, next);
   return p;
 }
 __device__ __forceinline__ void run_next(const PagedAttnArgs& a, PagedRun& r) {
@@ -214,7 +216,7 @@ struct PagedNames {
 // Where CTA c's piece of the unit is.  A CTA has two places: one for the piece that
 // goes on with a unit, one for the piece that begins one, which only c0's can be.
 __device__ __forceinline__ float* piece_part(const PagedAttnArgs& a, const PagedPiece& p, int cta, int stride) {
-  return a.part + (int64_t)(2 * cta + (cta == p.c0 ? p.first_place : 0)) * stride;
+  return a.part + (int64_t)(2 * cta + (cta == p.c0)) * stride;
 }
 
 // Devices whose kernel may take its shared memory; set again by whoever comes twice

@@ -48,7 +48,8 @@ struct Cfg {
   static constexpr int ST = (HD == 128 ? 4 : NH == 1 ? 8 : 6) * NH;
   static_assert(ST / 2 < 8, "v_clean");
   static constexpr int Q_OFF = ST * SLOT;
-  static constexpr int SMEM = Q_OFF + NH * Q_HALF + 1024;  // + alignment slack
+  static constexpr int STAGE_OFF = Q_OFF + NH * Q_HALF, STAGE = HD == 128 ? 32 * 64 : 0;  // of a warp: 64 bytes of 32 rows of the output
+  static constexpr int SMEM = STAGE_OFF + 4 * NH * STAGE + 1024;           // + alignment slack
   static constexpr int ROWS = NH * HALF_ROWS, THREADS = NH * 128 + 128, PER_SM = 2 / NH;
   static_assert(PER_SM * (SMEM + 2048) <= 228 * 1024, "shared memory, with 1 KB static and 1 KB of the system's");
   // the launch's registers are shared out anew: a softmax thread holds a tile's scores
@@ -246,6 +247,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
       const PagedPiece p = run_piece(a, run, ROWS);
       const int len = p.it.len;
       const bool down = downward(p);
+      if (p.t1 <= p.t0) break;
       PagedNames names(a, p, TILE, down);
       if (k >= 2 && !wait(&bars.d_empty[k & 1], k / 2 - 1)) break;
       if (lane == 0) {
@@ -591,7 +593,31 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
       const bool whole = t0 == 0 && t1 == p.it.tiles, fix = p.poison != 0;
       constexpr int STRIDE = ROWS * (HD + 2);
       float* part = piece_part(a, p, blockIdx.x, STRIDE);
-      auto store = [&](const float (&v)[16], int c) {  // 16 values of the row from dim c on
+      // 16 values of the thread's row from dim c on.  A thread's row is far from its
+      // neighbours', so rows go through shared memory, 64 bytes at a time, and four lanes
+      // write them to a row.
+      const int out_row = row < rows ? 1 : 0;
+      int64_t out_at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)head * HD;
+      uint8_t* stage = smem + F::STAGE_OFF + warp * F::STAGE;
+      auto chunk = [&](int r, int ch) { return reinterpret_cast<uint4*>(stage + r * 64 + ((ch ^ (r >> 1 & 3)) << 4)); };
+      auto flush = [&](int c) {  // the staged values are those from dim c on
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = j * 8 + (lane >> 2), ch = lane & 3;
+          const int64_t at = __shfl_sync(0xffffffffu, out_at, r) + c;
+          const bool some = __shfl_sync(0xffffffffu, out_row, r);
+          const uint4 x = *chunk(r, ch);
+          uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (at << (a.out32 ? 2 : 1))) + ch * 4;
+          if (!some) continue;
+          if (a.vec_out) *reinterpret_cast<uint4*>(y) = x;
+          else y[0] = x.x, y[1] = x.y, y[2] = x.z, y[3] = x.w;
+        }
+        __syncwarp();
+      };
+      auto store = [&](const float (&v)[16], int c) {
+        if constexpr (F::STAGE == 0) {
+          if (row >= rows) return;
         const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)head * HD + c;
         if (a.out32) {
           float* y = static_cast<float*>(a.out) + at;
@@ -616,6 +642,21 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = w[e];
           }
+        }
+          return;
+        }
+        if (a.out32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *chunk(lane, e) = make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]),
+                                         __float_as_uint(v[4 * e + 3]));
+          flush(c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *chunk(lane, (c >> 3 & 2) + e) = make_uint4(H::pack(v[8 * e], v[8 * e + 1]), H::pack(v[8 * e + 2], v[8 * e + 3]),
+                                                        H::pack(v[8 * e + 4], v[8 * e + 5]), H::pack(v[8 * e + 6], v[8 * e + 7]));
+          if (c & 16) flush(c - 16);
         }
       };
       if (mine) {
@@ -642,7 +683,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] *= inv;
-            if (row < rows) store(v, c);
+            store(v, c);
           } else {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
@@ -701,7 +742,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
               float y[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) y[e] = v[g + e] * inv;
-              if (row < rows) store(y, d0 + g);
+              store(y, d0 + g);
             }
           }
           if (tid == 0) a.count[p.unit] = 0;

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(THREADS) paged_step_kernel(const __grid_consta
         x.tiles = (paged_limit(x.past, token, x.len, x.prefix) + a.g.tile - 1) / a.g.tile;
       }
       Sum2 total;
-      const Sum2 e = block_scan<WARPS>({x.tiles, 0}, &total, tiles_of[i0 / THREADS & 1]);
+      const Sum2 e = block_scan<WARPS>({i < items ? x.tiles + a.g.extra : 0, 0}, &total, tiles_of[i0 / THREADS & 1]);
       x.tile0 = base.a + e.a;
       if (i < items) list[i] = x;
       base.a += total.a;
@@ -285,7 +285,7 @@ bool paged_geometry(int requests, int max_rows, int max_new, int heads, int kv_h
     return false;
   g->G = heads / kv_heads;
   const int64_t most = (int64_t)max_new * g->G;
-  paged_kind(most, &g->rows, &g->tile);
+  paged_kind(most, &g->rows, &g->tile, &g->extra);
   const int64_t by_request = requests * ((most + g->rows - 1) / g->rows),
                 by_rows = requests + (int64_t)max_rows * g->G / g->rows;
   g->max_items = by_request < by_rows ? by_request : by_rows;
@@ -333,7 +333,7 @@ int odi_cuda_paged_step(const odi_cuda_page_tables* t, const odi_cuda_paged_batc
       (int64_t)t->num_pages * t->page_size > 0x7fffffffll || (int64_t)t->requests * t->max_pages > (1 << 30) ||
       (int64_t)t->max_pages * t->page_size > 0x7fffffffll)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: page_size, max_pages or num_pages out of range");
-  if (a.g.max_items * ((int64_t)t->max_pages * t->page_size / a.g.tile + 1) > 0x7fffffffll)
+  if (a.g.max_items * ((int64_t)t->max_pages * t->page_size / a.g.tile + 1 + a.g.extra) > 0x7fffffffll)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: more work than 2^31 tiles");
   a.t = *t, a.b = *batch, a.keep = d_keep, a.fresh = d_new, a.prefix = d_prefix, a.page_shift = page_shift_of(t->page_size);
   // one CTA where its threads see to everything in a few passes; else eight
