@@ -68,6 +68,8 @@ struct Cfg {
   static_assert(128 * REGS_FEW + 128 * MG * REGS_MMA <= THREADS * REGS_LAUNCH, "register split");
   static_assert(PER_SM * (SMEM + 2048) <= 228 * 1024, "shared memory, with 1 KB static and 1 KB of the system's");
 };
+// pieces that the producer may be ahead: those before the one at the products are with the joiners
+constexpr int ND = 3;
 constexpr int JOINERS = 96;  // threads that join and write out
 
 template <typename T, int HD, int MG, bool FANCY>
@@ -78,8 +80,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   using H = Half16<T>;
   constexpr int KS = HD / 16, ROWS = 16 * MG, ST = F::ST, PLANES = HD / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t full[ST], empty[ST], d_full[2], d_empty[2], fold_full, fold_empty, jbar;
-  __shared__ PagedPiece pieces[2];
+  __shared__ uint64_t full[ST], empty[ST], d_full[ND], d_empty[ND], fold_full, fold_empty, jbar;
+  __shared__ PagedPiece pieces[ND];
   __shared__ float2 wml[4 * MG][16];
   __shared__ PagedFound found;
   __shared__ int is_last;
@@ -88,7 +90,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   pdl_launch_dependents();
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 4 * MG);
-    for (int i = 0; i < 2; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4 * MG + 3);
+    for (int i = 0; i < ND; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 4 * MG + 3);
     mbar_init(&fold_full, 4 * MG);
     mbar_init(&fold_empty, 3);
     mbar_init(&jbar, JOINERS);
@@ -120,10 +122,10 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       const int len = p.it.len;
       if (p.t1 <= p.t0) break;
       PagedNames names(a, p, TILE, false);
-      if (k >= 2 && !wait(&d_empty[k & 1], k / 2 - 1)) break;
+      if (k >= ND && !wait(&d_empty[k % ND], k / ND - 1)) break;
       if (lane == 0) {
-        pieces[k & 1] = p;
-        mbar_arrive(&d_full[k & 1]);
+        pieces[k % ND] = p;
+        mbar_arrive(&d_full[k % ND]);
       }
       ++k;
       if (run.x < run.end) run_next(a, run);
@@ -148,9 +150,9 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         }
       }
     }
-    if (ok && (k < 2 || wait(&d_empty[k & 1], k / 2 - 1)) && lane == 0) {
-      pieces[k & 1].last = 1;
-      mbar_arrive(&d_full[k & 1]);
+    if (ok && (k < ND || wait(&d_empty[k % ND], k / ND - 1)) && lane == 0) {
+      pieces[k % ND].last = 1;
+      mbar_arrive(&d_full[k % ND]);
     }
     for (int i = max(0, n - ST); i < n; ++i) wait(&full[i % ST], i / ST);  // no copy outlives the CTA
     return;
@@ -166,8 +168,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     return wait(&jbar, syncs++);
   };
   for (int k = 0;; ++k) {
-    if (!wait(&d_full[k & 1], k / 2)) return;
-    const PagedPiece& p = pieces[k & 1];
+    if (!wait(&d_full[k % ND], k / ND)) return;
+    const PagedPiece& p = pieces[k % ND];
     if (p.last) return;
     const int t0 = p.t0, t1 = p.t1, rows = p.rows, least = p.least, len = p.it.len;
     const bool whole = t0 == 0 && t1 == p.it.tiles;
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&d_empty[k & 1]);
+    if (lane == 0) mbar_arrive(&d_empty[k % ND]);
   }
   }
 
@@ -300,8 +302,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   float* fold = reinterpret_cast<float*>(smem + F::FOLD_OFF + mg * F::FOLD);
   int n = 0;
   for (int k = 0;; ++k) {
-    if (!wait(&d_full[k & 1], k / 2)) return;
-    PagedPiece& p = pieces[k & 1];
+    if (!wait(&d_full[k % ND], k / ND)) return;
+    PagedPiece& p = pieces[k % ND];
     if (p.last) return;
     const int t0 = p.t0, t1 = p.t1, rows = p.rows - mg * 16, least = p.least, len = p.it.len, past = p.it.past;
     const int R0 = p.it.i * ROWS + mg * 16;  // the group's first row of the request
@@ -424,19 +426,26 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
             // What not every row sees must not reach the rows that do not: 0 * NaN is
             // NaN.  Values that are not finite leave here; rows that see them get them
             // when the piece ends.
+            uint32_t zero = 0;  // 0 times all values: 0 if every one is finite
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
+              for (int i = 0; i < 4; ++i) zero = H::times0(b[dt][i], zero);
+            if (__any_sync(0xffffffffu, zero & 0x7fff7fffu)) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int j = j0 + (i & 1) * 8 + e;
-                  const uint32_t ex = H::EXP << (16 * e);
-                  if (j >= least && (b[dt][i] & ex) == ex) {
-                    b[dt][i] &= ~(0xffffu << (16 * e));
-                    bad = bad || j < len;
+              for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const int j = j0 + (i & 1) * 8 + e;
+                    const uint32_t ex = H::EXP << (16 * e);
+                    if (j >= least && (b[dt][i] & ex) == ex) {
+                      b[dt][i] &= ~(0xffffu << (16 * e));
+                      bad = bad || j < len;
+                    }
                   }
-                }
+            }
           }
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt) {
@@ -467,7 +476,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       if (bad) p.poison = 1;
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&fold_full), mbar_arrive(&d_empty[k & 1]);
+    if (lane == 0) mbar_arrive(&fold_full), mbar_arrive(&d_empty[k % ND]);
   }
 }
 
