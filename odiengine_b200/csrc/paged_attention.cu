@@ -64,7 +64,7 @@ struct Cfg {
   static constexpr int THREADS = 128 * MG + 128, PER_SM = MG == 1 ? 2 : 1;
   // the launch's registers are shared out anew: a warp at the products holds O (64),
   // Q (32) and operands
-  static constexpr int REGS_LAUNCH = MG == 1 ? 128 : 168, REGS_FEW = 80, REGS_MMA = MG == 1 ? 176 : 208;
+  static constexpr int REGS_LAUNCH = MG == 1 ? 128 : 168, REGS_FEW = 104, REGS_MMA = MG == 1 ? 152 : 200;
   static_assert(128 * REGS_FEW + 128 * MG * REGS_MMA <= THREADS * REGS_LAUNCH, "register split");
   static_assert(PER_SM * (SMEM + 2048) <= 228 * 1024, "shared memory, with 1 KB static and 1 KB of the system's");
 };
@@ -244,48 +244,67 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       }
       if (!sync()) return;
       if (is_last) {
-        // three places of the unit by two pieces at a time, so that loads overlap
+        // Three places of the unit by four pieces at a time, so that loads overlap; a
+        // lane has the factor of one piece for its row, whose LANES lanes share theirs.
+        constexpr int LANES = HD / 4;
 #pragma unroll 1
-        for (int i0 = jt; i0 < rows * (HD / 4); i0 += 3 * JOINERS) {
+        for (int i0 = jt & ~31; i0 < rows * LANES; i0 += 3 * JOINERS) {
           float top[3], L[3];
           float4 v[3];
           int at[3];
 #pragma unroll
           for (int u = 0; u < 3; ++u) {
             top[u] = -INFINITY, L[u] = 0.f, v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            at[u] = min(i0 + u * JOINERS, rows * (HD / 4) - 1);
+            at[u] = min(i0 + lane + u * JOINERS, rows * LANES - 1);
           }
 #pragma unroll 1
-          for (int q0 = c0; q0 <= c1; q0 += 2) {
-            float2 ml[3][2];
-            float4 x[3][2];
+          for (int q0 = c0; q0 <= c1; q0 += LANES) {
+            const int q = q0 + lane % LANES, some = min(LANES, c1 - q0 + 1);
+            float2 ml[3];
+            float f[3];
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const float* src = piece_part(a, p, min(q0 + w, c1), STRIDE);
-#pragma unroll
-              for (int u = 0; u < 3; ++u) {
-                ml[u][w] = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * (at[u] / (HD / 4))));
-                x[u][w] = __ldcg(reinterpret_cast<const float4*>(src) + at[u]);
-              }
+            for (int u = 0; u < 3; ++u) {
+              ml[u] = make_float2(-INFINITY, 0.f);
+              if (q <= c1) ml[u] = __ldcg(reinterpret_cast<const float2*>(piece_part(a, p, q, STRIDE) + ROWS * HD + 2 * (at[u] / LANES)));
             }
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              if (q0 + w > c1) break;
+            for (int u = 0; u < 3; ++u) {
+              float now = fmaxf(top[u], ml[u].x);
 #pragma unroll
-              for (int u = 0; u < 3; ++u) {
-                const float now = fmaxf(top[u], ml[u][w].x);
-                const float fo = top[u] == now ? 1.f : pa_ex2(top[u] - now), fn = ml[u][w].x == now ? 1.f : pa_ex2(ml[u][w].x - now);
-                top[u] = now;
-                L[u] = L[u] * fo + ml[u][w].y * fn;
-                v[u].x = v[u].x * fo + x[u][w].x * fn, v[u].y = v[u].y * fo + x[u][w].y * fn;
-                v[u].z = v[u].z * fo + x[u][w].z * fn, v[u].w = v[u].w * fo + x[u][w].w * fn;
+              for (int o = LANES / 2; o; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+              const float fo = top[u] == now ? 1.f : pa_ex2(top[u] - now);
+              f[u] = ml[u].x == now ? 1.f : pa_ex2(ml[u].x - now);
+              float l = ml[u].y * f[u];
+#pragma unroll
+              for (int o = LANES / 2; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+              top[u] = now, L[u] = fmaf(L[u], fo, l);
+              v[u].x *= fo, v[u].y *= fo, v[u].z *= fo, v[u].w *= fo;
+            }
+#pragma unroll 1
+            for (int w0 = 0; w0 < some; w0 += 4) {
+              float4 x[3][4];
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const float4* src = reinterpret_cast<const float4*>(piece_part(a, p, q0 + min(w0 + w, some - 1), STRIDE));
+#pragma unroll
+                for (int u = 0; u < 3; ++u) x[u][w] = __ldcg(src + at[u]);
+              }
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                if (w0 + w >= some) break;
+#pragma unroll
+                for (int u = 0; u < 3; ++u) {
+                  const float g = __shfl_sync(0xffffffffu, f[u], (lane & ~(LANES - 1)) | (w0 + w));
+                  v[u].x = fmaf(x[u][w].x, g, v[u].x), v[u].y = fmaf(x[u][w].y, g, v[u].y);
+                  v[u].z = fmaf(x[u][w].z, g, v[u].z), v[u].w = fmaf(x[u][w].w, g, v[u].w);
+                }
               }
             }
           }
 #pragma unroll
           for (int u = 0; u < 3; ++u)
-            if (i0 + u * JOINERS < rows * (HD / 4))
-              store(at[u] / (HD / 4), at[u] % (HD / 4) * 4, v[u], L[u] == 0.f ? 0.f : 1.f / L[u]);
+            if (i0 + lane + u * JOINERS < rows * LANES)
+              store(at[u] / LANES, at[u] % LANES * 4, v[u], L[u] == 0.f ? 0.f : 1.f / L[u]);
         }
         if (jt == 0) a.count[p.unit] = 0;
       }
