@@ -234,16 +234,16 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     __syncwarp();
     if (lane == 0) mbar_arrive(&fold_empty);
     if (!whole) {
-      // the last piece to arrive joins them all
-      const int c0 = p.c0, c1 = p.c1;
-      if (!sync()) return;
-      if (jt == 0) {
-        __threadfence();
-        is_last = atomicAdd(a.count + p.unit, 1) == c1 - c0;
-        __threadfence();
-      }
-      if (!sync()) return;
-      if (is_last) {
+      // the last piece to arrive joins them
+      for (PagedJoin join = join_first(a, p, 16);; join = join_next(a, p)) {
+        if (!sync()) return;
+        if (jt == 0) {
+          __threadfence();
+          is_last = atomicAdd(join.counter, 1) == join.n - 1;
+          __threadfence();
+        }
+        if (!sync()) return;
+        if (!is_last) break;
         // Three places of the unit by four pieces at a time, so that loads overlap; a
         // lane has the factor of one piece for its row, whose LANES lanes share theirs.
         constexpr int LANES = HD / 4;
@@ -258,14 +258,16 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
             at[u] = min(i0 + lane + u * JOINERS, rows * LANES - 1);
           }
 #pragma unroll 1
-          for (int q0 = c0; q0 <= c1; q0 += LANES) {
-            const int q = q0 + lane % LANES, some = min(LANES, c1 - q0 + 1);
+          for (int q0 = 0; q0 < join.n; q0 += LANES) {
+            const int q = q0 + lane % LANES, some = min(LANES, join.n - q0);
             float2 ml[3];
             float f[3];
 #pragma unroll
             for (int u = 0; u < 3; ++u) {
               ml[u] = make_float2(-INFINITY, 0.f);
-              if (q <= c1) ml[u] = __ldcg(reinterpret_cast<const float2*>(piece_part(a, p, q, STRIDE) + ROWS * HD + 2 * (at[u] / LANES)));
+              if (q < join.n)
+                ml[u] = __ldcg(reinterpret_cast<const float2*>(piece_part(a, p, join.first + q * join.step, STRIDE) + ROWS * HD +
+                                                               2 * (at[u] / LANES)));
             }
 #pragma unroll
             for (int u = 0; u < 3; ++u) {
@@ -285,7 +287,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
               float4 x[3][4];
 #pragma unroll
               for (int w = 0; w < 4; ++w) {
-                const float4* src = reinterpret_cast<const float4*>(piece_part(a, p, q0 + min(w0 + w, some - 1), STRIDE));
+                const float4* src = reinterpret_cast<const float4*>(
+                    piece_part(a, p, join.first + (q0 + min(w0 + w, some - 1)) * join.step, STRIDE));
 #pragma unroll
                 for (int u = 0; u < 3; ++u) x[u][w] = __ldcg(src + at[u]);
               }
@@ -302,11 +305,20 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
             }
           }
 #pragma unroll
-          for (int u = 0; u < 3; ++u)
-            if (i0 + lane + u * JOINERS < rows * LANES)
-              store(at[u] / LANES, at[u] % LANES * 4, v[u], L[u] == 0.f ? 0.f : 1.f / L[u]);
+          for (int u = 0; u < 3; ++u) {
+            if (i0 + lane + u * JOINERS >= rows * LANES) break;
+            const int r = at[u] / LANES, d = at[u] % LANES * 4;
+            if (join.final) {
+              store(r, d, v[u], L[u] == 0.f ? 0.f : 1.f / L[u]);
+            } else {  // in its first piece's place: this warp's lanes alone read that row of it
+              float* to = piece_part(a, p, join.first, STRIDE);
+              *reinterpret_cast<float4*>(to + r * HD + d) = v[u];
+              if (d == 0) *reinterpret_cast<float2*>(to + ROWS * HD + 2 * r) = make_float2(top[u], L[u]);
+            }
+          }
         }
-        if (jt == 0) a.count[p.unit] = 0;
+        if (jt == 0) *join.counter = 0;
+        if (join.final) break;
       }
     }
     __syncwarp();
@@ -578,9 +590,11 @@ using namespace odi_cuda;
 
 extern "C" {
 
-// Error word, pieces, then a counter per unit.  The pieces' place has one size,
-// so that a scratch serves any batch whose counters fit.
-constexpr size_t PART_OFF = 256, COUNT_OFF = PART_OFF + (size_t)2 * PAGED_SMS * PAGED_ROWS_MAX * (128 + 2) * 4;
+// Error word, pieces, counters of groups of pieces, then a counter per unit.  The
+// pieces' place has one size, so that a scratch serves any batch whose counters fit.
+constexpr size_t PART_OFF = 256, GROUP_OFF = PART_OFF + (size_t)2 * PAGED_SMS * PAGED_ROWS_MAX * (128 + 2) * 4,
+                 COUNT_OFF = GROUP_OFF + 2 * paged_ctas(16) * 4;
+static_assert(paged_ctas(16) >= paged_ctas(128) && paged_ctas(16) >= paged_ctas(PAGED_ROWS_MAX), "counters of groups");
 static_assert(paged_ctas(16) * 16 <= PAGED_SMS * PAGED_ROWS_MAX && paged_ctas(128) * 128 <= PAGED_SMS * PAGED_ROWS_MAX, "pieces of narrow items");
 
 size_t odi_cuda_attention_paged_scratch_bytes(int requests, int max_rows, int max_new, int heads, int kv_heads, int head_dim) {
@@ -643,6 +657,7 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.least = 3;
   a.err = static_cast<int*>(d_scratch);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + PART_OFF);
+  a.group = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + GROUP_OFF);
   a.count = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + COUNT_OFF);
   const bool fancy = softcap > 0.f || d_slopes;
   cudaStream_t s = (cudaStream_t)stream;

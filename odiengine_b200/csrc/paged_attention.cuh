@@ -7,8 +7,9 @@
 // number of tiles however the requests' lengths lie; an item counts for some more than
 // it has, for what its beginning and its end cost.  A unit inside one run is
 // finished there; the pieces of one that is cut go to the scratch, and the last
-// CTA to arrive joins them in the order of the positions.  Which pieces there are
-// depends on the lengths alone, so repeats are bit-identical.
+// CTA to arrive joins them in the order of the positions; many pieces first in groups,
+// so that no CTA joins more than a few.  Which pieces there are depends on the lengths
+// alone, so repeats are bit-identical.
 #pragma once
 
 #include <cuda.h>
@@ -44,6 +45,7 @@ struct PagedAttnArgs {
   int extra;         // tiles that an item counts beside its own
   float* part;       // [2 * CTAs][rows][HD + 2]
   int* count;        // arrivals per unit, zero between launches
+  int* group;        // arrivals per group of pieces, by its first piece's place
   int* err;
 };
 
@@ -217,6 +219,27 @@ struct PagedNames {
 // goes on with a unit, one for the piece that begins one, which only c0's can be.
 __device__ __forceinline__ float* piece_part(const PagedAttnArgs& a, const PagedPiece& p, int cta, int stride) {
   return a.part + (int64_t)(2 * cta + (cta == p.c0)) * stride;
+}
+
+// How a unit's pieces are joined: `n` of them from CTA `first` on, `step` apart, who
+// arrive at `counter`; when they are one, the unit is done or its groups are next.
+struct PagedJoin {
+  int first, step, n;
+  int* counter;
+  bool final;
+};
+// Up to `at_once` pieces are joined at once, more of them in groups of about the root
+// of their number: 38 pieces of one token of 64/8 heads over 30,000 positions take 36 us
+// so, 41 at once; of 16 tokens 55 and 85.
+__device__ __forceinline__ PagedJoin join_first(const PagedAttnArgs& a, const PagedPiece& p, int at_once) {
+  const int n = p.c1 - p.c0 + 1;
+  if (n <= at_once) return {p.c0, 1, n, a.count + p.unit, true};
+  const int size = (int)ceilf(sqrtf((float)n)), first = p.c0 + ((int)blockIdx.x - p.c0) / size * size;
+  return {first, 1, min(size, p.c1 - first + 1), a.group + 2 * first + (first == p.c0), false};
+}
+__device__ __forceinline__ PagedJoin join_next(const PagedAttnArgs& a, const PagedPiece& p) {
+  const int n = p.c1 - p.c0 + 1, size = (int)ceilf(sqrtf((float)n));
+  return {p.c0, size, (n + size - 1) / size, a.count + p.unit, true};
 }
 
 // Devices whose kernel may take its shared memory; set again by whoever comes twice

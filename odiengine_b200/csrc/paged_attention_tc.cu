@@ -693,63 +693,72 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
         fence_before();
       }
       if (!whole) {
-        *reinterpret_cast<float2*>(part + ROWS * HD + 2 * row) = make_float2(ref, L);
-        const int c0 = p.c0, c1 = p.c1;
-        mbar_arrive(&bars.join);
-        ok = wait(&bars.join, joins++);
-        if (!ok) break;
-        if (tid == 0) {
-          __threadfence();
-          is_last = atomicAdd(a.count + p.unit, 1) == c1 - c0;
-          __threadfence();
-        }
-        mbar_arrive(&bars.join);
-        ok = wait(&bars.join, joins++);
-        if (!ok) break;
-        if (is_last) {
-          auto piece = [&](int c) { return piece_part(a, p, c, STRIDE); };
-          float top = -INFINITY, all = 0.f;
+        const bool warp_rows = (row & ~31) < rows;
+        if (warp_rows) *reinterpret_cast<float2*>(part + ROWS * HD + 2 * row) = make_float2(ref, L);
+        for (PagedJoin join = join_first(a, p, 8);; join = join_next(a, p)) {
+          mbar_arrive(&bars.join);
+          ok = wait(&bars.join, joins++);
+          if (!ok) break;
+          if (tid == 0) {
+            __threadfence();
+            is_last = atomicAdd(join.counter, 1) == join.n - 1;
+            __threadfence();
+          }
+          mbar_arrive(&bars.join);
+          ok = wait(&bars.join, joins++);
+          if (!ok || !is_last) break;
+          if (warp_rows) {
+            auto piece = [&](int q) { return piece_part(a, p, join.first + q * join.step, STRIDE); };
+            float* to = piece_part(a, p, join.first, STRIDE);
+            float top = -INFINITY, all = 0.f;
 #pragma unroll 4
-          for (int c = c0; c <= c1; ++c) top = max3(top, __ldcg(reinterpret_cast<const float2*>(piece(c) + ROWS * HD + 2 * row)).x, -INFINITY);
+            for (int q = 0; q < join.n; ++q) top = max3(top, __ldcg(reinterpret_cast<const float2*>(piece(q) + ROWS * HD + 2 * row)).x, -INFINITY);
 #pragma unroll 1
-          for (int d0 = 0; d0 < HD; d0 += 32) {
-            float v[32];
+            for (int d0 = 0; d0 < HD; d0 += 32) {
+              float v[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0.f;
-            all = 0.f;
+              for (int e = 0; e < 32; ++e) v[e] = 0.f;
+              all = 0.f;
 #pragma unroll 2
-            for (int c = c0; c <= c1; ++c) {
-              const float* src = piece(c);
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * row));
-              float4 x[8];
+              for (int q = 0; q < join.n; ++q) {
+                const float* src = piece(q);
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * HD + 2 * row));
+                float4 x[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(src + ((d0 / 4 + e) * ROWS + row) * 4));
-              // a piece in which the row saw nothing left no sums
-              const bool some = !(ml.x == -INFINITY && ml.y == 0.f);
-              const float f = ml.x == top ? 1.f : pa_ex2(ml.x - top);
-              if (some) {
-                all = fmaf(ml.y, f, all);
+                for (int e = 0; e < 8; ++e) x[e] = __ldcg(reinterpret_cast<const float4*>(src + ((d0 / 4 + e) * ROWS + row) * 4));
+                // a piece in which the row saw nothing left no sums
+                const bool some = !(ml.x == -INFINITY && ml.y == 0.f);
+                const float f = ml.x == top ? 1.f : pa_ex2(ml.x - top);
+                if (some) {
+                  all = fmaf(ml.y, f, all);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  v[4 * e] = fmaf(x[e].x, f, v[4 * e]), v[4 * e + 1] = fmaf(x[e].y, f, v[4 * e + 1]);
-                  v[4 * e + 2] = fmaf(x[e].z, f, v[4 * e + 2]), v[4 * e + 3] = fmaf(x[e].w, f, v[4 * e + 3]);
+                  for (int e = 0; e < 8; ++e) {
+                    v[4 * e] = fmaf(x[e].x, f, v[4 * e]), v[4 * e + 1] = fmaf(x[e].y, f, v[4 * e + 1]);
+                    v[4 * e + 2] = fmaf(x[e].z, f, v[4 * e + 2]), v[4 * e + 3] = fmaf(x[e].w, f, v[4 * e + 3]);
+                  }
                 }
               }
-            }
-            const float inv = all == 0.f ? 0.f : 1.f / all;
+              if (join.final) {
+                const float inv = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll
-            for (int g = 0; g < 32; g += 16) {
-              float y[16];
+                for (int g = 0; g < 32; g += 16) {
+                  float y[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] = v[g + e] * inv;
-              store(y, d0 + g);
+                  for (int e = 0; e < 16; ++e) y[e] = v[g + e] * inv;
+                  store(y, d0 + g);
+                }
+              } else {  // in its first piece's place, whose row no other thread reads
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  *reinterpret_cast<float4*>(to + ((d0 / 4 + e) * ROWS + row) * 4) =
+                      make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+              }
             }
+            if (!join.final) *reinterpret_cast<float2*>(to + ROWS * HD + 2 * row) = make_float2(top, all);
           }
-          if (tid == 0) a.count[p.unit] = 0;
+          if (tid == 0) *join.counter = 0;
+          if (join.final) break;
         }
-        // nobody sets is_last again before all have read it
-        mbar_arrive(&bars.join);
-        ok = wait(&bars.join, joins++);
         if (!ok) break;
       }
       n += 2 * (t1 - t0), c_clean += clean;

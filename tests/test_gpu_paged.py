@@ -246,6 +246,32 @@ def test_attention_of_rows_that_are_not_aligned(cuda_lib, new, heads, shift, pad
     assert (out[:, :shift] == 5).all() and (out[:, shift + w:] == 5).all()
 
 
+@pytest.mark.parametrize("new,heads,kv", [(1, 3, 3), (2, 8, 1), (3, 8, 1), (9, 10, 1), (40, 8, 1), (1, 1, 1)])
+@pytest.mark.parametrize("hd,dtype", [(64, "bf16"), (128, "f16")])
+@pytest.mark.parametrize("past", [3300, 9000])
+def test_attention_of_many_pieces(cuda_lib, new, heads, kv, hd, dtype, past):
+    """One request whose few heads are cut into dozens of pieces, which join in
+    groups; a NaN that the last rows see, and calls that follow one another."""
+    from odiengine_b200 import paged
+
+    s = Setup([past], [new], heads, kv, hd, dtype, 64, seed=past + new)
+    slopes = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device="cuda") / heads)
+    scale = 1 / math.sqrt(hd)
+    for option in (None, slopes):
+        out = torch.empty((new, heads * hd), dtype=torch.float32, device="cuda")
+        paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=scale, slopes=option, scratch=s.scratch)
+        s.check(out, scale, 0.0, option)
+        again = torch.empty_like(out)
+        paged.attention_paged(s.q, s.cache, s.tables, s.batch, again, scale=scale, slopes=option, scratch=s.scratch)
+        assert torch.equal(out, again)
+    slot = int(s.batch.slots[new - 1])
+    s.cache.v[slot // 64, :, slot % 64, 5] = math.nan
+    paged.attention_paged(s.q, s.cache, s.tables, s.batch, again, scale=scale, slopes=slopes, scratch=s.scratch)
+    assert torch.equal(out[:-1], again[:-1])
+    assert again[-1].view(heads, hd)[:, 5].isnan().all() and again[-1].isnan().sum() == heads
+    assert cuda_lib_status(s.scratch) == 0 and not s.scratch[-4 * kv:].any()
+
+
 def cuda_lib_status(scratch):
     return int(scratch[:4].view(torch.int32).item())
 
