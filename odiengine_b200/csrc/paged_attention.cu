@@ -9,7 +9,15 @@
 // and HBM bounds the kernel.  A producer warp brings tiles of 64 positions, page
 // by page, into a ring by TMA; for each 16 rows there are four warps, which take
 // 16 positions of a tile each with softmax statistics of their own, so that no
-// barrier stands between tiles, and join when a piece ends.
+// barrier stands between tiles, and join when a piece ends: three more warps do that
+// beside the next piece.
+//
+// 64 requests of one token, 64/8 heads of 128 dims over 300 to 8,100 positions: 183 us,
+// 6.3 TB/s.  Where requests are short or few, latency is the bound: a tile takes a warp
+// about 1 us, an item some 2 us beside its tiles (its queries' way from memory, the
+// join); 512 such requests over up to 200 positions take 70 us, HBM would 32; one token
+// of 32 heads over 518 positions 9.6 us.  17 to 32 rows leave one CTA per SM: 16
+// requests of 2 to 5 tokens with a cap 58 us, 49 without, HBM 29.
 //
 // q . k and o are summed in fp32.  The weights enter the second product rounded
 // to the cache's type, relative to a reference that moves only when a weight
@@ -652,9 +660,11 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   a.slopes = d_slopes;
   a.vec = !((uintptr_t)d_q & 15) && !(ld_q & 7);
   a.vec_out = !((uintptr_t)d_out & 15) && !(ld_out & 7);
-  // a CTA takes three tiles at least: one token of 32 heads over 518 positions takes
-  // 11.2 us so, 12.9 with one tile and 15.0 with five
-  a.least = 3;
+  // Tiles that a CTA takes at least: fewer are more pieces to join.  mma.sync, one token
+  // of 32 heads over 100, 518 and 2000 positions: 5.5, 9.7 and 13.6 us with two, 7.8, 9.7
+  // and 13.5 with one, 5.4, 10.7 and 13.6 with four; tcgen05, 16 tokens of 64/8 heads over
+  // 500 and 2000: 16.5 and 22.2 us with four, 17.5 and 24.4 with two, 16.8 and 22.1 with five.
+  a.least = g.rows <= 32 ? 2 : 4;
   a.err = static_cast<int*>(d_scratch);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d_scratch) + PART_OFF);
   a.group = reinterpret_cast<int*>(static_cast<uint8_t*>(d_scratch) + GROUP_OFF);
