@@ -17,7 +17,7 @@
 // about 1 us, an item some 2 us beside its tiles (its queries' way from memory, the
 // join); 512 such requests over up to 200 positions take 70 us, HBM would 32; one token
 // of 32 heads over 518 positions 9.6 us.  17 to 32 rows leave one CTA per SM: 16
-// requests of 2 to 5 tokens with a cap 58 us, 49 without, HBM 29.
+// requests of 2 to 5 tokens with a cap 55 us, 49 without, HBM 29.
 //
 // q . k and o are summed in fp32.  The weights enter the second product rounded
 // to the cache's type, relative to a reference that moves only when a weight
@@ -64,7 +64,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 // MG: groups of 16 rows.  One group: two CTAs per SM; two: one.
 template <int HD, int MG>
 struct Cfg {
-  static constexpr int PLANE = TILE * 128, SLOT = HD / 64 * PLANE;  // K or V of one tile
+  static constexpr int SLOT = TILE * HD * 2;  // K or V of one tile
   static constexpr int ST = (HD == 128 ? 5 : 10) * MG;
   static constexpr int FOLD = 4 * 16 * HD * 4;  // a group's sums
   static constexpr int FOLD_OFF = ST * SLOT;
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
                      const __grid_constant__ CUtensorMap vmap) {
   using F = Cfg<HD, MG>;
   using H = Half16<T>;
-  constexpr int KS = HD / 16, ROWS = 16 * MG, ST = F::ST, PLANES = HD / 64;
+  constexpr int KS = HD / 16, ROWS = 16 * MG, ST = F::ST;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[ST], empty[ST], d_full[ND], d_empty[ND], fold_full, fold_empty, jbar;
   __shared__ PagedPiece pieces[ND];
@@ -113,15 +113,14 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   }
   PagedRun run;
   if (!run_begin(a, run, &found)) return;
-  const int P = a.c.page_size;
+  const int P = a.c.page_size, BR = min(P, TILE);  // BR rows to a box, its planes of 64 dims one after the other
   auto wait = [&](uint64_t* bar, int phase) { return mbar_wait(bar, phase & 1, a.err, ERR_PAGED_WAIT); };
 
   if (warp >= 4 * MG) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REGS_FEW));
   if (warp == 4 * MG) {
-    // ---- producer: a lane brings one box of K or V, one 64-dim half of it
-    const int BR = min(P, TILE), boxes = TILE / BR;
-    const int box = lane / PLANES, plane = lane % PLANES;
+    // ---- producer: a lane brings one box of K or V
+    const int boxes = TILE / BR, box = lane;
     const int rows_all = a.c.num_pages * a.c.kv_heads * P;
     int n = 0, k = 0;
     bool ok = true;
@@ -154,7 +153,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
           }
           if (lane == 0) mbar_arrive_expect_tx(&full[s], live * BR * HD * 2);
           __syncwarp();
-          if (box < live) pa_tma(smem + s * F::SLOT + plane * F::PLANE + box * BR * 128, v ? &vmap : &kmap, plane * 64, y, &full[s]);
+          if (box < live) pa_tma_3d(smem + s * F::SLOT + box * BR * HD * 2, v ? &vmap : &kmap, 0, y, 0, &full[s]);
         }
       }
     }
@@ -337,7 +336,11 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   // ---- products: a warp has 16 rows and positions 16 wq .. + 15 of every tile
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REGS_MMA));
   const int g = lane >> 2, c = lane & 3, mg = warp >> 2, wq = warp & 3;
-  const uint32_t base = smem_u32(smem);
+  const uint32_t base = smem_u32(smem), plane = BR * 128;
+  // where its rows of a slot are: those that the lane addresses of K, and of V
+  const int rk = wq * 16 + (lane >> 4) * 8 + (lane & 7), rv = wq * 16 + (lane >> 3 & 1) * 8 + (lane & 7);
+  const uint32_t box = (uint32_t)(wq * 16 / BR * BR * HD * 2), in_box = wq * 16 / BR * BR;
+  const uint32_t k_at = base + box + (rk - in_box) * 128, v_at = base + box + (rv - in_box) * 128;
   float* fold = reinterpret_cast<float*>(smem + F::FOLD_OFF + mg * F::FOLD);
   int n = 0;
   for (int k = 0;; ++k) {
@@ -381,15 +384,14 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         float sc[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-        const int pr = wq * 16 + (lane >> 4) * 8 + (lane & 7);
-        const uint32_t ka = base + sk * F::SLOT + pr * 128;
+        const uint32_t ka = k_at + sk * F::SLOT;
 #pragma unroll
         for (int k0 = 0; k0 < KS; k0 += 4) {
           uint32_t b[4][4];
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
             const int chunk = 2 * (k0 + ks) + (lane >> 3 & 1);
-            ldsm4(b[ks], ka + (chunk >> 3) * F::PLANE + (((chunk & 7) ^ (pr & 7)) << 4));
+            ldsm4(b[ks], ka + (chunk >> 3) * plane + (((chunk & 7) ^ (lane & 7)) << 4));
           }
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks) {
@@ -450,8 +452,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       if (!wait(&full[sv], (n + 1) / ST)) return;
       if (live_group) {
         // ---- O += P V
-        const int pr = wq * 16 + (lane >> 3 & 1) * 8 + (lane & 7);
-        const uint32_t va = base + sv * F::SLOT + pr * 128;
+        const uint32_t va = v_at + sv * F::SLOT;
         const int j0 = pw + 2 * c;
 #pragma unroll
         for (int d0 = 0; d0 < KS; d0 += 4) {
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt) {
             const int chunk = 2 * (d0 + dt) + (lane >> 4);
-            ldsm4_t(b[dt], va + (chunk >> 3) * F::PLANE + (((chunk & 7) ^ (pr & 7)) << 4));
+            ldsm4_t(b[dt], va + (chunk >> 3) * plane + (((chunk & 7) ^ (lane & 7)) << 4));
           }
           if (masked) {
             // What not every row sees must not reach the rows that do not: 0 * NaN is
@@ -524,7 +525,7 @@ static cudaError_t launch(PagedAttnArgs& a, cudaStream_t s) {
   using F = Cfg<HD, MG>;
   auto kern = paged_mma_kernel<T, HD, MG, FANCY>;
   CUtensorMap maps[2];
-  if (cudaError_t e = paged_maps(a.c, TILE, maps)) return e;
+  if (cudaError_t e = paged_maps(a.c, TILE, true, maps)) return e;
   static PagedReady ready;
   if (cudaError_t e = ready.set((const void*)kern, F::SMEM)) return e;
   return launch_pdl_smem(kern, dim3(paged_ctas(16 * MG)), dim3(F::THREADS), F::SMEM, s, a, maps[0], maps[1]);
@@ -548,16 +549,20 @@ static EncodeFn encode_fn() {
   return fn;
 }
 
-// K and V as 2-D tensors of rows; a box is (part of) one page of one kv head, 64
-// dims wide, in the 128-byte swizzle.  x is 0 or 64 values: 16-byte boundaries.
-cudaError_t paged_maps(const PagedView& c, int tile, CUtensorMap* maps) {
+// K and V as tensors of rows; a box is (part of) one page of one kv head, 64 dims wide,
+// in the 128-byte swizzle.  x is 0 or 64 values: 16-byte boundaries.  With `planes` a
+// box has all planes of 64 dims, one after the other: half the boxes at 128 dims, which
+// with pages of 16 were more than one warp could send (16 requests of 2 to 5 tokens
+// 49 us so, 57 with a box per plane).
+cudaError_t paged_maps(const PagedView& c, int tile, bool planes, CUtensorMap* maps) {
   const EncodeFn enc = encode_fn();
   if (!enc) return cudaErrorNotSupported;
-  const cuuint64_t dims[2] = {(cuuint64_t)c.hd, (cuuint64_t)c.num_pages * c.kv_heads * c.page_size};
-  const cuuint64_t strides[1] = {(cuuint64_t)c.hd * 2};
-  const cuuint32_t box[2] = {64u, (cuuint32_t)(c.page_size < tile ? c.page_size : tile)}, ones[2] = {1, 1};
+  const cuuint64_t dims[3] = {planes ? 64u : (cuuint64_t)c.hd, (cuuint64_t)c.num_pages * c.kv_heads * c.page_size,
+                              (cuuint64_t)c.hd / 64};
+  const cuuint64_t strides[2] = {(cuuint64_t)c.hd * 2, 128};
+  const cuuint32_t box[3] = {64u, (cuuint32_t)(c.page_size < tile ? c.page_size : tile), (cuuint32_t)c.hd / 64}, ones[3] = {1, 1, 1};
   for (int i = 0; i < 2; ++i)
-    if (enc(&maps[i], c.dtype == ODI_CUDA_PAGED_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+    if (enc(&maps[i], c.dtype == ODI_CUDA_PAGED_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes ? 3 : 2,
             i ? c.v : c.k, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return cudaErrorInvalidValue;

@@ -108,6 +108,14 @@ __device__ __forceinline__ void pa_tma(void* dst, const CUtensorMap* map, int x,
       : "memory");
 }
 
+__device__ __forceinline__ void pa_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -258,7 +266,7 @@ struct PagedReady {
   }
 };
 
-cudaError_t paged_maps(const PagedView& c, int tile, CUtensorMap* maps);
+cudaError_t paged_maps(const PagedView& c, int tile, bool planes, CUtensorMap* maps);
 cudaError_t paged_q_map(const PagedAttnArgs& a, int tokens, CUtensorMap* map);
 cudaError_t launch_paged_mma(PagedAttnArgs& a, int groups, bool fancy, cudaStream_t s);
 cudaError_t launch_paged_tc(PagedAttnArgs& a, int rows, cudaStream_t s);

@@ -168,14 +168,6 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
 // What a score goes through: nothing but the scale; a distance bias; a cap (and a bias).
 enum { PLAIN = 0, BIAS = 1, CAP = 2 };
 
-__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-
 struct Piece {
   PagedPiece p;
   int end[2];  // tiles of the unit that each half of its rows sees
@@ -405,7 +397,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
             mbar_arrive_expect_tx(&bars.q_full[h], F::Q_HALF);
 #pragma unroll
             for (int pl = 0; pl < PLANES; ++pl)
-              tma_3d(smem + F::Q_OFF + h * F::Q_HALF + pl * F::Q_PLANE, &qmap, pl * 64, p.kvh * a.G, token, &bars.q_full[h]);
+              pa_tma_3d(smem + F::Q_OFF + h * F::Q_HALF + pl * F::Q_PLANE, &qmap, pl * 64, p.kvh * a.G, token, &bars.q_full[h]);
           }
           continue;
         }
@@ -788,7 +780,7 @@ static cudaError_t launch(PagedAttnArgs& a, cudaStream_t s) {
   using F = Cfg<HD, NH>;
   auto kern = paged_tc_kernel<T, HD, MODE, NH>;
   CUtensorMap maps[3];
-  if (cudaError_t e = paged_maps(a.c, TILE, maps)) return e;
+  if (cudaError_t e = paged_maps(a.c, TILE, false, maps)) return e;
   // whole tokens of a group: boxes of 64 dims, G heads, 128 / G tokens
   a.q_boxes = a.vec && HALF_ROWS % a.G == 0;
   maps[2] = maps[0];
