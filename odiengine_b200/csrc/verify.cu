@@ -17,9 +17,9 @@
 // request each fold its rows' sums, find the row where its drafts end, and add
 // up as many of that row's weights; the last to arrive finds the token.
 //
-// 81 rows of 128,259 ids of 16 requests take 33 us, 2.3 TB/s: HBM would let them take
-// 11, the 11 operations of 64 bits per id 8, and two launches whose CTAs end with
-// joins do the rest.  5 rows of 32,000 ids take 12 us, nearly all of it latency.
+// 81 rows of 128,259 ids of 16 requests take 31 us, 2.5 TB/s: HBM would let them take
+// 11, the 12 operations of 64 bits per id 9, and two launches whose CTAs end with
+// joins do the rest.  5 rows of 32,000 ids take 11 us, nearly all of it latency.
 #include <math.h>
 
 #include "../../include/odi_cuda.h"
@@ -43,7 +43,6 @@ struct VerifyArgs {
   int requests, rows, slices, stats;  // pieces of a row: of the draw, of the sums
   int64_t V;
   double unit;      // 256 / (T ln 2)
-  float reach;      // 256000 / unit
   double2* stat;    // [rows][stats]: largest logit, sum
   double2* part;    // [requests][slices]: sums of max(p - q, 0) and of p
   int* count;       // [requests] arrivals, zero between launches
@@ -119,18 +118,18 @@ __constant__ double TWO_TO_256THS[256] = {  // 2^(i / 256)
 // 2^(k / 256) from a table times a Taylor polynomial (the next term is below 2^-54):
 // the table-driven method of Tang (1989).  k is whole by the addition of 1.5 * 2^52,
 // whose low word then holds it; conversions and roundings of 64 bits run at a
-// quarter of an add's rate.  11 operations in 64 bits, of which an SM does 64 a cycle.
+// quarter of an add's rate.  What is below 2^-1000 counts as that, or as 0: t is
+// compared in 64 bits, since fp32 need not have a logit that lies as far below m
+// (3e9 has neighbours 256 apart).  12 operations in 64 bits, of which an SM does 64 a
+// cycle.
 struct Exp64 {
   const double* table;  // in shared memory
   double unit, md;
-  float least;          // logits below it count as it: there the result is below 2^-999
   __device__ __forceinline__ Exp64(const double* table, const VerifyArgs& a, float m) : table(table), unit(a.unit) {
     md = m == -INFINITY ? 0.0 : (double)m;
-    least = m == -INFINITY ? 0.f : m - a.reach;
   }
-  __device__ __forceinline__ double operator()(float x) const {
+  __device__ __forceinline__ double at(double t) const {
     constexpr double c = 0.0027076061740622863, magic = 6755399441055744.0;  // ln 2 / 256
-    const double t = ((double)max_nan(x, least) - md) * unit;
     const double s = t + magic;
     const int i = __double2loint(s);
     const double r = t - (s - magic);
@@ -141,11 +140,14 @@ struct Exp64 {
     p *= table[i & 255];
     return __hiloint2double(__double2hiint(p) + ((i & ~255) << 12), __double2loint(p));
   }
-  __device__ __forceinline__ double or_zero(float x) const { return x < least ? 0.0 : (*this)(x); }
-  static __device__ __forceinline__ float max_nan(float a, float b) {
-    float m;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-    return m;
+  static constexpr double LEAST = -256000.0;
+  __device__ __forceinline__ double operator()(float x) const {
+    const double t = ((double)x - md) * unit;
+    return at(t < LEAST ? LEAST : t);  // NaN stays
+  }
+  __device__ __forceinline__ double or_zero(float x) const {
+    const double t = ((double)x - md) * unit;
+    return t < LEAST ? 0.0 : at(t);
   }
 };
 __device__ __forceinline__ void fill_table(double* table) { table[threadIdx.x] = TWO_TO_256THS[threadIdx.x]; }
@@ -431,7 +433,6 @@ int odi_cuda_verify_sampled(const float* d_logits, int64_t ld, const int32_t* d_
   a.u_accept = d_u_accept, a.u_next = d_u_next, a.accepted = d_accepted, a.next = d_next;
   a.requests = requests, a.rows = rows, a.V = V;
   a.unit = 369.3299304757364 / temperature;  // 256 / ln 2
-  a.reach = (float)(256000.0 / a.unit);
   a.count = static_cast<int*>(d_scratch);
   a.stat = reinterpret_cast<double2*>(static_cast<uint8_t*>(d_scratch) + COUNT_BYTES);
   a.part = a.stat + (int64_t)rows * slices_of(V);
