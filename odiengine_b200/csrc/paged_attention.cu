@@ -380,6 +380,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       if (!wait(&full[sk], n / ST)) return;
       uint32_t pf[4];
       if (live_group) {
+        __syncwarp();  // ldmatrix and mma want whole warps, and a wait may let lanes go one by one
         // ---- S = Q K^T
         float sc[2][4];
 #pragma unroll
@@ -451,6 +452,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       }
       if (!wait(&full[sv], (n + 1) / ST)) return;
       if (live_group) {
+        __syncwarp();
         // ---- O += P V
         const uint32_t va = v_at + sv * F::SLOT;
         const int j0 = pw + 2 * c;

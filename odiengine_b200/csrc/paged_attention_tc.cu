@@ -665,6 +665,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
           uint32_t o[16];
+          __syncwarp();  // lanes part ways below, at what is not finite and where rows end
           ld16(o, o_addr + c);
           float v[16];
 #pragma unroll

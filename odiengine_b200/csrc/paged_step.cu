@@ -67,10 +67,13 @@ __device__ __forceinline__ Sum2 block_scan(Sum2 v, Sum2* total, Sum2* warps) {
   return {s.a - v.a + (warp ? p.a : 0), s.b - v.b + (warp ? p.b : 0)};
 }
 
+// The cluster's barrier, an .aligned one, wants whole warps; lanes come to it from a
+// loop that they leave at different times.
 __device__ __forceinline__ void step_barrier(int C) {
   if (C == 1) {
     __syncthreads();
   } else {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }

@@ -51,3 +51,46 @@ def test_verify_rows_whose_largest_logits_have_it_all(cuda_lib, top, temperature
     want = paged_ref.verify(logits, tokens.tolist(), starts, ua.tolist(), un.tolist(), temperature, None if q is None else q.numpy())
     assert got[0].tolist() == want[0] and got[1].tolist() == want[1], (got, want)
     assert want[0][0] == want[0][2] == 1 and want[0][6] == 0  # p = 1 is kept, p = 0 is not
+
+
+# ---- lanes that part ways ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("past,new,heads,kv,hd", [([70], [45], 3, 3, 64), ([0, 130], [77, 40], 5, 1, 64), ([300], [260], 3, 3, 64),
+                                                  ([90], [45], 3, 3, 128)])
+@pytest.mark.parametrize("out32", [False, True])
+def test_rows_that_end_inside_a_warp(cuda_lib, past, new, heads, kv, hd, out32):
+    """Values that are not finite, which each row gets back for the positions that it
+    sees, in items whose last warp has rows and lanes without one."""
+    from odiengine_b200 import paged
+
+    s = Setup(past, new, heads, kv, hd, "f16", 32)
+    row = 0
+    for N in new:
+        for j, x in ((1, math.nan), (N // 3, math.inf), (N - 2, -math.inf)):
+            slot = int(s.batch.slots[row + j])
+            s.cache.v[slot // 32, :, slot % 32, (7 * j) % hd] = x
+        row += N
+    out = torch.empty(s.q.shape, dtype=torch.float32 if out32 else s.q.dtype, device="cuda")
+    paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=0.1, scratch=s.scratch)
+    s.check(out, 0.1)
+    assert cuda_lib_status(s.scratch) == 0
+
+
+@pytest.mark.parametrize("B,drops", [(300, 1), (300, 37), (1500, 9001), (2048, 8191)])
+def test_steps_that_drop_any_number_of_pages(cuda_lib, B, drops):
+    """Pages dropped by some lanes of some warps of a cluster, before the barrier that
+    all of them share."""
+    from odiengine_b200 import paged
+
+    P, wide = 16, 8
+    t = paged.PageTables.new(B, wide, B * wide, P)
+    batch = paged.PagedBatch(t, max_rows=B * wide * P, max_new=wide * P, heads=4, kv_heads=4)
+    ref = paged_ref.Tables(t.table.tolist(), t.lens.tolist(), t.free.tolist(), B * wide)
+    full, each = [wide * P] * B, [drops // B + (b < drops % B) for b in range(B)]
+    for new, keep in ((full, None), ([P + 1 if d > 1 else 0 for d in each], [(wide - min(d, wide)) * P for d in each]),
+                      ([1] * B, [0] * B)):
+        status, starts, lens, pos, slots = ref.step(P, new, keep, wide * P, B * wide * P)
+        paged.paged_step(t, batch, ints(new), keep=None if keep is None else ints(keep))
+        assert batch.status() == status == 0
+        assert t.table.tolist() == ref.table and t.free.tolist() == ref.free and t.free_count.item() == ref.count
+        assert batch.starts.tolist() == starts and batch.positions.tolist() == pos and batch.slots.tolist() == slots
