@@ -67,6 +67,10 @@ def _new(shape, dtype, device, stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
+def _apart(what: str, handle, dev: int) -> None:
+    raise ValueError(f"{what}: must be on cuda:{dev}, is on cuda:{handle.index}")
+
+
 class PagedCache:
     """One layer's K and V: fp16 or bf16 [num_pages, kv_heads, page_size, head_dim]."""
 
@@ -161,6 +165,8 @@ def paged_step(tables: PageTables, batch: PagedBatch, new, keep=None, prefix=Non
     more (int32 [requests]); prefix[b] positions see one another both ways.
     Tables and batch are brought up to date."""
     dev, B = tables.index, tables.requests
+    if batch.index != dev:
+        _apart("batch", batch, dev)
     i32 = torch.int32
     _call(dev, stream, lib().odi_cuda_paged_step, tables._ref, batch._ref,
           None if keep is None else _flat(keep, i32, "keep", dev, B), _flat(new, i32, "new", dev, B),
@@ -174,6 +180,8 @@ def qk_rope_append_paged(qkv, cache: PagedCache, batch: PagedBatch, q_out=None, 
     at their positions, k and v stored at their slots.  Returns the rotated q
     in q_out [T, heads * head_dim] of the cache's type."""
     dev, hd, f32 = cache.index, cache.head_dim, torch.float32
+    if batch.index != dev:
+        _apart("batch", batch, dev)
     ld = _rows2(qkv, f32, "qkv", dev, None, (heads + 2 * cache.kv_heads) * hd)
     T = qkv.shape[0]
     if q_out is None:
@@ -202,6 +210,10 @@ def attention_paged(q, cache: PagedCache, tables: PageTables, batch: PagedBatch,
     softcap); slopes fp32 [heads]: scores lose slope * distance.  out: of the
     cache's type (the default) or fp32; rows behind the batch's last are left."""
     dev, w = cache.index, batch.heads * cache.head_dim
+    if tables.index != dev:
+        _apart("tables", tables, dev)
+    if batch.index != dev:
+        _apart("batch", batch, dev)
     ld = _rows2(q, cache.dtype, "q", dev, None, w)
     T = q.shape[0]
     if out is None:
@@ -288,6 +300,8 @@ class PagedDecoder:
         self.cfg, self.w, self.temperature = cfg, weights, temperature
         dev = torch.device("cuda" if device is None else device)
         self.device = dev = torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev
+        if weights.token_embd.get_device() != dev.index:
+            raise ValueError(f"weights: must be on {dev}, are on {weights.token_embd.device}")
         self.requests, self.max_drafts, self.chunk = requests, max_drafts, chunk
         self.softcap, self.slopes = softcap, slopes
         self.page_size, self.num_pages = page_size, num_pages
