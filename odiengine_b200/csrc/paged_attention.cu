@@ -21,9 +21,11 @@
 //
 // q . k and o are summed in fp32.  The weights enter the second product rounded
 // to the cache's type, relative to a reference that moves only when a weight
-// would pass 2^8: half a step of that type per weight, independent from weight
-// to weight, which is no more than the output's own rounding; their sum is taken
-// before the rounding.
+// would pass 2^8 of it; their sum is taken before the rounding.  That is half a step of
+// the type per weight, independent from weight to weight, so that the sum of many is
+// off by less than the rounding of an output of that type; of an fp32 output it is the
+// whole error.  fp16's steps end: what a row's largest weight outweighs 2^31 times
+// has no weight, which is off by 2^-32 of the largest per position at most.
 #include <cstdio>
 
 #include "paged_attention.cuh"
@@ -33,7 +35,6 @@ namespace odi_cuda {
 namespace pmma {
 
 constexpr int TILE = 64;
-constexpr float MOVE = 8.f;  // log2 of what a weight may reach before the reference moves
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   using F = Cfg<HD, MG>;
   using H = Half16<T>;
   constexpr int KS = HD / 16, ROWS = 16 * MG, ST = F::ST;
+  constexpr float MOVE = H::BELOW + PAGED_MOVE;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[ST], empty[ST], d_full[ND], d_empty[ND], fold_full, fold_empty, jbar;
   __shared__ PagedPiece pieces[ND];
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         if (__any_sync(0xffffffffu, mx[0] > m[0] + MOVE || mx[1] > m[1] + MOVE)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float top = mx[e] > m[e] + MOVE ? mx[e] : m[e];
+            const float top = mx[e] > m[e] + MOVE ? mx[e] - H::BELOW : m[e];
             const float f = m[e] == top ? 1.f : pa_ex2(m[e] - top);
             m[e] = top;
             l[e] *= f;

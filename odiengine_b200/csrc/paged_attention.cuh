@@ -67,10 +67,17 @@ __device__ __forceinline__ int pa_token(const PagedAttnArgs& a, int r) {
   return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.inv_G);
 }
 
+// log2 of what a weight may reach before the reference moves, and how far below the
+// largest score the reference stands when it has moved.  fp16 ends at 2^16 and its steps
+// at 2^-24: with the reference 7 lower, weights are up to 2^15, the largest of a row is 2^7
+// at least, and one of 2^-21 of that has its 11 bits (2^-14 without), one of 2^-31 some.
+constexpr float PAGED_MOVE = 8.f;
+
 template <typename T>
 struct Half16;
 template <>
 struct Half16<__half> {
+  static constexpr float BELOW = 7.f;
   static constexpr uint32_t EXP = 0x7c00u;
   static constexpr bool BF = false;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
@@ -86,6 +93,7 @@ struct Half16<__half> {
 };
 template <>
 struct Half16<__nv_bfloat16> {
+  static constexpr float BELOW = 0.f;
   static constexpr uint32_t EXP = 0x7f80u;
   static constexpr bool BF = true;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {

@@ -38,7 +38,6 @@ namespace odi_cuda {
 namespace ptc {
 
 constexpr int TILE = 64, HALF_ROWS = 128;
-constexpr float MOVE = 8.f;
 // Of eight pairs of weights one is exponentiated on the FMA pipe.  The loop over 64
 // scores of a row, two warps per scheduler: 933 cycles so, 1188 without, 964 with
 // three; without the order that the volatile statements keep 1290.
@@ -187,6 +186,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
   using F = Cfg<HD, NH>;
   using H = Half16<T>;
   constexpr int ST = F::ST, PLANES = HD / 64, ROWS = F::ROWS;
+  constexpr float MOVE = H::BELOW + PAGED_MOVE;
   constexpr int PRODUCER = 4 * NH, PRODUCTS = PRODUCER + 1, LOADER = PRODUCER + 3;  // warps
   // With a distance bias a long piece goes from its last tile to its first: scores
   // only fall that way, and the reference stays where the first tiles put it (2048
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
         const bool move = !(mx <= ref + MOVE) && ref == ref;  // a row that is NaN stays so
         if (__any_sync(0xffffffffu, move)) {
           // a NaN among the scores, or +inf, leaves no weight: the row is NaN from here on
-          const float top = !move ? ref : mx == INFINITY ? __int_as_float(0x7fc00000) : mx;
+          const float top = !move ? ref : mx == INFINITY ? __int_as_float(0x7fc00000) : mx - H::BELOW;
           const float f = top == ref ? 1.f : pa_ex2(ref - top);
           ref = top;
           sum[0].x *= f, sum[0].y *= f, sum[1].x *= f, sum[1].y *= f;

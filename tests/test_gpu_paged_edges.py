@@ -53,6 +53,51 @@ def test_verify_rows_whose_largest_logits_have_it_all(cuda_lib, top, temperature
     assert want[0][0] == want[0][2] == 1 and want[0][6] == 0  # p = 1 is kept, p = 0 is not
 
 
+# ---- attention ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,heads,kv,hd", [(1, 4, 4, 128), (1, 8, 1, 64), (1, 128, 128, 64), (3, 8, 1, 128), (70, 2, 2, 128), (40, 8, 1, 64), (300, 4, 2, 64)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("nats", [12.0, 17.0, 18.0, 20.0])
+@pytest.mark.parametrize("own", [0.0, 0.001])
+def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats, own):
+    """One key some nats above all others, whose values are 0 or small: what the
+    others add is there.  A weight is off by half a step of its type, 2^-20 and its
+    score's error; in fp16, whose steps end, by 2^-32 of the row's largest weight: half
+    of 2^-24, that weight standing at 2^7 or above."""
+    from odiengine_b200 import paged
+
+    past = 3000 - new
+    s = Setup([past], [new], heads, kv, hd, dtype, 64, seed=int(nats))
+    scale = 1 / math.sqrt(hd)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    base = torch.randn(hd, device="cuda", generator=g)
+    base = base / base.norm() * math.sqrt(hd)
+    # every query along one direction, the keys but one across it or nearly so
+    s.q.copy_((base * (1 + 0.01 * torch.randn((new, heads, 1), device="cuda", generator=g))).reshape(new, -1))
+    keys = torch.randn(s.cache.k.shape, device="cuda", generator=g)
+    keys -= (keys @ base)[..., None] * base / hd
+    s.cache.k.copy_(keys * 0.3)
+    s.cache.v.copy_(1 + 0.5 * torch.randn(s.cache.v.shape, device="cuda", generator=g))
+    slot = int(s.tables.table[0, 1500 // 64]) * 64 + 1500 % 64
+    s.cache.k[slot // 64, :, slot % 64] = base * (nats / (scale * hd))
+    s.cache.v[slot // 64, :, slot % 64] = own
+    out = torch.empty((new, heads * hd), dtype=torch.float32, device="cuda")
+    paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=scale, scratch=s.scratch)
+    q, k, v = (t.cpu().double() for t in (s.q, s.rows(s.cache.k, 0), s.rows(s.cache.v, 0)))
+    x = q.view(new, kv, heads // kv, hd)
+    see = (torch.arange(past + new)[None] <= torch.arange(past, past + new)[:, None])[:, None, None]
+    sc = torch.einsum("tkgd,knd->tkgn", x, k) * scale
+    ds = torch.einsum("tkgd,knd->tkgn", x.abs(), k.abs()) * scale * 2.0 ** -21
+    p = torch.exp((sc - sc.masked_fill(~see, -math.inf).amax(-1, keepdim=True)).masked_fill(~see, -math.inf))
+    l = p.sum(-1, keepdim=True)
+    want = torch.einsum("tkgn,knd->tkgd", p, v) / l
+    err = p * (torch.finfo(s.cache.dtype).eps / 2 + 2.0 ** -20 + ds) + (2.0 ** -32 * see if dtype == "f16" else 0.0)
+    tol = torch.einsum("tkgn,knd->tkgd", err, v.abs()) / l + want.abs() * ((p * (ds + 2.0 ** -20)).sum(-1, keepdim=True) / l + 2.0 ** -23)
+    off = (out.cpu().double().view(want.shape) - want).abs()
+    assert (off <= tol).all(), (off.max(), (off / tol).max())
+    assert cuda_lib_status(s.scratch) == 0
+
+
 # ---- lanes that part ways ------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("past,new,heads,kv,hd", [([70], [45], 3, 3, 64), ([0, 130], [77, 40], 5, 1, 64), ([300], [260], 3, 3, 64),
