@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     for (int e = 0; e < 2; ++e) {
       const bool live = e * 8 + g < rows;
       const int R = R0 + (live ? e * 8 + g : 0), token = pa_token(a, R), head = p.kvh * a.G + R - token * a.G;
-      tok[e] = (float)(past + token);
+      tok[e] = (float)token;
       lim[e] = live ? paged_limit(past, token, len, p.it.prefix) : 0;
       slope[e] = FANCY && a.slopes && live ? __ldg(a.slopes + head) * 1.4426950408889634f : 0.f;
       m[e] = -INFINITY, l[e] = 0.f;
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
         if (lane == 0) mbar_arrive(&empty[sk]);
         // ---- scores, weights
         float mx[2];
-        const float at = (float)(pw + 2 * c);  // positions are whole below 2^24
+        const float at = (float)(pw + 2 * c - past);  // as tok, from the first new token: whole below 2^24, far ones to 2^-24
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           mx[e] = -INFINITY;

@@ -98,6 +98,36 @@ def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats
     assert cuda_lib_status(s.scratch) == 0
 
 
+@pytest.mark.parametrize("new", [[1], [3], [40]])
+def test_distances_behind_16_million_positions(cuda_lib, new):
+    """Distances count whole positions where fp32 no longer tells two neighbouring
+    positions apart."""
+    from odiengine_b200 import paged
+
+    past, heads, hd, P, near = (1 << 24) + 5, 4, 64, 128, 4096
+    n = past + new[0]
+    pages = -(-n // P)
+    pools = [torch.zeros((pages, 1, P, hd), dtype=torch.float16, device="cuda") for _ in range(2)]
+    cache = paged.PagedCache(*pools)
+    t = paged.PageTables(torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous(), ints([past]),
+                         torch.zeros(pages, dtype=torch.int32, device="cuda"), ints([0]), P)
+    t.lens.fill_(n)  # the new tokens' pages are there
+    batch = paged.PagedBatch(t, max_rows=new[0], max_new=new[0], heads=heads, kv_heads=1)
+    paged.paged_step(t, batch, ints(new), keep=ints([past]))
+    assert batch.status() == 0
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for pool in pools:
+        pool.view(-1, hd)[n - near:n] = torch.randn((near, hd), device="cuda", generator=g).half()
+    q = torch.randn((new[0], heads * hd), device="cuda", generator=g).half()
+    slopes = torch.tensor([0.25, 0.5, 1.0, 2.0], device="cuda")
+    scratch = paged.attention_paged_scratch(cache, batch)
+    out = paged.attention_paged(q, cache, t, batch, scale=0.125, slopes=slopes, scratch=scratch)
+    k, v = (pool.view(-1, hd)[n - near:n][None] for pool in pools)  # beyond, the weights are below e^-900
+    want, tol = paged_ref.attention(q, k, v, near - new[0], heads, 0.125, 0.0, slopes)
+    assert paged_ref.within(out, want, tol, out.dtype), (out.cpu().double() - want).abs().max()
+    assert cuda_lib_status(scratch) == 0
+
+
 # ---- lanes that part ways ------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("past,new,heads,kv,hd", [([70], [45], 3, 3, 64), ([0, 130], [77, 40], 5, 1, 64), ([300], [260], 3, 3, 64),
