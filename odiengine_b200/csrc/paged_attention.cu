@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       }
       if (fix) {
         const int row_lim = paged_limit(p.it.past, pa_token(a, p.it.i * ROWS + r), len, p.it.prefix);
-        for (int j = max(t0 * TILE, least); j < min(t1 * TILE, row_lim); ++j) {
+        for (int j = max(t0 * TILE, least); j < min(t1 * TILE, row_lim) && j >> a.c.page_shift < a.max_pages; ++j) {
           const int page = __ldcg(a.table + (int64_t)p.it.b * a.max_pages + (j >> a.c.page_shift));
           if ((unsigned)page >= (unsigned)a.c.num_pages) continue;
           const unsigned short* src = static_cast<const unsigned short*>(a.c.v) +

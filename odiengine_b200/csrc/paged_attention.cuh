@@ -216,7 +216,8 @@ struct PagedNames {
   int last, block, cur, next;  // entries there are; the 32 at hand
   __device__ __forceinline__ PagedNames(const PagedAttnArgs& a, const PagedPiece& p, int tile, bool down)
       : row(a.table + (int64_t)p.it.b * a.max_pages), step(down ? -1 : 1) {
-    last = (min(p.it.len, p.t1 * tile) + a.c.page_size - 1) >> a.c.page_shift;
+    // a list made with wider tables than these names pages that they do not have
+    last = min((min(p.it.len, p.t1 * tile) + a.c.page_size - 1) >> a.c.page_shift, a.max_pages);
     block = ((down ? p.t1 - 1 : p.t0) * tile >> a.c.page_shift) >> 5;
     cur = load(block), next = load(block + step);
   }

@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(o[e]);
           if (fix)
-            for (int j = max(t0 * TILE, p.least); j < min(t1 * TILE, lim); ++j) {
+            for (int j = max(t0 * TILE, p.least); j < min(t1 * TILE, lim) && j >> a.c.page_shift < a.max_pages; ++j) {
               const int page = __ldcg(a.table + (int64_t)p.it.b * a.max_pages + (j >> a.c.page_shift));
               if ((unsigned)page >= (unsigned)a.c.num_pages) continue;
               const unsigned short* src = reinterpret_cast<const unsigned short*>(a.c.v) +

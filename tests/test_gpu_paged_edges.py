@@ -169,3 +169,32 @@ def test_steps_that_drop_any_number_of_pages(cuda_lib, B, drops):
         assert batch.status() == status == 0
         assert t.table.tolist() == ref.table and t.free.tolist() == ref.free and t.free_count.item() == ref.count
         assert batch.starts.tolist() == starts and batch.positions.tolist() == pos and batch.slots.tolist() == slots
+
+
+# ---- tables that are not the step's ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new", [[3, 1], [70, 40]])
+@pytest.mark.parametrize("nan", [False, True])
+def test_tables_narrower_than_the_steps(cuda_lib, new, nan):
+    """A step made with tables of more pages per request: the pages that these do not
+    have read as zeros, as ones that they do not name, and the error word says so."""
+    from odiengine_b200 import paged
+
+    heads, kv, hd, P, wide = 4, 1, 64, 32, 3
+    s = Setup([200, 40], new, heads, kv, hd, "f16", P)
+    assert s.tables.max_pages > wide
+    if nan:  # a value behind the narrow table's end, and one before it
+        for r in (1, new[0]):
+            slot = int(s.batch.slots[r])
+            s.cache.v[slot // P, :, slot % P, 5] = math.nan
+    t = paged.PageTables(s.tables.table[:, :wide].contiguous(), s.tables.lens, s.tables.free, s.tables.free_count, P)
+    out = paged.attention_paged(s.q, s.cache, t, s.batch, scale=0.1, scratch=s.scratch)
+    assert cuda_lib_status(s.scratch) != 0
+    s.scratch[:4].zero_()
+    row = 0
+    for b, N in enumerate(new):
+        k, v = (s.rows(pool, b).clone() for pool in (s.cache.k, s.cache.v))
+        k[:, wide * P:], v[:, wide * P:] = 0, 0
+        want, tol = paged_ref.attention(s.q[row:row + N], k, v, s.past[b], heads, 0.1)
+        assert paged_ref.within(out[row:row + N], want, tol, out.dtype)
+        row += N
