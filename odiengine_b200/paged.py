@@ -262,14 +262,6 @@ def verify_sampled(logits, tokens, starts, u_accept, u_next, accepted=None, next
     return accepted, next
 
 
-class _Pass:
-    """What a forward pass of up to max_rows rows keeps: its batch and scratch."""
-
-    def __init__(self, cache, tables, max_rows: int, max_new: int, heads: int):
-        self.batch = PagedBatch(tables, max_rows=max_rows, max_new=max_new, heads=heads, kv_heads=cache.kv_heads)
-        self.scratch = attention_paged_scratch(cache, self.batch)
-
-
 class PagedDecoder:
     """Decoding of several sequences at once, over one paged cache: the model of
     decode.DecodeModel for every request's new tokens in one pass.
@@ -310,9 +302,11 @@ class PagedDecoder:
             self.tables = PageTables.new(requests, -(-cfg.ctx // page_size), num_pages, page_size, dev)
             decode_rows = requests * (1 + max_drafts)
             self.rows = T = max(decode_rows, chunk)
-            # single tokens and drafts apart from chunks: they have kernels of their own
-            self._decode = _Pass(self.caches[0], self.tables, decode_rows, 1 + max_drafts, cfg.heads)
-            self._chunks = _Pass(self.caches[0], self.tables, T, chunk, cfg.heads)
+            # single tokens, drafts and chunks apart: the batch's max_new chooses attention's kernel
+            batch = lambda rows, new: PagedBatch(self.tables, max_rows=rows, max_new=new, heads=cfg.heads, kv_heads=cfg.kv_heads)  # noqa: E731
+            self._single, self._drafts, self._chunks = batch(requests, 1), batch(decode_rows, 1 + max_drafts), batch(T, chunk)
+            self.attention_ws = max((attention_paged_scratch(self.caches[0], b) for b in (self._single, self._drafts, self._chunks)),
+                                    key=lambda ws: ws.numel())
             f32, w = torch.float32, cfg.heads * cfg.head_dim
             new = lambda *s, dt=f32: torch.empty(s, dtype=dt, device=dev)  # noqa: E731
             self.x, self.qkv, self.q = new(T, cfg.hidden), new(T, cfg.qkv_rows), new(T, w, dt=dtype)
@@ -347,22 +341,22 @@ class PagedDecoder:
         check(lib().odi_cuda_matmul_fused(dw.dtype, dw.data_ptr, x.data_ptr(), y.data_ptr(), T, dw.N, dw.K, self.cfg.act_mode,
                                           ws.data_ptr(), ws.numel(), FLAG_PDL, ctypes.byref(o), _raw_stream(self.device.index)))
 
-    def _forward(self, p: _Pass, tokens: dict, logits: bool) -> None:
+    def _forward(self, batch: PagedBatch, tokens: dict, logits: bool) -> None:
         """The new tokens of some requests, {request: tokens}, in the requests' order."""
         cfg, rows = self.cfg, [t for b in range(self.requests) for t in tokens.get(b, ())]
         T, stream = len(rows), _raw_stream(self.device.index)
         host = torch.tensor([self._len, [len(tokens.get(b, ())) for b in range(self.requests)]], dtype=torch.int32)
         keep, fresh = host.to(self.device)
-        paged_step(self.tables, p.batch, fresh, keep=keep)
+        paged_step(self.tables, batch, fresh, keep=keep)
         self.states[:T].copy_(torch.tensor([[t, 0, 0, 0] for t in rows], dtype=torch.int32))
         for r in range(T):
             check(lib().odi_cuda_embed(self.w.token_embd.data_ptr(), cfg.vocab, cfg.hidden, self.states.data_ptr() + 16 * r,
                                        self.x.data_ptr() + 4 * cfg.hidden * r, None, None, None, stream))
         for cache, lw in zip(self.caches, self.w.layers):
             self._product(lw.wqkv, self.x, self.qkv, T, norm=lw.attn_norm)
-            qk_rope_append_paged(self.qkv[:T], cache, p.batch, self.q[:T], heads=cfg.heads, theta=cfg.theta)
-            attention_paged(self.q[:T], cache, self.tables, p.batch, self.attn[:T], scale=cfg.head_dim ** -0.5,
-                            softcap=self.softcap, slopes=self.slopes, scratch=p.scratch)
+            qk_rope_append_paged(self.qkv[:T], cache, batch, self.q[:T], heads=cfg.heads, theta=cfg.theta)
+            attention_paged(self.q[:T], cache, self.tables, batch, self.attn[:T], scale=cfg.head_dim ** -0.5,
+                            softcap=self.softcap, slopes=self.slopes, scratch=self.attention_ws)
             self._product(lw.wo, self.attn, self.x, T, accumulate=True)
             self._product(lw.wgu, self.x, self.gu, T, norm=lw.ffn_norm)
             self._product(lw.wdown, self.gu, self.x, T, swiglu=True, accumulate=True)
@@ -371,14 +365,14 @@ class PagedDecoder:
 
     def status(self) -> int:
         """OR of the device error words (0: no bounded wait gave up, every page was one)."""
-        words = [ws[:4].view(torch.int32) for ws in (self._decode.scratch, self._chunks.scratch, self.products_ws)]
+        words = [ws[:4].view(torch.int32) for ws in (self.attention_ws, self.products_ws)]
         v = 0
         for x in torch.cat(words).cpu().tolist():
             v |= x
         return v
 
-    def _check(self, p: _Pass) -> None:
-        st, refused = self.status(), p.batch.status()
+    def _check(self, batch: PagedBatch) -> None:
+        st, refused = self.status(), batch.status()
         if st or refused:
             raise RuntimeError(f"paged decoding: a device wait gave up or a page was none (error word {st:#x}), or a request "
                                f"was refused (status {refused})")
@@ -451,9 +445,10 @@ class PagedDecoder:
                     self._len[b] += len(t)
                     self._todo[b] = self._todo[b][len(t):]
             if decode:
-                self._forward(self._decode, decode, True)
-                accepted, nxt = self._choose(decode)
-                self._check(self._decode)
+                batch = self._single if all(len(t) == 1 for t in decode.values()) else self._drafts
+                self._forward(batch, decode, True)
+                accepted, nxt = self._choose(batch, decode)
+                self._check(batch)
                 if any(nxt[b] < 0 for b in decode):
                     raise RuntimeError("step: logits without a finite value")
                 for b, t in decode.items():
@@ -462,7 +457,7 @@ class PagedDecoder:
                     self._todo[b] = [nxt[b]]
         return out
 
-    def _choose(self, decode: dict):
+    def _choose(self, batch: PagedBatch, decode: dict):
         """Drafts kept and the next token of each request, by the last pass's logits."""
         T = sum(len(t) for t in decode.values())
         if self.temperature is None:
@@ -479,6 +474,6 @@ class PagedDecoder:
         u = torch.rand(T + self.requests, device=self.device, generator=self.generator)
         self.u_accept, self.u_next = u[:T], u[T:]
         tokens = self.states[:T, 0].contiguous()
-        accepted, nxt = verify_sampled(self.logits[:T], tokens, self._decode.batch.starts, self.u_accept, self.u_next,
+        accepted, nxt = verify_sampled(self.logits[:T], tokens, batch.starts, self.u_accept, self.u_next,
                                        temperature=self.temperature, scratch=self.verify_ws)
         return accepted.tolist(), nxt.tolist()
