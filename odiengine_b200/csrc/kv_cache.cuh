@@ -23,17 +23,25 @@ struct KvView {
 
 // Checks a caller's cache descriptor; `who` opens the error message.
 int kv_view(const odi_cuda_kv_cache* c, KvView* v, const char* who);
-// Whether n rows of wa values, lda apart, share memory with n rows of wb, ldb apart.
-inline bool rows_overlap(const float* a, int64_t lda, int64_t wa, const float* b, int64_t ldb, int64_t wb, int64_t n) {
+// Whether n rows of wa bytes, lda apart, share memory with n rows of wb, ldb apart.
+inline bool byte_rows_overlap(const void* a, int64_t lda, int64_t wa, const void* b, int64_t ldb, int64_t wb, int64_t n) {
   const intptr_t A = (intptr_t)a, B = (intptr_t)b;
-  if (n < 1 || A + 4 * ((n - 1) * lda + wa) <= B || B + 4 * ((n - 1) * ldb + wb) <= A) return false;
+  if (n < 1 || A + (n - 1) * lda + wa <= B || B + (n - 1) * ldb + wb <= A) return false;
+  if (lda == ldb && lda > 0) {  // columns of one buffer: row j of b begins `at` bytes into row j + rows of a
+    const int64_t rows = (B - A >= 0 ? B - A : B - A - lda + 1) / lda, at = B - A - rows * lda;
+    return (at < wa && rows > -n && rows < n) || (lda - at < wb && rows + 1 > -n && rows + 1 < n);
+  }
   for (int64_t i = 0, j = 0; i < n && j < n;) {
-    const intptr_t x = A + 4 * i * lda, y = B + 4 * j * ldb;
-    if (x + 4 * wa <= y) ++i;
-    else if (y + 4 * wb <= x) ++j;
+    const intptr_t x = A + i * lda, y = B + j * ldb;
+    if (x + wa <= y) ++i;
+    else if (y + wb <= x) ++j;
     else return true;
   }
   return false;
+}
+// The same of fp32 rows, in values.
+inline bool rows_overlap(const float* a, int64_t lda, int64_t wa, const float* b, int64_t ldb, int64_t wb, int64_t n) {
+  return byte_rows_overlap(a, 4 * lda, 4 * wa, b, 4 * ldb, 4 * wb, n);
 }
 // A launch's status as the C ABI's.
 int kv_launched(cudaError_t e, const char* what);

@@ -177,9 +177,8 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
   if ((int64_t)tokens * rows > 0x7fffffffll)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append_paged: too many rows");
   if (!tokens) return ODI_CUDA_OK;
-  const uintptr_t x = (uintptr_t)d_qkv, x1 = x + 4 * (uintptr_t)((tokens - 1) * ld_qkv + rows * a.c.hd),
-                  y = (uintptr_t)d_q_out, y1 = y + 2 * (uintptr_t)((tokens - 1) * ld_q + (int64_t)heads * a.c.hd);
-  if (x < y1 && y < x1) return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append_paged: d_q_out overlaps d_qkv");
+  if (byte_rows_overlap(d_qkv, 4 * ld_qkv, 4 * rows * a.c.hd, d_q_out, 2 * ld_q, 2ll * heads * a.c.hd, tokens))
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append_paged: d_q_out overlaps d_qkv");
   a.turns.r = pow((double)theta, -2.0 / a.c.hd);
   double sq = a.c.hd == 128 ? a.turns.r * a.turns.r : a.turns.r;
   for (int k = 0; k < 5; ++k, sq *= sq) a.turns.square[k] = sq;

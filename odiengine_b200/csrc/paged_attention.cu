@@ -655,9 +655,9 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
                                                              batch->kv_heads, a.c.hd))
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: scratch too small");
   if (!tokens) return ODI_CUDA_OK;
-  const uintptr_t x = (uintptr_t)d_q, x1 = x + 2 * (uintptr_t)((tokens - 1) * ld_q + width), y = (uintptr_t)d_out,
-                  y1 = y + (out32 ? 4 : 2) * (uintptr_t)((tokens - 1) * ld_out + width);
-  if (x < y1 && y < x1) return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: d_out overlaps d_q");
+  const int64_t size = out32 ? 4 : 2;
+  if (byte_rows_overlap(d_q, 2 * ld_q, 2 * width, d_out, size * ld_out, size * width, tokens))
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: d_out overlaps d_q");
   a.q = d_q, a.ld_q = ld_q, a.out = d_out, a.ld_out = ld_out, a.out32 = out32;
   a.table = tables->table, a.max_pages = tables->max_pages;
   a.header = batch->work, a.max_items = (int)g.max_items;

@@ -198,3 +198,30 @@ def test_tables_narrower_than_the_steps(cuda_lib, new, nan):
         want, tol = paged_ref.attention(s.q[row:row + N], k, v, s.past[b], heads, 0.1)
         assert paged_ref.within(out[row:row + N], want, tol, out.dtype)
         row += N
+
+
+# ---- columns of one buffer -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new", [[2, 1], [50, 20]])
+def test_inputs_and_outputs_in_columns_of_one_buffer(cuda_lib, new):
+    """Rows that lie between one another without sharing a byte are no overlap."""
+    from odiengine_b200 import paged
+
+    heads, kv, hd, T = 4, 2, 64, sum(new)
+    s = Setup([100, 3], new, heads, kv, hd, "bf16", 32)
+    w = heads * hd
+    both = torch.full((T, 2 * w), math.nan, dtype=s.q.dtype, device="cuda")
+    for q, out in ((both[:, :w], both[:, w:]), (both[:, w:], both[:, :w])):
+        q.copy_(s.q)
+        paged.attention_paged(q, s.cache, s.tables, s.batch, out, scale=0.1, scratch=s.scratch)
+        assert torch.equal(q, s.q)
+        s.check(out, 0.1)
+    W = (heads + 2 * kv) * hd
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn((T, W), device="cuda", generator=g)
+    want = paged.qk_rope_append_paged(qkv, s.cache, s.batch, heads=heads, theta=1e4)
+    wide = torch.empty((T, W + w // 2), device="cuda")  # q as 16-bit values behind each row
+    wide[:, :W] = qkv
+    got = wide.view(torch.bfloat16)[:, 2 * W:]
+    paged.qk_rope_append_paged(wide[:, :W], s.cache, s.batch, got, heads=heads, theta=1e4)
+    assert torch.equal(got, want) and torch.equal(wide[:, :W], qkv)
