@@ -43,6 +43,10 @@ inline bool byte_rows_overlap(const void* a, int64_t lda, int64_t wa, const void
 inline bool rows_overlap(const float* a, int64_t lda, int64_t wa, const float* b, int64_t ldb, int64_t wb, int64_t n) {
   return byte_rows_overlap(a, 4 * lda, 4 * wa, b, 4 * ldb, 4 * wb, n);
 }
+// Whether two runs of bytes share memory; null pointers share none.
+inline bool bytes_overlap(const void* a, int64_t wa, const void* b, int64_t wb) {
+  return a && b && byte_rows_overlap(a, wa, wa, b, wb, wb, 1);
+}
 // A launch's status as the C ABI's.
 int kv_launched(cudaError_t e, const char* what);
 

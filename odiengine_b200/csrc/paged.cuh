@@ -20,6 +20,7 @@ struct PagedView {
   int dtype;  // ODI_CUDA_PAGED_F16 / ODI_CUDA_PAGED_BF16
   int kv_heads, hd, page_size, num_pages;
   int page_shift;
+  int64_t bytes() const { return 2ll * num_pages * kv_heads * page_size * hd; }  // of k, and of v
 };
 
 // How attention cuts a batch's rows: an item is up to `rows` of the new tokens *

@@ -179,6 +179,10 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
   if (!tokens) return ODI_CUDA_OK;
   if (byte_rows_overlap(d_qkv, 4 * ld_qkv, 4 * rows * a.c.hd, d_q_out, 2 * ld_q, 2ll * heads * a.c.hd, tokens))
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append_paged: d_q_out overlaps d_qkv");
+  const int64_t q_bytes = 2 * ((tokens - 1) * ld_q + (int64_t)heads * a.c.hd), qkv_bytes = 4 * ((tokens - 1) * ld_qkv + rows * a.c.hd);
+  for (const void* pool : {a.c.k, a.c.v})
+    if (bytes_overlap(d_q_out, q_bytes, pool, a.c.bytes()) || bytes_overlap(d_qkv, qkv_bytes, pool, a.c.bytes()))
+      return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "qk_rope_append_paged: d_q_out or d_qkv overlaps the cache");
   a.turns.r = pow((double)theta, -2.0 / a.c.hd);
   double sq = a.c.hd == 128 ? a.turns.r * a.turns.r : a.turns.r;
   for (int k = 0; k < 5; ++k, sq *= sq) a.turns.square[k] = sq;

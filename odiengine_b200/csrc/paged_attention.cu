@@ -658,6 +658,10 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
   const int64_t size = out32 ? 4 : 2;
   if (byte_rows_overlap(d_q, 2 * ld_q, 2 * width, d_out, size * ld_out, size * width, tokens))
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: d_out overlaps d_q");
+  const int64_t out_bytes = size * ((tokens - 1) * ld_out + width);
+  if (bytes_overlap(d_out, out_bytes, a.c.k, a.c.bytes()) || bytes_overlap(d_out, out_bytes, a.c.v, a.c.bytes()) ||
+      bytes_overlap(d_out, out_bytes, d_scratch, (int64_t)scratch_bytes) || bytes_overlap(d_out, out_bytes, d_slopes, 4ll * batch->heads))
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "attention_paged: d_out overlaps the cache, the slopes or the scratch");
   a.q = d_q, a.ld_q = ld_q, a.out = d_out, a.ld_out = ld_out, a.out32 = out32;
   a.table = tables->table, a.max_pages = tables->max_pages;
   a.header = batch->work, a.max_items = (int)g.max_items;

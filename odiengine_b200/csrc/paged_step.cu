@@ -339,6 +339,16 @@ int odi_cuda_paged_step(const odi_cuda_page_tables* t, const odi_cuda_paged_batc
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: page_size, max_pages or num_pages out of range");
   if (a.g.max_items * ((int64_t)t->max_pages * t->page_size / a.g.tile + 1 + a.g.extra) > 0x7fffffffll)
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: more work than 2^31 tiles");
+  // d_keep and d_new are read before lengths and rows are written, d_prefix after;
+  // pages are dropped beside all three
+  const int64_t B = t->requests, n = 4 * B;
+  for (const void* in : {d_keep, d_new, d_prefix})
+    if (bytes_overlap(in, n, t->table, n * t->max_pages) || bytes_overlap(in, n, t->free_pages, 4ll * t->num_pages))
+      return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: d_keep, d_new or d_prefix overlaps the tables");
+  if (bytes_overlap(d_prefix, n, t->lens, n) || bytes_overlap(d_prefix, n, t->free_count, 4) || bytes_overlap(d_prefix, n, batch->starts, n + 4) ||
+      bytes_overlap(d_prefix, n, batch->lens, n) || bytes_overlap(d_prefix, n, batch->positions, 4ll * batch->max_rows) ||
+      bytes_overlap(d_prefix, n, batch->slots, 4ll * batch->max_rows))
+    return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "paged_step: d_prefix overlaps what the step writes");
   a.t = *t, a.b = *batch, a.keep = d_keep, a.fresh = d_new, a.prefix = d_prefix, a.page_shift = page_shift_of(t->page_size);
   // one CTA where its threads see to everything in a few passes; else eight
   const bool small = t->requests <= 256 && batch->max_rows <= 1024;

@@ -428,6 +428,13 @@ int odi_cuda_verify_sampled(const float* d_logits, int64_t ld, const int32_t* d_
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "verify_sampled: misaligned buffer");
   if (scratch_bytes < odi_cuda_verify_scratch_bytes(rows, requests, V))
     return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "verify_sampled: scratch too small");
+  const int64_t n = 4ll * requests, logit_bytes = 4 * ((rows - 1) * ld + V), prob_bytes = 4 * ((rows - 1) * ld_probs + V);
+  for (const void* out : {d_accepted, d_next})
+    if (bytes_overlap(out, n, d_tokens, 4ll * rows) || bytes_overlap(out, n, d_starts, n + 4) || bytes_overlap(out, n, d_u_accept, 4ll * rows) ||
+        bytes_overlap(out, n, d_u_next, n) || bytes_overlap(out, n, d_logits, logit_bytes) || bytes_overlap(out, n, d_draft_probs, prob_bytes) ||
+        bytes_overlap(out, n, d_scratch, (int64_t)scratch_bytes))
+      return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "verify_sampled: an output overlaps what the call reads or its scratch");
+  if (bytes_overlap(d_accepted, n, d_next, n)) return set_error(ODI_CUDA_ERR_INVALID_ARGUMENT, "verify_sampled: the outputs overlap");
   VerifyArgs a{};
   a.logits = d_logits, a.ld = ld, a.tokens = d_tokens, a.starts = d_starts, a.probs = d_draft_probs, a.ld_p = ld_probs;
   a.u_accept = d_u_accept, a.u_next = d_u_next, a.accepted = d_accepted, a.next = d_next;
