@@ -586,7 +586,7 @@ typedef struct odi_cuda_paged_batch {
 
 /* Bits of a step's status; 0: every request got its rows. */
 enum {
-  ODI_CUDA_PAGED_NO_PAGES = 1,       /* refused: not enough free pages */
+  ODI_CUDA_PAGED_NO_PAGES = 1,       /* refused: not enough free pages, or not enough for one before it */
   ODI_CUDA_PAGED_TOO_LONG = 2,       /* refused: longer than max_pages pages */
   ODI_CUDA_PAGED_BAD_NEW = 4,        /* refused: new below 0 or above max_new */
   ODI_CUDA_PAGED_TOO_MANY_ROWS = 8,  /* refused: rows past max_rows */
@@ -602,7 +602,9 @@ size_t odi_cuda_paged_work_bytes(int requests, int max_rows, int max_new, int he
  * request that keeps 0 and takes 0 is over); a request whose pages are not
  * there is refused: it keeps what it kept, its rows have no slots, and
  * attention leaves its rows as they were.  Requests are served in their
- * order.  d_prefix (NULL: 0): the first d_prefix[b] positions see one another
+ * order: once one is refused for want of pages, so are those after it that
+ * need a page, though fewer would do for them; those that need none are
+ * served.  d_prefix (NULL: 0): the first d_prefix[b] positions see one another
  * both ways, once they are in the cache. */
 int odi_cuda_paged_step(const odi_cuda_page_tables* tables, const odi_cuda_paged_batch* batch, const int32_t* d_keep,
                         const int32_t* d_new, const int32_t* d_prefix, void* stream);

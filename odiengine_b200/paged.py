@@ -163,7 +163,9 @@ class PagedBatch:
 def paged_step(tables: PageTables, batch: PagedBatch, new, keep=None, prefix=None, stream=None) -> None:
     """Request b keeps keep[b] of its positions (None: all) and takes new[b]
     more (int32 [requests]); prefix[b] positions see one another both ways.
-    Tables and batch are brought up to date."""
+    Tables and batch are brought up to date.  Pages are handed out in the
+    requests' order: one that finds too few is refused (batch.status()), and with
+    it those after it that need any."""
     dev, B = tables.index, tables.requests
     if batch.index != dev:
         _apart("batch", batch, dev)

@@ -225,3 +225,30 @@ def test_inputs_and_outputs_in_columns_of_one_buffer(cuda_lib, new):
     got = wide.view(torch.bfloat16)[:, 2 * W:]
     paged.qk_rope_append_paged(wide[:, :W], s.cache, s.batch, got, heads=heads, theta=1e4)
     assert torch.equal(got, want) and torch.equal(wide[:, :W], qkv)
+
+
+# ---- who gets pages --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("B", [4, 300])
+def test_requests_behind_one_without_pages(cuda_lib, B):
+    """Five pages are free: the first request wants two, the second ten, and those after
+    it one each or none.  The second is refused and with it who needs a page."""
+    from odiengine_b200 import paged
+
+    P = 16
+    t = paged.PageTables.new(B, 12, 5 + B, P)
+    batch = paged.PagedBatch(t, max_rows=1000 if B == 4 else 6000, max_new=160, heads=2, kv_heads=2)
+    paged.paged_step(t, batch, ints([1 if b > 2 else 0 for b in range(B)]))
+    free = 5 + B - (B - 3)
+    t.free_count.fill_(5)
+    new = [2 * P, 10 * P, 1] + [P - 1 if b % 2 else P for b in range(3, B)]  # the odd ones' page is there
+    paged.paged_step(t, batch, ints(new))
+    assert batch.status() == paged.NO_PAGES and free >= 5
+    assert t.free_count.item() == 3
+    served = [b == 0 or b > 2 and b % 2 == 1 for b in range(B)]
+    had = [1 if b > 2 else 0 for b in range(B)]
+    assert batch.lens.tolist() == [had[b] + new[b] if served[b] else 0 for b in range(B)]
+    assert t.lens.tolist() == [had[b] + (new[b] if served[b] else 0) for b in range(B)]
+    starts, slots = batch.starts.tolist(), batch.slots.tolist()
+    for b in range(B):
+        assert all((s >= 0) == served[b] for s in slots[starts[b]:starts[b + 1]]) and starts[b + 1] - starts[b] == new[b]
