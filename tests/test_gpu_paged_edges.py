@@ -128,6 +128,37 @@ def test_distances_behind_16_million_positions(cuda_lib, new):
     assert cuda_lib_status(scratch) == 0
 
 
+@pytest.mark.parametrize("past,new,heads,kv,hd,P", [
+    ([40000], [1], 8, 1, 128, 128), ([30000, 70], [5, 1], 16, 2, 128, 16), ([9000], [3], 16, 2, 64, 32), ([20000], [16], 16, 2, 128, 64),
+    ([0, 4000], [1500, 129], 4, 4, 64, 16), ([8100], [300], 8, 1, 128, 128)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_every_tile_counts_once(cuda_lib, past, new, heads, kv, hd, P, dtype):
+    """Queries of zero weigh all positions alike, and a position's values are 1 in the
+    dim that its run of 16 has: the outputs count positions, exactly but for the division."""
+    from odiengine_b200 import paged
+
+    s = Setup(past, new, heads, kv, hd, dtype, P)
+    s.q.zero_()
+    s.cache.v.zero_()
+    for b in range(len(new)):
+        j = torch.arange(past[b] + new[b], device="cuda")
+        slot = s.tables.table[b].long()[j // P] * P + j % P
+        s.cache.v[slot // P, :, slot % P, j // 16 % hd] = 1.0
+    out = torch.empty(s.q.shape, dtype=torch.float32, device="cuda")
+    paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=0.1, scratch=s.scratch)
+    row = 0
+    for b, N in enumerate(new):
+        n = past[b] + N
+        ones = torch.zeros((n, hd), dtype=torch.float64)
+        ones[torch.arange(n), torch.arange(n) // 16 % hd] = 1.0
+        upto = torch.arange(past[b] + 1, n + 1)
+        want = ones.cumsum(0)[upto - 1] / upto[:, None]
+        got = out[row:row + N].cpu().double().view(N, heads, hd)
+        # a reciprocal and a product, each off by 2^-24; sums of whole numbers are exact
+        assert ((got - want[:, None]).abs() <= 2.0 ** -22 * want[:, None]).all()
+        row += N
+
+
 # ---- lanes that part ways ------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("past,new,heads,kv,hd", [([70], [45], 3, 3, 64), ([0, 130], [77, 40], 5, 1, 64), ([300], [260], 3, 3, 64),
