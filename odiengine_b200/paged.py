@@ -155,9 +155,11 @@ class PagedBatch:
                                     kv_heads, self.page_size)
         self._ref = ctypes.addressof(self._struct)
 
-    def status(self) -> int:
-        """The last step's status bits (NO_PAGES, ...); waits for it."""
-        return int(self.work[0].item())
+    def status(self, stream=None) -> int:
+        """The last step's status bits (NO_PAGES, ...).  `stream`: the step's, or one
+        that comes after it (default: the current one); the call waits for it."""
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            return int(self.work[0].item())
 
 
 def paged_step(tables: PageTables, batch: PagedBatch, new, keep=None, prefix=None, stream=None) -> None:

@@ -283,3 +283,20 @@ def test_requests_behind_one_without_pages(cuda_lib, B):
     starts, slots = batch.starts.tolist(), batch.slots.tolist()
     for b in range(B):
         assert all((s >= 0) == served[b] for s in slots[starts[b]:starts[b + 1]]) and starts[b + 1] - starts[b] == new[b]
+
+
+# ---- streams -----------------------------------------------------------------------------------------------------------
+
+def test_the_status_of_a_step_on_another_stream(cuda_lib):
+    """Read on the step's stream it is the step's, however late that runs."""
+    from odiengine_b200 import paged
+
+    t = paged.PageTables.new(2, 2, 3, 16)
+    batch = paged.PagedBatch(t, max_rows=64, max_new=32, heads=1, kv_heads=1)
+    side = torch.cuda.Stream()
+    new = ints([20, 20])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    paged.paged_step(t, batch, new, stream=side)
+    assert batch.status(side) == paged.NO_PAGES
