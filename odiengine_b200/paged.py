@@ -280,9 +280,9 @@ class PagedDecoder:
     that follow: those drafts that the target keeps, and one more.  With a
     temperature they are sampled (drafts are verified by verify_sampled, random
     numbers from `generator` or a generator of its own); without one greedy.  The
-    weights keep gate|up in [gate | up] order.  softcap, slopes: the model's
-    capped scores or distance biases.  Calls run on the current stream, which may
-    differ from call to call; one at a time."""
+    weights keep gate|up in [gate | up] order.  softcap, slopes: as
+    attention_paged has them, for scores of q and k that are rotated as always.  Calls
+    run on the current stream, which may differ from call to call; one at a time."""
 
     def __init__(self, cfg, weights, *, requests: int, num_pages: int, page_size: int = 16, dtype=torch.float16,
                  max_drafts: int = 7, chunk: int = 256, temperature=None, generator=None, softcap: float = 0.0, slopes=None,

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import paged_ref
-from oracle.llama import LlamaRef
+from oracle.llama import LlamaRef, rms_norm, rope
 from test_gpu_decode import _oracle_weights, _tiny
 from test_gpu_paged_decoder import TOL
 
@@ -74,4 +74,82 @@ def test_single_tokens_run_in_a_batch_of_single_tokens(cuda_lib, monkeypatch, te
             else:
                 assert out[b] == [*lists[b][1:1 + acc[i]], nxt[i]]
             refs[b][1].extend(lists[b][:len(out[b])])
+    assert d.status() == 0
+
+
+class OptionsRef(LlamaRef):
+    """LlamaRef with capped scores and distance biases; rows of the cache in its type."""
+
+    def __init__(self, cfg, W, softcap, slopes, dtype):
+        super().__init__(cfg, W)
+        self.softcap, self.slopes, self.dtype = softcap, slopes, dtype
+
+    def cached(self, x):
+        return torch.from_numpy(x).to(self.dtype).double().numpy()
+
+    def step(self, token, pos):
+        cfg, W = self.cfg, self.W
+        H, KV, hd, F = cfg.heads, cfg.kv_heads, cfg.head_dim, cfg.ffn
+        x = W["token_embd"][token].astype(np.float64)
+        for layer in range(cfg.layers):
+            qkv = W[f"wqkv.{layer}"] @ rms_norm(x, W[f"attn_norm.{layer}"], cfg.eps)
+            q, k, v = (qkv[a * hd:b * hd].reshape(-1, hd).copy() for a, b in ((0, H), (H, H + KV), (H + KV, H + 2 * KV)))
+            rope(q, pos, cfg.theta)
+            rope(k, pos, cfg.theta)
+            self.kc[layer, :, pos], self.vc[layer, :, pos] = self.cached(k), self.cached(v)
+            att = np.zeros((H, hd))
+            for h in range(H):
+                s = self.kc[layer, h * KV // H, :pos + 1] @ q[h] / np.sqrt(hd)
+                if self.softcap:
+                    s = self.softcap * np.tanh(s / self.softcap)
+                s = s - self.slopes[h] * np.arange(pos, -1, -1)
+                p = np.exp(s - s.max())
+                att[h] = p / p.sum() @ self.vc[layer, h * KV // H, :pos + 1]
+            x = x + W[f"wo.{layer}"] @ att.reshape(-1)
+            gu = W[f"wgu.{layer}"] @ rms_norm(x, W[f"ffn_norm.{layer}"], cfg.eps)
+            g, u = gu[:F], gu[F:]
+            x = x + W[f"wdown.{layer}"] @ (g / (1.0 + np.exp(-g)) * u)
+        return W["output"] @ rms_norm(x, W["out_norm"], cfg.eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("softcap,biased", [(0.3, False), (0.0, True), (0.5, True)])
+def test_capped_scores_and_distance_biases(cuda_lib, dtype, softcap, biased):
+    """Both come after the rotation; prompts in chunks, single tokens and drafts.  The
+    norms' weights are tripled, so that scores are about as large as the caps."""
+    from odiengine_b200.paged import PagedDecoder
+
+    cfg, mw = model(seed=11)
+    for lw in mw.layers:
+        lw.attn_norm.mul_(3)
+    slopes = 2.0 ** -np.arange(1, cfg.heads + 1, dtype=np.float64) if biased else np.zeros(cfg.heads)
+    refs = [OptionsRef(cfg, _oracle_weights(cuda_lib, cfg, mw), softcap, slopes, dtype) for _ in range(2)]
+    plain = LlamaRef(cfg, refs[0].W)
+    d = PagedDecoder(cfg, mw, requests=2, num_pages=8, dtype=dtype, max_drafts=3, chunk=20, softcap=softcap,
+                     slopes=torch.tensor(slopes, dtype=torch.float32, device="cuda") if biased else None)
+    rng = np.random.default_rng(2)
+    prompts = [rng.integers(0, cfg.vocab, n).tolist() for n in (30, 4)]
+    for p in prompts:
+        d.add(p)
+    while d.left(0) or d.left(1):
+        d.step()
+    toks = [p[:-1] for p in prompts]
+    for b in range(2):
+        assert d._len[b] == len(toks[b])
+        for i, t in enumerate(toks[b]):
+            refs[b].step(t, i)
+            if b == 0:
+                plain.step(t, i)
+    for drafts in ({}, {0: [5, 6, 7], 1: [8]}):
+        fed = [[d._todo[b][0], *drafts.get(b, ())] for b in range(2)]
+        out, row = d.step(drafts), 0
+        for b in range(2):
+            want = np.stack([refs[b].step(t, len(toks[b]) + i) for i, t in enumerate(fed[b])])
+            got = d.logits[row:row + len(fed[b])].cpu().numpy().astype(np.float64)
+            row += len(fed[b])
+            assert np.abs(got - want).max() <= TOL[dtype] * np.abs(want).max(), np.abs(got - want).max() / np.abs(want).max()
+            if b == 0 and not drafts:  # the options do something
+                other = plain.step(fed[0][0], len(toks[0]))
+                assert np.abs(other - want[0]).max() > 3 * TOL[dtype] * np.abs(want).max()
+            toks[b] = toks[b] + fed[b][:len(out[b])]
     assert d.status() == 0
