@@ -628,7 +628,10 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
  * both 4-byte aligned, and they may not overlap.  tokens: rows that d_q and
  * d_out have.  Rows behind the batch's last, and of refused requests, are
  * left as they were.  A row all of whose scores are -inf is zero.  Scores,
- * softmax and sums are fp32; the weights are rounded to the cache's type.
+ * softmax and sums are fp32.  The weights are rounded to the cache's type (in
+ * fp16 also to 2^-32 of the row's largest, whichever is more); for an fp32
+ * output they are sums of two parts of that type, off by 2^-20 of them, in
+ * bf16 by 2^-16.
  * scale is positive; softcap is at most 1024 (a capped score is off by 2^-21
  * of the cap at most).
  * Scratch: odi_cuda_attention_paged_scratch_bytes, 16-byte aligned, zero

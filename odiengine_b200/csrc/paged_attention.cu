@@ -23,9 +23,12 @@
 // to the cache's type, relative to a reference that moves only when a weight
 // would pass 2^8 of it; their sum is taken before the rounding.  That is half a step of
 // the type per weight, independent from weight to weight, so that the sum of many is
-// off by less than the rounding of an output of that type; of an fp32 output it is the
-// whole error.  fp16's steps end: what a row's largest weight outweighs 2^31 times
-// has no weight, which is off by 2^-32 of the largest per position at most.
+// off by less than the rounding of an output of that type.  fp16's steps end: what a
+// row's largest weight outweighs 2^31 times has no weight, which is off by 2^-32 of the
+// largest per position at most.  For an fp32 output the weights are sums of two parts,
+// and the second product is made twice: 64 requests with bf16 caches are off by 5e-6 of
+// the output's norm, 1.6e-3 with one part.  Where HBM is the bound that costs nothing;
+// 512 short requests take 91 us, 78 with one part, 16 with drafts and a cap 60 and 55.
 #include <cstdio>
 
 #include "paged_attention.cuh"
@@ -81,7 +84,7 @@ struct Cfg {
 constexpr int ND = 3;
 constexpr int JOINERS = 96;  // threads that join and write out
 
-template <typename T, int HD, int MG, bool FANCY>
+template <typename T, int HD, int MG, bool FANCY, bool OUT32>
 __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     paged_mma_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap) {
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
       const int R = p.it.i * ROWS + r, token = pa_token(a, R);
       const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)(p.kvh * a.G + R - token * a.G) * HD + d;
-      if (a.out32) {
+      if (OUT32) {
         float* y = static_cast<float*>(a.out) + at;
         if (a.vec_out) *reinterpret_cast<float4*>(y) = v;
         else y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       const int pw = t * TILE + wq * 16;  // the warp's first position
       const bool masked = pw + 16 > least;
       if (!wait(&full[sk], n / ST)) return;
-      uint32_t pf[4];
+      uint32_t pf[4], pr[4];  // weights, and what their rounding left
       if (live_group) {
         __syncwarp();  // ldmatrix and mma want whole warps, and a wait may let lanes go one by one
         // ---- S = Q K^T
@@ -446,8 +449,8 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
             w[i] = pa_ex2(sc[i >> 1][2 * e + (i & 1)] - ref);
             l[e] += w[i];
           }
-          pf[e] = H::pack(w[0], w[1]);
-          pf[2 + e] = H::pack(w[2], w[3]);
+          pf[e] = OUT32 ? H::split(make_float2(w[0], w[1]), pr[e]) : H::pack(w[0], w[1]);
+          pf[2 + e] = OUT32 ? H::split(make_float2(w[2], w[3]), pr[2 + e]) : H::pack(w[2], w[3]);
         }
       } else if (lane == 0) {
         mbar_arrive(&empty[sk]);
@@ -496,6 +499,13 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
             mma<T>(o[2 * (d0 + dt)], pf, b[dt][0], b[dt][1]);
             mma<T>(o[2 * (d0 + dt) + 1], pf, b[dt][2], b[dt][3]);
           }
+          if (OUT32) {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+              mma<T>(o[2 * (d0 + dt)], pr, b[dt][0], b[dt][1]);
+              mma<T>(o[2 * (d0 + dt) + 1], pr, b[dt][2], b[dt][3]);
+            }
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -510,7 +520,7 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
       for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-        if (c == 0) wml[warp][e * 8 + g] = make_float2(m[e], l[e]);
+        if (c == 0) wml[warp][e * 8 + g] = make_float2(m[e], OUT32 ? l[e] * H::PARTS : l[e]);
         // 8-dim blocks in an order of the row's own, so that no two rows meet in a bank
 #pragma unroll
         for (int d = 0; d < HD / 8; ++d)
@@ -524,10 +534,10 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
   }
 }
 
-template <typename T, int HD, int MG, bool FANCY>
+template <typename T, int HD, int MG, bool FANCY, bool OUT32>
 static cudaError_t launch(PagedAttnArgs& a, cudaStream_t s) {
   using F = Cfg<HD, MG>;
-  auto kern = paged_mma_kernel<T, HD, MG, FANCY>;
+  auto kern = paged_mma_kernel<T, HD, MG, FANCY, OUT32>;
   CUtensorMap maps[2];
   if (cudaError_t e = paged_maps(a.c, TILE, true, maps)) return e;
   static PagedReady ready;
@@ -589,12 +599,14 @@ cudaError_t paged_q_map(const PagedAttnArgs& a, int tokens, CUtensorMap* map) {
 
 cudaError_t launch_paged_mma(PagedAttnArgs& a, int groups, bool fancy, cudaStream_t s) {
   const bool bf = a.c.dtype == ODI_CUDA_PAGED_BF16;
-  auto by_rows = [&](auto t, auto hd) {
+  auto by_out = [&](auto t, auto hd, auto out) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
-    if (groups == 1) return fancy ? pmma::launch<T, HD, 1, true>(a, s) : pmma::launch<T, HD, 1, false>(a, s);
-    return fancy ? pmma::launch<T, HD, 2, true>(a, s) : pmma::launch<T, HD, 2, false>(a, s);
+    constexpr bool OUT32 = decltype(out)::value;
+    if (groups == 1) return fancy ? pmma::launch<T, HD, 1, true, OUT32>(a, s) : pmma::launch<T, HD, 1, false, OUT32>(a, s);
+    return fancy ? pmma::launch<T, HD, 2, true, OUT32>(a, s) : pmma::launch<T, HD, 2, false, OUT32>(a, s);
   };
+  auto by_rows = [&](auto t, auto hd) { return a.out32 ? by_out(t, hd, std::true_type{}) : by_out(t, hd, std::false_type{}); };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;
   if (a.c.hd == 128) return bf ? by_rows(__nv_bfloat16{}, D128{}) : by_rows(__half{}, D128{});

@@ -85,6 +85,19 @@ struct Half16<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float up(uint16_t x) { return __half2float(__ushort_as_half(x)); }
+  // Two weights as a sum of two parts each, to 2^-20 of them (or half of 2^-24).  The first
+  // is cut off, not rounded, and the last bit of the second is set where the first is
+  // not 0: neither is negative and no part of a weight is 0, or an infinity of V's would
+  // become a NaN.
+  static constexpr float PARTS = 1.f;  // what the parts' sum is of the weight
+  static __device__ __forceinline__ uint32_t split(float2 x, uint32_t& rest) {
+    uint32_t y;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(x.y), "f"(x.x));
+    const __half2 h = *reinterpret_cast<const __half2*>(&y);
+    const float2 r = __ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), x);
+    rest = pack(r.x, r.y) | (__hne2_mask(h, __half2half2(__ushort_as_half(0))) & 0x00010001u);
+    return y;
+  }
   // Pairs: 0 * x + y, NaN where x is not finite.
   static __device__ __forceinline__ uint32_t times0(uint32_t x, uint32_t y) {
     const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0)), *reinterpret_cast<const __half2*>(&y));
@@ -101,6 +114,15 @@ struct Half16<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float up(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+  // To 2^-16 of them; the second part is not 0 because the sum is a little more than the weight.
+  static constexpr float PARTS = 1.f + 0x1p-17f;
+  static __device__ __forceinline__ uint32_t split(float2 x, uint32_t& rest) {
+    uint32_t y;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(x.y), "f"(x.x));
+    const float2 r = __ffma2_rn(x, make_float2(PARTS, PARTS), make_float2(-__uint_as_float(y << 16), -__uint_as_float(y & 0xffff0000u)));
+    rest = pack(r.x, r.y);
+    return y;
+  }
   static __device__ __forceinline__ uint32_t times0(uint32_t x, uint32_t y) {
     const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __bfloat162bfloat162(__ushort_as_bfloat16(0)),
                                      *reinterpret_cast<const __nv_bfloat162*>(&y));

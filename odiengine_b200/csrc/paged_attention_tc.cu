@@ -29,6 +29,10 @@
 // prompts of 333 to 1200 tokens of 32/32 heads of 64 dims with biases 91, without 67;
 // 16 tokens over 30,000 positions 55.
 //
+// An fp32 output takes the weights as two 16-bit parts, the second where the other half
+// of S was, and a second product: 2048 tokens over 14,001 positions 1190 us, 970 with
+// one part, alone 112 and 105 (off by 5e-6 of the output's norm, 1.4e-3 with one).
+//
 // Every wait is bounded; a role whose wait gives up sets the error word and
 // leaves its loop, and the CTA ends at one barrier that every role reaches.
 #include "paged_attention.cuh"
@@ -179,7 +183,7 @@ struct Bars {
   uint64_t d_full[2], d_empty[2], join, drain[2];
 };
 
-template <typename T, int HD, int MODE, int NH>
+template <typename T, int HD, int MODE, int NH, bool OUT32>
 __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
     paged_tc_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap) {
@@ -331,6 +335,10 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
             const uint64_t v = desc(ring + nv % ST * F::SLOT, F::PLANE);
 #pragma unroll
             for (int ks = 0; ks < TILE / 16; ++ks) mma_ts(o_col, s_col + b * 64 + ks * 8, v + ks * (2048 >> 4), ID_O, i > first || ks > 0);
+            if (OUT32) {
+#pragma unroll
+              for (int ks = 0; ks < TILE / 16; ++ks) mma_ts(o_col, s_col + b * 64 + 32 + ks * 8, v + ks * (2048 >> 4), ID_O, 1);
+            }
             commit(&bars.pv_done[h][b]);
             commit(&bars.empty[nv % ST]);
           }
@@ -522,6 +530,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
         const float2 sc2 = make_float2(scale, scale), nr2 = make_float2(nref, nref);
         // eight pairs at a time, sums and packing one group behind
         float2 w[2][8];
+        uint32_t rest[OUT32 ? 32 : 1];  // what the rounding of the weights left
 #pragma unroll
         for (int g = 0; g <= 4; ++g) {
           if (g < 4) {
@@ -538,11 +547,13 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
             for (int e = 0; e < 8; ++e) {
               const float2 v = w[(g - 1) & 1][e];
               sum[e & 1] = __fadd2_rn(sum[e & 1], v);
-              s[8 * (g - 1) + e] = H::pack(v.x, v.y);
+              if constexpr (OUT32) s[8 * (g - 1) + e] = H::split(v, rest[8 * (g - 1) + e]);
+              else s[8 * (g - 1) + e] = H::pack(v.x, v.y);
             }
           }
         }
         st32(s, s_addr);
+        if constexpr (OUT32) st32(rest, s_addr + 32);
         wait_st();
         if (t >= t1 - clean && (NH == 1 || h == (t < d.end[1] ? 1 : 0))) {
           // the last half at work takes what is not finite out of V: thread = position, half its dims
@@ -590,7 +601,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
       if (!ok) break;
       __syncwarp();
       fence_after();
-      const float L = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      const float L = ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) * (OUT32 ? H::PARTS : 1.f);
       const bool whole = t0 == 0 && t1 == p.it.tiles, fix = p.poison != 0;
       constexpr int STRIDE = ROWS * (HD + 2);
       float* part = piece_part(a, p, blockIdx.x, STRIDE);
@@ -609,7 +620,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
           const int64_t at = __shfl_sync(0xffffffffu, out_at, r) + c;
           const bool some = __shfl_sync(0xffffffffu, out_row, r);
           const uint4 x = *chunk(r, ch);
-          uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (at << (a.out32 ? 2 : 1))) + ch * 4;
+          uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.out) + (at << (OUT32 ? 2 : 1))) + ch * 4;
           if (!some) continue;
           if (a.vec_out) *reinterpret_cast<uint4*>(y) = x;
           else y[0] = x.x, y[1] = x.y, y[2] = x.z, y[3] = x.w;
@@ -620,7 +631,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
         if constexpr (F::STAGE == 0) {
           if (row >= rows) return;
         const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)head * HD + c;
-        if (a.out32) {
+        if (OUT32) {
           float* y = static_cast<float*>(a.out) + at;
           if (a.vec_out) {
 #pragma unroll
@@ -646,7 +657,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
         }
           return;
         }
-        if (a.out32) {
+        if (OUT32) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             *chunk(lane, e) = make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]),
@@ -776,10 +787,10 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
   }
 }
 
-template <typename T, int HD, int MODE, int NH>
+template <typename T, int HD, int MODE, int NH, bool OUT32>
 static cudaError_t launch(PagedAttnArgs& a, cudaStream_t s) {
   using F = Cfg<HD, NH>;
-  auto kern = paged_tc_kernel<T, HD, MODE, NH>;
+  auto kern = paged_tc_kernel<T, HD, MODE, NH, OUT32>;
   CUtensorMap maps[3];
   if (cudaError_t e = paged_maps(a.c, TILE, false, maps)) return e;
   // whole tokens of a group: boxes of 64 dims, G heads, 128 / G tokens
@@ -798,13 +809,19 @@ cudaError_t launch_paged_tc(PagedAttnArgs& a, int rows, cudaStream_t s) {
   using namespace ptc;
   static_assert(Cfg<128, 2>::ROWS == PAGED_ROWS_MAX, "the scratch's pieces");
   const int mode = a.cap_log2 != 0.f ? CAP : a.slopes ? BIAS : PLAIN;
-  auto by_mode = [&](auto t, auto hd, auto nh) {
+  auto by_mode = [&](auto t, auto hd, auto nh, auto out) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value, NH = decltype(nh)::value;
-    return mode == CAP ? launch<T, HD, CAP, NH>(a, s) : mode == BIAS ? launch<T, HD, BIAS, NH>(a, s) : launch<T, HD, PLAIN, NH>(a, s);
+    constexpr bool OUT32 = decltype(out)::value;
+    return mode == CAP    ? launch<T, HD, CAP, NH, OUT32>(a, s)
+           : mode == BIAS ? launch<T, HD, BIAS, NH, OUT32>(a, s)
+                          : launch<T, HD, PLAIN, NH, OUT32>(a, s);
+  };
+  auto by_out = [&](auto t, auto hd, auto nh) {
+    return a.out32 ? by_mode(t, hd, nh, std::true_type{}) : by_mode(t, hd, nh, std::false_type{});
   };
   auto by_rows = [&](auto t, auto hd) {
-    return rows == HALF_ROWS ? by_mode(t, hd, std::integral_constant<int, 1>{}) : by_mode(t, hd, std::integral_constant<int, 2>{});
+    return rows == HALF_ROWS ? by_out(t, hd, std::integral_constant<int, 1>{}) : by_out(t, hd, std::integral_constant<int, 2>{});
   };
   using D64 = std::integral_constant<int, 64>;
   using D128 = std::integral_constant<int, 128>;

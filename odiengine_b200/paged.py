@@ -212,7 +212,8 @@ def attention_paged(q, cache: PagedCache, tables: PageTables, batch: PagedBatch,
     head_dim]) over their requests' positions: those up to a row's own, and its
     request's prefix.  softcap: scores are capped by softcap * tanh(s /
     softcap); slopes fp32 [heads]: scores lose slope * distance.  out: of the
-    cache's type (the default) or fp32; rows behind the batch's last are left."""
+    cache's type (the default), with softmax weights of that type, or fp32, with
+    weights of twice its bits; rows behind the batch's last are left."""
     dev, w = cache.index, batch.heads * cache.head_dim
     if tables.index != dev:
         _apart("tables", tables, dev)

@@ -98,6 +98,80 @@ def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats
     assert cuda_lib_status(s.scratch) == 0
 
 
+def close_attention(s, b, row, scale, softcap=0.0, slopes=None):
+    """Request b in 64 bits, and how far an fp32 output may be off.  A weight is off by the
+    square of half a step of its type (two parts, each rounded), fp16's smallest steps
+    (2^-32 of the row's largest), 2^-20 and its score's error; a sum by a step of fp32 per
+    product of 16 positions, of which each part makes one."""
+    past, N = s.past[b], s.new[b]
+    n, half = past + N, torch.finfo(s.cache.dtype).eps / 2
+    q, k, v = (t.cpu().double() for t in (s.q[row:row + N], s.rows(s.cache.k, b), s.rows(s.cache.v, b)))
+    x = q.view(N, s.kv, s.heads // s.kv, s.hd)
+    far = (torch.arange(past, n)[:, None] - torch.arange(n)[None])[:, None, None].double()
+    sc = torch.einsum("tkgd,knd->tkgn", x, k) * scale
+    ds = torch.einsum("tkgd,knd->tkgn", x.abs(), k.abs()) * scale * 2.0 ** -21
+    if softcap:
+        sc, ds = softcap * torch.tanh(sc / softcap), ds + softcap * 2.0 ** -21
+    if slopes is not None:
+        bias = slopes.cpu().double().view(1, s.kv, -1, 1) * far.abs()
+        sc, ds = sc - bias, ds + (bias + (sc - bias).abs()) * 2.0 ** -23
+    sc = sc.masked_fill(far < 0, -math.inf)
+    p = torch.exp(sc - sc.amax(-1, keepdim=True))
+    ds = ds.masked_fill(far < 0, 0.0)
+    l = p.sum(-1, keepdim=True)
+    want = torch.einsum("tkgn,knd->tkgd", p, v) / l
+    rel = half * half + 2.0 ** -20 + 2 * (n // 16 + 8) * 2.0 ** -23
+    tiny = 2.0 ** -32 * (far >= 0).double().expand_as(p) if s.cache.dtype is torch.float16 else 0.0
+    tol = torch.einsum("tkgn,knd->tkgd", p * (rel + ds) + tiny, v.abs()) / l
+    return want.reshape(N, -1), (tol + want.abs() * ((p * (ds + rel)).sum(-1, keepdim=True) / l)).reshape(N, -1)
+
+
+@pytest.mark.parametrize("past,new,heads,kv,hd,P", [
+    ([99], [1], 4, 4, 128, 16), ([150, 3, 0], [1, 1, 1], 8, 1, 64, 32), ([120, 40], [3, 2], 16, 2, 128, 16), ([100, 0], [90, 200], 4, 2, 128, 64),
+    ([0, 33], [129, 40], 8, 1, 64, 16), ([60], [300], 3, 3, 64, 128)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("option", ["plain", "cap", "slopes", "both"])
+def test_an_fp32_output_is_more_than_16_bits(cuda_lib, past, new, heads, kv, hd, P, dtype, option):
+    """Weights enter in two parts, so that what an fp32 output is off by is not their
+    rounding to the cache's type."""
+    from odiengine_b200 import paged
+
+    s = Setup(past, new, heads, kv, hd, dtype, P)
+    slopes = torch.linspace(0.01, 0.3, heads, device="cuda") if option in ("slopes", "both") else None
+    cap, scale = 3.0 if option in ("cap", "both") else 0.0, 1 / math.sqrt(hd)
+    out = torch.empty(s.q.shape, dtype=torch.float32, device="cuda")
+    paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=scale, softcap=cap, slopes=slopes, scratch=s.scratch)
+    row = 0
+    for b, N in enumerate(new):
+        want, tol = close_attention(s, b, row, scale, cap, slopes)
+        off = (out[row:row + N].cpu().double() - want).abs()
+        assert (off <= tol).all(), (b, off.max(), (off / tol).max())
+        row += N
+    assert cuda_lib_status(s.scratch) == 0
+
+
+@pytest.mark.parametrize("past,new,heads,kv,hd", [([200], [1], 4, 4, 128), ([300], [3], 8, 1, 64), ([150], [70], 4, 2, 128), ([200], [129], 3, 3, 64)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("out32", [False, True])
+@pytest.mark.parametrize("even", [False, True])
+def test_infinities_that_all_rows_see(cuda_lib, past, new, heads, kv, hd, dtype, out32, even):
+    """Infinite values of positions that every row sees stay infinities of their sign, and
+    both signs a NaN: also where all weights are powers of two (queries of zero), which
+    one 16-bit part holds whole."""
+    from odiengine_b200 import paged
+
+    s = Setup(past, new, heads, kv, hd, dtype, 32)
+    if even:
+        s.q.zero_()
+    for j, d, x in ((0, 1, math.inf), (40, 2, -math.inf), (99, 3, math.inf), (100, 3, -math.inf), (140, 5, math.inf), (141, 5, math.inf)):
+        slot = int(s.tables.table[0, j // 32]) * 32 + j % 32
+        s.cache.v[slot // 32, :, slot % 32, d] = x
+    out = torch.empty(s.q.shape, dtype=torch.float32 if out32 else s.q.dtype, device="cuda")
+    paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=0.1, scratch=s.scratch)
+    s.check(out, 0.1)
+    assert cuda_lib_status(s.scratch) == 0
+
+
 @pytest.mark.parametrize("new", [[1], [3], [40]])
 def test_distances_behind_16_million_positions(cuda_lib, new):
     """Distances count whole positions where fp32 no longer tells two neighbouring
