@@ -187,8 +187,9 @@ __global__ void __launch_bounds__(Cfg<HD, MG>::THREADS, Cfg<HD, MG>::PER_SM)
     const bool whole = t0 == 0 && t1 == p.it.tiles;
     constexpr int STRIDE = ROWS * (HD + 2);
     float* part = piece_part(a, p, blockIdx.x, STRIDE);
-    // a row's value divided by its sum, to where it goes
+    // a row's value divided by its sum, to where it goes; nothing that weighs nothing
     auto store = [&](int r, int d, float4 v, float inv) {
+      if (inv == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
       v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
       const int R = p.it.i * ROWS + r, token = pa_token(a, R);
       const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)(p.kvh * a.G + R - token * a.G) * HD + d;

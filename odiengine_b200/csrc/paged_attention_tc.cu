@@ -630,31 +630,31 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
       auto store = [&](const float (&v)[16], int c) {
         if constexpr (F::STAGE == 0) {
           if (row >= rows) return;
-        const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)head * HD + c;
-        if (OUT32) {
-          float* y = static_cast<float*>(a.out) + at;
-          if (a.vec_out) {
+          const int64_t at = (int64_t)(p.it.start + token) * a.ld_out + (int64_t)head * HD + c;
+          if (OUT32) {
+            float* y = static_cast<float*>(a.out) + at;
+            if (a.vec_out) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              reinterpret_cast<float4*>(y)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+              for (int e = 0; e < 4; ++e)
+                reinterpret_cast<float4*>(y)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) y[e] = v[e];
+            }
           } else {
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = v[e];
+            for (int e = 0; e < 8; ++e) w[e] = H::pack(v[2 * e], v[2 * e + 1]);
+            uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at);
+            if (a.vec_out) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                reinterpret_cast<uint4*>(y)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = w[e];
+            }
           }
-        } else {
-          uint32_t w[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = H::pack(v[2 * e], v[2 * e + 1]);
-          uint32_t* y = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at);
-          if (a.vec_out) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              reinterpret_cast<uint4*>(y)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = w[e];
-          }
-        }
           return;
         }
         if (OUT32) {
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
             }
           if (whole) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] *= inv;
+            for (int e = 0; e < 16; ++e) v[e] = inv == 0.f ? 0.f : v[e] * inv;  // nothing that weighs nothing
             store(v, c);
           } else {
 #pragma unroll
@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(Cfg<HD, NH>::THREADS, Cfg<HD, NH>::PER_SM)
                 for (int g = 0; g < 32; g += 16) {
                   float y[16];
 #pragma unroll
-                  for (int e = 0; e < 16; ++e) y[e] = v[g + e] * inv;
+                  for (int e = 0; e < 16; ++e) y[e] = inv == 0.f ? 0.f : v[g + e] * inv;
                   store(y, d0 + g);
                 }
               } else {  // in its first piece's place, whose row no other thread reads

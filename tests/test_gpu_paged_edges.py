@@ -172,6 +172,32 @@ def test_infinities_that_all_rows_see(cuda_lib, past, new, heads, kv, hd, dtype,
     assert cuda_lib_status(s.scratch) == 0
 
 
+@pytest.mark.parametrize("past,new,heads,kv,hd", [([200], [1], 4, 4, 128), ([3000], [2], 8, 1, 64), ([150], [70], 4, 2, 128), ([2000], [129], 3, 3, 64)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("out32", [False, True])
+@pytest.mark.parametrize("values", ["finite", "inf", "nan"])
+def test_rows_all_of_whose_scores_are_minus_infinity_are_zero(cuda_lib, past, new, heads, kv, hd, dtype, out32, values):
+    """Keys of -inf in one dim that the first head's queries look at and the others' do not;
+    whatever values stand there."""
+    from odiengine_b200 import paged
+
+    s = Setup(past, new, heads, kv, hd, dtype, 64)
+    T, G = sum(new), heads // kv
+    q = s.q.view(T, kv, G, hd)
+    s.cache.k[..., 7] = -math.inf
+    q[..., 7] = 0.0  # 0 * -inf is NaN: the other heads' queries see NaN
+    q[:, :, 0, 7] = 2.0
+    if values != "finite":
+        slot = int(s.tables.table[0, 1]) * 64 + 5
+        s.cache.v[slot // 64, :, slot % 64, 3] = math.inf if values == "inf" else math.nan
+    out = torch.full(s.q.shape, 9.0, dtype=torch.float32 if out32 else s.q.dtype, device="cuda")
+    paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=0.1, scratch=s.scratch)
+    got = out.view(T, kv, G, hd)
+    assert (got[:, :, 0] == 0).all()
+    assert G == 1 or torch.isnan(got[:, :, 1:]).all()
+    assert cuda_lib_status(s.scratch) == 0
+
+
 @pytest.mark.parametrize("new", [[1], [3], [40]])
 def test_distances_behind_16_million_positions(cuda_lib, new):
     """Distances count whole positions where fp32 no longer tells two neighbouring
