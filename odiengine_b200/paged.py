@@ -250,6 +250,8 @@ def verify_sampled(logits, tokens, starts, u_accept, u_next, accepted=None, next
     draft_probs fp32 [rows, V] (None: 1).  Returns accepted and next (int32
     [requests]): drafts kept, and the token after them, drawn with u_next."""
     dev, f32, i32 = logits.get_device(), torch.float32, torch.int32
+    if logits.dim() != 2 or starts.numel() < 2:
+        raise ValueError(f"verify_sampled: logits [rows, V] and starts [requests + 1] wanted, got {tuple(logits.shape)} and {tuple(starts.shape)}")
     R, V = logits.shape
     B = starts.numel() - 1
     ld = _rows2(logits, f32, "logits", dev, R, V)

@@ -82,3 +82,10 @@ def test_a_decoder_refuses_weights_of_another_device():
     w = ModelWeights(token_embd=z(10, 4, on=0))
     with pytest.raises(ValueError, match="cuda:1"):
         paged.PagedDecoder(None, w, requests=1, num_pages=1, device="cuda:1")
+
+
+@pytest.mark.parametrize("logits,starts", [((5,), 3), ((5, 7, 1), 3), ((5, 7), 0), ((5, 7), 1)])
+def test_verify_refuses_logits_or_starts_of_no_shape(calls, logits, starts):
+    with pytest.raises(ValueError, match="wanted"):
+        paged.verify_sampled(z(*logits), z(5, dtype=I32), z(starts, dtype=I32), z(5), z(2), scratch=z(8, dtype=torch.uint8))
+    assert not calls
