@@ -15,9 +15,10 @@
 // 64 requests of one token, 64/8 heads of 128 dims over 300 to 8,100 positions: 183 us,
 // 6.3 TB/s.  Where requests are short or few, latency is the bound: a tile takes a warp
 // about 1 us, an item some 2 us beside its tiles (its queries' way from memory, the
-// join); 512 such requests over up to 200 positions take 70 us, HBM would 32; one token
-// of 32 heads over 518 positions 9.6 us.  17 to 32 rows leave one CTA per SM: 16
-// requests of 2 to 5 tokens with a cap 55 us, 49 without, HBM 29.
+// join); 512 such requests over up to 200 positions take 69 us, HBM would 32; one token
+// of 32 heads over 518 positions 9.5 us.  17 to 32 rows leave one CTA per SM, whose
+// second group of warps has no row where a request has 16 or fewer (the width is the
+// batch's): 16 requests of 2 to 5 tokens with a cap 56 us, 52 without, HBM 29.
 //
 // q . k and o are summed in fp32.  The weights enter the second product rounded
 // to the cache's type, relative to a reference that moves only when a weight

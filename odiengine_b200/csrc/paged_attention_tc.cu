@@ -20,17 +20,17 @@
 // reference of a row moves only when a weight would pass 2^8, so O is rescaled a few
 // times per row.
 //
-// 2048 tokens of 64/8 heads over 14,001 positions: 940 to 1000 us, 1.0 to 1.07 PFLOP/s,
-// at 1.6 GHz under the 1 kW power cap; 2048 over 4000 303 us, with distance biases 350,
-// with a cap 605 (its second exponential and a reciprocal per score).  What bounds it
+// 2048 tokens of 64/8 heads over 14,001 positions: 955 to 980 us, 1.03 to 1.05 PFLOP/s,
+// at 1.6 GHz under the 1 kW power cap; 2048 over 4000 301 us, with distance biases 352,
+// with a cap 610 (its second exponential and a reciprocal per score).  What bounds it
 // is the softmax: a step of 64 positions takes 0.9 to 1.3 us, of which the products
 // are half.  An item takes another 4 to 5 us (queries, first scores, epilogue), a
-// piece of one that is cut as much again for its join: 2048 tokens alone 92 us, seven
+// piece of one that is cut as much again for its join: 2048 tokens alone 90 us, seven
 // prompts of 333 to 1200 tokens of 32/32 heads of 64 dims with biases 91, without 67;
 // 16 tokens over 30,000 positions 55.
 //
 // An fp32 output takes the weights as two 16-bit parts, the second where the other half
-// of S was, and a second product: 2048 tokens over 14,001 positions 1190 us, 970 with
+// of S was, and a second product: 2048 tokens over 14,001 positions 1190 us, 977 with
 // one part, alone 112 and 105 (off by 5e-6 of the output's norm, 1.4e-3 with one).
 //
 // Every wait is bounded; a role whose wait gives up sets the error word and
