@@ -630,7 +630,7 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
  * left as they were.  A row all of whose scores are -inf is zero.  Scores,
  * softmax and sums are fp32.  The weights are rounded to the cache's type (in
  * fp16 also to 2^-32 of the row's largest, whichever is more); for an fp32
- * output they are sums of two parts of that type, off by 2^-20 of them, in
+ * output they are sums of two parts of that type, off by 2^-19 of them, in
  * bf16 by 2^-16.
  * scale is positive; softcap is at most 1024 (a capped score is off by 2^-21
  * of the cap at most).
@@ -657,9 +657,9 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
  * 0) of the row that refused (from p if that is 0 everywhere), or from p of
  * the last row: the first id whose running sum is over u_next times the
  * whole.  Random numbers are in [0, 1).  A draft outside the vocabulary is
- * refused.  -inf logits have no weight, +inf ones share it all; a row with a
- * NaN or with no finite logit keeps no draft and gives -1, as does a request
- * without rows.  In 64 bits throughout.
+ * refused.  -inf logits have no weight, +inf ones (which count as fp32's
+ * largest value) share it all; a row with a NaN or with nothing but -inf keeps
+ * no draft and gives -1, as does a request without rows.  In 64 bits throughout.
  * Scratch: 16-byte aligned, zero before its first use, for calls that need
  * no more on one stream.  rows up to 65535, requests up to 16384. */
 size_t odi_cuda_verify_scratch_bytes(int rows, int requests, int64_t V);

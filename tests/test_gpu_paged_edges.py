@@ -99,12 +99,13 @@ def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats
 
 
 def close_attention(s, b, row, scale, softcap=0.0, slopes=None):
-    """Request b in 64 bits, and how far an fp32 output may be off.  A weight is off by the
-    square of half a step of its type (two parts, each rounded), fp16's smallest steps
-    (2^-32 of the row's largest), 2^-20 and its score's error; a sum by a step of fp32 per
+    """Request b in 64 bits, and how far an fp32 output may be off.  A weight is off by its
+    two parts: the first is cut off at a step of its type (2^-7 or 2^-10 of it), the second off
+    by half a step of that, 2^-16, or in fp16, whose last bit is set, by one and a half,
+    1.5 * 2^-20; by fp16's smallest steps (2^-32 of the row's largest), 2^-20 and its score's error; a sum by a step of fp32 per
     product of 16 positions, of which each part makes one."""
     past, N = s.past[b], s.new[b]
-    n, half = past + N, torch.finfo(s.cache.dtype).eps / 2
+    n, parts = past + N, 1.5 * 2.0 ** -20 if s.cache.dtype is torch.float16 else 2.0 ** -16
     q, k, v = (t.cpu().double() for t in (s.q[row:row + N], s.rows(s.cache.k, b), s.rows(s.cache.v, b)))
     x = q.view(N, s.kv, s.heads // s.kv, s.hd)
     far = (torch.arange(past, n)[:, None] - torch.arange(n)[None])[:, None, None].double()
@@ -120,7 +121,7 @@ def close_attention(s, b, row, scale, softcap=0.0, slopes=None):
     ds = ds.masked_fill(far < 0, 0.0)
     l = p.sum(-1, keepdim=True)
     want = torch.einsum("tkgn,knd->tkgd", p, v) / l
-    rel = half * half + 2.0 ** -20 + 2 * (n // 16 + 8) * 2.0 ** -23
+    rel = parts + 2.0 ** -20 + 2 * (n // 16 + 8) * 2.0 ** -23
     tiny = 2.0 ** -32 * (far >= 0).double().expand_as(p) if s.cache.dtype is torch.float16 else 0.0
     tol = torch.einsum("tkgn,knd->tkgd", p * (rel + ds) + tiny, v.abs()) / l
     return want.reshape(N, -1), (tol + want.abs() * ((p * (ds + rel)).sum(-1, keepdim=True) / l)).reshape(N, -1)
