@@ -630,8 +630,8 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
  * left as they were.  A row all of whose scores are -inf is zero.  Scores,
  * softmax and sums are fp32.  The weights are rounded to the cache's type (in
  * fp16 also to 2^-32 of the row's largest, whichever is more); for an fp32
- * output they are sums of two parts of that type, off by 2^-19 of them, in
- * bf16 by 2^-16.
+ * output they are sums of two parts of that type, off by 2^-19 of them (or
+ * 2^-30 of the row's largest, whichever is more), in bf16 by 2^-16.
  * scale is positive; softcap is at most 1024 (a capped score is off by 2^-21
  * of the cap at most).
  * Scratch: odi_cuda_attention_paged_scratch_bytes, 16-byte aligned, zero

@@ -85,10 +85,10 @@ struct Half16<__half> {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float up(uint16_t x) { return __half2float(__ushort_as_half(x)); }
-  // Two weights as a sum of two parts each, to 2^-19 of them (or half of 2^-24).  The first
-  // is cut off, not rounded, and the last bit of the second (2^-20 of the weight at most,
-  // beside 2^-21 for its rounding) is set where the first is not 0: neither is negative and no part of a weight is 0, or an infinity of V's would
-  // become a NaN.
+  // Two weights as a sum of two parts each, to 2^-19 of them (or 2^-23).  The first
+  // is cut off, not rounded, and the last bit of the second (2^-20 of the weight at most, or
+  // 2^-24, beside half as much for its rounding) is set where the first is not 0: neither
+  // is negative, and no part of a weight is 0, or an infinity of V's would become a NaN.
   static constexpr float PARTS = 1.f;  // what the parts' sum is of the weight
   static __device__ __forceinline__ uint32_t split(float2 x, uint32_t& rest) {
     uint32_t y;

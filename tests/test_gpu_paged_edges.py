@@ -59,11 +59,13 @@ def test_verify_rows_whose_largest_logits_have_it_all(cuda_lib, top, temperature
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("nats", [12.0, 17.0, 18.0, 20.0])
 @pytest.mark.parametrize("own", [0.0, 0.001])
-def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats, own):
+@pytest.mark.parametrize("out32", [True, False])
+def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats, own, out32):
     """One key some nats above all others, whose values are 0 or small: what the
     others add is there.  A weight is off by half a step of its type, 2^-20 and its
-    score's error; in fp16, whose steps end, by 2^-32 of the row's largest weight: half
-    of 2^-24, that weight standing at 2^7 or above."""
+    score's error; in fp16, whose steps end, by 2^-32 of the row's largest weight: half of
+    2^-24, that weight standing at 2^7 or above.  Weights of two parts (an fp32 output): one
+    and a half of 2^-24, the second part's last bit and rounding.  Then the output's own."""
     from odiengine_b200 import paged
 
     past = 3000 - new
@@ -81,7 +83,7 @@ def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats
     slot = int(s.tables.table[0, 1500 // 64]) * 64 + 1500 % 64
     s.cache.k[slot // 64, :, slot % 64] = base * (nats / (scale * hd))
     s.cache.v[slot // 64, :, slot % 64] = own
-    out = torch.empty((new, heads * hd), dtype=torch.float32, device="cuda")
+    out = torch.empty((new, heads * hd), dtype=torch.float32 if out32 else s.q.dtype, device="cuda")
     paged.attention_paged(s.q, s.cache, s.tables, s.batch, out, scale=scale, scratch=s.scratch)
     q, k, v = (t.cpu().double() for t in (s.q, s.rows(s.cache.k, 0), s.rows(s.cache.v, 0)))
     x = q.view(new, kv, heads // kv, hd)
@@ -91,8 +93,10 @@ def test_a_key_that_outweighs_the_rest(cuda_lib, new, heads, kv, hd, dtype, nats
     p = torch.exp((sc - sc.masked_fill(~see, -math.inf).amax(-1, keepdim=True)).masked_fill(~see, -math.inf))
     l = p.sum(-1, keepdim=True)
     want = torch.einsum("tkgn,knd->tkgd", p, v) / l
-    err = p * (torch.finfo(s.cache.dtype).eps / 2 + 2.0 ** -20 + ds) + (2.0 ** -32 * see if dtype == "f16" else 0.0)
+    err = p * (torch.finfo(s.cache.dtype).eps / 2 + 2.0 ** -20 + ds) + ((1.5 * 2.0 ** -31 if out32 else 2.0 ** -32) * see if dtype == "f16" else 0.0)
     tol = torch.einsum("tkgn,knd->tkgd", err, v.abs()) / l + want.abs() * ((p * (ds + 2.0 ** -20)).sum(-1, keepdim=True) / l + 2.0 ** -23)
+    own_step = torch.finfo(out.dtype).eps / 2 * (want.abs() + tol)
+    tol = tol + (own_step.clamp(min=2.0 ** -25) if out.dtype is torch.float16 else own_step)
     off = (out.cpu().double().view(want.shape) - want).abs()
     assert (off <= tol).all(), (off.max(), (off / tol).max())
     assert cuda_lib_status(s.scratch) == 0
@@ -102,8 +106,9 @@ def close_attention(s, b, row, scale, softcap=0.0, slopes=None):
     """Request b in 64 bits, and how far an fp32 output may be off.  A weight is off by its
     two parts: the first is cut off at a step of its type (2^-7 or 2^-10 of it), the second off
     by half a step of that, 2^-16, or in fp16, whose last bit is set, by one and a half,
-    1.5 * 2^-20; by fp16's smallest steps (2^-32 of the row's largest), 2^-20 and its score's error; a sum by a step of fp32 per
-    product of 16 positions, of which each part makes one."""
+    1.5 * 2^-20, or of fp16's smallest steps (2^-24, the largest weight standing at 2^7 or
+    above); by 2^-20 and its score's error; a sum by a step of fp32 per product of 16
+    positions, of which each part makes one."""
     past, N = s.past[b], s.new[b]
     n, parts = past + N, 1.5 * 2.0 ** -20 if s.cache.dtype is torch.float16 else 2.0 ** -16
     q, k, v = (t.cpu().double() for t in (s.q[row:row + N], s.rows(s.cache.k, b), s.rows(s.cache.v, b)))
@@ -122,7 +127,7 @@ def close_attention(s, b, row, scale, softcap=0.0, slopes=None):
     l = p.sum(-1, keepdim=True)
     want = torch.einsum("tkgn,knd->tkgd", p, v) / l
     rel = parts + 2.0 ** -20 + 2 * (n // 16 + 8) * 2.0 ** -23
-    tiny = 2.0 ** -32 * (far >= 0).double().expand_as(p) if s.cache.dtype is torch.float16 else 0.0
+    tiny = 1.5 * 2.0 ** -31 * (far >= 0).double().expand_as(p) if s.cache.dtype is torch.float16 else 0.0
     tol = torch.einsum("tkgn,knd->tkgd", p * (rel + ds) + tiny, v.abs()) / l
     return want.reshape(N, -1), (tol + want.abs() * ((p * (ds + rel)).sum(-1, keepdim=True) / l)).reshape(N, -1)
 
