@@ -605,7 +605,8 @@ size_t odi_cuda_paged_work_bytes(int requests, int max_rows, int max_new, int he
  * order: once one is refused for want of pages, so are those after it that
  * need a page, though fewer would do for them; those that need none are
  * served.  d_prefix (NULL: 0): the first d_prefix[b] positions see one another
- * both ways, once they are in the cache. */
+ * both ways, once they are in the cache; it may not overlap what the step
+ * writes. */
 int odi_cuda_paged_step(const odi_cuda_page_tables* tables, const odi_cuda_paged_batch* batch, const int32_t* d_keep,
                         const int32_t* d_new, const int32_t* d_prefix, void* stream);
 
