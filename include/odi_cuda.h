@@ -615,7 +615,7 @@ int odi_cuda_paged_step(const odi_cuda_page_tables* tables, const odi_cuda_paged
  * (head_dim weights; NULL: none), then the rotation of odi_cuda_rope_kv at
  * the row's position, its angle reduced in 64 bits.  k and v go to the row's
  * slot, rotated q rows, rounded to the cache's type, to d_q_out (ld_q apart,
- * even; 4-byte aligned; it may not overlap d_qkv).  Rows without a slot are
+ * even; 4-byte aligned; its rows may not overlap d_qkv's, nor either the cache).  Rows without a slot are
  * not written. */
 int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const float* d_q_norm, const float* d_k_norm,
                                   float eps, void* d_q_out, int64_t ld_q, const odi_cuda_paged_cache* cache,
@@ -626,7 +626,8 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
  * > 0: softcap * tanh(s / softcap); with d_slopes (fp32 [heads]): minus
  * slope * |i - j|.  d_q: rotated rows of the cache's type, ld_q apart (even),
  * heads * head_dim values; d_out: of the cache's type or fp32, ld_out apart;
- * both 4-byte aligned, and they may not overlap.  tokens: rows that d_q and
+ * both 4-byte aligned.  Their rows may not overlap, nor d_out the cache, the
+ * slopes or the scratch.  tokens: rows that d_q and
  * d_out have.  Rows behind the batch's last, and of refused requests, are
  * left as they were.  A row all of whose scores are -inf is zero.  Scores,
  * softmax and sums are fp32.  The weights are rounded to the cache's type (in
@@ -638,8 +639,8 @@ int odi_cuda_qk_rope_append_paged(const float* d_qkv, int64_t ld_qkv, const floa
  * Scratch: odi_cuda_attention_paged_scratch_bytes, 16-byte aligned, zero
  * before its first use; calls of any layer, and of any batch that needs no
  * more, on one stream share it.  Its first word is an error word (odi_cuda_workspace_status):
- * a bounded wait that gave up, or a table entry that names no page (such a
- * page reads as zeros). */
+ * a bounded wait that gave up, or a table entry that names no page or that the
+ * table is too narrow to have (such a page reads as zeros). */
 enum { ODI_CUDA_PAGED_OUT_CACHE = 0, ODI_CUDA_PAGED_OUT_F32 = 1 };
 size_t odi_cuda_attention_paged_scratch_bytes(int requests, int max_rows, int max_new, int heads, int kv_heads, int head_dim);
 int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged_cache* cache,
@@ -661,6 +662,7 @@ int odi_cuda_attention_paged(const void* d_q, int64_t ld_q, const odi_cuda_paged
  * refused.  -inf logits have no weight, +inf ones (which count as fp32's
  * largest value) share it all; a row with a NaN or with nothing but -inf keeps
  * no draft and gives -1, as does a request without rows.  In 64 bits throughout.
+ * The outputs may not overlap one another or what the call reads.
  * Scratch: 16-byte aligned, zero before its first use, for calls that need
  * no more on one stream.  rows up to 65535, requests up to 16384. */
 size_t odi_cuda_verify_scratch_bytes(int rows, int requests, int64_t V);
